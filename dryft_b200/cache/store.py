@@ -25,6 +25,7 @@ from typing import Dict, List, Mapping, Optional, Sequence, Tuple
 
 import torch
 
+from ..ops.kernels import kv4_token_bytes
 from .slots import CacheError, FreeList, PageLedger, pages_for
 
 
@@ -40,7 +41,9 @@ class KVNeed:
     is its own business); those rows live in pages of their own that are never given back early, and reach the mixer as
     ``CacheEntry.pooled``.  With a ``pool``, ``window`` is how many of the last tokens' rows must stay (the mixer's own
     window or the block it is still to summarise, whichever is longer).  ``keep_first``: with a ``window``, the sequence's first
-    ``keep_first`` tokens stay visible to every query, and the pages that hold them are never given back early."""
+    ``keep_first`` tokens stay visible to every query, and the pages that hold them are never given back early.  ``bits=4``: keys
+    and values are held in 4 bits, ``bits_group`` numbers of a head sharing a scale; the pages are then bytes ``[pages, kv_heads, page bytes]``
+    (``csrc/four_bit.cuh``) and the mixer reads and writes them with the kernels for that form."""
 
     kv_heads: int
     head_dim: int
@@ -50,6 +53,8 @@ class KVNeed:
     values: bool = True
     pool: Optional[int] = None
     keep_first: int = 0
+    bits: int = 16
+    bits_group: int = 64
 
 
 @dataclass(frozen=True)
@@ -76,6 +81,19 @@ class CacheEntry:
     # blocks as the step it borrows from reads that step's rows)
     pooled: Optional["CacheEntry"] = None
     fills_pooled: bool = False
+    # of a group held in 4 bits: pages [pages, kv_heads, page_size, head_dim] of the engine's type, which all run steps of the group put
+    # values into for a step's prompt attention
+    scratch: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+
+
+def _check_bits4(need: KVNeed) -> None:
+    if need.bits != 4:
+        raise CacheError(f"keys and values are held in 16 bits (the engine's type) or 4, got bits={need.bits}")
+    if not need.values or need.pool is not None or need.v_head_dim not in (None, need.head_dim):
+        raise CacheError("a cache in 4 bits holds keys and values of one size, without pooled rows")
+    if need.head_dim % 16 or not 0 < need.head_dim <= 256 or need.bits_group not in (16, 32, 64, 128) or need.head_dim % need.bits_group:
+        raise CacheError(f"a cache in 4 bits takes head sizes 16..256 in steps of 16 and whole groups of 16, 32, 64 or 128 numbers, got "
+                         f"head_dim={need.head_dim}, bits_group={need.bits_group}")
 
 
 class _KVGroup:
@@ -89,9 +107,18 @@ class _KVGroup:
         self.trims = trim and (need.window is not None or need.chunk is not None)
         self.ledger = PageLedger(n_pages, page_size, max_pages_per_slot, need.window if trim else None,
                                  need.chunk if trim else None, need.keep_first if trim else 0)
-        shape = (len(run_steps), n_pages, need.kv_heads, page_size, need.head_dim)
-        self.k = torch.zeros(shape, dtype=dtype, device=device)
-        self.v = torch.zeros(shape[:-1] + (need.v_head_dim or need.head_dim,), dtype=dtype, device=device) if need.values else None
+        self.scratch: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+        if need.bits != 16:
+            _check_bits4(need)
+            token = kv4_token_bytes(need.head_dim, need.bits_group)
+            self.k = torch.zeros((len(run_steps), n_pages, need.kv_heads, page_size * token), dtype=torch.uint8, device=device)
+            self.v = torch.zeros_like(self.k)
+            shape = (n_pages, need.kv_heads, page_size, need.head_dim)
+            self.scratch = (torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
+        else:
+            shape = (len(run_steps), n_pages, need.kv_heads, page_size, need.head_dim)
+            self.k = torch.zeros(shape, dtype=dtype, device=device)
+            self.v = torch.zeros(shape[:-1] + (need.v_head_dim or need.head_dim,), dtype=dtype, device=device) if need.values else None
         self.page_table_host = torch.zeros((max_slots, max_pages_per_slot), dtype=torch.int32)
         self.page_table = torch.zeros((max_slots, max_pages_per_slot), dtype=torch.int32, device=device)
         self.dirty: set = set()
@@ -101,7 +128,8 @@ class _KVGroup:
         self.staged: Optional[torch.cuda.Event] = None
 
     def bytes(self) -> int:
-        return (self.k.numel() + (self.v.numel() if self.v is not None else 0)) * self.k.element_size()
+        held = [self.k] + ([self.v] if self.v is not None else []) + list(self.scratch or ())
+        return sum(t.numel() * t.element_size() for t in held)
 
 
 class SequenceCache:
@@ -209,7 +237,7 @@ class SequenceCache:
         if loc is None:
             return None
         g = self._groups[loc[0]]
-        entry = CacheEntry(g.k[loc[1]], g.v[loc[1]] if g.v is not None else None, g.page_table, self.page_size, g.need.window)
+        entry = CacheEntry(g.k[loc[1]], g.v[loc[1]] if g.v is not None else None, g.page_table, self.page_size, g.need.window, scratch=g.scratch)
         ploc = self._pooled_of.get(run_step)
         if ploc is not None:
             pg = self._groups[ploc[0]]

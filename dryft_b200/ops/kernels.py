@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
+from dataclasses import dataclass
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -2443,3 +2444,285 @@ def wkv_decode(r, k, v, g, low, w2, w0, u, norm_w, eps: float, h, last, tok_slot
     _ok(wkv_lib().dryft_wkv_decode(_act(h, "h"), *ptrs[:4], lds[0], ptrs[4], lds[4], rank, _ptr(w2), _ptr(w0), _ptr(u), _ptr(norm_w), float(eps),
                                    _ptr(h), width, _ptr(last), _ptr(tok_slot), n, heads, d, dv, _ptr(state), _ptr(out), _stream()),
         f"wkv_decode ({heads} heads of {d})")
+
+
+# ----------------------------------------------------------------------------- 4 bits: weights, the cache, attention over it
+# A group of 16, 32, 64 or 128 consecutive numbers shares a scale s and a middle z, both bfloat16; code c (0..15) stands for
+# z + (c - 7.5) s.  csrc/four_bit.cuh has the arithmetic and the layouts.
+BITS4_GROUPS = (16, 32, 64, 128)
+LINEAR4_ROWS = 64      # rows of x that ``linear4`` takes
+
+
+def _bits4_group(size: int, group: int, what: str) -> None:
+    if group not in BITS4_GROUPS:
+        raise KernelError(f"{what}: numbers that share a scale come in groups of 16, 32, 64 or 128, got {group}")
+    if size <= 0 or size % group:
+        raise KernelError(f"{what}: {size} numbers are not whole groups of {group}")
+
+
+def linear4_lib() -> ctypes.CDLL:
+    """Products with weights held in 4 bits."""
+    return _single_lib("linear4", {
+        "dryft_linear4": [_i, _i, _p, _ll, _p, _p, _p, _i, _i, _i, _i, _p],
+        "dryft_weight4_expand": [_i, _p, _p, _p, _i, _i, _i, _p],
+    })
+
+
+@dataclass(frozen=True)
+class Weight4:
+    """A matrix ``[n, k]`` held in 4 bits, laid out once for the products (``pack_weight4`` makes it).  ``codes``: uint8, 16 rows by 64 inputs
+    as a warp's lanes read them; ``scales``: bfloat16, (s, z) of every row and group."""
+
+    codes: torch.Tensor     # uint8 [tiles of 16 rows, blocks of 64 inputs, 512]
+    scales: torch.Tensor    # bfloat16 [tiles, k / group, 8, 2, 2]
+    n: int
+    k: int
+    group: int
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return (self.n, self.k)
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return torch.uint8
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + 2 * self.scales.numel()
+
+    def rows(self, first: int, end: int) -> "Weight4":
+        """Rows ``first`` to ``end``; ``first`` is a multiple of 16, as tiles are."""
+        if first % 16 or not 0 <= first < end <= self.n:
+            raise KernelError(f"Weight4.rows: {first}..{end} of {self.n} rows; the first is a multiple of 16")
+        return Weight4(self.codes[first // 16:(end + 15) // 16], self.scales[first // 16:(end + 15) // 16], end - first, self.k, self.group)
+
+    def __getitem__(self, at: slice) -> "Weight4":
+        if not isinstance(at, slice) or at.step not in (None, 1):
+            raise KernelError("Weight4: only a range of rows can be taken")
+        first, end, _ = at.indices(self.n)
+        return self.rows(first, end)
+
+
+def _group_codes(x: torch.Tensor, group: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Codes (uint8) and (s, z) of ``x`` ``[..., size]`` in the arithmetic of csrc/four_bit.cuh."""
+    parts = x.float().unflatten(-1, (-1, group))
+    lo, hi = parts.aminmax(dim=-1, keepdim=True)
+    s, z = ((hi - lo) / torch.full_like(lo, 15.0)).bfloat16(), ((hi + lo) * 0.5).bfloat16()
+    bad = ~(s.isfinite() & z.isfinite())
+    s, z = s.masked_fill(bad, float("nan")), z.masked_fill(bad, float("nan"))
+    c = ((parts - z.float()) / s.float() + 7.5).round().clamp(0, 15)
+    c = torch.where(s > 0, c, torch.full_like(c, 8.0)).to(torch.uint8)
+    return c.flatten(-2), torch.cat([s, z], -1)
+
+
+def pack_weight4(w: torch.Tensor, group: int = 64) -> Weight4:
+    """``w`` ``[n, k]`` (float32 or bfloat16) in 4 bits: rounded to the nearest code of its group, laid out for the products.  ``k`` is a multiple of
+    ``group`` (16, 32, 64 or 128).  Done once, when weights are loaded."""
+    _act(w, "weight")
+    if w.dim() != 2:
+        raise KernelError(f"pack_weight4: a weight is [outputs, inputs], got shape {tuple(w.shape)}")
+    n, k = w.shape
+    _bits4_group(k, group, "pack_weight4")
+    if n <= 0:
+        raise KernelError("pack_weight4: no rows")
+    tiles, blocks = (n + 15) // 16, (k + 63) // 64
+    codes = torch.empty(tiles, blocks, 512, dtype=torch.uint8, device=w.device)
+    scales = torch.empty(tiles, k // group, 8, 2, 2, dtype=torch.bfloat16, device=w.device)
+    step = max(1, (1 << 24) // (16 * k))           # tiles at a time: bounds what this holds beside the result
+    for t0 in range(0, tiles, step):
+        part = w[t0 * 16:(t0 + step) * 16]
+        c, sz = _group_codes(part, group)
+        nt = (part.shape[0] + 15) // 16
+        full = torch.full((nt * 16, blocks * 64), 8, dtype=torch.uint8, device=w.device)
+        full[:part.shape[0], :k] = c
+        # [tile, row half h, r, block, step s, quarter c, pair i, e] -> bytes of lane (r, c), word s: nibble 2 i + h of half e
+        a = full.view(nt, 2, 8, blocks, 4, 4, 2, 2).permute(0, 3, 2, 5, 4, 7, 6, 1)   # tile, block, r, c, s, e, i, h
+        codes[t0:t0 + nt] = (a[..., 0] | (a[..., 1] << 4)).reshape(nt, blocks, 512)
+        fs = torch.zeros(nt * 16, k // group, 2, dtype=torch.bfloat16, device=w.device)
+        fs[:part.shape[0]] = sz
+        scales[t0:t0 + nt] = fs.view(nt, 2, 8, k // group, 2).permute(0, 3, 2, 1, 4)
+    return Weight4(codes, scales, n, k, group)
+
+
+def _need_weight4(w: Weight4) -> None:
+    if not isinstance(w, Weight4):
+        raise KernelError(f"weight: expected a Weight4 (pack_weight4 makes one), got {type(w).__name__}")
+    _bits4_group(w.k, w.group, "Weight4")
+    tiles = (w.n + 15) // 16
+    _need(w.codes, "weight codes", torch.uint8, (tiles, (w.k + 63) // 64, 512))
+    _need(w.scales, "weight scales", torch.bfloat16, (tiles, w.k // w.group, 8, 2, 2))
+
+
+def _rows_in(x, name: str, width: int) -> int:
+    """Rows of ``width`` numbers that may lie ``x.stride(0)`` apart, on 16-byte boundaries; the distance."""
+    if not isinstance(x, torch.Tensor) or x.device.type != "cuda":
+        raise KernelError(f"{name}: expected a tensor on a CUDA device")
+    if x.dim() != 2 or x.shape[1] != width or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise KernelError(f"{name}: expected rows of {width} consecutive numbers, got shape {tuple(x.shape)}, strides {x.stride()}")
+    step = x.stride(0) if x.shape[0] > 1 else width
+    if step < width or (step * x.element_size()) % 16 or x.data_ptr() % 16:
+        raise KernelError(f"{name}: rows start on 16-byte boundaries and do not overlap (stride {x.stride(0)}, address {x.data_ptr():#x})")
+    return step
+
+
+def linear4(x, w: Weight4, out) -> None:
+    """``out = x @ w.T`` for up to 64 rows; ``x`` float32 or bfloat16, ``out`` of the same type or float32."""
+    _need_weight4(w)
+    step = _rows_in(x, "x", w.k)
+    m = x.shape[0]
+    if m > LINEAR4_ROWS:
+        raise KernelError(f"linear4 takes up to {LINEAR4_ROWS} rows, got {m}")
+    is_bf16 = _act(x, "x")
+    out_bf16 = _act(out, "out")
+    if out_bf16 and not is_bf16:
+        raise KernelError("linear4: 32-bit activations give 32-bit results")
+    _need(out, "out", None, (m, w.n))
+    _ok(linear4_lib().dryft_linear4(is_bf16, out_bf16, _ptr(x), step, _ptr(w.codes), _ptr(w.scales), _ptr(out), m, w.n, w.k, w.group, _stream()), "linear4")
+
+
+def weight4_expand(w: Weight4, out) -> None:
+    """``out`` ``[n, k]`` (float32 or bfloat16): what the codes stand for, for products of many rows."""
+    _need_weight4(w)
+    _need(out, "out", None, (w.n, w.k))
+    _ok(linear4_lib().dryft_weight4_expand(_act(out, "out"), _ptr(w.codes), _ptr(w.scales), _ptr(out), w.n, w.k, w.group, _stream()), "weight4_expand")
+
+
+def kv4_lib() -> ctypes.CDLL:
+    """The paged cache held in 4 bits: new tokens in, pages out."""
+    return _single_lib("kv4", {
+        "dryft_kv4_store": [_i, _p, _p, _ll, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p],
+        "dryft_kv4_expand": [_i, _p, _p, _p, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p],
+    })
+
+
+def kv4_token_bytes(head_dim: int, group: int) -> int:
+    """Bytes of one token's key (or value) of one head: codes, filled up to whole units of 32 numbers, and the groups' (s, z)."""
+    return 16 * ((head_dim + 31) // 32) + 4 * (head_dim // group)
+
+
+def _kv4_pages(k_pages, v_pages, page_table, head_dim: int, group: int) -> Tuple[int, int]:
+    """(key heads, tokens a page) of pages held in 4 bits."""
+    if head_dim <= 0 or head_dim % 16 or head_dim > 256:
+        raise KernelError(f"a cache in 4 bits takes head sizes 16..256 in steps of 16, got head_dim={head_dim}")
+    _bits4_group(head_dim, group, "a cache in 4 bits")
+    _need(k_pages, "k_pages", torch.uint8, (None, None, None))
+    _need(v_pages, "v_pages", torch.uint8, tuple(k_pages.shape))
+    _need(page_table, "page_table", torch.int32, (None, None))
+    page, rest = divmod(k_pages.shape[2], kv4_token_bytes(head_dim, group))
+    if rest or page % 16 or page <= 0:
+        raise KernelError(f"k_pages: {k_pages.shape[2]} bytes are not a page of whole 16 tokens of {kv4_token_bytes(head_dim, group)} bytes")
+    if k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16:
+        raise KernelError("k_pages, v_pages: pages start on 16-byte boundaries")
+    return k_pages.shape[1], page
+
+
+def kv4_store(k, v, tok_slot, tok_pos, k_pages, v_pages, page_table, group: int) -> None:
+    """The keys and values ``[n, kv_heads, head_dim]`` of ``n`` tokens into their places in the cache, in 4 bits.  Rows may lie further apart than their
+    length (columns of a fused projection).  Tokens of slot -1 are padding.  ``tok_slot`` and ``tok_pos`` name every place at most once."""
+    if not isinstance(k, torch.Tensor) or k.dim() != 3 or not isinstance(v, torch.Tensor) or v.shape != k.shape or v.dtype != k.dtype:
+        raise KernelError("kv4_store: k and v are [tokens, kv heads, head size] of the same shape and type")
+    n, n_kv, d = k.shape
+    heads, page = _kv4_pages(k_pages, v_pages, page_table, d, group)
+    if heads != n_kv:
+        raise KernelError(f"kv4_store: {n_kv} key heads, the pages have {heads}")
+    for t, nm in ((k, "k"), (v, "v")):
+        if t.device.type != "cuda":
+            raise KernelError(f"{nm}: is on {t.device}; dryft_b200 kernels run on a CUDA device only")
+        if t.stride(2) != 1 or (n_kv > 1 and t.stride(1) != d):
+            raise KernelError(f"{nm}: a token's heads follow one another (strides {t.stride()})")
+        if t.data_ptr() % 16 or (n > 1 and (t.stride(0) * t.element_size()) % 16):
+            raise KernelError(f"{nm}: rows start on 16-byte boundaries")
+    if n > 1 and k.stride(0) != v.stride(0):
+        raise KernelError("kv4_store: k and v rows lie equally far apart")
+    for t, nm in ((tok_slot, "tok_slot"), (tok_pos, "tok_pos")):
+        _need(t, nm, torch.int32)
+        if t.numel() < n:
+            raise KernelError("kv4_store: token index arrays shorter than the batch")
+    _ok(kv4_lib().dryft_kv4_store(_act(k, "k"), _ptr(k), _ptr(v), k.stride(0) if n > 1 else n_kv * d, _ptr(tok_slot), _ptr(tok_pos), _ptr(k_pages), _ptr(v_pages),
+                                  _ptr(page_table), page_table.shape[1], n, n_kv, d, group, page, _stream()), "kv4_store")
+
+
+def kv4_expand(k_pages, v_pages, page_table, cu_q, seq_slot, tok_pos, k_out, v_out, group: int, max_kv: int, window: Optional[int] = None) -> None:
+    """What the pages of a step's sequences stand for, into ``k_out`` and ``v_out`` ``[pages, kv_heads, page, head_dim]`` at the same page numbers, tokens
+    behind a sequence's end as zeros.  Sequence ``b`` brings the tokens ``cu_q[b]..cu_q[b + 1] - 1`` (none: it is left out) and ends with the last of
+    them; ``max_kv``: no sequence is longer.  ``window``: pages that none of them sees are left as they are."""
+    if not isinstance(k_out, torch.Tensor) or k_out.dim() != 4:
+        raise KernelError("kv4_expand: k_out is [pages, kv heads, page, head size]")
+    d = k_out.shape[3]
+    n_kv, page = _kv4_pages(k_pages, v_pages, page_table, d, group)
+    _need(k_out, "k_out", None, (k_pages.shape[0], n_kv, page, d))
+    _need(v_out, "v_out", k_out.dtype, tuple(k_out.shape))
+    for t, nm in ((cu_q, "cu_q"), (seq_slot, "seq_slot"), (tok_pos, "tok_pos")):
+        _need(t, nm, torch.int32)
+    n = seq_slot.numel()
+    if cu_q.numel() < n + 1:
+        raise KernelError("kv4_expand: cu_q is shorter than the sequences")
+    if n > 65535:
+        raise KernelError(f"kv4_expand takes up to 65,535 sequences, got {n}")
+    pages = min((max_kv + page - 1) // page, page_table.shape[1])
+    _ok(kv4_lib().dryft_kv4_expand(_act(k_out, "k_out"), _ptr(k_pages), _ptr(v_pages), _ptr(page_table), page_table.shape[1], _ptr(cu_q), _ptr(seq_slot),
+                                   _ptr(tok_pos), _ptr(k_out), _ptr(v_out), n, pages, n_kv, d, group, page, int(window or 0), _stream()), "kv4_expand")
+
+
+def attn4_lib(head_dim: int, heads: int, page: int, group: int) -> ctypes.CDLL:
+    """Attention over the cache in 4 bits, compiled for a head size, the query heads of a key head, a page and a group of 4-bit numbers."""
+    if head_dim <= 0 or head_dim % 16 or head_dim > 256:
+        raise KernelError(f"attention over a cache in 4 bits takes head sizes 16..256 in steps of 16, got head_dim={head_dim}")
+    if heads < 1 or heads > 16:
+        raise KernelError(f"attention kernels take 1..16 query heads per kv head, got {heads}")
+    _bits4_group(head_dim, group, "attention over a cache in 4 bits")
+    if page <= 0 or page % 16:
+        raise KernelError(f"pages are whole tiles of 16 tokens, got {page}")
+    key = ("attn4", head_dim, heads, page, group)
+    with _lock:
+        lib = _variants.get(key)
+        if lib is None:
+            path = build.build_library("attn4", ("attn4.cu",), {"DRYFT_HEAD_DIM": head_dim, "DRYFT_GROUP": heads, "DRYFT_PAGE": page, "DRYFT_BITS_GROUP": group})
+            lib = _load(path)
+            lib.dryft_attn4_rows.argtypes = [_i, _p, _p, _p, _p, _i, _p, _p, _p, _p, _p, _i, _i, _i, _f, _i, _p]
+            lib.dryft_attn4_rows.restype = _i
+            lib.dryft_attn4_sizes.argtypes = [_i]
+            if tuple(lib.dryft_attn4_sizes(i) for i in range(4)) != (head_dim, heads, page, group):
+                raise KernelError(f"{path} was compiled for other sizes")
+            _variants[key] = lib
+        return lib
+
+
+def attn4_splits(n: int, n_kv: int, max_kv: int, window: Optional[int]) -> int:
+    """Into how many blocks the keys of a row and key head are cut: about two blocks a multiprocessor, at least 64 keys each."""
+    keys = min(max_kv, window) if window else max_kv
+    return max(1, min(32, 296 // max(1, n * n_kv), (keys + 63) // 64))
+
+
+def attn4_rows(q, k_pages, v_pages, page_table, tok_slot, tok_pos, out, scale: float, window: Optional[int], group: int, max_kv: int) -> None:
+    """Attention of ``n`` query rows ``q`` ``[n, heads, head_dim]`` over the cache in 4 bits: row ``i`` sees the keys 0..``tok_pos[i]`` (the last ``window``
+    of them) of slot ``tok_slot[i]``; a row of slot -1 is padding and gets zeros.  ``max_kv``: no sequence is longer (a bound; how the keys are cut
+    over blocks follows from it)."""
+    if not isinstance(q, torch.Tensor) or q.dim() != 3:
+        raise KernelError("attn4_rows: q is [rows, heads, head size]")
+    n, n_heads, d = q.shape
+    _need(q, "q")
+    is_bf16 = _act(q, "q")
+    n_kv, page = _kv4_pages(k_pages, v_pages, page_table, d, group)
+    if n_heads % n_kv:
+        raise KernelError(f"attn4_rows: {n_heads} query heads are not a multiple of {n_kv} kv heads")
+    _need(out, "attention output", q.dtype, (n, n_heads * d))
+    for t, nm in ((tok_slot, "tok_slot"), (tok_pos, "tok_pos")):
+        _need(t, nm, torch.int32)
+        if t.numel() < n:
+            raise KernelError("attn4_rows: token index arrays shorter than the batch")
+    if window is not None and window <= 0:
+        raise KernelError(f"attn4_rows: a window is a positive number of keys, got {window}")
+    lib = attn4_lib(d, n_heads // n_kv, page, group)
+    s = attn4_splits(n, n_kv, max_kv, window)
+    part_o = part_ml = None
+    if s > 1:
+        part_o = torch.empty((n, n_heads, s, d), dtype=torch.float32, device=q.device)
+        part_ml = torch.empty((n, n_heads, s, 2), dtype=torch.float32, device=q.device)
+    _ok(lib.dryft_attn4_rows(is_bf16, _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(page_table), page_table.shape[1], _ptr(tok_slot), _ptr(tok_pos), _ptr(out),
+                             _ptr(part_o), _ptr(part_ml), n, n_kv, s, float(scale), int(window or 0), _stream()), f"attn4_rows (head_dim {d})",
+        n_kernels=2 if s > 1 else 1)

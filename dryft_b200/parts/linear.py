@@ -8,7 +8,9 @@ Which product runs:
   * bfloat16, many rows (prefill): cuBLAS through ``torch.mm``, 32-bit accumulation — the library
     product the reference itself uses (``F.linear``, ``engine/dryft_qwen3/model.py:153,179,180``);
   * bfloat16 activations with a weight the checkpoint stores in 32-bit: the weight stays 32-bit,
-    the activations are widened, the 32-bit product runs and its result is rounded once.
+    the activations are widened, the 32-bit product runs and its result is rounded once;
+  * weights held in 4 bits (``ops.kernels.Weight4``): the kernel that reads the codes up to 64 rows, above that the
+    weights are taken out of their 4 bits for the product above.
 """
 
 from __future__ import annotations
@@ -27,6 +29,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, rt: Runtime, out_dtype: Optional[to
     n = w.shape[0]
     if w.shape[1] != k:
         raise ValueError(f"linear: activations have width {k}, weight is {tuple(w.shape)}")
+    if isinstance(w, K.Weight4):
+        return _linear4(x, w, out_dtype)
     if x.dtype == torch.float32:
         if w.dtype != torch.float32:
             raise ValueError(f"linear: 32-bit activations need a 32-bit weight, got {w.dtype}")
@@ -55,6 +59,34 @@ def linear(x: torch.Tensor, w: torch.Tensor, rt: Runtime, out_dtype: Optional[to
     if out_dtype == torch.bfloat16:
         return torch.mm(x, w.t())
     return torch.mm(x, w.t(), out_dtype=out_dtype)
+
+
+EXPAND_BYTES = 48 << 20   # of weights at a time that a product of many rows takes out of their 4 bits: they stay in L2 until the product has read them
+
+
+def _linear4(x: torch.Tensor, w: K.Weight4, out_dtype: torch.dtype) -> torch.Tensor:
+    """Up to ``K.LINEAR4_ROWS`` rows the kernel reads the codes; more rows take the weights out of their 4 bits, a part at a time, for the product
+    that such rows run on otherwise."""
+    m, (n, k) = x.shape[0], w.shape
+    if m <= K.LINEAR4_ROWS:
+        out = torch.empty((m, n), dtype=out_dtype, device=x.device)
+        K.linear4(x, w, out)
+        return out
+    out = torch.empty((m, n), dtype=out_dtype, device=x.device)
+    step = max(16, EXPAND_BYTES // (k * x.element_size()) // 16 * 16)
+    part = torch.empty((min(step, n), k), dtype=x.dtype, device=x.device)
+    for first in range(0, n, step):
+        end = min(n, first + step)
+        K.weight4_expand(w.rows(first, end), part[:end - first])
+        if x.dtype == torch.float32:
+            y = torch.empty((m, end - first), dtype=torch.float32, device=x.device)
+            K.gemm_nt_f32(x, part[:end - first], y)
+            out[:, first:end] = y
+        elif out_dtype == torch.bfloat16:
+            torch.mm(x, part[:end - first].t(), out=out[:, first:end])
+        else:
+            out[:, first:end] = torch.mm(x, part[:end - first].t(), out_dtype=out_dtype)
+    return out
 
 
 def fusable_rows(n_rows: int, k: int, rt: Runtime, normed: bool = False) -> bool:
