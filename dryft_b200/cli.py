@@ -6,6 +6,7 @@ model, ``--seed``, ``--samples``, ``--workload name,b,in,out``.  Token ids in an
     python -m dryft_b200 generate --model DIR --prompt-ids 1,2,3 --prompt-ids 4,5 --max-new-tokens 8
     python -m dryft_b200 generate --tiny --workload demo,3,9,8 --temperature 0.7 --top-k 20 --seed 1
     python -m dryft_b200 bench --model DIR --workload b1,1,512,32 --workload b16,16,512,128 --samples 5
+    python -m dryft_b200 bench --model DIR --workload b8,8,512,64 --weight-bits 4 --cache-bits 4
     python -m dryft_b200 random-model --preset tiny-b --seed 1 --out DIR
     python -m dryft_b200 replay --model DIR --dtype float32 --out DIR --max-tokens 4096 < trace.jsonl
 """
@@ -45,7 +46,7 @@ def _model_dir(args) -> str:
 def _engine(args):
     from .engine.api import Engine
 
-    kw = dict(dtype=args.dtype, cuda_graphs=not args.no_cuda_graph)
+    kw = dict(dtype=args.dtype, cuda_graphs=not args.no_cuda_graph, weight_bits=args.weight_bits, cache_bits=args.cache_bits)
     if args.max_batch:
         kw["max_batch"] = args.max_batch
     if args.max_seq_len:
@@ -138,6 +139,8 @@ def main(argv=None) -> int:
         p.add_argument("--max-batch", type=int, default=0)
         p.add_argument("--max-seq-len", type=int, default=0)
         p.add_argument("--no-cuda-graph", action="store_true")
+        p.add_argument("--weight-bits", type=int, default=16, choices=[4, 16], help="4: matrices held in 4 bits")
+        p.add_argument("--cache-bits", type=int, default=16, choices=[4, 16], help="4: keys and values held in 4 bits")
 
     g = sub.add_parser("generate", help="generate token ids from token ids")
     common(g)

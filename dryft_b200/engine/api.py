@@ -55,6 +55,11 @@ class EngineOptions:
     # (engine/dryft_qwen3/model.py:28-32): as close to 32-bit as the default, 1.3 times further from a plain bfloat16
     # evaluation.  Off by default: the default path keeps the reference's rounding points.
     norm_ahead: bool = False
+    # Matrices, or keys and values, held in 4 bits instead of the engine's type: groups of ``bits_group`` consecutive numbers (fewer where a size
+    # consists of no whole ones) share a scale and a middle (csrc/four_bit.cuh).  For the dense decoder; a model with other parts is refused.
+    weight_bits: int = 16
+    cache_bits: int = 16
+    bits_group: int = 64
     tcgen05: bool = True                   # prefill attention and experts' products on tcgen05 / TMEM / TMA where the sizes allow
     # steps of up to this many rows run sublayers that read the same input (a mixer beside a feed-forward, two mixers side
     # by side) on streams of their own, joined before their results are summed: in a captured step they are parallel
@@ -115,6 +120,8 @@ class Engine:
         torch.backends.cudnn.allow_tf32 = False
         if opts.prefill_chunk_tokens is not None and opts.prefill_chunk_tokens <= 0:
             raise ValueError(f"prefill_chunk_tokens must be positive, got {opts.prefill_chunk_tokens}")
+        if opts.bits_group not in (16, 32, 64, 128):
+            raise ValueError(f"bits_group is 16, 32, 64 or 128, got {opts.bits_group}")
         self.config = config
         self.spec = spec
         self.options = opts
@@ -123,7 +130,7 @@ class Engine:
         props = torch.cuda.get_device_properties(dev)
         self.rt = Runtime(dtype=dtype, device=dev, page_size=opts.page_size, sm_count=props.multi_processor_count,
                           small_m_max=opts.small_m_max, stream_m_max=opts.stream_m_max, fuse_decode=opts.fuse_decode, pdl=opts.pdl, tcgen05=opts.tcgen05, norm_ahead=opts.norm_ahead,
-                          branch_rows=opts.branch_rows)
+                          branch_rows=opts.branch_rows, weight_bits=opts.weight_bits, cache_bits=opts.cache_bits, bits_group=opts.bits_group)
         with torch.cuda.device(dev), torch.no_grad():
             self.model = DecoderModel(spec, source, self.rt)
             self.max_seq_len = opts.max_seq_len or min(spec.max_positions, 8192)

@@ -15,7 +15,8 @@ import torch
 
 from ..cache.store import KVNeed, SequenceCache, StateNeed
 from ..config.spec import ModelSpec
-from ..parts.base import BLOCKS, EMBEDDINGS, FAMILIES, FFNS, HEADS, MIXERS, NORMS, Residual, Runtime, StepContext
+from ..ops.kernels import Weight4
+from ..parts.base import BLOCKS, EMBEDDINGS, FAMILIES, FFNS, FOUR_BIT, HEADS, MIXERS, NORMS, Residual, Runtime, StepContext
 
 
 class DecoderModel:
@@ -23,6 +24,7 @@ class DecoderModel:
         spec.validate()
         self.spec = spec
         self.rt = rt
+        self._check_bits(rt)
         self.vocab_size = spec.vocab_size
         self.hidden_size = spec.hidden_size
         self.embedding = EMBEDDINGS.get(spec.embedding.kind)(spec.embedding.params, spec.embedding_prefix, weights, rt)
@@ -46,6 +48,22 @@ class DecoderModel:
         self.joints = {j.name: FAMILIES[j.family].get(j.spec.kind)(j.spec.params, j.prefix, weights, rt) for j in spec.joints}
         self.keeps_x0 = any(st.enter is not None for st in spec.schedule)
 
+    def _check_bits(self, rt: Runtime) -> None:
+        """Weights or a cache in 4 bits are for models all of whose parts serve them: nothing is left at 16 bits unasked."""
+        for what, bits in (("weights", rt.weight_bits), ("a cache", rt.cache_bits)):
+            if bits not in (4, 16):
+                raise ValueError(f"{what} in {bits} bits: 16 (the engine's type) or 4")
+        if rt.weight_bits == 16 and rt.cache_bits == 16:
+            return
+        kinds = {"mixer": MIXERS, "ffn": FFNS, "head": HEADS}
+        wanted = [("mixer", layer.mixer.kind) for layer in self.spec.layers]
+        if rt.weight_bits == 4:
+            wanted += [("ffn", layer.ffn.kind) for layer in self.spec.layers if layer.ffn is not None] + [("head", self.spec.head.kind)]
+            wanted += [(e.family, e.spec.kind) for layer in self.spec.layers for e in layer.extra if e.family in kinds]
+        for family, kind in wanted:
+            if not getattr(kinds[family].get(kind), FOUR_BIT, False):
+                raise ValueError(f"4 bits are not served by this model's {family} {kind!r}")
+
     # what each run step asks of the cache
     def cache_needs(self) -> Tuple[List[Tuple[Optional[KVNeed], Optional[StateNeed]]], List[Optional[int]]]:
         needs, borrow = [], []
@@ -66,6 +84,9 @@ class DecoderModel:
         def visit(obj):
             nonlocal total
             for v in vars(obj).values():
+                if isinstance(v, Weight4) and v.codes.data_ptr() not in seen:
+                    seen.add(v.codes.data_ptr())
+                    total += v.nbytes()
                 if isinstance(v, torch.Tensor) and v.is_floating_point() and v.dim() >= 1:
                     key = v.data_ptr()
                     if key not in seen:

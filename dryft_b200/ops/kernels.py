@@ -2453,6 +2453,14 @@ BITS4_GROUPS = (16, 32, 64, 128)
 LINEAR4_ROWS = 64      # rows of x that ``linear4`` takes
 
 
+def bits4_group(size: int, most: int = 64) -> int:
+    """The largest group of up to ``most`` numbers that ``size`` consists of whole ones of."""
+    for g in sorted(BITS4_GROUPS, reverse=True):
+        if g <= most and size > 0 and size % g == 0:
+            return g
+    raise KernelError(f"{size} numbers are not whole groups of 16 to {most}: not held in 4 bits")
+
+
 def _bits4_group(size: int, group: int, what: str) -> None:
     if group not in BITS4_GROUPS:
         raise KernelError(f"{what}: numbers that share a scale come in groups of 16, 32, 64 or 128, got {group}")
@@ -2595,6 +2603,7 @@ def kv4_lib() -> ctypes.CDLL:
     """The paged cache held in 4 bits: new tokens in, pages out."""
     return _single_lib("kv4", {
         "dryft_kv4_store": [_i, _p, _p, _ll, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p],
+        "dryft_kv4_rope_store": [_i, _p, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _p],
         "dryft_kv4_expand": [_i, _p, _p, _p, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p],
     })
 
@@ -2646,10 +2655,44 @@ def kv4_store(k, v, tok_slot, tok_pos, k_pages, v_pages, page_table, group: int)
                                   _ptr(page_table), page_table.shape[1], n, n_kv, d, group, page, _stream()), "kv4_store")
 
 
+def kv4_rope_store(qkv, q_norm_w, k_norm_w, inv_freq, tok_slot, tok_pos, q_out, k_pages, v_pages, page_table, n_heads: int, n_kv_heads: int,
+                   head_dim: int, rotary_dim: int, eps: float, group: int, cs_table=None) -> None:
+    """``qk_norm_rope_store`` with the cache in 4 bits: per-head norm and rotation of the rows' queries and keys, queries to ``q_out``, keys and values into
+    the cache as ``kv4_store`` puts them there.  ``cs_table`` as there."""
+    n = qkv.shape[0]
+    width = (n_heads + 2 * n_kv_heads) * head_dim
+    _need(qkv, "qkv", None, (n, width))
+    is_bf16 = _act(qkv, "qkv")
+    heads, page = _kv4_pages(k_pages, v_pages, page_table, head_dim, group)
+    if heads != n_kv_heads:
+        raise KernelError(f"kv4_rope_store: {n_kv_heads} key heads, the pages have {heads}")
+    if rotary_dim < 0 or rotary_dim % 2 or rotary_dim > head_dim:
+        raise KernelError(f"kv4_rope_store: {rotary_dim} rotated dims of a head of {head_dim}")
+    has_norm = q_norm_w is not None
+    if has_norm:
+        _need(q_norm_w, "q_norm weight", torch.float32, (head_dim,))
+        _need(k_norm_w, "k_norm weight", torch.float32, (head_dim,))
+    if rotary_dim:
+        _need(inv_freq, "inv_freq", torch.float32, (rotary_dim // 2,))
+    _need(tok_slot, "tok_slot", torch.int32)
+    _need(tok_pos, "tok_pos", torch.int32)
+    if tok_slot.numel() < n or tok_pos.numel() < n:
+        raise KernelError("kv4_rope_store: token index arrays shorter than the batch")
+    _need(q_out, "q_out", qkv.dtype, (n, n_heads, head_dim))
+    if cs_table is not None:
+        _need(cs_table, "cs_table", qkv.dtype, (None, 2, rotary_dim // 2))
+        if cs_table.shape[0] < n:
+            raise KernelError("kv4_rope_store: cos/sin table shorter than the batch")
+    _ok(kv4_lib().dryft_kv4_rope_store(is_bf16, _ptr(qkv), width, _ptr(q_norm_w), _ptr(k_norm_w), _ptr(inv_freq), _ptr(cs_table), _ptr(tok_slot), _ptr(tok_pos),
+                                       _ptr(q_out), _ptr(k_pages), _ptr(v_pages), _ptr(page_table), page_table.shape[1], n, n_heads, n_kv_heads, head_dim,
+                                       rotary_dim, group, page, float(eps), int(has_norm), _stream()), "kv4_rope_store")
+
+
 def kv4_expand(k_pages, v_pages, page_table, cu_q, seq_slot, tok_pos, k_out, v_out, group: int, max_kv: int, window: Optional[int] = None) -> None:
     """What the pages of a step's sequences stand for, into ``k_out`` and ``v_out`` ``[pages, kv_heads, page, head_dim]`` at the same page numbers, tokens
     behind a sequence's end as zeros.  Sequence ``b`` brings the tokens ``cu_q[b]..cu_q[b + 1] - 1`` (none: it is left out) and ends with the last of
-    them; ``max_kv``: no sequence is longer.  ``window``: pages that none of them sees are left as they are."""
+    them; ``max_kv``: no sequence is longer (0: as long as the page table allows).  ``window``: pages that none of them sees are left
+    as they are."""
     if not isinstance(k_out, torch.Tensor) or k_out.dim() != 4:
         raise KernelError("kv4_expand: k_out is [pages, kv heads, page, head size]")
     d = k_out.shape[3]
@@ -2663,7 +2706,7 @@ def kv4_expand(k_pages, v_pages, page_table, cu_q, seq_slot, tok_pos, k_out, v_o
         raise KernelError("kv4_expand: cu_q is shorter than the sequences")
     if n > 65535:
         raise KernelError(f"kv4_expand takes up to 65,535 sequences, got {n}")
-    pages = min((max_kv + page - 1) // page, page_table.shape[1])
+    pages = min((max_kv + page - 1) // page, page_table.shape[1]) if max_kv > 0 else page_table.shape[1]
     _ok(kv4_lib().dryft_kv4_expand(_act(k_out, "k_out"), _ptr(k_pages), _ptr(v_pages), _ptr(page_table), page_table.shape[1], _ptr(cu_q), _ptr(seq_slot),
                                    _ptr(tok_pos), _ptr(k_out), _ptr(v_out), n, pages, n_kv, d, group, page, int(window or 0), _stream()), "kv4_expand")
 

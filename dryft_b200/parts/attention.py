@@ -23,7 +23,7 @@ from ..cache.store import CacheEntry, KVNeed, StateNeed
 from ..config.spec import PartSpec
 from ..ops import kernels as K
 from .base import NORMS, POSITIONS, Runtime, StepContext, TensorInfo, fused_rms, register_mixer
-from .linear import fusable_rows, linear, weighted_for
+from .linear import fusable_rows, held, linear, weighted_for
 
 PREFILL_TILE = 64      # query rows per block of the mma.sync prefill kernel
 PREFILL_TILE_TC = 128  # query rows per block of the tcgen05 prefill kernel
@@ -31,6 +31,8 @@ PREFILL_TILE_TC = 128  # query rows per block of the tcgen05 prefill kernel
 
 @register_mixer("attention")
 class Attention:
+    serves_four_bits = True
+
     @staticmethod
     def tensors(params: Mapping, prefix: str) -> Dict[str, TensorInfo]:
         h, nh, nkv, d = params["hidden_size"], params["num_heads"], params["num_kv_heads"], params["head_dim"]
@@ -60,8 +62,8 @@ class Attention:
         self.q_dim = self.n_heads * self.head_dim
         self.kv_dim = self.n_kv * self.head_dim
         names = [prefix + f"{p}_proj.weight" for p in ("q", "k", "v")]
-        self.w_qkv = weights.load_fused(names, [self.q_dim, self.kv_dim, self.kv_dim], self.hidden)
-        self.w_o = weights.load(prefix + "o_proj.weight", "matrix")
+        self.w_qkv = held(weights.load_fused(names, [self.q_dim, self.kv_dim, self.kv_dim], self.hidden), rt)
+        self.w_o = held(weights.load(prefix + "o_proj.weight", "matrix"), rt)
         qk: Optional[PartSpec] = params.get("qk_norm")
         self.qk_eps = 0.0
         self.q_norm_w = self.k_norm_w = None
@@ -88,8 +90,15 @@ class Attention:
             K.attention_prefill_lib(self.head_dim, self.group, rt.page_size)
         if self.use_decode_kernel:
             K.attention_decode_lib(self.head_dim, self.group, rt.page_size)
+        self.bits_group: Optional[int] = None     # the cache in 4 bits: numbers of a head that share a scale
+        if rt.cache_bits == 4:
+            self.bits_group = K.bits4_group(self.head_dim, rt.bits_group)
+            K.kv4_lib()
+            K.attn4_lib(self.head_dim, self.group, rt.page_size, self.bits_group)
 
     def kv_need(self) -> Optional[KVNeed]:
+        if self.bits_group is not None:
+            return KVNeed(self.n_kv, self.head_dim, self.window, bits=4, bits_group=self.bits_group)
         return KVNeed(self.n_kv, self.head_dim, self.window)
 
     def state_need(self) -> Optional[StateNeed]:
@@ -173,6 +182,8 @@ class Attention:
         n = qkv.shape[0]
         dev = qkv.device
         h = qkv
+        if self.bits_group is not None:
+            return self._attend4(qkv, ctx, cache, owns_cache)
         if ctx.decode and self.use_decode_kernel:
             # one launch: q/k norm + RoPE + cache write + split attention + combine
             o = torch.empty((n, self.q_dim), dtype=h.dtype, device=dev)
@@ -192,12 +203,38 @@ class Attention:
                              self.position.rotary_dim, self.qk_eps, write_kv=owns_cache,
                              cs_table=table_of(ctx) if table_of is not None else None,
                              zero_tail=owns_cache and not ctx.decode and (self.use_prefill_tc or self.use_prefill_kernel))
-        o = torch.empty((n, self.q_dim), dtype=h.dtype, device=dev)
+        return self._attend_pages(q, cache.k, cache.v, cache.page_table, ctx)
+
+    def _attend4(self, qkv: torch.Tensor, ctx: StepContext, cache: CacheEntry, owns_cache: bool) -> torch.Tensor:
+        """``_attend`` over a cache in 4 bits.  Decode steps read the codes.  A prompt's tokens see the values that the codes stand for, their own
+        step's too, so that a result does not depend on how the prompt was cut into steps: the sequences' pages are put into the group's
+        scratch pages, and the prompt attention reads those."""
+        n, dev = qkv.shape[0], qkv.device
+        q = torch.empty((n, self.n_heads, self.head_dim), dtype=qkv.dtype, device=dev)
+        table_of = getattr(self.position, "table", None)
+        table = table_of(ctx) if table_of is not None else None
+        if owns_cache:
+            K.kv4_rope_store(qkv, self.q_norm_w, self.k_norm_w, self.position.inv_freq, ctx.tok_slot, ctx.tok_pos, q, cache.k, cache.v, cache.page_table,
+                             self.n_heads, self.n_kv, self.head_dim, self.position.rotary_dim, self.qk_eps, self.bits_group, cs_table=table)
+        else:
+            K.qk_norm_rope_store(qkv, self.q_norm_w, self.k_norm_w, self.position.inv_freq, ctx.tok_slot, ctx.tok_pos, q, None, None, None, self.n_heads,
+                                 self.n_kv, self.head_dim, self.position.rotary_dim, self.qk_eps, write_kv=False, cs_table=table)
+        if ctx.decode:
+            o = torch.empty((n, self.q_dim), dtype=qkv.dtype, device=dev)
+            K.attn4_rows(q, cache.k, cache.v, cache.page_table, ctx.tok_slot, ctx.tok_pos, o, self.scale, self.window, self.bits_group, ctx.max_kv)
+            return o
+        k, v = cache.scratch
+        K.kv4_expand(cache.k, cache.v, cache.page_table, ctx.cu_q, ctx.seq_slot[:ctx.n_seqs], ctx.tok_pos, k, v, self.bits_group, ctx.max_kv, self.window)
+        return self._attend_pages(q, k, v, cache.page_table, ctx)
+
+    def _attend_pages(self, q: torch.Tensor, k_pages, v_pages, page_table, ctx: StepContext) -> torch.Tensor:
+        n, dev = q.shape[0], q.device
+        o = torch.empty((n, self.q_dim), dtype=q.dtype, device=dev)
         if self.use_prefill_tc and not ctx.decode and ctx.n_tiles > 0 and ctx.tile_size <= PREFILL_TILE_TC:
-            K.attn_prefill_tc(q, cache.k, cache.v, cache.page_table, ctx.tile_tok0, ctx.tile_rows, ctx.tok_slot, ctx.tok_pos,
+            K.attn_prefill_tc(q, k_pages, v_pages, page_table, ctx.tile_tok0, ctx.tile_rows, ctx.tok_slot, ctx.tok_pos,
                               o, ctx.n_tiles, self.scale, self.window)
         elif self.use_prefill_kernel and not ctx.decode and ctx.n_tiles > 0 and ctx.tile_size <= PREFILL_TILE:
-            K.attn_prefill(q, cache.k, cache.v, cache.page_table, ctx.tile_tok0, ctx.tile_rows, ctx.tok_slot, ctx.tok_pos,
+            K.attn_prefill(q, k_pages, v_pages, page_table, ctx.tile_tok0, ctx.tile_rows, ctx.tok_slot, ctx.tok_pos,
                            o, ctx.n_tiles, self.scale, self.window)
         else:
             s = self._n_splits(n)
@@ -205,6 +242,6 @@ class Attention:
             if s > 1:
                 part_o = torch.empty((n, self.n_heads, s, self.head_dim), dtype=torch.float32, device=dev)
                 part_ml = torch.empty((n, self.n_heads, s, 2), dtype=torch.float32, device=dev)
-            K.attn_rows(q, cache.k, cache.v, cache.page_table, ctx.tok_slot, ctx.tok_pos, o, self.scale, self.window,
+            K.attn_rows(q, k_pages, v_pages, page_table, ctx.tok_slot, ctx.tok_pos, o, self.scale, self.window,
                         s, part_o, part_ml)
         return o

@@ -19,6 +19,9 @@ block       ``__init__(norm_mixer, mixer, norm_ffn, ffn)`` (``norm_ffn`` and ``f
             ``forward(res, ctx, cache, state, owns_cache)`` -> ``Residual``: the stream, plus either the
             not-yet-added output of the block's last part (so the next norm can fuse the add) or the
             stream's sums of squares (so the next fused product can normalise it).
+Optional: ``serves_four_bits = True`` says that a mixer, feed-forward or head holds its matrices in 4 bits when ``rt.weight_bits`` is 4
+            (``parts/linear.py:held``) and that a mixer asks for a cache in 4 bits when ``rt.cache_bits`` is 4; a model whose other
+            parts would be asked to is refused.
 Optional, for few rows (decode): a mixer or feed-forward may offer
             ``forward_normed(x, ss, ss_parts, norm, ...) -> (ss, ss_parts)``: it normalises ``x`` itself
             inside its first product, adds its output into ``x`` in place inside its last product, and
@@ -66,6 +69,9 @@ class Runtime:
     pdl: bool = True             # launch decode products, joins and experts' products as programmatic dependents
     norm_ahead: bool = False     # fused decode: a residual product leaves the stream weighted for the next norm (one rounding fewer than the reference)
     tcgen05: bool = True         # attention of prompts and experts' products on tcgen05.mma / tensor memory / TMA where sizes allow
+    weight_bits: int = 16        # 4: the parts' matrices are held in 4 bits (ops/kernels.py:Weight4)
+    cache_bits: int = 16         # 4: keys and values are held in 4 bits
+    bits_group: int = 64         # numbers that share a scale where something is held in 4 bits (fewer where a size consists of no whole ones)
     branch_rows: int = 0         # steps of up to this many rows run independent sublayers on streams of their own (0: in turn)
     side_streams: list = field(default_factory=list, repr=False, compare=False)
 
@@ -101,6 +107,9 @@ class Runtime:
     @property
     def is_bf16(self) -> bool:
         return self.dtype == torch.bfloat16
+
+
+FOUR_BIT = "serves_four_bits"   # attribute of parts whose matrices (and, of a mixer, whose cache) can be held in 4 bits
 
 
 @dataclass

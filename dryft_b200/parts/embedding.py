@@ -13,7 +13,7 @@ import torch
 
 from ..ops import kernels as K
 from .base import Residual, Runtime, StepContext, TensorInfo, fused_rms, register_embedding, register_head
-from .linear import fusable_rows, linear
+from .linear import fusable_rows, held, linear
 
 
 @register_embedding("embedding")
@@ -89,6 +89,8 @@ class SinusoidEmbedding:
 
 @register_head("lm_head")
 class LMHead:
+    serves_four_bits = True   # (a tied head keeps a copy in 4 bits beside the embedding's table)
+
     @staticmethod
     def tensors(params: Mapping, prefix: str) -> Dict[str, TensorInfo]:
         return {prefix + params.get("name", "weight"): TensorInfo((params["vocab_size"], params["hidden_size"]), "matrix",
@@ -112,6 +114,7 @@ class LMHead:
                 del other
         else:
             self.weight = weights.load(name, "matrix")
+        self.weight = held(self.weight, rt)
         # ``params["softcap"]``: logits <- cap * tanh(logits / cap), in 32-bit, after the product
         self.softcap = float(params["softcap"]) if params.get("softcap") is not None else None
         if self.softcap is not None:

@@ -12,11 +12,13 @@ import torch
 
 from ..ops import kernels as K
 from .base import Runtime, StepContext, TensorInfo, fused_rms, register_ffn
-from .linear import fusable_rows, linear, weighted_for
+from .linear import fusable_rows, held, linear, weighted_for
 
 
 @register_ffn("swiglu")
 class SwiGLU:
+    serves_four_bits = True
+
     @staticmethod
     def tensors(params: Mapping, prefix: str) -> Dict[str, TensorInfo]:
         h, i = params["hidden_size"], params["intermediate_size"]
@@ -30,9 +32,9 @@ class SwiGLU:
         self.rt = rt
         self.hidden = int(params["hidden_size"])
         self.inter = int(params["intermediate_size"])
-        self.w_gate_up = weights.load_fused(
-            [prefix + "gate_proj.weight", prefix + "up_proj.weight"], [self.inter, self.inter], self.hidden)
-        self.w_down = weights.load(prefix + "down_proj.weight", "matrix")
+        self.w_gate_up = held(weights.load_fused(
+            [prefix + "gate_proj.weight", prefix + "up_proj.weight"], [self.inter, self.inter], self.hidden), rt)
+        self.w_down = held(weights.load(prefix + "down_proj.weight", "matrix"), rt)
 
     def can_fuse(self, n_rows: int, norm) -> bool:
         rt = self.rt

@@ -61,6 +61,11 @@ def linear(x: torch.Tensor, w: torch.Tensor, rt: Runtime, out_dtype: Optional[to
     return torch.mm(x, w.t(), out_dtype=out_dtype)
 
 
+def held(w: torch.Tensor, rt: Runtime):
+    """A part's matrix as the engine holds it: as loaded, or in 4 bits."""
+    return K.pack_weight4(w, K.bits4_group(w.shape[1], rt.bits_group)) if rt.weight_bits == 4 else w
+
+
 EXPAND_BYTES = 48 << 20   # of weights at a time that a product of many rows takes out of their 4 bits: they stay in L2 until the product has read them
 
 
