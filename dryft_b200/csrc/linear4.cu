@@ -2,20 +2,21 @@
 //
 // The weights' layout.  16 rows of W by 64 inputs are 32 lanes x 16 bytes: lane (r, c) holds word s = 0..3 for the inputs 16 s + 4c + e, nibble i of the low
 // half being row r (i even) or r + 8 (i odd), e = 2 (i / 2), and of the high half the same with e + 1 -- the order in which the lane's registers of a
-// 16 x 16 operand come out of the word (`code_pair`).  Blocks of 64 inputs of a tile of 16 rows follow one another, then the next tile; the last block and the last tile
-// are filled up with codes that nothing reads as numbers.  Beside them [tile][group][r][row r, row r + 8] of (s, z).
+// 16 x 16 operand come out of the word (`code_pair`).  Blocks of 64 inputs of a tile of 16 rows follow one another, an even number of them, then the next tile.  Beside
+// them [tile][group][r][row r, row r + 8] of (s, z).  Behind the last input and the last row s and z are zeros.
 #include "four_bit.cuh"
 
 namespace {
 constexpr int WARPS = 4, ROWS = 8;
+__host__ __device__ constexpr int blocks_of(int k) { return (k + 127) / 128 * 2; }                              // of 64 inputs, as laid out
+__host__ __device__ constexpr int groups_of(int k, int group) { return (k + 127) / 128 * 128 / group; }
 
-// A block per 16 rows of W and ROWS rows of x, the inputs dealt out to the warps in blocks of 64.
-template <typename T, typename O>
-__global__ void __launch_bounds__(WARPS * 32) linear4_rows_kernel(const T* x, long long x_stride, const uint4* __restrict__ codes, const uint2* __restrict__ scales,
-                                                                  O* y, int m, int n, int k, int group) {
+// 32-bit: a block per 16 rows of W and ROWS rows of x, the inputs dealt out to the warps in blocks of 64.
+__global__ void __launch_bounds__(WARPS * 32) linear4_f32_kernel(const float* x, long long x_stride, const uint4* __restrict__ codes,
+                                                                 const uint2* __restrict__ scales, float* y, int m, int n, int k, int group) {
   __shared__ float part[WARPS][2][ROWS][8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
-  const int tile = blockIdx.x, m0 = blockIdx.y * ROWS, rows = min(ROWS, m - m0), blocks = (k + 63) / 64, groups = k / group;
+  const int tile = blockIdx.x, m0 = blockIdx.y * ROWS, rows = min(ROWS, m - m0), blocks = blocks_of(k), groups = groups_of(k, group);
   float acc[2][ROWS];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) acc[0][i] = acc[1][i] = 0.f;
@@ -38,7 +39,7 @@ __global__ void __launch_bounds__(WARPS * 32) linear4_rows_kernel(const T* x, lo
         if (i >= rows) break;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float xv = to_f32<T>(x[(m0 + i) * x_stride + at + 4 * c + e]);
+          const float xv = x[(m0 + i) * x_stride + at + 4 * c + e];
           acc[0][i] = fmaf(w[0][e], xv, acc[0][i]);
           acc[1][i] = fmaf(w[1][e], xv, acc[1][i]);
         }
@@ -60,14 +61,14 @@ __global__ void __launch_bounds__(WARPS * 32) linear4_rows_kernel(const T* x, lo
     float v = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) v += part[w][row >> 3][mm][row & 7];
-    if (tile * 16 + row < n) y[(size_t)(m0 + mm) * n + tile * 16 + row] = from_f32<O>(v);
+    if (tile * 16 + row < n) y[(size_t)(m0 + mm) * n + tile * 16 + row] = v;
   }
 }
 
 // A warp per block of 64 inputs of a tile: what its codes stand for, in T.
 template <typename T>
 __global__ void __launch_bounds__(256) weight4_expand_kernel(const uint4* __restrict__ codes, const uint2* __restrict__ scales, T* w, int n, int k, int group) {
-  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, blocks = (k + 63) / 64, groups = k / group;
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, blocks = blocks_of(k), groups = groups_of(k, group);
   const long long at = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), total = (long long)((n + 15) / 16) * blocks;
   if (at >= total) return;
   const long long tile = at / blocks;
@@ -90,25 +91,398 @@ __global__ void __launch_bounds__(256) weight4_expand_kernel(const uint4* __rest
   }
 }
 
-template <typename T, typename O>
-int rows(const void* x, long long x_stride, const void* codes, const void* scales, void* y, int m, int n, int k, int group, cudaStream_t st) {
-  linear4_rows_kernel<T, O><<<dim3((n + 15) / 16, (m + ROWS - 1) / ROWS), WARPS * 32, 0, st>>>((const T*)x, x_stride, (const uint4*)codes, (const uint2*)scales,
-                                                                                             (O*)y, m, n, k, group);
-  return launch_status();
+// ---------------------------------------------------------------------------------------------- bfloat16: tensor cores
+// y^T = W x^T on mma.sync.m16n8k16: 16 rows of W are the 16-row operand, straight from the codes (16 + c, `code_pair`), eight rows of x the columns.  A group's
+// products are summed over 16 + c in a 32-bit accumulator of their own, then  y += s acc + (z - 23.5 s) sum_k x  in 32 bits, so nothing is rounded below
+// 32 bits before the result.  The warps of a block share a tile's inputs: each walks its own blocks of 64, their sums meet in shared memory.
+typedef __nv_bfloat16 bf16;
+constexpr int MMA_WARPS = 8;
+
+__device__ __forceinline__ float2 two_of(unsigned w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from));
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N)); }
+__device__ __forceinline__ unsigned word_of(uint4 v, int s) { return s == 0 ? v.x : s == 1 ? v.y : s == 2 ? v.z : v.w; }
+
+// A group's sums into the results: rows r and r + 8 of W, columns 2c and 2c + 1 of x, whose sums over the group are s0 and s1.
+__device__ __forceinline__ void add_group(float (&acc)[4], const float (&part)[4], uint2 sz, float s0, float s1) {
+  const GroupCode lo = unpack_code(sz.x), hi = unpack_code(sz.y);
+  const float zl = fmaf(-CODE_BIAS, lo.s, lo.z), zh = fmaf(-CODE_BIAS, hi.s, hi.z);
+  acc[0] = fmaf(lo.s, part[0], fmaf(zl, s0, acc[0]));
+  acc[1] = fmaf(lo.s, part[1], fmaf(zl, s1, acc[1]));
+  acc[2] = fmaf(hi.s, part[2], fmaf(zh, s0, acc[2]));
+  acc[3] = fmaf(hi.s, part[3], fmaf(zh, s1, acc[3]));
+}
+
+// The warps' sums of R tiles of W and NT of x, in the warps' order, into the results.  `red`: [warp][R][NT][lane][4].
+template <int NT, int R, typename O>
+__device__ __forceinline__ void join_warps(float (&acc)[R][NT][4], float* red, O* y, int m, int n, int row0) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __syncthreads();   // the last tile's sums have been read
+#pragma unroll
+  for (int t = 0; t < R; ++t)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      *reinterpret_cast<float4*>(red + ((warp * R + t) * NT + j) * 128 + lane * 4) = make_float4(acc[t][j][0], acc[t][j][1], acc[t][j][2], acc[t][j][3]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[t][j][e] = 0.f;
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < R * NT * 128; i += MMA_WARPS * 32) {
+    const int row = i % (16 * R), col = i / (16 * R), t = row >> 4;
+    // row (row & 15), column (col & 7) of a tile: lane (row & 7) * 4 + (col & 7) / 2, element 2 (row & 15 >= 8) + (col & 1)
+    const int place = (t * NT + (col >> 3)) * 128 + ((row & 7) * 4 + ((col & 7) >> 1)) * 4 + 2 * ((row >> 3) & 1) + (col & 1);
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < MMA_WARPS; ++w) v += red[w * R * NT * 128 + place];
+    if (row0 + row < n && col < m) y[(size_t)col * n + row0 + row] = from_f32<O>(v);
+  }
+}
+
+// Few rows of x (up to 16), all of whose numbers fit in shared memory: bound by the codes' bytes.  A block of 16 warps is 16 / TEAM teams; a team takes
+// a tile of 16 rows of W at a time, its warps the tile's inputs in turn shares.  Each warp copies its own share of the codes into its own ring, SLOTS - 1 slots of
+// PB blocks of 64 inputs ahead, across the ends of tiles, so that the requests never drain; a lane reads what it copied itself, and nothing waits for another warp
+// but a tile's end.
+constexpr int FEW_WARPS = 16;
+
+template <int NT, int GS, int TEAM, int PB, int SLOTS> struct Few {
+  static constexpr int SCALES = GS == 8 ? 1 : PB * 4 / GS;    // groups that begin in a slot
+  static constexpr int SLOT = PB * 512 + SCALES * 256;
+  static constexpr int REDS = TEAM == FEW_WARPS ? 1 : 2;       // buffers for a tile's sums
+  static constexpr size_t RED_BYTES = (size_t)REDS * FEW_WARPS * NT * 512, RING_BYTES = (size_t)FEW_WARPS * SLOTS * SLOT;
+  __host__ __device__ static int slots_of(int k) { return blocks_of(k) / PB; }   // of a tile
+  // rows of x lie 32 bytes further apart than a multiple of 128, which keeps a warp's reads of eight rows apart
+  __host__ __device__ static int row_bytes(int k) { return blocks_of(k) * 128 + 32; }
+  static size_t bytes(int m, int k) { return RED_BYTES + RING_BYTES + (size_t)slots_of(k) * SCALES * NT * 64 + (size_t)m * row_bytes(k); }
+};
+
+template <int NT, int GS, int TEAM, int PB, int SLOTS, typename O>
+__global__ void __launch_bounds__(FEW_WARPS * 32, 1) linear4_few_kernel(const bf16* x, long long x_stride, const uint4* __restrict__ codes,
+                                                                        const uint2* __restrict__ scales, O* y, int m, int n, int k, int group_bits) {
+  typedef Few<NT, GS, TEAM, PB, SLOTS> F;
+  constexpr int SCALES = F::SCALES, SLOT = F::SLOT, TEAMS = FEW_WARPS / TEAM, STEPS = PB * 4 / SCALES;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3, team = warp / TEAM;
+  const int tiles = (n + 15) / 16, slots = F::slots_of(k), row_bytes = F::row_bytes(k);
+  float* const red = reinterpret_cast<float*>(smem);
+  float4* const xs = reinterpret_cast<float4*>(smem + F::RED_BYTES);   // [slot][SCALES][NT][c]: sums of columns 2c, 2c + 1 over the group, -23.5 times them
+  unsigned char* const rings = reinterpret_cast<unsigned char*>(xs + slots * SCALES * NT * 4);
+  unsigned char* const rows = rings + F::RING_BYTES;
+  const int per = (slots + TEAM - 1) / TEAM, s0 = min(slots, warp % TEAM * per), ns = min(slots, s0 + per) - s0;
+  // the team's tiles: block and team together count through them, the block's number first
+  const int first = blockIdx.x + team * gridDim.x, step = gridDim.x * TEAMS, mine = first < tiles ? (tiles - 1 - first) / step + 1 : 0;
+  const int total = mine * ns;   // the warp's slots
+
+  // Slot i of the warp goes into place i mod SLOTS of its ring.  Codes and scales lie slot behind slot, tile behind tile.  (A group of 128 has two slots of one
+  // block: the scale is then the same for both.)
+  int sent = 0, until = ns;
+  unsigned at = first * slots + s0;
+  const unsigned jump = step * slots - ns, ring = (unsigned)__cvta_generic_to_shared(rings + warp * F::RING_BYTES / FEW_WARPS) + lane * 16;
+  const unsigned ring_scales = ring - lane * 8 + PB * 512;
+  const uint4* const my_codes = codes + lane;
+  const uint2* const my_scales = scales + r;
+  const int half_scale = GS < 8 && PB == 1 && group_bits == 7;
+  auto request = [&](int place) {
+    if (sent < total) {
+      const uint4* const from = my_codes + (size_t)at * (PB * 32);
+      const uint2* const from_scale = my_scales + (size_t)(PB == 1 && GS == 4 ? at >> half_scale : at) * (SCALES * 8);
+#pragma unroll
+      for (int i = 0; i < PB; ++i) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ring + place * SLOT + i * 512), "l"(from + i * 32));
+#pragma unroll
+      for (int g = 0; g < SCALES; ++g)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(ring_scales + place * SLOT + g * 256), "l"(from_scale + g * 8));
+      ++at;
+      if (--until == 0) {
+        until = ns;
+        at += jump;
+      }
+    }
+    ++sent;
+    copies_end();
+  };
+  let_next_launch_in();
+#pragma unroll
+  for (int i = 0; i < SLOTS - 1; ++i) request(i);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int pieces = blocks_of(k) * 8;   // of 16 bytes in a row of x
+  for (int row = 0; row < m; ++row)
+    for (int i = threadIdx.x; i < pieces; i += FEW_WARPS * 32) {
+      unsigned char* const to = rows + (size_t)row * row_bytes + i * 16;
+      if (8 * i < k)
+        copy16(to, x + row * x_stride + 8 * i);
+      else
+        *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);
+    }
+  copies_end();
+  copies_wait<0>();
+  __syncthreads();
+  const unsigned char* at_row[NT];   // the lane's share of the first step of its column; columns behind the last one repeat it
+#pragma unroll
+  for (int j = 0; j < NT; ++j) at_row[j] = rows + (size_t)min(8 * j + r, m - 1) * row_bytes + 8 * c;
+  for (int i = warp; i < slots * SCALES; i += FEW_WARPS)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      float sum = 0.f;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        const uint2 v = *reinterpret_cast<const uint2*>(at_row[j] + (i * STEPS + s) * 32);
+        const float2 p = two_of(v.x), q = two_of(v.y);
+        sum += (p.x + p.y) + (q.x + q.y);
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      const float a = __shfl_sync(0xffffffffu, sum, 8 * c), b = __shfl_sync(0xffffffffu, sum, 8 * c + 4);
+      if (r == 0) xs[(i * NT + j) * 4 + c] = make_float4(a, b, -CODE_BIAS * a, -CODE_BIAS * b);
+    }
+  __syncthreads();
+
+  float acc[NT][4];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+  int tile = 0;
+  // A team's sums of a tile, in the warps' order; with two buffers the last tile's are read while this one's are written.
+  const int out_row = threadIdx.x & 15, out_col = threadIdx.x % (TEAM * 32) >> 4;   // lane (row & 7) * 4 + (col & 7) / 2, element 2 (row >= 8) + (col & 1)
+  const float* const out_from = red + team * TEAM * NT * 128 + (out_row & 7) * 16 + ((out_col & 7) >> 1) * 4 + 2 * (out_row >> 3) + (out_col & 1);
+  auto tile_done = [&] {
+    const int buffer = F::REDS == 2 ? (tile & 1) * FEW_WARPS * NT * 128 : 0;
+    if (F::REDS == 1 && tile > 0) __syncthreads();
+    float* const to = red + buffer + warp * NT * 128 + lane * 4;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      *reinterpret_cast<float4*>(to + j * 128) = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
+      acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+    }
+    asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(TEAM * 32) : "memory");
+    const int row = (first + tile * step) * 16 + out_row;
+#pragma unroll
+    for (int i = 0; i < (NT * 128 + TEAM * 32 - 1) / (TEAM * 32); ++i) {
+      const int col = out_col + i * (TEAM * 2);
+      if (col >= NT * 8) continue;
+      const float* const place = out_from + buffer + (col >> 3) * 128;
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < TEAM; ++w) v += place[w * NT * 128];
+      if (row < n && col < m) y[(size_t)col * n + row] = from_f32<O>(v);
+    }
+    ++tile;
+  };
+  if (ns == 0)
+    for (int t = 0; t < mine; ++t) tile_done();
+  const unsigned char* const my_ring = rings + warp * F::RING_BYTES / FEW_WARPS;
+  int here = s0;
+  for (int i = 0; i < total; i += SLOTS) {
+#pragma unroll
+    for (int u = 0; u < SLOTS; ++u) {
+      if (i + u >= total) break;
+      request((u + SLOTS - 1) % SLOTS);   // into the place that was read last
+      copies_wait<SLOTS - 1>();
+      const unsigned char* const from = my_ring + u * SLOT;
+      uint4 w[PB];
+#pragma unroll
+      for (int b = 0; b < PB; ++b) w[b] = *reinterpret_cast<const uint4*>(from + b * 512 + lane * 16);
+      const float4* const my_xs = xs + here * (SCALES * NT * 4) + c;
+#pragma unroll
+      for (int g = 0; g < SCALES; ++g) {
+        const uint2 sz = *reinterpret_cast<const uint2*>(from + PB * 512 + g * 256 + lane * 8);
+        const GroupCode lo = unpack_code(sz.x), hi = unpack_code(sz.y);
+        float4 sum[NT];
+        float part[NT][4];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          sum[j] = my_xs[(g * NT + j) * 4];
+          part[j][0] = part[j][2] = sum[j].z;    // the products are summed on top of what takes the 23.5 out
+          part[j][1] = part[j][3] = sum[j].w;
+        }
+#pragma unroll
+        for (int q = g * STEPS; q < (g + 1) * STEPS; ++q) {
+          const unsigned v = word_of(w[q / 4], q % 4), a0 = code_pair(v, 0), a1 = code_pair(v, 1), a2 = code_pair(v, 2), a3 = code_pair(v, 3);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const uint2 bx = *reinterpret_cast<const uint2*>(at_row[j] + here * (PB * 128) + q * 32);
+            mma_16816(part[j], a0, a1, a2, a3, bx.x, bx.y);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          acc[j][0] = fmaf(lo.s, part[j][0], fmaf(lo.z, sum[j].x, acc[j][0]));
+          acc[j][1] = fmaf(lo.s, part[j][1], fmaf(lo.z, sum[j].y, acc[j][1]));
+          acc[j][2] = fmaf(hi.s, part[j][2], fmaf(hi.z, sum[j].x, acc[j][2]));
+          acc[j][3] = fmaf(hi.s, part[j][3], fmaf(hi.z, sum[j].y, acc[j][3]));
+        }
+      }
+      if (++here == s0 + ns) {
+        here = s0;
+        tile_done();
+      }
+    }
+  }
+  copies_wait<0>();
+}
+
+// More rows, or more inputs than fit: R tiles of 16 rows of W against NT of x, a block of 64 inputs at a time from registers, the next one on its way.
+template <int NT, int R, int GS> struct Chunk {
+  uint4 w[R];
+  uint2 sz[R][4 / GS], x[NT][4];
+};
+
+template <int NT, int R, int GS, typename O>
+__global__ void __launch_bounds__(MMA_WARPS * 32) linear4_mma_kernel(const bf16* x, long long x_stride, const uint4* __restrict__ codes,
+                                                                     const uint2* __restrict__ scales, O* y, int m, int n, int k, int group) {
+  constexpr int NG = 4 / GS;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
+  const int blocks = blocks_of(k), groups = groups_of(k, group), tiles = (n + 15) / 16;
+  const int per = (blocks + MMA_WARPS - 1) / MMA_WARPS, b0 = min(blocks, warp * per), b1 = min(blocks, b0 + per);
+  auto load = [&](Chunk<NT, R, GS>& q, int b) {
+#pragma unroll
+    for (int t = 0; t < R; ++t) {
+      const int tile = min((int)blockIdx.x * R + t, tiles - 1);   // the last unit may repeat a tile; it is not stored twice
+      q.w[t] = codes[((size_t)tile * blocks + b) * 32 + lane];
+#pragma unroll
+      for (int g = 0; g < NG; ++g) q.sz[t][g] = scales[((size_t)tile * groups + (64 * b + 16 * GS * g) / group) * 8 + r];
+    }
+  };
+  auto load_x = [&](Chunk<NT, R, GS>& q, int b) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int col = 64 * b + 16 * s + 4 * c, row = 8 * j + r;
+        q.x[j][s] = col < k && row < m ? __ldcg(reinterpret_cast<const uint2*>(x + row * x_stride + col)) : make_uint2(0, 0);
+      }
+  };
+  let_next_launch_in();
+  Chunk<NT, R, GS> now;
+  if (b0 < b1) load(now, b0);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (b0 < b1) load_x(now, b0);
+  float acc[R][NT][4];
+#pragma unroll
+  for (int t = 0; t < R; ++t)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[t][j][e] = 0.f;
+  for (int b = b0; b < b1; ++b) {
+    Chunk<NT, R, GS> next;
+    if (b + 1 < b1) {
+      load(next, b + 1);
+      load_x(next, b + 1);
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float part[R][NT][4], sum[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        sum[j] = 0.f;
+#pragma unroll
+        for (int t = 0; t < R; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) part[t][j][e] = 0.f;
+      }
+#pragma unroll
+      for (int s = g * GS; s < (g + 1) * GS; ++s) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const float2 p = two_of(now.x[j][s].x), q = two_of(now.x[j][s].y);
+          sum[j] += (p.x + p.y) + (q.x + q.y);
+        }
+#pragma unroll
+        for (int t = 0; t < R; ++t) {
+          const unsigned v = word_of(now.w[t], s), a0 = code_pair(v, 0), a1 = code_pair(v, 1), a2 = code_pair(v, 2), a3 = code_pair(v, 3);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) mma_16816(part[t][j], a0, a1, a2, a3, now.x[j][s].x, now.x[j][s].y);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
+        sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
+        const float s0 = __shfl_sync(0xffffffffu, sum[j], 8 * c), s1 = __shfl_sync(0xffffffffu, sum[j], 8 * c + 4);
+#pragma unroll
+        for (int t = 0; t < R; ++t) add_group(acc[t][j], part[t][j], now.sz[t][g], s0, s1);
+      }
+    }
+    now = next;
+  }
+  join_warps<NT, R, O>(acc, reinterpret_cast<float*>(smem), y, m, n, blockIdx.x * R * 16);
+}
+
+constexpr size_t SMEM_MOST = 227 * 1024;
+
+template <typename... P, typename... A> int launch(void (*kern)(P...), bool& asked, int grid, int threads, size_t bytes, int pdl, cudaStream_t st, A... a) {
+  if (!asked) {   // (asking twice does no harm)
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_MOST);
+    if (e != cudaSuccess) return (int)e;
+    asked = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, (P)a...);
+  return e != cudaSuccess ? (int)e : launch_status();
+}
+
+struct Args { const void *x; long long x_stride; const void *codes, *scales; void* y; int m, n, k, group, pdl; cudaStream_t st; };
+
+template <int NT, int GS, int TEAM, int PB, int SLOTS, typename O> int few(const Args& a) {
+  static bool asked = false;
+  const int tiles = (a.n + 15) / 16;
+  return launch(linear4_few_kernel<NT, GS, TEAM, PB, SLOTS, O>, asked, tiles < 148 ? tiles : 148, FEW_WARPS * 32, Few<NT, GS, TEAM, PB, SLOTS>::bytes(a.m, a.k), a.pdl,
+                a.st, (const bf16*)a.x, a.x_stride, (const uint4*)a.codes, (const uint2*)a.scales, (O*)a.y, a.m, a.n, a.k, __builtin_ctz(a.group));
+}
+// Four warps a tile where shared memory has room for their rings (x of 8 rows: up to about 6,000 inputs), else all sixteen with shorter rings.  2,560 inputs,
+// one row, four / eight / sixteen warps a tile: 151,936 outputs 55.6 / 63.6 / 81.9 us, 6,144 outputs 4.8 / 5.4 / 5.7 us (a tile's end costs each warp as much as
+// half a slot); 2,560 outputs of 9,728 inputs, hardly more tiles than multiprocessors, 9.6 / 9.7 / 10.2 us.
+template <int NT, int GS, typename O> bool few_rows(const Args& a, int* rc) {
+  constexpr int GM = GS == 8 ? 4 : GS;
+  if (Few<NT, GS, 4, 2, 4>::bytes(a.m, a.k) <= SMEM_MOST) return *rc = few<NT, GS, 4, 2, 4, O>(a), true;
+  if (Few<NT, GM, 16, 1, 4>::bytes(a.m, a.k) <= SMEM_MOST) return *rc = few<NT, GM, 16, 1, 4, O>(a), true;
+  return false;
+}
+template <int NT, int R, int GS, typename O> int more(const Args& a) {
+  static bool asked = false;
+  return launch(linear4_mma_kernel<NT, R, GS, O>, asked, ((a.n + 15) / 16 + R - 1) / R, MMA_WARPS * 32, (size_t)MMA_WARPS * R * NT * 512, a.pdl, a.st, (const bf16*)a.x, a.x_stride,
+                (const uint4*)a.codes, (const uint2*)a.scales, (O*)a.y, a.m, a.n, a.k, a.group);
+}
+template <int GS, typename O> int by_rows(const Args& a) {
+  constexpr int GM = GS == 8 ? 4 : GS;
+  const int nt = (a.m + 7) / 8;
+  int rc;
+  if (nt == 1) return few_rows<1, GS, O>(a, &rc) ? rc : more<1, 2, GM, O>(a);
+  if (nt == 2) return few_rows<2, GS, O>(a, &rc) ? rc : more<2, 2, GM, O>(a);
+  if (nt <= 4) return more<4, 2, GM, O>(a);
+  if (nt <= 6) return more<6, 2, GM, O>(a);
+  return more<8, 2, GM, O>(a);
+}
+template <typename O> int by_group(const Args& a) {
+  return (a.group == 128 ? by_rows<8, O> : a.group == 64 ? by_rows<4, O> : a.group == 32 ? by_rows<2, O> : by_rows<1, O>)(a);
 }
 }  // namespace
 
 DRYFT_API int dryft_linear4(int is_bf16, int out_bf16, const void* x, long long x_stride, const void* codes, const void* scales, void* y, int m, int n, int k,
-                            int group, void* stream) {
+                            int group, int pdl, void* stream) {
   if (m <= 0 || n <= 0) return 0;
-  typedef __nv_bfloat16 bf16;
-  auto f = is_bf16 ? (out_bf16 ? rows<bf16, bf16> : rows<bf16, float>) : rows<float, float>;
-  return f(x, x_stride, codes, scales, y, m, n, k, group, (cudaStream_t)stream);
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (is_bf16) return (out_bf16 ? by_group<bf16> : by_group<float>)({x, x_stride, codes, scales, y, m, n, k, group, pdl, st});
+  linear4_f32_kernel<<<dim3((n + 15) / 16, (m + ROWS - 1) / ROWS), WARPS * 32, 0, st>>>((const float*)x, x_stride, (const uint4*)codes, (const uint2*)scales,
+                                                                                       (float*)y, m, n, k, group);
+  return launch_status();
 }
 
 DRYFT_API int dryft_weight4_expand(int is_bf16, const void* codes, const void* scales, void* w, int n, int k, int group, void* stream) {
   if (n <= 0) return 0;
-  const long long total = (long long)((n + 15) / 16) * ((k + 63) / 64);
+  const long long total = (long long)((n + 15) / 16) * blocks_of(k);
   const unsigned grid = (unsigned)((total + 7) / 8);
   if (is_bf16)
     weight4_expand_kernel<__nv_bfloat16><<<grid, 256, 0, (cudaStream_t)stream>>>((const uint4*)codes, (const uint2*)scales, (__nv_bfloat16*)w, n, k, group);

@@ -2471,7 +2471,7 @@ def _bits4_group(size: int, group: int, what: str) -> None:
 def linear4_lib() -> ctypes.CDLL:
     """Products with weights held in 4 bits."""
     return _single_lib("linear4", {
-        "dryft_linear4": [_i, _i, _p, _ll, _p, _p, _p, _i, _i, _i, _i, _p],
+        "dryft_linear4": [_i, _i, _p, _ll, _p, _p, _p, _i, _i, _i, _i, _i, _p],
         "dryft_weight4_expand": [_i, _p, _p, _p, _i, _i, _i, _p],
     })
 
@@ -2481,11 +2481,22 @@ class Weight4:
     """A matrix ``[n, k]`` held in 4 bits, laid out once for the products (``pack_weight4`` makes it).  ``codes``: uint8, 16 rows by 64 inputs
     as a warp's lanes read them; ``scales``: bfloat16, (s, z) of every row and group."""
 
-    codes: torch.Tensor     # uint8 [tiles of 16 rows, blocks of 64 inputs, 512]
-    scales: torch.Tensor    # bfloat16 [tiles, k / group, 8, 2, 2]
+    codes: torch.Tensor     # uint8 [tiles of 16 rows, blocks of 64 inputs (an even number), 512]
+    scales: torch.Tensor    # bfloat16 [tiles, groups (of as many inputs), 8, 2, 2]
     n: int
     k: int
     group: int
+
+    def __post_init__(self) -> None:
+        """What every use of a weight relies on is looked at once, here."""
+        _bits4_group(self.k, self.group, "Weight4")
+        tiles, wide = (self.n + 15) // 16, (self.k + 127) // 128 * 128
+        for t, name, dtype, shape in ((self.codes, "codes", torch.uint8, (tiles, wide // 64, 512)),
+                                      (self.scales, "scales", torch.bfloat16, (tiles, wide // self.group, 8, 2, 2))):
+            if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.data_ptr() % 16:
+                raise KernelError(f"Weight4: {name} are {dtype} of shape {shape}, contiguous, on a 16-byte boundary")
+        if self.n <= 0 or self.codes.device != self.scales.device:
+            raise KernelError("Weight4: no rows, or codes and scales on two devices")
 
     @property
     def shape(self) -> Tuple[int, int]:
@@ -2537,9 +2548,10 @@ def pack_weight4(w: torch.Tensor, group: int = 64) -> Weight4:
     _bits4_group(k, group, "pack_weight4")
     if n <= 0:
         raise KernelError("pack_weight4: no rows")
-    tiles, blocks = (n + 15) // 16, (k + 63) // 64
+    tiles, wide = (n + 15) // 16, (k + 127) // 128 * 128
+    blocks, groups = wide // 64, wide // group
     codes = torch.empty(tiles, blocks, 512, dtype=torch.uint8, device=w.device)
-    scales = torch.empty(tiles, k // group, 8, 2, 2, dtype=torch.bfloat16, device=w.device)
+    scales = torch.empty(tiles, groups, 8, 2, 2, dtype=torch.bfloat16, device=w.device)
     step = max(1, (1 << 24) // (16 * k))           # tiles at a time: bounds what this holds beside the result
     for t0 in range(0, tiles, step):
         part = w[t0 * 16:(t0 + step) * 16]
@@ -2550,35 +2562,41 @@ def pack_weight4(w: torch.Tensor, group: int = 64) -> Weight4:
         # [tile, row half h, r, block, step s, quarter c, pair i, e] -> bytes of lane (r, c), word s: nibble 2 i + h of half e
         a = full.view(nt, 2, 8, blocks, 4, 4, 2, 2).permute(0, 3, 2, 5, 4, 7, 6, 1)   # tile, block, r, c, s, e, i, h
         codes[t0:t0 + nt] = (a[..., 0] | (a[..., 1] << 4)).reshape(nt, blocks, 512)
-        fs = torch.zeros(nt * 16, k // group, 2, dtype=torch.bfloat16, device=w.device)
-        fs[:part.shape[0]] = sz
-        scales[t0:t0 + nt] = fs.view(nt, 2, 8, k // group, 2).permute(0, 3, 2, 1, 4)
+        fs = torch.zeros(nt * 16, groups, 2, dtype=torch.bfloat16, device=w.device)
+        fs[:part.shape[0], :k // group] = sz
+        scales[t0:t0 + nt] = fs.view(nt, 2, 8, groups, 2).permute(0, 3, 2, 1, 4)
     return Weight4(codes, scales, n, k, group)
 
 
 def _need_weight4(w: Weight4) -> None:
     if not isinstance(w, Weight4):
         raise KernelError(f"weight: expected a Weight4 (pack_weight4 makes one), got {type(w).__name__}")
-    _bits4_group(w.k, w.group, "Weight4")
-    tiles = (w.n + 15) // 16
-    _need(w.codes, "weight codes", torch.uint8, (tiles, (w.k + 63) // 64, 512))
-    _need(w.scales, "weight scales", torch.bfloat16, (tiles, w.k // w.group, 8, 2, 2))
+    if not w.codes.is_cuda:
+        raise KernelError(f"weight: is on {w.device}; dryft_b200 kernels run on a CUDA device only")
 
 
 def _rows_in(x, name: str, width: int) -> int:
     """Rows of ``width`` numbers that may lie ``x.stride(0)`` apart, on 16-byte boundaries; the distance."""
-    if not isinstance(x, torch.Tensor) or x.device.type != "cuda":
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise KernelError(f"{name}: expected a tensor on a CUDA device")
-    if x.dim() != 2 or x.shape[1] != width or (x.shape[1] > 1 and x.stride(1) != 1):
-        raise KernelError(f"{name}: expected rows of {width} consecutive numbers, got shape {tuple(x.shape)}, strides {x.stride()}")
-    step = x.stride(0) if x.shape[0] > 1 else width
-    if step < width or (step * x.element_size()) % 16 or x.data_ptr() % 16:
-        raise KernelError(f"{name}: rows start on 16-byte boundaries and do not overlap (stride {x.stride(0)}, address {x.data_ptr():#x})")
+    shape = x.shape
+    if len(shape) != 2 or shape[1] != width:
+        raise KernelError(f"{name}: expected rows of {width} numbers, got shape {tuple(shape)}")
+    step, one = x.stride()
+    if shape[0] == 1:
+        step = width
+    if one != 1 or step < width or (step * x.element_size()) % 16 or x.data_ptr() % 16:
+        raise KernelError(f"{name}: rows of consecutive numbers start on 16-byte boundaries and do not overlap (strides {x.stride()}, address {x.data_ptr():#x})")
     return step
 
 
-def linear4(x, w: Weight4, out) -> None:
-    """``out = x @ w.T`` for up to 64 rows; ``x`` float32 or bfloat16, ``out`` of the same type or float32."""
+_linear4_fn = None
+
+
+def linear4(x, w: Weight4, out, pdl: bool = False) -> None:
+    """``out = x @ w.T`` for up to 64 rows; ``x`` float32 or bfloat16, ``out`` of the same type or float32.  ``pdl``: a programmatic dependent (its
+    first weights are requested while the launch before it drains)."""
+    global _linear4_fn, launch_count
     _need_weight4(w)
     step = _rows_in(x, "x", w.k)
     m = x.shape[0]
@@ -2589,7 +2607,12 @@ def linear4(x, w: Weight4, out) -> None:
     if out_bf16 and not is_bf16:
         raise KernelError("linear4: 32-bit activations give 32-bit results")
     _need(out, "out", None, (m, w.n))
-    _ok(linear4_lib().dryft_linear4(is_bf16, out_bf16, _ptr(x), step, _ptr(w.codes), _ptr(w.scales), _ptr(out), m, w.n, w.k, w.group, _stream()), "linear4")
+    if _linear4_fn is None:
+        _linear4_fn = linear4_lib().dryft_linear4
+    rc = _linear4_fn(is_bf16, out_bf16, x.data_ptr(), step, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), m, w.n, w.k, w.group, pdl, _stream())
+    if rc:
+        _ok(rc, "linear4")
+    launch_count += 1
 
 
 def weight4_expand(w: Weight4, out) -> None:

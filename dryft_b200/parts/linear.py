@@ -30,7 +30,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, rt: Runtime, out_dtype: Optional[to
     if w.shape[1] != k:
         raise ValueError(f"linear: activations have width {k}, weight is {tuple(w.shape)}")
     if isinstance(w, K.Weight4):
-        return _linear4(x, w, out_dtype)
+        return _linear4(x, w, rt, out_dtype)
     if x.dtype == torch.float32:
         if w.dtype != torch.float32:
             raise ValueError(f"linear: 32-bit activations need a 32-bit weight, got {w.dtype}")
@@ -69,13 +69,13 @@ def held(w: torch.Tensor, rt: Runtime):
 EXPAND_BYTES = 48 << 20   # of weights at a time that a product of many rows takes out of their 4 bits: they stay in L2 until the product has read them
 
 
-def _linear4(x: torch.Tensor, w: K.Weight4, out_dtype: torch.dtype) -> torch.Tensor:
+def _linear4(x: torch.Tensor, w: K.Weight4, rt: Runtime, out_dtype: torch.dtype) -> torch.Tensor:
     """Up to ``K.LINEAR4_ROWS`` rows the kernel reads the codes; more rows take the weights out of their 4 bits, a part at a time, for the product
     that such rows run on otherwise."""
     m, (n, k) = x.shape[0], w.shape
     if m <= K.LINEAR4_ROWS:
         out = torch.empty((m, n), dtype=out_dtype, device=x.device)
-        K.linear4(x, w, out)
+        K.linear4(x, w, out, pdl=rt.pdl)
         return out
     out = torch.empty((m, n), dtype=out_dtype, device=x.device)
     step = max(16, EXPAND_BYTES // (k * x.element_size()) // 16 * 16)

@@ -78,7 +78,7 @@ def test_layout_of_packed_weights(n, k, group, dtype):
     w[0, :group] = 0.5
     w4 = K.pack_weight4(w, group)
     values, s, z = P.group_values(w, group)
-    codes, scales = w4.codes.view(-1, (k + 63) // 64, 32, 4, 4), w4.scales.double()
+    codes, scales = w4.codes.view(-1, (k + 127) // 128 * 2, 32, 4, 4), w4.scales.double()
     for row in range(n):
         tile, h, r = row // 16, (row % 16) // 8, row % 8
         for col in range(k):
