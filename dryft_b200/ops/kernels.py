@@ -2758,10 +2758,17 @@ def attn4_lib(head_dim: int, heads: int, page: int, group: int) -> ctypes.CDLL:
         return lib
 
 
-def attn4_splits(n: int, n_kv: int, max_kv: int, window: Optional[int]) -> int:
-    """Into how many blocks the keys of a row and key head are cut: about two blocks a multiprocessor, at least 64 keys each."""
-    keys = min(max_kv, window) if window else max_kv
-    return max(1, min(32, 296 // max(1, n * n_kv), (keys + 63) // 64))
+ATTN4_CLUSTER = 8   # up to this many splits of the tensor-core kernel are the blocks of a cluster
+
+
+def attn4_splits(blocks: int, max_kv: int, window: Optional[int], bf16: bool) -> int:
+    """Into how many splits the keys of each of ``blocks`` (row, key head, eight query heads) are cut: two blocks a multiprocessor, with a tile of 16 keys
+    for each of a block's eight warps (32-bit: 64 keys) at least.  Long sequences are cut further, up to a cluster, as they differ in length."""
+    keys = max(1, min(max_kv, window) if window else max_kv)
+    if not bf16:
+        return max(1, min(32, 296 // max(1, blocks), (keys + 63) // 64))
+    fill = min((296 + blocks - 1) // max(1, blocks), (keys + 127) // 128)
+    return max(1, min(64, fill), min(ATTN4_CLUSTER, (keys + 1023) // 1024))
 
 
 def attn4_rows(q, k_pages, v_pages, page_table, tok_slot, tok_pos, out, scale: float, window: Optional[int], group: int, max_kv: int) -> None:
@@ -2783,12 +2790,17 @@ def attn4_rows(q, k_pages, v_pages, page_table, tok_slot, tok_pos, out, scale: f
             raise KernelError("attn4_rows: token index arrays shorter than the batch")
     if window is not None and window <= 0:
         raise KernelError(f"attn4_rows: a window is a positive number of keys, got {window}")
-    lib = attn4_lib(d, n_heads // n_kv, page, group)
-    s = attn4_splits(n, n_kv, max_kv, window)
+    of = n_heads // n_kv
+    lib = attn4_lib(d, of, page, group)
+    blocks = n * n_kv * ((of + 7) // 8)
+    s = attn4_splits(blocks, max_kv, window, bool(is_bf16))
+    if blocks * s >= 1 << 31:
+        raise KernelError(f"attn4_rows: {n} rows are more than a launch takes")
+    joined = s > (ATTN4_CLUSTER if is_bf16 else 1)
     part_o = part_ml = None
-    if s > 1:
+    if joined:
         part_o = torch.empty((n, n_heads, s, d), dtype=torch.float32, device=q.device)
         part_ml = torch.empty((n, n_heads, s, 2), dtype=torch.float32, device=q.device)
     _ok(lib.dryft_attn4_rows(is_bf16, _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(page_table), page_table.shape[1], _ptr(tok_slot), _ptr(tok_pos), _ptr(out),
                              _ptr(part_o), _ptr(part_ml), n, n_kv, s, float(scale), int(window or 0), _stream()), f"attn4_rows (head_dim {d})",
-        n_kernels=2 if s > 1 else 1)
+        n_kernels=2 if joined else 1)

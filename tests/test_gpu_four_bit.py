@@ -280,6 +280,18 @@ def test_a_poisoned_token_poisons_its_readers_only():
     assert out.isnan().all(-1).tolist() == [True, True, False, False] and not out[2:].isnan().any()
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("n", [145, 2100])
+def test_a_poisoned_key_alone_in_its_tile_is_not_lost(n, dtype):
+    """The last key, alone in its tile and so with its warp (or its split) alone, has a score of NaN: the row's output is NaN."""
+    c = Cache([n, n], 1, 64, 64, 64, dtype)
+    c.keys[0][n - 1, 0, 3] = float("nan")
+    c.fill()
+    out = torch.empty(2, 128, dtype=dtype, device=DEV)
+    K().attn4_rows(torch.randn(2, 2, 64).to(dtype).to(DEV), c.k, c.v, c.pt, i32([0, 1]), i32([n - 1, n - 1]), out, 0.125, None, 64, n)
+    assert out[0].isnan().all() and out[1].isfinite().all()
+
+
 def test_the_same_bits_every_time_and_on_another_stream():
     c = Cache([2000, 31, 700], 2, 128, 64)
     c.fill()
