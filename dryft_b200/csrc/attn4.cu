@@ -2,7 +2,7 @@
 // head), -DDRYFT_PAGE and -DDRYFT_BITS_GROUP (numbers that share a scale).
 //
 // Row n at position p of slot s sees the keys j with  max(0, p + 1 - window) <= j <= p  (window <= 0: all of them); a row of slot -1 is padding, its output zeros.
-// A block takes up to eight query heads of a (row, key head) and one split of its keys.  Splits are whole tiles of 16 keys.  Up to eight splits are the blocks of
+// A block takes up to eight query heads of a (row, key head) and one split of its keys.  Splits are whole tiles of 16 keys.  Up to 16 splits are the blocks of
 // a thread-block cluster and meet in its shared memory; more leave (acc, m, l) in memory and a second launch joins them.  Either way in the splits' order.
 #include "four_bit.cuh"
 
@@ -17,6 +17,8 @@ constexpr size_t TILE = kv4_tile_bytes(PAGE, D, BG);
 static_assert(D % 16 == 0 && D <= 256 && D % BG == 0 && BG % 16 == 0 && BG <= 128, "head size in steps of 16, whole groups");
 static_assert(G >= 1 && G <= 16 && PAGE % 16 == 0, "1..16 query heads per key head, pages of whole tiles of 16 tokens");
 
+__device__ __forceinline__ void wait_before_reading() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 struct Span { int first, end; };   // keys of a split: whole tiles of 16, `least` of them at least, cut at the row's first and last key
 __device__ __forceinline__ Span span_of(int pos, int window, int split, int splits, int least) {
   const int lo = window > 0 && pos + 1 > window ? pos + 1 - window : 0;
@@ -27,10 +29,9 @@ __device__ __forceinline__ Span span_of(int pos, int window, int split, int spli
 
 // What a block knows of its work: head tile `ht` (of eight query heads) of a key head of a row, and its split.
 constexpr int HEAD_TILES = (G + 7) / 8, HEADS = G < 8 ? G : 8;   // (query heads of a block; the last tile may have fewer)
-struct Work { int n, head, ht, split; };
-__device__ __forceinline__ Work work_of(unsigned block, int n_kv, int splits) {
-  const unsigned i = block / splits, j = i / HEAD_TILES;
-  return {(int)(j / n_kv), (int)(j % n_kv), (int)(i % HEAD_TILES), (int)(block % splits)};
+struct Work { int n, head, ht, split, n_kv, splits; };
+__device__ __forceinline__ Work work_of_block() {   // grid (splits, key heads x head tiles, rows)
+  return {(int)blockIdx.z, (int)blockIdx.y / HEAD_TILES, (int)blockIdx.y % HEAD_TILES, (int)blockIdx.x, (int)gridDim.y / HEAD_TILES, (int)gridDim.x};
 }
 
 // ---------------------------------------------------------------------------------------------- bfloat16: tensor cores
@@ -40,10 +41,14 @@ __device__ __forceinline__ Work work_of(unsigned block, int n_kv, int splits) {
 // Scores, running maximum and sums are 32-bit.  A warp walks tiles of 16 keys of its own, copied STAGES - 1 tiles ahead into its own ring.  The maximum
 // of a column follows the scores only when one exceeds it by more than 2^8: what is summed stays below 2^8 times the number of keys.
 typedef __nv_bfloat16 bf16;
-constexpr int STEPS = D / 16, WARPS = 8, STAGES = D <= 128 ? 4 : 3;
-constexpr int CODES = 256 * UNITS, SCALES = 64 * GROUPS, STAGE = 2 * (CODES + SCALES);   // bytes of a tile's keys (or values), of their scales, of both
-constexpr int PART = D * 8 + 16;                                                           // floats: O^T [dim][head], maxima, sums
-constexpr size_t RING = (size_t)WARPS * STAGES * STAGE, JOIN = (size_t)(WARPS + 1) * PART * 4, SMEM = RING > JOIN ? RING : JOIN;
+constexpr int STEPS = D / 16, UNIT = PAGE % 32 ? 1 : 2, STAGES = D <= 128 ? 4 / UNIT : 2, MOST_SPLITS = 16;   // UNIT: tiles that are copied together
+constexpr int CODES = 256 * UNITS, SCALES = 64 * GROUPS, STAGE = UNIT * 2 * (CODES + SCALES);   // bytes of a tile's keys (or values), of their scales; of a stage
+constexpr int PART = STEPS * 128;                                                          // floats of a warp's O^T: [step][lane][4]
+template <int WARPS> struct Block {
+  static constexpr size_t RING = (size_t)WARPS * STAGES * STAGE, JOIN = (size_t)WARPS * PART * 4, TOP_AT = RING > JOIN ? RING : JOIN;
+  static constexpr size_t SMEM = TOP_AT + (WARPS * 16 + 16) * 4;                           // ... then the warps' maxima and sums, and the block's
+  static constexpr int AT_ONCE = D <= 128 ? 16 / WARPS : 8 / WARPS;                        // blocks a multiprocessor that the registers leave room for
+};
 
 __device__ __forceinline__ unsigned transposed(unsigned v) {   // an 8 x 8 fragment of 16-bit values
   unsigned r;
@@ -60,69 +65,215 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float of_block(const float* p, int block) {   // *p in another block of the cluster
-  unsigned at;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((unsigned)__cvta_generic_to_shared(p)), "r"(block));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+__device__ __forceinline__ unsigned in_block(unsigned at, int block) {   // the same place of another block of the cluster
+  unsigned r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(block));
+  return r;
+}
+__device__ __forceinline__ float4 cluster_load4(unsigned at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
   return v;
 }
+// N words from shared memory, in as few loads as their alignment (that of N words) allows
+template <int N> __device__ __forceinline__ void load_words(unsigned (&w)[N], const unsigned char* from) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(from)[i];
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const uint2 v = reinterpret_cast<const uint2*>(from)[i];
+      w[2 * i] = v.x; w[2 * i + 1] = v.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const unsigned*>(from)[i];
+  }
+}
 
-__global__ void __launch_bounds__(WARPS * 32, D <= 128 ? 2 : 1) attn4_mma_kernel(const bf16* __restrict__ q, const unsigned char* __restrict__ k_pages,
-                                                                                 const unsigned char* __restrict__ v_pages, const int* __restrict__ page_table,
-                                                                                 int max_pages, const int* __restrict__ tok_slot, const int* __restrict__ tok_pos,
-                                                                                 bf16* out, float* part_o, float* part_ml, int n_kv, int splits, int cluster, float scale,
-                                                                                 int window) {
+// Where a column's maximum starts: below every score but -inf, and what -inf is above it is -inf, not NaN.
+constexpr float LOWEST = -3.402823466e38f;
+
+// What a warp keeps of its eight columns (query heads); a lane has the columns 2c and 2c + 1, and in `acc` the dims 16 j + 2r and + 1 of both.
+struct Columns {
+  float acc[STEPS][4], off[GROUPS][2], less[GROUPS][4], top[2], sum[2];   // less: -23.5 sum p', from products with a constant
+};
+
+// A tile of 16 keys.  EDGE: keys may be out of the row's sight; such a key may hold anything, so its scales are taken for zeros.
+template <bool EDGE>
+__device__ __forceinline__ void tile_of_keys(Columns& o, const unsigned char* k, const unsigned char* k_scales, const unsigned char* v, const unsigned char* v_scales,
+                                             const uint2 (&qf)[STEPS], const float (&qs)[GROUPS][2], float scale2, int key0, Span keys) {
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const bool seen0 = !EDGE || (key0 + r >= keys.first && key0 + r < keys.end), seen1 = !EDGE || (key0 + r + 8 >= keys.first && key0 + r + 8 < keys.end);
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  {
+    unsigned lo[UNITS], hi[UNITS], lo_s[GROUPS], hi_s[GROUPS];
+    load_words<UNITS>(lo, k + r * ROW + c * UNITS * 4);
+    load_words<UNITS>(hi, k + (r + 8) * ROW + c * UNITS * 4);
+    load_words<GROUPS>(lo_s, k_scales + r * GROUPS * 4);
+    load_words<GROUPS>(hi_s, k_scales + (r + 8) * GROUPS * 4);
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      float part[4] = {-CODE_BIAS * qs[g][0], -CODE_BIAS * qs[g][1], -CODE_BIAS * qs[g][0], -CODE_BIAS * qs[g][1]};
+#pragma unroll
+      for (int j = g * BG / 16; j < (g + 1) * BG / 16; ++j) {
+        const int h = 2 * (j & 1);
+        mma_16816(part, code_pair(lo[j / 2], h), code_pair(hi[j / 2], h), code_pair(lo[j / 2], h + 1), code_pair(hi[j / 2], h + 1), qf[j].x, qf[j].y);
+      }
+      const GroupCode a = unpack_code(lo_s[g]), b = unpack_code(hi_s[g]);
+      s[0] = fmaf(a.s, part[0], fmaf(a.z, qs[g][0], s[0]));
+      s[1] = fmaf(a.s, part[1], fmaf(a.z, qs[g][1], s[1]));
+      s[2] = fmaf(b.s, part[2], fmaf(b.z, qs[g][0], s[2]));
+      s[3] = fmaf(b.s, part[3], fmaf(b.z, qs[g][1], s[3]));
+    }
+  }
+  if (EDGE) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = (i < 2 ? seen0 : seen1) ? s[i] * scale2 : -INFINITY;
+    scale2 = 1.f;
+  }
+  float d[4];   // powers of two above the maximum
+#pragma unroll
+  for (int i = 0; i < 4; ++i) d[i] = fmaf(s[i], scale2, -o.top[i & 1]);
+  if (__any_sync(0xffffffffu, fmaxf(fmaxf(d[0], d[1]), fmaxf(d[2], d[3])) > 8.f)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float m = fmaxf(o.top[i], fmaxf(s[i] * scale2, s[i + 2] * scale2));
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+      const float lower = exp2_fast(o.top[i] - m);
+      o.top[i] = m;
+      o.sum[i] *= lower;
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        o.off[g][i] *= lower;
+        o.less[g][i] *= lower;   // (its lower rows are not read)
+      }
+#pragma unroll
+      for (int j = 0; j < STEPS; ++j) {
+        o.acc[j][i] *= lower;
+        o.acc[j][i + 2] *= lower;
+      }
+      d[i] = fmaf(s[i], scale2, -m);
+      d[i + 2] = fmaf(s[i + 2], scale2, -m);
+    }
+  }
+  float p[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    p[i] = exp2_fast(d[i]);
+    o.sum[i & 1] += p[i];
+  }
+  unsigned vw[2 * UNITS], lo_s[GROUPS], hi_s[GROUPS];
+  load_words<2 * UNITS>(vw, v + lane * UNITS * 8);
+  load_words<GROUPS>(lo_s, v_scales + r * GROUPS * 4);
+  load_words<GROUPS>(hi_s, v_scales + (r + 8) * GROUPS * 4);
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    const GroupCode a = unpack_code(seen0 ? lo_s[g] : 0u), b = unpack_code(seen1 ? hi_s[g] : 0u);
+    const __nv_bfloat162 w0 = __floats2bfloat162_rn(p[0] * a.s, p[1] * a.s), w1 = __floats2bfloat162_rn(p[2] * b.s, p[3] * b.s);
+    const unsigned b0 = transposed(*reinterpret_cast<const unsigned*>(&w0)), b1 = transposed(*reinterpret_cast<const unsigned*>(&w1));
+    o.off[g][0] = fmaf(p[0], a.z, fmaf(p[2], b.z, o.off[g][0]));
+    o.off[g][1] = fmaf(p[1], a.z, fmaf(p[3], b.z, o.off[g][1]));
+    constexpr unsigned LESS = 0xc1bcc1bcu;   // two bfloat16 -23.5
+    mma_16816(o.less[g], LESS, LESS, LESS, LESS, b0, b1);
+#pragma unroll
+    for (int j = g * BG / 16; j < (g + 1) * BG / 16; ++j) {
+      const unsigned x = vw[j / 2 * 2], y = vw[j / 2 * 2 + 1];
+      const int h = 2 * (j & 1);
+      mma_16816(o.acc[j], code_pair(x, h), code_pair(x, h + 1), code_pair(y, h), code_pair(y, h + 1), b0, b1);
+    }
+  }
+}
+
+template <int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, Block<WARPS>::AT_ONCE) attn4_mma_kernel(const bf16* q, const unsigned char* k_pages, const unsigned char* v_pages,
+                                                                                      const int* __restrict__ page_table, int max_pages,
+                                                                                      const int* __restrict__ tok_slot, const int* __restrict__ tok_pos, bf16* out,
+                                                                                      float* part_o, float* part_ml, int cluster, int least, float scale, int window) {
   extern __shared__ __align__(16) unsigned char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
-  const Work w = work_of(blockIdx.x, n_kv, splits);
+  const Work w = work_of_block();
+  const int n_kv = w.n_kv, splits = w.splits;
   const int slot = tok_slot[w.n], pos = tok_pos[w.n], heads = min(8, G - 8 * w.ht);
   const size_t head0 = ((size_t)w.n * n_kv + w.head) * G + 8 * w.ht;   // the block's first query head
+  let_next_launch_in();
   if (slot < 0) {                                                      // (the whole cluster)
+    wait_before_reading();
     if (w.split == 0)
       for (int i = threadIdx.x; i < heads * D; i += WARPS * 32) out[head0 * D + i] = from_f32<bf16>(0.f);
     return;
   }
-  const Span keys = span_of(pos, window, w.split, splits, WARPS);
-  const int t0 = keys.first / 16, t1 = (keys.end + 15) / 16;
+  const Span keys = span_of(pos, window, w.split, splits, least);
+  // the warp's units of UNIT tiles: its share of the split's, one behind the other
+  constexpr int KEYS = UNIT * 16;
+  const int u0 = keys.first / KEYS, units = keys.end > keys.first ? (keys.end + KEYS - 1) / KEYS - u0 : 0;
+  const int a = u0 + units * warp / WARPS, b = u0 + units * (warp + 1) / WARPS;
+
+  Columns o;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    o.top[i] = LOWEST;
+    o.sum[i] = 0.f;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) o.off[g][i] = o.less[g][i] = o.less[g][i + 2] = 0.f;
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j) o.acc[j][i] = o.acc[j][i + 2] = 0.f;
+  }
+  if (units == 0 && splits > 1 && !cluster) {   // a split without keys: sums of zero, which the join does not look behind
+    wait_before_reading();
+    if (threadIdx.x < heads) *reinterpret_cast<float2*>(part_ml + ((head0 + threadIdx.x) * splits + w.split) * 2) = make_float2(LOWEST, 0.f);
+    return;
+  }
+  constexpr int PER_PAGE = PAGE / KEYS;
   const int* const pages = page_table + (size_t)slot * max_pages;
-
-  float acc[STEPS][4], off[GROUPS][2], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-#pragma unroll
-  for (int j = 0; j < STEPS; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-#pragma unroll
-  for (int g = 0; g < GROUPS; ++g) off[g][0] = off[g][1] = 0.f;
-
-  if (keys.first < keys.end) {
+  int page0 = a / PER_PAGE, held = 0;   // page numbers of 32 pages, one a lane
+  auto fetch = [&] { held = a < b && page0 + lane <= (b - 1) / PER_PAGE ? pages[page0 + lane] : 0; };
+  fetch();
+  wait_before_reading();
+  if (a < b) {
     unsigned char* const ring = smem + warp * STAGES * STAGE;
     const unsigned ring_at = (unsigned)__cvta_generic_to_shared(ring) + lane * 16;
-    // page numbers of 32 pages, one a lane
-    int page0 = t0 * 16 / PAGE, held = 0;
-    auto fetch = [&](int p) { held = p + lane <= (t1 - 1) * 16 / PAGE ? pages[p + lane] : 0; };
-    fetch(page0);
-    int ask = t0 + warp, put = 0;
+    constexpr int C = UNIT * CODES, S = UNIT * SCALES;   // a stage: keys' codes, values' codes, keys' scales, values' scales
+    const unsigned char *kp = nullptr, *vp = nullptr;    // the next unit's codes, less what a unit has, and its scales in the same way
+    const unsigned char *ksp = nullptr, *vsp = nullptr;
+    int ask = a, put = 0;
     auto request = [&] {
-      const int p = ask * 16 / PAGE;
-      if (ask < t1 && p - page0 >= 32) fetch(page0 = p);
-      const int page = __shfl_sync(0xffffffffu, held, (p - page0) & 31);
-      if (ask < t1) {
-        const size_t at = ((size_t)page * n_kv + w.head) * TILE;
-        const unsigned char *k = k_pages + at, *v = v_pages + at;
-        const int in_page = ask % (PAGE / 16);
+      if (ask < b) {
+        if (ask % PER_PAGE == 0 || ask == a) {
+          if (ask / PER_PAGE - page0 >= 32) {
+            page0 = ask / PER_PAGE;
+            fetch();
+          }
+          const size_t at = ((size_t)__shfl_sync(0xffffffffu, held, ask / PER_PAGE - page0) * n_kv + w.head) * TILE + lane * 16;
+          kp = k_pages + at + ask % PER_PAGE * C;
+          vp = v_pages + at + ask % PER_PAGE * C;
+          ksp = k_pages + at + ROW * PAGE + ask % PER_PAGE * S;
+          vsp = v_pages + at + ROW * PAGE + ask % PER_PAGE * S;
+        }
         const unsigned to = ring_at + put * STAGE;
 #pragma unroll
-        for (int i = 0; i < (CODES + 511) / 512; ++i)
-          if (CODES % 512 == 0 || i * 512 + lane * 16 < CODES) {
-            copy16(to + i * 512, k + in_page * CODES + i * 512 + lane * 16);
-            copy16(to + CODES + i * 512, v + in_page * CODES + i * 512 + lane * 16);
+        for (int i = 0; i < C; i += 512)
+          if (C - i >= 512 || i + lane * 16 < C) {
+            copy16(to + i, kp + i);
+            copy16(to + C + i, vp + i);
           }
 #pragma unroll
-        for (int i = 0; i < (2 * SCALES + 511) / 512; ++i) {   // keys' scales, then values'
-          const int x = i * 512 + lane * 16;
-          if (x < 2 * SCALES) copy16(to + 2 * CODES + i * 512, (x < SCALES ? k : v - SCALES) + (size_t)ROW * PAGE + in_page * SCALES + x);
-        }
+        for (int i = 0; i < S; i += 512)
+          if (S - i >= 512 || i + lane * 16 < S) {
+            copy16(to + 2 * C + i, ksp + i);
+            copy16(to + 2 * C + S + i, vsp + i);
+          }
+        kp += C;
+        vp += C;
+        ksp += S;
+        vsp += S;
         put = put + 1 == STAGES ? 0 : put + 1;
-        ask += WARPS;
+        ++ask;
       }
       asm volatile("cp.async.commit_group;");
     };
@@ -134,179 +285,148 @@ __global__ void __launch_bounds__(WARPS * 32, D <= 128 ? 2 : 1) attn4_mma_kernel
     float qs[GROUPS][2];
 #pragma unroll
     for (int j = 0; j < STEPS; ++j)
-      qf[j] = r < heads ? *reinterpret_cast<const uint2*>(q + (head0 + r) * D + 16 * j + 4 * c) : make_uint2(0, 0);
+      qf[j] = r < heads ? __ldcg(reinterpret_cast<const uint2*>(q + (head0 + r) * D + 16 * j + 4 * c)) : make_uint2(0, 0);
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
-      float s = 0.f;
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = g * BG / 16; j < (g + 1) * BG / 16; ++j)
-        s += (__uint_as_float(qf[j].x << 16) + __uint_as_float(qf[j].x & 0xffff0000u)) + (__uint_as_float(qf[j].y << 16) + __uint_as_float(qf[j].y & 0xffff0000u));
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      s += __shfl_xor_sync(0xffffffffu, s, 2);
-      qs[g][0] = __shfl_sync(0xffffffffu, s, 8 * c);
-      qs[g][1] = __shfl_sync(0xffffffffu, s, 8 * c + 4);
+      for (int j = g * BG / 16; j < (g + 1) * BG / 16; ++j) mma_16816(s, ONES_BF16, ONES_BF16, ONES_BF16, ONES_BF16, qf[j].x, qf[j].y);
+      qs[g][0] = s[0];
+      qs[g][1] = s[1];
     }
     const float scale2 = scale * 1.4426950408889634f;   // scores in powers of two
 
-    int get = 0;
+    const unsigned char* st = ring;
 #pragma unroll 1
-    for (int t = t0 + warp; t < t1; t += WARPS) {
+    for (int u = a; u < b; ++u) {
       __syncwarp();   // every lane has read the stage that the next request writes
       request();
       asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1));
       __syncwarp();
-      const unsigned char* const st = ring + get * STAGE;
-      get = get + 1 == STAGES ? 0 : get + 1;
-      const bool seen[2] = {t * 16 + r >= keys.first && t * 16 + r < keys.end, t * 16 + r + 8 >= keys.first && t * 16 + r + 8 < keys.end};
-      float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int g = 0; g < GROUPS; ++g) {
-        float part[4] = {-CODE_BIAS * qs[g][0], -CODE_BIAS * qs[g][1], -CODE_BIAS * qs[g][0], -CODE_BIAS * qs[g][1]};
-#pragma unroll
-        for (int j = g * BG / 16; j < (g + 1) * BG / 16; ++j) {
-          const unsigned lo = *reinterpret_cast<const unsigned*>(st + r * ROW + (c * UNITS + j / 2) * 4);
-          const unsigned hi = *reinterpret_cast<const unsigned*>(st + (r + 8) * ROW + (c * UNITS + j / 2) * 4);
-          mma_16816(part, code_pair(lo, 2 * (j & 1)), code_pair(hi, 2 * (j & 1)), code_pair(lo, 2 * (j & 1) + 1), code_pair(hi, 2 * (j & 1) + 1), qf[j].x, qf[j].y);
-        }
-        const GroupCode lo = unpack_code(*reinterpret_cast<const unsigned*>(st + 2 * CODES + (r * GROUPS + g) * 4));
-        const GroupCode hi = unpack_code(*reinterpret_cast<const unsigned*>(st + 2 * CODES + ((r + 8) * GROUPS + g) * 4));
-        s[0] = fmaf(lo.s, part[0], fmaf(lo.z, qs[g][0], s[0]));
-        s[1] = fmaf(lo.s, part[1], fmaf(lo.z, qs[g][1], s[1]));
-        s[2] = fmaf(hi.s, part[2], fmaf(hi.z, qs[g][0], s[2]));
-        s[3] = fmaf(hi.s, part[3], fmaf(hi.z, qs[g][1], s[3]));
+      if (u * KEYS >= keys.first && u * KEYS + KEYS <= keys.end) {
+#pragma unroll 1
+        for (int i = 0; i < UNIT; ++i)
+          tile_of_keys<false>(o, st + i * CODES, st + 2 * C + i * SCALES, st + C + i * CODES, st + 2 * C + S + i * SCALES, qf, qs, scale2, 0, keys);
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < UNIT; ++i)
+          if (u * KEYS + i * 16 < keys.end && u * KEYS + i * 16 + 16 > keys.first)
+            tile_of_keys<true>(o, st + i * CODES, st + 2 * C + i * SCALES, st + C + i * CODES, st + 2 * C + S + i * SCALES, qf, qs, scale2, u * KEYS + i * 16, keys);
       }
-      float p[4];
-      bool over = false;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[i] = seen[i >> 1] ? s[i] * scale2 : -INFINITY;
-        over |= s[i] > top[i & 1] + 8.f;
-      }
-      if (__any_sync(0xffffffffu, over)) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float m = fmaxf(top[i], fmaxf(s[i], s[i + 2]));
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-          const float lower = m == top[i] ? 1.f : exp2_fast(top[i] - m);
-          top[i] = m;
-          sum[i] *= lower;
-#pragma unroll
-          for (int g = 0; g < GROUPS; ++g) off[g][i] *= lower;
-#pragma unroll
-          for (int j = 0; j < STEPS; ++j) {
-            acc[j][i] *= lower;
-            acc[j][i + 2] *= lower;
-          }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p[i] = s[i] == -INFINITY ? 0.f : exp2_fast(s[i] - top[i & 1]);
-        sum[i & 1] += p[i];
-      }
-#pragma unroll
-      for (int g = 0; g < GROUPS; ++g) {
-        // a key that is not seen may hold anything: its scale and middle are taken for zeros
-        const unsigned lo_w = *reinterpret_cast<const unsigned*>(st + 2 * CODES + SCALES + (r * GROUPS + g) * 4);
-        const unsigned hi_w = *reinterpret_cast<const unsigned*>(st + 2 * CODES + SCALES + ((r + 8) * GROUPS + g) * 4);
-        const GroupCode lo = unpack_code(seen[0] ? lo_w : 0u), hi = unpack_code(seen[1] ? hi_w : 0u);
-        const __nv_bfloat162 w0 = __floats2bfloat162_rn(p[0] * lo.s, p[1] * lo.s), w1 = __floats2bfloat162_rn(p[2] * hi.s, p[3] * hi.s);
-        const unsigned b0 = *reinterpret_cast<const unsigned*>(&w0), b1 = *reinterpret_cast<const unsigned*>(&w1);
-        off[g][0] = fmaf(p[0], lo.z, fmaf(p[2], hi.z, off[g][0]));
-        off[g][1] = fmaf(p[1], lo.z, fmaf(p[3], hi.z, off[g][1]));
-        off[g][0] = fmaf(-CODE_BIAS, __uint_as_float(b0 << 16) + __uint_as_float(b1 << 16), off[g][0]);
-        off[g][1] = fmaf(-CODE_BIAS, __uint_as_float(b0 & 0xffff0000u) + __uint_as_float(b1 & 0xffff0000u), off[g][1]);
-        const unsigned t0_ = transposed(b0), t1_ = transposed(b1);
-#pragma unroll
-        for (int j = g * BG / 16; j < (g + 1) * BG / 16; ++j) {
-          const uint2 v = *reinterpret_cast<const uint2*>(st + CODES + (lane * UNITS + j / 2) * 8);
-          const int h = 2 * (j & 1);
-          mma_16816(acc[j], code_pair(v.x, h), code_pair(v.x, h + 1), code_pair(v.y, h), code_pair(v.y, h + 1), t0_, t1_);
-        }
-      }
+      st = st == ring + (STAGES - 1) * STAGE ? ring : st + STAGE;
     }
     asm volatile("cp.async.wait_group 0;");
     // what the lanes of a column have of its sums
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+      for (int x = 4; x < 32; x <<= 1) {
+        o.sum[i] += __shfl_xor_sync(0xffffffffu, o.sum[i], x);
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) off[g][i] += __shfl_xor_sync(0xffffffffu, off[g][i], o);
+        for (int g = 0; g < GROUPS; ++g) o.off[g][i] += __shfl_xor_sync(0xffffffffu, o.off[g][i], x);
       }
   }
 
-  // the block's part: the warps' sums in the warps' order.  A warp leaves its own in shared memory as they are, [dim][head] and the maxima and sums.
+  // The block's part.  The warps' maxima first; then each puts its sums on the block's maximum, and they are added in the warps' order.
+  float* const tops = reinterpret_cast<float*>(smem + Block<WARPS>::TOP_AT);   // [warp][8] maxima, [warp][8] sums, then the block's [8][2]
+  float* const sums = tops + WARPS * 8;
+  float2* const whole = reinterpret_cast<float2*>(sums + WARPS * 8);
+  float4* const parts = reinterpret_cast<float4*>(smem);         // [warp][step][lane]
+  if (r == 0) *reinterpret_cast<float2*>(tops + warp * 8 + 2 * c) = make_float2(o.top[0], o.top[1]);
   __syncthreads();
-  float* const parts = reinterpret_cast<float*>(smem);
-  {
-    float* const mine = parts + (warp + 1) * PART;
+  float top[2] = {LOWEST, LOWEST}, by[2];
 #pragma unroll
-    for (int j = 0; j < STEPS; ++j)
+  for (int x = 0; x < WARPS; ++x) {
+    const float2 m = *reinterpret_cast<const float2*>(tops + x * 8 + 2 * c);
+    top[0] = fmaxf(top[0], m.x);
+    top[1] = fmaxf(top[1], m.y);
+  }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mine[(16 * j + 2 * r + (i >> 1)) * 8 + 2 * c + (i & 1)] = acc[j][i] + off[16 * j / BG][i & 1];
-    if (r == 0)
+  for (int i = 0; i < 2; ++i) by[i] = exp2_fast(o.top[i] - top[i]);   // (1 where nothing has been seen: zeros, or the NaN of scores that are NaN)
+  if (r == 0) *reinterpret_cast<float2*>(sums + warp * 8 + 2 * c) = make_float2(o.sum[0] * by[0], o.sum[1] * by[1]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        mine[D * 8 + 2 * c + i] = top[i];
-        mine[D * 8 + 8 + 2 * c + i] = sum[i];
-      }
+  for (int j = 0; j < STEPS; ++j) {
+    const int g = 16 * j / BG;
+    const float e0 = o.off[g][0] + o.less[g][0], e1 = o.off[g][1] + o.less[g][1];
+    parts[(warp * STEPS + j) * 32 + lane] =
+        make_float4((o.acc[j][0] + e0) * by[0], (o.acc[j][1] + e1) * by[1], (o.acc[j][2] + e0) * by[0], (o.acc[j][3] + e1) * by[1]);
   }
   __syncthreads();
-  const bool alone = splits == 1;
-  const int h = threadIdx.x & 7;
-  {
-    float m = -INFINITY, l = 0.f, by[WARPS];
+  float l[2] = {0.f, 0.f};
 #pragma unroll
-    for (int x = 0; x < WARPS; ++x) m = fmaxf(m, parts[(x + 1) * PART + D * 8 + h]);
+  for (int x = 0; x < WARPS; ++x) {
+    const float2 v = *reinterpret_cast<const float2*>(sums + x * 8 + 2 * c);
+    l[0] += v.x;
+    l[1] += v.y;
+  }
+  auto write = [&](int j, int from, float4 v, float l0, float l1) {   // dims 16 j + 2 (row of lane `from`) and the next of heads 2c, 2c + 1
+    bf16* const to = out + (head0 + 2 * c) * D + 16 * j + 2 * (from >> 2);
+    const float i0 = 1.f / l0, i1 = 1.f / l1;
+    if (2 * c < heads) *reinterpret_cast<__nv_bfloat162*>(to) = __floats2bfloat162_rn(v.x * i0, v.z * i0);
+    if (2 * c + 1 < heads) *reinterpret_cast<__nv_bfloat162*>(to + D) = __floats2bfloat162_rn(v.y * i1, v.w * i1);
+  };
+  for (int j = warp; j < STEPS; j += WARPS) {
+    float4 v = parts[j * 32 + lane];
 #pragma unroll
-    for (int x = 0; x < WARPS; ++x) {
-      const float mx = parts[(x + 1) * PART + D * 8 + h];
-      by[x] = mx == -INFINITY ? 0.f : exp2_fast(mx - m);
-      l = fmaf(by[x], parts[(x + 1) * PART + D * 8 + 8 + h], l);
+    for (int x = 1; x < WARPS; ++x) {
+      const float4 y = parts[(x * STEPS + j) * 32 + lane];
+      v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
     }
-    const float inv = 1.f / l;
-    for (int dim = threadIdx.x >> 3; dim < D; dim += WARPS * 4) {
-      float v = 0.f;
+    if (splits == 1)
+      write(j, lane, v, l[0], l[1]);
+    else if (cluster)
+      parts[j * 32 + lane] = v;
+    else {
 #pragma unroll
-      for (int x = 0; x < WARPS; ++x) v = fmaf(by[x], parts[(x + 1) * PART + dim * 8 + h], v);
-      if (h >= heads) continue;
-      if (alone)
-        out[(head0 + h) * D + dim] = from_f32<bf16>(v * inv);
-      else if (cluster)
-        parts[dim * 8 + h] = v;
-      else
-        part_o[((head0 + h) * splits + w.split) * D + dim] = v;
-    }
-    if (!alone && threadIdx.x < heads) {
-      float* const to = cluster ? parts + D * 8 + h : part_ml + ((head0 + h) * splits + w.split) * 2;
-      to[0] = m;
-      to[cluster ? 8 : 1] = l;
+      for (int i = 0; i < 2; ++i)
+        if (2 * c + i < heads)
+          *reinterpret_cast<float2*>(part_o + ((head0 + 2 * c + i) * splits + w.split) * D + 16 * j + 2 * r) = i ? make_float2(v.y, v.w) : make_float2(v.x, v.z);
     }
   }
-  if (alone || !cluster) return;
-  // every block of the cluster joins its share of the dims, over the splits in their order
+  if (splits == 1) return;
+  if (warp == 0 && r == 0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (cluster)
+        whole[2 * c + i] = make_float2(top[i], l[i]);
+      else if (2 * c + i < heads)
+        *reinterpret_cast<float2*>(part_ml + ((head0 + 2 * c + i) * splits + w.split) * 2) = make_float2(top[i], l[i]);
+    }
+  }
+  if (!cluster) return;
+  // every block of the cluster joins its share of the steps' lanes, over the splits in their order
   cluster_barrier();
-  if (h < heads) {
-    float m = -INFINITY, l = 0.f, by[8];
+  {
+    const unsigned whole_at = (unsigned)__cvta_generic_to_shared(whole), parts_at = (unsigned)__cvta_generic_to_shared(parts);
+    for (int i = threadIdx.x * splits + w.split; i < STEPS * 32; i += WARPS * 32 * splits) {
+      const int col = 2 * (i & 3);
+      float m0 = LOWEST, m1 = LOWEST, l0 = 0.f, l1 = 0.f;
+      float2 w0[MOST_SPLITS], w1[MOST_SPLITS];
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      by[x] = x < splits ? of_block(parts + D * 8 + h, x) : -INFINITY;
-      m = fmaxf(m, by[x]);
-    }
+      for (int x = 0; x < MOST_SPLITS; ++x) {
+        w0[x] = w1[x] = make_float2(LOWEST, 0.f);
+        if (x < splits) {
+          const float4 v = cluster_load4(in_block(whole_at + col * 8, x));
+          w0[x] = make_float2(v.x, v.y);
+          w1[x] = make_float2(v.z, v.w);
+        }
+        m0 = fmaxf(m0, w0[x].x);
+        m1 = fmaxf(m1, w1[x].x);
+      }
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      by[x] = by[x] == -INFINITY ? 0.f : exp2_fast(by[x] - m);
-      if (x < splits) l = fmaf(by[x], of_block(parts + D * 8 + 8 + h, x), l);
-    }
-    for (int dim = (threadIdx.x >> 3) * splits + w.split; dim < D; dim += WARPS * 4 * splits) {
-      float v = 0.f;
-#pragma unroll
-      for (int x = 0; x < 8; ++x)
-        if (x < splits) v = fmaf(by[x], of_block(parts + dim * 8 + h, x), v);
-      out[(head0 + h) * D + dim] = from_f32<bf16>(v / l);
+      for (int x = 0; x < MOST_SPLITS; ++x)
+        if (x < splits) {
+          const float b0 = exp2_fast(w0[x].x - m0), b1 = exp2_fast(w1[x].x - m1);
+          l0 = fmaf(b0, w0[x].y, l0);
+          l1 = fmaf(b1, w1[x].y, l1);
+          const float4 y = cluster_load4(in_block(parts_at + i * 16, x));
+          v = make_float4(fmaf(b0, y.x, v.x), fmaf(b1, y.y, v.y), fmaf(b0, y.z, v.z), fmaf(b1, y.w, v.w));
+        }
+      bf16* const to = out + (head0 + col) * D + 16 * (i >> 5) + 2 * ((i & 31) >> 2);
+      const float i0 = 1.f / l0, i1 = 1.f / l1;
+      if (col < heads) *reinterpret_cast<__nv_bfloat162*>(to) = __floats2bfloat162_rn(v.x * i0, v.z * i0);
+      if (col + 1 < heads) *reinterpret_cast<__nv_bfloat162*>(to + D) = __floats2bfloat162_rn(v.y * i1, v.w * i1);
     }
   }
   cluster_barrier();   // a block's shared memory stays until the others have read it
@@ -319,10 +439,11 @@ constexpr int THREADS = 128, DIMS = (D + THREADS - 1) / THREADS;
 __global__ void __launch_bounds__(THREADS) attn4_f32_kernel(const float* __restrict__ q, const unsigned char* __restrict__ k_pages,
                                                             const unsigned char* __restrict__ v_pages, const int* __restrict__ page_table, int max_pages,
                                                             const int* __restrict__ tok_slot, const int* __restrict__ tok_pos, float* out, float* part_o,
-                                                            float* part_ml, int n_kv, int splits, float scale, int window) {
+                                                            float* part_ml, float scale, int window) {
   __shared__ float qs[HEADS][D], ps[HEADS][THREADS], red[THREADS / 32][HEADS], total[THREADS / 32][HEADS], top[HEADS], sum[HEADS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Work w = work_of(blockIdx.x, n_kv, splits);
+  const Work w = work_of_block();
+  const int n_kv = w.n_kv, splits = w.splits;
   const int slot = tok_slot[w.n], pos = tok_pos[w.n], heads = min(8, G - 8 * w.ht);
   const size_t head0 = ((size_t)w.n * n_kv + w.head) * G + 8 * w.ht;
   if (slot < 0) {
@@ -435,27 +556,37 @@ __global__ void __launch_bounds__(THREADS) attn4_f32_kernel(const float* __restr
   }
 }
 
-// A block per (row, query head): the splits' sums joined in their order.  Maxima are powers of two.
+// A warp per (row, query head): the splits' sums joined in their order.  Maxima are powers of two; a split without keys has sums of zero.
 template <typename T>
-__global__ void __launch_bounds__(THREADS) attn4_join_kernel(const float* part_o, const float* part_ml, const int* __restrict__ tok_slot, T* out, int n_heads, int splits) {
+__global__ void __launch_bounds__(THREADS) attn4_join_kernel(const float* part_o, const float* part_ml, const int* __restrict__ tok_slot, T* out, int n_heads, int total,
+                                                             int splits) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const unsigned n = blockIdx.x / n_heads;
-  if (tok_slot[n] < 0) return;   // the first launch wrote its zeros
-  const size_t h = blockIdx.x;
-  float m = -INFINITY, l = 0.f;
-  for (int s = 0; s < splits; ++s) m = fmaxf(m, __ldcg(part_ml + (h * splits + s) * 2));
-  for (int s = 0; s < splits; ++s) {
-    const float ms = __ldcg(part_ml + (h * splits + s) * 2);
-    l = fmaf(__ldcg(part_ml + (h * splits + s) * 2 + 1), ms == -INFINITY ? 0.f : exp2f(ms - m), l);   // (a split of NaN alone has no maximum, its sum is NaN)
-  }
-  for (int x = threadIdx.x; x < D; x += THREADS) {
-    float a = 0.f;
-    for (int s = 0; s < splits; ++s) {
-      const float ms = __ldcg(part_ml + (h * splits + s) * 2);
-      a = fmaf(__ldcg(part_o + (h * splits + s) * D + x), ms == -INFINITY ? 0.f : exp2f(ms - m), a);
+  const int h = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (h >= total || tok_slot[h / n_heads] < 0) return;   // (padding: the first launch wrote its zeros)
+  constexpr int MINE = (D + 31) / 32;
+  float m = -INFINITY, l = 0.f, a[MINE];
+#pragma unroll
+  for (int i = 0; i < MINE; ++i) a[i] = 0.f;
+  const float2* const ml = reinterpret_cast<const float2*>(part_ml) + (size_t)h * splits;
+  for (int s0 = 0; s0 < splits; s0 += 32) m = fmaxf(m, s0 + lane < splits ? __ldcg(ml + s0 + lane).x : -INFINITY);
+  m = warp_max(m);
+  const float* const o = part_o + (size_t)h * splits * D;
+  for (int s0 = 0; s0 < splits; s0 += 32) {
+    const float2 v = s0 + lane < splits ? __ldcg(ml + s0 + lane) : make_float2(-INFINITY, 0.f);
+    const float mine = v.x == -INFINITY ? 0.f : exp2f(v.x - m);
+#pragma unroll 4
+    for (int s = 0; s < min(32, splits - s0); ++s) {
+      const float by = __shfl_sync(0xffffffffu, mine, s), sum = __shfl_sync(0xffffffffu, v.y, s);
+      if (sum == 0.f) continue;   // no keys: its partial sums may not have been written
+      l = fmaf(sum, by, l);       // (the sum of a split whose scores are all NaN is NaN, whatever it is multiplied with)
+#pragma unroll
+      for (int i = 0; i < MINE; ++i)
+        if (D % 32 == 0 || lane + 32 * i < D) a[i] = fmaf(__ldcg(o + (size_t)(s0 + s) * D + lane + 32 * i), by, a[i]);
     }
-    out[h * D + x] = from_f32<T>(a / l);
   }
+#pragma unroll
+  for (int i = 0; i < MINE; ++i)
+    if (D % 32 == 0 || lane + 32 * i < D) out[(size_t)h * D + lane + 32 * i] = from_f32<T>(a[i] / l);
 }
 
 struct Args {
@@ -465,16 +596,16 @@ struct Args {
   const int *tok_slot, *tok_pos;
   void* out;
   float *part_o, *part_ml;
-  int n, n_kv, splits;
+  int n, n_kv, splits, least;
   float scale;
-  int window;
+  int window, pdl;
   cudaStream_t st;
 };
 
 template <typename... P, typename... A>
-int launch(void (*kern)(P...), unsigned grid, int threads, size_t bytes, int cluster, bool dependent, cudaStream_t st, A... a) {
+int launch(void (*kern)(P...), dim3 grid, int threads, size_t bytes, int cluster, bool dependent, cudaStream_t st, A... a) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = st;
@@ -497,36 +628,43 @@ int launch(void (*kern)(P...), unsigned grid, int threads, size_t bytes, int clu
   return e != cudaSuccess ? (int)e : launch_status();
 }
 
+dim3 grid_of(const Args& a) { return dim3(a.splits, a.n_kv * HEAD_TILES, a.n); }
+
 template <typename T> int join(const Args& a) {
-  return launch(attn4_join_kernel<T>, (unsigned)a.n * a.n_kv * G, THREADS, 0, 1, true, a.st, a.part_o, a.part_ml, a.tok_slot, (T*)a.out, a.n_kv * G, a.splits);
+  const int total = a.n * a.n_kv * G;
+  return launch(attn4_join_kernel<T>, dim3((total + THREADS / 32 - 1) / (THREADS / 32)), THREADS, 0, 1, true, a.st, a.part_o, a.part_ml, a.tok_slot, (T*)a.out, a.n_kv * G,
+                total, a.splits);
 }
 
 int rows_f32(const Args& a) {
-  const int rc = launch(attn4_f32_kernel, (unsigned)a.n * a.n_kv * HEAD_TILES * a.splits, THREADS, 0, 1, false, a.st, (const float*)a.q,
-                        (const unsigned char*)a.k_pages, (const unsigned char*)a.v_pages, a.page_table, a.max_pages, a.tok_slot, a.tok_pos, (float*)a.out, a.part_o,
-                        a.part_ml, a.n_kv, a.splits, a.scale, a.window);
+  const int rc = launch(attn4_f32_kernel, grid_of(a), THREADS, 0, 1, false, a.st, (const float*)a.q, (const unsigned char*)a.k_pages, (const unsigned char*)a.v_pages,
+                        a.page_table, a.max_pages, a.tok_slot, a.tok_pos, (float*)a.out, a.part_o, a.part_ml, a.scale, a.window);
   return rc || a.splits == 1 ? rc : join<float>(a);
 }
 
-int rows_bf16(const Args& a) {
+template <int WARPS> int rows_bf16(const Args& a) {
   static bool asked = false;
   if (!asked) {   // (asking twice does no harm)
-    const cudaError_t e = cudaFuncSetAttribute(attn4_mma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
+    cudaError_t e = cudaFuncSetAttribute(attn4_mma_kernel<WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Block<WARPS>::SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(attn4_mma_kernel<WARPS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return (int)e;
     asked = true;
   }
-  const int cluster = a.splits > 1 && a.splits <= 8;
-  const int rc = launch(attn4_mma_kernel, (unsigned)a.n * a.n_kv * HEAD_TILES * a.splits, WARPS * 32, SMEM, cluster ? a.splits : 1, false, a.st, (const bf16*)a.q,
+  const int cluster = a.splits > 1 && a.part_o == nullptr;
+  if (cluster && a.splits > MOST_SPLITS) return DRYFT_ERR_UNSUPPORTED;
+  const int rc = launch(attn4_mma_kernel<WARPS>, grid_of(a), WARPS * 32, Block<WARPS>::SMEM, cluster ? a.splits : 1, a.pdl != 0, a.st, (const bf16*)a.q,
                         (const unsigned char*)a.k_pages, (const unsigned char*)a.v_pages, a.page_table, a.max_pages, a.tok_slot, a.tok_pos, (bf16*)a.out, a.part_o,
-                        a.part_ml, a.n_kv, a.splits, cluster, a.scale, a.window);
+                        a.part_ml, cluster, a.least, a.scale, a.window);
   return rc || a.splits == 1 || cluster ? rc : join<bf16>(a);
 }
 }  // namespace
 
 DRYFT_API int dryft_attn4_rows(int is_bf16, const void* q, const void* k_pages, const void* v_pages, const int* page_table, int max_pages, const int* tok_slot,
-                               const int* tok_pos, void* out, float* part_o, float* part_ml, int n, int n_kv, int splits, float scale, int window, void* stream) {
+                               const int* tok_pos, void* out, float* part_o, float* part_ml, int n, int n_kv, int splits, int least, int warps, float scale, int window,
+                               int pdl, void* stream) {
   if (n <= 0) return 0;
-  return (is_bf16 ? rows_bf16 : rows_f32)({q, k_pages, v_pages, page_table, max_pages, tok_slot, tok_pos, out, part_o, part_ml, n, n_kv, splits, scale, window,
+  if (n > 65535 || n_kv * HEAD_TILES > 65535) return DRYFT_ERR_UNSUPPORTED;
+  return (!is_bf16 ? rows_f32 : warps == 4 ? rows_bf16<4> : rows_bf16<8>)({q, k_pages, v_pages, page_table, max_pages, tok_slot, tok_pos, out, part_o, part_ml, n, n_kv, splits, least, scale, window, pdl,
                                            (cudaStream_t)stream});
 }
 DRYFT_API int dryft_attn4_sizes(int which) { return which == 0 ? D : which == 1 ? G : which == 2 ? PAGE : BG; }

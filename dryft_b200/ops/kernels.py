@@ -13,6 +13,7 @@ captured by ``torch.cuda.graph``.
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 from dataclasses import dataclass
 from typing import Dict, Optional, Tuple
@@ -2641,15 +2642,36 @@ def _kv4_pages(k_pages, v_pages, page_table, head_dim: int, group: int) -> Tuple
     if head_dim <= 0 or head_dim % 16 or head_dim > 256:
         raise KernelError(f"a cache in 4 bits takes head sizes 16..256 in steps of 16, got head_dim={head_dim}")
     _bits4_group(head_dim, group, "a cache in 4 bits")
-    _need(k_pages, "k_pages", torch.uint8, (None, None, None))
-    _need(v_pages, "v_pages", torch.uint8, tuple(k_pages.shape))
-    _need(page_table, "page_table", torch.int32, (None, None))
-    page, rest = divmod(k_pages.shape[2], kv4_token_bytes(head_dim, group))
+    try:
+        shape = k_pages.shape
+        fine = (k_pages.is_cuda and v_pages.is_cuda and page_table.is_cuda and k_pages.dtype is torch.uint8 and v_pages.dtype is torch.uint8
+                and page_table.dtype is torch.int32 and len(shape) == 3 and v_pages.shape == shape and page_table.dim() == 2
+                and k_pages.is_contiguous() and v_pages.is_contiguous() and page_table.is_contiguous())
+    except AttributeError:
+        fine = False
+    if not fine:
+        _need(k_pages, "k_pages", torch.uint8, (None, None, None))
+        _need(v_pages, "v_pages", torch.uint8, tuple(k_pages.shape))
+        _need(page_table, "page_table", torch.int32, (None, None))
+    page, rest = divmod(shape[2], kv4_token_bytes(head_dim, group))
     if rest or page % 16 or page <= 0:
-        raise KernelError(f"k_pages: {k_pages.shape[2]} bytes are not a page of whole 16 tokens of {kv4_token_bytes(head_dim, group)} bytes")
+        raise KernelError(f"k_pages: {shape[2]} bytes are not a page of whole 16 tokens of {kv4_token_bytes(head_dim, group)} bytes")
     if k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16:
         raise KernelError("k_pages, v_pages: pages start on 16-byte boundaries")
-    return k_pages.shape[1], page
+    return shape[1], page
+
+
+def _tokens(tok_slot, tok_pos, n: int, what: str) -> None:
+    """Slots and positions of ``n`` tokens."""
+    try:
+        if (tok_slot.is_cuda and tok_pos.is_cuda and tok_slot.dtype is torch.int32 and tok_pos.dtype is torch.int32 and tok_slot.is_contiguous()
+                and tok_pos.is_contiguous() and tok_slot.numel() >= n and tok_pos.numel() >= n):
+            return
+    except AttributeError:
+        pass
+    for t, nm in ((tok_slot, "tok_slot"), (tok_pos, "tok_pos")):
+        _need(t, nm, torch.int32)
+    raise KernelError(f"{what}: token index arrays shorter than the batch")
 
 
 def kv4_store(k, v, tok_slot, tok_pos, k_pages, v_pages, page_table, group: int) -> None:
@@ -2670,10 +2692,7 @@ def kv4_store(k, v, tok_slot, tok_pos, k_pages, v_pages, page_table, group: int)
             raise KernelError(f"{nm}: rows start on 16-byte boundaries")
     if n > 1 and k.stride(0) != v.stride(0):
         raise KernelError("kv4_store: k and v rows lie equally far apart")
-    for t, nm in ((tok_slot, "tok_slot"), (tok_pos, "tok_pos")):
-        _need(t, nm, torch.int32)
-        if t.numel() < n:
-            raise KernelError("kv4_store: token index arrays shorter than the batch")
+    _tokens(tok_slot, tok_pos, n, "kv4_store")
     _ok(kv4_lib().dryft_kv4_store(_act(k, "k"), _ptr(k), _ptr(v), k.stride(0) if n > 1 else n_kv * d, _ptr(tok_slot), _ptr(tok_pos), _ptr(k_pages), _ptr(v_pages),
                                   _ptr(page_table), page_table.shape[1], n, n_kv, d, group, page, _stream()), "kv4_store")
 
@@ -2697,10 +2716,7 @@ def kv4_rope_store(qkv, q_norm_w, k_norm_w, inv_freq, tok_slot, tok_pos, q_out, 
         _need(k_norm_w, "k_norm weight", torch.float32, (head_dim,))
     if rotary_dim:
         _need(inv_freq, "inv_freq", torch.float32, (rotary_dim // 2,))
-    _need(tok_slot, "tok_slot", torch.int32)
-    _need(tok_pos, "tok_pos", torch.int32)
-    if tok_slot.numel() < n or tok_pos.numel() < n:
-        raise KernelError("kv4_rope_store: token index arrays shorter than the batch")
+    _tokens(tok_slot, tok_pos, n, "kv4_rope_store")
     _need(q_out, "q_out", qkv.dtype, (n, n_heads, head_dim))
     if cs_table is not None:
         _need(cs_table, "cs_table", qkv.dtype, (None, 2, rotary_dim // 2))
@@ -2749,7 +2765,7 @@ def attn4_lib(head_dim: int, heads: int, page: int, group: int) -> ctypes.CDLL:
         if lib is None:
             path = build.build_library("attn4", ("attn4.cu",), {"DRYFT_HEAD_DIM": head_dim, "DRYFT_GROUP": heads, "DRYFT_PAGE": page, "DRYFT_BITS_GROUP": group})
             lib = _load(path)
-            lib.dryft_attn4_rows.argtypes = [_i, _p, _p, _p, _p, _i, _p, _p, _p, _p, _p, _i, _i, _i, _f, _i, _p]
+            lib.dryft_attn4_rows.argtypes = [_i, _p, _p, _p, _p, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _f, _i, _i, _p]
             lib.dryft_attn4_rows.restype = _i
             lib.dryft_attn4_sizes.argtypes = [_i]
             if tuple(lib.dryft_attn4_sizes(i) for i in range(4)) != (head_dim, heads, page, group):
@@ -2758,49 +2774,56 @@ def attn4_lib(head_dim: int, heads: int, page: int, group: int) -> ctypes.CDLL:
         return lib
 
 
-ATTN4_CLUSTER = 8   # up to this many splits of the tensor-core kernel are the blocks of a cluster
+ATTN4_CLUSTER = 16   # up to this many splits of the tensor-core kernel can be the blocks of a cluster
 
 
-def attn4_splits(blocks: int, max_kv: int, window: Optional[int], bf16: bool) -> int:
-    """Into how many splits the keys of each of ``blocks`` (row, key head, eight query heads) are cut: two blocks a multiprocessor, with a tile of 16 keys
-    for each of a block's eight warps (32-bit: 64 keys) at least.  Long sequences are cut further, up to a cluster, as they differ in length."""
+@functools.lru_cache(maxsize=4096)
+def attn4_plan(blocks: int, max_kv: int, window: Optional[int], bf16: bool) -> Tuple[int, int, int, bool]:
+    """How the keys of each of ``blocks`` (row, key head, eight query heads) are cut: (splits, tiles of 16 keys that a split has at least, warps a block,
+    whether the splits are the blocks of a cluster).
+
+    More blocks than multiprocessors are cut only where sequences are long, and may differ in length: 1,024 keys a split, joined by a second launch (64 rows
+    of up to 8,192 keys, eight key heads of 128: 98 us, as clusters of eight 153, in one split 128, two 116).  Fewer are cut as far as they fill the multiprocessors, the splits a
+    cluster: a split costs its block about 3 us, so it has 1,024 keys (of few rows 256) at least (eight rows of 8,000 keys: 29 us in two splits, 50 in one; of
+    650 keys 8.6 and 7.9; one row of 4,000 keys: 9.1 in eight, 11.6 in four; 64 query heads, 16,383 keys: 17.9 in sixteen, 18.4 in eight)."""
     keys = max(1, min(max_kv, window) if window else max_kv)
     if not bf16:
-        return max(1, min(32, 296 // max(1, blocks), (keys + 63) // 64))
-    fill = min((296 + blocks - 1) // max(1, blocks), (keys + 127) // 128)
-    return max(1, min(64, fill), min(ATTN4_CLUSTER, (keys + 1023) // 1024))
+        return max(1, min(32, 296 // max(1, blocks), (keys + 63) // 64)), 1, 4, False
+    if blocks > 148:
+        return (min(64, (keys + 1023) // 1024), 64, 4, False) if keys > 2048 else (1, 1, 4, False)
+    s = max(1, min(ATTN4_CLUSTER, 148 // max(1, blocks), keys // (256 if blocks <= 16 else 1024)))
+    return s, 8, 8, s > 1
 
 
-def attn4_rows(q, k_pages, v_pages, page_table, tok_slot, tok_pos, out, scale: float, window: Optional[int], group: int, max_kv: int) -> None:
+def attn4_rows(q, k_pages, v_pages, page_table, tok_slot, tok_pos, out, scale: float, window: Optional[int], group: int, max_kv: int, pdl: bool = False) -> None:
     """Attention of ``n`` query rows ``q`` ``[n, heads, head_dim]`` over the cache in 4 bits: row ``i`` sees the keys 0..``tok_pos[i]`` (the last ``window``
     of them) of slot ``tok_slot[i]``; a row of slot -1 is padding and gets zeros.  ``max_kv``: no sequence is longer (a bound; how the keys are cut
-    over blocks follows from it)."""
+    over blocks follows from it).  ``pdl``: a programmatic dependent; ``tok_slot``, ``tok_pos`` and ``page_table`` are then older than the launch
+    before it."""
     if not isinstance(q, torch.Tensor) or q.dim() != 3:
         raise KernelError("attn4_rows: q is [rows, heads, head size]")
     n, n_heads, d = q.shape
     _need(q, "q")
     is_bf16 = _act(q, "q")
     n_kv, page = _kv4_pages(k_pages, v_pages, page_table, d, group)
-    if n_heads % n_kv:
+    of, rest = divmod(n_heads, n_kv)
+    if rest:
         raise KernelError(f"attn4_rows: {n_heads} query heads are not a multiple of {n_kv} kv heads")
     _need(out, "attention output", q.dtype, (n, n_heads * d))
-    for t, nm in ((tok_slot, "tok_slot"), (tok_pos, "tok_pos")):
-        _need(t, nm, torch.int32)
-        if t.numel() < n:
-            raise KernelError("attn4_rows: token index arrays shorter than the batch")
+    _tokens(tok_slot, tok_pos, n, "attn4_rows")
     if window is not None and window <= 0:
         raise KernelError(f"attn4_rows: a window is a positive number of keys, got {window}")
-    of = n_heads // n_kv
-    lib = attn4_lib(d, of, page, group)
-    blocks = n * n_kv * ((of + 7) // 8)
-    s = attn4_splits(blocks, max_kv, window, bool(is_bf16))
-    if blocks * s >= 1 << 31:
-        raise KernelError(f"attn4_rows: {n} rows are more than a launch takes")
-    joined = s > (ATTN4_CLUSTER if is_bf16 else 1)
-    part_o = part_ml = None
-    if joined:
-        part_o = torch.empty((n, n_heads, s, d), dtype=torch.float32, device=q.device)
-        part_ml = torch.empty((n, n_heads, s, 2), dtype=torch.float32, device=q.device)
-    _ok(lib.dryft_attn4_rows(is_bf16, _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(page_table), page_table.shape[1], _ptr(tok_slot), _ptr(tok_pos), _ptr(out),
-                             _ptr(part_o), _ptr(part_ml), n, n_kv, s, float(scale), int(window or 0), _stream()), f"attn4_rows (head_dim {d})",
+    lib = _variants.get(("attn4", d, of, page, group)) or attn4_lib(d, of, page, group)
+    tiles = n_kv * ((of + 7) // 8)
+    if n > 65535 or tiles > 65535:
+        raise KernelError(f"attn4_rows takes up to 65,535 rows and key heads, got {n} and {n_kv}")
+    s, least, warps, cluster = attn4_plan(n * tiles, max_kv, window, bool(is_bf16))
+    part_o = part_ml = 0
+    joined = s > 1 and not cluster
+    if joined:   # every split's sums, then its maximum and what its weights come to
+        parts = torch.empty(n * n_heads * s * (d + 2), dtype=torch.float32, device=q.device)
+        part_o = parts.data_ptr()
+        part_ml = part_o + 4 * n * n_heads * s * d
+    _ok(lib.dryft_attn4_rows(is_bf16, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), page_table.shape[1], tok_slot.data_ptr(),
+                             tok_pos.data_ptr(), out.data_ptr(), part_o, part_ml, n, n_kv, s, least, warps, scale, window or 0, pdl, _stream()), "attn4_rows",
         n_kernels=2 if joined else 1)
