@@ -4,8 +4,80 @@
 namespace {
 constexpr int WARPS = 4;
 
-// Lowest and highest of a lane's numbers in steps 0 and 1 of its unit, over the group: `near` lanes next to one another hold a unit.
-__device__ __forceinline__ void group_range(float (&lo)[2], float (&hi)[2], int near, int group) {
+// The range of a lane's numbers.  fminf and fmaxf pass over NaN, so whether there was one is kept beside them: x * 0 is NaN for it (and for an infinity).
+struct Range {
+  float lo = INFINITY, hi = -INFINITY, not_finite = 0.f;
+  __device__ __forceinline__ void add(float x) {
+    lo = fminf(lo, x);
+    hi = fmaxf(hi, x);
+    not_finite = fmaf(x, 0.f, not_finite);
+  }
+  __device__ __forceinline__ void close() {   // a range with such a number is everything
+    lo = not_finite == 0.f ? lo : -INFINITY;
+    hi = not_finite == 0.f ? hi : INFINITY;
+  }
+};
+
+// The codes of a group's numbers without a division each.  The definition (`code_of`) rounds t / s, t = x - z, and then t / s + 7.5, to 32 bits, and that to a whole
+// number.  With j the whole number nearest to t times 1 / s and e = t - j s (j s is exact, so e is rounded once, and 0 where t is a multiple of s), j + e / s is
+// t / s up to 2^-22, and exact where e is 0 -- which is every tie.  Only where e is neither 0 nor beyond 10^-5 s could those roundings decide: then the group's numbers
+// are divided after all.  (Three numbers in a thousand are ties where x is bfloat16.)
+constexpr float ROUND = 12582912.f;   // 1.5 * 2^23: adding it rounds to whole numbers, ties to even
+struct Coder {
+  GroupCode g;
+  float inv;
+  unsigned closest = ~0u;   // bits of the least |e| that is not 0, less 1
+  __device__ __forceinline__ Coder(float lo, float hi) : g(group_code(lo, hi)), inv(inverse(g.s)) {}
+  __device__ __forceinline__ Coder(GroupCode code, float inverse) : g(code), inv(inverse) {}
+  static __device__ __forceinline__ float inverse(float s) { return s > 1e-36f ? __fdividef(1.f, s) : 0.f; }   // (its last bits do not matter)
+  // `word` + code << shift + ROUND's bits << shift, which the caller takes out (`round_bits`)
+  __device__ __forceinline__ unsigned add(unsigned word, float x, int shift) {
+    const float t = __fadd_rn(x, -g.z), j = __fadd_rn(__fadd_rn(__fmul_rn(t, inv), ROUND), -ROUND), e = fmaf(-j, g.s, t);
+    closest = min(closest, (__float_as_uint(e) & 0x7fffffffu) - 1u);
+    const float y = __fadd_rn(fmaf(e, inv, j), 7.5f);
+    return word + (__float_as_uint(__fadd_rn(fminf(fmaxf(y, 0.f), 15.f), ROUND)) << shift);
+  }
+  __device__ __forceinline__ bool undecided() const { return closest < __float_as_uint(g.s * 1e-5f) || (inv == 0.f && g.s > 0.f); }
+};
+__device__ __forceinline__ constexpr unsigned round_bits(unsigned places) {   // ROUND's bits at every nibble of `places` (a bit each)
+  unsigned sum = 0;
+  for (int i = 0; i < 8; ++i)
+    if (places >> i & 1) sum += 0x4b400000u << (4 * i);
+  return sum;
+}
+
+// Consecutive numbers of a row: two or four, on a boundary of as many
+template <typename T, int N> __device__ __forceinline__ void load_row(float (&x)[N], const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (N == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p);
+      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+      const float2 v = *reinterpret_cast<const float2*>(p);
+      x[0] = v.x; x[1] = v.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const unsigned v = reinterpret_cast<const unsigned*>(p)[i / 2];
+      x[i] = __uint_as_float(v << 16);
+      x[i + 1] = __uint_as_float(v & 0xffff0000u);
+    }
+  }
+}
+
+// Where a token's rows of one head go.
+struct Place { unsigned char *k, *v; int t; };
+__device__ __forceinline__ Place place_of(unsigned char* k_pages, unsigned char* v_pages, const int* page_table, int max_pages, int slot, int pos, int page, int n_kv,
+                                          int head, size_t tile) {
+  const int whole = page == 64 ? pos >> 6 : pos / page;
+  const size_t at = ((size_t)page_table[(size_t)slot * max_pages + whole] * n_kv + head) * tile;
+  return {k_pages + at, v_pages + at, pos - whole * page};
+}
+
+// The range of a lane's numbers, which `near` lanes at a distance of `apart` share, over the group: of the two steps of a unit, and of further lanes for groups
+// of more than a unit.
+__device__ __forceinline__ void group_range(float (&lo)[2], float (&hi)[2], int near, int apart, int group) {
   if (group >= 32) {
     lo[0] = lo[1] = fminf(lo[0], lo[1]);
     hi[0] = hi[1] = fmaxf(hi[0], hi[1]);
@@ -14,56 +86,64 @@ __device__ __forceinline__ void group_range(float (&lo)[2], float (&hi)[2], int 
   for (int o = 1; o < lanes; o <<= 1) {
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      lo[p] = fminf(lo[p], __shfl_xor_sync(0xffffffffu, lo[p], o));
-      hi[p] = fmaxf(hi[p], __shfl_xor_sync(0xffffffffu, hi[p], o));
+      lo[p] = fminf(lo[p], __shfl_xor_sync(0xffffffffu, lo[p], o * apart));
+      hi[p] = fmaxf(hi[p], __shfl_xor_sync(0xffffffffu, hi[p], o * apart));
     }
   }
 }
-// fminf and fmaxf pass over NaN: a number that is not finite makes the range infinite
-__device__ __forceinline__ void widen(float x, float& lo, float& hi) {
-  const bool fine = fabsf(x) < INFINITY;
-  lo = fminf(lo, fine ? x : -INFINITY);
-  hi = fmaxf(hi, fine ? x : INFINITY);
-}
 
-// Where a token's rows of one head go.
-struct Place { unsigned char *k, *v; int t; };
-__device__ __forceinline__ Place place_of(unsigned char* k_pages, unsigned char* v_pages, const int* page_table, int max_pages, int slot, int pos, int page, int n_kv,
-                                          int head, size_t tile) {
-  const size_t at = ((size_t)page_table[(size_t)slot * max_pages + pos / page] * n_kv + head) * tile;
-  return {k_pages + at, v_pages + at, pos % page};
-}
-
-// A token's key of one head, by a warp: 4 U lanes of eight dims.
-template <typename T>
-__device__ __forceinline__ void store_key(const T* row, unsigned char* tile, int t, int d, int group, int page) {
-  const int lane = threadIdx.x & 31, u = lane >> 2, c = lane & 3, units = kv4_units(d);
-  float x[2][4], lo[2], hi[2];
+// A token's key of one head: 4 U lanes of eight dims, `part` this lane's number among them (of as many as the next power of two).  Every lane of the warp
+// calls this; `have` false: for nothing.
+template <typename T> __device__ __forceinline__ void load_key(float (&x)[2][4], const T* row, int part, int d, bool have) {
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
-    lo[p] = INFINITY;
-    hi[p] = -INFINITY;
-    const int at = 32 * u + 16 * p + 4 * c;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x[p][e] = at < d ? to_f32<T>(row[at + e]) : 0.f;
-      if (at < d) widen(x[p][e], lo[p], hi[p]);
-    }
+    const int at = 32 * (part >> 2) + 16 * p + 4 * (part & 3);
+    x[p][0] = x[p][1] = x[p][2] = x[p][3] = 0.f;
+    if (have && at < d) load_row<T, 4>(x[p], row + at);
   }
-  group_range(lo, hi, 4, group);
+}
+template <int GS> __device__ __forceinline__ void store_key(const float (&x)[2][4], bool have, int part, unsigned char* tile, int t, int d, int page) {
+  constexpr int group = 16 * GS;
+  const int u = part >> 2, c = part & 3, units = kv4_units(d);
+  float lo[2], hi[2];
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    Range range;
+    if (have && 32 * u + 16 * p < d) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) range.add(x[p][e]);
+    }
+    range.close();
+    lo[p] = range.lo;
+    hi[p] = range.hi;
+  }
+  group_range(lo, hi, 4, 1, group);
+  if (!have || u >= units) return;
   unsigned* const scales = reinterpret_cast<unsigned*>(tile + (size_t)kv4_row_bytes(d) * page) + t * (d / group);
   unsigned word = 0;
+  constexpr int STEPS = GS == 1 ? 1 : 2;   // of the unit that share a scale
 #pragma unroll
-  for (int p = 0; p < 2; ++p) {
-    const GroupCode g = group_code(lo[p], hi[p]);
+  for (int p = 0; p < 2; p += STEPS) {
     const int at = 32 * u + 16 * p;
-    if (at < d) {
+    if (at >= d) continue;
+    Coder code(lo[p], hi[p]);
+    unsigned steps = 0u - (STEPS == 2 ? round_bits(0xff) : p ? round_bits(0xcc) : round_bits(0x33));
+    const auto place = [](int q, int e) { return 8 * q + 4 * (e >> 1) + 16 * (e & 1); };
 #pragma unroll
-      for (int e = 0; e < 4; ++e) word |= code_of(x[p][e], g) << (8 * p + 4 * (e >> 1) + 16 * (e & 1));
-      if (c == 0 && at % group == 0) scales[at / group] = pack_code(g);
+    for (int q = p; q < p + STEPS; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) steps = code.add(steps, x[q][e], place(q, e));
+    if (code.undecided()) {
+      steps = 0;
+#pragma unroll
+      for (int q = p; q < p + STEPS; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) steps |= code_of(x[q][e], code.g) << place(q, e);
     }
+    word |= steps;
+    if (c == 0 && at % group == 0) scales[at / group] = pack_code(code.g);
   }
-  if (u < units) *reinterpret_cast<unsigned*>(tile + (size_t)t * kv4_row_bytes(d) + (c * units + u) * 4) = word;
+  *reinterpret_cast<unsigned*>(tile + (size_t)t * kv4_row_bytes(d) + (c * units + u) * 4) = word;
 }
 
 // A token's value of one head, by a warp: 8 U lanes of four dims.
@@ -73,45 +153,177 @@ __device__ __forceinline__ void store_value(const T* row, unsigned char* tile, i
   unsigned* const scales = reinterpret_cast<unsigned*>(tile + (size_t)kv4_row_bytes(d) * page) + t * (d / group);
   for (int u0 = 0; u0 < units; u0 += 4) {
     const int u = u0 + (lane >> 3), r = lane & 7;
-    float x[2][2], lo[2], hi[2];
+    float x[2][2] = {}, lo[2], hi[2];
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      lo[p] = INFINITY;
-      hi[p] = -INFINITY;
+      Range range;
       const int at = 32 * u + 16 * p + 2 * r;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        x[p][e] = at < d ? to_f32<T>(row[at + e]) : 0.f;
-        if (at < d) widen(x[p][e], lo[p], hi[p]);
+      if (at < d) {
+        load_row<T, 2>(x[p], row + at);
+        range.add(x[p][0]);
+        range.add(x[p][1]);
       }
+      range.close();
+      lo[p] = range.lo;
+      hi[p] = range.hi;
     }
-    group_range(lo, hi, 8, group);
+    group_range(lo, hi, 8, 1, group);
+    if (u >= units) continue;
     unsigned bits = 0;
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const GroupCode g = group_code(lo[p], hi[p]);
       const int at = 32 * u + 16 * p;
       if (at < d) {
-        bits |= (code_of(x[p][0], g) | code_of(x[p][1], g) << 4) << (8 * p);
-        if (r == 0 && at % group == 0) scales[at / group] = pack_code(g);
+        Coder code(lo[p], hi[p]);
+        unsigned both = code.add(code.add(0u - round_bits(3), x[p][0], 0), x[p][1], 4);
+        if (code.undecided()) both = code_of(x[p][0], code.g) | code_of(x[p][1], code.g) << 4;
+        bits |= both << (8 * p);
+        if (r == 0 && at % group == 0) scales[at / group] = pack_code(code.g);
       }
     }
-    if (u < units) *reinterpret_cast<unsigned short*>(tile + kv4_value_at(t, r, u, units)) = (unsigned short)bits;
+    *reinterpret_cast<unsigned short*>(tile + kv4_value_at(t, r, u, units)) = (unsigned short)bits;
   }
 }
 
-// A warp per (token, key head).
-template <typename T>
+// Up to 16 tokens that follow one another in a tile of 16, tile places i0 to i0 + count - 1: the UB units from u0 on of their values of one head, by a warp.
+// Lane (r, c) takes what it would read, four tokens; GS: steps of 16 dims that share a scale.
+template <typename T, int UB, int GS>
+__device__ __forceinline__ void store_tile_values(const T* rows, long long stride, unsigned char* tile, int t0, int i0, int count, int u0, int d, int page) {
+  constexpr int NG = 2 * UB / GS;   // groups of UB units
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, units = kv4_units(d), groups = d / (16 * GS);
+  unsigned* const scales = reinterpret_cast<unsigned*>(tile + (size_t)kv4_row_bytes(d) * page);
+  unsigned bits[UB][2];
+#pragma unroll
+  for (int b = 0; b < UB; ++b) bits[b][0] = bits[b][1] = 0;
+  const bool all = 2 * c >= i0 && 2 * c + 9 < i0 + count;   // the lane's four tokens are written together
+  float x[4][2 * UB][2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int s = 0; s < 2 * UB; ++s) {
+      const int k = 2 * c + (i & 1) + 8 * (i >> 1), at = 32 * u0 + 16 * s + 2 * r;
+      x[i][s][0] = x[i][s][1] = 0.f;
+      if (k >= i0 && k < i0 + count && at < d) load_row<T, 2>(x[i][s], rows + (k - i0) * stride + at);
+    }
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    // the ranges of the lane's four tokens, over the lanes of the group; lane row r & 3 works out one token's scale for all
+    float lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      Range range;
+#pragma unroll
+      for (int s = g * GS; s < (g + 1) * GS; ++s)
+        if (32 * u0 + 16 * s < d) {
+          range.add(x[i][s][0]);
+          range.add(x[i][s][1]);
+        }
+      range.close();
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        range.lo = fminf(range.lo, __shfl_xor_sync(0xffffffffu, range.lo, o));
+        range.hi = fmaxf(range.hi, __shfl_xor_sync(0xffffffffu, range.hi, o));
+      }
+      if ((r & 3) == i) {
+        lo = range.lo;
+        hi = range.hi;
+      }
+    }
+    const GroupCode one = group_code(lo, hi);
+    const unsigned packed = pack_code(one);
+    const float inverse = Coder::inverse(one.s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = 2 * c + (i & 1) + 8 * (i >> 1);
+      const unsigned sz = __shfl_sync(0xffffffffu, packed, i * 4 + c);
+      Coder code(unpack_code(sz), __shfl_sync(0xffffffffu, inverse, i * 4 + c));
+      if (k < i0 || k >= i0 + count || 32 * u0 + 16 * GS * g >= d) continue;
+      unsigned half[(GS + 1) / 2] = {};   // the 16 bits of each unit of the group (or of one step of it)
+#pragma unroll
+      for (int s = g * GS; s < (g + 1) * GS; ++s) {
+        unsigned& h = half[s / 2 - g * GS / 2];
+        h = code.add(code.add(h - round_bits(s & 1 ? 0xc : 0x3), x[i][s][0], 8 * (s & 1)), x[i][s][1], 8 * (s & 1) + 4);
+      }
+      if (code.undecided()) {
+#pragma unroll
+        for (int s = g * GS; s < (g + 1) * GS; ++s) {
+          unsigned& h = half[s / 2 - g * GS / 2];
+          if (GS == 1 || (s & 1) == 0) h = 0;
+          h |= (code_of(x[i][s][0], code.g) | code_of(x[i][s][1], code.g) << 4) << (8 * (s & 1));
+        }
+      }
+#pragma unroll
+      for (int s = g * GS; s < (g + 1) * GS; s += 2) bits[s / 2][i >> 1] |= half[s / 2 - g * GS / 2] << (16 * (i & 1));
+      if (r == 0) scales[(t0 + k) * groups + (32 * u0) / (16 * GS) + g] = sz;
+    }
+  }
+  if (!all) {   // ... or 16 bits each
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = 2 * c + (i & 1) + 8 * (i >> 1);
+      if (k < i0 || k >= i0 + count) continue;
+#pragma unroll
+      for (int b = 0; b < UB; ++b)
+        *reinterpret_cast<unsigned short*>(tile + kv4_value_at(t0 + k, r, u0 + b, units)) = (unsigned short)(bits[b][i >> 1] >> (16 * (i & 1)));
+    }
+  }
+  if (all) {
+#pragma unroll
+    for (int b = 0; b < UB; ++b) *reinterpret_cast<uint2*>(tile + kv4_value_at(t0 + 2 * c, r, u0 + b, units)) = make_uint2(bits[b][0], bits[b][1]);
+  }
+}
+
+// Grid (blocks, key heads).  Keys by the first `key_blocks` blocks, values by the others.
+// Keys: as many lanes for a token as a row has words of eight dims, or the next power of two; a thread takes KEY_TOKENS tokens.
+// Values: a warp per `span` consecutive tokens of the launch and UB units.  Tokens that follow one another in one tile of 16 places of a page are
+// stored together, by the warp that has the first of them.
+constexpr int KEY_TOKENS = 4;
+template <typename T, int UB, int GS>
 __global__ void __launch_bounds__(WARPS * 32) kv4_store_kernel(const T* k, const T* v, long long stride, const int* __restrict__ tok_slot,
                                                                const int* __restrict__ tok_pos, unsigned char* k_pages, unsigned char* v_pages,
-                                                               const int* __restrict__ page_table, int max_pages, int n_kv, int d, int group, int page) {
-  const int head = blockIdx.y * WARPS + (threadIdx.x >> 5);
-  const long long n = blockIdx.x;
-  const int slot = tok_slot[n], pos = tok_pos[n];
-  if (slot < 0 || head >= n_kv) return;
-  const Place at = place_of(k_pages, v_pages, page_table, max_pages, slot, pos, page, n_kv, head, kv4_tile_bytes(page, d, group));
-  store_key(k + n * stride + (size_t)head * d, at.k, at.t, d, group, page);
-  store_value(v + n * stride + (size_t)head * d, at.v, at.t, d, group, page);
+                                                               const int* __restrict__ page_table, int max_pages, int n, int d, int page, int span, int key_blocks,
+                                                               int lane_bits) {
+  const int lane = threadIdx.x & 31, head = blockIdx.y, n_kv = gridDim.y;
+  constexpr int GROUP = 16 * GS;
+  const size_t tile_bytes = kv4_tile_bytes(page, d, GROUP);
+  if ((int)blockIdx.x < key_blocks) {
+    const int at_once = (WARPS * 32) >> lane_bits, part = threadIdx.x & ((1 << lane_bits) - 1);
+    const int t0 = blockIdx.x * (at_once * KEY_TOKENS) + (threadIdx.x >> lane_bits);
+    float x[KEY_TOKENS][2][4];
+    int slot[KEY_TOKENS], pos[KEY_TOKENS];
+#pragma unroll
+    for (int i = 0; i < KEY_TOKENS; ++i) {
+      const int t = t0 + i * at_once;
+      slot[i] = t < n ? tok_slot[t] : -1;
+      pos[i] = t < n ? tok_pos[t] : 0;
+      load_key<T>(x[i], k + (long long)t * stride + (size_t)head * d, part, d, t < n);
+    }
+#pragma unroll
+    for (int i = 0; i < KEY_TOKENS; ++i) {
+      Place at = {};
+      if (slot[i] >= 0) at = place_of(k_pages, v_pages, page_table, max_pages, slot[i], pos[i], page, n_kv, head, tile_bytes);
+      store_key<GS>(x[i], slot[i] >= 0, part, at.k, at.t, d, page);
+    }
+    return;
+  }
+  const int job = (blockIdx.x - key_blocks) * WARPS + (threadIdx.x >> 5), parts = kv4_units(d) / UB;
+  const long long n0 = (long long)(job / parts) * span;
+  if (n0 >= n) return;
+  // the launch's tokens from n0 on, one a lane: those that begin a run, and (of the 32 that are looked at) where runs go on
+  const long long mine = n0 + lane;
+  const int slot = mine < n ? tok_slot[mine] : -1, pos = mine < n ? tok_pos[mine] : 0;
+  const bool goes_on = mine < n && mine > 0 && slot >= 0 && tok_slot[mine - 1] == slot && tok_pos[mine - 1] == pos - 1 && pos % 16 != 0;
+  const unsigned on = __ballot_sync(0xffffffffu, goes_on);
+  unsigned first = __ballot_sync(0xffffffffu, lane < span && slot >= 0 && !goes_on);
+  while (first) {
+    const int i = __ffs(first) - 1;
+    first &= first - 1;
+    const unsigned behind = i == 31 ? 0u : ~(on >> (i + 1));   // a run has at most 16 tokens, and begins among the first 16
+    const int count = behind ? min(16, __ffs(behind)) : 16;
+    const int s = __shfl_sync(0xffffffffu, slot, i), p = __shfl_sync(0xffffffffu, pos, i);
+    const Place at = place_of(k_pages, v_pages, page_table, max_pages, s, p, page, n_kv, head, tile_bytes);
+    store_tile_values<T, UB, GS>(v + (n0 + i) * stride + (size_t)head * d, stride, at.v, at.t / 16 * 16, at.t % 16, count, (job % parts) * UB, d, page);
+  }
 }
 
 // The same behind a fused projection (rows q | k | v): per-head norm and rotation of queries and keys first, a warp per (token, head).  Formulas and
@@ -122,7 +334,7 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_rope_store_kernel(const T* qkv
                                                                     const int* __restrict__ tok_pos, T* q_out, unsigned char* k_pages, unsigned char* v_pages,
                                                                     const int* __restrict__ page_table, int max_pages, int n_heads, int n_kv, int d, int rot,
                                                                     int group, int page, float eps, int has_norm) {
-  __shared__ T rows[WARPS][256];
+  __shared__ __align__(16) T rows[WARPS][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = blockIdx.y * WARPS + warp, half = rot >> 1;
   const long long n = blockIdx.x;
   if (head >= n_heads + 2 * n_kv) return;
@@ -165,54 +377,128 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_rope_store_kernel(const T* qkv
     row[j + half] = from_f32<T>(__fadd_rn(rnd<T>(__fmul_rn(b, cs)), rnd<T>(__fmul_rn(a, sn))));
   }
   __syncwarp();
-  if (head >= n_heads) return store_key(row, at.k, at.t, d, group, page);
+  if (head >= n_heads) {
+    float k[2][4];
+    load_key<T>(k, row, lane, d, true);
+    if (group == 16) return store_key<1>(k, true, lane, at.k, at.t, d, page);
+    if (group == 32) return store_key<2>(k, true, lane, at.k, at.t, d, page);
+    if (group == 64) return store_key<4>(k, true, lane, at.k, at.t, d, page);
+    return store_key<8>(k, true, lane, at.k, at.t, d, page);
+  }
   for (int i = lane; i < d; i += 32) q_row[i] = row[i];
+}
+
+// What a pair of codes (`code_pair`) stands for, in T: z + (c - 7.5) s, rounded once.  c - 7.5 is exact in bfloat16.
+template <typename T> struct Pair;
+template <> struct Pair<__nv_bfloat16> { typedef unsigned type; };
+template <> struct Pair<float> { typedef float2 type; };
+template <typename T> __device__ __forceinline__ typename Pair<T>::type values_of(unsigned pair, unsigned sz_lo, unsigned sz_hi) {
+  if constexpr (sizeof(T) == 2) {
+    const __nv_bfloat162 less = __floats2bfloat162_rn(-CODE_BIAS, -CODE_BIAS);
+    const unsigned s = __byte_perm(sz_lo, sz_hi, 0x5410), z = __byte_perm(sz_lo, sz_hi, 0x7632);
+    const __nv_bfloat162 v = __hfma2(__hadd2(*reinterpret_cast<const __nv_bfloat162*>(&pair), less), *reinterpret_cast<const __nv_bfloat162*>(&s),
+                                     *reinterpret_cast<const __nv_bfloat162*>(&z));
+    return *reinterpret_cast<const unsigned*>(&v);
+  } else {
+    const GroupCode a = unpack_code(sz_lo), b = unpack_code(sz_hi);
+    return make_float2(fmaf(__uint_as_float(pair << 16) - CODE_BIAS, a.s, a.z), fmaf(__uint_as_float(pair & 0xffff0000u) - CODE_BIAS, b.s, b.z));
+  }
 }
 
 // Blocks per (sequence, key head), each every gridDim.x-th page of it: the page's tokens as values, those behind the sequence's end as zeros.  Pages before the
 // first key that the step's first token of the sequence sees (window <= 0: every key) are left alone: they may be another sequence's by now.
+// A thread takes a word of a key (eight dims of a token) or a unit of a lane's values (four dims of four tokens); neighbours fill whole sectors.
 template <typename T>
-__global__ void __launch_bounds__(256) kv4_expand_kernel(const unsigned char* k_pages, const unsigned char* v_pages, const int* __restrict__ page_table,
-                                                         int max_pages, const int* __restrict__ cu_q, const int* __restrict__ seq_slot,
-                                                         const int* __restrict__ tok_pos, T* k_out, T* v_out, int n_kv, int d, int group, int page, int window) {
+__global__ void __launch_bounds__(256, 4) kv4_expand_kernel(const unsigned char* __restrict__ k_pages, const unsigned char* __restrict__ v_pages,
+                                                         const int* __restrict__ page_table, int max_pages, const int* __restrict__ cu_q,
+                                                         const int* __restrict__ seq_slot, const int* __restrict__ tok_pos, T* k_out, T* v_out, int n_kv, int d,
+                                                         int group_bits, int page, int window) {
+  typedef typename Pair<T>::type P;
   const int b = blockIdx.z, head = blockIdx.y, slot = seq_slot[b];
   if (slot < 0 || cu_q[b + 1] <= cu_q[b]) return;
   const int end = tok_pos[cu_q[b + 1] - 1] + 1, first = window > 0 ? max(0, tok_pos[cu_q[b]] + 1 - window) / page : 0;
-  const int units = kv4_units(d), groups = d / group;
+  const int units = kv4_units(d), groups = d >> group_bits, row = kv4_row_bytes(d), words = 4 * units;
+  const size_t tile_bytes = kv4_tile_bytes(page, d, 1 << group_bits);
+  // keys: the thread's word, and its tokens, `t_step` apart.  Values: its lane row r, unit u, and its (tile, c), `j_step` apart.
+  const int t_step = 256 / words, kt0 = threadIdx.x / words, kx = threadIdx.x % words, ku = kx >> 2, kc = kx & 3;
+  const int j_step = 32 / units, j0 = (threadIdx.x >> 3) / units, u = (threadIdx.x >> 3) % units, r = threadIdx.x & 7;
   for (int p = first + blockIdx.x; p * page < end; p += gridDim.x) {
     const size_t at_page = (size_t)page_table[(size_t)slot * max_pages + p] * n_kv + head;
-    const unsigned char *kt = k_pages + at_page * kv4_tile_bytes(page, d, group), *vt = v_pages + at_page * kv4_tile_bytes(page, d, group);
-    const unsigned *ks = reinterpret_cast<const unsigned*>(kt + (size_t)kv4_row_bytes(d) * page), *vs = reinterpret_cast<const unsigned*>(vt + (size_t)kv4_row_bytes(d) * page);
+    const unsigned char *kt = k_pages + at_page * tile_bytes, *vt = v_pages + at_page * tile_bytes;
+    const unsigned *ks = reinterpret_cast<const unsigned*>(kt + (size_t)row * page), *vs = reinterpret_cast<const unsigned*>(vt + (size_t)row * page);
     T *ko = k_out + at_page * page * d, *vo = v_out + at_page * page * d;
-    for (int i = threadIdx.x; i < page * d; i += blockDim.x) {
-      const int t = i / d, x = i % d, u = x / 32, h = (x >> 4) & 1;
-      float kv = 0.f, vv = 0.f;
-      if (p * page + t < end) {
-        const int c = (x & 15) >> 2, e = x & 3, r = (x & 15) >> 1;
-        const unsigned kw = *reinterpret_cast<const unsigned*>(kt + (size_t)t * kv4_row_bytes(d) + (c * units + u) * 4);
-        const unsigned vw = *reinterpret_cast<const unsigned short*>(vt + kv4_value_at(t, r, u, units));
-        kv = value_of(kw >> (8 * h + 4 * (e >> 1) + 16 * (e & 1)) & 15u, unpack_code(ks[t * groups + x / group]));
-        vv = value_of(vw >> (8 * h + 4 * (x & 1)) & 15u, unpack_code(vs[t * groups + x / group]));
+    const int left = end - p * page;
+    if (kt0 < t_step)
+#pragma unroll 2
+      for (int t = kt0; t < page; t += t_step) {
+        const bool have = t < left;
+        const unsigned w = have ? *reinterpret_cast<const unsigned*>(kt + t * row + (kc * units + ku) * 4) : 0u;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const int at = 32 * ku + 16 * s;
+          if (at >= d) continue;
+          const unsigned sz = have ? ks[t * groups + (at >> group_bits)] : 0u;
+          P* const to = reinterpret_cast<P*>(ko + t * d + at + 4 * kc);
+          const P a = values_of<T>(code_pair(w, 2 * s), sz, sz), e = values_of<T>(code_pair(w, 2 * s + 1), sz, sz);
+          if constexpr (sizeof(T) == 2)
+            *reinterpret_cast<uint2*>(to) = make_uint2(a, e);
+          else
+            *reinterpret_cast<float4*>(to) = make_float4(a.x, a.y, e.x, e.y);
+        }
       }
-      ko[i] = from_f32<T>(kv);
-      vo[i] = from_f32<T>(vv);
-    }
+    if (j0 < j_step)
+#pragma unroll 2
+      for (int j = j0; j < page / 4; j += j_step) {
+        const int c = j & 3, tile = j >> 2, k0 = tile * 16 + 2 * c;
+        const uint2 w = *reinterpret_cast<const uint2*>(vt + (tile * 256 + (r * 4 + c) * 8) * units + u * 8);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)   // tokens k0, k0 + 1 and k0 + 8, k0 + 9
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const int at = 32 * u + 16 * s;
+            if (at >= d) continue;
+            const unsigned x = h ? w.y : w.x, a = code_pair(x, 2 * s), e = code_pair(x, 2 * s + 1);
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+              const int t = k0 + 8 * h + o;
+              const unsigned sz = t < left ? vs[t * groups + (at >> group_bits)] : 0u;
+              *reinterpret_cast<P*>(vo + t * d + at + 2 * r) = values_of<T>(__byte_perm(a, e, o ? 0x7632 : 0x5410), sz, sz);
+            }
+          }
+      }
   }
 }
 
+template <typename T, int UB, int GS>
+int store_as(const void* k, const void* v, long long stride, const int* tok_slot, const int* tok_pos, void* k_pages, void* v_pages, const int* page_table,
+             int max_pages, int n, int n_kv, int d, int page, cudaStream_t st) {
+  // few tokens: a warp each, so that none waits for another; many: a warp for 16, most of which begin one run
+  const int span = n > 512 ? 16 : 1, lane_bits = d > 128 ? 5 : d > 64 ? 4 : d > 32 ? 3 : 2;
+  const int key_tokens = (WARPS * 32 >> lane_bits) * KEY_TOKENS, key_blocks = (n + key_tokens - 1) / key_tokens;
+  const int warps = (n + span - 1) / span * (kv4_units(d) / UB), value_blocks = (warps + WARPS - 1) / WARPS;
+  kv4_store_kernel<T, UB, GS><<<dim3(key_blocks + value_blocks, n_kv), WARPS * 32, 0, st>>>(
+      (const T*)k, (const T*)v, stride, tok_slot, tok_pos, (unsigned char*)k_pages, (unsigned char*)v_pages, page_table, max_pages, n, d, page, span, key_blocks, lane_bits);
+  return launch_status();
+}
 template <typename T>
 int store(const void* k, const void* v, long long stride, const int* tok_slot, const int* tok_pos, void* k_pages, void* v_pages, const int* page_table,
           int max_pages, int n, int n_kv, int d, int group, int page, cudaStream_t st) {
-  kv4_store_kernel<T><<<dim3(n, (n_kv + WARPS - 1) / WARPS), WARPS * 32, 0, st>>>((const T*)k, (const T*)v, stride, tok_slot, tok_pos, (unsigned char*)k_pages,
-                                                                                 (unsigned char*)v_pages, page_table, max_pages, n_kv, d, group, page);
-  return launch_status();
+#define DRYFT_STORE(UB, GS) return store_as<T, UB, GS>(k, v, stride, tok_slot, tok_pos, k_pages, v_pages, page_table, max_pages, n, n_kv, d, page, st)
+  switch (group) {   // units that a warp takes: those of a group
+    case 16: DRYFT_STORE(1, 1);
+    case 32: DRYFT_STORE(1, 2);
+    case 64: DRYFT_STORE(2, 4);
+    case 128: DRYFT_STORE(4, 8);
+  }
+#undef DRYFT_STORE
+  return DRYFT_ERR_UNSUPPORTED;
 }
 template <typename T>
 int expand(const void* k_pages, const void* v_pages, const int* page_table, int max_pages, const int* cu_q, const int* seq_slot, const int* tok_pos, void* k_out,
            void* v_out, int n_seqs, int pages, int n_kv, int d, int group, int page, int window, cudaStream_t st) {
   const int blocks = 4096 / (n_kv * n_seqs) + 1;   // of a sequence and head: a few thousand blocks, however long the sequences may be
   kv4_expand_kernel<T><<<dim3(blocks < pages ? blocks : pages, n_kv, n_seqs), 256, 0, st>>>((const unsigned char*)k_pages, (const unsigned char*)v_pages, page_table, max_pages, cu_q,
-                                                                  seq_slot, tok_pos, (T*)k_out, (T*)v_out, n_kv, d, group, page, window);
+                                                                  seq_slot, tok_pos, (T*)k_out, (T*)v_out, n_kv, d, __builtin_ctz(group), page, window);
   return launch_status();
 }
 template <typename T>
