@@ -65,28 +65,39 @@ __global__ void __launch_bounds__(WARPS * 32) linear4_f32_kernel(const float* x,
   }
 }
 
-// A warp per block of 64 inputs of a tile: what its codes stand for, in T.
-template <typename T>
-__global__ void __launch_bounds__(256) weight4_expand_kernel(const uint4* __restrict__ codes, const uint2* __restrict__ scales, T* w, int n, int k, int group) {
-  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, blocks = blocks_of(k), groups = groups_of(k, group);
+// A warp per block of 64 inputs of a tile: what its codes stand for.  PART 0: in float32, 1: rounded to bfloat16, 2: what that rounding left, rounded to bfloat16.
+// A lane writes four numbers of a row at a time; four neighbours fill a sector.
+template <int PART>
+__global__ void __launch_bounds__(256) weight4_expand_kernel(const uint4* __restrict__ codes, const uint2* __restrict__ scales, void* w, int n, int k, int group_bits) {
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, blocks = blocks_of(k), groups = groups_of(k, 1 << group_bits);
   const long long at = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), total = (long long)((n + 15) / 16) * blocks;
   if (at >= total) return;
   const long long tile = at / blocks;
   const int b = (int)(at % blocks);
-  const uint4 raw = codes[at * 32 + lane];
+  const uint4 raw = __ldcs(codes + at * 32 + lane);
   const unsigned words[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
     const int col = 64 * b + 16 * s;
     if (col >= k) break;
-    const uint2 sz = scales[(tile * groups + col / group) * 8 + r];
-    const GroupCode g[2] = {unpack_code(sz.x), unpack_code(sz.y)};
+    const uint2 sz = scales[(tile * groups + (col >> group_bits)) * 8 + r];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const long long row = tile * 16 + r + 8 * h;
       if (row >= n) continue;
+      const GroupCode g = unpack_code(h ? sz.y : sz.x);
+      float v[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[row * k + col + 4 * c + e] = from_f32<T>(value_of(words[s] >> (4 * (2 * (e >> 1) + h) + 16 * (e & 1)) & 15u, g[h]));
+      for (int e = 0; e < 4; ++e) v[e] = value_of(words[s] >> (4 * (2 * (e >> 1) + h) + 16 * (e & 1)) & 15u, g);
+      if (PART == 0) {
+        *reinterpret_cast<float4*>((float*)w + row * k + col + 4 * c) = make_float4(v[0], v[1], v[2], v[3]);
+      } else {
+        if (PART == 2)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] -= rnd<__nv_bfloat16>(v[e]);   // exact
+        const __nv_bfloat162 x = __floats2bfloat162_rn(v[0], v[1]), y = __floats2bfloat162_rn(v[2], v[3]);
+        *reinterpret_cast<uint2*>((__nv_bfloat16*)w + row * k + col + 4 * c) = make_uint2(*reinterpret_cast<const unsigned*>(&x), *reinterpret_cast<const unsigned*>(&y));
+      }
     }
   }
 }
@@ -480,13 +491,11 @@ DRYFT_API int dryft_linear4(int is_bf16, int out_bf16, const void* x, long long 
   return launch_status();
 }
 
-DRYFT_API int dryft_weight4_expand(int is_bf16, const void* codes, const void* scales, void* w, int n, int k, int group, void* stream) {
+// part 0: float32; 1: bfloat16; 2: the rest of that rounding in bfloat16
+DRYFT_API int dryft_weight4_expand(int part, const void* codes, const void* scales, void* w, int n, int k, int group, void* stream) {
   if (n <= 0) return 0;
   const long long total = (long long)((n + 15) / 16) * blocks_of(k);
-  const unsigned grid = (unsigned)((total + 7) / 8);
-  if (is_bf16)
-    weight4_expand_kernel<__nv_bfloat16><<<grid, 256, 0, (cudaStream_t)stream>>>((const uint4*)codes, (const uint2*)scales, (__nv_bfloat16*)w, n, k, group);
-  else
-    weight4_expand_kernel<float><<<grid, 256, 0, (cudaStream_t)stream>>>((const uint4*)codes, (const uint2*)scales, (float*)w, n, k, group);
+  auto kern = part == 0 ? weight4_expand_kernel<0> : part == 1 ? weight4_expand_kernel<1> : weight4_expand_kernel<2>;
+  kern<<<(unsigned)((total + 7) / 8), 256, 0, (cudaStream_t)stream>>>((const uint4*)codes, (const uint2*)scales, w, n, k, __builtin_ctz(group));
   return launch_status();
 }

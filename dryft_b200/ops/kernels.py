@@ -2616,11 +2616,16 @@ def linear4(x, w: Weight4, out, pdl: bool = False) -> None:
     launch_count += 1
 
 
-def weight4_expand(w: Weight4, out) -> None:
-    """``out`` ``[n, k]`` (float32 or bfloat16): what the codes stand for, for products of many rows."""
+def weight4_expand(w: Weight4, out, rest: bool = False) -> None:
+    """``out`` ``[n, k]`` (float32 or bfloat16): what the codes stand for, for products of many rows.  ``rest``: what rounding that to bfloat16 leaves, itself
+    rounded to bfloat16 (the two together are off by 2^-17)."""
     _need_weight4(w)
     _need(out, "out", None, (w.n, w.k))
-    _ok(linear4_lib().dryft_weight4_expand(_act(out, "out"), _ptr(w.codes), _ptr(w.scales), _ptr(out), w.n, w.k, w.group, _stream()), "weight4_expand")
+    is_bf16 = _act(out, "out")
+    if rest and not is_bf16:
+        raise KernelError("weight4_expand: the rest of a rounding is bfloat16")
+    _ok(linear4_lib().dryft_weight4_expand(2 if rest else is_bf16, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), w.n, w.k, w.group, _stream()),
+        "weight4_expand")
 
 
 def kv4_lib() -> ctypes.CDLL:

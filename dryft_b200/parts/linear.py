@@ -66,31 +66,34 @@ def held(w: torch.Tensor, rt: Runtime):
     return K.pack_weight4(w, K.bits4_group(w.shape[1], rt.bits_group)) if rt.weight_bits == 4 else w
 
 
-EXPAND_BYTES = 48 << 20   # of weights at a time that a product of many rows takes out of their 4 bits: they stay in L2 until the product has read them
+EXPAND_BYTES = 256 << 20   # of weights at a time that a product of many rows takes out of their 4 bits (which bounds what that holds)
 
 
 def _linear4(x: torch.Tensor, w: K.Weight4, rt: Runtime, out_dtype: torch.dtype) -> torch.Tensor:
-    """Up to ``K.LINEAR4_ROWS`` rows the kernel reads the codes; more rows take the weights out of their 4 bits, a part at a time, for the product
-    that such rows run on otherwise."""
+    """Up to ``K.LINEAR4_ROWS`` rows the kernel reads the codes; more rows take the weights out of their 4 bits, for the product that such rows run on
+    otherwise.  For 32-bit results from bfloat16 activations the weights are taken out as two bfloat16 numbers whose sum they are, with a product each."""
     m, (n, k) = x.shape[0], w.shape
+    out = torch.empty((m, n), dtype=out_dtype, device=x.device)
     if m <= K.LINEAR4_ROWS:
-        out = torch.empty((m, n), dtype=out_dtype, device=x.device)
         K.linear4(x, w, out, pdl=rt.pdl)
         return out
-    out = torch.empty((m, n), dtype=out_dtype, device=x.device)
     step = max(16, EXPAND_BYTES // (k * x.element_size()) // 16 * 16)
-    part = torch.empty((min(step, n), k), dtype=x.dtype, device=x.device)
+    buf = torch.empty((min(step, n), k), dtype=x.dtype, device=x.device)
     for first in range(0, n, step):
         end = min(n, first + step)
-        K.weight4_expand(w.rows(first, end), part[:end - first])
+        part, rows, at = buf[:end - first], w if end - first == n else w.rows(first, end), out[:, first:end]
+        K.weight4_expand(rows, part)
         if x.dtype == torch.float32:
-            y = torch.empty((m, end - first), dtype=torch.float32, device=x.device)
-            K.gemm_nt_f32(x, part[:end - first], y)
-            out[:, first:end] = y
+            y = at if end - first == n else torch.empty((m, end - first), dtype=torch.float32, device=x.device)
+            K.gemm_nt_f32(x, part, y)
+            if y is not at:
+                at.copy_(y)
         elif out_dtype == torch.bfloat16:
-            torch.mm(x, part[:end - first].t(), out=out[:, first:end])
+            torch.mm(x, part.t(), out=at)
         else:
-            out[:, first:end] = torch.mm(x, part[:end - first].t(), out_dtype=out_dtype)
+            y = torch.mm(x, part.t(), out_dtype=out_dtype)
+            K.weight4_expand(rows, part, rest=True)
+            torch.add(y, torch.mm(x, part.t(), out_dtype=out_dtype), out=at)
     return out
 
 
