@@ -107,7 +107,6 @@ __global__ void __launch_bounds__(256) weight4_expand_kernel(const uint4* __rest
 // products are summed over 16 + c in a 32-bit accumulator of their own, then  y += s acc + (z - 23.5 s) sum_k x  in 32 bits, so nothing is rounded below
 // 32 bits before the result.  The warps of a block share a tile's inputs: each walks its own blocks of 64, their sums meet in shared memory.
 typedef __nv_bfloat16 bf16;
-constexpr int MMA_WARPS = 8;
 
 __device__ __forceinline__ float2 two_of(unsigned w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 
@@ -117,41 +116,6 @@ __device__ __forceinline__ void copy16(void* to, const void* from) {
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N)); }
 __device__ __forceinline__ unsigned word_of(uint4 v, int s) { return s == 0 ? v.x : s == 1 ? v.y : s == 2 ? v.z : v.w; }
-
-// A group's sums into the results: rows r and r + 8 of W, columns 2c and 2c + 1 of x, whose sums over the group are s0 and s1.
-__device__ __forceinline__ void add_group(float (&acc)[4], const float (&part)[4], uint2 sz, float s0, float s1) {
-  const GroupCode lo = unpack_code(sz.x), hi = unpack_code(sz.y);
-  const float zl = fmaf(-CODE_BIAS, lo.s, lo.z), zh = fmaf(-CODE_BIAS, hi.s, hi.z);
-  acc[0] = fmaf(lo.s, part[0], fmaf(zl, s0, acc[0]));
-  acc[1] = fmaf(lo.s, part[1], fmaf(zl, s1, acc[1]));
-  acc[2] = fmaf(hi.s, part[2], fmaf(zh, s0, acc[2]));
-  acc[3] = fmaf(hi.s, part[3], fmaf(zh, s1, acc[3]));
-}
-
-// The warps' sums of R tiles of W and NT of x, in the warps' order, into the results.  `red`: [warp][R][NT][lane][4].
-template <int NT, int R, typename O>
-__device__ __forceinline__ void join_warps(float (&acc)[R][NT][4], float* red, O* y, int m, int n, int row0) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  __syncthreads();   // the last tile's sums have been read
-#pragma unroll
-  for (int t = 0; t < R; ++t)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      *reinterpret_cast<float4*>(red + ((warp * R + t) * NT + j) * 128 + lane * 4) = make_float4(acc[t][j][0], acc[t][j][1], acc[t][j][2], acc[t][j][3]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[t][j][e] = 0.f;
-    }
-  __syncthreads();
-  for (int i = threadIdx.x; i < R * NT * 128; i += MMA_WARPS * 32) {
-    const int row = i % (16 * R), col = i / (16 * R), t = row >> 4;
-    // row (row & 15), column (col & 7) of a tile: lane (row & 7) * 4 + (col & 7) / 2, element 2 (row & 15 >= 8) + (col & 1)
-    const int place = (t * NT + (col >> 3)) * 128 + ((row & 7) * 4 + ((col & 7) >> 1)) * 4 + 2 * ((row >> 3) & 1) + (col & 1);
-    float v = 0.f;
-#pragma unroll
-    for (int w = 0; w < MMA_WARPS; ++w) v += red[w * R * NT * 128 + place];
-    if (row0 + row < n && col < m) y[(size_t)col * n + row0 + row] = from_f32<O>(v);
-  }
-}
 
 // Few rows of x (up to 16), all of whose numbers fit in shared memory: bound by the codes' bytes.  A block of 16 warps is 16 / TEAM teams; a team takes
 // a tile of 16 rows of W at a time, its warps the tile's inputs in turn shares.  Each warp copies its own share of the codes into its own ring, SLOTS - 1 slots of
@@ -333,95 +297,6 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) linear4_few_kernel(const bf
   copies_wait<0>();
 }
 
-// More rows, or more inputs than fit: R tiles of 16 rows of W against NT of x, a block of 64 inputs at a time from registers, the next one on its way.
-template <int NT, int R, int GS> struct Chunk {
-  uint4 w[R];
-  uint2 sz[R][4 / GS], x[NT][4];
-};
-
-template <int NT, int R, int GS, typename O>
-__global__ void __launch_bounds__(MMA_WARPS * 32) linear4_mma_kernel(const bf16* x, long long x_stride, const uint4* __restrict__ codes,
-                                                                     const uint2* __restrict__ scales, O* y, int m, int n, int k, int group) {
-  constexpr int NG = 4 / GS;
-  extern __shared__ __align__(16) unsigned char smem[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
-  const int blocks = blocks_of(k), groups = groups_of(k, group), tiles = (n + 15) / 16;
-  const int per = (blocks + MMA_WARPS - 1) / MMA_WARPS, b0 = min(blocks, warp * per), b1 = min(blocks, b0 + per);
-  auto load = [&](Chunk<NT, R, GS>& q, int b) {
-#pragma unroll
-    for (int t = 0; t < R; ++t) {
-      const int tile = min((int)blockIdx.x * R + t, tiles - 1);   // the last unit may repeat a tile; it is not stored twice
-      q.w[t] = codes[((size_t)tile * blocks + b) * 32 + lane];
-#pragma unroll
-      for (int g = 0; g < NG; ++g) q.sz[t][g] = scales[((size_t)tile * groups + (64 * b + 16 * GS * g) / group) * 8 + r];
-    }
-  };
-  auto load_x = [&](Chunk<NT, R, GS>& q, int b) {
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int col = 64 * b + 16 * s + 4 * c, row = 8 * j + r;
-        q.x[j][s] = col < k && row < m ? __ldcg(reinterpret_cast<const uint2*>(x + row * x_stride + col)) : make_uint2(0, 0);
-      }
-  };
-  let_next_launch_in();
-  Chunk<NT, R, GS> now;
-  if (b0 < b1) load(now, b0);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (b0 < b1) load_x(now, b0);
-  float acc[R][NT][4];
-#pragma unroll
-  for (int t = 0; t < R; ++t)
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[t][j][e] = 0.f;
-  for (int b = b0; b < b1; ++b) {
-    Chunk<NT, R, GS> next;
-    if (b + 1 < b1) {
-      load(next, b + 1);
-      load_x(next, b + 1);
-    }
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      float part[R][NT][4], sum[NT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        sum[j] = 0.f;
-#pragma unroll
-        for (int t = 0; t < R; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) part[t][j][e] = 0.f;
-      }
-#pragma unroll
-      for (int s = g * GS; s < (g + 1) * GS; ++s) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const float2 p = two_of(now.x[j][s].x), q = two_of(now.x[j][s].y);
-          sum[j] += (p.x + p.y) + (q.x + q.y);
-        }
-#pragma unroll
-        for (int t = 0; t < R; ++t) {
-          const unsigned v = word_of(now.w[t], s), a0 = code_pair(v, 0), a1 = code_pair(v, 1), a2 = code_pair(v, 2), a3 = code_pair(v, 3);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) mma_16816(part[t][j], a0, a1, a2, a3, now.x[j][s].x, now.x[j][s].y);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
-        sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
-        const float s0 = __shfl_sync(0xffffffffu, sum[j], 8 * c), s1 = __shfl_sync(0xffffffffu, sum[j], 8 * c + 4);
-#pragma unroll
-        for (int t = 0; t < R; ++t) add_group(acc[t][j], part[t][j], now.sz[t][g], s0, s1);
-      }
-    }
-    now = next;
-  }
-  join_warps<NT, R, O>(acc, reinterpret_cast<float*>(smem), y, m, n, blockIdx.x * R * 16);
-}
-
 constexpr size_t SMEM_MOST = 227 * 1024;
 
 template <typename... P, typename... A> int launch(void (*kern)(P...), bool& asked, int grid, int threads, size_t bytes, int pdl, cudaStream_t st, A... a) {
@@ -455,36 +330,30 @@ template <int NT, int GS, int TEAM, int PB, int SLOTS, typename O> int few(const
 // Four warps a tile where shared memory has room for their rings (x of 8 rows: up to about 6,000 inputs), else all sixteen with shorter rings.  2,560 inputs,
 // one row, four / eight / sixteen warps a tile: 151,936 outputs 55.6 / 63.6 / 81.9 us, 6,144 outputs 4.8 / 5.4 / 5.7 us (a tile's end costs each warp as much as
 // half a slot); 2,560 outputs of 9,728 inputs, hardly more tiles than multiprocessors, 9.6 / 9.7 / 10.2 us.
-template <int NT, int GS, typename O> bool few_rows(const Args& a, int* rc) {
+template <int NT, int GS, typename O> int few_rows(const Args& a) {
   constexpr int GM = GS == 8 ? 4 : GS;
-  if (Few<NT, GS, 4, 2, 4>::bytes(a.m, a.k) <= SMEM_MOST) return *rc = few<NT, GS, 4, 2, 4, O>(a), true;
-  if (Few<NT, GM, 16, 1, 4>::bytes(a.m, a.k) <= SMEM_MOST) return *rc = few<NT, GM, 16, 1, 4, O>(a), true;
-  return false;
+  if (Few<NT, GS, 4, 2, 4>::bytes(a.m, a.k) <= SMEM_MOST) return few<NT, GS, 4, 2, 4, O>(a);
+  return few<NT, GM, 16, 1, 4, O>(a);
 }
-template <int NT, int R, int GS, typename O> int more(const Args& a) {
-  static bool asked = false;
-  return launch(linear4_mma_kernel<NT, R, GS, O>, asked, ((a.n + 15) / 16 + R - 1) / R, MMA_WARPS * 32, (size_t)MMA_WARPS * R * NT * 512, a.pdl, a.st, (const bf16*)a.x, a.x_stride,
-                (const uint4*)a.codes, (const uint2*)a.scales, (O*)a.y, a.m, a.n, a.k, a.group);
+template <int NT> bool fits(int m, int k, int group) {
+  return (group >= 64 ? Few<NT, 4, 16, 1, 4>::bytes(m, k) : group == 32 ? Few<NT, 2, 16, 1, 4>::bytes(m, k) : Few<NT, 1, 16, 1, 4>::bytes(m, k)) <= SMEM_MOST;
 }
-template <int GS, typename O> int by_rows(const Args& a) {
-  constexpr int GM = GS == 8 ? 4 : GS;
-  const int nt = (a.m + 7) / 8;
-  int rc;
-  if (nt == 1) return few_rows<1, GS, O>(a, &rc) ? rc : more<1, 2, GM, O>(a);
-  if (nt == 2) return few_rows<2, GS, O>(a, &rc) ? rc : more<2, 2, GM, O>(a);
-  if (nt <= 4) return more<4, 2, GM, O>(a);
-  if (nt <= 6) return more<6, 2, GM, O>(a);
-  return more<8, 2, GM, O>(a);
-}
+bool takes(int m, int k, int group) { return m <= 8 ? fits<1>(m, k, group) : m <= 16 && fits<2>(m, k, group); }
+
+template <int GS, typename O> int by_rows(const Args& a) { return a.m <= 8 ? few_rows<1, GS, O>(a) : few_rows<2, GS, O>(a); }
 template <typename O> int by_group(const Args& a) {
   return (a.group == 128 ? by_rows<8, O> : a.group == 64 ? by_rows<4, O> : a.group == 32 ? by_rows<2, O> : by_rows<1, O>)(a);
 }
 }  // namespace
 
+// Whether the kernel for few rows of bfloat16 takes so many rows of so many inputs (they have to fit in shared memory).
+DRYFT_API int dryft_linear4_takes(int m, int k, int group) { return takes(m, k, group); }
+
 DRYFT_API int dryft_linear4(int is_bf16, int out_bf16, const void* x, long long x_stride, const void* codes, const void* scales, void* y, int m, int n, int k,
                             int group, int pdl, void* stream) {
   if (m <= 0 || n <= 0) return 0;
   const cudaStream_t st = (cudaStream_t)stream;
+  if (is_bf16 && !takes(m, k, group)) return DRYFT_ERR_UNSUPPORTED;
   if (is_bf16) return (out_bf16 ? by_group<bf16> : by_group<float>)({x, x_stride, codes, scales, y, m, n, k, group, pdl, st});
   linear4_f32_kernel<<<dim3((n + 15) / 16, (m + ROWS - 1) / ROWS), WARPS * 32, 0, st>>>((const float*)x, x_stride, (const uint4*)codes, (const uint2*)scales,
                                                                                        (float*)y, m, n, k, group);

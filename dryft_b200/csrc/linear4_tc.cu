@@ -1,0 +1,494 @@
+// Products with weights held in 4 bits (four_bit.cuh, linear4.cu has their layout) for up to 256 rows of bfloat16, on the 5th-generation tensor cores.
+//
+// Computed transposed: a tile is 128 rows of W against all rows of x, padded to NB = 32, 64, 128 or 256, its 128 x NB sums in tensor memory.  A unit is
+// 64 inputs of a tile: its codes (4 KB) and scales come by TMA into a ring, eight warps take them out of their 4 bits, each 16 rows of W, into a stage
+// of shared memory as the 128 x 64 operand that tcgen05.mma reads (K-major, 128-byte swizzle); x's 64 inputs come by TMA too.  (Codes requested into registers
+// instead, four units ahead: every unit waits for them at the fence in front of the products, 1 us a unit.)  So the weights cross memory at 4.5 bits
+// and are multiplied as bfloat16 z + (c - 7.5) s: one rounding of 2^-9 of each weight.  For 32-bit results (LOW) the rest of that rounding is a second
+// operand with a product of its own, which leaves 2^-18.
+//
+// Work is cut evenly: block i of G takes the units [i U / G, (i + 1) U / G) in (tile, inputs) order.  A run that covers its tile's inputs is finished from tensor
+// memory; else its sums go to a workspace, and a second launch adds a tile's pieces in the blocks' order.  No block waits for another.
+//
+// Warps: 0 copies x, 1 issues the products, 22 copies codes (a thread each), 2 to 5 read the sums, 6 to 21 take weights out.  Every wait on a barrier is bounded by a clock; a
+// waiter that gives up raises *err, every role leaves its loop, the block lets its copies and products end and frees its tensor memory.
+#include "four_bit.cuh"
+#include "drain.h"
+#include <cuda.h>
+#include <type_traits>
+
+namespace {
+typedef __nv_bfloat16 bf16;
+constexpr int BM = 128, BK = 64, W_BYTES = BM * BK * 2, WARPS = 23, TAKERS = 16;
+constexpr long long WAIT_CYCLES = 2000000000LL;
+constexpr unsigned SLEEP_NS = 10000;   // a waiter sleeps up to so long before it asks again: asking takes issue slots from those it waits for
+
+__device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(void* bar, unsigned count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(void* bar, unsigned bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(void* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(void* bar, unsigned parity) {
+  unsigned ok;
+  asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
+               : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(SLEEP_NS) : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait(void* bar, unsigned parity, int* err, volatile int* failed, int site) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*failed) return false;
+    if (clock64() - t0 > WAIT_CYCLES) {
+      if (err) atomicCAS(err, 0, 200 + site);   // the first wait that gave up names its place
+      *failed = 1;
+      return false;
+    }
+  }
+  return true;
+}
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, void* bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
+}
+// K-major operand tile, 128-byte swizzle: rows of 64 bf16 (128 bytes), 8-row groups 1024 bytes apart.
+__device__ __forceinline__ unsigned long long umma_desc(const void* smem_tile) {
+  unsigned long long d = 0;
+  d |= (unsigned long long)((smem_u32(smem_tile) & 0x3FFFF) >> 4);
+  d |= (unsigned long long)1 << 16;
+  d |= (unsigned long long)(1024 >> 4) << 32;
+  d |= (unsigned long long)1 << 46;
+  d |= (unsigned long long)2 << 61;
+  return d;
+}
+// kind::f16 instruction descriptor: D fp32, A and B bf16, both K-major, N >> 3 at bit 17, M >> 4 at bit 24
+__host__ __device__ constexpr unsigned idesc(int m, int n) { return (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24); }
+__device__ __forceinline__ void umma(unsigned d_tmem, unsigned long long a_desc, unsigned long long b_desc, unsigned id, unsigned accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(id), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_commit(void* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(unsigned taddr, float (&v)[16]) {
+  unsigned r[16];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                 "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+struct Params { void* y; float* pieces; int* err; int m, n, blocks, group_bits, tiles; };
+
+// KU: blocks of 64 inputs in a unit, two where two stages of them fit: every handshake between the roles costs the same for twice the work (48 rows, 19,456
+// outputs of 2,560 inputs: 28.6 us with units of 64 inputs).  GN: groups that begin in a unit.
+template <int NB, bool LOW> constexpr int units_of() { return 2 * 2 * (W_BYTES * (LOW ? 2 : 1) + NB * BK * 2) <= 176 * 1024 ? 2 : 1; }
+template <int NB, int GN, bool LOW> struct Layout {
+  static constexpr int KU = units_of<NB, LOW>(), W_SIDE = W_BYTES * KU;                          // a stage: weights (LOW: and their rests), then x, block by block
+  static constexpr int X_BLOCK = NB * BK * 2, X_BYTES = X_BLOCK * KU, STAGE_BYTES = W_SIDE * (LOW ? 2 : 1) + X_BYTES;   // multiples of 1024
+  static constexpr int RING = KU == 2 ? 4 : 8;                                                    // units whose codes are on their way
+  static constexpr int CODE_BYTES = 4096 * KU, SCALE_BYTES = 512 * GN, SLOT_BYTES = CODE_BYTES + SCALE_BYTES, RING_BYTES = RING * SLOT_BYTES;   // multiples of 128
+  static constexpr int ROOM = 225 * 1024 - RING_BYTES, STAGES = STAGE_BYTES * 6 <= ROOM ? 6 : ROOM / STAGE_BYTES;
+  // Teams of warps that take units' weights out in turn.  A parity tells two phases of a barrier apart, not three: a team that waits for the products of the unit that
+  // had its stage before has to know that those of the unit before that are done.  It has written its last unit, TEAMS before this one, into a stage that the products
+  // of the unit TEAMS + STAGES before this one had left; so TEAMS is at most STAGES.
+  static constexpr int TEAMS = STAGES >= 4 ? 4 : 2, TEAM = TAKERS / TEAMS;
+  static_assert(STAGES >= 2 && TEAMS <= STAGES && TEAMS <= RING, "phases of a stage's barrier");
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + RING_BYTES + 8 * (3 * STAGES + 2 * RING + 4) + 64, TMEM_COLS = 2 * NB;
+  static_assert(SMEM_BYTES <= 227 * 1024, "of a block");
+};
+// (32 bits: the launcher sees to U G being below 2^32)
+__device__ __forceinline__ unsigned first_unit(unsigned U, unsigned G, unsigned i) { return U * i / G; }
+// the block that has unit u: the last one that begins at or before it
+__device__ __forceinline__ unsigned block_of(unsigned U, unsigned G, unsigned u) { return ((u + 1) * G - 1) / U; }
+
+// 16 rows of W of one block of a unit by a warp, into the operand: rows r and r + 8, four inputs (8 bytes) of each of four steps.
+template <int GN, bool LOW, int KU> __device__ __forceinline__ void take_out(unsigned char* to, int block, int row0, uint4 raw, const uint2 (&sz)[GN]) {
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const unsigned words[4] = {raw.x, raw.y, raw.z, raw.w};
+  const __nv_bfloat162 less = __floats2bfloat162_rn(-CODE_BIAS, -CODE_BIAS);
+  // row (r or r + 8), 16-byte chunk 2s + c / 2, which the swizzle puts at chunk ^ (row & 7)
+  const unsigned place = smem_u32(to) + (row0 + r) * 128 + (((c >> 1) ^ r) << 4) + (c & 1) * 8;
+  const auto put = [](unsigned at, unsigned x, unsigned y) { asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(x), "r"(y) : "memory"); };
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int g = (4 * block + s) * GN / (4 * KU);
+      const unsigned one = h ? sz[g].y : sz[g].x;
+      const unsigned a = code_pair(words[s], h), b = code_pair(words[s], 2 + h);   // inputs 16 s + 4c, + 1 and + 2, + 3
+      const unsigned at = (place ^ (32 * s)) + 1024 * h;
+      if constexpr (!LOW) {
+        const unsigned ss = __byte_perm(one, one, 0x1010), zz = __byte_perm(one, one, 0x3232);
+        const __nv_bfloat162 s2 = *reinterpret_cast<const __nv_bfloat162*>(&ss), z2 = *reinterpret_cast<const __nv_bfloat162*>(&zz);
+        const __nv_bfloat162 x = __hfma2(__hadd2(*reinterpret_cast<const __nv_bfloat162*>(&a), less), s2, z2);
+        const __nv_bfloat162 y = __hfma2(__hadd2(*reinterpret_cast<const __nv_bfloat162*>(&b), less), s2, z2);
+        put(at, *reinterpret_cast<const unsigned*>(&x), *reinterpret_cast<const unsigned*>(&y));
+      } else {
+        const GroupCode code = unpack_code(one);
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned p = e < 2 ? a : b;
+          v[e] = fmaf(__uint_as_float(e & 1 ? p & 0xffff0000u : p << 16) - CODE_BIAS, code.s, code.z);
+        }
+        const __nv_bfloat162 x = __floats2bfloat162_rn(v[0], v[1]), y = __floats2bfloat162_rn(v[2], v[3]);
+        const __nv_bfloat162 xl = __floats2bfloat162_rn(v[0] - __low2float(x), v[1] - __high2float(x));
+        const __nv_bfloat162 yl = __floats2bfloat162_rn(v[2] - __low2float(y), v[3] - __high2float(y));
+        put(at, *reinterpret_cast<const unsigned*>(&x), *reinterpret_cast<const unsigned*>(&y));
+        put(at + W_BYTES * KU, *reinterpret_cast<const unsigned*>(&xl), *reinterpret_cast<const unsigned*>(&yl));
+      }
+    }
+}
+
+template <int NB, int GN, bool LOW>
+__global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_codes,
+                                                                   const __grid_constant__ CUtensorMap map_scales, const Params p) {
+  typedef Layout<NB, GN, LOW> L;
+  constexpr int STAGES = L::STAGES, RING = L::RING, KU = L::KU;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* const stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  unsigned char* const ring = stages + STAGES * L::STAGE_BYTES;
+  unsigned long long* const w_full = reinterpret_cast<unsigned long long*>(ring + L::RING_BYTES);                // [S] weights (8 warps) -> products
+  unsigned long long* const x_full = w_full + STAGES;                                                             // [S] TMA -> products
+  unsigned long long* const empty = x_full + STAGES;                                                              // [S] products -> both
+  unsigned long long* const acc_full = empty + STAGES;                                                            // [2] a run's sums -> their readers
+  unsigned long long* const acc_empty = acc_full + 2;                                                             // [2] read (128 arrivals) -> products
+  unsigned long long* const c_full = acc_empty + 2;                                                               // [RING] TMA -> weights
+  unsigned long long* const c_empty = c_full + RING;                                                              // [RING] taken out (8 warps) -> TMA
+  unsigned* const tmem_slot = reinterpret_cast<unsigned*>(c_empty + RING);
+  __shared__ int failed_s, issued_s, codes_issued_s;
+  __shared__ unsigned long long drained_s;
+  volatile int* const failed = &failed_s;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, KB = p.blocks / KU;
+  const int U = p.tiles * KB, u0 = first_unit(U, gridDim.x, blockIdx.x), u1 = first_unit(U, gridDim.x, blockIdx.x + 1), n_units = u1 - u0;
+
+  if (threadIdx.x == 0) {
+    failed_s = issued_s = codes_issued_s = 0;
+    mbar_init(&drained_s, 1);
+    for (int s = 0; s < RING; ++s) {
+      mbar_init(&c_full[s], 1);
+      mbar_init(&c_empty[s], L::TEAM);
+    }
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&w_full[s], L::TEAM);
+      mbar_init(&x_full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 128);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(L::TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const unsigned tmem = *tmem_slot;
+  let_next_launch_in();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      int i = 0;
+      for (; i < n_units; ++i) {
+        const int s = i % STAGES;
+        if (i >= STAGES && !mbar_wait(&empty[s], (unsigned)(((i / STAGES) - 1) & 1), p.err, failed, 1)) break;
+        mbar_expect_tx(&x_full[s], L::X_BYTES);
+        unsigned char* const to = stages + (size_t)s * L::STAGE_BYTES + (LOW ? 2 : 1) * L::W_SIDE;
+#pragma unroll
+        for (int b = 0; b < KU; ++b) tma_load_2d(to + b * L::X_BLOCK, &map_x, ((u0 + i) % KB * KU + b) * BK, 0, &x_full[s]);
+      }
+      issued_s = i;
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // (one thread's instructions are this loop's pace: stage, turn and descriptors are counted up, not worked out)
+      constexpr unsigned ID = idesc(BM, NB);
+      const unsigned long long w_desc0 = umma_desc(stages), x_desc0 = umma_desc(stages + (LOW ? 2 : 1) * L::W_SIDE);
+      bool ok = true;
+      int run = 0, s = 0, kb = u0 % KB;   // runs of one tile's units that this block has begun
+      unsigned par = 0, first = 1;
+      for (int i = 0; i < n_units; ++i) {
+        ok = mbar_wait(&w_full[s], par, p.err, failed, 2) && mbar_wait(&x_full[s], par, p.err, failed, 3);
+        if (ok && first && run >= 2) {   // the sums that this buffer held have been read
+          ok = mbar_wait(&acc_empty[run & 1], (unsigned)(((run >> 1) - 1) & 1), p.err, failed, 4);
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        }
+        if (!ok) break;
+        const unsigned long long w_desc = w_desc0 + (unsigned)(s * (L::STAGE_BYTES >> 4)), x_desc = x_desc0 + (unsigned)(s * (L::STAGE_BYTES >> 4));
+        const unsigned d = tmem + (unsigned)((run & 1) * NB);
+#pragma unroll
+        for (int b = 0; b < KU; ++b)
+#pragma unroll
+          for (int kk = 0; kk < BK / 16; ++kk) {
+            const unsigned long long w = w_desc + b * (W_BYTES >> 4) + kk * 2, x = x_desc + b * (L::X_BLOCK >> 4) + kk * 2;
+            umma(d, w, x, ID, b + kk > 0 ? 1u : first ^ 1u);
+            if (LOW) umma(d, w + (L::W_SIDE >> 4), x, ID, 1u);
+          }
+        umma_commit(&empty[s]);
+        first = 0;
+        if (++kb == KB || i == n_units - 1) {
+          umma_commit(&acc_full[run & 1]);
+          ++run;
+          kb = 0;
+          first = 1;
+        }
+        if (++s == STAGES) {
+          s = 0;
+          par ^= 1;
+        }
+      }
+    }
+  } else if (warp < 6) {
+    const int q = warp & 3, row = q * 32 + lane;   // the quarter of tensor memory that this warp may read; W row of the tile
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    int run = 0;
+    for (int u = u0; u < u1; ++run) {
+      const int tile = u / KB, b = run & 1, begin = tile * KB, end = min(u1, begin + KB);
+      const bool whole = u == begin && end == begin + KB;
+      u = end;
+      bool ok = mbar_wait(&acc_full[b], (unsigned)((run >> 1) & 1), p.err, failed, 5);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const unsigned from = tmem + ((unsigned)(q * 32) << 16) + (unsigned)(b * NB);
+      const int out = tile * BM + row;
+      // a piece: of this block, its first tile's (0) or its last one's (1); [slot][NB][128]
+      float* const piece = p.pieces + (size_t)(2 * blockIdx.x + (u0 < begin ? 1 : 0)) * BM * NB + row;
+#pragma unroll 1
+      for (int m0 = 0; m0 < NB; m0 += 16) {
+        float v[16];
+        tmem_ld16(from + m0, v);
+        if (whole) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (m0 + j < p.m && out < p.n) {
+              if (LOW) reinterpret_cast<float*>(p.y)[(size_t)(m0 + j) * p.n + out] = v[j];
+              else reinterpret_cast<bf16*>(p.y)[(size_t)(m0 + j) * p.n + out] = __float2bfloat16_rn(v[j]);
+            }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (m0 + j < p.m) __stcg(piece + (size_t)(m0 + j) * BM, v[j]);
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      mbar_arrive(&acc_empty[b]);
+    }
+  } else if (warp == 6 + TAKERS) {
+    if (lane == 0) {   // codes depend on no earlier launch
+      int i = 0;
+      for (; i < n_units; ++i) {
+        const int s = i % RING;
+        if (i >= RING && !mbar_wait(&c_empty[s], (unsigned)(((i / RING) - 1) & 1), p.err, failed, 7)) break;
+        const int tile = (u0 + i) / KB, kb = (u0 + i) % KB;
+        unsigned char* const to = ring + s * L::SLOT_BYTES;
+        mbar_expect_tx(&c_full[s], L::SLOT_BYTES);
+        tma_load_2d(to, &map_codes, kb * (128 * KU), tile * 8, &c_full[s]);
+        tma_load_2d(to + L::CODE_BYTES, &map_scales, ((kb * (64 * KU)) >> p.group_bits) * 16, tile * 8, &c_full[s]);
+      }
+      codes_issued_s = i;
+    }
+  } else {
+    // teams take the units in turn, so that one's waits and fence are another's work
+    constexpr int TEAM = L::TEAM;
+    const int w = (warp - 6) % TEAM;
+    for (int i = (warp - 6) / TEAM; i < n_units; i += L::TEAMS) {
+      const int s = i % STAGES, cs = i % RING;
+      bool ok = mbar_wait(&c_full[cs], (unsigned)((i / RING) & 1), p.err, failed, 8);
+      if (ok && i >= STAGES) ok = mbar_wait(&empty[s], (unsigned)(((i / STAGES) - 1) & 1), p.err, failed, 6);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const unsigned char* const from = ring + cs * L::SLOT_BYTES;
+#pragma unroll
+      for (int t = w; t < 8; t += TEAM) {   // 16 rows of W
+        uint2 sz[GN];
+#pragma unroll
+        for (int g = 0; g < GN; ++g) sz[g] = *reinterpret_cast<const uint2*>(from + L::CODE_BYTES + (t * GN + g) * 64 + (lane >> 2) * 8);
+#pragma unroll
+        for (int b = 0; b < KU; ++b) {
+          const uint4 raw = *reinterpret_cast<const uint4*>(from + (t * KU + b) * 512 + lane * 16);
+          take_out<GN, LOW, KU>(stages + (size_t)s * L::STAGE_BYTES + b * W_BYTES, b, 16 * t, raw, sz);
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the tensor core reads through the async proxy
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&w_full[s]);
+        mbar_arrive(&c_empty[cs]);
+      }
+    }
+  }
+
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (*failed) {
+    // a wait ran out: give copies and products that may still be in flight a bounded time to end
+    const long long t0 = clock64();
+    auto expired = [&] { return clock64() - t0 > WAIT_CYCLES; };
+    if (threadIdx.x == 0) ring_drain(issued_s, STAGES, [&](int s, unsigned parity) { return mbar_try_wait(&x_full[s], parity); }, expired);
+    if (threadIdx.x == (6 + TAKERS) * 32) ring_drain(codes_issued_s, RING, [&](int s, unsigned parity) { return mbar_try_wait(&c_full[s], parity); }, expired);
+    if (threadIdx.x == 32) {   // the thread that issued the products
+      umma_commit(&drained_s);
+      while (!mbar_try_wait(&drained_s, 0) && !expired()) {}
+    }
+    __syncthreads();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::TMEM_COLS) : "memory");
+  }
+}
+
+// Tiles that several blocks had pieces of: a block per tile and two rows of x, a thread per W row; the pieces in the blocks' order.
+constexpr int JOIN_ROWS = 2;
+template <int NB, typename O>
+__global__ void __launch_bounds__(128) linear4_pieces_kernel(const float* pieces, O* y, int m, int n, unsigned blocks, unsigned tiles, unsigned G) {   // blocks: units of a tile
+  const unsigned U = tiles * blocks, begin = blockIdx.x * blocks, first = block_of(U, G, begin), last = block_of(U, G, begin + blocks - 1);
+  if (first == last) return;
+  const int out = blockIdx.x * BM + threadIdx.x, m0 = blockIdx.y * JOIN_ROWS;
+  constexpr size_t SLOT = (size_t)BM * NB;
+  // the first block's last piece if its units began in the tile before; every other block begins with this tile
+  const float* const from = pieces + (size_t)m0 * BM + threadIdx.x;
+  const float* const head = from + (2 * first + (first_unit(U, G, first) < begin ? 1 : 0)) * SLOT;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  float v[JOIN_ROWS];
+#pragma unroll
+  for (int j = 0; j < JOIN_ROWS; ++j) v[j] = m0 + j < m ? __ldcg(head + j * BM) : 0.f;
+#pragma unroll 8
+  for (unsigned i = first + 1; i <= last; ++i)
+#pragma unroll
+    for (int j = 0; j < JOIN_ROWS; ++j)
+      if (m0 + j < m) v[j] += __ldcg(from + 2 * i * SLOT + j * BM);
+  if (out < n)
+#pragma unroll
+    for (int j = 0; j < JOIN_ROWS; ++j)
+      if (m0 + j < m) y[(size_t)(m0 + j) * n + out] = from_f32<O>(v[j]);
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  if (!fn) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess) fn = (EncodeTiledFn)p;
+  }
+  return fn;
+}
+
+int sm_count() {
+  static int sms = 0;
+  if (sms == 0) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) sms = 148;
+  }
+  return sms;
+}
+
+template <typename... P, typename... A> int launch(void (*kern)(P...), dim3 grid, int threads, size_t bytes, bool dependent, cudaStream_t st, A... a) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, (P)a...);
+  return e != cudaSuccess ? (int)e : launch_status();
+}
+
+struct Operands { EncodeTiledFn enc; const void *x, *codes, *scales; long long x_stride; int k, group; };
+// rows of `wide` elements, `step` bytes apart, in boxes of box_wide x box_rows; zeros out of range
+bool encode(EncodeTiledFn enc, CUtensorMap* map, CUtensorMapDataType type, const void* base, long long wide, long long rows, long long step, int box_wide, int box_rows,
+            CUtensorMapSwizzle swizzle) {
+  const cuuint64_t dims[2] = {(cuuint64_t)wide, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)step};
+  const cuuint32_t box[2] = {(cuuint32_t)box_wide, (cuuint32_t)box_rows}, ones[2] = {1, 1};
+  return enc(map, type, 2, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+int padded_rows(int m) { return m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256; }
+int blocks_of(int k) { return (k + 127) / 128 * 2; }
+// the launch's blocks: one a multiprocessor, if there are as many units
+int grid_of(int n, int units) {
+  const long long all = (long long)((n + BM - 1) / BM) * units;
+  return (int)(all < sm_count() ? all : sm_count());
+}
+
+template <int NB, int GN, bool LOW> int run(const Operands& o, const Params& p, int pdl, cudaStream_t st) {
+  typedef Layout<NB, GN, LOW> L;
+  constexpr int KU = L::KU;
+  const int units = p.blocks / KU, G = grid_of(p.n, units), tiles16 = (p.n + 15) / 16, groups = p.blocks * 64 / o.group;
+  if ((long long)p.tiles * units * (G + 1) >= 1ll << 31) return DRYFT_ERR_UNSUPPORTED;
+  CUtensorMap x, codes, scales;
+  if (!encode(o.enc, &x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, o.x, o.k, p.m, o.x_stride * 2, BK, NB, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !encode(o.enc, &codes, CU_TENSOR_MAP_DATA_TYPE_UINT32, o.codes, (long long)p.blocks * 128, tiles16, (long long)p.blocks * 512, 128 * KU, 8, CU_TENSOR_MAP_SWIZZLE_NONE) ||
+      !encode(o.enc, &scales, CU_TENSOR_MAP_DATA_TYPE_UINT32, o.scales, (long long)groups * 16, tiles16, (long long)groups * 64, 16 * GN, 8, CU_TENSOR_MAP_SWIZZLE_NONE))
+    return DRYFT_ERR_UNSUPPORTED;
+  auto kern = linear4_tc_kernel<NB, GN, LOW>;
+  static bool asked[64] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return DRYFT_ERR_UNSUPPORTED;
+  if (!asked[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM_BYTES);
+    if (e != cudaSuccess) return (int)e;
+    asked[dev] = true;
+  }
+  const int rc = launch(kern, dim3(G), WARPS * 32, L::SMEM_BYTES, pdl != 0, st, x, codes, scales, p);
+  if (rc || G == p.tiles) return rc;   // (a tile a block: no pieces)
+  typedef typename std::conditional<LOW, float, bf16>::type O;
+  return launch(linear4_pieces_kernel<NB, O>, dim3(p.tiles, (p.m + JOIN_ROWS - 1) / JOIN_ROWS), 128, 0, true, st, (const float*)p.pieces, (O*)p.y, p.m, p.n,
+                units, p.tiles, G);
+}
+template <int NB, bool LOW> int by_group(const Operands& o, const Params& p, int pdl, cudaStream_t st) {
+  constexpr int WIDE = 64 * units_of<NB, LOW>();   // inputs of a unit
+  switch (o.group) {
+    case 128: return run<NB, 1, LOW>(o, p, pdl, st);
+    case 64: return run<NB, WIDE / 64, LOW>(o, p, pdl, st);
+    case 32: return run<NB, WIDE / 32, LOW>(o, p, pdl, st);
+    case 16: return run<NB, WIDE / 16, LOW>(o, p, pdl, st);
+  }
+  return DRYFT_ERR_UNSUPPORTED;
+}
+}  // namespace
+
+// Floats of the workspace that a launch needs.
+DRYFT_API long long dryft_linear4_tc_pieces(int m, int n, int k) { return 2ll * grid_of(n, blocks_of(k)) * BM * padded_rows(m); }
+
+// y [m, n] = x [m, k] w^T, m <= 256; x bfloat16, rows x_stride numbers apart on 16-byte boundaries; y bfloat16 or (out_f32) float32.
+DRYFT_API int dryft_linear4_tc(int out_f32, const void* x, long long x_stride, const void* codes, const void* scales, void* y, float* pieces, int m, int n, int k,
+                               int group, int pdl, int* err, void* stream) {
+  if (m <= 0 || n <= 0) return 0;
+  if (m > 256 || k <= 0 || k % 16) return DRYFT_ERR_UNSUPPORTED;
+  const Operands o = {encode_fn(), x, codes, scales, x_stride, k, group};
+  if (!o.enc) return DRYFT_ERR_UNSUPPORTED;
+  const Params p = {y, pieces, err, m, n, blocks_of(k), __builtin_ctz(group), (n + BM - 1) / BM};
+  const cudaStream_t st = (cudaStream_t)stream;
+#define DRYFT_TC(NB) (out_f32 ? by_group<NB, true>(o, p, pdl, st) : by_group<NB, false>(o, p, pdl, st))
+  switch (padded_rows(m)) {
+    case 32: return DRYFT_TC(32);
+    case 64: return DRYFT_TC(64);
+    case 128: return DRYFT_TC(128);
+    default: return DRYFT_TC(256);
+  }
+#undef DRYFT_TC
+}

@@ -2451,7 +2451,7 @@ def wkv_decode(r, k, v, g, low, w2, w0, u, norm_w, eps: float, h, last, tok_slot
 # A group of 16, 32, 64 or 128 consecutive numbers shares a scale s and a middle z, both bfloat16; code c (0..15) stands for
 # z + (c - 7.5) s.  csrc/four_bit.cuh has the arithmetic and the layouts.
 BITS4_GROUPS = (16, 32, 64, 128)
-LINEAR4_ROWS = 64      # rows of x that ``linear4`` takes
+LINEAR4_ROWS, LINEAR4_ROWS_F32 = 256, 64      # rows of x that ``linear4`` takes
 
 
 def bits4_group(size: int, most: int = 64) -> int:
@@ -2473,6 +2473,7 @@ def linear4_lib() -> ctypes.CDLL:
     """Products with weights held in 4 bits."""
     return _single_lib("linear4", {
         "dryft_linear4": [_i, _i, _p, _ll, _p, _p, _p, _i, _i, _i, _i, _i, _p],
+        "dryft_linear4_takes": [_i, _i, _i],
         "dryft_weight4_expand": [_i, _p, _p, _p, _i, _i, _i, _p],
     })
 
@@ -2591,26 +2592,52 @@ def _rows_in(x, name: str, width: int) -> int:
     return step
 
 
-_linear4_fn = None
+def linear4_tc_lib() -> ctypes.CDLL:
+    """Products of up to 256 rows with weights held in 4 bits (tcgen05, tensor memory, TMA)."""
+    lib = _single_lib("linear4_tc", {"dryft_linear4_tc": [_i, _p, _ll, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p]})
+    lib.dryft_linear4_tc_pieces.argtypes = [_i, _i, _i]
+    lib.dryft_linear4_tc_pieces.restype = _ll
+    return lib
+
+
+_linear4_fn = _linear4_tc_fn = None
+
+
+@functools.lru_cache(maxsize=4096)
+def linear4_plan(m: int, n: int, k: int, group: int, bf16: bool) -> int:
+    """Which kernel a product runs on: 0 for the one for few rows (up to 16, as long as x fits in its shared memory; float32: up to 64), else the floats of
+    workspace that the tensor memory kernel needs.  16 rows, 2,560 outputs of 9,728 inputs, which do not fit: 14.4 us on the latter; 19,456 of 2,560, which
+    do: 14.8 us on the former and 20.4 on the latter."""
+    if not bf16 or linear4_lib().dryft_linear4_takes(m, k, group):
+        return 0
+    return int(linear4_tc_lib().dryft_linear4_tc_pieces(m, n, k))
 
 
 def linear4(x, w: Weight4, out, pdl: bool = False) -> None:
-    """``out = x @ w.T`` for up to 64 rows; ``x`` float32 or bfloat16, ``out`` of the same type or float32.  ``pdl``: a programmatic dependent (its
+    """``out = x @ w.T``; ``x`` bfloat16, up to 256 rows (float32: 64), ``out`` of the same type or float32.  ``pdl``: a programmatic dependent (its
     first weights are requested while the launch before it drains)."""
-    global _linear4_fn, launch_count
+    global _linear4_fn, _linear4_tc_fn, launch_count
     _need_weight4(w)
     step = _rows_in(x, "x", w.k)
     m = x.shape[0]
-    if m > LINEAR4_ROWS:
-        raise KernelError(f"linear4 takes up to {LINEAR4_ROWS} rows, got {m}")
     is_bf16 = _act(x, "x")
+    if m > (LINEAR4_ROWS if is_bf16 else LINEAR4_ROWS_F32):
+        raise KernelError(f"linear4 takes up to {LINEAR4_ROWS} rows ({LINEAR4_ROWS_F32} of float32), got {m}")
     out_bf16 = _act(out, "out")
     if out_bf16 and not is_bf16:
         raise KernelError("linear4: 32-bit activations give 32-bit results")
     _need(out, "out", None, (m, w.n))
-    if _linear4_fn is None:
-        _linear4_fn = linear4_lib().dryft_linear4
-    rc = _linear4_fn(is_bf16, out_bf16, x.data_ptr(), step, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), m, w.n, w.k, w.group, pdl, _stream())
+    floats = linear4_plan(m, w.n, w.k, w.group, bool(is_bf16))
+    if floats:
+        if _linear4_tc_fn is None:
+            _linear4_tc_fn = linear4_tc_lib().dryft_linear4_tc
+        pieces = torch.empty(floats, dtype=torch.float32, device=x.device)
+        rc = _linear4_tc_fn(not out_bf16, x.data_ptr(), step, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), pieces.data_ptr(), m, w.n, w.k, w.group,
+                            pdl, error_flag(x.device).data_ptr(), _stream())
+    else:
+        if _linear4_fn is None:
+            _linear4_fn = linear4_lib().dryft_linear4
+        rc = _linear4_fn(is_bf16, out_bf16, x.data_ptr(), step, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), m, w.n, w.k, w.group, pdl, _stream())
     if rc:
         _ok(rc, "linear4")
     launch_count += 1

@@ -37,18 +37,35 @@ def test_expanded_weights_are_the_codes_values(n, k, group, dtype):
     assert torch.equal(out.cpu(), values.to(F32).to(dtype))       # one 32-bit rounding of z + (c - 7.5) s, then the type's
 
 
-@pytest.mark.parametrize("m", [1, 2, 7, 8, 9, 16, 17, 31, 40, 64])
+@pytest.mark.parametrize("m,dtype,out", [(m, *types) for types in ((BF, BF), (BF, F32), (F32, F32)) for m in ((1, 2, 7, 8, 9, 16) if types[0] == BF else (1, 2, 8, 9, 31, 64))])
 @pytest.mark.parametrize("n,k,group", [(1, 16, 16), (389, 80, 16), (17, 64, 64), (250, 1280, 64), (100, 96, 32), (160, 2560, 128), (48, 9728, 64), (5000, 128, 128)])
-@pytest.mark.parametrize("dtype,out", [(BF, BF), (BF, F32), (F32, F32)])
-def test_products_with_four_bit_weights(m, n, k, group, dtype, out):
+def test_products_with_four_bit_weights(n, k, group, m, dtype, out):
     w, x = _weights(n, k, dtype), torch.randn(m, k).to(dtype)
     values, s, _ = P.group_values(w, group)
     y = torch.full((m, n), float("nan"), dtype=out, device=DEV)
     K().linear4(x.to(DEV), K().pack_weight4(w.to(DEV), group), y)
-    _near(y, P.linear(x, values), P.linear_slack(x, values, s, group, out))
+    slack = P.linear_slack(x, values, s, group, out)
+    if K().linear4_plan(m, n, k, group, dtype == BF):    # x does not fit beside the kernel's rings: weights are taken out tile by tile, as below
+        slack = slack + (2.0**-8 if out == BF else 2.0**-17) * (x.double().abs() @ values.abs().T)
+    _near(y, P.linear(x, values), slack)
 
 
-@pytest.mark.parametrize("m", [65, 200])
+@pytest.mark.parametrize("m", [17, 32, 33, 64, 65, 128, 129, 200, 256])
+@pytest.mark.parametrize("n,k,group", [(1, 16, 16), (389, 80, 16), (17, 64, 64), (250, 1280, 64), (100, 96, 32), (160, 2560, 128), (128, 9728, 64), (20000, 128, 128)])
+@pytest.mark.parametrize("out", [BF, F32])
+def test_products_on_weights_taken_out_tile_by_tile(m, n, k, group, out):
+    """Tiles that one block finishes, that several share, and that outnumber the blocks.  Weights are multiplied as bfloat16 numbers, one (2^-9 of each) or, for
+    32-bit results, two (2^-18), doubled."""
+    w, x = _weights(n, k, BF), torch.randn(m, k).to(BF)
+    values, s, _ = P.group_values(w, group)
+    w4, y = K().pack_weight4(w.to(DEV), group), torch.full((m, n), float("nan"), dtype=out, device=DEV)
+    for _ in range(2):
+        K().linear4(x.to(DEV), w4, y, pdl=True)
+    K().check_error_flags()
+    _near(y, P.linear(x, values), P.linear_slack(x, values, s, group, out) + (2.0**-8 if out == BF else 2.0**-17) * (x.double().abs() @ values.abs().T))
+
+
+@pytest.mark.parametrize("m", [257, 300])
 @pytest.mark.parametrize("dtype,out", [(BF, BF), (BF, F32), (F32, F32)])
 def test_products_of_many_rows(m, dtype, out, monkeypatch):
     """More rows than the kernel takes: weights out of their 4 bits, in parts (here of 64 rows of W)."""

@@ -20,7 +20,8 @@ def _group(size):
 
 
 class Plain(P.PlainQwen3):
-    """The plain model with its matrices replaced by what their 4-bit form stands for.  ``logits(ids, held)``: attention reads the keys and values ``held``
+    """The plain model with its matrices replaced by what their 4-bit form stands for, in the model's own precision: its bfloat16 evaluation has bfloat16
+    weights (as the products of many rows have; those of few rows do not round them).  ``logits(ids, held)``: attention reads the keys and values ``held``
     (one pair of [tokens, kv heads, d] a layer) instead of the layer's own, which ``made`` has afterwards."""
 
     def __init__(self, cfg, tensors, dtype, weights):
@@ -32,7 +33,7 @@ class Plain(P.PlainQwen3):
         if weights:
             for name, t in self.t.items():
                 if t.dim() == 2 and "embed" not in name:
-                    self.t[name] = F.group_values(t, _group(t.shape[1]))[0].to(F32)
+                    self.t[name] = F.group_values(t, _group(t.shape[1]))[0].to(F32).to(dtype)
 
     def logits(self, ids, held=None):
         kept, self.made = P.causal_attention, []
