@@ -7,43 +7,54 @@
 #include "four_bit.cuh"
 
 namespace {
-constexpr int WARPS = 4, ROWS = 8;
+constexpr int WARPS = 8;
 __host__ __device__ constexpr int blocks_of(int k) { return (k + 127) / 128 * 2; }                              // of 64 inputs, as laid out
 __host__ __device__ constexpr int groups_of(int k, int group) { return (k + 127) / 128 * 128 / group; }
 
-// 32-bit: a block per 16 rows of W and ROWS rows of x, the inputs dealt out to the warps in blocks of 64.
-__global__ void __launch_bounds__(WARPS * 32) linear4_f32_kernel(const float* x, long long x_stride, const uint4* __restrict__ codes,
-                                                                 const uint2* __restrict__ scales, float* y, int m, int n, int k, int group) {
+// 32-bit: a block per 16 rows of W and ROWS rows of x, the inputs dealt out to the warps in blocks of 64.  A lane has four inputs of rows r and r + 8 of W at a time: four
+// numbers of each row of x (the eight lanes of a quarter read the same ones), 8 ROWS multiply-adds.  The sums of a row do not depend on how many there are.
+template <int ROWS>
+__global__ void __launch_bounds__(WARPS * 32, 2) linear4_f32_kernel(const float* x, long long x_stride, const uint4* __restrict__ codes,
+                                                                 const uint2* __restrict__ scales, float* y, int m, int n, int k, int group_bits) {
   __shared__ float part[WARPS][2][ROWS][8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
-  const int tile = blockIdx.x, m0 = blockIdx.y * ROWS, rows = min(ROWS, m - m0), blocks = blocks_of(k), groups = groups_of(k, group);
+  const int tile = blockIdx.x, m0 = blockIdx.y * ROWS, rows = min(ROWS, m - m0), blocks = blocks_of(k), groups = groups_of(k, 1 << group_bits);
+  const float* const x0 = x + m0 * x_stride + 4 * c;
   float acc[2][ROWS];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) acc[0][i] = acc[1][i] = 0.f;
-  for (int b = warp; b < blocks; b += WARPS) {
+  for (int b = warp; b * 64 < k; b += WARPS) {
     const uint4 raw = codes[((size_t)tile * blocks + b) * 32 + lane];
     const unsigned words[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const int at = 64 * b + 16 * s;
       if (at >= k) break;
-      const uint2 sz = scales[((size_t)tile * groups + at / group) * 8 + r];
+      float4 xv[ROWS];
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i)
+        if (i < rows) xv[i] = *reinterpret_cast<const float4*>(x0 + i * x_stride + at);
+      const uint2 sz = scales[((size_t)tile * groups + (at >> group_bits)) * 8 + r];
       const GroupCode g[2] = {unpack_code(sz.x), unpack_code(sz.y)};
       float w[2][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) w[h][e] = value_of(words[s] >> (4 * (2 * (e >> 1) + h) + 16 * (e & 1)) & 15u, g[h]);
-#pragma unroll
-      for (int i = 0; i < ROWS; ++i) {
-        if (i >= rows) break;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float xv = x[(m0 + i) * x_stride + at + 4 * c + e];
-          acc[0][i] = fmaf(w[0][e], xv, acc[0][i]);
-          acc[1][i] = fmaf(w[1][e], xv, acc[1][i]);
+        for (int e = 0; e < 4; e += 2) {
+          const unsigned pair = code_pair(words[s], e + h);
+          w[h][e] = fmaf(__uint_as_float(pair << 16) - CODE_BIAS, g[h].s, g[h].z);
+          w[h][e + 1] = fmaf(__uint_as_float(pair & 0xffff0000u) - CODE_BIAS, g[h].s, g[h].z);
         }
-      }
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i)
+        if (i < rows)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            acc[h][i] = fmaf(w[h][0], xv[i].x, acc[h][i]);
+            acc[h][i] = fmaf(w[h][1], xv[i].y, acc[h][i]);
+            acc[h][i] = fmaf(w[h][2], xv[i].z, acc[h][i]);
+            acc[h][i] = fmaf(w[h][3], xv[i].w, acc[h][i]);
+          }
     }
   }
 #pragma unroll
@@ -355,8 +366,10 @@ DRYFT_API int dryft_linear4(int is_bf16, int out_bf16, const void* x, long long 
   const cudaStream_t st = (cudaStream_t)stream;
   if (is_bf16 && !takes(m, k, group)) return DRYFT_ERR_UNSUPPORTED;
   if (is_bf16) return (out_bf16 ? by_group<bf16> : by_group<float>)({x, x_stride, codes, scales, y, m, n, k, group, pdl, st});
-  linear4_f32_kernel<<<dim3((n + 15) / 16, (m + ROWS - 1) / ROWS), WARPS * 32, 0, st>>>((const float*)x, x_stride, (const uint4*)codes, (const uint2*)scales,
-                                                                                       (float*)y, m, n, k, group);
+  const int rows = m == 1 ? 1 : m <= 4 ? 4 : m <= 8 ? 8 : 16;
+  auto kern = rows == 1 ? linear4_f32_kernel<1> : rows == 4 ? linear4_f32_kernel<4> : rows == 8 ? linear4_f32_kernel<8> : linear4_f32_kernel<16>;
+  kern<<<dim3((n + 15) / 16, (m + rows - 1) / rows), WARPS * 32, 0, st>>>((const float*)x, x_stride, (const uint4*)codes, (const uint2*)scales, (float*)y, m, n, k,
+                                                                         __builtin_ctz(group));
   return launch_status();
 }
 

@@ -221,7 +221,8 @@ class Attention:
                                  self.n_kv, self.head_dim, self.position.rotary_dim, self.qk_eps, write_kv=False, cs_table=table)
         if ctx.decode:
             o = torch.empty((n, self.q_dim), dtype=qkv.dtype, device=dev)
-            K.attn4_rows(q, cache.k, cache.v, cache.page_table, ctx.tok_slot, ctx.tok_pos, o, self.scale, self.window, self.bits_group, ctx.max_kv)
+            K.attn4_rows(q, cache.k, cache.v, cache.page_table, ctx.tok_slot, ctx.tok_pos, o, self.scale, self.window, self.bits_group, ctx.max_kv,
+                         pdl=self.rt.pdl)
             return o
         k, v = cache.scratch
         K.kv4_expand(cache.k, cache.v, cache.page_table, ctx.cu_q, ctx.seq_slot[:ctx.n_seqs], ctx.tok_pos, k, v, self.bits_group, ctx.max_kv, self.window)
