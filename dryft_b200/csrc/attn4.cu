@@ -643,12 +643,14 @@ int rows_f32(const Args& a) {
 }
 
 template <int WARPS> int rows_bf16(const Args& a) {
-  static bool asked = false;
-  if (!asked) {   // (asking twice does no harm)
+  static bool asked[64] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return DRYFT_ERR_UNSUPPORTED;
+  if (!asked[dev]) {   // (asking twice does no harm)
     cudaError_t e = cudaFuncSetAttribute(attn4_mma_kernel<WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Block<WARPS>::SMEM);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(attn4_mma_kernel<WARPS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return (int)e;
-    asked = true;
+    asked[dev] = true;
   }
   const int cluster = a.splits > 1 && a.part_o == nullptr;
   if (cluster && a.splits > MOST_SPLITS) return DRYFT_ERR_UNSUPPORTED;

@@ -337,6 +337,8 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_rope_store_kernel(const T* qkv
   __shared__ __align__(16) T rows[WARPS][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = blockIdx.y * WARPS + warp, half = rot >> 1;
   const long long n = blockIdx.x;
+  if (gridDim.x <= SIGNAL_ROWS) let_next_launch_in();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (head >= n_heads + 2 * n_kv) return;
   const int slot = tok_slot[n], pos = tok_pos[n];
   const T* src = qkv + n * stride + (size_t)head * d;
@@ -504,20 +506,28 @@ int expand(const void* k_pages, const void* v_pages, const int* page_table, int 
 template <typename T>
 int rope_store(const void* qkv, int stride, const float* wq, const float* wk, const float* inv_freq, const void* cs_table, const int* tok_slot, const int* tok_pos,
                void* q_out, void* k_pages, void* v_pages, const int* page_table, int max_pages, int n, int n_heads, int n_kv, int d, int rot, int group, int page,
-               float eps, int has_norm, cudaStream_t st) {
-  kv4_rope_store_kernel<T><<<dim3(n, (n_heads + 2 * n_kv + WARPS - 1) / WARPS), WARPS * 32, 0, st>>>(
-      (const T*)qkv, stride, wq, wk, inv_freq, (const T*)cs_table, tok_slot, tok_pos, (T*)q_out, (unsigned char*)k_pages, (unsigned char*)v_pages, page_table,
-      max_pages, n_heads, n_kv, d, rot, group, page, eps, has_norm);
-  return launch_status();
+               float eps, int has_norm, int pdl, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(n, (n_heads + 2 * n_kv + WARPS - 1) / WARPS);
+  cfg.blockDim = dim3(WARPS * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_rope_store_kernel<T>, (const T*)qkv, stride, wq, wk, inv_freq, (const T*)cs_table, tok_slot, tok_pos, (T*)q_out,
+                                           (unsigned char*)k_pages, (unsigned char*)v_pages, page_table, max_pages, n_heads, n_kv, d, rot, group, page, eps, has_norm);
+  return e != cudaSuccess ? (int)e : launch_status();
 }
 }  // namespace
 
 DRYFT_API int dryft_kv4_rope_store(int is_bf16, const void* qkv, int stride, const float* wq, const float* wk, const float* inv_freq, const void* cs_table,
                                    const int* tok_slot, const int* tok_pos, void* q_out, void* k_pages, void* v_pages, const int* page_table, int max_pages, int n,
-                                   int n_heads, int n_kv, int d, int rot, int group, int page, float eps, int has_norm, void* stream) {
+                                   int n_heads, int n_kv, int d, int rot, int group, int page, float eps, int has_norm, int pdl, void* stream) {
   if (n <= 0) return 0;
   return (is_bf16 ? rope_store<__nv_bfloat16> : rope_store<float>)(qkv, stride, wq, wk, inv_freq, cs_table, tok_slot, tok_pos, q_out, k_pages, v_pages, page_table,
-                                                                  max_pages, n, n_heads, n_kv, d, rot, group, page, eps, has_norm, (cudaStream_t)stream);
+                                                                  max_pages, n, n_heads, n_kv, d, rot, group, page, eps, has_norm, pdl, (cudaStream_t)stream);
 }
 
 DRYFT_API int dryft_kv4_store(int is_bf16, const void* k, const void* v, long long stride, const int* tok_slot, const int* tok_pos, void* k_pages, void* v_pages,

@@ -145,9 +145,16 @@ template <int NT, int GS, int TEAM, int PB, int SLOTS> struct Few {
   static size_t bytes(int m, int k) { return RED_BYTES + RING_BYTES + (size_t)slots_of(k) * SCALES * NT * 64 + (size_t)m * row_bytes(k); }
 };
 
-template <int NT, int GS, int TEAM, int PB, int SLOTS, typename O>
+// What stands around the product in a decoder's layer is done on its way (rounding points as in gemm_decode.cu):
+//   norm_w: x is RMS-normed first, every block for itself: T(T(x rsqrt(mean x^2 + eps)) w);
+//   RESIDUAL: y += the result, in place;  SILU: W holds N / 2 gate rows, then as many rows to multiply with; a team takes a tile of either in turn, y = T(silu(gate)) up.
+enum Mode { STORE_BF16 = 0, STORE_F32 = 1, RESIDUAL = 2, SILU = 3 };
+__device__ __forceinline__ float bfr(float v) { return rnd<bf16>(v); }
+
+template <int NT, int GS, int TEAM, int PB, int SLOTS>
 __global__ void __launch_bounds__(FEW_WARPS * 32, 1) linear4_few_kernel(const bf16* x, long long x_stride, const uint4* __restrict__ codes,
-                                                                        const uint2* __restrict__ scales, O* y, int m, int n, int k, int group_bits) {
+                                                                        const uint2* __restrict__ scales, void* y, int m, int n, int k, int group_bits, int mode,
+                                                                        const float* __restrict__ norm_w, float eps) {
   typedef Few<NT, GS, TEAM, PB, SLOTS> F;
   constexpr int SCALES = F::SCALES, SLOT = F::SLOT, TEAMS = FEW_WARPS / TEAM, STEPS = PB * 4 / SCALES;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -159,14 +166,17 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) linear4_few_kernel(const bf
   unsigned char* const rows = rings + F::RING_BYTES;
   const int per = (slots + TEAM - 1) / TEAM, s0 = min(slots, warp % TEAM * per), ns = min(slots, s0 + per) - s0;
   // the team's tiles: block and team together count through them, the block's number first
-  const int first = blockIdx.x + team * gridDim.x, step = gridDim.x * TEAMS, mine = first < tiles ? (tiles - 1 - first) / step + 1 : 0;
+  const int half = mode == SILU ? tiles / 2 : 0, turns = mode == SILU ? half : tiles;   // a turn: a tile, or a gate tile and the one `half` tiles behind it
+  const int first = blockIdx.x + team * gridDim.x, step = gridDim.x * TEAMS, mine = (first < turns ? (turns - 1 - first) / step + 1 : 0) * (mode == SILU ? 2 : 1);
   const int total = mine * ns;   // the warp's slots
 
   // Slot i of the warp goes into place i mod SLOTS of its ring.  Codes and scales lie slot behind slot, tile behind tile.  (A group of 128 has two slots of one
   // block: the scale is then the same for both.)
   int sent = 0, until = ns;
   unsigned at = first * slots + s0;
-  const unsigned jump = step * slots - ns, ring = (unsigned)__cvta_generic_to_shared(rings + warp * F::RING_BYTES / FEW_WARPS) + lane * 16;
+  unsigned jump = mode == SILU ? half * slots - ns : step * slots - ns;   // from a tile's last slot to the next tile's first one
+  const unsigned jumps = step * slots - 2 * ns;                           // SILU: of the two jumps of a turn
+  const unsigned ring = (unsigned)__cvta_generic_to_shared(rings + warp * F::RING_BYTES / FEW_WARPS) + lane * 16;
   const unsigned ring_scales = ring - lane * 8 + PB * 512;
   const uint4* const my_codes = codes + lane;
   const uint2* const my_scales = scales + r;
@@ -184,6 +194,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) linear4_few_kernel(const bf
       if (--until == 0) {
         until = ns;
         at += jump;
+        if (mode == SILU) jump = jumps - jump;
       }
     }
     ++sent;
@@ -205,6 +216,44 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) linear4_few_kernel(const bf
   copies_end();
   copies_wait<0>();
   __syncthreads();
+  if (norm_w != nullptr) {   // the warps share the rows, or a row
+    const int wr = m == 1 ? 16 : m == 2 ? 8 : m <= 4 ? 4 : m <= 8 ? 2 : 1, row = warp / wr, part = warp % wr;
+    unsigned char* const at_x = rows + (size_t)row * row_bytes;
+    float ss = 0.f;
+    if (row < m)
+      for (int i = part * 32 + lane; 8 * i < k; i += wr * 32) {
+        const uint4 v = *reinterpret_cast<const uint4*>(at_x + i * 16);
+        const unsigned e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 p = two_of(e[j]);
+          ss = fmaf(p.x, p.x, fmaf(p.y, p.y, ss));
+        }
+      }
+    ss = warp_sum(ss);
+    if (lane == 0) red[warp] = ss;
+    __syncthreads();
+    if (row < m) {
+      ss = 0.f;
+      for (int i = 0; i < wr; ++i) ss += red[row * wr + i];
+      const float inv = rsqrtf(ss / (float)k + eps);
+      for (int i = part * 32 + lane; 8 * i < k; i += wr * 32) {
+        uint4* const cell = reinterpret_cast<uint4*>(at_x + i * 16);
+        const uint4 v = *cell;
+        unsigned e[4] = {v.x, v.y, v.z, v.w};
+        const float4 w0 = reinterpret_cast<const float4*>(norm_w)[2 * i], w1 = reinterpret_cast<const float4*>(norm_w)[2 * i + 1];
+        const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 p = two_of(e[j]);
+          const __nv_bfloat162 q = __floats2bfloat162_rn(bfr(p.x * inv) * w[2 * j], bfr(p.y * inv) * w[2 * j + 1]);
+          e[j] = *reinterpret_cast<const unsigned*>(&q);
+        }
+        *cell = make_uint4(e[0], e[1], e[2], e[3]);
+      }
+    }
+    __syncthreads();
+  }
   const unsigned char* at_row[NT];   // the lane's share of the first step of its column; columns behind the last one repeat it
 #pragma unroll
   for (int j = 0; j < NT; ++j) at_row[j] = rows + (size_t)min(8 * j + r, m - 1) * row_bytes + 8 * c;
@@ -229,6 +278,8 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) linear4_few_kernel(const bf
 #pragma unroll
   for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
   int tile = 0;
+  constexpr int OUTS = (NT * 128 + TEAM * 32 - 1) / (TEAM * 32);   // results of a thread
+  float gate[OUTS];
   // A team's sums of a tile, in the warps' order; with two buffers the last tile's are read while this one's are written.
   const int out_row = threadIdx.x & 15, out_col = threadIdx.x % (TEAM * 32) >> 4;   // lane (row & 7) * 4 + (col & 7) / 2, element 2 (row >= 8) + (col & 1)
   const float* const out_from = red + team * TEAM * NT * 128 + (out_row & 7) * 16 + ((out_col & 7) >> 1) * 4 + 2 * (out_row >> 3) + (out_col & 1);
@@ -242,16 +293,28 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) linear4_few_kernel(const bf
       acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
     }
     asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(TEAM * 32) : "memory");
-    const int row = (first + tile * step) * 16 + out_row;
+    const int turn = mode == SILU ? tile >> 1 : tile, row = (first + turn * step) * 16 + out_row;
 #pragma unroll
-    for (int i = 0; i < (NT * 128 + TEAM * 32 - 1) / (TEAM * 32); ++i) {
+    for (int i = 0; i < OUTS; ++i) {
       const int col = out_col + i * (TEAM * 2);
       if (col >= NT * 8) continue;
       const float* const place = out_from + buffer + (col >> 3) * 128;
       float v = 0.f;
 #pragma unroll
       for (int w = 0; w < TEAM; ++w) v += place[w * NT * 128];
-      if (row < n && col < m) y[(size_t)col * n + row] = from_f32<O>(v);
+      if (row >= n || col >= m) continue;
+      bf16* const to = reinterpret_cast<bf16*>(y) + (size_t)col * n + row;
+      if (mode == STORE_BF16) {
+        *to = __float2bfloat16_rn(v);
+      } else if (mode == STORE_F32) {
+        reinterpret_cast<float*>(y)[(size_t)col * n + row] = v;
+      } else if (mode == RESIDUAL) {
+        *to = __float2bfloat16_rn(ld_prev_bf16(to) + bfr(v));
+      } else if ((tile & 1) == 0) {
+        gate[i] = bfr(v);
+      } else {
+        reinterpret_cast<bf16*>(y)[(size_t)col * (n / 2) + row] = __float2bfloat16_rn(bfr(gate[i] / (1.f + expf(-gate[i]))) * bfr(v));
+      }
     }
     ++tile;
   };
@@ -310,11 +373,13 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) linear4_few_kernel(const bf
 
 constexpr size_t SMEM_MOST = 227 * 1024;
 
-template <typename... P, typename... A> int launch(void (*kern)(P...), bool& asked, int grid, int threads, size_t bytes, int pdl, cudaStream_t st, A... a) {
-  if (!asked) {   // (asking twice does no harm)
+template <typename... P, typename... A> int launch(void (*kern)(P...), bool (&asked)[64], int grid, int threads, size_t bytes, int pdl, cudaStream_t st, A... a) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return DRYFT_ERR_UNSUPPORTED;
+  if (!asked[dev]) {   // (asking twice does no harm)
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_MOST);
     if (e != cudaSuccess) return (int)e;
-    asked = true;
+    asked[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
@@ -330,42 +395,54 @@ template <typename... P, typename... A> int launch(void (*kern)(P...), bool& ask
   return e != cudaSuccess ? (int)e : launch_status();
 }
 
-struct Args { const void *x; long long x_stride; const void *codes, *scales; void* y; int m, n, k, group, pdl; cudaStream_t st; };
+struct Args {
+  const void* x;
+  long long x_stride;
+  const void *codes, *scales;
+  void* y;
+  int m, n, k, group, mode;
+  const float* norm_w;
+  float eps;
+  int pdl;
+  cudaStream_t st;
+};
 
-template <int NT, int GS, int TEAM, int PB, int SLOTS, typename O> int few(const Args& a) {
-  static bool asked = false;
-  const int tiles = (a.n + 15) / 16;
-  return launch(linear4_few_kernel<NT, GS, TEAM, PB, SLOTS, O>, asked, tiles < 148 ? tiles : 148, FEW_WARPS * 32, Few<NT, GS, TEAM, PB, SLOTS>::bytes(a.m, a.k), a.pdl,
-                a.st, (const bf16*)a.x, a.x_stride, (const uint4*)a.codes, (const uint2*)a.scales, (O*)a.y, a.m, a.n, a.k, __builtin_ctz(a.group));
+template <int NT, int GS, int TEAM, int PB, int SLOTS> int few(const Args& a) {
+  static bool asked[64] = {false};
+  const int tiles = (a.n + 15) / 16, turns = a.mode == SILU ? tiles / 2 : tiles;
+  return launch(linear4_few_kernel<NT, GS, TEAM, PB, SLOTS>, asked, turns < 148 ? turns : 148, FEW_WARPS * 32, Few<NT, GS, TEAM, PB, SLOTS>::bytes(a.m, a.k), a.pdl, a.st,
+                (const bf16*)a.x, a.x_stride, (const uint4*)a.codes, (const uint2*)a.scales, a.y, a.m, a.n, a.k, __builtin_ctz(a.group), a.mode, a.norm_w, a.eps);
 }
 // Four warps a tile where shared memory has room for their rings (x of 8 rows: up to about 6,000 inputs), else all sixteen with shorter rings.  2,560 inputs,
 // one row, four / eight / sixteen warps a tile: 151,936 outputs 55.6 / 63.6 / 81.9 us, 6,144 outputs 4.8 / 5.4 / 5.7 us (a tile's end costs each warp as much as
 // half a slot); 2,560 outputs of 9,728 inputs, hardly more tiles than multiprocessors, 9.6 / 9.7 / 10.2 us.
-template <int NT, int GS, typename O> int few_rows(const Args& a) {
+template <int NT, int GS> int few_rows(const Args& a) {
   constexpr int GM = GS == 8 ? 4 : GS;
-  if (Few<NT, GS, 4, 2, 4>::bytes(a.m, a.k) <= SMEM_MOST) return few<NT, GS, 4, 2, 4, O>(a);
-  return few<NT, GM, 16, 1, 4, O>(a);
+  if (Few<NT, GS, 4, 2, 4>::bytes(a.m, a.k) <= SMEM_MOST) return few<NT, GS, 4, 2, 4>(a);
+  return few<NT, GM, 16, 1, 4>(a);
 }
 template <int NT> bool fits(int m, int k, int group) {
   return (group >= 64 ? Few<NT, 4, 16, 1, 4>::bytes(m, k) : group == 32 ? Few<NT, 2, 16, 1, 4>::bytes(m, k) : Few<NT, 1, 16, 1, 4>::bytes(m, k)) <= SMEM_MOST;
 }
 bool takes(int m, int k, int group) { return m <= 8 ? fits<1>(m, k, group) : m <= 16 && fits<2>(m, k, group); }
 
-template <int GS, typename O> int by_rows(const Args& a) { return a.m <= 8 ? few_rows<1, GS, O>(a) : few_rows<2, GS, O>(a); }
-template <typename O> int by_group(const Args& a) {
-  return (a.group == 128 ? by_rows<8, O> : a.group == 64 ? by_rows<4, O> : a.group == 32 ? by_rows<2, O> : by_rows<1, O>)(a);
-}
+template <int GS> int by_rows(const Args& a) { return a.m <= 8 ? few_rows<1, GS>(a) : few_rows<2, GS>(a); }
 }  // namespace
 
 // Whether the kernel for few rows of bfloat16 takes so many rows of so many inputs (they have to fit in shared memory).
 DRYFT_API int dryft_linear4_takes(int m, int k, int group) { return takes(m, k, group); }
 
-DRYFT_API int dryft_linear4(int is_bf16, int out_bf16, const void* x, long long x_stride, const void* codes, const void* scales, void* y, int m, int n, int k,
-                            int group, int pdl, void* stream) {
+// mode: Mode.  Modes beyond storing, and norm_w (which has k numbers on a 16-byte boundary; null: no norm), are the bfloat16 kernel's; SILU wants n to be a multiple of 32.
+DRYFT_API int dryft_linear4(int is_bf16, int mode, const void* x, long long x_stride, const void* codes, const void* scales, void* y, int m, int n, int k, int group,
+                            const float* norm_w, float eps, int pdl, void* stream) {
   if (m <= 0 || n <= 0) return 0;
   const cudaStream_t st = (cudaStream_t)stream;
-  if (is_bf16 && !takes(m, k, group)) return DRYFT_ERR_UNSUPPORTED;
-  if (is_bf16) return (out_bf16 ? by_group<bf16> : by_group<float>)({x, x_stride, codes, scales, y, m, n, k, group, pdl, st});
+  if (is_bf16) {
+    if (!takes(m, k, group) || (mode == SILU && n % 32) || ((uintptr_t)norm_w & 15)) return DRYFT_ERR_UNSUPPORTED;
+    const Args a = {x, x_stride, codes, scales, y, m, n, k, group, mode, norm_w, eps, pdl, st};
+    return (group == 128 ? by_rows<8> : group == 64 ? by_rows<4> : group == 32 ? by_rows<2> : by_rows<1>)(a);
+  }
+  if (mode != STORE_F32 || norm_w) return DRYFT_ERR_UNSUPPORTED;
   const int rows = m == 1 ? 1 : m <= 4 ? 4 : m <= 8 ? 8 : 16;
   auto kern = rows == 1 ? linear4_f32_kernel<1> : rows == 4 ? linear4_f32_kernel<4> : rows == 8 ? linear4_f32_kernel<8> : linear4_f32_kernel<16>;
   kern<<<dim3((n + 15) / 16, (m + rows - 1) / rows), WARPS * 32, 0, st>>>((const float*)x, x_stride, (const uint4*)codes, (const uint2*)scales, (float*)y, m, n, k,

@@ -144,7 +144,7 @@ class DecoderModel:
             return None
         if res.closer is not None:   # streams that only their block arrangement knows how to join
             return self.head.forward(res.closer.final_rows(res, self.final_norm, want_rows, n_want))
-        if (all_rows and res.delta is None and res.ss is not None and hasattr(self.head, "forward_normed")
+        if (all_rows and res.delta is None and (res.ss is not None or (getattr(self.head, "own_sums", False) and res.x.dtype == torch.bfloat16)) and hasattr(self.head, "forward_normed")
                 and self.head.can_fuse(res.x.shape[0], self.final_norm)):
             xw = res.xw if res.xw_norm is self.final_norm else None
             return self.head.forward_normed(res.x, res.ss, res.ss_parts, self.final_norm, **({"xw": xw} if xw is not None else {}))

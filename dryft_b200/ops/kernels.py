@@ -2472,7 +2472,7 @@ def _bits4_group(size: int, group: int, what: str) -> None:
 def linear4_lib() -> ctypes.CDLL:
     """Products with weights held in 4 bits."""
     return _single_lib("linear4", {
-        "dryft_linear4": [_i, _i, _p, _ll, _p, _p, _p, _i, _i, _i, _i, _i, _p],
+        "dryft_linear4": [_i, _i, _p, _ll, _p, _p, _p, _i, _i, _i, _i, _p, _f, _i, _p],
         "dryft_linear4_takes": [_i, _i, _i],
         "dryft_weight4_expand": [_i, _p, _p, _p, _i, _i, _i, _p],
     })
@@ -2613,9 +2613,27 @@ def linear4_plan(m: int, n: int, k: int, group: int, bf16: bool) -> int:
     return int(linear4_tc_lib().dryft_linear4_tc_pieces(m, n, k))
 
 
-def linear4(x, w: Weight4, out, pdl: bool = False) -> None:
+def linear4_fuses(m: int, w) -> bool:
+    """Whether ``linear4`` takes norms, sums and activations with its product: few rows of bfloat16."""
+    return isinstance(w, Weight4) and 0 < m <= 16 and linear4_plan(m, w.n, w.k, w.group, True) == 0
+
+
+# Rows up to which the models' steps leave the norm and the residual sum to the products: every block norms the rows for itself, which saves two launches a
+# layer and costs more with every row.  36 layers 2,560 wide, ms a step, left / not left to them: 1 row 1.61 / 1.69, 2 rows 1.71 / 1.77, 4 rows 1.82 / 1.88,
+# 8 rows 2.12 / 2.02, 16 rows 2.59 / 2.58.  (SiLU and the multiplication stay with the product at up to 16 rows.)
+LINEAR4_NORM_ROWS = 4
+
+
+_LINEAR4_MODES = {"store": 0, "residual": 2, "silu": 3}
+
+
+def linear4(x, w: Weight4, out, pdl: bool = False, mode: str = "store", norm_w=None, eps: float = 0.0) -> None:
     """``out = x @ w.T``; ``x`` bfloat16, up to 256 rows (float32: 64), ``out`` of the same type or float32.  ``pdl``: a programmatic dependent (its
-    first weights are requested while the launch before it drains)."""
+    first weights are requested while the launch before it drains).
+
+    With few rows of bfloat16 (``linear4_fuses``) also what stands around a decoder's products: ``norm_w`` (float32 ``[k]``): RMS norm of ``x`` first;
+    ``mode="residual"``: ``out += `` the result, in place; ``mode="silu"``: ``w`` holds gate rows, then as many others, and ``out`` ``[m, n / 2]`` is
+    ``silu(gate) * other``.  Rounding points are those of the bfloat16 products (``gemm_small_m``)."""
     global _linear4_fn, _linear4_tc_fn, launch_count
     _need_weight4(w)
     step = _rows_in(x, "x", w.k)
@@ -2626,7 +2644,15 @@ def linear4(x, w: Weight4, out, pdl: bool = False) -> None:
     out_bf16 = _act(out, "out")
     if out_bf16 and not is_bf16:
         raise KernelError("linear4: 32-bit activations give 32-bit results")
-    _need(out, "out", None, (m, w.n))
+    code = _LINEAR4_MODES.get(mode, -1)
+    if code or norm_w is not None:
+        if code < 0:
+            raise KernelError(f"linear4: mode is one of {', '.join(_LINEAR4_MODES)}, got {mode!r}")
+        if not linear4_fuses(m, w) or not is_bf16 or (code and not out_bf16) or (code == 3 and w.n % 32):
+            raise KernelError(f"linear4: norms, sums and activations are for few rows of bfloat16, halves of whole tiles; got {m} rows, {tuple(w.shape)}, mode {mode}")
+        if norm_w is not None:
+            _need(norm_w, "norm weight", torch.float32, (w.k,))
+    _need(out, "out", None, (m, w.n // 2 if code == 3 else w.n))
     floats = linear4_plan(m, w.n, w.k, w.group, bool(is_bf16))
     if floats:
         if _linear4_tc_fn is None:
@@ -2637,7 +2663,8 @@ def linear4(x, w: Weight4, out, pdl: bool = False) -> None:
     else:
         if _linear4_fn is None:
             _linear4_fn = linear4_lib().dryft_linear4
-        rc = _linear4_fn(is_bf16, out_bf16, x.data_ptr(), step, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), m, w.n, w.k, w.group, pdl, _stream())
+        rc = _linear4_fn(is_bf16, code or not out_bf16, x.data_ptr(), step, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), m, w.n, w.k, w.group,
+                         norm_w.data_ptr() if norm_w is not None else 0, eps, pdl, _stream())
     if rc:
         _ok(rc, "linear4")
     launch_count += 1
@@ -2659,7 +2686,7 @@ def kv4_lib() -> ctypes.CDLL:
     """The paged cache held in 4 bits: new tokens in, pages out."""
     return _single_lib("kv4", {
         "dryft_kv4_store": [_i, _p, _p, _ll, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p],
-        "dryft_kv4_rope_store": [_i, _p, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _p],
+        "dryft_kv4_rope_store": [_i, _p, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _p],
         "dryft_kv4_expand": [_i, _p, _p, _p, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p],
     })
 
@@ -2730,9 +2757,9 @@ def kv4_store(k, v, tok_slot, tok_pos, k_pages, v_pages, page_table, group: int)
 
 
 def kv4_rope_store(qkv, q_norm_w, k_norm_w, inv_freq, tok_slot, tok_pos, q_out, k_pages, v_pages, page_table, n_heads: int, n_kv_heads: int,
-                   head_dim: int, rotary_dim: int, eps: float, group: int, cs_table=None) -> None:
+                   head_dim: int, rotary_dim: int, eps: float, group: int, cs_table=None, pdl: bool = False) -> None:
     """``qk_norm_rope_store`` with the cache in 4 bits: per-head norm and rotation of the rows' queries and keys, queries to ``q_out``, keys and values into
-    the cache as ``kv4_store`` puts them there.  ``cs_table`` as there."""
+    the cache as ``kv4_store`` puts them there.  ``cs_table`` as there.  ``pdl``: a programmatic dependent."""
     n = qkv.shape[0]
     width = (n_heads + 2 * n_kv_heads) * head_dim
     _need(qkv, "qkv", None, (n, width))
@@ -2756,7 +2783,7 @@ def kv4_rope_store(qkv, q_norm_w, k_norm_w, inv_freq, tok_slot, tok_pos, q_out, 
             raise KernelError("kv4_rope_store: cos/sin table shorter than the batch")
     _ok(kv4_lib().dryft_kv4_rope_store(is_bf16, _ptr(qkv), width, _ptr(q_norm_w), _ptr(k_norm_w), _ptr(inv_freq), _ptr(cs_table), _ptr(tok_slot), _ptr(tok_pos),
                                        _ptr(q_out), _ptr(k_pages), _ptr(v_pages), _ptr(page_table), page_table.shape[1], n, n_heads, n_kv_heads, head_dim,
-                                       rotary_dim, group, page, float(eps), int(has_norm), _stream()), "kv4_rope_store")
+                                       rotary_dim, group, page, float(eps), int(has_norm), int(pdl), _stream()), "kv4_rope_store")
 
 
 def kv4_expand(k_pages, v_pages, page_table, cu_q, seq_slot, tok_pos, k_out, v_out, group: int, max_kv: int, window: Optional[int] = None) -> None:

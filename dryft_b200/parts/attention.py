@@ -23,7 +23,7 @@ from ..cache.store import CacheEntry, KVNeed, StateNeed
 from ..config.spec import PartSpec
 from ..ops import kernels as K
 from .base import NORMS, POSITIONS, Runtime, StepContext, TensorInfo, fused_rms, register_mixer
-from .linear import fusable_rows, held, linear, weighted_for
+from .linear import four_bits_fuse, fusable_rows, held, linear, weighted_for
 
 PREFILL_TILE = 64      # query rows per block of the mma.sync prefill kernel
 PREFILL_TILE_TC = 128  # query rows per block of the tcgen05 prefill kernel
@@ -138,8 +138,15 @@ class Attention:
     def can_fuse(self, n_rows: int, norm) -> bool:
         """Few rows, bfloat16 everywhere, widths the weight-streaming product takes."""
         rt = self.rt
+        if isinstance(self.w_qkv, K.Weight4):
+            return four_bits_fuse(n_rows, norm, rt, self.w_qkv, self.w_o)
         return (rt.fuse_decode and rt.is_bf16 and fusable_rows(n_rows, self.hidden, rt, normed=True) and fusable_rows(n_rows, self.q_dim, rt)
                 and fused_rms(norm) is not None and self.w_qkv.dtype == torch.bfloat16 and self.w_o.dtype == torch.bfloat16)
+
+    @property
+    def own_sums(self) -> bool:
+        """Whether ``forward_normed`` needs no sums of squares of the stream, and leaves none."""
+        return isinstance(self.w_qkv, K.Weight4)
 
     weighted_ahead = True   # forward_normed takes ``xw`` / ``next_norm`` and returns the weighted stream too
 
@@ -153,6 +160,10 @@ class Attention:
         w = self.w_qkv if owns_cache else self.w_qkv[: self.q_dim]
         qkv = torch.empty((n, w.shape[0]), dtype=x.dtype, device=x.device)
         norm_w, eps = fused_rms(norm)
+        if isinstance(w, K.Weight4):   # these products sum their rows' squares themselves
+            K.linear4(x, w, qkv, pdl=self.rt.pdl, norm_w=norm_w, eps=eps)
+            K.linear4(self._attend(qkv, ctx, cache, owns_cache), self.w_o, x, pdl=self.rt.pdl, mode="residual")
+            return None, 0, None
         small = self.rt.small_m_max
         if xw is not None and K.weighted_ahead_supported(self.hidden):
             K.fused_product(x, w, qkv, small_m_max=small, xw_in=xw, norm_w=norm_w, ss_in=ss, ss_parts=ss_parts, eps=eps, pdl=self.rt.pdl)
@@ -215,7 +226,8 @@ class Attention:
         table = table_of(ctx) if table_of is not None else None
         if owns_cache:
             K.kv4_rope_store(qkv, self.q_norm_w, self.k_norm_w, self.position.inv_freq, ctx.tok_slot, ctx.tok_pos, q, cache.k, cache.v, cache.page_table,
-                             self.n_heads, self.n_kv, self.head_dim, self.position.rotary_dim, self.qk_eps, self.bits_group, cs_table=table)
+                             self.n_heads, self.n_kv, self.head_dim, self.position.rotary_dim, self.qk_eps, self.bits_group, cs_table=table,
+                             pdl=self.rt.pdl)
         else:
             K.qk_norm_rope_store(qkv, self.q_norm_w, self.k_norm_w, self.position.inv_freq, ctx.tok_slot, ctx.tok_pos, q, None, None, None, self.n_heads,
                                  self.n_kv, self.head_dim, self.position.rotary_dim, self.qk_eps, write_kv=False, cs_table=table)

@@ -25,7 +25,8 @@ Optional: ``serves_four_bits = True`` says that a mixer, feed-forward or head ho
 Optional, for few rows (decode): a mixer or feed-forward may offer
             ``forward_normed(x, ss, ss_parts, norm, ...) -> (ss, ss_parts)``: it normalises ``x`` itself
             inside its first product, adds its output into ``x`` in place inside its last product, and
-            returns the new sums of squares; ``can_fuse(n_rows, norm)`` says when.
+            returns the new sums of squares; ``can_fuse(n_rows, norm)`` says when.  ``own_sums``: it sums the squares itself,
+            takes none and returns ``None`` for them (the parts of a block agree on that).
 """
 
 from __future__ import annotations

@@ -33,7 +33,7 @@ class PreNormBlock:
 
     def _fusable(self, n_rows: int) -> bool:
         m, f = self.mixer, self.ffn
-        if f is None:
+        if f is None or getattr(m, "own_sums", False) != getattr(f, "own_sums", False):
             return False
         return (hasattr(m, "forward_normed") and hasattr(f, "forward_normed")
                 and m.can_fuse(n_rows, self.norm_mixer) and f.can_fuse(n_rows, self.norm_ffn))
@@ -53,7 +53,7 @@ class PreNormBlock:
             xw = res.xw if res.xw_norm is self.norm_mixer else None
             ahead_m = getattr(self.mixer, "weighted_ahead", False)
             ahead_f = getattr(self.ffn, "weighted_ahead", False)
-            if ss is None:
+            if ss is None and not getattr(self.mixer, "own_sums", False):
                 ss = torch.empty(K.SS_STRIDE, dtype=torch.float32, device=x.device)
                 if ahead_m and weighted_for(self.norm_mixer, x.shape[1], x.shape[1], self.mixer.rt, x.shape[0]):
                     xw = torch.empty_like(x)

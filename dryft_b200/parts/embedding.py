@@ -13,7 +13,7 @@ import torch
 
 from ..ops import kernels as K
 from .base import Residual, Runtime, StepContext, TensorInfo, fused_rms, register_embedding, register_head
-from .linear import fusable_rows, held, linear
+from .linear import four_bits_fuse, fusable_rows, held, linear
 
 
 @register_embedding("embedding")
@@ -131,8 +131,15 @@ class LMHead:
         """32-bit logits ``[rows, vocab]``."""
         return self._cap(linear(h, self.weight, self.rt, out_dtype=torch.float32))
 
+    @property
+    def own_sums(self) -> bool:
+        """Whether ``forward_normed`` needs no sums of squares of the stream."""
+        return isinstance(self.weight, K.Weight4)
+
     def can_fuse(self, n_rows: int, norm) -> bool:
         rt = self.rt
+        if isinstance(self.weight, K.Weight4):
+            return four_bits_fuse(n_rows, norm, rt, self.weight)
         return (rt.fuse_decode and rt.is_bf16 and fusable_rows(n_rows, self.weight.shape[1], rt, normed=True)
                 and fused_rms(norm) is not None and self.weight.dtype == torch.bfloat16)
 
@@ -141,6 +148,9 @@ class LMHead:
         weighted by the final norm's weight already."""
         out = torch.empty((x.shape[0], self.vocab), dtype=torch.float32, device=x.device)
         norm_w, eps = fused_rms(norm)
+        if isinstance(self.weight, K.Weight4):
+            K.linear4(x, self.weight, out, pdl=self.rt.pdl, norm_w=norm_w, eps=eps)
+            return self._cap(out)
         small = self.rt.small_m_max
         if xw is not None and K.weighted_ahead_supported(x.shape[1]):
             K.fused_product(x, self.weight, out, small_m_max=small, xw_in=xw, norm_w=norm_w, ss_in=ss, ss_parts=ss_parts, eps=eps, pdl=self.rt.pdl)

@@ -12,7 +12,7 @@ import torch
 
 from ..ops import kernels as K
 from .base import Runtime, StepContext, TensorInfo, fused_rms, register_ffn
-from .linear import fusable_rows, held, linear, weighted_for
+from .linear import four_bits_fuse, fusable_rows, held, linear, weighted_for
 
 
 @register_ffn("swiglu")
@@ -38,8 +38,15 @@ class SwiGLU:
 
     def can_fuse(self, n_rows: int, norm) -> bool:
         rt = self.rt
+        if isinstance(self.w_gate_up, K.Weight4):
+            return self.inter % 16 == 0 and four_bits_fuse(n_rows, norm, rt, self.w_gate_up, self.w_down)
         return (rt.fuse_decode and rt.is_bf16 and fusable_rows(n_rows, self.hidden, rt, normed=True) and fusable_rows(n_rows, self.inter, rt)
                 and fused_rms(norm) is not None and self.w_gate_up.dtype == torch.bfloat16 and self.w_down.dtype == torch.bfloat16)
+
+    @property
+    def own_sums(self) -> bool:
+        """Whether ``forward_normed`` needs no sums of squares of the stream, and leaves none."""
+        return isinstance(self.w_gate_up, K.Weight4)
 
     weighted_ahead = True   # forward_normed takes ``xw`` / ``next_norm`` and returns the weighted stream too
 
@@ -50,6 +57,10 @@ class SwiGLU:
         n = x.shape[0]
         act = torch.empty((n, self.inter), dtype=x.dtype, device=x.device)
         norm_w, eps = fused_rms(norm)
+        if isinstance(self.w_gate_up, K.Weight4):   # these products sum their rows' squares themselves
+            K.linear4(x, self.w_gate_up, act, pdl=self.rt.pdl, mode="silu", norm_w=norm_w, eps=eps)
+            K.linear4(act, self.w_down, x, pdl=self.rt.pdl, mode="residual")
+            return None, 0, None
         small = self.rt.small_m_max
         if xw is not None and K.weighted_ahead_supported(self.hidden):
             K.fused_product(x, self.w_gate_up, act, small_m_max=small, mode="silu", xw_in=xw, norm_w=norm_w, ss_in=ss, ss_parts=ss_parts,
@@ -69,9 +80,11 @@ class SwiGLU:
         return ss_out, parts, xw_out
 
     def _rows(self, h: torch.Tensor) -> torch.Tensor:
-        gu = linear(h, self.w_gate_up, self.rt)
         act = torch.empty((h.shape[0], self.inter), dtype=h.dtype, device=h.device)
-        K.silu_mul(gu, act)
+        if h.dtype == torch.bfloat16 and self.inter % 16 == 0 and K.linear4_fuses(h.shape[0], self.w_gate_up):
+            K.linear4(h, self.w_gate_up, act, pdl=self.rt.pdl, mode="silu")
+        else:
+            K.silu_mul(linear(h, self.w_gate_up, self.rt), act)
         return linear(act, self.w_down, self.rt)
 
     def forward(self, h: torch.Tensor, ctx: StepContext) -> torch.Tensor:

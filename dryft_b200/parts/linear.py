@@ -66,6 +66,12 @@ def held(w: torch.Tensor, rt: Runtime):
     return K.pack_weight4(w, K.bits4_group(w.shape[1], rt.bits_group)) if rt.weight_bits == 4 else w
 
 
+def four_bits_fuse(n_rows: int, norm, rt: Runtime, *weights) -> bool:
+    """Whether the norm before a step's products with 4-bit weights, and the sums behind them, are the products' own work."""
+    return (rt.fuse_decode and rt.is_bf16 and n_rows <= K.LINEAR4_NORM_ROWS and fused_rms(norm) is not None
+            and all(K.linear4_fuses(n_rows, w) for w in weights))
+
+
 EXPAND_BYTES = 256 << 20   # of weights at a time that a product of many rows takes out of their 4 bits (which bounds what that holds)
 
 

@@ -83,6 +83,41 @@ def test_products_of_many_rows(m, dtype, out, monkeypatch):
     _near(y, P.linear(x, values), slack)
 
 
+@pytest.mark.parametrize("m", [1, 2, 3, 5, 8, 9, 16])
+@pytest.mark.parametrize("n,k,group", [(32, 16, 16), (64, 64, 64), (96, 96, 32), (1312, 2560, 128), (192, 80, 16), (10016, 128, 64)])
+def test_products_with_the_norm_before_and_the_sum_or_activation_behind(m, n, k, group):
+    """The norm against 64 bits (its two roundings are allowed one unit, 2^-8, of each number; the other half is left to their signs).  What follows a product
+    is held to the last bit: the same kernel's plain product, rounded where the products of bfloat16 weights round, and the activation of its own launch."""
+    w, x, norm = _weights(n, k, BF) / k**0.5, torch.randn(m, k).to(BF), (1 + 0.2 * torch.randn(k)).to(DEV)
+    values, s, _ = P.group_values(w, group)
+    w4, eps, xd = K().pack_weight4(w.to(DEV), group), 1e-6, x.to(DEV)
+    h = x.double() * torch.rsqrt((x.double()**2).mean(1, keepdim=True) + eps) * norm.double().cpu()
+    new = lambda cols, dtype=BF: torch.full((m, cols), float("nan"), dtype=dtype, device=DEV)
+    out32 = new(n, F32)
+    K().linear4(xd, w4, out32, norm_w=norm, eps=eps)
+    _near(out32, P.linear(h, values), P.linear_slack(h.to(BF), values, s, group, F32) + (2.0**-8 + 1e-5) * (h.abs() @ values.abs().T))
+    y0 = torch.randn(m, n, device=DEV).to(BF)
+    for more in ({}, dict(norm_w=norm, eps=eps)):
+        plain, wide, total, act, want = new(n), new(n, F32), y0.clone(), new(n // 2), new(n // 2)
+        K().linear4(xd, w4, plain, **more)
+        K().linear4(xd, w4, wide, **more)
+        assert torch.equal(plain, wide.to(BF))
+        K().linear4(xd, w4, total, pdl=True, mode="residual", **more)
+        assert torch.equal(total, (y0.float() + plain.float()).to(BF))
+        K().linear4(xd, w4, act, pdl=True, mode="silu", **more)
+        K().silu_mul(plain, want)
+        assert torch.equal(act, want)
+
+
+def test_modes_that_are_refused():
+    w4, t = K().pack_weight4(torch.randn(48, 64, device=DEV)), lambda *shape, dtype=BF: torch.zeros(shape, dtype=dtype, device=DEV)
+    for x, out, more in ((t(17, 64), t(17, 48), dict(mode="residual")), (t(1, 64, dtype=F32), t(1, 48, dtype=F32), dict(norm_w=t(64, dtype=F32))), (t(1, 64), t(1, 24), dict(mode="silu")),
+                         (t(1, 64), t(1, 48, dtype=F32), dict(mode="residual")), (t(1, 64), t(1, 48), dict(mode="relu")), (t(1, 64), t(1, 48), dict(norm_w=t(64))),
+                         (t(1, 64), t(1, 48), dict(norm_w=t(63, dtype=F32)))):
+        with pytest.raises(K().KernelError):
+            K().linear4(x, w4, out, **more)
+
+
 def test_a_rows_bits_do_not_depend_on_the_other_rows_among_eight():
     n, k = 250, 2560
     w4, x = K().pack_weight4(_weights(n, k, BF).to(DEV)), torch.randn(8, k, device=DEV).to(BF)
