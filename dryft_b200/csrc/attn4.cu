@@ -433,14 +433,20 @@ __global__ void __launch_bounds__(WARPS * 32, Block<WARPS>::AT_ONCE) attn4_mma_k
 }
 
 // ---------------------------------------------------------------------------------------------- 32-bit
-// A thread per key for the scores, a thread per dim for the values, everything in 32-bit multiply-adds.
-constexpr int THREADS = 128, DIMS = (D + THREADS - 1) / THREADS;
+// Every product is a 32-bit multiply-add (no tensor core keeps 24 bits).  A warp takes every eighth tile of 16 keys of the split, with a running maximum and sums of
+// its own, joined in the warps' order behind the last one.  Scores: two lanes a key, half of the dims each.  Values: a lane keeps four dims (times QUADS) of every
+// head and walks the tile's tokens, whose codes are four 8-byte words of the layout; where a head has fewer than 32 such quads, lanes share the tokens.
+// A tile's codes, keys' and values', are requested before its scores are formed: what bounds the kernel is that chain (page number, codes, scores, weights, sums),
+// about 2 us a tile and warp.  13 rows, windows of 100 keys, three key heads of 48: 6.4 us (13.7 with a thread a key and a thread a dim, the values' 128 loads one
+// behind the other); eight rows of 500 keys, eight key heads of 128: 10 us (29.2).
+constexpr int THREADS = 128, F32_WARPS = 8, QUADS = (8 * UNITS + 31) / 32, SHARE = 8 * UNITS <= 8 ? 4 : 8 * UNITS <= 16 ? 2 : 1;
 
-__global__ void __launch_bounds__(THREADS) attn4_f32_kernel(const float* __restrict__ q, const unsigned char* __restrict__ k_pages,
-                                                            const unsigned char* __restrict__ v_pages, const int* __restrict__ page_table, int max_pages,
-                                                            const int* __restrict__ tok_slot, const int* __restrict__ tok_pos, float* out, float* part_o,
-                                                            float* part_ml, float scale, int window) {
-  __shared__ float qs[HEADS][D], ps[HEADS][THREADS], red[THREADS / 32][HEADS], total[THREADS / 32][HEADS], top[HEADS], sum[HEADS];
+__global__ void __launch_bounds__(F32_WARPS * 32) attn4_f32_kernel(const float* __restrict__ q, const unsigned char* __restrict__ k_pages,
+                                                                   const unsigned char* __restrict__ v_pages, const int* __restrict__ page_table, int max_pages,
+                                                                   const int* __restrict__ tok_slot, const int* __restrict__ tok_pos, float* out, float* part_o,
+                                                                   float* part_ml, float scale, int window) {
+  __shared__ __align__(16) float qs[HEADS][D];   // the queries, later the block's sums
+  __shared__ float ps[F32_WARPS][16][HEADS], tops[F32_WARPS][HEADS], sums[F32_WARPS][HEADS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Work w = work_of_block();
   const int n_kv = w.n_kv, splits = w.splits;
@@ -448,110 +454,163 @@ __global__ void __launch_bounds__(THREADS) attn4_f32_kernel(const float* __restr
   const size_t head0 = ((size_t)w.n * n_kv + w.head) * G + 8 * w.ht;
   if (slot < 0) {
     if (w.split == 0)
-      for (int i = tid; i < heads * D; i += THREADS) out[head0 * D + i] = 0.f;
+      for (int i = tid; i < heads * D; i += F32_WARPS * 32) out[head0 * D + i] = 0.f;
     return;
   }
   const Span keys = span_of(pos, window, w.split, splits, 1);
-  for (int i = tid; i < HEADS * D; i += THREADS) qs[i / D][i % D] = i / D < heads ? q[head0 * D + i] : 0.f;
-  if (tid < HEADS) {
-    top[tid] = -INFINITY;
-    sum[tid] = 0.f;
-  }
-  float acc[DIMS][HEADS];
-#pragma unroll
-  for (int i = 0; i < DIMS; ++i)
-#pragma unroll
-    for (int g = 0; g < HEADS; ++g) acc[i][g] = 0.f;
+  for (int i = tid; i < HEADS * D; i += F32_WARPS * 32) qs[i / D][i % D] = i / D < heads ? q[head0 * D + i] : 0.f;
   __syncthreads();
-  const int* pages = page_table + (size_t)slot * max_pages;
-  for (int j0 = keys.first; j0 < keys.end; j0 += THREADS) {
-    const int j = j0 + tid;
+  float acc[QUADS][4][HEADS], top[HEADS], sum[HEADS];
+#pragma unroll
+  for (int g = 0; g < HEADS; ++g) {
+    top[g] = LOWEST;
+    sum[g] = 0.f;
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][e][g] = 0.f;
+  }
+  const int key = lane & 15, half = lane >> 4, part = SHARE > 1 ? lane / (8 * UNITS) : 0;
+  const int* const pages = page_table + (size_t)slot * max_pages;
+  for (int t = keys.first / 16 + warp; t * 16 < keys.end; t += F32_WARPS) {
+    const size_t page_at = ((size_t)pages[t * 16 / PAGE] * n_kv + w.head) * TILE;
+    const int in_page = t * 16 % PAGE;
+    const unsigned char* const kt = k_pages + page_at;
+    const unsigned char* const vt = v_pages + page_at;
+    const bool seen = t * 16 + key >= keys.first && t * 16 + key < keys.end;
+    // a key's codes: quarters 2 half and 2 half + 1 of its row, UNITS words each; a quad's: the tokens' words, four tokens each
+    unsigned kw[2 * UNITS], ks[GROUPS];
+    load_words<2 * UNITS>(kw, kt + (size_t)(in_page + key) * ROW + half * UNITS * 8);
+    load_words<GROUPS>(ks, kt + (size_t)ROW * PAGE + (size_t)(in_page + key) * GROUPS * 4);
+    uint2 vw[QUADS][4 / SHARE];
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) {
+      const int at = SHARE > 1 ? lane % (8 * UNITS) : lane + 32 * i, r = at & 7, u = at >> 3;
+#pragma unroll
+      for (int c = 0; c < 4 / SHARE; ++c)
+        vw[i][c] = u < UNITS && part < SHARE
+                       ? *reinterpret_cast<const uint2*>(vt + kv4_value_at(in_page + 2 * (c + part * (4 / SHARE)), r, u, UNITS)) : make_uint2(0, 0);
+    }
     float s[HEADS];
 #pragma unroll
-    for (int g = 0; g < HEADS; ++g) s[g] = j < keys.end ? 0.f : -INFINITY;
-    if (j < keys.end) {
-      const unsigned char* kt = k_pages + ((size_t)pages[j / PAGE] * n_kv + w.head) * TILE;
-      const unsigned* sz = reinterpret_cast<const unsigned*>(kt + (size_t)ROW * PAGE) + (j % PAGE) * GROUPS;
-      const unsigned* words = reinterpret_cast<const unsigned*>(kt + (size_t)(j % PAGE) * ROW);
-      for (int i = 0; i < D / 4; ++i) {   // four numbers of one step and quarter
-        const int c = i & 3, step = i >> 2;
-        const unsigned word = words[c * UNITS + step / 2] >> (8 * (step & 1));
-        const GroupCode gc = unpack_code(sz[step * 16 / BG]);
+    for (int g = 0; g < HEADS; ++g) s[g] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float v = value_of(word >> (4 * (e >> 1) + 16 * (e & 1)) & 15u, gc);
+    for (int step = 0; step < D / 16; ++step) {
+      const GroupCode gc = unpack_code(ks[step * 16 / BG]);
 #pragma unroll
-          for (int g = 0; g < HEADS; ++g) s[g] = fmaf(v, qs[g][step * 16 + 4 * c + e], s[g]);
+      for (int c = 0; c < 2; ++c) {   // four numbers of one step and quarter
+        const unsigned word = kw[c * UNITS + step / 2] >> (8 * (step & 1));
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = value_of(word >> (4 * (e >> 1) + 16 * (e & 1)) & 15u, gc);
+#pragma unroll
+        for (int g = 0; g < HEADS; ++g) {
+          const float4 x = *reinterpret_cast<const float4*>(&qs[g][step * 16 + 4 * (2 * half + c)]);
+          s[g] = fmaf(v[0], x.x, fmaf(v[1], x.y, fmaf(v[2], x.z, fmaf(v[3], x.w, s[g]))));
         }
       }
-#pragma unroll
-      for (int g = 0; g < HEADS; ++g) s[g] *= scale;
     }
+    float lower[HEADS];
 #pragma unroll
     for (int g = 0; g < HEADS; ++g) {
-      const float m = warp_max(s[g]);
-      if (lane == 0) red[warp][g] = m;
-    }
-    __syncthreads();
-    float lower[HEADS], most[HEADS];
-#pragma unroll
-    for (int g = 0; g < HEADS; ++g) {
-      float m = top[g];
-#pragma unroll
-      for (int x = 0; x < THREADS / 32; ++x) m = fmaxf(m, red[x][g]);
+      s[g] += __shfl_xor_sync(0xffffffffu, s[g], 16);
+      s[g] = seen ? s[g] * scale : -INFINITY;
+      const float m = fmaxf(top[g], warp_max(s[g]));
       lower[g] = m == top[g] ? 1.f : expf(top[g] - m);
-      most[g] = m;
-      s[g] = s[g] == -INFINITY ? 0.f : expf(s[g] - m);
-      ps[g][tid] = s[g];
-      const float l = warp_sum(s[g]);
-      if (lane == 0) total[warp][g] = l;
+      top[g] = m;
+      const float p = s[g] == -INFINITY ? 0.f : expf(s[g] - m);
+      sum[g] = fmaf(sum[g], lower[g], p);   // (of the lane's keys; either half has them)
+      if (half == 0) ps[warp][key][g] = p;
+#pragma unroll
+      for (int i = 0; i < QUADS; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][e][g] *= lower[g];
     }
-    __syncthreads();
+    __syncwarp();
 #pragma unroll
-    for (int g = 0; g < HEADS; ++g)
-      if (tid == g) {
-        float l = 0.f;
+    for (int i = 0; i < QUADS; ++i) {
+      const int u = SHARE > 1 ? lane % (8 * UNITS) >> 3 : (lane + 32 * i) >> 3;
+      if (u >= UNITS || part >= SHARE) continue;
 #pragma unroll
-        for (int x = 0; x < THREADS / 32; ++x) l += total[x][g];
-        sum[g] = sum[g] * lower[g] + l;
-        top[g] = most[g];
-      }
-    const int count = min(THREADS, keys.end - j0);
+      for (int x = 0; x < 16 / SHARE; ++x) {   // word x / 4's token x % 4
+        const int c = x >> 2, tok = 2 * (c + part * (4 / SHARE)) + (x & 1) + 8 * ((x >> 1) & 1), j = t * 16 + tok;
+        const unsigned word = (x & 2 ? vw[i][c].y : vw[i][c].x) >> (16 * (x & 1));
+        const unsigned* const sz = reinterpret_cast<const unsigned*>(vt + (size_t)ROW * PAGE) + (in_page + tok) * GROUPS;
+        const bool there = j >= keys.first && j < keys.end;   // (what is out of sight may be anything)
+        const int g0 = 32 * u / BG, g1 = min(GROUPS - 1, (32 * u + 16) / BG);
+        const GroupCode a = unpack_code(there ? sz[g0] : 0u), b = BG >= 32 ? a : unpack_code(there ? sz[g1] : 0u);
+        const float v[4] = {value_of(word & 15u, a), value_of(word >> 4 & 15u, a), value_of(word >> 8 & 15u, b), value_of(word >> 12 & 15u, b)};
 #pragma unroll
-    for (int i = 0; i < DIMS; ++i) {
-      const int x = tid + i * THREADS;
+        for (int g = 0; g < HEADS; ++g) {
+          const float p = ps[warp][tok][g];
 #pragma unroll
-      for (int g = 0; g < HEADS; ++g) acc[i][g] *= lower[g];
-      if (x < D)
-        for (int t = 0; t < count; ++t) {
-          const int key = j0 + t;
-          const unsigned char* vt = v_pages + ((size_t)pages[key / PAGE] * n_kv + w.head) * TILE;
-          const unsigned word = *reinterpret_cast<const unsigned short*>(vt + kv4_value_at(key % PAGE, (x & 15) >> 1, x >> 5, UNITS));
-          const unsigned sz = reinterpret_cast<const unsigned*>(vt + (size_t)ROW * PAGE)[(key % PAGE) * GROUPS + x / BG];
-          const float v = value_of(word >> (8 * ((x >> 4) & 1) + 4 * (x & 1)) & 15u, unpack_code(sz));
-#pragma unroll
-          for (int g = 0; g < HEADS; ++g) acc[i][g] = fmaf(ps[g][t], v, acc[i][g]);
+          for (int e = 0; e < 4; ++e) acc[i][e][g] = fmaf(p, v[e], acc[i][e][g]);
         }
+      }
+    }
+    __syncwarp();
+  }
+  // the warps' sums on the block's maximum, in their order
+#pragma unroll
+  for (int g = 0; g < HEADS; ++g) {
+#pragma unroll
+    for (int x = 1; x < 16; x <<= 1) sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], x);
+    if (lane == 0) {
+      tops[warp][g] = top[g];
+      sums[warp][g] = sum[g];
+    }
+    if constexpr (SHARE > 1) {
+#pragma unroll
+      for (int x = 16; x >= 8 * UNITS; x >>= 1)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[0][e][g] += __shfl_xor_sync(0xffffffffu, acc[0][e][g], x);
     }
   }
   __syncthreads();
+  float total[HEADS];
+#pragma unroll
+  for (int g = 0; g < HEADS; ++g) {
+    float m = LOWEST, l = 0.f;
+#pragma unroll
+    for (int x = 0; x < F32_WARPS; ++x) m = fmaxf(m, tops[x][g]);
+#pragma unroll
+    for (int x = 0; x < F32_WARPS; ++x) l = fmaf(sums[x][g], tops[x][g] == m ? 1.f : expf(tops[x][g] - m), l);
+    const float by = top[g] == m ? 1.f : expf(top[g] - m);
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][e][g] *= by;
+    top[g] = m;
+    total[g] = l;
+  }
+#pragma unroll 1
+  for (int x = 0; x < F32_WARPS; ++x) {
+    if (warp == x)
+#pragma unroll
+      for (int i = 0; i < QUADS; ++i) {
+        const int at = SHARE > 1 ? lane % (8 * UNITS) : lane + 32 * i, r = at & 7, u = at >> 3;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int dim = 16 * (2 * u + (e >> 1)) + 2 * r + (e & 1);
+          if (dim >= D || part > 0) continue;
+#pragma unroll
+          for (int g = 0; g < HEADS; ++g) qs[g][dim] = x == 0 ? acc[i][e][g] : qs[g][dim] + acc[i][e][g];
+        }
+      }
+    __syncthreads();
+  }
+#pragma unroll
   for (int g = 0; g < HEADS; ++g) {
     if (g >= heads) break;
-#pragma unroll
-    for (int i = 0; i < DIMS; ++i) {
-      const int x = tid + i * THREADS;
-      if (x >= D) continue;
-      float a = 0.f;
-#pragma unroll
-      for (int e = 0; e < HEADS; ++e) a = e == g ? acc[i][e] : a;
+    for (int x = tid; x < D; x += F32_WARPS * 32) {
       if (splits == 1)
-        out[(head0 + g) * D + x] = a / sum[g];
+        out[(head0 + g) * D + x] = qs[g][x] / total[g];
       else
-        part_o[((head0 + g) * splits + w.split) * D + x] = a;
+        part_o[((head0 + g) * splits + w.split) * D + x] = qs[g][x];
     }
     if (splits > 1 && tid == 0) {
       part_ml[((head0 + g) * splits + w.split) * 2] = top[g] * 1.4426950408889634f;   // in powers of two, as the join takes them
-      part_ml[((head0 + g) * splits + w.split) * 2 + 1] = sum[g];
+      part_ml[((head0 + g) * splits + w.split) * 2 + 1] = total[g];
     }
   }
 }
@@ -637,7 +696,7 @@ template <typename T> int join(const Args& a) {
 }
 
 int rows_f32(const Args& a) {
-  const int rc = launch(attn4_f32_kernel, grid_of(a), THREADS, 0, 1, false, a.st, (const float*)a.q, (const unsigned char*)a.k_pages, (const unsigned char*)a.v_pages,
+  const int rc = launch(attn4_f32_kernel, grid_of(a), F32_WARPS * 32, 0, 1, false, a.st, (const float*)a.q, (const unsigned char*)a.k_pages, (const unsigned char*)a.v_pages,
                         a.page_table, a.max_pages, a.tok_slot, a.tok_pos, (float*)a.out, a.part_o, a.part_ml, a.scale, a.window);
   return rc || a.splits == 1 ? rc : join<float>(a);
 }

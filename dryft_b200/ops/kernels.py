@@ -2627,8 +2627,9 @@ LINEAR4_NORM_ROWS = 4
 _LINEAR4_MODES = {"store": 0, "residual": 2, "silu": 3}
 
 
-def linear4(x, w: Weight4, out, pdl: bool = False, mode: str = "store", norm_w=None, eps: float = 0.0) -> None:
-    """``out = x @ w.T``; ``x`` bfloat16, up to 256 rows (float32: 64), ``out`` of the same type or float32.  ``pdl``: a programmatic dependent (its
+def linear4(x, w: Weight4, out=None, pdl: bool = False, mode: str = "store", norm_w=None, eps: float = 0.0, out_dtype=None):
+    """``out = x @ w.T``; ``x`` bfloat16, up to 256 rows (float32: 64), ``out`` of the same type or float32 (none: a new tensor, of ``out_dtype`` or ``x``'s
+    type).  Returns ``out``.  ``pdl``: a programmatic dependent (its
     first weights are requested while the launch before it drains).
 
     With few rows of bfloat16 (``linear4_fuses``) also what stands around a decoder's products: ``norm_w`` (float32 ``[k]``): RMS norm of ``x`` first;
@@ -2641,6 +2642,10 @@ def linear4(x, w: Weight4, out, pdl: bool = False, mode: str = "store", norm_w=N
     is_bf16 = _act(x, "x")
     if m > (LINEAR4_ROWS if is_bf16 else LINEAR4_ROWS_F32):
         raise KernelError(f"linear4 takes up to {LINEAR4_ROWS} rows ({LINEAR4_ROWS_F32} of float32), got {m}")
+    given = out is not None
+    if not given:
+        cols = w.n // 2 if mode == "silu" else w.n
+        out = x.new_empty((m, cols)) if out_dtype is None or out_dtype is x.dtype else torch.empty((m, cols), dtype=out_dtype, device=x.device)
     out_bf16 = _act(out, "out")
     if out_bf16 and not is_bf16:
         raise KernelError("linear4: 32-bit activations give 32-bit results")
@@ -2652,7 +2657,8 @@ def linear4(x, w: Weight4, out, pdl: bool = False, mode: str = "store", norm_w=N
             raise KernelError(f"linear4: norms, sums and activations are for few rows of bfloat16, halves of whole tiles; got {m} rows, {tuple(w.shape)}, mode {mode}")
         if norm_w is not None:
             _need(norm_w, "norm weight", torch.float32, (w.k,))
-    _need(out, "out", None, (m, w.n // 2 if code == 3 else w.n))
+    if given:
+        _need(out, "out", None, (m, w.n // 2 if code == 3 else w.n))
     floats = linear4_plan(m, w.n, w.k, w.group, bool(is_bf16))
     if floats:
         if _linear4_tc_fn is None:
@@ -2668,6 +2674,7 @@ def linear4(x, w: Weight4, out, pdl: bool = False, mode: str = "store", norm_w=N
     if rc:
         _ok(rc, "linear4")
     launch_count += 1
+    return out
 
 
 def weight4_expand(w: Weight4, out, rest: bool = False) -> None:
@@ -2680,6 +2687,17 @@ def weight4_expand(w: Weight4, out, rest: bool = False) -> None:
         raise KernelError("weight4_expand: the rest of a rounding is bfloat16")
     _ok(linear4_lib().dryft_weight4_expand(2 if rest else is_bf16, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), w.n, w.k, w.group, _stream()),
         "weight4_expand")
+
+
+_kv4_fns = None   # (store, expand)
+
+
+def _kv4_calls():
+    global _kv4_fns
+    if _kv4_fns is None:
+        lib = kv4_lib()
+        _kv4_fns = (lib.dryft_kv4_store, lib.dryft_kv4_expand)
+    return _kv4_fns
 
 
 def kv4_lib() -> ctypes.CDLL:
@@ -2742,18 +2760,22 @@ def kv4_store(k, v, tok_slot, tok_pos, k_pages, v_pages, page_table, group: int)
     heads, page = _kv4_pages(k_pages, v_pages, page_table, d, group)
     if heads != n_kv:
         raise KernelError(f"kv4_store: {n_kv} key heads, the pages have {heads}")
+    is_bf16, apart = _act(k, "k"), n_kv * d
     for t, nm in ((k, "k"), (v, "v")):
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise KernelError(f"{nm}: is on {t.device}; dryft_b200 kernels run on a CUDA device only")
-        if t.stride(2) != 1 or (n_kv > 1 and t.stride(1) != d):
+        rows, heads, one = t.stride()
+        if one != 1 or (n_kv > 1 and heads != d):
             raise KernelError(f"{nm}: a token's heads follow one another (strides {t.stride()})")
-        if t.data_ptr() % 16 or (n > 1 and (t.stride(0) * t.element_size()) % 16):
+        if t.data_ptr() % 16 or (n > 1 and rows * (2 if is_bf16 else 4) % 16):
             raise KernelError(f"{nm}: rows start on 16-byte boundaries")
-    if n > 1 and k.stride(0) != v.stride(0):
-        raise KernelError("kv4_store: k and v rows lie equally far apart")
+        if n > 1:
+            if t is v and rows != apart:
+                raise KernelError("kv4_store: k and v rows lie equally far apart")
+            apart = rows
     _tokens(tok_slot, tok_pos, n, "kv4_store")
-    _ok(kv4_lib().dryft_kv4_store(_act(k, "k"), _ptr(k), _ptr(v), k.stride(0) if n > 1 else n_kv * d, _ptr(tok_slot), _ptr(tok_pos), _ptr(k_pages), _ptr(v_pages),
-                                  _ptr(page_table), page_table.shape[1], n, n_kv, d, group, page, _stream()), "kv4_store")
+    _ok(_kv4_calls()[0](is_bf16, k.data_ptr(), v.data_ptr(), apart, tok_slot.data_ptr(), tok_pos.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                        page_table.data_ptr(), page_table.shape[1], n, n_kv, d, group, page, _stream()), "kv4_store")
 
 
 def kv4_rope_store(qkv, q_norm_w, k_norm_w, inv_freq, tok_slot, tok_pos, q_out, k_pages, v_pages, page_table, n_heads: int, n_kv_heads: int,
@@ -2795,18 +2817,29 @@ def kv4_expand(k_pages, v_pages, page_table, cu_q, seq_slot, tok_pos, k_out, v_o
         raise KernelError("kv4_expand: k_out is [pages, kv heads, page, head size]")
     d = k_out.shape[3]
     n_kv, page = _kv4_pages(k_pages, v_pages, page_table, d, group)
-    _need(k_out, "k_out", None, (k_pages.shape[0], n_kv, page, d))
-    _need(v_out, "v_out", k_out.dtype, tuple(k_out.shape))
-    for t, nm in ((cu_q, "cu_q"), (seq_slot, "seq_slot"), (tok_pos, "tok_pos")):
-        _need(t, nm, torch.int32)
+    shape, ints = k_out.shape, torch.int32
+    try:
+        fine = (shape[0] == k_pages.shape[0] and shape[1] == n_kv and shape[2] == page and v_out.shape == shape and v_out.dtype is k_out.dtype and k_out.is_cuda
+                and v_out.is_cuda and k_out.is_contiguous() and v_out.is_contiguous() and cu_q.is_cuda and seq_slot.is_cuda and tok_pos.is_cuda
+                and cu_q.dtype is ints and seq_slot.dtype is ints and tok_pos.dtype is ints and cu_q.is_contiguous() and seq_slot.is_contiguous()
+                and tok_pos.is_contiguous())
+    except AttributeError:
+        fine = False
+    if not fine:   # what is wrong
+        _need(k_out, "k_out", None, (k_pages.shape[0], n_kv, page, d))
+        _need(v_out, "v_out", k_out.dtype, tuple(shape))
+        for t, nm in ((cu_q, "cu_q"), (seq_slot, "seq_slot"), (tok_pos, "tok_pos")):
+            _need(t, nm, ints)
     n = seq_slot.numel()
     if cu_q.numel() < n + 1:
         raise KernelError("kv4_expand: cu_q is shorter than the sequences")
     if n > 65535:
         raise KernelError(f"kv4_expand takes up to 65,535 sequences, got {n}")
-    pages = min((max_kv + page - 1) // page, page_table.shape[1]) if max_kv > 0 else page_table.shape[1]
-    _ok(kv4_lib().dryft_kv4_expand(_act(k_out, "k_out"), _ptr(k_pages), _ptr(v_pages), _ptr(page_table), page_table.shape[1], _ptr(cu_q), _ptr(seq_slot),
-                                   _ptr(tok_pos), _ptr(k_out), _ptr(v_out), n, pages, n_kv, d, group, page, int(window or 0), _stream()), "kv4_expand")
+    pages = most = page_table.shape[1]
+    if max_kv > 0:
+        pages = min((max_kv + page - 1) // page, most)
+    _ok(_kv4_calls()[1](_act(k_out, "k_out"), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), most, cu_q.data_ptr(), seq_slot.data_ptr(),
+                        tok_pos.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), n, pages, n_kv, d, group, page, int(window or 0), _stream()), "kv4_expand")
 
 
 def attn4_lib(head_dim: int, heads: int, page: int, group: int) -> ctypes.CDLL:
@@ -2844,10 +2877,13 @@ def attn4_plan(blocks: int, max_kv: int, window: Optional[int], bf16: bool) -> T
     More blocks than multiprocessors are cut only where sequences are long, and may differ in length: 1,024 keys a split, joined by a second launch (64 rows
     of up to 8,192 keys, eight key heads of 128: 98 us, as clusters of eight 153, in one split 128, two 116).  Fewer are cut as far as they fill the multiprocessors, the splits a
     cluster: a split costs its block about 3 us, so it has 1,024 keys (of few rows 256) at least (eight rows of 8,000 keys: 29 us in two splits, 50 in one; of
-    650 keys 8.6 and 7.9; one row of 4,000 keys: 9.1 in eight, 11.6 in four; 64 query heads, 16,383 keys: 17.9 in sixteen, 18.4 in eight)."""
+    650 keys 8.6 and 7.9; one row of 4,000 keys: 9.1 in eight, 11.6 in four; 64 query heads, 16,383 keys: 17.9 in sixteen, 18.4 in eight).
+
+    In 32 bits a split has 128 keys at least, a tile a warp, and the blocks are two a multiprocessor at most (two key heads of 64, one row of 700 keys: 9.2 us in
+    six splits, 16.2 in one, 10.7 in eleven; 16 rows of 2,000 keys: 15.3 in eight, 21.1 in sixteen; 100 keys: 6.5 in one, 8.4 in two)."""
     keys = max(1, min(max_kv, window) if window else max_kv)
     if not bf16:
-        return max(1, min(32, 296 // max(1, blocks), (keys + 63) // 64)), 1, 4, False
+        return max(1, min(32, 296 // max(1, blocks), keys // 128)), 1, 8, False
     if blocks > 148:
         return (min(64, (keys + 1023) // 1024), 64, 4, False) if keys > 2048 else (1, 1, 4, False)
     s = max(1, min(ATTN4_CLUSTER, 148 // max(1, blocks), keys // (256 if blocks <= 16 else 1024)))

@@ -78,11 +78,11 @@ EXPAND_BYTES = 256 << 20   # of weights at a time that a product of many rows ta
 def _linear4(x: torch.Tensor, w: K.Weight4, rt: Runtime, out_dtype: torch.dtype) -> torch.Tensor:
     """Up to ``K.LINEAR4_ROWS`` rows the kernels read the codes; more rows take the weights out of their 4 bits, for the product that such rows run on
     otherwise.  For 32-bit results from bfloat16 activations the weights are taken out as two bfloat16 numbers whose sum they are, with a product each."""
-    m, (n, k) = x.shape[0], w.shape
-    out = torch.empty((m, n), dtype=out_dtype, device=x.device)
+    m = x.shape[0]
     if m <= (K.LINEAR4_ROWS if x.dtype == torch.bfloat16 else K.LINEAR4_ROWS_F32):
-        K.linear4(x, w, out, pdl=rt.pdl)
-        return out
+        return K.linear4(x, w, pdl=rt.pdl, out_dtype=out_dtype)
+    n, k = w.shape
+    out = torch.empty((m, n), dtype=out_dtype, device=x.device)
     step = max(16, EXPAND_BYTES // (k * x.element_size()) // 16 * 16)
     buf = torch.empty((min(step, n), k), dtype=x.dtype, device=x.device)
     for first in range(0, n, step):
