@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(256) weight4_expand_kernel(const uint4* __rest
 
 // ---------------------------------------------------------------------------------------------- bfloat16: tensor cores
 // y^T = W x^T on mma.sync.m16n8k16: 16 rows of W are the 16-row operand, straight from the codes (16 + c, `code_pair`), eight rows of x the columns.  A group's
-// products are summed over 16 + c in a 32-bit accumulator of their own, then  y += s acc + (z - 23.5 s) sum_k x  in 32 bits, so nothing is rounded below
+// products are summed over 16 + c from zero (a constant that no instruction has to put there), then  y += s acc + (z - 23.5 s) sum_k x  in 32 bits, so nothing is rounded below
 // 32 bits before the result.  The warps of a block share a tile's inputs: each walks its own blocks of 64, their sums meet in shared memory.
 typedef __nv_bfloat16 bf16;
 
@@ -128,7 +128,9 @@ __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_gro
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N)); }
 __device__ __forceinline__ unsigned word_of(uint4 v, int s) { return s == 0 ? v.x : s == 1 ? v.y : s == 2 ? v.z : v.w; }
 
-// Few rows of x (up to 16), all of whose numbers fit in shared memory: bound by the codes' bytes.  A block of 16 warps is 16 / TEAM teams; a team takes
+// Few rows of x (up to 16), all of whose numbers fit in shared memory.  Bound by issue: a slot of 128 inputs is 200 instructions of a warp, half of them on the
+// pipe for logic (which takes one every other cycle, 64% busy); the 64 that take the codes apart are a third of all.  One row, 151,936 outputs of 2,560 inputs: 56 us,
+// 3,900 GB/s, 60% of a copy's rate; 6,144 outputs 4.7 us, 19,456 9.9 us, of which some 3 us are the launch and the first bytes' way.  A block of 16 warps is 16 / TEAM teams; a team takes
 // a tile of 16 rows of W at a time, its warps the tile's inputs in turn shares.  Each warp copies its own share of the codes into its own ring, SLOTS - 1 slots of
 // PB blocks of 64 inputs ahead, across the ends of tiles, so that the requests never drain; a lane reads what it copied itself, and nothing waits for another warp
 // but a tile's end.
@@ -142,7 +144,7 @@ template <int NT, int GS, int TEAM, int PB, int SLOTS> struct Few {
   __host__ __device__ static int slots_of(int k) { return blocks_of(k) / PB; }   // of a tile
   // rows of x lie 32 bytes further apart than a multiple of 128, which keeps a warp's reads of eight rows apart
   __host__ __device__ static int row_bytes(int k) { return blocks_of(k) * 128 + 32; }
-  static size_t bytes(int m, int k) { return RED_BYTES + RING_BYTES + (size_t)slots_of(k) * SCALES * NT * 64 + (size_t)m * row_bytes(k); }
+  static size_t bytes(int m, int k) { return RED_BYTES + RING_BYTES + (size_t)slots_of(k) * SCALES * NT * 32 + (size_t)m * row_bytes(k); }
 };
 
 // What stands around the product in a decoder's layer is done on its way (rounding points as in gemm_decode.cu):
@@ -151,30 +153,33 @@ template <int NT, int GS, int TEAM, int PB, int SLOTS> struct Few {
 enum Mode { STORE_BF16 = 0, STORE_F32 = 1, RESIDUAL = 2, SILU = 3 };
 __device__ __forceinline__ float bfr(float v) { return rnd<bf16>(v); }
 
-template <int NT, int GS, int TEAM, int PB, int SLOTS>
+// ALONE: no norm, and the result is stored (one row, 151,936 outputs of 2,560 inputs: 56.2 us so, 57.9 where the kernel asks what to do)
+template <int NT, int GS, int TEAM, int PB, int SLOTS, bool ALONE>
 __global__ void __launch_bounds__(FEW_WARPS * 32, 1) linear4_few_kernel(const bf16* x, long long x_stride, const uint4* __restrict__ codes,
-                                                                        const uint2* __restrict__ scales, void* y, int m, int n, int k, int group_bits, int mode,
+                                                                        const uint2* __restrict__ scales, void* y, int m, int n, int k, int group_bits, int how,
                                                                         const float* __restrict__ norm_w, float eps) {
+  const int mode = ALONE && how != STORE_F32 ? STORE_BF16 : how;
+  const bool fused_silu = !ALONE && mode == SILU;
   typedef Few<NT, GS, TEAM, PB, SLOTS> F;
   constexpr int SCALES = F::SCALES, SLOT = F::SLOT, TEAMS = FEW_WARPS / TEAM, STEPS = PB * 4 / SCALES;
   extern __shared__ __align__(16) unsigned char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3, team = warp / TEAM;
   const int tiles = (n + 15) / 16, slots = F::slots_of(k), row_bytes = F::row_bytes(k);
   float* const red = reinterpret_cast<float*>(smem);
-  float4* const xs = reinterpret_cast<float4*>(smem + F::RED_BYTES);   // [slot][SCALES][NT][c]: sums of columns 2c, 2c + 1 over the group, -23.5 times them
+  float2* const xs = reinterpret_cast<float2*>(smem + F::RED_BYTES);   // [slot][SCALES][NT][c]: sums of columns 2c, 2c + 1 over the group
   unsigned char* const rings = reinterpret_cast<unsigned char*>(xs + slots * SCALES * NT * 4);
   unsigned char* const rows = rings + F::RING_BYTES;
   const int per = (slots + TEAM - 1) / TEAM, s0 = min(slots, warp % TEAM * per), ns = min(slots, s0 + per) - s0;
   // the team's tiles: block and team together count through them, the block's number first
-  const int half = mode == SILU ? tiles / 2 : 0, turns = mode == SILU ? half : tiles;   // a turn: a tile, or a gate tile and the one `half` tiles behind it
-  const int first = blockIdx.x + team * gridDim.x, step = gridDim.x * TEAMS, mine = (first < turns ? (turns - 1 - first) / step + 1 : 0) * (mode == SILU ? 2 : 1);
+  const int half = fused_silu ? tiles / 2 : 0, turns = fused_silu ? half : tiles;   // a turn: a tile, or a gate tile and the one `half` tiles behind it
+  const int first = blockIdx.x + team * gridDim.x, step = gridDim.x * TEAMS, mine = (first < turns ? (turns - 1 - first) / step + 1 : 0) * (fused_silu ? 2 : 1);
   const int total = mine * ns;   // the warp's slots
 
   // Slot i of the warp goes into place i mod SLOTS of its ring.  Codes and scales lie slot behind slot, tile behind tile.  (A group of 128 has two slots of one
   // block: the scale is then the same for both.)
   int sent = 0, until = ns;
   unsigned at = first * slots + s0;
-  unsigned jump = mode == SILU ? half * slots - ns : step * slots - ns;   // from a tile's last slot to the next tile's first one
+  unsigned jump = fused_silu ? half * slots - ns : step * slots - ns;   // from a tile's last slot to the next tile's first one
   const unsigned jumps = step * slots - 2 * ns;                           // SILU: of the two jumps of a turn
   const unsigned ring = (unsigned)__cvta_generic_to_shared(rings + warp * F::RING_BYTES / FEW_WARPS) + lane * 16;
   const unsigned ring_scales = ring - lane * 8 + PB * 512;
@@ -194,7 +199,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) linear4_few_kernel(const bf
       if (--until == 0) {
         until = ns;
         at += jump;
-        if (mode == SILU) jump = jumps - jump;
+        if (fused_silu) jump = jumps - jump;
       }
     }
     ++sent;
@@ -216,7 +221,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) linear4_few_kernel(const bf
   copies_end();
   copies_wait<0>();
   __syncthreads();
-  if (norm_w != nullptr) {   // the warps share the rows, or a row
+  if (!ALONE && norm_w != nullptr) {   // the warps share the rows, or a row
     const int wr = m == 1 ? 16 : m == 2 ? 8 : m <= 4 ? 4 : m <= 8 ? 2 : 1, row = warp / wr, part = warp % wr;
     unsigned char* const at_x = rows + (size_t)row * row_bytes;
     float ss = 0.f;
@@ -270,7 +275,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) linear4_few_kernel(const bf
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       const float a = __shfl_sync(0xffffffffu, sum, 8 * c), b = __shfl_sync(0xffffffffu, sum, 8 * c + 4);
-      if (r == 0) xs[(i * NT + j) * 4 + c] = make_float4(a, b, -CODE_BIAS * a, -CODE_BIAS * b);
+      if (r == 0) xs[(i * NT + j) * 4 + c] = make_float2(a, b);
     }
   __syncthreads();
 
@@ -293,7 +298,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) linear4_few_kernel(const bf
       acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
     }
     asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(TEAM * 32) : "memory");
-    const int turn = mode == SILU ? tile >> 1 : tile, row = (first + turn * step) * 16 + out_row;
+    const int turn = fused_silu ? tile >> 1 : tile, row = (first + turn * step) * 16 + out_row;
 #pragma unroll
     for (int i = 0; i < OUTS; ++i) {
       const int col = out_col + i * (TEAM * 2);
@@ -306,7 +311,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) linear4_few_kernel(const bf
       bf16* const to = reinterpret_cast<bf16*>(y) + (size_t)col * n + row;
       if (mode == STORE_BF16) {
         *to = __float2bfloat16_rn(v);
-      } else if (mode == STORE_F32) {
+      } else if (ALONE || mode == STORE_F32) {
         reinterpret_cast<float*>(y)[(size_t)col * n + row] = v;
       } else if (mode == RESIDUAL) {
         *to = __float2bfloat16_rn(ld_prev_bf16(to) + bfr(v));
@@ -332,18 +337,18 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) linear4_few_kernel(const bf
       uint4 w[PB];
 #pragma unroll
       for (int b = 0; b < PB; ++b) w[b] = *reinterpret_cast<const uint4*>(from + b * 512 + lane * 16);
-      const float4* const my_xs = xs + here * (SCALES * NT * 4) + c;
+      const float2* const my_xs = xs + here * (SCALES * NT * 4) + c;
 #pragma unroll
       for (int g = 0; g < SCALES; ++g) {
         const uint2 sz = *reinterpret_cast<const uint2*>(from + PB * 512 + g * 256 + lane * 8);
         const GroupCode lo = unpack_code(sz.x), hi = unpack_code(sz.y);
-        float4 sum[NT];
+        float2 sum[NT];
         float part[NT][4];
+        const float lo_z = fmaf(-CODE_BIAS, lo.s, lo.z), hi_z = fmaf(-CODE_BIAS, hi.s, hi.z);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           sum[j] = my_xs[(g * NT + j) * 4];
-          part[j][0] = part[j][2] = sum[j].z;    // the products are summed on top of what takes the 23.5 out
-          part[j][1] = part[j][3] = sum[j].w;
+          part[j][0] = part[j][1] = part[j][2] = part[j][3] = 0.f;
         }
 #pragma unroll
         for (int q = g * STEPS; q < (g + 1) * STEPS; ++q) {
@@ -356,10 +361,10 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) linear4_few_kernel(const bf
         }
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          acc[j][0] = fmaf(lo.s, part[j][0], fmaf(lo.z, sum[j].x, acc[j][0]));
-          acc[j][1] = fmaf(lo.s, part[j][1], fmaf(lo.z, sum[j].y, acc[j][1]));
-          acc[j][2] = fmaf(hi.s, part[j][2], fmaf(hi.z, sum[j].x, acc[j][2]));
-          acc[j][3] = fmaf(hi.s, part[j][3], fmaf(hi.z, sum[j].y, acc[j][3]));
+          acc[j][0] = fmaf(lo.s, part[j][0], fmaf(lo_z, sum[j].x, acc[j][0]));
+          acc[j][1] = fmaf(lo.s, part[j][1], fmaf(lo_z, sum[j].y, acc[j][1]));
+          acc[j][2] = fmaf(hi.s, part[j][2], fmaf(hi_z, sum[j].x, acc[j][2]));
+          acc[j][3] = fmaf(hi.s, part[j][3], fmaf(hi_z, sum[j].y, acc[j][3]));
         }
       }
       if (++here == s0 + ns) {
@@ -407,26 +412,27 @@ struct Args {
   cudaStream_t st;
 };
 
-template <int NT, int GS, int TEAM, int PB, int SLOTS> int few(const Args& a) {
+template <int NT, int GS, int TEAM, int PB, int SLOTS, bool ALONE> int few(const Args& a) {
   static bool asked[64] = {false};
   const int tiles = (a.n + 15) / 16, turns = a.mode == SILU ? tiles / 2 : tiles;
-  return launch(linear4_few_kernel<NT, GS, TEAM, PB, SLOTS>, asked, turns < 148 ? turns : 148, FEW_WARPS * 32, Few<NT, GS, TEAM, PB, SLOTS>::bytes(a.m, a.k), a.pdl, a.st,
+  return launch(linear4_few_kernel<NT, GS, TEAM, PB, SLOTS, ALONE>, asked, turns < 148 ? turns : 148, FEW_WARPS * 32, Few<NT, GS, TEAM, PB, SLOTS>::bytes(a.m, a.k), a.pdl, a.st,
                 (const bf16*)a.x, a.x_stride, (const uint4*)a.codes, (const uint2*)a.scales, a.y, a.m, a.n, a.k, __builtin_ctz(a.group), a.mode, a.norm_w, a.eps);
 }
 // Four warps a tile where shared memory has room for their rings (x of 8 rows: up to about 6,000 inputs), else all sixteen with shorter rings.  2,560 inputs,
 // one row, four / eight / sixteen warps a tile: 151,936 outputs 55.6 / 63.6 / 81.9 us, 6,144 outputs 4.8 / 5.4 / 5.7 us (a tile's end costs each warp as much as
 // half a slot); 2,560 outputs of 9,728 inputs, hardly more tiles than multiprocessors, 9.6 / 9.7 / 10.2 us.
-template <int NT, int GS> int few_rows(const Args& a) {
+template <int NT, int GS, bool ALONE> int few_rows(const Args& a) {
   constexpr int GM = GS == 8 ? 4 : GS;
-  if (Few<NT, GS, 4, 2, 4>::bytes(a.m, a.k) <= SMEM_MOST) return few<NT, GS, 4, 2, 4>(a);
-  return few<NT, GM, 16, 1, 4>(a);
+  if (Few<NT, GS, 4, 2, 4>::bytes(a.m, a.k) <= SMEM_MOST) return few<NT, GS, 4, 2, 4, ALONE>(a);
+  return few<NT, GM, 16, 1, 4, ALONE>(a);
 }
 template <int NT> bool fits(int m, int k, int group) {
   return (group >= 64 ? Few<NT, 4, 16, 1, 4>::bytes(m, k) : group == 32 ? Few<NT, 2, 16, 1, 4>::bytes(m, k) : Few<NT, 1, 16, 1, 4>::bytes(m, k)) <= SMEM_MOST;
 }
 bool takes(int m, int k, int group) { return m <= 8 ? fits<1>(m, k, group) : m <= 16 && fits<2>(m, k, group); }
 
-template <int GS> int by_rows(const Args& a) { return a.m <= 8 ? few_rows<1, GS>(a) : few_rows<2, GS>(a); }
+template <int GS, bool ALONE> int by_mode(const Args& a) { return a.m <= 8 ? few_rows<1, GS, ALONE>(a) : few_rows<2, GS, ALONE>(a); }
+template <int GS> int by_rows(const Args& a) { return a.mode <= STORE_F32 && a.norm_w == nullptr ? by_mode<GS, true>(a) : by_mode<GS, false>(a); }
 }  // namespace
 
 // Whether the kernel for few rows of bfloat16 takes so many rows of so many inputs (they have to fit in shared memory).
