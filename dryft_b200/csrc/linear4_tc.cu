@@ -114,10 +114,13 @@ __device__ __forceinline__ unsigned block_of(unsigned U, unsigned G, unsigned u)
 // 16 rows of W of one block of a unit by a warp, into the operand: rows r and r + 8, four inputs (8 bytes) of each of four steps.
 template <int GN, bool LOW, int KU> __device__ __forceinline__ void take_out(unsigned char* to, int block, int row0, uint4 raw, const uint2 (&sz)[GN]) {
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const unsigned words[4] = {raw.x, raw.y, raw.z, raw.w};
+  // Odd rows take the steps in the order 2, 3, 0, 1 where the block has one scale a row: the swizzle puts a step's 32 bytes of rows r and r + 1 at the same banks.
+  constexpr bool TURN = GN <= KU;
+  const bool odd = TURN && (r & 1);
+  const unsigned words[4] = {odd ? raw.z : raw.x, odd ? raw.w : raw.y, odd ? raw.x : raw.z, odd ? raw.y : raw.w};
   const __nv_bfloat162 less = __floats2bfloat162_rn(-CODE_BIAS, -CODE_BIAS);
   // row (r or r + 8), 16-byte chunk 2s + c / 2, which the swizzle puts at chunk ^ (row & 7)
-  const unsigned place = smem_u32(to) + (row0 + r) * 128 + (((c >> 1) ^ r) << 4) + (c & 1) * 8;
+  const unsigned place = (smem_u32(to) + (row0 + r) * 128 + (((c >> 1) ^ r) << 4) + (c & 1) * 8) ^ (odd ? 64 : 0);
   const auto put = [](unsigned at, unsigned x, unsigned y) { asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(x), "r"(y) : "memory"); };
 #pragma unroll
   for (int s = 0; s < 4; ++s)
