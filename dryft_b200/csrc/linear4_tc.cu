@@ -19,7 +19,7 @@
 
 namespace {
 typedef __nv_bfloat16 bf16;
-constexpr int BM = 128, BK = 64, W_BYTES = BM * BK * 2, WARPS = 23, TAKERS = 16;
+constexpr int BM = 128, BK = 64, WARPS = 23, TAKERS = 16;
 constexpr long long WAIT_CYCLES = 2000000000LL;
 constexpr unsigned SLEEP_NS = 10000;   // a waiter sleeps up to so long before it asks again: asking takes issue slots from those it waits for
 
@@ -68,10 +68,16 @@ __device__ __forceinline__ unsigned long long umma_desc(const void* smem_tile) {
 }
 // kind::f16 instruction descriptor: D fp32, A and B bf16, both K-major, N >> 3 at bit 17, M >> 4 at bit 24
 __host__ __device__ constexpr unsigned idesc(int m, int n) { return (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24); }
-__device__ __forceinline__ void umma(unsigned d_tmem, unsigned long long a_desc, unsigned long long b_desc, unsigned id, unsigned accumulate) {
+// D[tmem] (+)= A[tmem] B[smem]
+__device__ __forceinline__ void umma(unsigned d_tmem, unsigned a_tmem, unsigned long long b_desc, unsigned id, unsigned accumulate) {
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-               ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(id), "r"(accumulate) : "memory");
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(id), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ bool elected() {   // one lane of the warp
+  unsigned one;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(one));
+  return one != 0;
 }
 __device__ __forceinline__ void umma_commit(void* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -89,21 +95,24 @@ __device__ __forceinline__ void tmem_ld16(unsigned taddr, float (&v)[16]) {
 
 struct Params { void* y; float* pieces; int* err; int m, n, blocks, group_bits, tiles; };
 
-// KU: blocks of 64 inputs in a unit, two where two stages of them fit: every handshake between the roles costs the same for twice the work (48 rows, 19,456
+// KU: blocks of 64 inputs in a unit, two where enough stages of x fit: every handshake between the roles costs the same for twice the work (48 rows, 19,456
 // outputs of 2,560 inputs: 28.6 us with units of 64 inputs).  GN: groups that begin in a unit.
-template <int NB, bool LOW> constexpr int units_of() { return 2 * 2 * (W_BYTES * (LOW ? 2 : 1) + NB * BK * 2) <= 176 * 1024 ? 2 : 1; }
+template <int NB> constexpr int units_of() { return NB == 256 ? 1 : 2; }
 template <int NB, int GN, bool LOW> struct Layout {
-  static constexpr int KU = units_of<NB, LOW>(), W_SIDE = W_BYTES * KU;                          // a stage: weights (LOW: and their rests), then x, block by block
-  static constexpr int X_BLOCK = NB * BK * 2, X_BYTES = X_BLOCK * KU, STAGE_BYTES = W_SIDE * (LOW ? 2 : 1) + X_BYTES;   // multiples of 1024
-  static constexpr int RING = KU == 2 ? 4 : 8;                                                    // units whose codes are on their way
+  static constexpr int KU = units_of<NB>(), X_BLOCK = NB * BK * 2, STAGE_BYTES = X_BLOCK * KU;   // a stage of x, block by block; multiples of 1024
+  static constexpr int RING = 8;                                                                 // units whose codes are on their way
   static constexpr int CODE_BYTES = 4096 * KU, SCALE_BYTES = 512 * GN, SLOT_BYTES = CODE_BYTES + SCALE_BYTES, RING_BYTES = RING * SLOT_BYTES;   // multiples of 128
-  static constexpr int ROOM = 225 * 1024 - RING_BYTES, STAGES = STAGE_BYTES * 6 <= ROOM ? 6 : ROOM / STAGE_BYTES;
+  // tensor memory: sums of ACCS runs, then the stages of weights (LOW: and of their rests), two inputs a column
+  static constexpr int ACCS = NB == 256 ? 1 : 2, W_COLS = BK / 2 * KU, STAGE_COLS = W_COLS * (LOW ? 2 : 1), W_COL0 = ACCS * NB, TMEM_COLS = 512;
+  static constexpr int ROOM = (225 * 1024 - RING_BYTES) / STAGE_BYTES, COLS = (TMEM_COLS - W_COL0) / STAGE_COLS, FIT = ROOM < COLS ? ROOM : COLS;
+  static constexpr int STAGES = FIT < 6 ? FIT : 6;
   // Teams of warps that take units' weights out in turn.  A parity tells two phases of a barrier apart, not three: a team that waits for the products of the unit that
   // had its stage before has to know that those of the unit before that are done.  It has written its last unit, TEAMS before this one, into a stage that the products
   // of the unit TEAMS + STAGES before this one had left; so TEAMS is at most STAGES.
   static constexpr int TEAMS = STAGES >= 4 ? 4 : 2, TEAM = TAKERS / TEAMS;
   static_assert(STAGES >= 2 && TEAMS <= STAGES && TEAMS <= RING, "phases of a stage's barrier");
-  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + RING_BYTES + 8 * (3 * STAGES + 2 * RING + 4) + 64, TMEM_COLS = 2 * NB;
+  static_assert(W_COL0 + STAGES * STAGE_COLS <= TMEM_COLS, "of tensor memory");
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + RING_BYTES + 8 * (3 * STAGES + 2 * RING + 4) + 64;
   static_assert(SMEM_BYTES <= 227 * 1024, "of a block");
 };
 // (32 bits: the launcher sees to U G being below 2^32)
@@ -111,46 +120,41 @@ __device__ __forceinline__ unsigned first_unit(unsigned U, unsigned G, unsigned 
 // the block that has unit u: the last one that begins at or before it
 __device__ __forceinline__ unsigned block_of(unsigned U, unsigned G, unsigned u) { return ((u + 1) * G - 1) / U; }
 
-// 16 rows of W of one block of a unit by a warp, into the operand: rows r and r + 8, four inputs (8 bytes) of each of four steps.
-template <int GN, bool LOW, int KU> __device__ __forceinline__ void take_out(unsigned char* to, int block, int row0, uint4 raw, const uint2 (&sz)[GN]) {
-  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  // Odd rows take the steps in the order 2, 3, 0, 1 where the block has one scale a row: the swizzle puts a step's 32 bytes of rows r and r + 1 at the same banks.
-  constexpr bool TURN = GN <= KU;
-  const bool odd = TURN && (r & 1);
-  const unsigned words[4] = {odd ? raw.z : raw.x, odd ? raw.w : raw.y, odd ? raw.x : raw.z, odd ? raw.y : raw.w};
+__device__ __forceinline__ void tmem_st_16x64(unsigned taddr, const unsigned (&v)[16]) {   // 16 lanes' 32 columns; a lane has rows r, r + 8 and columns 8 s + 2c, + 1
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+               ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+                 "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+}
+// 16 rows of W of one block of a unit by a warp, into tensor memory: rows r and r + 8, four inputs (two columns) of each of four steps.
+template <int GN, bool LOW, int KU> __device__ __forceinline__ void take_out(unsigned to, int block, uint4 raw, const uint2 (&sz)[GN]) {
+  const unsigned words[4] = {raw.x, raw.y, raw.z, raw.w};
   const __nv_bfloat162 less = __floats2bfloat162_rn(-CODE_BIAS, -CODE_BIAS);
-  // row (r or r + 8), 16-byte chunk 2s + c / 2, which the swizzle puts at chunk ^ (row & 7)
-  const unsigned place = (smem_u32(to) + (row0 + r) * 128 + (((c >> 1) ^ r) << 4) + (c & 1) * 8) ^ (odd ? 64 : 0);
-  const auto put = [](unsigned at, unsigned x, unsigned y) { asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(x), "r"(y) : "memory"); };
+  unsigned v[16], rest[16];
 #pragma unroll
   for (int s = 0; s < 4; ++s)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int g = (4 * block + s) * GN / (4 * KU);
       const unsigned one = h ? sz[g].y : sz[g].x;
-      const unsigned a = code_pair(words[s], h), b = code_pair(words[s], 2 + h);   // inputs 16 s + 4c, + 1 and + 2, + 3
-      const unsigned at = (place ^ (32 * s)) + 1024 * h;
-      if constexpr (!LOW) {
-        const unsigned ss = __byte_perm(one, one, 0x1010), zz = __byte_perm(one, one, 0x3232);
-        const __nv_bfloat162 s2 = *reinterpret_cast<const __nv_bfloat162*>(&ss), z2 = *reinterpret_cast<const __nv_bfloat162*>(&zz);
-        const __nv_bfloat162 x = __hfma2(__hadd2(*reinterpret_cast<const __nv_bfloat162*>(&a), less), s2, z2);
-        const __nv_bfloat162 y = __hfma2(__hadd2(*reinterpret_cast<const __nv_bfloat162*>(&b), less), s2, z2);
-        put(at, *reinterpret_cast<const unsigned*>(&x), *reinterpret_cast<const unsigned*>(&y));
-      } else {
-        const GroupCode code = unpack_code(one);
-        float v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const unsigned p = e < 2 ? a : b;
-          v[e] = fmaf(__uint_as_float(e & 1 ? p & 0xffff0000u : p << 16) - CODE_BIAS, code.s, code.z);
+      for (int e = 0; e < 2; ++e) {   // inputs 16 s + 4c + 2e, + 1
+        const unsigned pair = code_pair(words[s], 2 * e + h);
+        if constexpr (!LOW) {
+          const unsigned ss = __byte_perm(one, one, 0x1010), zz = __byte_perm(one, one, 0x3232);
+          const __nv_bfloat162 x = __hfma2(__hadd2(*reinterpret_cast<const __nv_bfloat162*>(&pair), less), *reinterpret_cast<const __nv_bfloat162*>(&ss),
+                                           *reinterpret_cast<const __nv_bfloat162*>(&zz));
+          v[4 * s + 2 * h + e] = *reinterpret_cast<const unsigned*>(&x);
+        } else {
+          const GroupCode code = unpack_code(one);
+          const float a = fmaf(__uint_as_float(pair << 16) - CODE_BIAS, code.s, code.z), b = fmaf(__uint_as_float(pair & 0xffff0000u) - CODE_BIAS, code.s, code.z);
+          const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(a - __low2float(x), b - __high2float(x));
+          v[4 * s + 2 * h + e] = *reinterpret_cast<const unsigned*>(&x);
+          rest[4 * s + 2 * h + e] = *reinterpret_cast<const unsigned*>(&y);
         }
-        const __nv_bfloat162 x = __floats2bfloat162_rn(v[0], v[1]), y = __floats2bfloat162_rn(v[2], v[3]);
-        const __nv_bfloat162 xl = __floats2bfloat162_rn(v[0] - __low2float(x), v[1] - __high2float(x));
-        const __nv_bfloat162 yl = __floats2bfloat162_rn(v[2] - __low2float(y), v[3] - __high2float(y));
-        put(at, *reinterpret_cast<const unsigned*>(&x), *reinterpret_cast<const unsigned*>(&y));
-        put(at + W_BYTES * KU, *reinterpret_cast<const unsigned*>(&xl), *reinterpret_cast<const unsigned*>(&yl));
       }
     }
+  tmem_st_16x64(to, v);
+  if constexpr (LOW) tmem_st_16x64(to + BK / 2 * KU, rest);
 }
 
 template <int NB, int GN, bool LOW>
@@ -173,7 +177,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
   __shared__ unsigned long long drained_s;
   volatile int* const failed = &failed_s;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, KB = p.blocks / KU;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, KB = p.blocks / KU;
   const int U = p.tiles * KB, u0 = first_unit(U, gridDim.x, blockIdx.x), u1 = first_unit(U, gridDim.x, blockIdx.x + 1), n_units = u1 - u0;
 
   if (threadIdx.x == 0) {
@@ -201,7 +205,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const unsigned tmem = *tmem_slot;
+  const unsigned tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   let_next_launch_in();
 
   if (warp == 0) {
@@ -211,50 +215,49 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
       for (; i < n_units; ++i) {
         const int s = i % STAGES;
         if (i >= STAGES && !mbar_wait(&empty[s], (unsigned)(((i / STAGES) - 1) & 1), p.err, failed, 1)) break;
-        mbar_expect_tx(&x_full[s], L::X_BYTES);
-        unsigned char* const to = stages + (size_t)s * L::STAGE_BYTES + (LOW ? 2 : 1) * L::W_SIDE;
+        mbar_expect_tx(&x_full[s], L::STAGE_BYTES);
+        unsigned char* const to = stages + (size_t)s * L::STAGE_BYTES;
 #pragma unroll
         for (int b = 0; b < KU; ++b) tma_load_2d(to + b * L::X_BLOCK, &map_x, ((u0 + i) % KB * KU + b) * BK, 0, &x_full[s]);
       }
       issued_s = i;
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      // (one thread's instructions are this loop's pace: stage, turn and descriptors are counted up, not worked out)
-      constexpr unsigned ID = idesc(BM, NB);
-      const unsigned long long w_desc0 = umma_desc(stages), x_desc0 = umma_desc(stages + (LOW ? 2 : 1) * L::W_SIDE);
-      bool ok = true;
-      int run = 0, s = 0, kb = u0 % KB;   // runs of one tile's units that this block has begun
-      unsigned par = 0, first = 1;
-      for (int i = 0; i < n_units; ++i) {
-        ok = mbar_wait(&w_full[s], par, p.err, failed, 2) && mbar_wait(&x_full[s], par, p.err, failed, 3);
-        if (ok && first && run >= 2) {   // the sums that this buffer held have been read
-          ok = mbar_wait(&acc_empty[run & 1], (unsigned)(((run >> 1) - 1) & 1), p.err, failed, 4);
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        }
-        if (!ok) break;
-        const unsigned long long w_desc = w_desc0 + (unsigned)(s * (L::STAGE_BYTES >> 4)), x_desc = x_desc0 + (unsigned)(s * (L::STAGE_BYTES >> 4));
-        const unsigned d = tmem + (unsigned)((run & 1) * NB);
+    // The whole warp walks the units and one lane issues: what the products are given is then the same for every lane, and stays in uniform registers.
+    constexpr unsigned ID = idesc(BM, NB);
+    const unsigned long long x_desc0 = umma_desc(stages);
+    const bool issues = elected();
+    int run = 0, s = 0, kb = u0 % KB;   // runs of one tile's units that this block has begun
+    unsigned par = 0, first = 1;
+    for (int i = 0; i < n_units; ++i) {
+      bool ok = mbar_wait(&w_full[s], par, p.err, failed, 2) && mbar_wait(&x_full[s], par, p.err, failed, 3);
+      if (ok && first && run >= L::ACCS)   // the sums that this buffer held have been read
+        ok = mbar_wait(&acc_empty[run % L::ACCS], (unsigned)((run / L::ACCS - 1) & 1), p.err, failed, 4);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const unsigned long long x_desc = x_desc0 + (unsigned)(s * (L::STAGE_BYTES >> 4));
+      const unsigned d = tmem + (unsigned)(run % L::ACCS * NB), w = tmem + L::W_COL0 + (unsigned)(s * L::STAGE_COLS);
+      const bool last = kb + 1 == KB || i == n_units - 1;
+      if (issues) {
 #pragma unroll
         for (int b = 0; b < KU; ++b)
 #pragma unroll
           for (int kk = 0; kk < BK / 16; ++kk) {
-            const unsigned long long w = w_desc + b * (W_BYTES >> 4) + kk * 2, x = x_desc + b * (L::X_BLOCK >> 4) + kk * 2;
-            umma(d, w, x, ID, b + kk > 0 ? 1u : first ^ 1u);
-            if (LOW) umma(d, w + (L::W_SIDE >> 4), x, ID, 1u);
+            const unsigned long long x = x_desc + b * (L::X_BLOCK >> 4) + kk * 2;
+            const unsigned from = w + b * (BK / 2) + kk * 8;
+            umma(d, from, x, ID, b + kk > 0 ? 1u : first ^ 1u);
+            if (LOW) umma(d, from + L::W_COLS, x, ID, 1u);
           }
         umma_commit(&empty[s]);
-        first = 0;
-        if (++kb == KB || i == n_units - 1) {
-          umma_commit(&acc_full[run & 1]);
-          ++run;
-          kb = 0;
-          first = 1;
-        }
-        if (++s == STAGES) {
-          s = 0;
-          par ^= 1;
-        }
+        if (last) umma_commit(&acc_full[run % L::ACCS]);
+      }
+      __syncwarp();
+      first = last;
+      run += last;
+      kb = last ? 0 : kb + 1;
+      if (++s == STAGES) {
+        s = 0;
+        par ^= 1;
       }
     }
   } else if (warp < 6) {
@@ -262,10 +265,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
     asm volatile("griddepcontrol.wait;" ::: "memory");
     int run = 0;
     for (int u = u0; u < u1; ++run) {
-      const int tile = u / KB, b = run & 1, begin = tile * KB, end = min(u1, begin + KB);
+      const int tile = u / KB, b = run % L::ACCS, begin = tile * KB, end = min(u1, begin + KB);
       const bool whole = u == begin && end == begin + KB;
       u = end;
-      bool ok = mbar_wait(&acc_full[b], (unsigned)((run >> 1) & 1), p.err, failed, 5);
+      bool ok = mbar_wait(&acc_full[b], (unsigned)(run / L::ACCS & 1), p.err, failed, 5);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -310,26 +313,29 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
   } else {
     // teams take the units in turn, so that one's waits and fence are another's work
     constexpr int TEAM = L::TEAM;
-    const int w = (warp - 6) % TEAM;
+    const int q = warp & 3, upper = (warp - 6) % TEAM >> 2;   // the quarter of tensor memory that this warp may write; of a team of eight, which half of it
     for (int i = (warp - 6) / TEAM; i < n_units; i += L::TEAMS) {
       const int s = i % STAGES, cs = i % RING;
       bool ok = mbar_wait(&c_full[cs], (unsigned)((i / RING) & 1), p.err, failed, 8);
       if (ok && i >= STAGES) ok = mbar_wait(&empty[s], (unsigned)(((i / STAGES) - 1) & 1), p.err, failed, 6);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const unsigned char* const from = ring + cs * L::SLOT_BYTES;
 #pragma unroll
-      for (int t = w; t < 8; t += TEAM) {   // 16 rows of W
+      for (int j = 0; j < 8 / TEAM; ++j) {   // 16 rows of W
+        const int t = 2 * q + j + upper;
         uint2 sz[GN];
 #pragma unroll
         for (int g = 0; g < GN; ++g) sz[g] = *reinterpret_cast<const uint2*>(from + L::CODE_BYTES + (t * GN + g) * 64 + (lane >> 2) * 8);
 #pragma unroll
         for (int b = 0; b < KU; ++b) {
           const uint4 raw = *reinterpret_cast<const uint4*>(from + (t * KU + b) * 512 + lane * 16);
-          take_out<GN, LOW, KU>(stages + (size_t)s * L::STAGE_BYTES + b * W_BYTES, b, 16 * t, raw, sz);
+          take_out<GN, LOW, KU>(tmem + ((unsigned)(16 * t) << 16) + (unsigned)(L::W_COL0 + s * L::STAGE_COLS + b * (BK / 2)), b, raw, sz);
         }
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the tensor core reads through the async proxy
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&w_full[s]);
@@ -346,7 +352,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
     auto expired = [&] { return clock64() - t0 > WAIT_CYCLES; };
     if (threadIdx.x == 0) ring_drain(issued_s, STAGES, [&](int s, unsigned parity) { return mbar_try_wait(&x_full[s], parity); }, expired);
     if (threadIdx.x == (6 + TAKERS) * 32) ring_drain(codes_issued_s, RING, [&](int s, unsigned parity) { return mbar_try_wait(&c_full[s], parity); }, expired);
-    if (threadIdx.x == 32) {   // the thread that issued the products
+    if (warp == 1 && elected()) {   // the thread that issued the products
       umma_commit(&drained_s);
       while (!mbar_try_wait(&drained_s, 0) && !expired()) {}
     }
@@ -463,7 +469,7 @@ template <int NB, int GN, bool LOW> int run(const Operands& o, const Params& p, 
                 units, p.tiles, G);
 }
 template <int NB, bool LOW> int by_group(const Operands& o, const Params& p, int pdl, cudaStream_t st) {
-  constexpr int WIDE = 64 * units_of<NB, LOW>();   // inputs of a unit
+  constexpr int WIDE = 64 * units_of<NB>();   // inputs of a unit
   switch (o.group) {
     case 128: return run<NB, 1, LOW>(o, p, pdl, st);
     case 64: return run<NB, WIDE / 64, LOW>(o, p, pdl, st);
