@@ -1,16 +1,22 @@
 // Products with weights held in 4 bits (four_bit.cuh, linear4.cu has their layout) for up to 256 rows of bfloat16, on the 5th-generation tensor cores.
 //
 // Computed transposed: a tile is 128 rows of W against all rows of x, padded to NB = 32, 64, 128 or 256, its 128 x NB sums in tensor memory.  A unit is
-// 64 inputs of a tile: its codes (4 KB) and scales come by TMA into a ring, eight warps take them out of their 4 bits, each 16 rows of W, into a stage
-// of shared memory as the 128 x 64 operand that tcgen05.mma reads (K-major, 128-byte swizzle); x's 64 inputs come by TMA too.  (Codes requested into registers
-// instead, four units ahead: every unit waits for them at the fence in front of the products, 1 us a unit.)  So the weights cross memory at 4.5 bits
+// 128 inputs of a tile (64 with 256 rows of x): its codes (8 KB) and scales come by TMA into a ring of eight, a team of warps takes them out of their 4 bits, 16 rows
+// of W a warp at a time, and stores them into tensor memory, where tcgen05.mma takes its first operand from: a lane's codes are rows r and r + 8 and the inputs of two
+// neighbouring columns, which is the shape 16x256b as it stands.  x comes by TMA, K-major in a 128-byte swizzle.  So the weights cross memory at 4.5 bits
 // and are multiplied as bfloat16 z + (c - 7.5) s: one rounding of 2^-9 of each weight.  For 32-bit results (LOW) the rest of that rounding is a second
 // operand with a product of its own, which leaves 2^-18.
 //
 // Work is cut evenly: block i of G takes the units [i U / G, (i + 1) U / G) in (tile, inputs) order.  A run that covers its tile's inputs is finished from tensor
 // memory; else its sums go to a workspace, and a second launch adds a tile's pieces in the blocks' order.  No block waits for another.
 //
-// Warps: 0 copies x, 1 issues the products, 22 copies codes (a thread each), 2 to 5 read the sums, 6 to 21 take weights out.  Every wait on a barrier is bounded by a clock; a
+// What bounds it: every tile reads all of x again, from L2: at 48 rows a unit is 9 KB of codes and 12 KB of x a multiprocessor every 0.5 us, 6 TB/s in all, at 128
+// rows 7 TB/s.  48 rows: 2,560 outputs of 9,728 inputs 12.6 us (of which some 3 us the launch and 3 us the join), 19,456 of 2,560 16.8 us, 151,936 of 2,560 79 us
+// (32-bit results 175); 256 rows, 19,456 of 2,560: 39 us.  (Steps on the way, 48 rows, 19,456 of 2,560: codes requested into registers, 1 us a unit of 64; weights
+// written into shared memory as the operand 22 us; into tensor memory 21.4, by then bound by the one thread that issued products, 500 cycles a unit to put their
+// operands into uniform registers; with a whole warp that walks the loop 17.5; one barrier for weights and x, asked ahead of the products before, 16.7.)
+//
+// Warps: 0 copies x, 1 issues the products, 22 copies codes (a lane each issues), 2 to 5 read the sums, 6 to 21 take weights out.  Every wait on a barrier is bounded by a clock; a
 // waiter that gives up raises *err, every role leaves its loop, the block lets its copies and products end and frees its tensor memory.
 #include "four_bit.cuh"
 #include "drain.h"
@@ -37,6 +43,11 @@ __device__ __forceinline__ bool mbar_try_wait(void* bar, unsigned parity) {
   unsigned ok;
   asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
                : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(SLEEP_NS) : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_test(void* bar, unsigned parity) {   // (does not sleep)
+  unsigned ok;
+  asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
   return ok != 0;
 }
 __device__ __forceinline__ bool mbar_wait(void* bar, unsigned parity, int* err, volatile int* failed, int site) {
@@ -112,7 +123,7 @@ template <int NB, int GN, bool LOW> struct Layout {
   static constexpr int TEAMS = STAGES >= 4 ? 4 : 2, TEAM = TAKERS / TEAMS;
   static_assert(STAGES >= 2 && TEAMS <= STAGES && TEAMS <= RING, "phases of a stage's barrier");
   static_assert(W_COL0 + STAGES * STAGE_COLS <= TMEM_COLS, "of tensor memory");
-  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + RING_BYTES + 8 * (3 * STAGES + 2 * RING + 4) + 64;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + RING_BYTES + 8 * (2 * STAGES + 2 * RING + 4) + 64;
   static_assert(SMEM_BYTES <= 227 * 1024, "of a block");
 };
 // (32 bits: the launcher sees to U G being below 2^32)
@@ -165,13 +176,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
   extern __shared__ unsigned char smem_raw[];
   unsigned char* const stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* const ring = stages + STAGES * L::STAGE_BYTES;
-  unsigned long long* const w_full = reinterpret_cast<unsigned long long*>(ring + L::RING_BYTES);                // [S] weights (8 warps) -> products
-  unsigned long long* const x_full = w_full + STAGES;                                                             // [S] TMA -> products
-  unsigned long long* const empty = x_full + STAGES;                                                              // [S] products -> both
+  unsigned long long* const full = reinterpret_cast<unsigned long long*>(ring + L::RING_BYTES);                  // [S] weights (a team), x (TMA) -> products
+  unsigned long long* const empty = full + STAGES;                                                                // [S] products -> both
   unsigned long long* const acc_full = empty + STAGES;                                                            // [2] a run's sums -> their readers
   unsigned long long* const acc_empty = acc_full + 2;                                                             // [2] read (128 arrivals) -> products
   unsigned long long* const c_full = acc_empty + 2;                                                               // [RING] TMA -> weights
-  unsigned long long* const c_empty = c_full + RING;                                                              // [RING] taken out (8 warps) -> TMA
+  unsigned long long* const c_empty = c_full + RING;                                                              // [RING] taken out (a team) -> TMA
   unsigned* const tmem_slot = reinterpret_cast<unsigned*>(c_empty + RING);
   __shared__ int failed_s, issued_s, codes_issued_s;
   __shared__ unsigned long long drained_s;
@@ -188,8 +198,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
       mbar_init(&c_empty[s], L::TEAM);
     }
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&w_full[s], L::TEAM);
-      mbar_init(&x_full[s], 1);
+      mbar_init(&full[s], L::TEAM + 1);
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -208,29 +217,38 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
   const unsigned tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   let_next_launch_in();
 
+  // The warps that copy and the one that issues products walk their units as a whole, and one lane issues: what an instruction is given is then the same for every lane,
+  // and stays in uniform registers.  Places are counted up, not worked out: a unit takes 700 cycles, and a division is a tenth of that.
   if (warp == 0) {
-    if (lane == 0) {
-      asm volatile("griddepcontrol.wait;" ::: "memory");
-      int i = 0;
-      for (; i < n_units; ++i) {
-        const int s = i % STAGES;
-        if (i >= STAGES && !mbar_wait(&empty[s], (unsigned)(((i / STAGES) - 1) & 1), p.err, failed, 1)) break;
-        mbar_expect_tx(&x_full[s], L::STAGE_BYTES);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const bool issues = elected();
+    int i = 0, s = 0, kb = u0 % KB;
+    unsigned par = 1;   // (the first turn finds every stage free)
+    for (; i < n_units; ++i) {
+      if (i >= STAGES && !__all_sync(0xffffffffu, mbar_wait(&empty[s], par, p.err, failed, 1))) break;
+      if (issues) {
+        mbar_expect_tx(&full[s], L::STAGE_BYTES);
         unsigned char* const to = stages + (size_t)s * L::STAGE_BYTES;
 #pragma unroll
-        for (int b = 0; b < KU; ++b) tma_load_2d(to + b * L::X_BLOCK, &map_x, ((u0 + i) % KB * KU + b) * BK, 0, &x_full[s]);
+        for (int b = 0; b < KU; ++b) tma_load_2d(to + b * L::X_BLOCK, &map_x, (kb * KU + b) * BK, 0, &full[s]);
       }
-      issued_s = i;
+      __syncwarp();
+      kb = kb + 1 == KB ? 0 : kb + 1;
+      if (++s == STAGES) {
+        s = 0;
+        par ^= 1;
+      }
     }
+    if (lane == 0) issued_s = i;
   } else if (warp == 1) {
-    // The whole warp walks the units and one lane issues: what the products are given is then the same for every lane, and stays in uniform registers.
     constexpr unsigned ID = idesc(BM, NB);
     const unsigned long long x_desc0 = umma_desc(stages);
     const bool issues = elected();
     int run = 0, s = 0, kb = u0 % KB;   // runs of one tile's units that this block has begun
     unsigned par = 0, first = 1;
+    bool there = false;   // the next unit is, as of the last one's products: asked before they are issued, which hides the answer's way
     for (int i = 0; i < n_units; ++i) {
-      bool ok = mbar_wait(&w_full[s], par, p.err, failed, 2) && mbar_wait(&x_full[s], par, p.err, failed, 3);
+      bool ok = there || mbar_wait(&full[s], par, p.err, failed, 2);
       if (ok && first && run >= L::ACCS)   // the sums that this buffer held have been read
         ok = mbar_wait(&acc_empty[run % L::ACCS], (unsigned)((run / L::ACCS - 1) & 1), p.err, failed, 4);
       if (!__all_sync(0xffffffffu, ok)) break;
@@ -238,6 +256,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
       const unsigned long long x_desc = x_desc0 + (unsigned)(s * (L::STAGE_BYTES >> 4));
       const unsigned d = tmem + (unsigned)(run % L::ACCS * NB), w = tmem + L::W_COL0 + (unsigned)(s * L::STAGE_COLS);
       const bool last = kb + 1 == KB || i == n_units - 1;
+      const int ahead = s + 1 == STAGES ? 0 : s + 1;
+      there = mbar_test(&full[ahead], ahead == 0 ? par ^ 1 : par);   // (behind the last unit: of a phase that nobody waits for)
       if (issues) {
 #pragma unroll
         for (int b = 0; b < KU; ++b)
@@ -255,10 +275,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
       first = last;
       run += last;
       kb = last ? 0 : kb + 1;
-      if (++s == STAGES) {
-        s = 0;
-        par ^= 1;
-      }
+      s = ahead;
+      par ^= ahead == 0;
     }
   } else if (warp < 6) {
     const int q = warp & 3, row = q * 32 + lane;   // the quarter of tensor memory that this warp may read; W row of the tile
@@ -296,20 +314,29 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       mbar_arrive(&acc_empty[b]);
     }
-  } else if (warp == 6 + TAKERS) {
-    if (lane == 0) {   // codes depend on no earlier launch
-      int i = 0;
-      for (; i < n_units; ++i) {
-        const int s = i % RING;
-        if (i >= RING && !mbar_wait(&c_empty[s], (unsigned)(((i / RING) - 1) & 1), p.err, failed, 7)) break;
-        const int tile = (u0 + i) / KB, kb = (u0 + i) % KB;
+  } else if (warp == 6 + TAKERS) {   // codes depend on no earlier launch
+    const bool issues = elected();
+    int i = 0, s = 0, kb = u0 % KB, tile = u0 / KB;
+    unsigned par = 1;
+    for (; i < n_units; ++i) {
+      if (i >= RING && !__all_sync(0xffffffffu, mbar_wait(&c_empty[s], par, p.err, failed, 7))) break;
+      if (issues) {
         unsigned char* const to = ring + s * L::SLOT_BYTES;
         mbar_expect_tx(&c_full[s], L::SLOT_BYTES);
         tma_load_2d(to, &map_codes, kb * (128 * KU), tile * 8, &c_full[s]);
         tma_load_2d(to + L::CODE_BYTES, &map_scales, ((kb * (64 * KU)) >> p.group_bits) * 16, tile * 8, &c_full[s]);
       }
-      codes_issued_s = i;
+      __syncwarp();
+      if (++kb == KB) {
+        kb = 0;
+        ++tile;
+      }
+      if (++s == RING) {
+        s = 0;
+        par ^= 1;
+      }
     }
+    if (lane == 0) codes_issued_s = i;
   } else {
     // teams take the units in turn, so that one's waits and fence are another's work
     constexpr int TEAM = L::TEAM;
@@ -338,7 +365,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&w_full[s]);
+        mbar_arrive(&full[s]);
         mbar_arrive(&c_empty[cs]);
       }
     }
@@ -350,7 +377,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
     // a wait ran out: give copies and products that may still be in flight a bounded time to end
     const long long t0 = clock64();
     auto expired = [&] { return clock64() - t0 > WAIT_CYCLES; };
-    if (threadIdx.x == 0) ring_drain(issued_s, STAGES, [&](int s, unsigned parity) { return mbar_try_wait(&x_full[s], parity); }, expired);
+    if (threadIdx.x == 0) ring_drain(issued_s, STAGES, [&](int s, unsigned parity) { return mbar_try_wait(&full[s], parity); }, expired);   // (or as long, where weights are missing)
     if (threadIdx.x == (6 + TAKERS) * 32) ring_drain(codes_issued_s, RING, [&](int s, unsigned parity) { return mbar_try_wait(&c_full[s], parity); }, expired);
     if (warp == 1 && elected()) {   // the thread that issued the products
       umma_commit(&drained_s);
