@@ -418,24 +418,31 @@ template <int NT, int GS, int TEAM, int PB, int SLOTS, bool ALONE> int few(const
   return launch(linear4_few_kernel<NT, GS, TEAM, PB, SLOTS, ALONE>, asked, turns < 148 ? turns : 148, FEW_WARPS * 32, Few<NT, GS, TEAM, PB, SLOTS>::bytes(a.m, a.k), a.pdl, a.st,
                 (const bf16*)a.x, a.x_stride, (const uint4*)a.codes, (const uint2*)a.scales, a.y, a.m, a.n, a.k, __builtin_ctz(a.group), a.mode, a.norm_w, a.eps);
 }
-// Four warps a tile where shared memory has room for their rings (x of 8 rows: up to about 6,000 inputs), else all sixteen with shorter rings.  2,560 inputs,
-// one row, four / eight / sixteen warps a tile: 151,936 outputs 55.6 / 63.6 / 81.9 us, 6,144 outputs 4.8 / 5.4 / 5.7 us (a tile's end costs each warp as much as
-// half a slot); 2,560 outputs of 9,728 inputs, hardly more tiles than multiprocessors, 9.6 / 9.7 / 10.2 us.
+// Four warps a tile where shared memory has room for their rings beside x (eight rows: up to about 6,000 inputs), else all sixteen with shorter rings, which only
+// 32-bit results use.  2,560 inputs, one row, four / eight / sixteen warps a tile: 151,936 outputs 55.6 / 63.6 / 81.9 us, 6,144 outputs 4.8 / 5.4 / 5.7 us (a tile's
+// end costs each warp as much as half a slot).  Where only the sixteen fit, the tensor memory kernel is as fast or faster (16 rows of 4,096 inputs, 24,576 outputs:
+// 21.3 us and 29.1; 8 rows of 9,728 inputs, 2,560 outputs: 11.4 and 12.1), but not where it has two products to make for 32 bits.
+constexpr int slots_of_group(int gs) { return gs == 1 ? 2 : gs == 2 ? 3 : 4; }   // as many as 98 KB hold: the scales of small groups are longer than the codes
+template <int NT, int GS> bool four_fit(int m, int k) { return Few<NT, GS, 4, 2, slots_of_group(GS)>::bytes(m, k) <= SMEM_MOST; }
+template <int NT, int GS> bool sixteen_fit(int m, int k) { return Few<NT, GS == 8 ? 4 : GS, 16, 1, 4>::bytes(m, k) <= SMEM_MOST; }
+template <int NT> int fits(int m, int k, int group) {
+  if (group == 128 ? four_fit<NT, 8>(m, k) : group == 64 ? four_fit<NT, 4>(m, k) : group == 32 ? four_fit<NT, 2>(m, k) : four_fit<NT, 1>(m, k)) return 1;
+  return (group >= 64 ? sixteen_fit<NT, 4>(m, k) : group == 32 ? sixteen_fit<NT, 2>(m, k) : sixteen_fit<NT, 1>(m, k)) ? 2 : 0;
+}
+int takes(int m, int k, int group) { return m <= 8 ? fits<1>(m, k, group) : m <= 16 ? fits<2>(m, k, group) : 0; }
+
 template <int NT, int GS, bool ALONE> int few_rows(const Args& a) {
   constexpr int GM = GS == 8 ? 4 : GS;
-  if (Few<NT, GS, 4, 2, 4>::bytes(a.m, a.k) <= SMEM_MOST) return few<NT, GS, 4, 2, 4, ALONE>(a);
-  return few<NT, GM, 16, 1, 4, ALONE>(a);
+  if (four_fit<NT, GS>(a.m, a.k)) return few<NT, GS, 4, 2, slots_of_group(GS), ALONE>(a);
+  if constexpr (ALONE) return few<NT, GM, 16, 1, 4, true>(a);
+  return DRYFT_ERR_UNSUPPORTED;
 }
-template <int NT> bool fits(int m, int k, int group) {
-  return (group >= 64 ? Few<NT, 4, 16, 1, 4>::bytes(m, k) : group == 32 ? Few<NT, 2, 16, 1, 4>::bytes(m, k) : Few<NT, 1, 16, 1, 4>::bytes(m, k)) <= SMEM_MOST;
-}
-bool takes(int m, int k, int group) { return m <= 8 ? fits<1>(m, k, group) : m <= 16 && fits<2>(m, k, group); }
-
 template <int GS, bool ALONE> int by_mode(const Args& a) { return a.m <= 8 ? few_rows<1, GS, ALONE>(a) : few_rows<2, GS, ALONE>(a); }
 template <int GS> int by_rows(const Args& a) { return a.mode <= STORE_F32 && a.norm_w == nullptr ? by_mode<GS, true>(a) : by_mode<GS, false>(a); }
 }  // namespace
 
-// Whether the kernel for few rows of bfloat16 takes so many rows of so many inputs (they have to fit in shared memory).
+// Whether the kernel for few rows of bfloat16 takes so many rows of so many inputs (they have to fit in shared memory): 1, with four warps a tile and whatever stands
+// around the product; 2, with sixteen, and the product alone; 0, not.
 DRYFT_API int dryft_linear4_takes(int m, int k, int group) { return takes(m, k, group); }
 
 // mode: Mode.  Modes beyond storing, and norm_w (which has k numbers on a 16-byte boundary; null: no norm), are the bfloat16 kernel's; SILU wants n to be a multiple of 32.

@@ -2604,11 +2604,14 @@ _linear4_fn = _linear4_tc_fn = None
 
 
 @functools.lru_cache(maxsize=4096)
-def linear4_plan(m: int, n: int, k: int, group: int, bf16: bool) -> int:
-    """Which kernel a product runs on: 0 for the one for few rows (up to 16, as long as x fits in its shared memory; float32: up to 64), else the floats of
-    workspace that the tensor memory kernel needs.  16 rows, 2,560 outputs of 9,728 inputs, which do not fit: 14.4 us on the latter; 19,456 of 2,560, which
-    do: 14.8 us on the former and 20.4 on the latter."""
-    if not bf16 or linear4_lib().dryft_linear4_takes(m, k, group):
+def linear4_plan(m: int, n: int, k: int, group: int, bf16: bool, f32_out: bool = False) -> int:
+    """Which kernel a product runs on: 0 for the one for few rows, else the floats of workspace that the tensor memory kernel needs.  The one for few rows takes
+    float32 (up to 64 rows), and up to 16 rows of bfloat16 that fit in shared memory beside its rings (16 rows, 6,144 outputs of 2,560 inputs: 7.7 us, on the
+    other one 9.7; 19,456 outputs: 14.5 and 14.4).  Where only its form with short rings fits, it is for 32-bit results alone (csrc/linear4.cu)."""
+    if not bf16:
+        return 0
+    takes = linear4_lib().dryft_linear4_takes(m, k, group)
+    if takes == 1 or (takes and f32_out):
         return 0
     return int(linear4_tc_lib().dryft_linear4_tc_pieces(m, n, k))
 
@@ -2659,7 +2662,7 @@ def linear4(x, w: Weight4, out=None, pdl: bool = False, mode: str = "store", nor
             _need(norm_w, "norm weight", torch.float32, (w.k,))
     if given:
         _need(out, "out", None, (m, w.n // 2 if code == 3 else w.n))
-    floats = linear4_plan(m, w.n, w.k, w.group, bool(is_bf16))
+    floats = linear4_plan(m, w.n, w.k, w.group, bool(is_bf16), not out_bf16)
     if floats:
         if _linear4_tc_fn is None:
             _linear4_tc_fn = linear4_tc_lib().dryft_linear4_tc
