@@ -18,6 +18,59 @@ struct Range {
   }
 };
 
+// Two numbers that follow one another, as they lie in memory, and the range of many such, which lanes can share.  Of bfloat16 numbers both ends are kept for two
+// numbers at once, by instructions that hand a NaN on, and (upper end, lower end with its sign turned) are shared as one word.
+__device__ __forceinline__ unsigned min2(unsigned a, unsigned b) {
+  unsigned r;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ unsigned max2(unsigned a, unsigned b) {
+  unsigned r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <typename T> struct Pairs;
+template <> struct Pairs<float> {
+  typedef float2 two;
+  typedef float4 four;
+  static __device__ __forceinline__ two half(four v, int i) { return i ? make_float2(v.z, v.w) : make_float2(v.x, v.y); }
+  Range r;
+  static __device__ __forceinline__ float first(two v) { return v.x; }
+  static __device__ __forceinline__ float second(two v) { return v.y; }
+  __device__ __forceinline__ void add(two v) {
+    r.add(v.x);
+    r.add(v.y);
+  }
+  __device__ __forceinline__ void close() { r.close(); }
+  __device__ __forceinline__ void share(int apart) {
+    r.lo = fminf(r.lo, __shfl_xor_sync(0xffffffffu, r.lo, apart));
+    r.hi = fmaxf(r.hi, __shfl_xor_sync(0xffffffffu, r.hi, apart));
+  }
+  __device__ __forceinline__ float2 ends() const { return make_float2(r.lo, r.hi); }
+};
+template <> struct Pairs<__nv_bfloat16> {
+  typedef unsigned two;
+  typedef uint2 four;
+  static __device__ __forceinline__ two half(four v, int i) { return i ? v.y : v.x; }
+  unsigned lo = 0x7f807f80u, hi = 0xff80ff80u;   // infinities; after `close`, hi is the word to share
+  static __device__ __forceinline__ float first(two v) { return __uint_as_float(v << 16); }
+  static __device__ __forceinline__ float second(two v) { return __uint_as_float(v & 0xffff0000u); }
+  __device__ __forceinline__ void add(two v) {
+    lo = min2(lo, v);
+    hi = max2(hi, v);
+  }
+  __device__ __forceinline__ void close() {
+    const unsigned l = min2(lo, __byte_perm(lo, lo, 0x1032)), h = max2(hi, __byte_perm(hi, hi, 0x1032));
+    hi = __byte_perm(h, l ^ 0x80008000u, 0x5410);
+  }
+  __device__ __forceinline__ void share(int apart) { hi = max2(hi, __shfl_xor_sync(0xffffffffu, hi, apart)); }
+  __device__ __forceinline__ float2 ends() const {   // a range with an infinity or a NaN is everything
+    const float h = first(hi), l = -second(hi);
+    return h < INFINITY && l > -INFINITY ? make_float2(l, h) : make_float2(-INFINITY, INFINITY);
+  }
+};
+
 // The codes of a group's numbers without a division each.  The definition (`code_of`) rounds t / s, t = x - z, and then t / s + 7.5, to 32 bits, and that to a whole
 // number.  With j the whole number nearest to t times 1 / s and e = t - j s (j s is exact, so e is rounded once, and 0 where t is a multiple of s), j + e / s is
 // t / s up to 2^-22, and exact where e is 0 -- which is every tie.  Only where e is neither 0 nor beyond 10^-5 s could those roundings decide: then the group's numbers
@@ -26,18 +79,18 @@ constexpr float ROUND = 12582912.f;   // 1.5 * 2^23: adding it rounds to whole n
 struct Coder {
   GroupCode g;
   float inv;
-  unsigned closest = ~0u;   // bits of the least |e| that is not 0, less 1
+  unsigned closest = ~0u;   // twice the bits of the least |e| that is not 0, less 1 (which drops the sign, and makes 0 the largest)
   __device__ __forceinline__ Coder(float lo, float hi) : g(group_code(lo, hi)), inv(inverse(g.s)) {}
   __device__ __forceinline__ Coder(GroupCode code, float inverse) : g(code), inv(inverse) {}
   static __device__ __forceinline__ float inverse(float s) { return s > 1e-36f ? __fdividef(1.f, s) : 0.f; }   // (its last bits do not matter)
   // `word` + code << shift + ROUND's bits << shift, which the caller takes out (`round_bits`)
   __device__ __forceinline__ unsigned add(unsigned word, float x, int shift) {
     const float t = __fadd_rn(x, -g.z), j = __fadd_rn(__fadd_rn(__fmul_rn(t, inv), ROUND), -ROUND), e = fmaf(-j, g.s, t);
-    closest = min(closest, (__float_as_uint(e) & 0x7fffffffu) - 1u);
+    closest = min(closest, 2u * __float_as_uint(e) - 1u);
     const float y = __fadd_rn(fmaf(e, inv, j), 7.5f);
     return word + (__float_as_uint(__fadd_rn(fminf(fmaxf(y, 0.f), 15.f), ROUND)) << shift);
   }
-  __device__ __forceinline__ bool undecided() const { return closest < __float_as_uint(g.s * 1e-5f) || (inv == 0.f && g.s > 0.f); }
+  __device__ __forceinline__ bool undecided() const { return closest < 2u * __float_as_uint(g.s * 1e-5f) || (inv == 0.f && g.s > 0.f); }
 };
 __device__ __forceinline__ constexpr unsigned round_bits(unsigned places) {   // ROUND's bits at every nibble of `places` (a bit each)
   unsigned sum = 0;
@@ -196,14 +249,14 @@ __device__ __forceinline__ void store_tile_values(const T* rows, long long strid
 #pragma unroll
   for (int b = 0; b < UB; ++b) bits[b][0] = bits[b][1] = 0;
   const bool all = 2 * c >= i0 && 2 * c + 9 < i0 + count;   // the lane's four tokens are written together
-  float x[4][2 * UB][2];
+  typedef Pairs<T> P;
+  typename P::two x[4][2 * UB] = {};
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int s = 0; s < 2 * UB; ++s) {
       const int k = 2 * c + (i & 1) + 8 * (i >> 1), at = 32 * u0 + 16 * s + 2 * r;
-      x[i][s][0] = x[i][s][1] = 0.f;
-      if (k >= i0 && k < i0 + count && at < d) load_row<T, 2>(x[i][s], rows + (k - i0) * stride + at);
+      if (k >= i0 && k < i0 + count && at < d) x[i][s] = *reinterpret_cast<const typename P::two*>(rows + (k - i0) * stride + at);
     }
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
@@ -211,22 +264,17 @@ __device__ __forceinline__ void store_tile_values(const T* rows, long long strid
     float lo = INFINITY, hi = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      Range range;
+      P range;
 #pragma unroll
       for (int s = g * GS; s < (g + 1) * GS; ++s)
-        if (32 * u0 + 16 * s < d) {
-          range.add(x[i][s][0]);
-          range.add(x[i][s][1]);
-        }
+        if (32 * u0 + 16 * s < d) range.add(x[i][s]);
       range.close();
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        range.lo = fminf(range.lo, __shfl_xor_sync(0xffffffffu, range.lo, o));
-        range.hi = fmaxf(range.hi, __shfl_xor_sync(0xffffffffu, range.hi, o));
-      }
+      for (int o = 4; o < 32; o <<= 1) range.share(o);
+      const float2 ends = range.ends();
       if ((r & 3) == i) {
-        lo = range.lo;
-        hi = range.hi;
+        lo = ends.x;
+        hi = ends.y;
       }
     }
     const GroupCode one = group_code(lo, hi);
@@ -242,14 +290,14 @@ __device__ __forceinline__ void store_tile_values(const T* rows, long long strid
 #pragma unroll
       for (int s = g * GS; s < (g + 1) * GS; ++s) {
         unsigned& h = half[s / 2 - g * GS / 2];
-        h = code.add(code.add(h - round_bits(s & 1 ? 0xc : 0x3), x[i][s][0], 8 * (s & 1)), x[i][s][1], 8 * (s & 1) + 4);
+        h = code.add(code.add(h - round_bits(s & 1 ? 0xc : 0x3), P::first(x[i][s]), 8 * (s & 1)), P::second(x[i][s]), 8 * (s & 1) + 4);
       }
       if (code.undecided()) {
 #pragma unroll
         for (int s = g * GS; s < (g + 1) * GS; ++s) {
           unsigned& h = half[s / 2 - g * GS / 2];
           if (GS == 1 || (s & 1) == 0) h = 0;
-          h |= (code_of(x[i][s][0], code.g) | code_of(x[i][s][1], code.g) << 4) << (8 * (s & 1));
+          h |= (code_of(P::first(x[i][s]), code.g) | code_of(P::second(x[i][s]), code.g) << 4) << (8 * (s & 1));
         }
       }
 #pragma unroll
@@ -273,11 +321,81 @@ __device__ __forceinline__ void store_tile_values(const T* rows, long long strid
   }
 }
 
+// KEY_TOKENS tokens' keys of one head, by each thread of the lanes that share a token: four dims of each step of a unit.  Quarter c of a unit works out the scale of
+// token c for all of them.
+constexpr int KEY_TOKENS = 4;
+template <typename T, int GS>
+__device__ __forceinline__ void store_keys(const typename Pairs<T>::two (&x)[KEY_TOKENS][2][2], const int (&slot)[KEY_TOKENS], const int (&pos)[KEY_TOKENS], int part,
+                                           unsigned char* k_pages, unsigned char* v_pages, const int* page_table, int max_pages, int n_kv, int head, int d, int page,
+                                           size_t tile_bytes) {
+  typedef Pairs<T> P;
+  constexpr int GROUP = 16 * GS, STEPS = GS == 1 ? 1 : 2, RANGES = 2 / STEPS;   // steps of the unit that share a scale; scales of a unit
+  const int lane = threadIdx.x & 31, u = part >> 2, c = part & 3, units = kv4_units(d);
+  unsigned packed[RANGES];
+  float inverse[RANGES];
+#pragma unroll
+  for (int p = 0; p < RANGES; ++p) {
+    float2 ends = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < KEY_TOKENS; ++i) {
+      P range;
+#pragma unroll
+      for (int q = p * STEPS; q < (p + 1) * STEPS; ++q)
+        if (32 * u + 16 * q < d) {
+          range.add(x[i][q][0]);
+          range.add(x[i][q][1]);
+        }
+      range.close();
+#pragma unroll
+      for (int o = 1; o < (GS > 2 ? 2 * GS : 4); o <<= 1) range.share(o);
+      const float2 e = range.ends();
+      if (c == i) ends = e;
+    }
+    const GroupCode one = group_code(ends.x, ends.y);
+    packed[p] = pack_code(one);
+    inverse[p] = Coder::inverse(one.s);
+  }
+#pragma unroll
+  for (int i = 0; i < KEY_TOKENS; ++i) {
+    unsigned sz[RANGES];
+    float inv[RANGES];
+#pragma unroll
+    for (int p = 0; p < RANGES; ++p) {
+      sz[p] = __shfl_sync(0xffffffffu, packed[p], (lane & ~3) + i);
+      inv[p] = __shfl_sync(0xffffffffu, inverse[p], (lane & ~3) + i);
+    }
+    if (slot[i] < 0 || u >= units) continue;
+    const Place at = place_of(k_pages, v_pages, page_table, max_pages, slot[i], pos[i], page, n_kv, head, tile_bytes);
+    unsigned word = 0;
+#pragma unroll
+    for (int p = 0; p < RANGES; ++p) {
+      const int dim = 32 * u + 16 * p * STEPS;
+      if (dim >= d) continue;
+      Coder code(unpack_code(sz[p]), inv[p]);
+      unsigned steps = 0u - (STEPS == 2 ? round_bits(0xff) : p ? round_bits(0xcc) : round_bits(0x33));
+      const auto place = [](int q, int e) { return 8 * q + 4 * (e >> 1) + 16 * (e & 1); };
+#pragma unroll
+      for (int q = p * STEPS; q < (p + 1) * STEPS; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) steps = code.add(steps, e & 1 ? P::second(x[i][q][e >> 1]) : P::first(x[i][q][e >> 1]), place(q, e));
+      if (code.undecided()) {
+        steps = 0;
+#pragma unroll
+        for (int q = p * STEPS; q < (p + 1) * STEPS; ++q)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) steps |= code_of(e & 1 ? P::second(x[i][q][e >> 1]) : P::first(x[i][q][e >> 1]), code.g) << place(q, e);
+      }
+      word |= steps;
+      if (c == 0 && dim % GROUP == 0) reinterpret_cast<unsigned*>(at.k + (size_t)kv4_row_bytes(d) * page)[at.t * (d / GROUP) + dim / GROUP] = sz[p];
+    }
+    *reinterpret_cast<unsigned*>(at.k + (size_t)at.t * kv4_row_bytes(d) + (c * units + u) * 4) = word;
+  }
+}
+
 // Grid (blocks, key heads).  Keys by the first `key_blocks` blocks, values by the others.
 // Keys: as many lanes for a token as a row has words of eight dims, or the next power of two; a thread takes KEY_TOKENS tokens.
 // Values: a warp per `span` consecutive tokens of the launch and UB units.  Tokens that follow one another in one tile of 16 places of a page are
 // stored together, by the warp that has the first of them.
-constexpr int KEY_TOKENS = 4;
 template <typename T, int UB, int GS>
 __global__ void __launch_bounds__(WARPS * 32) kv4_store_kernel(const T* k, const T* v, long long stride, const int* __restrict__ tok_slot,
                                                                const int* __restrict__ tok_pos, unsigned char* k_pages, unsigned char* v_pages,
@@ -289,21 +407,25 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_store_kernel(const T* k, const
   if ((int)blockIdx.x < key_blocks) {
     const int at_once = (WARPS * 32) >> lane_bits, part = threadIdx.x & ((1 << lane_bits) - 1);
     const int t0 = blockIdx.x * (at_once * KEY_TOKENS) + (threadIdx.x >> lane_bits);
-    float x[KEY_TOKENS][2][4];
+    typename Pairs<T>::two x[KEY_TOKENS][2][2] = {};
     int slot[KEY_TOKENS], pos[KEY_TOKENS];
 #pragma unroll
     for (int i = 0; i < KEY_TOKENS; ++i) {
       const int t = t0 + i * at_once;
       slot[i] = t < n ? tok_slot[t] : -1;
       pos[i] = t < n ? tok_pos[t] : 0;
-      load_key<T>(x[i], k + (long long)t * stride + (size_t)head * d, part, d, t < n);
-    }
+      const T* const row = k + (long long)t * stride + (size_t)head * d;
 #pragma unroll
-    for (int i = 0; i < KEY_TOKENS; ++i) {
-      Place at = {};
-      if (slot[i] >= 0) at = place_of(k_pages, v_pages, page_table, max_pages, slot[i], pos[i], page, n_kv, head, tile_bytes);
-      store_key<GS>(x[i], slot[i] >= 0, part, at.k, at.t, d, page);
+      for (int q = 0; q < 2; ++q) {
+        const int at = 32 * (part >> 2) + 16 * q + 4 * (part & 3);
+        if (t < n && at < d) {   // four numbers at once
+          const auto v = *reinterpret_cast<const typename Pairs<T>::four*>(row + at);
+          x[i][q][0] = Pairs<T>::half(v, 0);
+          x[i][q][1] = Pairs<T>::half(v, 1);
+        }
+      }
     }
+    store_keys<T, GS>(x, slot, pos, part, k_pages, v_pages, page_table, max_pages, n_kv, head, d, page, tile_bytes);
     return;
   }
   const int job = (blockIdx.x - key_blocks) * WARPS + (threadIdx.x >> 5), parts = kv4_units(d) / UB;
