@@ -392,6 +392,8 @@ __device__ __forceinline__ void store_keys(const typename Pairs<T>::two (&x)[KEY
   }
 }
 
+// Bound by issue: some 15 instructions a number for its code and 6 for the rest.  12,829 tokens, eight key heads of 128: 30.7 us, 2,200 GB/s (with
+// each number's range and every lane's scale for itself 37.6); eight tokens 2.5 us, a launch.
 // Grid (blocks, key heads).  Keys by the first `key_blocks` blocks, values by the others.
 // Keys: as many lanes for a token as a row has words of eight dims, or the next power of two; a thread takes KEY_TOKENS tokens.
 // Values: a warp per `span` consecutive tokens of the launch and UB units.  Tokens that follow one another in one tile of 16 places of a page are
@@ -529,32 +531,58 @@ template <typename T> __device__ __forceinline__ typename Pair<T>::type values_o
   }
 }
 
-// Blocks per (sequence, key head), each every gridDim.x-th page of it: the page's tokens as values, those behind the sequence's end as zeros.  Pages before the
-// first key that the step's first token of the sequence sees (window <= 0: every key) are left alone: they may be another sequence's by now.
-// A thread takes a word of a key (eight dims of a token) or a unit of a lane's values (four dims of four tokens); neighbours fill whole sectors.
+// Blocks per (sequence, key head), each every gridDim.x-th chunk of it (a page, or part of a long one): the chunk's tokens as values, those behind the sequence's end
+// as zeros.  Pages before the first key that the step's first token of the sequence sees (window <= 0: every key) are left alone: they may be another sequence's by now.
+// A chunk's codes and scales are copied into shared memory while the one before is taken out; then a thread takes a word of a key (eight dims of a token) or a unit
+// of a lane's values (four dims of four tokens), and neighbours fill whole sectors.  Bound by the bytes it writes, and by the way to its first ones: 64 sequences of up
+// to 8,192 tokens, eight key heads of 128, 286 us, 4,990 GB/s (read straight from memory 411); 13 prompts, 12,829 tokens, 21.8 us, 3,180 GB/s; 8 of 100, 4.6 us.
+__host__ __device__ inline int chunk_of(int page) { return page <= 64 ? page : page % 64 ? 16 : 64; }
+__device__ __forceinline__ void copy16(unsigned to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from)); }
 template <typename T>
 __global__ void __launch_bounds__(256, 4) kv4_expand_kernel(const unsigned char* __restrict__ k_pages, const unsigned char* __restrict__ v_pages,
-                                                         const int* __restrict__ page_table, int max_pages, const int* __restrict__ cu_q,
-                                                         const int* __restrict__ seq_slot, const int* __restrict__ tok_pos, T* k_out, T* v_out, int n_kv, int d,
-                                                         int group_bits, int page, int window) {
+                                                            const int* __restrict__ page_table, int max_pages, const int* __restrict__ cu_q,
+                                                            const int* __restrict__ seq_slot, const int* __restrict__ tok_pos, T* k_out, T* v_out, int n_kv, int d,
+                                                            int group_bits, int page, int window) {
   typedef typename Pair<T>::type P;
-  const int b = blockIdx.z, head = blockIdx.y, slot = seq_slot[b];
-  if (slot < 0 || cu_q[b + 1] <= cu_q[b]) return;
-  const int end = tok_pos[cu_q[b + 1] - 1] + 1, first = window > 0 ? max(0, tok_pos[cu_q[b]] + 1 - window) / page : 0;
+  extern __shared__ __align__(16) unsigned char held[];   // two chunks: keys' codes, keys' scales, values' codes, values' scales
+  const int b = blockIdx.z, head = blockIdx.y, slot = seq_slot[b], q0 = cu_q[b], q1 = cu_q[b + 1];
+  if (slot < 0 || q1 <= q0) return;
+  const int chunk = chunk_of(page), per_page = page / chunk, end = tok_pos[q1 - 1] + 1, first = window > 0 ? max(0, tok_pos[q0] + 1 - window) / page * per_page : 0;
   const int units = kv4_units(d), groups = d >> group_bits, row = kv4_row_bytes(d), words = 4 * units;
+  const int codes = chunk * row, side = codes + chunk * groups * 4;   // bytes of a chunk's keys (or values)
   const size_t tile_bytes = kv4_tile_bytes(page, d, 1 << group_bits);
+  const unsigned held_at = (unsigned)__cvta_generic_to_shared(held);
+  const auto page_of = [&](int p) { return (size_t)page_table[(size_t)slot * max_pages + p / per_page] * n_kv + head; };
+  const auto request = [&](int p, int buffer) {
+    if (p * chunk < end) {
+      const size_t at = page_of(p) * tile_bytes;
+      const int t0 = p % per_page * chunk;
+      for (int i = threadIdx.x * 16; i < side; i += 256 * 16) {
+        const size_t from = at + (i < codes ? (size_t)t0 * row + i : (size_t)row * page + (size_t)t0 * groups * 4 + (i - codes));
+        copy16(held_at + buffer * 2 * side + i, k_pages + from);
+        copy16(held_at + (buffer * 2 + 1) * side + i, v_pages + from);
+      }
+    }
+    asm volatile("cp.async.commit_group;");
+  };
   // keys: the thread's word, and its tokens, `t_step` apart.  Values: its lane row r, unit u, and its (tile, c), `j_step` apart.
   const int t_step = 256 / words, kt0 = threadIdx.x / words, kx = threadIdx.x % words, ku = kx >> 2, kc = kx & 3;
   const int j_step = 32 / units, j0 = (threadIdx.x >> 3) / units, u = (threadIdx.x >> 3) % units, r = threadIdx.x & 7;
-  for (int p = first + blockIdx.x; p * page < end; p += gridDim.x) {
-    const size_t at_page = (size_t)page_table[(size_t)slot * max_pages + p] * n_kv + head;
-    const unsigned char *kt = k_pages + at_page * tile_bytes, *vt = v_pages + at_page * tile_bytes;
-    const unsigned *ks = reinterpret_cast<const unsigned*>(kt + (size_t)row * page), *vs = reinterpret_cast<const unsigned*>(vt + (size_t)row * page);
-    T *ko = k_out + at_page * page * d, *vo = v_out + at_page * page * d;
-    const int left = end - p * page;
+  request(first + blockIdx.x, 0);
+  int buffer = 0;
+  const int last = (end + page - 1) / page * per_page;   // (the last page is filled up, by zeros)
+  for (int p = first + blockIdx.x; p < last; p += gridDim.x, buffer ^= 1) {
+    request(p + gridDim.x, buffer ^ 1);
+    const size_t out_at = (page_of(p) * page + p % per_page * chunk) * d;
+    asm volatile("cp.async.wait_group 1;");
+    __syncthreads();
+    const unsigned char *kt = held + buffer * 2 * side, *vt = kt + side;
+    const unsigned *ks = reinterpret_cast<const unsigned*>(kt + codes), *vs = reinterpret_cast<const unsigned*>(vt + codes);
+    T *ko = k_out + out_at, *vo = v_out + out_at;
+    const int left = end - p * chunk;
     if (kt0 < t_step)
 #pragma unroll 2
-      for (int t = kt0; t < page; t += t_step) {
+      for (int t = kt0; t < chunk; t += t_step) {
         const bool have = t < left;
         const unsigned w = have ? *reinterpret_cast<const unsigned*>(kt + t * row + (kc * units + ku) * 4) : 0u;
 #pragma unroll
@@ -572,7 +600,7 @@ __global__ void __launch_bounds__(256, 4) kv4_expand_kernel(const unsigned char*
       }
     if (j0 < j_step)
 #pragma unroll 2
-      for (int j = j0; j < page / 4; j += j_step) {
+      for (int j = j0; j < chunk / 4; j += j_step) {
         const int c = j & 3, tile = j >> 2, k0 = tile * 16 + 2 * c;
         const uint2 w = *reinterpret_cast<const uint2*>(vt + (tile * 256 + (r * 4 + c) * 8) * units + u * 8);
 #pragma unroll
@@ -590,7 +618,9 @@ __global__ void __launch_bounds__(256, 4) kv4_expand_kernel(const unsigned char*
             }
           }
       }
+    __syncthreads();   // the next but one chunk goes where this one was
   }
+  asm volatile("cp.async.wait_group 0;");
 }
 
 template <typename T, int UB, int GS>
@@ -620,9 +650,15 @@ int store(const void* k, const void* v, long long stride, const int* tok_slot, c
 template <typename T>
 int expand(const void* k_pages, const void* v_pages, const int* page_table, int max_pages, const int* cu_q, const int* seq_slot, const int* tok_pos, void* k_out,
            void* v_out, int n_seqs, int pages, int n_kv, int d, int group, int page, int window, cudaStream_t st) {
-  const int blocks = 4096 / (n_kv * n_seqs) + 1;   // of a sequence and head: a few thousand blocks, however long the sequences may be
-  kv4_expand_kernel<T><<<dim3(blocks < pages ? blocks : pages, n_kv, n_seqs), 256, 0, st>>>((const unsigned char*)k_pages, (const unsigned char*)v_pages, page_table, max_pages, cu_q,
-                                                                  seq_slot, tok_pos, (T*)k_out, (T*)v_out, n_kv, d, __builtin_ctz(group), page, window);
+  const int chunk = chunk_of(page), chunks = pages * (page / chunk), bytes = 4 * chunk * (kv4_row_bytes(d) + 4 * (d / group));
+  const int blocks = 4096 / (n_kv * n_seqs) + 1;   // of a sequence and head: a few thousand blocks, however long the sequences may be (1,500: 64 ragged ones 345 us, not 286)
+  if (bytes > 48 * 1024) {   // (asking twice does no harm)
+    const cudaError_t e = cudaFuncSetAttribute(kv4_expand_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return (int)e;
+  }
+  kv4_expand_kernel<T><<<dim3(blocks < chunks ? blocks : chunks, n_kv, n_seqs), 256, bytes, st>>>((const unsigned char*)k_pages, (const unsigned char*)v_pages, page_table,
+                                                                                                 max_pages, cu_q, seq_slot, tok_pos, (T*)k_out, (T*)v_out, n_kv, d,
+                                                                                                 __builtin_ctz(group), page, window);
   return launch_status();
 }
 template <typename T>

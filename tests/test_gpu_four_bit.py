@@ -190,7 +190,7 @@ SHAPES = [(1, 16, 16), (2, 32, 32), (3, 48, 16), (2, 64, 64), (2, 80, 16), (1, 9
 
 @pytest.mark.parametrize("kv,d,group", SHAPES)
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("page", [16, 48, 64, 80, 128])
 def test_stored_tokens_come_back_as_their_codes_values(kv, d, group, dtype, page):
     lens = [1, 15, 64, 65, 200]
     c = Cache(lens, kv, d, group, page, dtype)
