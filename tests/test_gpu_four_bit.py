@@ -109,6 +109,19 @@ def test_products_with_the_norm_before_and_the_sum_or_activation_behind(m, n, k,
         assert torch.equal(act, want)
 
 
+def test_many_rows_of_results_that_begin_anywhere():
+    """685 rows of 439 outputs: held against the sum of 8,496 products as a whole, whose rounding to bfloat16 (of weights and result: 2^-9 each at most, and half of
+    that in the mean) may be its only error: 2^-9 times the square root of 2 of the whole."""
+    L = importlib.import_module("dryft_b200.parts.linear")
+    from dryft_b200.parts.base import Runtime
+
+    m, n, k = 685, 439, 8496
+    w, x = torch.randn(n, k).to(BF), torch.randn(m, k).to(BF)
+    want = P.linear(x, P.group_values(w, 16)[0])
+    y = L.linear(x.to(DEV), K().pack_weight4(w.to(DEV), 16), Runtime(dtype=BF, device=torch.device(DEV)))
+    assert (y.double().cpu() - want).norm() <= 2.0**-9 * 2**0.5 * want.norm()
+
+
 def test_modes_that_are_refused():
     w4, t = K().pack_weight4(torch.randn(48, 64, device=DEV)), lambda *shape, dtype=BF: torch.zeros(shape, dtype=dtype, device=DEV)
     for x, out, more in ((t(17, 64), t(17, 48), dict(mode="residual")), (t(1, 64, dtype=F32), t(1, 48, dtype=F32), dict(norm_w=t(64, dtype=F32))), (t(1, 64), t(1, 24), dict(mode="silu")),
