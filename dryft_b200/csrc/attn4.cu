@@ -37,9 +37,13 @@ __device__ __forceinline__ Work work_of_block() {   // grid (splits, key heads x
 // ---------------------------------------------------------------------------------------------- bfloat16: tensor cores
 // S^T = K Q^T and O^T = V^T P^T on mma.sync.m16n8k16, the codes as bfloat16 16 + c straight out of the cache's words (`code_pair`):
 //   score  = s_k (sum (16 + c) q - 23.5 sum q) + z_k sum q          group by group, in 32 bits; sum q is the query's own
-//   output = sum p' (16 + c) + sum p z_v - 23.5 sum p'              p' = bf16(p s_v): the weight rounded with its scale, one rounding of 2^-9 as for plain P
+//   output = sum p' (16 + c) + sum p z_v - 23.5 sum p'              p' = bf16(p s_v): the weight rounded with its scale, one rounding of up to 2^-8 as for plain P
 // Scores, running maximum and sums are 32-bit.  A warp walks tiles of 16 keys of its own, copied STAGES - 1 tiles ahead into its own ring.  The maximum
 // of a column follows the scores only when one exceeds it by more than 2^8: what is summed stays below 2^8 times the number of keys.
+// What bounds it: issue.  A tile is some 400 instructions of its warp, 224 of them on the pipe for logic, which takes one every other cycle (taking 128 codes a lane
+// apart is half of those): with four warps on a scheduler that pipe is 69% busy and a tile takes 0.40 us of the scheduler, with two 0.34 us.  64 rows of up to 8,192
+// keys, 32 / 8 heads of 128: 98 us, 3,190 GB/s; one row of 16,383 keys, 64 / 8 heads: 18 us (16 us by way of memory, and a second launch on the host); eight rows of
+// 650 keys 8 us; one, 7.  Sixteen warps a block: 10.1 us for the eight rows; two tiles unrolled: as before.
 typedef __nv_bfloat16 bf16;
 constexpr int STEPS = D / 16, UNIT = PAGE % 32 ? 1 : 2, STAGES = D <= 128 ? 4 / UNIT : 2, MOST_SPLITS = 16;   // UNIT: tiles that are copied together
 constexpr int CODES = 256 * UNITS, SCALES = 64 * GROUPS, STAGE = UNIT * 2 * (CODES + SCALES);   // bytes of a tile's keys (or values), of their scales; of a stage

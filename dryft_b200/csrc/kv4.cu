@@ -392,7 +392,7 @@ __device__ __forceinline__ void store_keys(const typename Pairs<T>::two (&x)[KEY
   }
 }
 
-// Bound by issue: some 15 instructions a number for its code and 6 for the rest.  12,829 tokens, eight key heads of 128: 30.7 us, 2,200 GB/s (with
+// Bound by issue, 81% of its slots: 31 instructions a number, 15 of them for its code.  12,829 tokens, eight key heads of 128: 30.7 us, 2,200 GB/s (with
 // each number's range and every lane's scale for itself 37.6); eight tokens 2.5 us, a launch.
 // Grid (blocks, key heads).  Keys by the first `key_blocks` blocks, values by the others.
 // Keys: as many lanes for a token as a row has words of eight dims, or the next power of two; a thread takes KEY_TOKENS tokens.
@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_store_kernel(const T* k, const
 }
 
 // The same behind a fused projection (rows q | k | v): per-head norm and rotation of queries and keys first, a warp per (token, head).  Formulas and
-// rounding points are those of rope_kv.cu.
+// rounding points are those of rope_kv.cu.  A programmatic dependent: a decode step's launch is some 3 us of latency (loads, a norm's sum, angles, a range), no rate.
 template <typename T>
 __global__ void __launch_bounds__(WARPS * 32) kv4_rope_store_kernel(const T* qkv, int stride, const float* __restrict__ wq, const float* __restrict__ wk,
                                                                     const float* __restrict__ inv_freq, const T* cs_table, const int* __restrict__ tok_slot,
@@ -534,7 +534,7 @@ template <typename T> __device__ __forceinline__ typename Pair<T>::type values_o
 // Blocks per (sequence, key head), each every gridDim.x-th chunk of it (a page, or part of a long one): the chunk's tokens as values, those behind the sequence's end
 // as zeros.  Pages before the first key that the step's first token of the sequence sees (window <= 0: every key) are left alone: they may be another sequence's by now.
 // A chunk's codes and scales are copied into shared memory while the one before is taken out; then a thread takes a word of a key (eight dims of a token) or a unit
-// of a lane's values (four dims of four tokens), and neighbours fill whole sectors.  Bound by the bytes it writes, and by the way to its first ones: 64 sequences of up
+// of a lane's values (four dims of four tokens), and neighbours fill whole sectors.  Bound by issue (81% of its slots) and, where pages are few, by the way to the first bytes: 64 sequences of up
 // to 8,192 tokens, eight key heads of 128, 286 us, 4,990 GB/s (read straight from memory 411); 13 prompts, 12,829 tokens, 21.8 us, 3,180 GB/s; 8 of 100, 4.6 us.
 __host__ __device__ inline int chunk_of(int page) { return page <= 64 ? page : page % 64 ? 16 : 64; }
 __device__ __forceinline__ void copy16(unsigned to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from)); }

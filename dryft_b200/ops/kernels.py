@@ -2682,7 +2682,7 @@ def linear4(x, w: Weight4, out=None, pdl: bool = False, mode: str = "store", nor
 
 def weight4_expand(w: Weight4, out, rest: bool = False) -> None:
     """``out`` ``[n, k]`` (float32 or bfloat16): what the codes stand for, for products of many rows.  ``rest``: what rounding that to bfloat16 leaves, itself
-    rounded to bfloat16 (the two together are off by 2^-17)."""
+    rounded to bfloat16 (the two together are off by up to 2^-16)."""
     _need_weight4(w)
     _need(out, "out", None, (w.n, w.k))
     is_bf16 = _act(out, "out")

@@ -9,8 +9,8 @@ Which product runs:
     product the reference itself uses (``F.linear``, ``engine/dryft_qwen3/model.py:153,179,180``);
   * bfloat16 activations with a weight the checkpoint stores in 32-bit: the weight stays 32-bit,
     the activations are widened, the 32-bit product runs and its result is rounded once;
-  * weights held in 4 bits (``ops.kernels.Weight4``): the kernel that reads the codes up to 64 rows, above that the
-    weights are taken out of their 4 bits for the product above.
+  * weights held in 4 bits (``ops.kernels.Weight4``): up to 256 rows of bfloat16 (64 of float32) the kernels that
+    read the codes, above that the weights are taken out of their 4 bits for the products above.
 """
 
 from __future__ import annotations
