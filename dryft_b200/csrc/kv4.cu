@@ -650,12 +650,8 @@ int store(const void* k, const void* v, long long stride, const int* tok_slot, c
 template <typename T>
 int expand(const void* k_pages, const void* v_pages, const int* page_table, int max_pages, const int* cu_q, const int* seq_slot, const int* tok_pos, void* k_out,
            void* v_out, int n_seqs, int pages, int n_kv, int d, int group, int page, int window, cudaStream_t st) {
-  const int chunk = chunk_of(page), chunks = pages * (page / chunk), bytes = 4 * chunk * (kv4_row_bytes(d) + 4 * (d / group));
+  const int chunk = chunk_of(page), chunks = pages * (page / chunk), bytes = 4 * chunk * (kv4_row_bytes(d) + 4 * (d / group));   // 48 KB at most
   const int blocks = 4096 / (n_kv * n_seqs) + 1;   // of a sequence and head: a few thousand blocks, however long the sequences may be (1,500: 64 ragged ones 345 us, not 286)
-  if (bytes > 48 * 1024) {   // (asking twice does no harm)
-    const cudaError_t e = cudaFuncSetAttribute(kv4_expand_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return (int)e;
-  }
   kv4_expand_kernel<T><<<dim3(blocks < chunks ? blocks : chunks, n_kv, n_seqs), 256, bytes, st>>>((const unsigned char*)k_pages, (const unsigned char*)v_pages, page_table,
                                                                                                  max_pages, cu_q, seq_slot, tok_pos, (T*)k_out, (T*)v_out, n_kv, d,
                                                                                                  __builtin_ctz(group), page, window);

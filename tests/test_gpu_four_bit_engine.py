@@ -170,3 +170,39 @@ def test_what_is_refused(model_dirs):
     for kw in (dict(weight_bits=4), dict(cache_bits=4)):
         with pytest.raises(ValueError, match="not served"):
             Engine.from_config(preset("tevovik-tiny"), max_batch=2, max_seq_len=64, **kw)
+
+
+@pytest.mark.parametrize("n_seqs", [1, 3, 8, 24])
+def test_decode_at_production_widths_is_the_same_with_and_without_launch_overlap(n_seqs):
+    """Two layers 2,560 wide: a decode step whose launches overlap gives bit for bit the logits of the same launches one after the other, with norms, sums and
+    activations in the products (up to four rows) and as launches, on the kernels for few rows and for many; and, with the weights alone in 4 bits, stays within
+    bfloat16 rounding of the path of separate kernels."""
+    from dryft_b200.config import preset
+    from dryft_b200.engine.api import Engine
+
+    raw = dict(preset("qwen3-4b"))
+    raw.update(num_hidden_layers=2, vocab_size=8192, max_position_embeddings=2048)
+    g = torch.Generator().manual_seed(5)
+    prompts = [torch.randint(0, 8192, (n,), generator=g).tolist() for n in ((70, 3, 129, 64, 200, 17, 31, 90, 5, 250, 33, 128) * 2)[:n_seqs]]
+
+    def decode_logits(dtype="bfloat16", **opts):
+        eng = Engine.from_config(raw, seed=4, std=0.03, max_batch=32, max_seq_len=1024, max_tokens=16 * 1024, dtype=dtype, weight_bits=4, **opts)
+        outs = []
+        with torch.inference_mode():
+            s = eng.cache.open_sequences(len(prompts))
+            lg = eng.stepper.step(s, prompts, [[len(p) - 1] for p in prompts])
+            idx = torch.tensor(s, device="cuda")
+            for _ in range(5):
+                eng.cache.last_token[idx] = (torch.arange(len(prompts), device="cuda") * 37 + len(outs) * 11).int() % 8192
+                lg = eng.stepper.decode_from_state(s)[: len(prompts)].float()
+                outs.append(lg.cpu())
+            eng.cache.close_sequences(s)
+        del eng
+        torch.cuda.empty_cache()
+        return torch.stack(outs)
+
+    overlapped = decode_logits(cache_bits=4)
+    assert torch.equal(overlapped, decode_logits(cache_bits=4, cuda_graphs=False)) and torch.equal(overlapped, decode_logits(cache_bits=4, pdl=False))
+    fused, separate, exact = decode_logits(), decode_logits(fuse_decode=False), decode_logits("float32")
+    tol = H.bf16_tol(separate, exact)
+    assert H.rel_err(fused, separate) <= tol and H.rel_err(fused, exact) <= tol
