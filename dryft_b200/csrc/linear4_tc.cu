@@ -12,9 +12,10 @@
 //
 // What bounds it: every tile reads all of x again, from L2, which moves 9 TB/s at 48 rows (issue slots are used at 64% beside it, the tensor cores at 32%) and 10 at 256
 // rows (41 and 57%).  48 rows: 2,560 outputs of 9,728 inputs 12.6 us (of which some 3 us the launch and 3 us the join), 19,456 of 2,560 16.8 us, 151,936 of 2,560 78 us
-// (32-bit results 175: two products and twice the taking out); 128 and 256 rows, 19,456 of 2,560: 24 and 39 us.  (Steps on the way, 48 rows, 19,456 of 2,560: codes requested into registers, 1 us a unit of 64; weights
-// written into shared memory as the operand 22 us; into tensor memory 21.4, by then bound by the one thread that issued products, 500 cycles a unit to put their
-// operands into uniform registers; with a whole warp that walks the loop 17.5; one barrier for weights and x, asked ahead of the products before, 16.7.)
+// (32-bit results 175: two products and twice the taking out); 128 and 256 rows, 19,456 of 2,560: 24 and 39 us.
+// (Steps on the way, 48 rows, 19,456 of 2,560: weights written into shared memory as the operand 22 us; into tensor memory 21.4, by then bound by the one thread that
+// issued products, 500 cycles a unit to put their operands into uniform registers; with a whole warp that walks the loop 17.5; one barrier for weights and x, asked
+// ahead of the products before, 16.7.)
 //
 // Warps: 0 copies x, 1 issues the products, 22 copies codes (a lane each issues), 2 to 5 read the sums, 6 to 21 take weights out.  Every wait on a barrier is bounded by a clock; a
 // waiter that gives up raises *err, every role leaves its loop, the block lets its copies and products end and frees its tensor memory.
@@ -396,7 +397,10 @@ constexpr int JOIN_ROWS = 2;
 template <int NB, typename O>
 __global__ void __launch_bounds__(128) linear4_pieces_kernel(const float* pieces, O* y, int m, int n, unsigned blocks, unsigned tiles, unsigned G) {   // blocks: units of a tile
   const unsigned U = tiles * blocks, begin = blockIdx.x * blocks, first = block_of(U, G, begin), last = block_of(U, G, begin + blocks - 1);
-  if (first == last) return;
+  if (first == last) {   // (what follows this launch takes it that the one before is complete, also where no tile had pieces)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
   const int out = blockIdx.x * BM + threadIdx.x, m0 = blockIdx.y * JOIN_ROWS;
   constexpr size_t SLOT = (size_t)BM * NB;
   // the first block's last piece if its units began in the tile before; every other block begins with this tile
