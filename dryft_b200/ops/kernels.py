@@ -2636,9 +2636,11 @@ def linear4(x, w: Weight4, out=None, pdl: bool = False, mode: str = "store", nor
     first weights are requested while the launch before it drains).
 
     With few rows of bfloat16 (``linear4_fuses``) also what stands around a decoder's products: ``norm_w`` (float32 ``[k]``): RMS norm of ``x`` first;
-    ``mode="residual"``: ``out += `` the result, in place; ``mode="silu"``: ``w`` holds gate rows, then as many others, and ``out`` ``[m, n / 2]`` is
+    ``mode="residual"``: ``out += `` the result, in place (``out`` has to be given); ``mode="silu"``: ``w`` holds gate rows, then as many others, and ``out`` ``[m, n / 2]`` is
     ``silu(gate) * other``.  Rounding points are those of the bfloat16 products (``gemm_small_m``)."""
     global _linear4_fn, _linear4_tc_fn, launch_count
+    if out is None and mode == "residual":
+        raise KernelError("linear4: mode 'residual' adds to what out holds; no out was given")
     _need_weight4(w)
     step = _rows_in(x, "x", w.k)
     m = x.shape[0]
