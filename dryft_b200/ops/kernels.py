@@ -2592,6 +2592,13 @@ def _rows_in(x, name: str, width: int) -> int:
     return step
 
 
+def _words(t, name: str, numbers: int) -> None:
+    """A contiguous tensor that a kernel reads or writes in words of so many numbers begins on such a word's boundary (a view into another tensor may not)."""
+    word = numbers * t.element_size()
+    if t.data_ptr() % word:
+        raise KernelError(f"{name}: begins on a {word}-byte boundary, as words of {numbers} numbers do (address {t.data_ptr():#x})")
+
+
 def linear4_tc_lib() -> ctypes.CDLL:
     """Products of up to 256 rows with weights held in 4 bits (tcgen05, tensor memory, TMA)."""
     lib = _single_lib("linear4_tc", {"dryft_linear4_tc": [_i, _p, _ll, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p]})
@@ -2690,6 +2697,7 @@ def weight4_expand(w: Weight4, out, rest: bool = False) -> None:
     is_bf16 = _act(out, "out")
     if rest and not is_bf16:
         raise KernelError("weight4_expand: the rest of a rounding is bfloat16")
+    _words(out, "out", 4)
     _ok(linear4_lib().dryft_weight4_expand(2 if rest else is_bf16, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), w.n, w.k, w.group, _stream()),
         "weight4_expand")
 
@@ -2794,6 +2802,7 @@ def kv4_rope_store(qkv, q_norm_w, k_norm_w, inv_freq, tok_slot, tok_pos, q_out, 
     heads, page = _kv4_pages(k_pages, v_pages, page_table, head_dim, group)
     if heads != n_kv_heads:
         raise KernelError(f"kv4_rope_store: {n_kv_heads} key heads, the pages have {heads}")
+    _words(qkv, "qkv", 2)
     if rotary_dim < 0 or rotary_dim % 2 or rotary_dim > head_dim:
         raise KernelError(f"kv4_rope_store: {rotary_dim} rotated dims of a head of {head_dim}")
     has_norm = q_norm_w is not None
@@ -2840,6 +2849,8 @@ def kv4_expand(k_pages, v_pages, page_table, cu_q, seq_slot, tok_pos, k_out, v_o
         raise KernelError("kv4_expand: cu_q is shorter than the sequences")
     if n > 65535:
         raise KernelError(f"kv4_expand takes up to 65,535 sequences, got {n}")
+    _words(k_out, "k_out", 4)
+    _words(v_out, "v_out", 4)
     pages = most = page_table.shape[1]
     if max_kv > 0:
         pages = min((max_kv + page - 1) // page, most)
@@ -2910,6 +2921,9 @@ def attn4_rows(q, k_pages, v_pages, page_table, tok_slot, tok_pos, out, scale: f
     if rest:
         raise KernelError(f"attn4_rows: {n_heads} query heads are not a multiple of {n_kv} kv heads")
     _need(out, "attention output", q.dtype, (n, n_heads * d))
+    if is_bf16:   # (the 32-bit kernel reads and writes number by number)
+        _words(q, "q", 4)
+        _words(out, "attention output", 2)
     _tokens(tok_slot, tok_pos, n, "attn4_rows")
     if window is not None and window <= 0:
         raise KernelError(f"attn4_rows: a window is a positive number of keys, got {window}")
