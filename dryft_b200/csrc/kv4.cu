@@ -99,23 +99,31 @@ __device__ __forceinline__ constexpr unsigned round_bits(unsigned places) {   //
   return sum;
 }
 
-// Consecutive numbers of a row: two or four, on a boundary of as many
-template <typename T, int N> __device__ __forceinline__ void load_row(float (&x)[N], const T* p) {
+// Four consecutive numbers of a row in shared memory, on a boundary of as many
+template <typename T> __device__ __forceinline__ void load_four(float (&x)[4], const T* p) {
   if constexpr (sizeof(T) == 4) {
-    if constexpr (N == 4) {
-      const float4 v = *reinterpret_cast<const float4*>(p);
-      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-    } else {
-      const float2 v = *reinterpret_cast<const float2*>(p);
-      x[0] = v.x; x[1] = v.y;
-    }
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
   } else {
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
+    for (int i = 0; i < 4; i += 2) {
       const unsigned v = reinterpret_cast<const unsigned*>(p)[i / 2];
       x[i] = __uint_as_float(v << 16);
       x[i + 1] = __uint_as_float(v & 0xffff0000u);
     }
+  }
+}
+// What the launch before wrote, past L1 (`ld_prev`): a number, or two on a boundary of as many
+__device__ __forceinline__ float prev(const float* p) { return ld_prev(p); }
+__device__ __forceinline__ float prev(const __nv_bfloat16* p) { return ld_prev_bf16(p); }
+template <typename T> __device__ __forceinline__ void prev_two(float (&x)[2], const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    const float2 v = ld_prev(reinterpret_cast<const float2*>(p));
+    x[0] = v.x; x[1] = v.y;
+  } else {
+    const unsigned v = ld_prev(reinterpret_cast<const unsigned*>(p));
+    x[0] = __uint_as_float(v << 16);
+    x[1] = __uint_as_float(v & 0xffff0000u);
   }
 }
 
@@ -152,7 +160,7 @@ template <typename T> __device__ __forceinline__ void load_key(float (&x)[2][4],
   for (int p = 0; p < 2; ++p) {
     const int at = 32 * (part >> 2) + 16 * p + 4 * (part & 3);
     x[p][0] = x[p][1] = x[p][2] = x[p][3] = 0.f;
-    if (have && at < d) load_row<T, 4>(x[p], row + at);
+    if (have && at < d) load_four<T>(x[p], row + at);
   }
 }
 template <int GS> __device__ __forceinline__ void store_key(const float (&x)[2][4], bool have, int part, unsigned char* tile, int t, int d, int page) {
@@ -212,7 +220,7 @@ __device__ __forceinline__ void store_value(const T* row, unsigned char* tile, i
       Range range;
       const int at = 32 * u + 16 * p + 2 * r;
       if (at < d) {
-        load_row<T, 2>(x[p], row + at);
+        prev_two<T>(x[p], row + at);
         range.add(x[p][0]);
         range.add(x[p][1]);
       }
@@ -451,7 +459,8 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_store_kernel(const T* k, const
 }
 
 // The same behind a fused projection (rows q | k | v): per-head norm and rotation of queries and keys first, a warp per (token, head).  Formulas and
-// rounding points are those of rope_kv.cu.  A programmatic dependent: a decode step's launch is some 3 us of latency (loads, a norm's sum, angles, a range), no rate.
+// rounding points are those of rope_kv.cu.  A programmatic dependent, so rows and angles are read past L1.  A decode step's launch is some 3 us of latency (loads, a
+// norm's sum, angles, a range), no rate.
 template <typename T>
 __global__ void __launch_bounds__(WARPS * 32) kv4_rope_store_kernel(const T* qkv, int stride, const float* __restrict__ wq, const float* __restrict__ wk,
                                                                     const float* __restrict__ inv_freq, const T* cs_table, const int* __restrict__ tok_slot,
@@ -480,7 +489,7 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_rope_store_kernel(const T* qkv
   float x[8], ss = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    x[i] = lane + 32 * i < d ? to_f32<T>(src[lane + 32 * i]) : 0.f;
+    x[i] = lane + 32 * i < d ? prev(src + lane + 32 * i) : 0.f;
     ss = fmaf(x[i], x[i], ss);
   }
   const float inv = has_norm ? rsqrtf(warp_sum(ss) / (float)d + eps) : 1.f;
@@ -491,8 +500,8 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_rope_store_kernel(const T* qkv
   for (int j = lane; j < half; j += 32) {
     float sn, cs;
     if (cs_table != nullptr) {
-      cs = to_f32<T>(cs_table[n * rot + j]);
-      sn = to_f32<T>(cs_table[n * rot + half + j]);
+      cs = prev(cs_table + n * rot + j);
+      sn = prev(cs_table + n * rot + half + j);
     } else {
       sincosf((float)pos * inv_freq[j], &sn, &cs);
       cs = rnd<T>(cs);
