@@ -46,6 +46,29 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], unsigned a0, unsigned a
 }
 constexpr unsigned ONES_BF16 = 0x3f803f80u;   // two ones: a product with them sums the other operand, in the places where its products are
 
+// One output of a product, straight from its definition: sum over the inputs, in their order, of (z + (c - 7.5) s) x, for row `row` of the weights (linear4.cu has their
+// layout), x(i) being the activations.  By one thread and slow: for results that are not finite.  Where one of the sums that the fast forms are made of is an infinity,
+// what they add to it may be its opposite, and the NaN that they end in need not be the product's.
+template <typename X> __device__ __forceinline__ float defined_product(const uint4* codes, const uint2* scales, int row, int k, int group_bits, X x) {
+  const int wide = (k + 127) / 128 * 128, r = row & 7, h = row >> 3 & 1;   // inputs as laid out
+  const size_t tile = row >> 4;
+  codes += tile * (wide / 64) * 32 + r * 4;
+  scales += tile * (wide >> group_bits) * 8 + r;
+  float sum = 0.f;
+#pragma unroll 1
+  for (int at = 0; at < k; at += 16) {   // a step: word s of the four lanes of a row of its block
+    const uint2 sz = scales[(at >> group_bits) * 8];
+    const GroupCode g = unpack_code(h ? sz.y : sz.x);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const unsigned word = reinterpret_cast<const unsigned*>(codes + (at >> 6) * 32 + c)[at >> 4 & 3];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum = fmaf(value_of(word >> (4 * (2 * (e >> 1) + h) + 16 * (e & 1)) & 15u, g), x(at + 4 * c + e), sum);
+    }
+  }
+  return sum;
+}
+
 // ---------------------------------------------------------------------------------------------- the cache's pages
 // A page of one key head is one tile of bytes: its tokens' codes, then [token][group] of (s, z).  A token's codes take ROW = 16 ceil(d / 32) bytes.
 //

@@ -155,6 +155,11 @@ template <int NT, int GS, int TEAM, int PB, int SLOTS> struct Few {
 enum Mode { STORE_BF16 = 0, STORE_F32 = 1, RESIDUAL = 2, SILU = 3 };
 __device__ __forceinline__ float bfr(float v) { return rnd<bf16>(v); }
 
+// A result that is not finite, worked out again from the definition (x: a row in shared memory)
+__device__ __noinline__ float defined_result(const uint4* codes, const uint2* scales, int row, int k, int group_bits, const unsigned char* x) {
+  return defined_product(codes, scales, row, k, group_bits, [x](int i) { return __bfloat162float(reinterpret_cast<const bf16*>(x)[i]); });
+}
+
 // ALONE: no norm, and the result is stored (one row, 151,936 outputs of 2,560 inputs: 56.2 us so, 57.9 where the kernel asks what to do)
 template <int NT, int GS, int TEAM, int PB, int SLOTS, bool ALONE>
 __global__ void __launch_bounds__(FEW_WARPS * 32, 1) linear4_few_kernel(const bf16* x, long long x_stride, const uint4* __restrict__ codes,
@@ -310,6 +315,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) linear4_few_kernel(const bf
 #pragma unroll
       for (int w = 0; w < TEAM; ++w) v += place[w * NT * 128];
       if (row >= n || col >= m) continue;
+      if (!(fabsf(v) < INFINITY)) v = defined_result(codes, scales, row + (tile & 1) * half * 16, k, group_bits, rows + (size_t)col * row_bytes);
       bf16* const to = reinterpret_cast<bf16*>(y) + (size_t)col * n + row;
       if (mode == STORE_BF16) {
         *to = __float2bfloat16_rn(v);
