@@ -105,7 +105,15 @@ __device__ __forceinline__ void tmem_ld16(unsigned taddr, float (&v)[16]) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-struct Params { void* y; float* pieces; int* err; int m, n, blocks, group_bits, tiles; };
+struct Inputs { const bf16* x; long long x_stride; const uint4* codes; const uint2* scales; int k, group_bits; };
+struct Params { void* y; float* pieces; int* err; int m, n, blocks, group_bits, tiles; Inputs in; };
+
+// A 32-bit result that is not finite, worked out again from the definition: an infinity times a weight and times the rest of its rounding, which may be 0 or of the other sign,
+// is not what it is times their sum.
+__device__ __noinline__ float defined_result(const Inputs& in, int row, int m) {
+  const bf16* const x = in.x + m * in.x_stride;
+  return defined_product(in.codes, in.scales, row, in.k, in.group_bits, [x](int i) { return ld_prev_bf16(x + i); });
+}
 
 // KU: blocks of 64 inputs in a unit, two where enough stages of x fit: every handshake between the roles costs the same for twice the work (48 rows, 19,456
 // outputs of 2,560 inputs: 28.6 us with units of 64 inputs).  GN: groups that begin in a unit.
@@ -171,7 +179,7 @@ template <int GN, bool LOW, int KU> __device__ __forceinline__ void take_out(uns
 
 template <int NB, int GN, bool LOW>
 __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_codes,
-                                                                   const __grid_constant__ CUtensorMap map_scales, const Params p) {
+                                                                   const __grid_constant__ CUtensorMap map_scales, const __grid_constant__ Params p) {
   typedef Layout<NB, GN, LOW> L;
   constexpr int STAGES = L::STAGES, RING = L::RING, KU = L::KU;
   extern __shared__ unsigned char smem_raw[];
@@ -306,6 +314,18 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
               if (LOW) reinterpret_cast<float*>(p.y)[(size_t)(m0 + j) * p.n + out] = v[j];
               else reinterpret_cast<bf16*>(p.y)[(size_t)(m0 + j) * p.n + out] = __float2bfloat16_rn(v[j]);
             }
+          if constexpr (LOW) {
+            bool finite = true;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) finite = finite && (m0 + j >= p.m || fabsf(v[j]) < INFINITY);
+            if (!finite && out < p.n)
+#pragma unroll 1
+              for (int j = 0; j < 16 && m0 + j < p.m; ++j) {
+                float* const at = reinterpret_cast<float*>(p.y) + (size_t)(m0 + j) * p.n + out;
+                if (!(fabsf(*at) < INFINITY)) *at = defined_result(p.in, out, m0 + j);
+              }
+            __syncwarp();   // the next read of tensor memory is the whole warp's
+          }
         } else {
 #pragma unroll
           for (int j = 0; j < 16; ++j)
@@ -395,7 +415,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
 // Tiles that several blocks had pieces of: a block per tile and two rows of x, a thread per W row; the pieces in the blocks' order.
 constexpr int JOIN_ROWS = 2;
 template <int NB, typename O>
-__global__ void __launch_bounds__(128) linear4_pieces_kernel(const float* pieces, O* y, int m, int n, unsigned blocks, unsigned tiles, unsigned G) {   // blocks: units of a tile
+__global__ void __launch_bounds__(128) linear4_pieces_kernel(const float* pieces, O* y, int m, int n, unsigned blocks, unsigned tiles, unsigned G,   // blocks: units of a tile
+                                                             const __grid_constant__ Inputs in) {
   const unsigned U = tiles * blocks, begin = blockIdx.x * blocks, first = block_of(U, G, begin), last = block_of(U, G, begin + blocks - 1);
   if (first == last) {   // (what follows this launch takes it that the one before is complete, also where no tile had pieces)
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -418,7 +439,10 @@ __global__ void __launch_bounds__(128) linear4_pieces_kernel(const float* pieces
   if (out < n)
 #pragma unroll
     for (int j = 0; j < JOIN_ROWS; ++j)
-      if (m0 + j < m) y[(size_t)(m0 + j) * n + out] = from_f32<O>(v[j]);
+      if (m0 + j < m) {
+        if (sizeof(O) == 4 && !(fabsf(v[j]) < INFINITY)) v[j] = defined_result(in, out, m0 + j);
+        y[(size_t)(m0 + j) * n + out] = from_f32<O>(v[j]);
+      }
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
@@ -497,7 +521,7 @@ template <int NB, int GN, bool LOW> int run(const Operands& o, const Params& p, 
   if (rc || G == p.tiles) return rc;   // (a tile a block: no pieces)
   typedef typename std::conditional<LOW, float, bf16>::type O;
   return launch(linear4_pieces_kernel<NB, O>, dim3(p.tiles, (p.m + JOIN_ROWS - 1) / JOIN_ROWS), 128, 0, true, st, (const float*)p.pieces, (O*)p.y, p.m, p.n,
-                units, p.tiles, G);
+                units, p.tiles, G, p.in);
 }
 template <int NB, bool LOW> int by_group(const Operands& o, const Params& p, int pdl, cudaStream_t st) {
   constexpr int WIDE = 64 * units_of<NB>();   // inputs of a unit
@@ -521,7 +545,8 @@ DRYFT_API int dryft_linear4_tc(int out_f32, const void* x, long long x_stride, c
   if (m > 256 || k <= 0 || k % 16) return DRYFT_ERR_UNSUPPORTED;
   const Operands o = {encode_fn(), x, codes, scales, x_stride, k, group};
   if (!o.enc) return DRYFT_ERR_UNSUPPORTED;
-  const Params p = {y, pieces, err, m, n, blocks_of(k), __builtin_ctz(group), (n + BM - 1) / BM};
+  const Params p = {y, pieces, err, m, n, blocks_of(k), __builtin_ctz(group), (n + BM - 1) / BM,
+                    {(const bf16*)x, x_stride, (const uint4*)codes, (const uint2*)scales, k, __builtin_ctz(group)}};
   const cudaStream_t st = (cudaStream_t)stream;
 #define DRYFT_TC(NB) (out_f32 ? by_group<NB, true>(o, p, pdl, st) : by_group<NB, false>(o, p, pdl, st))
   switch (padded_rows(m)) {

@@ -65,3 +65,15 @@ def test_few_rows_with_a_sum_or_activation_behind(m):
     K().linear4(xd, w4, act, mode="silu")
     K().silu_mul(plain, want)
     assert torch.equal(act.isnan(), want.isnan()) and torch.equal(act.nan_to_num(nan=7.0), want.nan_to_num(nan=7.0))
+
+
+@pytest.mark.parametrize("out", [BF, F32])
+@pytest.mark.parametrize("n,k,group", [(40, 80, 16), (37, 128, 64), (250, 1280, 128), (129, 2432, 32)])
+@pytest.mark.parametrize("m", [17, 48, 130, 256])
+def test_weights_taken_out_tile_by_tile(m, n, k, group, out):
+    w, x = _inputs(m, n, k, BF)
+    values = P.group_values(w, group)[0]
+    y = K().linear4(x.to(DEV), K().pack_weight4(w.to(DEV), group), out_dtype=out)
+    K().check_error_flags()
+    for i in range(0, m, 16):
+        _check(y[i:i + 16], x[i:i + 16], values)
