@@ -88,6 +88,8 @@ def _linear4(x: torch.Tensor, w: K.Weight4, rt: Runtime, out_dtype: torch.dtype)
     # Rows of results that begin anywhere send the library to a product that cuts the sums over the inputs and adds the parts up in bfloat16 (685 rows, 439 outputs of
     # 8,496 inputs: off by 0.0044 of the whole instead of 0.0017, and 108 us instead of 13).  It is given whole tiles of 16 outputs then, and what they are copied.
     whole = x.dtype == torch.float32 or n % 8 == 0
+    # (an infinity's product with a weight's rest may be the opposite of its product with the weight, or NaN: the rests take their part in finite numbers only)
+    finite = torch.nan_to_num(x, nan=0.0, posinf=0.0, neginf=0.0) if out_dtype == torch.float32 and x.dtype == torch.bfloat16 else x
     for first in range(0, n, step):
         end = min(n, first + step)
         rows, at = w if end - first == n else w.rows(first, end), out[:, first:end]
@@ -107,7 +109,7 @@ def _linear4(x: torch.Tensor, w: K.Weight4, rt: Runtime, out_dtype: torch.dtype)
         else:
             y = torch.mm(x, wide.t(), out_dtype=out_dtype)
             K.weight4_expand(rows, part, rest=True)
-            torch.add(y[:, :end - first], torch.mm(x, wide.t(), out_dtype=out_dtype)[:, :end - first], out=at)
+            torch.add(y[:, :end - first], torch.mm(finite, wide.t(), out_dtype=out_dtype)[:, :end - first], out=at)
     return out
 
 

@@ -77,3 +77,14 @@ def test_weights_taken_out_tile_by_tile(m, n, k, group, out):
     K().check_error_flags()
     for i in range(0, m, 16):
         _check(y[i:i + 16], x[i:i + 16], values)
+
+
+@pytest.mark.parametrize("dtype,out", [(BF, BF), (BF, F32), (F32, F32)])
+@pytest.mark.parametrize("n", [40, 37])
+def test_many_rows(n, dtype, out):
+    from dryft_b200.parts.base import Runtime
+    from dryft_b200.parts.linear import linear
+
+    w, x = _inputs(300, n, 320, dtype)
+    y = linear(x.to(DEV), K().pack_weight4(w.to(DEV), 64), Runtime(dtype=dtype, device=torch.device(DEV)), out_dtype=out)
+    _check(y, x, P.group_values(w, 64)[0])
