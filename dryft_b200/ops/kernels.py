@@ -2542,7 +2542,7 @@ def _group_codes(x: torch.Tensor, group: int) -> Tuple[torch.Tensor, torch.Tenso
 
 def pack_weight4(w: torch.Tensor, group: int = 64) -> Weight4:
     """``w`` ``[n, k]`` (float32 or bfloat16) in 4 bits: rounded to the nearest code of its group, laid out for the products.  ``k`` is a multiple of
-    ``group`` (16, 32, 64 or 128).  Done once, when weights are loaded."""
+    ``group`` (16, 32, 64 or 128).  Done once, when weights are loaded.  Products on the same stream may follow at once, overlapped or not."""
     _act(w, "weight")
     if w.dim() != 2:
         raise KernelError(f"pack_weight4: a weight is [outputs, inputs], got shape {tuple(w.shape)}")
@@ -2567,6 +2567,9 @@ def pack_weight4(w: torch.Tensor, group: int = 64) -> Weight4:
         fs = torch.zeros(nt * 16, groups, 2, dtype=torch.bfloat16, device=w.device)
         fs[:part.shape[0], :k // group] = sz
         scales[t0:t0 + nt] = fs.view(nt, 2, 8, groups, 2).permute(0, 3, 2, 1, 4)
+    # Products that overlap the launch in front of them ask for their first weights before that launch has ended.  This one begins when all of the above is in memory,
+    # so it is there for whatever comes next.
+    torch.zeros(1, device=w.device)
     return Weight4(codes, scales, n, k, group)
 
 
@@ -2639,8 +2642,9 @@ _LINEAR4_MODES = {"store": 0, "residual": 2, "silu": 3}
 
 def linear4(x, w: Weight4, out=None, pdl: bool = False, mode: str = "store", norm_w=None, eps: float = 0.0, out_dtype=None):
     """``out = x @ w.T``; ``x`` bfloat16, up to 256 rows (float32: 64), ``out`` of the same type or float32 (none: a new tensor, of ``out_dtype`` or ``x``'s
-    type).  Returns ``out``.  ``pdl``: a programmatic dependent (its
-    first weights are requested while the launch before it drains).  Where ``x`` is infinite or not a number the result is what the definition's sum
+    type).  Returns ``out``.  ``pdl``: a programmatic dependent: its
+    first weights are requested while the launch before it drains, so codes and scales are older than the last launch in front of it that is not such a
+    dependent itself (``pack_weight4`` sees to that for those it makes).  Where ``x`` is infinite or not a number the result is what the definition's sum
     comes to (a result that is not finite is worked out again, input by input).
 
     With few rows of bfloat16 (``linear4_fuses``) also what stands around a decoder's products: ``norm_w`` (float32 ``[k]``): RMS norm of ``x`` first;
@@ -2796,7 +2800,7 @@ def kv4_rope_store(qkv, q_norm_w, k_norm_w, inv_freq, tok_slot, tok_pos, q_out, 
                    head_dim: int, rotary_dim: int, eps: float, group: int, cs_table=None, pdl: bool = False) -> None:
     """``qk_norm_rope_store`` with the cache in 4 bits: per-head norm and rotation of the rows' queries and keys, queries to ``q_out``, keys and values into
     the cache as ``kv4_store`` puts them there.  ``cs_table`` as there.  ``pdl``: a programmatic dependent; ``tok_slot``, ``tok_pos`` and ``page_table`` are
-    then older than the launch before it."""
+    then older than the last launch in front of it that is not such a dependent itself."""
     n = qkv.shape[0]
     width = (n_heads + 2 * n_kv_heads) * head_dim
     _need(qkv, "qkv", None, (n, width))
@@ -2911,8 +2915,8 @@ def attn4_plan(blocks: int, max_kv: int, window: Optional[int], bf16: bool) -> T
 def attn4_rows(q, k_pages, v_pages, page_table, tok_slot, tok_pos, out, scale: float, window: Optional[int], group: int, max_kv: int, pdl: bool = False) -> None:
     """Attention of ``n`` query rows ``q`` ``[n, heads, head_dim]`` over the cache in 4 bits: row ``i`` sees the keys 0..``tok_pos[i]`` (the last ``window``
     of them) of slot ``tok_slot[i]``; a row of slot -1 is padding and gets zeros.  ``max_kv``: no sequence is longer (a bound; how the keys are cut
-    over blocks follows from it).  ``pdl``: a programmatic dependent; ``tok_slot``, ``tok_pos`` and ``page_table`` are then older than the launch
-    before it."""
+    over blocks follows from it).  ``pdl``: a programmatic dependent; ``tok_slot``, ``tok_pos`` and ``page_table`` are then older than the last
+    launch in front of it that is not such a dependent itself."""
     if not isinstance(q, torch.Tensor) or q.dim() != 3:
         raise KernelError("attn4_rows: q is [rows, heads, head size]")
     n, n_heads, d = q.shape

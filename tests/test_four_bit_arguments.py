@@ -114,3 +114,25 @@ def test_a_projections_rows_begin_on_a_word(launches, dtype, at):
     else:
         call()
     assert len(launches) == (at % 2 == 0)
+
+
+@pytest.mark.parametrize("n,k", [(40, 64), (70, 128)])
+def test_a_launch_stands_behind_the_last_write_of_packed_weights(n, k):
+    """A product that overlaps the launch in front of it asks for its weights before that launch has ended: that launch must not be the one that wrote them."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    made = []   # of every operation that writes: the memory it writes to
+
+    class Ops(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            to = [a for a, info in zip(args, func._schema.arguments) if info.alias_info is not None and info.alias_info.is_write]
+            if not to and not any(r.alias_info for r in func._schema.returns) and "empty" not in str(func):
+                to = [out] if isinstance(out, torch.Tensor) else []
+            made.extend(t.untyped_storage().data_ptr() for t in to)
+            return out
+
+    with Ops():
+        w4 = K.pack_weight4(torch.randn(n, k))
+    mine = {t.untyped_storage().data_ptr() for t in (w4.codes, w4.scales)}
+    assert mine <= set(made) and made[-1] not in mine
