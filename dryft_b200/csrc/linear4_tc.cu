@@ -537,6 +537,11 @@ template <int NB, bool LOW> int by_group(const Operands& o, const Params& p, int
 
 // Floats of the workspace that a launch needs.
 DRYFT_API long long dryft_linear4_tc_pieces(int m, int n, int k) { return 2ll * grid_of(n, blocks_of(k)) * BM * padded_rows(m); }
+// Launches that it makes: one where every block has a whole tile, else a second one for the pieces.
+DRYFT_API int dryft_linear4_tc_launches(int m, int n, int k) {
+  const int units = blocks_of(k) / (padded_rows(m) == 256 ? units_of<256>() : units_of<128>());
+  return grid_of(n, units) == (n + BM - 1) / BM ? 1 : 2;
+}
 
 // y [m, n] = x [m, k] w^T, m <= 256; x bfloat16, rows x_stride numbers apart on 16-byte boundaries; y bfloat16 or (out_f32) float32.
 DRYFT_API int dryft_linear4_tc(int out_f32, const void* x, long long x_stride, const void* codes, const void* scales, void* y, float* pieces, int m, int n, int k,

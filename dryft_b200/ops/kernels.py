@@ -2604,7 +2604,7 @@ def _words(t, name: str, numbers: int) -> None:
 
 def linear4_tc_lib() -> ctypes.CDLL:
     """Products of up to 256 rows with weights held in 4 bits (tcgen05, tensor memory, TMA)."""
-    lib = _single_lib("linear4_tc", {"dryft_linear4_tc": [_i, _p, _ll, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p]})
+    lib = _single_lib("linear4_tc", {"dryft_linear4_tc": [_i, _p, _ll, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p], "dryft_linear4_tc_launches": [_i, _i, _i]})
     lib.dryft_linear4_tc_pieces.argtypes = [_i, _i, _i]
     lib.dryft_linear4_tc_pieces.restype = _ll
     return lib
@@ -2624,6 +2624,12 @@ def linear4_plan(m: int, n: int, k: int, group: int, bf16: bool, f32_out: bool =
     if takes == 1 or (takes and f32_out):
         return 0
     return int(linear4_tc_lib().dryft_linear4_tc_pieces(m, n, k))
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear4_launches(m: int, n: int, k: int) -> int:
+    """Launches of a product on the tensor memory kernel: a second one joins the pieces of tiles that several blocks share."""
+    return linear4_tc_lib().dryft_linear4_tc_launches(m, n, k)
 
 
 def linear4_fuses(m: int, w) -> bool:
@@ -2683,14 +2689,16 @@ def linear4(x, w: Weight4, out=None, pdl: bool = False, mode: str = "store", nor
         pieces = torch.empty(floats, dtype=torch.float32, device=x.device)
         rc = _linear4_tc_fn(not out_bf16, x.data_ptr(), step, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), pieces.data_ptr(), m, w.n, w.k, w.group,
                             pdl, error_flag(x.device).data_ptr(), _stream())
+        launches = _linear4_launches(m, w.n, w.k)
     else:
         if _linear4_fn is None:
             _linear4_fn = linear4_lib().dryft_linear4
         rc = _linear4_fn(is_bf16, code or not out_bf16, x.data_ptr(), step, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), m, w.n, w.k, w.group,
                          norm_w.data_ptr() if norm_w is not None else 0, eps, pdl, _stream())
+        launches = 1
     if rc:
         _ok(rc, "linear4")
-    launch_count += 1
+    launch_count += launches
     return out
 
 
