@@ -695,7 +695,7 @@ dim3 grid_of(const Args& a) { return dim3(a.splits, a.n_kv * HEAD_TILES, a.n); }
 
 template <typename T> int join(const Args& a) {
   const int total = a.n * a.n_kv * G;
-  return launch(attn4_join_kernel<T>, dim3((total + THREADS / 32 - 1) / (THREADS / 32)), THREADS, 0, 1, true, a.st, a.part_o, a.part_ml, a.tok_slot, (T*)a.out, a.n_kv * G,
+  return launch(attn4_join_kernel<T>, dim3((total + THREADS / 32 - 1) / (THREADS / 32)), THREADS, 0, 1, a.pdl & 2, a.st, a.part_o, a.part_ml, a.tok_slot, (T*)a.out, a.n_kv * G,
                 total, a.splits);
 }
 
@@ -717,13 +717,14 @@ template <int WARPS> int rows_bf16(const Args& a) {
   }
   const int cluster = a.splits > 1 && a.part_o == nullptr;
   if (cluster && a.splits > MOST_SPLITS) return DRYFT_ERR_UNSUPPORTED;
-  const int rc = launch(attn4_mma_kernel<WARPS>, grid_of(a), WARPS * 32, Block<WARPS>::SMEM, cluster ? a.splits : 1, a.pdl != 0, a.st, (const bf16*)a.q,
+  const int rc = launch(attn4_mma_kernel<WARPS>, grid_of(a), WARPS * 32, Block<WARPS>::SMEM, cluster ? a.splits : 1, a.pdl & 1, a.st, (const bf16*)a.q,
                         (const unsigned char*)a.k_pages, (const unsigned char*)a.v_pages, a.page_table, a.max_pages, a.tok_slot, a.tok_pos, (bf16*)a.out, a.part_o,
                         a.part_ml, cluster, a.least, a.scale, a.window);
   return rc || a.splits == 1 || cluster ? rc : join<bf16>(a);
 }
 }  // namespace
 
+// pdl: 1, the first launch is a programmatic dependent of the one before it (not in 32 bits); 2, the joining launch is one of the first; both or neither.
 DRYFT_API int dryft_attn4_rows(int is_bf16, const void* q, const void* k_pages, const void* v_pages, const int* page_table, int max_pages, const int* tok_slot,
                                const int* tok_pos, void* out, float* part_o, float* part_ml, int n, int n_kv, int splits, int least, int warps, float scale, int window,
                                int pdl, void* stream) {

@@ -403,7 +403,7 @@ template <typename... P, typename... A> int launch(void (*kern)(P...), bool (&as
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
+  cfg.numAttrs = pdl & 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, (P)a...);
   return e != cudaSuccess ? (int)e : launch_status();
 }

@@ -517,10 +517,10 @@ template <int NB, int GN, bool LOW> int run(const Operands& o, const Params& p, 
     if (e != cudaSuccess) return (int)e;
     asked[dev] = true;
   }
-  const int rc = launch(kern, dim3(G), WARPS * 32, L::SMEM_BYTES, pdl != 0, st, x, codes, scales, p);
+  const int rc = launch(kern, dim3(G), WARPS * 32, L::SMEM_BYTES, pdl & 1, st, x, codes, scales, p);
   if (rc || G == p.tiles) return rc;   // (a tile a block: no pieces)
   typedef typename std::conditional<LOW, float, bf16>::type O;
-  return launch(linear4_pieces_kernel<NB, O>, dim3(p.tiles, (p.m + JOIN_ROWS - 1) / JOIN_ROWS), 128, 0, true, st, (const float*)p.pieces, (O*)p.y, p.m, p.n,
+  return launch(linear4_pieces_kernel<NB, O>, dim3(p.tiles, (p.m + JOIN_ROWS - 1) / JOIN_ROWS), 128, 0, pdl & 2, st, (const float*)p.pieces, (O*)p.y, p.m, p.n,
                 units, p.tiles, G, p.in);
 }
 template <int NB, bool LOW> int by_group(const Operands& o, const Params& p, int pdl, cudaStream_t st) {
@@ -544,6 +544,7 @@ DRYFT_API int dryft_linear4_tc_launches(int m, int n, int k) {
 }
 
 // y [m, n] = x [m, k] w^T, m <= 256; x bfloat16, rows x_stride numbers apart on 16-byte boundaries; y bfloat16 or (out_f32) float32.
+// pdl: 1, the product is a programmatic dependent of the launch before it; 2, the pieces' launch is one of the product; both or neither.
 DRYFT_API int dryft_linear4_tc(int out_f32, const void* x, long long x_stride, const void* codes, const void* scales, void* y, float* pieces, int m, int n, int k,
                                int group, int pdl, int* err, void* stream) {
   if (m <= 0 || n <= 0) return 0;

@@ -2646,11 +2646,16 @@ LINEAR4_NORM_ROWS = 4
 _LINEAR4_MODES = {"store": 0, "residual": 2, "silu": 3}
 
 
-def linear4(x, w: Weight4, out=None, pdl: bool = False, mode: str = "store", norm_w=None, eps: float = 0.0, out_dtype=None):
+def _overlap(pdl: Optional[bool]) -> int:
+    """Which launches are programmatic dependents: 1, an operator's first one; 2, its second one, of the first."""
+    return 3 if pdl else 2 if pdl is None else 0
+
+
+def linear4(x, w: Weight4, out=None, pdl: Optional[bool] = None, mode: str = "store", norm_w=None, eps: float = 0.0, out_dtype=None):
     """``out = x @ w.T``; ``x`` bfloat16, up to 256 rows (float32: 64), ``out`` of the same type or float32 (none: a new tensor, of ``out_dtype`` or ``x``'s
     type).  Returns ``out``.  ``pdl``: a programmatic dependent: its
     first weights are requested while the launch before it drains, so codes and scales are older than the last launch in front of it that is not such a
-    dependent itself (``pack_weight4`` sees to that for those it makes).  Where ``x`` is infinite or not a number the result is what the definition's sum
+    dependent itself (``pack_weight4`` sees to that for those it makes); ``False``: no launch overlaps another; ``None``: only a second launch of this product its first.  Where ``x`` is infinite or not a number the result is what the definition's sum
     comes to (a result that is not finite is worked out again, input by input).
 
     With few rows of bfloat16 (``linear4_fuses``) also what stands around a decoder's products: ``norm_w`` (float32 ``[k]``): RMS norm of ``x`` first;
@@ -2688,13 +2693,13 @@ def linear4(x, w: Weight4, out=None, pdl: bool = False, mode: str = "store", nor
             _linear4_tc_fn = linear4_tc_lib().dryft_linear4_tc
         pieces = torch.empty(floats, dtype=torch.float32, device=x.device)
         rc = _linear4_tc_fn(not out_bf16, x.data_ptr(), step, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), pieces.data_ptr(), m, w.n, w.k, w.group,
-                            pdl, error_flag(x.device).data_ptr(), _stream())
+                            _overlap(pdl), error_flag(x.device).data_ptr(), _stream())
         launches = _linear4_launches(m, w.n, w.k)
     else:
         if _linear4_fn is None:
             _linear4_fn = linear4_lib().dryft_linear4
         rc = _linear4_fn(is_bf16, code or not out_bf16, x.data_ptr(), step, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), m, w.n, w.k, w.group,
-                         norm_w.data_ptr() if norm_w is not None else 0, eps, pdl, _stream())
+                         norm_w.data_ptr() if norm_w is not None else 0, eps, _overlap(pdl), _stream())
         launches = 1
     if rc:
         _ok(rc, "linear4")
@@ -2920,11 +2925,12 @@ def attn4_plan(blocks: int, max_kv: int, window: Optional[int], bf16: bool) -> T
     return s, 8, 8, s > 1
 
 
-def attn4_rows(q, k_pages, v_pages, page_table, tok_slot, tok_pos, out, scale: float, window: Optional[int], group: int, max_kv: int, pdl: bool = False) -> None:
+def attn4_rows(q, k_pages, v_pages, page_table, tok_slot, tok_pos, out, scale: float, window: Optional[int], group: int, max_kv: int,
+               pdl: Optional[bool] = None) -> None:
     """Attention of ``n`` query rows ``q`` ``[n, heads, head_dim]`` over the cache in 4 bits: row ``i`` sees the keys 0..``tok_pos[i]`` (the last ``window``
     of them) of slot ``tok_slot[i]``; a row of slot -1 is padding and gets zeros.  ``max_kv``: no sequence is longer (a bound; how the keys are cut
     over blocks follows from it).  ``pdl``: a programmatic dependent; ``tok_slot``, ``tok_pos`` and ``page_table`` are then older than the last
-    launch in front of it that is not such a dependent itself."""
+    launch in front of it that is not such a dependent itself; ``False``: no launch overlaps another; ``None``: only the one that joins splits the one before it."""
     if not isinstance(q, torch.Tensor) or q.dim() != 3:
         raise KernelError("attn4_rows: q is [rows, heads, head size]")
     n, n_heads, d = q.shape
@@ -2953,5 +2959,6 @@ def attn4_rows(q, k_pages, v_pages, page_table, tok_slot, tok_pos, out, scale: f
         part_o = parts.data_ptr()
         part_ml = part_o + 4 * n * n_heads * s * d
     _ok(lib.dryft_attn4_rows(is_bf16, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), page_table.shape[1], tok_slot.data_ptr(),
-                             tok_pos.data_ptr(), out.data_ptr(), part_o, part_ml, n, n_kv, s, least, warps, scale, window or 0, pdl, _stream()), "attn4_rows",
+                             tok_pos.data_ptr(), out.data_ptr(), part_o, part_ml, n, n_kv, s, least, warps, scale, window or 0, _overlap(pdl), _stream()),
+        "attn4_rows",
         n_kernels=2 if joined else 1)
