@@ -78,6 +78,8 @@ EXPAND_BYTES = 256 << 20   # of weights at a time that a product of many rows ta
 def _linear4(x: torch.Tensor, w: K.Weight4, rt: Runtime, out_dtype: torch.dtype) -> torch.Tensor:
     """Up to ``K.LINEAR4_ROWS`` rows the kernels read the codes; more rows take the weights out of their 4 bits, for the product that such rows run on
     otherwise.  For 32-bit results from bfloat16 activations the weights are taken out as two bfloat16 numbers whose sum they are, with a product each."""
+    if x.dtype == torch.float32 and out_dtype != torch.float32:   # as other weights: the 32-bit product, rounded once
+        return _linear4(x, w, rt, torch.float32).to(out_dtype)
     m = x.shape[0]
     if m <= (K.LINEAR4_ROWS if x.dtype == torch.bfloat16 else K.LINEAR4_ROWS_F32):
         return K.linear4(x, w, pdl=rt.pdl, out_dtype=out_dtype)

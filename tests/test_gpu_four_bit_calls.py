@@ -1,0 +1,31 @@
+"""Calls that the operators from 4 bits take as their 16-bit forms do."""
+
+import importlib
+
+import pytest
+import torch
+
+import plain_four_bit as P
+from test_gpu_four_bit import _near, _weights
+from test_gpu_kernels import DEV, K
+
+pytestmark = pytest.mark.gpu
+
+BF, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.mark.parametrize("m", [1, 64, 65, 200])
+@pytest.mark.parametrize("n", [40, 250])
+def test_32_bit_activations_and_a_result_of_16(m, n, monkeypatch):
+    """The 32-bit product, rounded once; weights taken out whole and in parts."""
+    L = importlib.import_module("dryft_b200.parts.linear")
+    from dryft_b200.parts.base import Runtime
+
+    w, x = _weights(n, 320, F32), torch.randn(m, 320)
+    w4, rt = K().pack_weight4(w.to(DEV), 64), Runtime(dtype=F32, device=torch.device(DEV))
+    for size in (L.EXPAND_BYTES, 64 * 320 * 4):
+        monkeypatch.setattr(L, "EXPAND_BYTES", size)
+        got, whole = L.linear(x.to(DEV), w4, rt, out_dtype=BF), L.linear(x.to(DEV), w4, rt)
+        values, s, _ = P.group_values(w, 64)
+        assert got.dtype == BF and torch.equal(got, whole.to(BF))
+        _near(whole, P.linear(x, values), P.linear_slack(x, values, s, 64, F32))
