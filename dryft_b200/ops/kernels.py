@@ -2801,7 +2801,7 @@ def kv4_store(k, v, tok_slot, tok_pos, k_pages, v_pages, page_table, group: int)
         if t.data_ptr() % 16 or (n > 1 and rows * (2 if is_bf16 else 4) % 16):
             raise KernelError(f"{nm}: rows start on 16-byte boundaries")
         if n > 1:
-            if t is v and rows != apart:
+            if nm == "v" and rows != apart:
                 raise KernelError("kv4_store: k and v rows lie equally far apart")
             apart = rows
     _tokens(tok_slot, tok_pos, n, "kv4_store")

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import plain_four_bit as P
-from test_gpu_four_bit import _near, _weights
+from test_gpu_four_bit import Cache, _near, _weights, i32
 from test_gpu_kernels import DEV, K
 
 pytestmark = pytest.mark.gpu
@@ -29,3 +29,17 @@ def test_32_bit_activations_and_a_result_of_16(m, n, monkeypatch):
         values, s, _ = P.group_values(w, 64)
         assert got.dtype == BF and torch.equal(got, whole.to(BF))
         _near(whole, P.linear(x, values), P.linear_slack(x, values, s, 64, F32))
+
+
+@pytest.mark.parametrize("n", [1, 5])
+def test_one_tensor_as_keys_and_values(n):
+    """Rows that lie apart, the same for both."""
+    c = Cache([n], 2, 64, 64)
+    rows = torch.randn(n, 5 * 64).to(BF)
+    c.keys[0] = c.values[0] = rows[:, 64:3 * 64].reshape(n, 2, 64)
+    c.fill()
+    want = c.k.clone(), c.v.clone()
+    c.k.fill_(255), c.v.fill_(255)
+    both = rows.to(DEV)[:, 64:3 * 64].view(n, 2, 64)
+    K().kv4_store(both, both, i32([0] * n), i32(range(n)), c.k, c.v, c.pt, 64)
+    assert torch.equal(c.k, want[0]) and torch.equal(c.v, want[1])
