@@ -110,7 +110,7 @@ struct Params { void* y; float* pieces; int* err; int m, n, blocks, group_bits, 
 
 // A 32-bit result that is not finite, worked out again from the definition: an infinity times a weight and times the rest of its rounding, which may be 0 or of the other sign,
 // is not what it is times their sum.
-__device__ __noinline__ float defined_result(const Inputs& in, int row, int m) {
+__device__ __noinline__ float defined_result(const Inputs in, int row, int m) {   // (a copy: what is handed on by its address is read again behind every barrier)
   const bf16* const x = in.x + m * in.x_stride;
   return defined_product(in.codes, in.scales, row, in.k, in.group_bits, [x](int i) { return ld_prev_bf16(x + i); });
 }
@@ -179,7 +179,7 @@ template <int GN, bool LOW, int KU> __device__ __forceinline__ void take_out(uns
 
 template <int NB, int GN, bool LOW>
 __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_codes,
-                                                                   const __grid_constant__ CUtensorMap map_scales, const __grid_constant__ Params p) {
+                                                                   const __grid_constant__ CUtensorMap map_scales, const Params p) {
   typedef Layout<NB, GN, LOW> L;
   constexpr int STAGES = L::STAGES, RING = L::RING, KU = L::KU;
   extern __shared__ unsigned char smem_raw[];
@@ -303,6 +303,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
       const int out = tile * BM + row;
       // a piece: of this block, its first tile's (0) or its last one's (1); [slot][NB][128]
       float* const piece = p.pieces + (size_t)(2 * blockIdx.x + (u0 < begin ? 1 : 0)) * BM * NB + row;
+      float none[2] = {0.f, 0.f};   // (LOW) of infinities and NaN among the tile's results
 #pragma unroll 1
       for (int m0 = 0; m0 < NB; m0 += 16) {
         float v[16];
@@ -315,16 +316,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
               else reinterpret_cast<bf16*>(p.y)[(size_t)(m0 + j) * p.n + out] = __float2bfloat16_rn(v[j]);
             }
           if constexpr (LOW) {
-            bool finite = true;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) finite = finite && (m0 + j >= p.m || fabsf(v[j]) < INFINITY);
-            if (!finite && out < p.n)
-#pragma unroll 1
-              for (int j = 0; j < 16 && m0 + j < p.m; ++j) {
-                float* const at = reinterpret_cast<float*>(p.y) + (size_t)(m0 + j) * p.n + out;
-                if (!(fabsf(*at) < INFINITY)) *at = defined_result(p.in, out, m0 + j);
-              }
-            __syncwarp();   // the next read of tensor memory is the whole warp's
+            for (int j = 0; j < 16; ++j) none[j & 1] = fmaf(v[j], 0.f, none[j & 1]);
           }
         } else {
 #pragma unroll
@@ -334,6 +327,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       mbar_arrive(&acc_empty[b]);
+      if (LOW && !(none[0] + none[1] == 0.f) && out < p.n)   // products go on meanwhile
+#pragma unroll 1
+        for (int m = 0; m < p.m; ++m) {
+          float* const at = reinterpret_cast<float*>(p.y) + (size_t)m * p.n + out;
+          if (!(fabsf(*at) < INFINITY)) *at = defined_result(p.in, out, m);
+        }
+      __syncwarp();   // reading tensor memory is the whole warp's
     }
   } else if (warp == 6 + TAKERS) {   // codes depend on no earlier launch
     const bool issues = elected();
@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
 constexpr int JOIN_ROWS = 2;
 template <int NB, typename O>
 __global__ void __launch_bounds__(128) linear4_pieces_kernel(const float* pieces, O* y, int m, int n, unsigned blocks, unsigned tiles, unsigned G,   // blocks: units of a tile
-                                                             const __grid_constant__ Inputs in) {
+                                                             const Inputs in) {
   const unsigned U = tiles * blocks, begin = blockIdx.x * blocks, first = block_of(U, G, begin), last = block_of(U, G, begin + blocks - 1);
   if (first == last) {   // (what follows this launch takes it that the one before is complete, also where no tile had pieces)
     asm volatile("griddepcontrol.wait;" ::: "memory");
