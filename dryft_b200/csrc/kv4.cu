@@ -113,15 +113,17 @@ template <typename T> __device__ __forceinline__ void load_four(float (&x)[4], c
     }
   }
 }
-// What the launch before wrote, past L1 (`ld_prev`): a number, or two on a boundary of as many
-__device__ __forceinline__ float prev(const float* p) { return ld_prev(p); }
-__device__ __forceinline__ float prev(const __nv_bfloat16* p) { return ld_prev_bf16(p); }
-template <typename T> __device__ __forceinline__ void prev_two(float (&x)[2], const T* p) {
+// What the launch before wrote: a number, or two on a boundary of as many.  DEPENDENT: past L1 (`ld_prev`)
+template <bool DEPENDENT> __device__ __forceinline__ float prev(const float* p) { return DEPENDENT ? ld_prev(p) : *p; }
+template <bool DEPENDENT> __device__ __forceinline__ float prev(const __nv_bfloat16* p) { return DEPENDENT ? ld_prev_bf16(p) : __bfloat162float(*p); }
+template <bool DEPENDENT, typename T> __device__ __forceinline__ void prev_two(float (&x)[2], const T* p) {
   if constexpr (sizeof(T) == 4) {
-    const float2 v = ld_prev(reinterpret_cast<const float2*>(p));
+    const float2* const at = reinterpret_cast<const float2*>(p);
+    const float2 v = DEPENDENT ? ld_prev(at) : *at;
     x[0] = v.x; x[1] = v.y;
   } else {
-    const unsigned v = ld_prev(reinterpret_cast<const unsigned*>(p));
+    const unsigned* const at = reinterpret_cast<const unsigned*>(p);
+    const unsigned v = DEPENDENT ? ld_prev(at) : *at;
     x[0] = __uint_as_float(v << 16);
     x[1] = __uint_as_float(v & 0xffff0000u);
   }
@@ -208,7 +210,7 @@ template <int GS> __device__ __forceinline__ void store_key(const float (&x)[2][
 }
 
 // A token's value of one head, by a warp: 8 U lanes of four dims.
-template <typename T>
+template <bool DEPENDENT, typename T>
 __device__ __forceinline__ void store_value(const T* row, unsigned char* tile, int t, int d, int group, int page) {
   const int lane = threadIdx.x & 31, units = kv4_units(d);
   unsigned* const scales = reinterpret_cast<unsigned*>(tile + (size_t)kv4_row_bytes(d) * page) + t * (d / group);
@@ -220,7 +222,7 @@ __device__ __forceinline__ void store_value(const T* row, unsigned char* tile, i
       Range range;
       const int at = 32 * u + 16 * p + 2 * r;
       if (at < d) {
-        prev_two<T>(x[p], row + at);
+        prev_two<DEPENDENT>(x[p], row + at);
         range.add(x[p][0]);
         range.add(x[p][1]);
       }
@@ -459,9 +461,9 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_store_kernel(const T* k, const
 }
 
 // The same behind a fused projection (rows q | k | v): per-head norm and rotation of queries and keys first, a warp per (token, head).  Formulas and
-// rounding points are those of rope_kv.cu.  A programmatic dependent, so rows and angles are read past L1.  A decode step's launch is some 3 us of latency (loads, a
-// norm's sum, angles, a range), no rate.
-template <typename T>
+// rounding points are those of rope_kv.cu.  A decode step's launch is some 3 us of latency (loads, a norm's sum, angles,
+// a range), no rate, and overlaps the one before it (DEPENDENT); a prompt's, 2,000 tokens of 32 / 8 heads of 128 in 52 us, does not, and its heads share a token's angles in L1.
+template <typename T, bool DEPENDENT>
 __global__ void __launch_bounds__(WARPS * 32) kv4_rope_store_kernel(const T* qkv, int stride, const float* __restrict__ wq, const float* __restrict__ wk,
                                                                     const float* __restrict__ inv_freq, const T* cs_table, const int* __restrict__ tok_slot,
                                                                     const int* __restrict__ tok_pos, T* q_out, unsigned char* k_pages, unsigned char* v_pages,
@@ -471,7 +473,7 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_rope_store_kernel(const T* qkv
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = blockIdx.y * WARPS + warp, half = rot >> 1;
   const long long n = blockIdx.x;
   if (gridDim.x <= SIGNAL_ROWS) let_next_launch_in();
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (DEPENDENT) asm volatile("griddepcontrol.wait;" ::: "memory");
   if (head >= n_heads + 2 * n_kv) return;
   const int slot = tok_slot[n], pos = tok_pos[n];
   const T* src = qkv + n * stride + (size_t)head * d;
@@ -483,13 +485,13 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_rope_store_kernel(const T* qkv
   }
   Place at = {};
   if (head >= n_heads) at = place_of(k_pages, v_pages, page_table, max_pages, slot, pos, page, n_kv, (head - n_heads) % n_kv, kv4_tile_bytes(page, d, group));
-  if (head >= n_heads + n_kv) return store_value(src, at.v, at.t, d, group, page);
+  if (head >= n_heads + n_kv) return store_value<DEPENDENT>(src, at.v, at.t, d, group, page);
   T* const row = rows[warp];
   const float* w = head < n_heads ? wq : wk;
   float x[8], ss = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    x[i] = lane + 32 * i < d ? prev(src + lane + 32 * i) : 0.f;
+    x[i] = lane + 32 * i < d ? prev<DEPENDENT>(src + lane + 32 * i) : 0.f;
     ss = fmaf(x[i], x[i], ss);
   }
   const float inv = has_norm ? rsqrtf(warp_sum(ss) / (float)d + eps) : 1.f;
@@ -500,8 +502,8 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_rope_store_kernel(const T* qkv
   for (int j = lane; j < half; j += 32) {
     float sn, cs;
     if (cs_table != nullptr) {
-      cs = prev(cs_table + n * rot + j);
-      sn = prev(cs_table + n * rot + half + j);
+      cs = prev<DEPENDENT>(cs_table + n * rot + j);
+      sn = prev<DEPENDENT>(cs_table + n * rot + half + j);
     } else {
       sincosf((float)pos * inv_freq[j], &sn, &cs);
       cs = rnd<T>(cs);
@@ -678,8 +680,10 @@ int rope_store(const void* qkv, int stride, const float* wq, const float* wk, co
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_rope_store_kernel<T>, (const T*)qkv, stride, wq, wk, inv_freq, (const T*)cs_table, tok_slot, tok_pos, (T*)q_out,
+  const bool dependent = pdl && n <= (int)SIGNAL_ROWS;
+  cfg.numAttrs = dependent ? 1 : 0;
+  const auto kern = dependent ? kv4_rope_store_kernel<T, true> : kv4_rope_store_kernel<T, false>;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, (const T*)qkv, stride, wq, wk, inv_freq, (const T*)cs_table, tok_slot, tok_pos, (T*)q_out,
                                            (unsigned char*)k_pages, (unsigned char*)v_pages, page_table, max_pages, n_heads, n_kv, d, rot, group, page, eps, has_norm);
   return e != cudaSuccess ? (int)e : launch_status();
 }

@@ -2812,7 +2812,7 @@ def kv4_store(k, v, tok_slot, tok_pos, k_pages, v_pages, page_table, group: int)
 def kv4_rope_store(qkv, q_norm_w, k_norm_w, inv_freq, tok_slot, tok_pos, q_out, k_pages, v_pages, page_table, n_heads: int, n_kv_heads: int,
                    head_dim: int, rotary_dim: int, eps: float, group: int, cs_table=None, pdl: bool = False) -> None:
     """``qk_norm_rope_store`` with the cache in 4 bits: per-head norm and rotation of the rows' queries and keys, queries to ``q_out``, keys and values into
-    the cache as ``kv4_store`` puts them there.  ``cs_table`` as there.  ``pdl``: a programmatic dependent; ``tok_slot``, ``tok_pos`` and ``page_table`` are
+    the cache as ``kv4_store`` puts them there.  ``cs_table`` as there.  ``pdl``: up to 64 tokens are a programmatic dependent; ``tok_slot``, ``tok_pos`` and ``page_table`` are
     then older than the last launch in front of it that is not such a dependent itself."""
     n = qkv.shape[0]
     width = (n_heads + 2 * n_kv_heads) * head_dim
