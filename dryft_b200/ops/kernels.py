@@ -2639,8 +2639,10 @@ def linear4_fuses(m: int, w) -> bool:
 
 # Rows up to which the models' steps leave the norm and the residual sum to the products: every block norms the rows for itself, which saves two launches a
 # layer and costs more with every row.  36 layers 2,560 wide, ms a step, left / not left to them: 1 row 1.61 / 1.69, 2 rows 1.71 / 1.77, 4 rows 1.82 / 1.88,
-# 8 rows 2.12 / 2.02, 16 rows 2.59 / 2.58.  (SiLU and the multiplication stay with the product at up to 16 rows.)
-LINEAR4_NORM_ROWS = 4
+# 8 rows 2.12 / 2.02, 16 rows 2.59 / 2.58.  A row costs as it is wide: up to so many numbers in all.  16 layers, us a step: 2,048 wide, 4 rows 493 / 513; 2,560 wide, 3 rows
+# 736 / 746; 4,096 wide, 2 rows 888 / 899, 3 rows 957 / 931, 4 rows 959 / 932; 8 layers 5,120 wide, 2 rows 838 / 862.  (SiLU and the multiplication stay with the product
+# at up to 16 rows.)
+LINEAR4_NORM_ROWS, LINEAR4_NORM_NUMBERS = 4, 10240
 
 
 _LINEAR4_MODES = {"store": 0, "residual": 2, "silu": 3}

@@ -67,8 +67,8 @@ def held(w: torch.Tensor, rt: Runtime):
 
 
 def four_bits_fuse(n_rows: int, norm, rt: Runtime, *weights) -> bool:
-    """Whether the norm before a step's products with 4-bit weights, and the sums behind them, are the products' own work."""
-    return (rt.fuse_decode and rt.is_bf16 and n_rows <= K.LINEAR4_NORM_ROWS and fused_rms(norm) is not None
+    """Whether the norm before a step's products with 4-bit weights (the first one's inputs are the normed rows), and the sums behind them, are the products' own work."""
+    return (rt.fuse_decode and rt.is_bf16 and n_rows <= K.LINEAR4_NORM_ROWS and n_rows * weights[0].k <= K.LINEAR4_NORM_NUMBERS and fused_rms(norm) is not None
             and all(K.linear4_fuses(n_rows, w) for w in weights))
 
 
