@@ -46,7 +46,8 @@ def _model_dir(args) -> str:
 def _engine(args):
     from .engine.api import Engine
 
-    kw = dict(dtype=args.dtype, cuda_graphs=not args.no_cuda_graph, weight_bits=args.weight_bits, cache_bits=args.cache_bits)
+    kw = dict(dtype=args.dtype, cuda_graphs=not args.no_cuda_graph, weight_bits=args.weight_bits, cache_bits=args.cache_bits,
+              bits_group=args.bits_group)
     if args.max_batch:
         kw["max_batch"] = args.max_batch
     if args.max_seq_len:
@@ -141,6 +142,7 @@ def main(argv=None) -> int:
         p.add_argument("--no-cuda-graph", action="store_true")
         p.add_argument("--weight-bits", type=int, default=16, choices=[4, 16], help="4: matrices held in 4 bits")
         p.add_argument("--cache-bits", type=int, default=16, choices=[4, 16], help="4: keys and values held in 4 bits")
+        p.add_argument("--bits-group", type=int, default=64, choices=[16, 32, 64, 128], help="numbers that share a scale where something is held in 4 bits")
 
     g = sub.add_parser("generate", help="generate token ids from token ids")
     common(g)

@@ -22,3 +22,21 @@ def test_norms_left_to_products_cost_as_rows_are_wide(monkeypatch, width, most):
     monkeypatch.setattr(L, "fused_rms", lambda norm: norm)
     rt, weights = Runtime(dtype=torch.bfloat16, device=torch.device("cpu")), (_weight(64, width), _weight(width, 9728))
     assert [L.four_bits_fuse(rows, "norm", rt, *weights) for rows in range(1, 8)] == [rows <= most for rows in range(1, 8)]
+
+
+def test_the_command_lines_numbers_that_share_a_scale(monkeypatch):
+    """``--bits-group`` reaches the engine, as its other two options for 4 bits do."""
+    from dryft_b200 import cli
+    from dryft_b200.engine import api
+
+    class Made(Exception):
+        pass
+
+    def made(*a, **kw):
+        raise Made(kw)
+
+    monkeypatch.setattr(api, "Engine", made)
+    for more, group in (([], 64), (["--bits-group", "128"], 128)):
+        with pytest.raises(Made) as e:
+            cli.main(["generate", "--model", "somewhere", "--prompt-ids", "1", "--weight-bits", "4"] + more)
+        assert e.value.args[0]["bits_group"] == group and e.value.args[0]["weight_bits"] == 4
