@@ -56,7 +56,7 @@ template <typename X> __device__ __forceinline__ float defined_product(const uin
   scales += tile * (wide >> group_bits) * 8 + r;
   float sum = 0.f;
 #pragma unroll 1
-  for (int at = 0; at < k; at += 16) {   // a step: word s of the four lanes of a row of its block
+  for (int at = 0; at < k && sum == sum; at += 16) {   // a step: word s of the four lanes of a row of its block (what is NaN stays NaN)
     const uint2 sz = scales[(at >> group_bits) * 8];
     const GroupCode g = unpack_code(h ? sz.y : sz.x);
 #pragma unroll

@@ -88,3 +88,12 @@ def test_many_rows(n, dtype, out):
     w, x = _inputs(300, n, 320, dtype)
     y = linear(x.to(DEV), K().pack_weight4(w.to(DEV), 64), Runtime(dtype=dtype, device=torch.device(DEV)), out_dtype=out)
     _check(y, x, P.group_values(w, 64)[0])
+
+
+@pytest.mark.parametrize("m,n", [(16, 5000), (256, 20000)])
+def test_every_result_not_finite(m, n):
+    """All of a launch's results are worked out again: slowly, and no bounded wait runs out over it."""
+    w4 = K().pack_weight4(torch.rand(n, 2560, device=DEV).to(BF) + 0.5)
+    y = K().linear4(torch.full((m, 2560), INF, dtype=BF, device=DEV), w4, out_dtype=F32)
+    K().check_error_flags()
+    assert (y == INF).all()
