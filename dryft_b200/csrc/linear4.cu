@@ -444,7 +444,7 @@ template <int NT, int GS, int TEAM, int PB, int SLOTS, bool ALONE> int few(const
   return launch(linear4_few_kernel<NT, GS, TEAM, PB, SLOTS, ALONE>, asked, turns < 148 ? turns : 148, FEW_WARPS * 32, Few<NT, GS, TEAM, PB, SLOTS>::bytes(a.m, a.k), a.pdl, a.st,
                 (const bf16*)a.x, a.x_stride, (const uint4*)a.codes, (const uint2*)a.scales, a.y, a.m, a.n, a.k, __builtin_ctz(a.group), a.mode, a.norm_w, a.eps);
 }
-// Four warps a tile where shared memory has room for their rings beside x (eight rows: up to about 6,000 inputs), else all sixteen with shorter rings, which only
+// Four warps a tile where shared memory has room for their rings beside x (eight rows: up to about 7,000 inputs), else all sixteen with shorter rings, which only
 // 32-bit results use.  2,560 inputs, one row, four / eight / sixteen warps a tile: 151,936 outputs 55.6 / 63.6 / 81.9 us, 6,144 outputs 4.8 / 5.4 / 5.7 us (a tile's
 // end costs each warp as much as half a slot).  Where only the sixteen fit, the tensor memory kernel is as fast or faster (16 rows of 4,096 inputs, 24,576 outputs:
 // 21.3 us and 29.1; 8 rows of 9,728 inputs, 2,560 outputs: 11.4 and 12.1), but not where it has two products to make for 32 bits.
