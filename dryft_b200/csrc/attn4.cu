@@ -6,6 +6,8 @@
 // a thread-block cluster and meet in its shared memory; more leave (acc, m, l) in memory and a second launch joins them.  Either way in the splits' order.
 #include "four_bit.cuh"
 
+#include <cuda_fp16.h>
+
 #if !defined(DRYFT_HEAD_DIM) || !defined(DRYFT_GROUP) || !defined(DRYFT_PAGE) || !defined(DRYFT_BITS_GROUP)
 #error "compile with -DDRYFT_HEAD_DIM=.. -DDRYFT_GROUP=.. -DDRYFT_PAGE=.. -DDRYFT_BITS_GROUP=.."
 #endif
@@ -35,14 +37,18 @@ __device__ __forceinline__ Work work_of_block() {   // grid (splits, key heads x
 }
 
 // ---------------------------------------------------------------------------------------------- bfloat16: tensor cores
-// S^T = K Q^T and O^T = V^T P^T on mma.sync.m16n8k16, the codes as bfloat16 16 + c straight out of the cache's words (`code_pair`):
+// S^T = K Q^T and O^T = V^T P^T on mma.sync.m16n8k16, the codes straight out of the cache's words: keys' as bfloat16 16 + c (`code_pair`), values' as float16 c - 8:
 //   score  = s_k (sum (16 + c) q - 23.5 sum q) + z_k sum q          group by group, in 32 bits; sum q is the query's own
-//   output = sum p' (16 + c) + sum p z_v - 23.5 sum p'              p' = bf16(p s_v): the weight rounded with its scale, one rounding of up to 2^-8 as for plain P
-// Scores, running maximum and sums are 32-bit.  A warp walks tiles of 16 keys of its own, copied STAGES - 1 tiles ahead into its own ring.  The maximum
+//   output = sum p' (c - 8) / unit + sum p (z_v + s_v / 2)          p' = fp16(p s_v unit): the weight rounded with its scale, by up to 2^-11
+// `unit` is a power of two that keeps p' between float16's ends: set when a tile's scales are larger than all before it (the first tile's are), so a weight whose scale is
+// less than 2^-20 of the largest loses bits, and nothing that shows.  Scores, running maximum and sums are 32-bit.  (Weights in bfloat16 and values as 16 + c, corrected by
+// -23.5 sum p': off by 0.0023 of the whole, not 0.0017, which the result's own rounding is; and the tensor cores cut sums off, not round them, which took another
+// 0.0013 of sums three times as large over 128 tiles.)
+// A warp walks tiles of 16 keys of its own, copied STAGES - 1 tiles ahead into its own ring.  The maximum
 // of a column follows the scores only when one exceeds it by more than 2^8: what is summed stays below 2^8 times the number of keys.
-// What bounds it: issue.  A tile is some 400 instructions of its warp, 224 of them on the pipe for logic, which takes one every other cycle (taking 128 codes a lane
-// apart is half of those): with four warps on a scheduler that pipe is 69% busy and a tile takes 0.40 us of the scheduler, with two 0.34 us.  64 rows of up to 8,192
-// keys, 32 / 8 heads of 128: 98 us, 3,190 GB/s; one row of 16,383 keys, 64 / 8 heads: 18 us (16 us by way of memory, and a second launch on the host); eight rows of
+// What bounds it: issue.  A tile is some 410 instructions of its warp, 212 of them on the pipe for logic, which takes one every other cycle (taking 128 codes a lane
+// apart is half of those): with four warps on a scheduler that pipe is 67% busy and a tile takes 0.39 us of the scheduler.  64 rows of up to 8,192
+// keys, 32 / 8 heads of 128: 96 us, 3,250 GB/s; one row of 16,383 keys, 64 / 8 heads: 17 us (16 us by way of memory, and a second launch on the host); eight rows of
 // 650 keys 8 us; one, 7.  Sixteen warps a block: 10.1 us for the eight rows; two tiles unrolled: as before.
 typedef __nv_bfloat16 bf16;
 constexpr int STEPS = D / 16, UNIT = PAGE % 32 ? 1 : 2, STAGES = D <= 128 ? 4 / UNIT : 2, MOST_SPLITS = 16;   // UNIT: tiles that are copied together
@@ -59,6 +65,31 @@ __device__ __forceinline__ unsigned transposed(unsigned v) {   // an 8 x 8 fragm
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
+// The codes of a word of values, less 8, as four pairs of float16: two of the four places of a half word lie in the mantissa as they are, above 1024 (c in its lowest
+// bits) and above 64 (c in bits 4..7), the other two a byte further up.  (A difference of float16 numbers that is exact.)
+__device__ __forceinline__ unsigned half_sub(unsigned x, unsigned y) {
+  unsigned r;
+  asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+  return r;
+}
+__device__ __forceinline__ void codes_less_8(unsigned (&v)[4], unsigned w) {
+  constexpr unsigned BY_1 = 0x64006400u, BY_16 = 0x54005400u, LESS_1 = 0x64086408u, LESS_16 = 0x54805480u;   // 1024 and 64, 1032 and 72
+  const unsigned u = w >> 8;
+  v[0] = half_sub((w & 0x000f000fu) | BY_1, LESS_1);
+  v[1] = half_sub((w & 0x00f000f0u) | BY_16, LESS_16);
+  v[2] = half_sub((u & 0x000f000fu) | BY_1, LESS_1);
+  v[3] = half_sub((u & 0x00f000f0u) | BY_16, LESS_16);
+}
+__device__ __forceinline__ void mma_16816_half(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned half_two(float x, float y) {
+  const __half2 v = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const unsigned*>(&v);
+}
+__device__ __forceinline__ float reciprocal(float power_of_two) { return __uint_as_float(0x7f000000u - __float_as_uint(power_of_two)); }   // 2^-126 to 2^126
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -104,8 +135,14 @@ constexpr float LOWEST = -3.402823466e38f;
 
 // What a warp keeps of its eight columns (query heads); a lane has the columns 2c and 2c + 1, and in `acc` the dims 16 j + 2r and + 1 of both.
 struct Columns {
-  float acc[STEPS][4], off[GROUPS][2], less[GROUPS][4], top[2], sum[2];   // less: -23.5 sum p', from products with a constant
+  float acc[STEPS][4], off[GROUPS][2], top[2], sum[2];
+  float unit;   // what `acc` is in, beside the scales: the warp's, 2^120 at most
 };
+constexpr float UNIT_MOST = 1.329227995784916e36f;   // 2^120
+// A lane's scales times the unit come to 255 at most (2^8 times that is a float16); where they come to more, the unit is set so that the largest becomes 2^WIDE to twice that:
+// all 2 GROUPS of a lane come to 128 at most then, and follow up to twice that size without another look.
+constexpr float SCALES_MOST = 255.f;
+constexpr unsigned WIDE = GROUPS <= 1 ? 5 : GROUPS <= 2 ? 4 : GROUPS <= 4 ? 3 : GROUPS <= 8 ? 2 : 1;
 
 // A tile of 16 keys.  EDGE: keys may be out of the row's sight; such a key may hold anything, so its scales are taken for zeros.
 template <bool EDGE>
@@ -140,10 +177,34 @@ __device__ __forceinline__ void tile_of_keys(Columns& o, const unsigned char* k,
     for (int i = 0; i < 4; ++i) s[i] = (i < 2 ? seen0 : seen1) ? s[i] * scale2 : -INFINITY;
     scale2 = 1.f;
   }
+  // the values' (s, z), in registers or, where they are many, read where they are used
+  constexpr bool HELD = GROUPS <= 4;
+  unsigned lo_s[HELD ? GROUPS : 1], hi_s[HELD ? GROUPS : 1];
+  if constexpr (HELD) {
+    load_words(lo_s, v_scales + r * GROUPS * 4);
+    load_words(hi_s, v_scales + (r + 8) * GROUPS * 4);
+  }
+  const auto value_scale = [&](int g, int half) {
+    if constexpr (HELD)
+      return unpack_code((half ? seen1 : seen0) ? (half ? hi_s[g] : lo_s[g]) : 0u);
+    else
+      return unpack_code((half ? seen1 : seen0) ? reinterpret_cast<const unsigned*>(v_scales)[(r + 8 * half) * GROUPS + g] : 0u);
+  };
+  float all = 0.f;   // of the lane's scales, in units
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) all = fmaf(value_scale(g, 0).s, o.unit, fmaf(value_scale(g, 1).s, o.unit, all));
   float d[4];   // powers of two above the maximum
 #pragma unroll
   for (int i = 0; i < 4; ++i) d[i] = fmaf(s[i], scale2, -o.top[i & 1]);
-  if (__any_sync(0xffffffffu, fmaxf(fmaxf(d[0], d[1]), fmaxf(d[2], d[3])) > 8.f)) {
+  if (__any_sync(0xffffffffu, (fmaxf(fmaxf(d[0], d[1]), fmaxf(d[2], d[3])) > 8.f) | !(all <= SCALES_MOST))) {
+    float most = 0.f;   // of the tile's scales (NaN is passed over)
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) most = fmaxf(most, fmaxf(value_scale(g, 0).s, value_scale(g, 1).s));
+#pragma unroll
+    for (int x = 4; x < 32; x <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
+    const float per_unit = reciprocal(o.unit);
+    if (most * o.unit >= (float)(2 << WIDE)) o.unit = __uint_as_float((254u + WIDE - (__float_as_uint(most) >> 23)) << 23);
+    const float less = o.unit * per_unit;   // the new unit in old ones, exact
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       float m = fmaxf(o.top[i], fmaxf(s[i] * scale2, s[i + 2] * scale2));
@@ -153,14 +214,11 @@ __device__ __forceinline__ void tile_of_keys(Columns& o, const unsigned char* k,
       o.top[i] = m;
       o.sum[i] *= lower;
 #pragma unroll
-      for (int g = 0; g < GROUPS; ++g) {
-        o.off[g][i] *= lower;
-        o.less[g][i] *= lower;   // (its lower rows are not read)
-      }
+      for (int g = 0; g < GROUPS; ++g) o.off[g][i] *= lower;
 #pragma unroll
       for (int j = 0; j < STEPS; ++j) {
-        o.acc[j][i] *= lower;
-        o.acc[j][i + 2] *= lower;
+        o.acc[j][i] *= lower * less;
+        o.acc[j][i + 2] *= lower * less;
       }
       d[i] = fmaf(s[i], scale2, -m);
       d[i + 2] = fmaf(s[i + 2], scale2, -m);
@@ -172,24 +230,25 @@ __device__ __forceinline__ void tile_of_keys(Columns& o, const unsigned char* k,
     p[i] = exp2_fast(d[i]);
     o.sum[i & 1] += p[i];
   }
-  unsigned vw[2 * UNITS], lo_s[GROUPS], hi_s[GROUPS];
+  unsigned vw[2 * UNITS];
   load_words<2 * UNITS>(vw, v + lane * UNITS * 8);
-  load_words<GROUPS>(lo_s, v_scales + r * GROUPS * 4);
-  load_words<GROUPS>(hi_s, v_scales + (r + 8) * GROUPS * 4);
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g) {
-    const GroupCode a = unpack_code(seen0 ? lo_s[g] : 0u), b = unpack_code(seen1 ? hi_s[g] : 0u);
-    const __nv_bfloat162 w0 = __floats2bfloat162_rn(p[0] * a.s, p[1] * a.s), w1 = __floats2bfloat162_rn(p[2] * b.s, p[3] * b.s);
-    const unsigned b0 = transposed(*reinterpret_cast<const unsigned*>(&w0)), b1 = transposed(*reinterpret_cast<const unsigned*>(&w1));
-    o.off[g][0] = fmaf(p[0], a.z, fmaf(p[2], b.z, o.off[g][0]));
-    o.off[g][1] = fmaf(p[1], a.z, fmaf(p[3], b.z, o.off[g][1]));
-    constexpr unsigned LESS = 0xc1bcc1bcu;   // two bfloat16 -23.5
-    mma_16816(o.less[g], LESS, LESS, LESS, LESS, b0, b1);
+    const GroupCode a = value_scale(g, 0), b = value_scale(g, 1);
+    const float as = a.s * o.unit, bs = b.s * o.unit;
+    unsigned x[4], y[4];
+    const unsigned b0 = transposed(half_two(p[0] * as, p[1] * as)), b1 = transposed(half_two(p[2] * bs, p[3] * bs));
+    const float az = fmaf(0.5f, a.s, a.z), bz = fmaf(0.5f, b.s, b.z);   // what code 8 stands for
+    o.off[g][0] = fmaf(p[0], az, fmaf(p[2], bz, o.off[g][0]));
+    o.off[g][1] = fmaf(p[1], az, fmaf(p[3], bz, o.off[g][1]));
 #pragma unroll
     for (int j = g * BG / 16; j < (g + 1) * BG / 16; ++j) {
-      const unsigned x = vw[j / 2 * 2], y = vw[j / 2 * 2 + 1];
       const int h = 2 * (j & 1);
-      mma_16816(o.acc[j], code_pair(x, h), code_pair(x, h + 1), code_pair(y, h), code_pair(y, h + 1), b0, b1);
+      if (h == 0 || j == g * BG / 16) {
+        codes_less_8(x, vw[j / 2 * 2]);
+        codes_less_8(y, vw[j / 2 * 2 + 1]);
+      }
+      mma_16816_half(o.acc[j], x[h], x[h + 1], y[h], y[h + 1], b0, b1);
     }
   }
 }
@@ -219,12 +278,13 @@ __global__ void __launch_bounds__(WARPS * 32, Block<WARPS>::AT_ONCE) attn4_mma_k
   const int a = u0 + units * warp / WARPS, b = u0 + units * (warp + 1) / WARPS;
 
   Columns o;
+  o.unit = UNIT_MOST;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     o.top[i] = LOWEST;
     o.sum[i] = 0.f;
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) o.off[g][i] = o.less[g][i] = o.less[g][i + 2] = 0.f;
+    for (int g = 0; g < GROUPS; ++g) o.off[g][i] = 0.f;
 #pragma unroll
     for (int j = 0; j < STEPS; ++j) o.acc[j][i] = o.acc[j][i + 2] = 0.f;
   }
@@ -348,12 +408,13 @@ __global__ void __launch_bounds__(WARPS * 32, Block<WARPS>::AT_ONCE) attn4_mma_k
 #pragma unroll
   for (int i = 0; i < 2; ++i) by[i] = exp2_fast(o.top[i] - top[i]);   // (1 where nothing has been seen: zeros, or the NaN of scores that are NaN)
   if (r == 0) *reinterpret_cast<float2*>(sums + warp * 8 + 2 * c) = make_float2(o.sum[0] * by[0], o.sum[1] * by[1]);
+  const float per_unit = reciprocal(o.unit);
 #pragma unroll
   for (int j = 0; j < STEPS; ++j) {
     const int g = 16 * j / BG;
-    const float e0 = o.off[g][0] + o.less[g][0], e1 = o.off[g][1] + o.less[g][1];
-    parts[(warp * STEPS + j) * 32 + lane] =
-        make_float4((o.acc[j][0] + e0) * by[0], (o.acc[j][1] + e1) * by[1], (o.acc[j][2] + e0) * by[0], (o.acc[j][3] + e1) * by[1]);
+    const float e0 = o.off[g][0], e1 = o.off[g][1];
+    parts[(warp * STEPS + j) * 32 + lane] = make_float4(fmaf(o.acc[j][0], per_unit, e0) * by[0], fmaf(o.acc[j][1], per_unit, e1) * by[1],
+                                                        fmaf(o.acc[j][2], per_unit, e0) * by[0], fmaf(o.acc[j][3], per_unit, e1) * by[1]);
   }
   __syncthreads();
   float l[2] = {0.f, 0.f};
