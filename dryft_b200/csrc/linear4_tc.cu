@@ -5,7 +5,8 @@
 // of W a warp at a time, and stores them into tensor memory, where tcgen05.mma takes its first operand from: a lane's codes are rows r and r + 8 and the inputs of two
 // neighbouring columns, which is the shape 16x256b as it stands.  x comes by TMA, K-major in a 128-byte swizzle.  So the weights cross memory at 4.5 bits
 // and are multiplied as bfloat16 z + (c - 7.5) s: one rounding, by up to 2^-8, of each weight (2^-9.2 in the mean square).  For 32-bit results (LOW)
-// the rest of that rounding is a second operand with a product of its own, which leaves 2^-16 (2^-18).
+// the rest of that rounding is a second operand with a product of its own, which leaves 2^-16 (2^-18), and inputs are summed 512 at a time (`SEGMENT`): in one piece
+// 30,000 outputs of 12,288 inputs were off by 22 millionths of the whole, now by 0.9; 32-bit multiply-adds in order are by 1.9.  That takes 128 rows at most; more are two passes.
 //
 // Work is cut evenly: block i of G takes the units [i U / G, (i + 1) U / G) in (tile, inputs) order.  A run that covers its tile's inputs is finished from tensor
 // memory; else its sums go to a workspace, and a second launch adds a tile's pieces in the blocks' order.  No block waits for another.
@@ -120,19 +121,23 @@ __device__ __noinline__ float defined_result(const Inputs in, int row, int m) { 
 template <int NB> constexpr int units_of() { return NB == 256 ? 1 : 2; }
 template <int NB, int GN, bool LOW> struct Layout {
   static constexpr int KU = units_of<NB>(), X_BLOCK = NB * BK * 2, STAGE_BYTES = X_BLOCK * KU;   // a stage of x, block by block; multiples of 1024
-  static constexpr int RING = 8;                                                                 // units whose codes are on their way
+  static constexpr int SUMS_BYTES = LOW ? NB * BM * 4 : 0;                                       // of segments (below)
+  static constexpr int RING = !LOW || NB < 128 ? 8 : NB < 256 ? 6 : 4;                           // units whose codes are on their way
   static constexpr int CODE_BYTES = 4096 * KU, SCALE_BYTES = 512 * GN, SLOT_BYTES = CODE_BYTES + SCALE_BYTES, RING_BYTES = RING * SLOT_BYTES;   // multiples of 128
   // tensor memory: sums of ACCS runs, then the stages of weights (LOW: and of their rests), two inputs a column
   static constexpr int ACCS = NB == 256 ? 1 : 2, W_COLS = BK / 2 * KU, STAGE_COLS = W_COLS * (LOW ? 2 : 1), W_COL0 = ACCS * NB, TMEM_COLS = 512;
-  static constexpr int ROOM = (225 * 1024 - RING_BYTES) / STAGE_BYTES, COLS = (TMEM_COLS - W_COL0) / STAGE_COLS, FIT = ROOM < COLS ? ROOM : COLS;
+  static constexpr int ROOM = (225 * 1024 - RING_BYTES - SUMS_BYTES) / STAGE_BYTES, COLS = (TMEM_COLS - W_COL0) / STAGE_COLS, FIT = ROOM < COLS ? ROOM : COLS;
   static constexpr int STAGES = FIT < 6 ? FIT : 6;
   // Teams of warps that take units' weights out in turn.  A parity tells two phases of a barrier apart, not three: a team that waits for the products of the unit that
   // had its stage before has to know that those of the unit before that are done.  It has written its last unit, TEAMS before this one, into a stage that the products
   // of the unit TEAMS + STAGES before this one had left; so TEAMS is at most STAGES.
   static constexpr int TEAMS = STAGES >= 4 ? 4 : 2, TEAM = TAKERS / TEAMS;
+  // Units that are summed in tensor memory at a time.  Every product there cuts what it adds to off, not rounds it: 2^-26 of the sum each in the mean, always towards zero.
+  // For 32-bit results 512 inputs, 64 products, are summed so; their sums are added up in shared memory by the threads that read them, rounded.
+  static constexpr int SEGMENT = LOW ? 512 / (BK * KU) : 1 << 30;
   static_assert(STAGES >= 2 && TEAMS <= STAGES && TEAMS <= RING, "phases of a stage's barrier");
   static_assert(W_COL0 + STAGES * STAGE_COLS <= TMEM_COLS, "of tensor memory");
-  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + RING_BYTES + 8 * (2 * STAGES + 2 * RING + 4) + 64;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + RING_BYTES + SUMS_BYTES + 8 * (2 * STAGES + 2 * RING + 4) + 64;
   static_assert(SMEM_BYTES <= 227 * 1024, "of a block");
 };
 // (32 bits: the launcher sees to U G being below 2^32)
@@ -185,7 +190,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
   extern __shared__ unsigned char smem_raw[];
   unsigned char* const stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* const ring = stages + STAGES * L::STAGE_BYTES;
-  unsigned long long* const full = reinterpret_cast<unsigned long long*>(ring + L::RING_BYTES);                  // [S] weights (a team), x (TMA) -> products
+  unsigned long long* const full = reinterpret_cast<unsigned long long*>(ring + L::RING_BYTES + L::SUMS_BYTES);  // [S] weights (a team), x (TMA) -> products
   unsigned long long* const empty = full + STAGES;                                                                // [S] products -> both
   unsigned long long* const acc_full = empty + STAGES;                                                            // [2] a run's sums -> their readers
   unsigned long long* const acc_empty = acc_full + 2;                                                             // [2] read (128 arrivals) -> products
@@ -255,6 +260,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
     const bool issues = elected();
     int run = 0, s = 0, kb = u0 % KB;   // runs of one tile's units that this block has begun
     unsigned par = 0, first = 1;
+    int left = LOW ? L::SEGMENT - kb % L::SEGMENT : 0;   // units of the segment
     bool there = false;   // the next unit is, as of the last one's products: asked before they are issued, which hides the answer's way
     for (int i = 0; i < n_units; ++i) {
       bool ok = there || mbar_wait(&full[s], par, p.err, failed, 2);
@@ -264,7 +270,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const unsigned long long x_desc = x_desc0 + (unsigned)(s * (L::STAGE_BYTES >> 4));
       const unsigned d = tmem + (unsigned)(run % L::ACCS * NB), w = tmem + L::W_COL0 + (unsigned)(s * L::STAGE_COLS);
-      const bool last = kb + 1 == KB || i == n_units - 1;
+      const bool tile_ends = kb + 1 == KB, last = tile_ends || i == n_units - 1 || (LOW && left == 1);
       const int ahead = s + 1 == STAGES ? 0 : s + 1;
       there = mbar_test(&full[ahead], ahead == 0 ? par ^ 1 : par);   // (behind the last unit: of a phase that nobody waits for)
       if (issues) {
@@ -283,7 +289,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
       __syncwarp();
       first = last;
       run += last;
-      kb = last ? 0 : kb + 1;
+      kb = tile_ends ? 0 : kb + 1;
+      if (LOW) left = last ? L::SEGMENT : left - 1;
       s = ahead;
       par ^= ahead == 0;
     }
@@ -291,9 +298,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
     const int q = warp & 3, row = q * 32 + lane;   // the quarter of tensor memory that this warp may read; W row of the tile
     asm volatile("griddepcontrol.wait;" ::: "memory");
     int run = 0;
+    float* const sums = reinterpret_cast<float*>(ring + L::RING_BYTES) + row;   // (LOW) [NB][128]: of a tile's segments so far; the thread's own row
     for (int u = u0; u < u1; ++run) {
-      const int tile = u / KB, b = run % L::ACCS, begin = tile * KB, end = min(u1, begin + KB);
-      const bool whole = u == begin && end == begin + KB;
+      const int tile = u / KB, b = run % L::ACCS, begin = tile * KB, part_end = min(u1, begin + KB);
+      const int end = LOW ? min(part_end, u + L::SEGMENT - (u - begin) % L::SEGMENT) : part_end;
+      const bool whole = u0 <= begin && part_end == begin + KB, more = LOW && u > begin && u > u0;   // more: not the first segment
       u = end;
       bool ok = mbar_wait(&acc_full[b], (unsigned)(run / L::ACCS & 1), p.err, failed, 5);
       ok = __all_sync(0xffffffffu, ok);
@@ -308,7 +317,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
       for (int m0 = 0; m0 < NB; m0 += 16) {
         float v[16];
         tmem_ld16(from + m0, v);
-        if (whole) {
+        if (LOW && more) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] += sums[(m0 + j) * BM];
+        }
+        if (LOW && end != part_end) {   // more of this tile's inputs follow
+#pragma unroll
+          for (int j = 0; j < 16; ++j) sums[(m0 + j) * BM] = v[j];
+        } else if (whole) {
 #pragma unroll
           for (int j = 0; j < 16; ++j)
             if (m0 + j < p.m && out < p.n) {
@@ -327,7 +343,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_tc_kernel(const __grid_
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       mbar_arrive(&acc_empty[b]);
-      if (LOW && !(none[0] + none[1] == 0.f) && out < p.n)   // products go on meanwhile
+      if (LOW && whole && end == part_end && !(none[0] + none[1] == 0.f) && out < p.n)   // products go on meanwhile
 #pragma unroll 1
         for (int m = 0; m < p.m; ++m) {
           float* const at = reinterpret_cast<float*>(p.y) + (size_t)m * p.n + out;
@@ -535,31 +551,41 @@ template <int NB, bool LOW> int by_group(const Operands& o, const Params& p, int
 }
 }  // namespace
 
-// Floats of the workspace that a launch needs.
+// Rows of a pass: with sums of segments in shared memory beside them no more than 128 fit.
+static int rows_of_pass(int out_f32, int m) { return out_f32 && m > 128 ? 128 : m; }
+
+// Floats of the workspace that a product needs.
 DRYFT_API long long dryft_linear4_tc_pieces(int m, int n, int k) { return 2ll * grid_of(n, blocks_of(k)) * BM * padded_rows(m); }
-// Launches that it makes: one where every block has a whole tile, else a second one for the pieces.
-DRYFT_API int dryft_linear4_tc_launches(int m, int n, int k) {
-  const int units = blocks_of(k) / (padded_rows(m) == 256 ? units_of<256>() : units_of<128>());
-  return grid_of(n, units) == (n + BM - 1) / BM ? 1 : 2;
+// Launches that it makes: for each pass one where every block has a whole tile, else a second one for the pieces.
+DRYFT_API int dryft_linear4_tc_launches(int out_f32, int m, int n, int k) {
+  const int rows = rows_of_pass(out_f32, m), units = blocks_of(k) / (padded_rows(rows) == 256 ? units_of<256>() : units_of<128>());
+  return (grid_of(n, units) == (n + BM - 1) / BM ? 1 : 2) * ((m + rows - 1) / rows);
 }
 
 // y [m, n] = x [m, k] w^T, m <= 256; x bfloat16, rows x_stride numbers apart on 16-byte boundaries; y bfloat16 or (out_f32) float32.
-// pdl: 1, the product is a programmatic dependent of the launch before it; 2, the pieces' launch is one of the product; both or neither.
+// pdl: 1, the product is a programmatic dependent of the launch before it; 2, its further launches are, each of the one before; both or neither.
 DRYFT_API int dryft_linear4_tc(int out_f32, const void* x, long long x_stride, const void* codes, const void* scales, void* y, float* pieces, int m, int n, int k,
                                int group, int pdl, int* err, void* stream) {
   if (m <= 0 || n <= 0) return 0;
   if (m > 256 || k <= 0 || k % 16) return DRYFT_ERR_UNSUPPORTED;
-  const Operands o = {encode_fn(), x, codes, scales, x_stride, k, group};
-  if (!o.enc) return DRYFT_ERR_UNSUPPORTED;
-  const Params p = {y, pieces, err, m, n, blocks_of(k), __builtin_ctz(group), (n + BM - 1) / BM,
-                    {(const bf16*)x, x_stride, (const uint4*)codes, (const uint2*)scales, k, __builtin_ctz(group)}};
+  const EncodeTiledFn enc = encode_fn();
+  if (!enc) return DRYFT_ERR_UNSUPPORTED;
   const cudaStream_t st = (cudaStream_t)stream;
-#define DRYFT_TC(NB) (out_f32 ? by_group<NB, true>(o, p, pdl, st) : by_group<NB, false>(o, p, pdl, st))
-  switch (padded_rows(m)) {
-    case 32: return DRYFT_TC(32);
-    case 64: return DRYFT_TC(64);
-    case 128: return DRYFT_TC(128);
-    default: return DRYFT_TC(256);
+  const int pass = rows_of_pass(out_f32, m);
+  for (int m0 = 0; m0 < m; m0 += pass) {
+    const bf16* const rows = (const bf16*)x + m0 * x_stride;
+    const int count = pass < m - m0 ? pass : m - m0, overlap = m0 == 0 ? pdl : pdl & 2 ? 3 : 0;
+    const Operands o = {enc, rows, codes, scales, x_stride, k, group};
+    const Params p = {(char*)y + (size_t)m0 * n * (out_f32 ? 4 : 2), pieces, err, count, n, blocks_of(k), __builtin_ctz(group), (n + BM - 1) / BM,
+                      {rows, x_stride, (const uint4*)codes, (const uint2*)scales, k, __builtin_ctz(group)}};
+    int rc = DRYFT_ERR_UNSUPPORTED;
+    switch (padded_rows(count)) {
+      case 32: rc = out_f32 ? by_group<32, true>(o, p, overlap, st) : by_group<32, false>(o, p, overlap, st); break;
+      case 64: rc = out_f32 ? by_group<64, true>(o, p, overlap, st) : by_group<64, false>(o, p, overlap, st); break;
+      case 128: rc = out_f32 ? by_group<128, true>(o, p, overlap, st) : by_group<128, false>(o, p, overlap, st); break;
+      case 256: rc = by_group<256, false>(o, p, overlap, st); break;   // (not for 32-bit results)
+    }
+    if (rc) return rc;
   }
-#undef DRYFT_TC
+  return 0;
 }

@@ -2604,7 +2604,7 @@ def _words(t, name: str, numbers: int) -> None:
 
 def linear4_tc_lib() -> ctypes.CDLL:
     """Products of up to 256 rows with weights held in 4 bits (tcgen05, tensor memory, TMA)."""
-    lib = _single_lib("linear4_tc", {"dryft_linear4_tc": [_i, _p, _ll, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p], "dryft_linear4_tc_launches": [_i, _i, _i]})
+    lib = _single_lib("linear4_tc", {"dryft_linear4_tc": [_i, _p, _ll, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p], "dryft_linear4_tc_launches": [_i, _i, _i, _i]})
     lib.dryft_linear4_tc_pieces.argtypes = [_i, _i, _i]
     lib.dryft_linear4_tc_pieces.restype = _ll
     return lib
@@ -2627,9 +2627,10 @@ def linear4_plan(m: int, n: int, k: int, group: int, bf16: bool, f32_out: bool =
 
 
 @functools.lru_cache(maxsize=4096)
-def _linear4_launches(m: int, n: int, k: int) -> int:
-    """Launches of a product on the tensor memory kernel: a second one joins the pieces of tiles that several blocks share."""
-    return linear4_tc_lib().dryft_linear4_tc_launches(m, n, k)
+def _linear4_launches(f32_out: bool, m: int, n: int, k: int) -> int:
+    """Launches of a product on the tensor memory kernel: a second one joins the pieces of tiles that several blocks share; 32-bit results of more than 128 rows
+    are two passes."""
+    return linear4_tc_lib().dryft_linear4_tc_launches(f32_out, m, n, k)
 
 
 def linear4_fuses(m: int, w) -> bool:
@@ -2649,7 +2650,7 @@ _LINEAR4_MODES = {"store": 0, "residual": 2, "silu": 3}
 
 
 def _overlap(pdl: Optional[bool]) -> int:
-    """Which launches are programmatic dependents: 1, an operator's first one; 2, its second one, of the first."""
+    """Which launches are programmatic dependents: 1, an operator's first one; 2, its further ones, each of the one before."""
     return 3 if pdl else 2 if pdl is None else 0
 
 
@@ -2657,7 +2658,8 @@ def linear4(x, w: Weight4, out=None, pdl: Optional[bool] = None, mode: str = "st
     """``out = x @ w.T``; ``x`` bfloat16, up to 256 rows (float32: 64), ``out`` of the same type or float32 (none: a new tensor, of ``out_dtype`` or ``x``'s
     type).  Returns ``out``.  ``pdl``: a programmatic dependent: its
     first weights are requested while the launch before it drains, so codes and scales are older than the last launch in front of it that is not such a
-    dependent itself (``pack_weight4`` sees to that for those it makes); ``False``: no launch overlaps another; ``None``: only a second launch of this product its first.  Where ``x`` is infinite or not a number the result is what the definition's sum
+    dependent itself (``pack_weight4`` sees to that for those it makes); ``False``: no launch overlaps another; ``None``: only this product's further launches, each the one
+    before.  Where ``x`` is infinite or not a number the result is what the definition's sum
     comes to (a result that is not finite is worked out again, input by input).
 
     With few rows of bfloat16 (``linear4_fuses``) also what stands around a decoder's products: ``norm_w`` (float32 ``[k]``): RMS norm of ``x`` first;
@@ -2696,7 +2698,7 @@ def linear4(x, w: Weight4, out=None, pdl: Optional[bool] = None, mode: str = "st
         pieces = torch.empty(floats, dtype=torch.float32, device=x.device)
         rc = _linear4_tc_fn(not out_bf16, x.data_ptr(), step, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), pieces.data_ptr(), m, w.n, w.k, w.group,
                             _overlap(pdl), error_flag(x.device).data_ptr(), _stream())
-        launches = _linear4_launches(m, w.n, w.k)
+        launches = _linear4_launches(not out_bf16, m, w.n, w.k)
     else:
         if _linear4_fn is None:
             _linear4_fn = linear4_lib().dryft_linear4

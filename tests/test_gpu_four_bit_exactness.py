@@ -1,4 +1,4 @@
-"""How exact attention over the 4-bit cache is as a whole, in bfloat16: its outputs' own rounding may be its only error that counts."""
+"""How exact the work from 4 bits is as a whole: bfloat16 attention, where the outputs' own rounding may be the only error that counts, and 32-bit results of products."""
 
 import pytest
 import torch
@@ -66,3 +66,23 @@ def test_values_of_zero_and_of_one_number(d, group):
     for b in (1, 2):
         want = P.attention(q[b].double(), P.group_values(c.keys[b], group)[0], P.group_values(c.values[b], group)[0], 199, P.scale_of(d))[0].flatten()
         assert ((out[b].double().cpu() - want).abs() <= 2.0**-8 * want.abs() + 2.0**-11 * want.abs().max() + 1e-5).all()
+
+
+@pytest.mark.parametrize("n,k,group", [(6886, 11184, 16), (20000, 5120, 64), (2560, 2560, 128), (19000, 528, 16), (389, 4096, 32), (129, 80, 16)])
+@pytest.mark.parametrize("m", [4, 17, 48, 128, 256, 300])
+def test_32_bit_results_of_many_inputs(m, n, k, group):
+    """Sums of 512 inputs are 64 additions on the tensor cores, which cut off less than 2^-24 of the sum each, half of that in the mean; what is summed in 32 bits from there on
+    rounds both ways.  Every row of weights is held against 64 bits over some rows of activations."""
+    from dryft_b200.parts.base import Runtime
+    from dryft_b200.parts.linear import linear
+
+    w = (torch.randn(n, k, device=DEV) * torch.exp(0.3 * torch.randn(n, 1, device=DEV))).to(BF)
+    x = (torch.randn(m, k, device=DEV) * torch.exp(0.5 * torch.randn(1, k, device=DEV))).to(BF)
+    w4, values = K().pack_weight4(w, group), torch.empty(n, k, device=DEV)
+    K().weight4_expand(w4, values)           # (held against 64 bits elsewhere)
+    y = linear(x, w4, Runtime(dtype=BF, device=torch.device(DEV)), out_dtype=torch.float32)
+    K().check_error_flags()
+    for rows in (slice(0, 8), slice(max(0, m - 8), m)):
+        want = x[rows].double() @ values.double().T
+        e = float((y[rows].double() - want).norm() / want.norm())
+        assert e <= 64 * 2.0**-25, f"off by {e:.3g} of the whole ({64 * 2.0**-25:.3g} allowed)"

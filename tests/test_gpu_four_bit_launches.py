@@ -47,6 +47,20 @@ def test_every_launch_of_a_product_is_counted(m, n, k, dtype):
     assert K().launch_count - before == made
 
 
+@pytest.mark.parametrize("m,n,k,passes", [(48, 2560, 1280, 1), (128, 148 * 128, 256, 1), (129, 389, 64, 2), (200, 2560, 1280, 2), (256, 148 * 128, 256, 2)])
+def test_every_launch_of_a_product_with_a_32_bit_result_is_counted(m, n, k, passes):
+    """More than 128 rows are two passes; with overlapped launches and without, the same bits."""
+    w4, x, y = K().pack_weight4(torch.randn(n, k, device=DEV), 16), torch.randn(m, k, device=DEV).to(BF), {}
+    for pdl in (True, None, False):
+        y[pdl] = K().linear4(x, w4, out_dtype=F32, pdl=pdl)
+        before = K().launch_count
+        made, overlapped = _captured(lambda: (x.mul_(1.0), K().linear4(x, w4, out_dtype=F32, pdl=pdl)))
+        assert K().launch_count - before == made - 1 and made - 1 in (passes, 2 * passes)
+        assert overlapped == {True: made - 1, None: made - 2, False: 0}[pdl]
+    assert torch.equal(y[True], y[False]) and torch.equal(y[None], y[False])
+    K().check_error_flags()
+
+
 @pytest.mark.parametrize("m,n,edges", [(4, 389, {True: 1, None: 0, False: 0}), (48, 2560, {True: 2, None: 1, False: 0})])
 def test_a_products_launches_follow_the_switch(m, n, edges):
     w4, x, y = K().pack_weight4(torch.randn(n, 1280, device=DEV)), torch.randn(m, 1280, device=DEV).to(BF), {}
