@@ -40,8 +40,8 @@ __device__ __forceinline__ Work work_of_block() {   // grid (splits, key heads x
 // S^T = K Q^T and O^T = V^T P^T on mma.sync.m16n8k16, the codes straight out of the cache's words: keys' as bfloat16 16 + c (`code_pair`), values' as float16 c - 8:
 //   score  = s_k (sum (16 + c) q - 23.5 sum q) + z_k sum q          group by group, in 32 bits; sum q is the query's own
 //   output = sum p' (c - 8) / unit + sum p (z_v + s_v / 2)          p' = fp16(p s_v unit): the weight rounded with its scale, by up to 2^-11
-// `unit` is a power of two that keeps p' between float16's ends: set when a tile's scales are larger than all before it (the first tile's are), so a weight whose scale is
-// less than 2^-20 of the largest loses bits, and nothing that shows.  Scores, running maximum and sums are 32-bit.  (Weights in bfloat16 and values as 16 + c, corrected by
+// `unit` is a power of two that keeps p' between float16's ends: set when a tile's scales are larger than all before it (the first tile's are), so a weight with a
+// scale is off by up to 2^-29 of the largest scale, where that is more than 2^-11 of its own (scales 2^18 apart).  Scores, running maximum and sums are 32-bit.  (Weights in bfloat16 and values as 16 + c, corrected by
 // -23.5 sum p': off by 0.0023 of the whole, not 0.0017, which the result's own rounding is; and the tensor cores cut sums off, not round them, which took another
 // 0.0013 of sums three times as large over 128 tiles.)
 // A warp walks tiles of 16 keys of its own, copied STAGES - 1 tiles ahead into its own ring.  The maximum

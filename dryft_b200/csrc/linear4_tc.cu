@@ -13,7 +13,7 @@
 //
 // What bounds it: every tile reads all of x again, from L2, which moves 9 TB/s at 48 rows (issue slots are used at 64% beside it, the tensor cores at 32%) and 10 at 256
 // rows (41 and 57%).  48 rows: 2,560 outputs of 9,728 inputs 12.6 us (of which some 3 us the launch and 3 us the join), 19,456 of 2,560 16.8 us, 151,936 of 2,560 78 us
-// (32-bit results 177: two products and twice the taking out); 128 and 256 rows, 19,456 of 2,560: 24 and 39 us.
+// (32-bit results 188: two products and twice the taking out); 128 and 256 rows, 19,456 of 2,560: 24 and 39 us.
 // (Steps on the way, 48 rows, 19,456 of 2,560: weights written into shared memory as the operand 22 us; into tensor memory 21.4, by then bound by the one thread that
 // issued products, 500 cycles a unit to put their operands into uniform registers; with a whole warp that walks the loop 17.5; one barrier for weights and x, asked
 // ahead of the products before, 16.7.)
