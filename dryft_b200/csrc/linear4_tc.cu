@@ -122,7 +122,7 @@ template <int NB> constexpr int units_of() { return NB == 256 ? 1 : 2; }
 template <int NB, int GN, bool LOW> struct Layout {
   static constexpr int KU = units_of<NB>(), X_BLOCK = NB * BK * 2, STAGE_BYTES = X_BLOCK * KU;   // a stage of x, block by block; multiples of 1024
   static constexpr int SUMS_BYTES = LOW ? NB * BM * 4 : 0;                                       // of segments (below)
-  static constexpr int RING = !LOW || NB < 128 ? 8 : NB < 256 ? 6 : 4;                           // units whose codes are on their way
+  static constexpr int RING = LOW && NB == 128 ? 6 : 8;                                          // units whose codes are on their way
   static constexpr int CODE_BYTES = 4096 * KU, SCALE_BYTES = 512 * GN, SLOT_BYTES = CODE_BYTES + SCALE_BYTES, RING_BYTES = RING * SLOT_BYTES;   // multiples of 128
   // tensor memory: sums of ACCS runs, then the stages of weights (LOW: and of their rests), two inputs a column
   static constexpr int ACCS = NB == 256 ? 1 : 2, W_COLS = BK / 2 * KU, STAGE_COLS = W_COLS * (LOW ? 2 : 1), W_COL0 = ACCS * NB, TMEM_COLS = 512;
@@ -135,6 +135,7 @@ template <int NB, int GN, bool LOW> struct Layout {
   // Units that are summed in tensor memory at a time.  Every product there cuts what it adds to off, not rounds it: 2^-26 of the sum each in the mean, always towards zero.
   // For 32-bit results 512 inputs, 64 products, are summed so; their sums are added up in shared memory by the threads that read them, rounded.
   static constexpr int SEGMENT = LOW ? 512 / (BK * KU) : 1 << 30;
+  static_assert(!LOW || NB <= 128, "sums of segments fit beside up to 128 rows");
   static_assert(STAGES >= 2 && TEAMS <= STAGES && TEAMS <= RING, "phases of a stage's barrier");
   static_assert(W_COL0 + STAGES * STAGE_COLS <= TMEM_COLS, "of tensor memory");
   static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + RING_BYTES + SUMS_BYTES + 8 * (2 * STAGES + 2 * RING + 4) + 64;

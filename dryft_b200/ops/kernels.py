@@ -2656,11 +2656,12 @@ def _overlap(pdl: Optional[bool]) -> int:
 
 def linear4(x, w: Weight4, out=None, pdl: Optional[bool] = None, mode: str = "store", norm_w=None, eps: float = 0.0, out_dtype=None):
     """``out = x @ w.T``; ``x`` bfloat16, up to 256 rows (float32: 64), ``out`` of the same type or float32 (none: a new tensor, of ``out_dtype`` or ``x``'s
-    type).  Returns ``out``.  ``pdl``: a programmatic dependent: its
-    first weights are requested while the launch before it drains, so codes and scales are older than the last launch in front of it that is not such a
-    dependent itself (``pack_weight4`` sees to that for those it makes); ``False``: no launch overlaps another; ``None``: only this product's further launches, each the one
-    before.  Where ``x`` is infinite or not a number the result is what the definition's sum
-    comes to (a result that is not finite is worked out again, input by input).
+    type).  Returns ``out``.
+
+    ``pdl``: a programmatic dependent: its first weights are requested while the launch before it drains, so codes and scales are older than the last launch in front
+    of it that is not such a dependent itself (``pack_weight4`` sees to that for those it makes); ``False``: no launch overlaps another; ``None``: only this product's
+    further launches, each the one before.  Where ``x`` is infinite or not a number the result is what the definition's sum comes to (a result that is not finite is
+    worked out again, input by input).
 
     With few rows of bfloat16 (``linear4_fuses``) also what stands around a decoder's products: ``norm_w`` (float32 ``[k]``): RMS norm of ``x`` first;
     ``mode="residual"``: ``out += `` the result, in place (``out`` has to be given); ``mode="silu"``: ``w`` holds gate rows, then as many others, and ``out`` ``[m, n / 2]`` is
