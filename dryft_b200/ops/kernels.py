@@ -2725,6 +2725,201 @@ def weight4_expand(w: Weight4, out, rest: bool = False) -> None:
         "weight4_expand")
 
 
+# ----------------------------------------------------------------------------- microscaled 4-bit floating point: rounding, values, products
+# A number is one of 0, 1/2, 1, 3/2, 2, 3, 4, 6 or minus that, times the scale of its group; csrc/fp4.cuh has the arithmetic and the layout.
+FP4_KINDS = {"mx": 0, "nv": 1}                # groups of 32 with powers of two; groups of 16 with 8-bit floats, and a factor for each row
+_FP4_BLOCK = {"mx": 16384 + 1024, "nv": 16384 + 2048}   # bytes of 128 rows by 256 inputs: codes and scales
+
+
+def fp4_lib() -> ctypes.CDLL:
+    """Rounding to microscaled 4-bit floating point, its values, products of two such operands (tcgen05)."""
+    global _fp4
+    with _lock:
+        if _fp4 is None:
+            lib = _load(build.build_library("fp4", FP4_SOURCES))
+            lib.dryft_fp4_quantise.argtypes = [_i, _i, _p, _ll, _p, _p, _i, _i, _i, _p]
+            lib.dryft_fp4_expand.argtypes = [_i, _i, _p, _p, _p, _i, _i, _p]
+            lib.dryft_linear_fp4.argtypes = [_i, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p, _p]
+            for name in ("dryft_fp4_quantise", "dryft_fp4_expand", "dryft_linear_fp4"):
+                getattr(lib, name).restype = _i
+            _fp4 = lib
+        return _fp4
+
+
+FP4_SOURCES = ("fp4.cu", "linear_fp4.cu")
+_fp4: Optional[ctypes.CDLL] = None
+
+
+def _fp4_kind(kind: str) -> int:
+    code = FP4_KINDS.get(kind) if isinstance(kind, str) else None
+    if code is None:
+        raise KernelError(f"kind of 4-bit floating point is one of {', '.join(FP4_KINDS)}, got {kind!r}")
+    return code
+
+
+def _fp4_shape(n: int, k: int, kind: str) -> Tuple[int, int, int]:
+    return ((n + 127) // 128, (k + 255) // 256, _FP4_BLOCK[kind])
+
+
+@dataclass(frozen=True)
+class Fp4:
+    """A matrix ``[n, k]`` held in microscaled 4-bit floating point (``fp4_quantise`` makes it), laid out for the tensor cores.  ``held``: uint8, blocks of 128 rows by
+    256 inputs, scales in front of codes; ``factors``: float32, one for each row (``"nv"``)."""
+
+    held: torch.Tensor                 # uint8 [blocks of 128 rows, blocks of 256 inputs, bytes of a block]
+    factors: Optional[torch.Tensor]    # float32 [n] (None for "mx")
+    n: int
+    k: int
+    kind: str
+
+    def __post_init__(self) -> None:
+        """What every use relies on is looked at once, here."""
+        _fp4_kind(self.kind)
+        if self.n <= 0 or self.k <= 0:
+            raise KernelError(f"Fp4: no numbers in [{self.n}, {self.k}]")
+        wanted = [(self.held, "held", torch.uint8, _fp4_shape(self.n, self.k, self.kind), 16)]
+        if self.kind == "nv":
+            wanted.append((self.factors, "factors", torch.float32, (self.n,), 4))
+        elif self.factors is not None:
+            raise KernelError("Fp4: rows have factors of their own in the kind 'nv' only")
+        for t, name, dtype, shape, word in wanted:
+            if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.data_ptr() % word:
+                raise KernelError(f"Fp4: {name} is {dtype} of shape {shape}, contiguous, on a {word}-byte boundary")
+            if t.device != self.held.device:
+                raise KernelError("Fp4: held and factors are on two devices")
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return (self.n, self.k)
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return torch.uint8
+
+    @property
+    def device(self) -> torch.device:
+        return self.held.device
+
+    def nbytes(self) -> int:
+        return self.held.numel() + (0 if self.factors is None else 4 * self.factors.numel())
+
+    def __getitem__(self, at: slice) -> "Fp4":
+        """A range of rows; its first is a multiple of 128, as blocks are."""
+        if not isinstance(at, slice) or at.step not in (None, 1):
+            raise KernelError("Fp4: only a range of rows can be taken")
+        first, end, _ = at.indices(self.n)
+        if first % 128 or not first < end:
+            raise KernelError(f"Fp4: rows {first}..{end} of {self.n}; the first is a multiple of 128")
+        return Fp4(self.held[first // 128:(end + 127) // 128], None if self.factors is None else self.factors[first:end], end - first, self.k, self.kind)
+
+
+def _on_current(t, name: str) -> None:
+    """Launches go to the current device's stream: what they read and write is there."""
+    if not t.is_cuda:
+        raise KernelError(f"{name}: is on {t.device}; dryft_b200 kernels run on a CUDA device only")
+    if t.get_device() != torch.cuda.current_device():
+        raise KernelError(f"{name}: is on {t.device}, and the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _need_fp4(w, name: str) -> None:
+    if not isinstance(w, Fp4):
+        raise KernelError(f"{name}: expected an Fp4 (fp4_quantise makes one), got {type(w).__name__}")
+    _on_current(w.held, name)
+
+
+def _fp4_rows(x, name: str) -> int:
+    """Rows of consecutive numbers, any distance apart; the distance."""
+    if not isinstance(x, torch.Tensor):
+        raise KernelError(f"{name}: expected a tensor, got {type(x).__name__}")
+    _act(x, name)
+    if x.dim() != 2:
+        raise KernelError(f"{name}: expected rows of numbers, got shape {tuple(x.shape)}")
+    step, one = x.stride()
+    if one != 1 and x.shape[1] > 1:
+        raise KernelError(f"{name}: the numbers of a row lie behind one another (strides {x.stride()})")
+    _on_current(x, name)
+    return step
+
+
+def _fp4_quantise(x, step: int, kind: str, pdl: bool) -> Fp4:
+    global launch_count
+    m, k = x.shape
+    held = torch.empty(_fp4_shape(m, k, kind), dtype=torch.uint8, device=x.device)
+    factors = torch.empty(m, dtype=torch.float32, device=x.device) if kind == "nv" else None
+    _ok(fp4_lib().dryft_fp4_quantise(x.dtype == torch.bfloat16, FP4_KINDS[kind], x.data_ptr(), step, held.data_ptr(), _ptr(factors), m, k, pdl, _stream()), "fp4_quantise")
+    return Fp4(held, factors, m, k, kind)
+
+
+def fp4_quantise(x, kind: str) -> Fp4:
+    """``x`` ``[rows, k]`` (float32 or bfloat16, rows any distance apart) in microscaled 4-bit floating point: ``"mx"``, groups of 32 numbers with a power of two as their
+    scale, or ``"nv"``, groups of 16 with an 8-bit float and a 32-bit factor for each row.  Any ``k``; a last group may be short.  A group with an infinity or a NaN stands for NaN.
+    For weights, once, when they are loaded, and for activations that several products read."""
+    _fp4_kind(kind)
+    step = _fp4_rows(x, "x")
+    if x.shape[0] == 0 or x.shape[1] == 0:
+        raise KernelError(f"fp4_quantise: no numbers in {tuple(x.shape)}")
+    return _fp4_quantise(x, step, kind, False)
+
+
+def fp4_expand(q: Fp4, out=None, out_dtype=torch.bfloat16):
+    """``out`` ``[n, k]`` (float32 or bfloat16; none: a new tensor, of ``out_dtype``): what the codes stand for.  Returns ``out``."""
+    _need_fp4(q, "q")
+    if out is None:
+        if out_dtype not in (torch.float32, torch.bfloat16):
+            raise KernelError(f"fp4_expand: values are float32 or bfloat16, got {out_dtype}")
+        out = torch.empty((q.n, q.k), dtype=out_dtype, device=q.device)
+    else:
+        _need(out, "out", None, (q.n, q.k))
+        _on_current(out, "out")
+    _ok(fp4_lib().dryft_fp4_expand(_act(out, "out"), FP4_KINDS[q.kind], q.held.data_ptr(), _ptr(q.factors), out.data_ptr(), q.n, q.k, _stream()), "fp4_expand")
+    return out
+
+
+def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = False, out_dtype=None):
+    """``out = x @ w.T`` with both operands in microscaled 4-bit floating point, summed in 32 bits; ``x`` float32 or bfloat16, rows any distance apart, rounded row by row to ``w``'s
+    kind on the way, or an ``Fp4`` of that kind.  ``out`` float32 or bfloat16 (none: a new tensor, of ``out_dtype`` or ``x``'s type; bfloat16 for an ``Fp4``).  Returns ``out``.
+
+    ``silu``: ``x`` ``[m, 2 k]`` holds gate columns, then as many others, and the product's operand is ``silu(gate) * other`` (rounding points are ``silu_mul``'s).
+
+    ``pdl``: a programmatic dependent of the launch before it; ``None``: only the product, of its own rounding; ``False``: no launch overlaps another.  Weights are read once the
+    launch in front of the rounding has ended, so they may be as new as that one (with an ``Fp4`` and ``pdl``: older than the launch in front)."""
+    _need_fp4(w, "weight")
+    given = isinstance(x, Fp4)
+    if given:
+        _need_fp4(x, "x")
+        if silu:
+            raise KernelError("linear_fp4: silu is taken of float32 or bfloat16 activations")
+        if x.kind != w.kind:
+            raise KernelError(f"linear_fp4: x is held as {x.kind!r}, the weight as {w.kind!r}")
+        m, width = x.n, x.k
+    else:
+        step = _fp4_rows(x, "x")
+        m, width = x.shape
+    if width != (2 * w.k if silu else w.k):
+        raise KernelError(f"linear_fp4: rows of {2 * w.k if silu else w.k} numbers go with a weight {w.shape}, got {width}")
+    if out is None:
+        dtype = out_dtype or (torch.bfloat16 if given else x.dtype)
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise KernelError(f"linear_fp4: results are float32 or bfloat16, got {dtype}")
+        out = torch.empty((m, w.n), dtype=dtype, device=w.device)
+    else:
+        _need(out, "out", None, (m, w.n))
+        _on_current(out, "out")
+    out_bf16 = _act(out, "out")
+    if m == 0:
+        return out
+    overlap = bool(pdl)
+    if not given:
+        if silu:
+            act = torch.empty((m, w.k), dtype=x.dtype, device=x.device)
+            silu_mul(x, act)
+            x, step = act, w.k
+        x, overlap = _fp4_quantise(x, step, w.kind, bool(pdl)), pdl is not False
+    _ok(fp4_lib().dryft_linear_fp4(FP4_KINDS[w.kind], out_bf16, x.held.data_ptr(), _ptr(x.factors), w.held.data_ptr(), _ptr(w.factors), out.data_ptr(), m, w.n, w.k, overlap,
+                                   error_flag(w.device).data_ptr(), _stream()), "linear_fp4")
+    return out
+
+
 _kv4_fns = None   # (store, expand)
 
 

@@ -10,7 +10,9 @@ Which product runs:
   * bfloat16 activations with a weight the checkpoint stores in 32-bit: the weight stays 32-bit,
     the activations are widened, the 32-bit product runs and its result is rounded once;
   * weights held in 4 bits (``ops.kernels.Weight4``): up to 256 rows of bfloat16 (64 of float32) the kernels that
-    read the codes, above that the weights are taken out of their 4 bits for the products above.
+    read the codes, above that the weights are taken out of their 4 bits for the products above;
+  * weights in microscaled 4-bit floating point (``ops.kernels.Fp4``): the activations' rows are rounded to it too, and
+    tcgen05.mma multiplies both as they are held, whatever their number.
 """
 
 from __future__ import annotations
@@ -31,6 +33,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, rt: Runtime, out_dtype: Optional[to
         raise ValueError(f"linear: activations have width {k}, weight is {tuple(w.shape)}")
     if isinstance(w, K.Weight4):
         return _linear4(x, w, rt, out_dtype)
+    if isinstance(w, K.Fp4):
+        return K.linear_fp4(x, w, pdl=rt.pdl, out_dtype=out_dtype)
     if x.dtype == torch.float32:
         if w.dtype != torch.float32:
             raise ValueError(f"linear: 32-bit activations need a 32-bit weight, got {w.dtype}")
