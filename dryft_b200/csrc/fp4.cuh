@@ -39,4 +39,9 @@ __device__ __forceinline__ float scale_value(unsigned byte, bool nv) {
   }
   return byte == MX_NAN ? __uint_as_float(0x7fffffffu) : byte == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);   // (2^-127 has no exponent bits)
 }
+// 32 bytes: a whole sector a lane
+__device__ __forceinline__ void st_words8(void* to, const unsigned* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
 }  // namespace fp4

@@ -13,7 +13,6 @@
 namespace {
 using namespace fp4;
 typedef __nv_bfloat16 bf16;
-constexpr int THREADS = 6 * 32;
 constexpr long long WAIT_CYCLES = 2000000000LL;
 constexpr unsigned SLEEP_NS = 10000;
 
@@ -33,10 +32,17 @@ __device__ __forceinline__ bool mbar_try_wait(void* bar, unsigned parity) {
                : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(SLEEP_NS) : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ bool mbar_wait(void* bar, unsigned parity, int* err, volatile int* failed, int site) {
-  if (mbar_try_wait(bar, parity)) return true;
+__device__ __forceinline__ bool mbar_try_wait_cluster(void* bar, unsigned parity) {   // for what other blocks of the cluster arrive at
+  unsigned ok;
+  asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
+               : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(SLEEP_NS) : "memory");
+  return ok != 0;
+}
+template <bool CLUSTER = false> __device__ __forceinline__ bool mbar_wait(void* bar, unsigned parity, int* err, volatile int* failed, int site) {
+  auto there = [&] { return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
+  if (there()) return true;
   const long long t0 = clock64();
-  while (!mbar_try_wait(bar, parity)) {
+  while (!there()) {
     if (*failed) return false;
     if (clock64() - t0 > WAIT_CYCLES) {
       if (err) atomicCAS(err, 0, 300 + site);   // the first wait that gave up names its place
@@ -60,24 +66,26 @@ __device__ __forceinline__ unsigned long long scales_desc(const void* smem) {
   return (unsigned long long)((smem_u32(smem) & 0x3FFFF) >> 4) | (unsigned long long)(128 >> 4) << 32 | (unsigned long long)1 << 46;
 }
 // 32 rows of 16 bytes into four columns, the same in each quarter of the lanes
-__device__ __forceinline__ void scales_to_tmem(unsigned taddr, unsigned long long desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+template <int CTAS = 1> __device__ __forceinline__ void scales_to_tmem(unsigned taddr, unsigned long long desc) {
+  if (CTAS == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");   // in both blocks, each from its own shared memory
 }
-// Instruction descriptor: A and B E2M1, N >> 3 at bit 17, scales' type at bit 23 (0 E4M3, 1 E8M0), M >> 7 at bit 27; which of a word's scales the instruction takes at
+// Instruction descriptor: A and B E2M1, N >> 3 at bit 17 (added by the caller), scales' type at bit 23 (0 E4M3, 1 E8M0), M >> 7 at bit 27; which of a word's scales the instruction takes at
 // bits 4 (B) and 29 (A): all four (NV), the first or the second two (MX).
-template <int KIND> __device__ __forceinline__ constexpr unsigned idesc(int n, int scale) {
-  return (1u << 7) | (1u << 10) | ((unsigned)(n >> 3) << 17) | (KIND == MX ? 1u << 23 : 0u) | (1u << 27) | ((unsigned)scale << 4) | ((unsigned)scale << 29);
+template <int KIND, int M = 128> __device__ __forceinline__ constexpr unsigned idesc(int scale) {
+  return (1u << 7) | (1u << 10) | (KIND == MX ? 1u << 23 : 0u) | ((unsigned)(M >> 7) << 27) | ((unsigned)scale << 4) | ((unsigned)scale << 29);
 }
 // D[tmem] (+)= A[smem] B[smem], 64 inputs
-template <int KIND> __device__ __forceinline__ void umma(unsigned d, unsigned long long a, unsigned long long b, unsigned id, unsigned sa, unsigned sb, unsigned accumulate) {
-  if (KIND == NV)
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(sa), "r"(sb), "r"(accumulate) : "memory");
-  else
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(sa), "r"(sb), "r"(accumulate) : "memory");
+#define DRYFT_FP4_MMA(group, kind)                                                                       \
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                         \
+               "tcgen05.mma.cta_group::" group "." kind " [%0], %1, %2, %3, [%4], [%5], p;\n\t}"           \
+               ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(sa), "r"(sb), "r"(accumulate) : "memory")
+template <int KIND, int CTAS = 1>
+__device__ __forceinline__ void umma(unsigned d, unsigned long long a, unsigned long long b, unsigned id, unsigned sa, unsigned sb, unsigned accumulate) {
+  if (KIND == NV && CTAS == 1) DRYFT_FP4_MMA("1", "kind::mxf4nvf4.block_scale.scale_vec::4X");
+  else if (KIND == NV) DRYFT_FP4_MMA("2", "kind::mxf4nvf4.block_scale.scale_vec::4X");
+  else if (CTAS == 1) DRYFT_FP4_MMA("1", "kind::mxf4.block_scale.scale_vec::2X");
+  else DRYFT_FP4_MMA("2", "kind::mxf4.block_scale.scale_vec::2X");
 }
 __device__ __forceinline__ bool elected() {   // one lane of the warp
   unsigned one;
@@ -106,35 +114,82 @@ struct Params {
   int m, n, blocks;   // blocks: of 256 inputs
 };
 
-template <int KIND, int NB> struct Layout {
+// SPLIT: a tile's inputs are shared out among a cluster's blocks.
+template <int KIND, int NB, bool SPLIT> struct Layout {
   typedef Format<KIND> F;
-  static constexpr int XB = NB > ROWS ? 2 : 1;                                   // blocks of x in a stage
-  static constexpr int X_CODES = NB * (INPUTS / 2), X_BYTES = XB * F::SCALE_BYTES + X_CODES, STAGE_BYTES = F::BLOCK_BYTES + X_BYTES;   // multiples of 1024
-  static constexpr int ROOM = 225 * 1024 / STAGE_BYTES, STAGES = ROOM < 12 ? ROOM : 12;
+  // warps that read sums: four take a quarter of the rows each, and PARTS fours a part of the columns, so that each scheduler has several to hide their latencies
+  static constexpr int PARTS = NB <= 16 ? 1 : NB <= 32 ? 2 : 4, READERS = 4 * PARTS, THREADS = (2 + READERS) * 32;
+  static constexpr int BB = NB > ROWS ? 2 : 1;                                   // blocks of the N side in a stage
+  static constexpr int B_CODES = NB * (INPUTS / 2), B_BYTES = BB * F::SCALE_BYTES + B_CODES, STAGE_BYTES = F::BLOCK_BYTES + B_BYTES;   // multiples of 1024
+  static constexpr int RESIDENT = NB > ROWS ? 1 : 2;                                 // blocks of a multiprocessor
+  static constexpr int ROOM = (RESIDENT == 2 ? 110 : 225) * 1024 / STAGE_BYTES, STAGES = ROOM < 12 ? ROOM : 12;
   // tensor memory: sums of ACCS tiles, then the scales of two stages
-  static constexpr int ACCS = NB > 128 ? 1 : 2, SCALE_COLS = 4 * F::WORDS * (1 + XB), NEED_COLS = ACCS * NB + 2 * SCALE_COLS;
+  static constexpr int ACCS = SPLIT || NB >= 128 ? 1 : 2, SCALE_COLS = 4 * F::WORDS * (1 + BB), NEED_COLS = ACCS * NB + 2 * SCALE_COLS;
   static constexpr int TMEM_COLS = NEED_COLS <= 128 ? 128 : NEED_COLS <= 256 ? 256 : 512;
   static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + 8 * (2 * STAGES + 4) + 16;
-  static_assert(NEED_COLS <= 512 && SMEM_BYTES <= 227 * 1024 && STAGES >= 3, "of a block");
+  static_assert(RESIDENT * TMEM_COLS <= 512 && RESIDENT * (SMEM_BYTES + 2048) <= 228 * 1024 && STAGES >= 3, "of a block");
+  static_assert(!SPLIT || (NB + 7 * 4) * ROWS * 4 <= STAGES * STAGE_BYTES, "sums fit where the stages were");
 };
 
-template <int KIND, int NB, typename O> __global__ void __launch_bounds__(THREADS, 1) linear_fp4_kernel(const Params p) {
-  typedef Layout<KIND, NB> L;
+__device__ __forceinline__ unsigned cluster_rank() {
+  unsigned r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ unsigned cluster_size() {
+  unsigned r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// into another block's shared memory, at the address that this block has the like at
+__device__ __forceinline__ void st_cluster(unsigned addr, unsigned rank, float a, float b, float c, float d) {
+  asm volatile("{ .reg .u32 a; mapa.shared::cluster.u32 a, %0, %1; st.shared::cluster.v4.f32 [a], {%2, %3, %4, %5}; }" ::"r"(addr), "r"(rank), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+constexpr int MOST_BLOCKS = 8;   // of a cluster
+
+// A warp's results: columns (rows of x) of one row of W a lane.
+template <int KIND, int COLS, typename O>
+__device__ __forceinline__ void write_columns(const Params& p, O* to, bool there, int cols, float (&v)[COLS / 16][16], float own, const float (&x_factor)[(COLS + 31) / 32]) {
+#pragma unroll
+  for (int c = 0; c < COLS / 16; ++c) {
+    if (16 * c >= cols) break;
+    if (KIND == NV)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[c][j] = v[c][j] * own * __shfl_sync(0xffffffffu, x_factor[c / 2], (16 * c + j) % 32);
+    if (there)   // (apart from the exchanges, which are all lanes')
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (16 * c + j < cols) to[(size_t)(16 * c + j) * p.n] = from_f32<O>(v[c][j]);
+  }
+}
+
+template <int KIND, int NB, bool SPLIT, typename O>
+__global__ void __launch_bounds__(Layout<KIND, NB, SPLIT>::THREADS, Layout<KIND, NB, SPLIT>::RESIDENT) linear_fp4_kernel(const Params p) {
+  typedef Layout<KIND, NB, SPLIT> L;
   typedef typename L::F F;
-  constexpr int STAGES = L::STAGES, XB = L::XB;
+  constexpr int STAGES = L::STAGES, BB = L::BB, READ_THREADS = L::READERS * 32;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* const stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned long long* const full = reinterpret_cast<unsigned long long*>(stages + STAGES * L::STAGE_BYTES);   // [S] copies -> products
   unsigned long long* const empty = full + STAGES;                                                             // [S] products -> copies
   unsigned long long* const acc_full = empty + STAGES;                                                         // [2] a tile's sums -> their readers
-  unsigned long long* const acc_empty = acc_full + 2;                                                          // [2] read (128 arrivals) -> products
+  unsigned long long* const acc_empty = acc_full + 2;                                                          // [2] read (by every reader) -> products
   unsigned* const tmem_slot = reinterpret_cast<unsigned*>(acc_empty + 2);
   __shared__ int failed_s, issued_s;
   __shared__ unsigned long long drained_s;
   volatile int* const failed = &failed_s;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, KB = p.blocks;
-  const int x_tiles = (p.m + NB - 1) / NB, tiles = (p.n + ROWS - 1) / ROWS * x_tiles;   // those of one W row range behind one another: W crosses memory once
+  const int x_tiles = (p.m + NB - 1) / NB, tiles = (p.n + ROWS - 1) / ROWS * x_tiles;   // those of one W row range are behind one another: W crosses memory once
+  // this block's tiles, and its share of their inputs
+  const unsigned rank = SPLIT ? cluster_rank() : 0, size = SPLIT ? cluster_size() : 1;
+  const int first_tile = blockIdx.x / size, step = SPLIT ? tiles : gridDim.x, k0 = SPLIT ? KB * rank / size : 0, k1 = SPLIT ? KB * (rank + 1) / size : KB;
+
+  // columns of a tile that has so many rows of x left: whole sixteens
+  auto columns = [](int left) { return left >= NB ? NB : (left + 15) / 16 * 16; };
 
   if (threadIdx.x == 0) {
     failed_s = issued_s = 0;
@@ -145,7 +200,7 @@ template <int KIND, int NB, typename O> __global__ void __launch_bounds__(THREAD
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 128);
+      mbar_init(&acc_empty[b], READ_THREADS);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -164,33 +219,34 @@ template <int KIND, int NB, typename O> __global__ void __launch_bounds__(THREAD
     int i = 0, s = 0;
     unsigned par = 1;   // (the first turn finds every stage free)
     bool ok = true, waited = false;
-    for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-      const unsigned char* const w = p.w + (size_t)(t / x_tiles) * KB * F::BLOCK_BYTES;
-      const unsigned char* const x = p.x + (size_t)(t % x_tiles) * XB * KB * F::BLOCK_BYTES;
-      const bool second = XB == 2 && (t % x_tiles) * NB + ROWS < p.m;   // (rows behind the last block of x: any numbers do)
-      for (int kb = 0; kb < KB; ++kb, ++i) {
+    for (int t = first_tile; ok && t < tiles; t += step) {
+      const unsigned char* w = p.w + ((size_t)(t / x_tiles) * KB + k0) * F::BLOCK_BYTES;
+      const unsigned char* x = p.x + ((size_t)(t % x_tiles) * BB * KB + k0) * F::BLOCK_BYTES;
+      const int left = p.m - t % x_tiles * NB;
+      const unsigned x_codes = columns(left) * (INPUTS / 2);                        // bytes of the rows that there are
+      for (int kb = k0; kb < k1; ++kb, ++i, w += F::BLOCK_BYTES, x += F::BLOCK_BYTES) {
         ok = i < STAGES || __all_sync(0xffffffffu, mbar_wait(&empty[s], par, p.err, failed, 1));
         if (!ok) break;
         unsigned char* const to = stages + (size_t)s * L::STAGE_BYTES;
         if (issues) {
-          mbar_expect_tx(&full[s], XB == 2 && !second ? F::BLOCK_BYTES * 2 : L::STAGE_BYTES);
-          bulk_load(to, w + (size_t)kb * F::BLOCK_BYTES, F::BLOCK_BYTES, &full[s]);
+          mbar_expect_tx(&full[s], F::BLOCK_BYTES + (BB == 2 && left > ROWS ? 2 : 1) * F::SCALE_BYTES + x_codes);
+          bulk_load(to, w, F::BLOCK_BYTES, &full[s]);   // W depends on no launch that may still be running
         }
-        if (!waited) {   // W depends on no launch that may still be running
+        if (!waited) {
           asm volatile("griddepcontrol.wait;" ::: "memory");
           waited = true;
         }
         if (issues) {
-          const unsigned char* const xb = x + (size_t)kb * F::BLOCK_BYTES;
-          if (XB == 1) bulk_load(to + F::BLOCK_BYTES, xb, L::X_BYTES, &full[s]);
+          if (BB == 1) bulk_load(to + F::BLOCK_BYTES, x, F::SCALE_BYTES + x_codes, &full[s]);
           else {
             unsigned char* const scales = to + F::BLOCK_BYTES;
-            unsigned char* const codes = scales + XB * F::SCALE_BYTES;
-            bulk_load(scales, xb, F::SCALE_BYTES, &full[s]);
-            bulk_load(codes, xb + F::SCALE_BYTES, CODE_BYTES, &full[s]);
-            if (second) {
-              bulk_load(scales + F::SCALE_BYTES, xb + (size_t)KB * F::BLOCK_BYTES, F::SCALE_BYTES, &full[s]);
-              bulk_load(codes + CODE_BYTES, xb + (size_t)KB * F::BLOCK_BYTES + F::SCALE_BYTES, CODE_BYTES, &full[s]);
+            unsigned char* const codes = scales + BB * F::SCALE_BYTES;
+            bulk_load(scales, x, F::SCALE_BYTES, &full[s]);
+            bulk_load(codes, x + F::SCALE_BYTES, min(x_codes, (unsigned)CODE_BYTES), &full[s]);
+            if (left > ROWS) {
+              const unsigned char* const next = x + (size_t)KB * F::BLOCK_BYTES;
+              bulk_load(scales + F::SCALE_BYTES, next, F::SCALE_BYTES, &full[s]);
+              bulk_load(codes + CODE_BYTES, next + F::SCALE_BYTES, x_codes - CODE_BYTES, &full[s]);
             }
           }
         }
@@ -207,32 +263,32 @@ template <int KIND, int NB, typename O> __global__ void __launch_bounds__(THREAD
     int s = 0, run = 0;
     unsigned par = 0, buffer = 0;
     bool ok = true;
-    for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x, ++run) {
-      const int b = run % L::ACCS;
-      const unsigned d = tmem + b * NB;
-      ok = run < L::ACCS || __all_sync(0xffffffffu, mbar_wait(&acc_empty[b], (unsigned)((run / L::ACCS - 1) & 1), p.err, failed, 4));
-      for (int kb = 0; ok && kb < KB; ++kb) {
+    for (int t = first_tile; ok && t < tiles; t += step, ++run) {
+      const int acc = run % L::ACCS;
+      const unsigned d = tmem + acc * NB, n_bits = (unsigned)(columns(p.m - t % x_tiles * NB) >> 3) << 17;
+      ok = run < L::ACCS || __all_sync(0xffffffffu, mbar_wait(&acc_empty[acc], (unsigned)((run / L::ACCS - 1) & 1), p.err, failed, 4));
+      for (int kb = k0; ok && kb < k1; ++kb) {
         ok = __all_sync(0xffffffffu, mbar_wait(&full[s], par, p.err, failed, 2));
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (issues) {
           unsigned char* const at = stages + (size_t)s * L::STAGE_BYTES;
-          const unsigned sw = tmem + L::ACCS * NB + buffer * L::SCALE_COLS, sx = sw + 4 * F::WORDS;
-          const unsigned long long w_scales = scales_desc(at), x_scales = scales_desc(at + F::BLOCK_BYTES);
-          const unsigned long long w = codes_desc(at + F::SCALE_BYTES), x = codes_desc(at + F::BLOCK_BYTES + XB * F::SCALE_BYTES);
+          const unsigned sa = tmem + L::ACCS * NB + buffer * L::SCALE_COLS, sb = sa + 4 * F::WORDS;
+          const unsigned long long a_scales = scales_desc(at), b_scales = scales_desc(at + F::BLOCK_BYTES);
+          const unsigned long long a = codes_desc(at + F::SCALE_BYTES), b = codes_desc(at + F::BLOCK_BYTES + BB * F::SCALE_BYTES);
 #pragma unroll
           for (int j = 0; j < F::WORDS; ++j) {
-            scales_to_tmem(sw + 4 * j, w_scales + j * (512 >> 4));
+            scales_to_tmem(sa + 4 * j, a_scales + j * (512 >> 4));
 #pragma unroll
-            for (int h = 0; h < XB; ++h) scales_to_tmem(sx + 4 * XB * j + 4 * h, x_scales + (j * 512 + h * F::SCALE_BYTES >> 4));
+            for (int h = 0; h < BB; ++h) scales_to_tmem(sb + 4 * BB * j + 4 * h, b_scales + ((j * 512 + h * F::SCALE_BYTES) >> 4));
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int word = j * F::WORDS / 4;
-            umma<KIND>(d, w + 2 * j, x + 2 * j, idesc<KIND>(NB, KIND == MX ? 2 * (j & 1) : 0), sw + 4 * word, sx + 4 * XB * word, kb > 0 || j > 0);
+            umma<KIND>(d, a + 2 * j, b + 2 * j, idesc<KIND>(KIND == MX ? 2 * (j & 1) : 0) | n_bits, sa + 4 * word, sb + 4 * BB * word, kb > k0 || j > 0);
           }
           umma_commit(&empty[s]);
-          if (kb == KB - 1) umma_commit(&acc_full[b]);
+          if (kb == k1 - 1) umma_commit(&acc_full[acc]);
         }
         __syncwarp();
         buffer ^= 1;
@@ -243,29 +299,96 @@ template <int KIND, int NB, typename O> __global__ void __launch_bounds__(THREAD
       }
     }
   } else {
-    const int q = warp & 3;   // the quarter of tensor memory that this warp may read
+    const int q = warp & 3;                              // the quarter of tensor memory that this warp may read
+    constexpr int COLS = NB / L::PARTS;                  // columns that this warp reads, from `first` on
+    const int first = (warp - 2) / 4 * COLS;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     int run = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++run) {
-      const int b = run % L::ACCS, row = t / x_tiles * ROWS + q * 32 + lane, m0 = t % x_tiles * NB;
-      const float wf = KIND == NV && row < p.n ? p.w_factors[row] : 1.f;
-      if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[b], (unsigned)(run / L::ACCS & 1), p.err, failed, 5))) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const unsigned from = tmem + ((unsigned)(q * 32) << 16) + b * NB;
-#pragma unroll 1
-      for (int j0 = 0; j0 < NB && m0 + j0 < p.m; j0 += 16) {
-        float v[16];
-        tmem_ld16(from + j0, v);
-        const float xf = KIND == NV && m0 + j0 + (lane & 15) < p.m ? ld_prev(p.x_factors + m0 + j0 + (lane & 15)) : 1.f;
+    for (int t = first_tile; t < tiles; t += step, ++run) {
+      const int acc = run % L::ACCS, row = t / x_tiles * ROWS + q * 32 + lane, col0 = t % x_tiles * NB + first, cols = min(COLS, p.m - col0);   // cols: may be none
+      const float own = KIND == NV && row < p.n ? __ldg(p.w_factors + row) : 1.f;
+      float x_factor[(COLS + 31) / 32];   // of the columns, a lane each (asked for here, where there is time)
+      if constexpr (KIND == NV)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float f = __shfl_sync(0xffffffffu, xf, j);
-          if (m0 + j0 + j < p.m && row < p.n) reinterpret_cast<O*>(p.y)[(size_t)(m0 + j0 + j) * p.n + row] = from_f32<O>(KIND == NV ? v[j] * wf * f : v[j]);
-        }
-      }
+        for (int c = 0; c < (COLS + 31) / 32; ++c) x_factor[c] = 32 * c + lane < cols ? ld_prev(p.x_factors + col0 + 32 * c + lane) : 1.f;
+      if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[acc], (unsigned)(run / L::ACCS & 1), p.err, failed, 5))) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if constexpr (SPLIT) break;   // (below)
+      // into registers all at once, so that the next tile's products may begin
+      const unsigned from = tmem + ((unsigned)(q * 32) << 16) + acc * NB + first;
+      float v[COLS / 16][16];
+#pragma unroll
+      for (int c = 0; c < COLS / 16; ++c)
+        if (16 * c < cols) tmem_ld16(from + 16 * c, v[c]);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      mbar_arrive(&acc_empty[b]);
+      mbar_arrive(&acc_empty[acc]);
+      write_columns<KIND, COLS>(p, reinterpret_cast<O*>(p.y) + (size_t)col0 * p.n + row, row < p.n, cols, v, own, x_factor);
       __syncwarp();
+    }
+  }
+
+  if constexpr (SPLIT) {
+    // Columns go to the cluster's blocks in turn, GROUP at a time: every block sends the others its sums, into what were the stages ([block][group][row][4]), and adds up what it
+    // was sent, in the order of the inputs.  All threads come by here, whatever their waits came to; what is sent when one gave up is nobody's result.
+    constexpr int GROUP = 4, GROUPS = NB / GROUP;
+    const unsigned per_block = (GROUPS + size - 1) / size;
+    const int q = warp & 3, part = (warp - 2) / 4;
+    const int row = first_tile / x_tiles * ROWS + q * 32 + lane, col0 = first_tile % x_tiles * NB, cols = min(NB, p.m - col0);
+    const float own = KIND == NV && warp >= 2 && row < p.n ? __ldg(p.w_factors + row) : 1.f;
+    float x_factor[(NB + 31) / 32];
+    if constexpr (KIND == NV)
+#pragma unroll
+      for (int c = 0; c < (NB + 31) / 32; ++c) x_factor[c] = warp >= 2 && 32 * c + lane < cols ? ld_prev(p.x_factors + col0 + 32 * c + lane) : 1.f;
+    auto place = [&](unsigned block, unsigned group) { return (unsigned)(((block * per_block + group) * GROUP / 4 * ROWS + q * 32 + lane) * 16); };
+    __syncwarp();
+    cluster_sync();   // every block's products have ended, so its stages are free
+    if (warp >= 2) {
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const unsigned from = tmem + ((unsigned)(q * 32) << 16);
+#pragma unroll 1
+      for (int c = part * (NB / L::PARTS); c < min(cols, (part + 1) * (NB / L::PARTS)); c += 16) {
+        float v[16];
+        tmem_ld16(from + c, v);
+#pragma unroll
+        for (int j = 0; j < 16; j += 4)
+          if (c + j < cols) {
+            const unsigned g = (c + j) / GROUP;
+            st_cluster(smem_u32(stages) + place(rank, g / size) + (c + j) % GROUP / 4 * ROWS * 16, g % size, v[j], v[j + 1], v[j + 2], v[j + 3]);
+          }
+      }
+    }
+    __syncwarp();
+    cluster_sync();
+    if (warp >= 2) {
+#pragma unroll 1
+      for (unsigned i = part; (rank + size * i) * GROUP < cols; i += L::PARTS) {
+        const int c = (rank + size * i) * GROUP;
+        float v[GROUP];
+#pragma unroll
+        for (int j = 0; j < GROUP; ++j) v[j] = 0.f;
+#pragma unroll 4
+        for (unsigned b = 0; b < size; ++b)
+#pragma unroll
+          for (int j = 0; j < GROUP; j += 4) {
+            const float4 t = *reinterpret_cast<const float4*>(stages + place(b, i) + j / 4 * ROWS * 16);
+            v[j] += t.x;
+            v[j + 1] += t.y;
+            v[j + 2] += t.z;
+            v[j + 3] += t.w;
+          }
+        if (KIND == NV) {
+          float f = x_factor[0];
+#pragma unroll
+          for (int h = 1; h < (NB + 31) / 32; ++h)
+            if (c >= 32 * h) f = x_factor[h];
+#pragma unroll
+          for (int j = 0; j < GROUP; ++j) v[j] = v[j] * own * __shfl_sync(0xffffffffu, f, (c + j) % 32);
+        }
+        if (row < p.n)
+#pragma unroll
+          for (int j = 0; j < GROUP; ++j)
+            if (c + j < cols) reinterpret_cast<O*>(p.y)[(size_t)(col0 + c + j) * p.n + row] = from_f32<O>(v[j]);
+      }
     }
   }
 
@@ -288,18 +411,267 @@ template <int KIND, int NB, typename O> __global__ void __launch_bounds__(THREAD
   }
 }
 
-int sm_count() {
-  static int sms = 0;
-  if (sms == 0) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) sms = 148;
-  }
-  return sms;
+// The same for many rows of x: two blocks on neighbouring multiprocessors have a tile of 256 rows of W (128 each) against `nb` rows of x, of which each holds half: a product's
+// operands then cross from L2 once for twice the work (8 copies' worth of L2 instead of 12, which is what the one-block tiles of 256 wait for).  The first block issues the products of
+// both.  The second one's copies complete barriers of its own; its warp 1 passes that on.
+template <int KIND> struct PairLayout {
+  typedef Format<KIND> F;
+  static constexpr int MOST_NB = 256, PARTS = 4, READERS = 4 * PARTS, THREADS = (2 + READERS) * 32, COLS = MOST_NB / PARTS;
+  static constexpr int X_AT = F::BLOCK_BYTES + 2 * F::SCALE_BYTES, STAGE_BYTES = X_AT + MOST_NB / 2 * (INPUTS / 2);   // W's block, x's scales (all of the tile's), half of x's codes
+  static constexpr int STAGES = 225 * 1024 / STAGE_BYTES;
+  static constexpr int SCALE_COLS = 4 * F::WORDS * 3, TMEM_COLS = 512;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + 8 * (3 * STAGES + 2) + 16;
+  static_assert(MOST_NB + 2 * SCALE_COLS <= TMEM_COLS && SMEM_BYTES <= 227 * 1024 && STAGE_BYTES % 1024 == 0, "of a block");
+};
+__device__ __forceinline__ void mbar_arrive_at(void* bar, unsigned rank) {   // of a block of the cluster
+  asm volatile("{ .reg .u32 a; mapa.shared::cluster.u32 a, %0, %1; mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a]; }" ::"r"(smem_u32(bar)), "r"(rank) : "memory");
+}
+__device__ __forceinline__ void umma_commit_both(void* bar) {   // in both blocks
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((unsigned short)3) : "memory");
 }
 
-template <int KIND, int NB, typename O> int run(const Params& p, bool dependent, cudaStream_t st) {
-  typedef Layout<KIND, NB> L;
-  auto kern = linear_fp4_kernel<KIND, NB, O>;
+template <int KIND, typename O> __global__ void __launch_bounds__(PairLayout<KIND>::THREADS, 1) linear_fp4_pair_kernel(const Params p, int nb) {
+  typedef PairLayout<KIND> L;
+  typedef typename L::F F;
+  constexpr int STAGES = L::STAGES;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* const stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  unsigned long long* const full = reinterpret_cast<unsigned long long*>(stages + STAGES * L::STAGE_BYTES);   // [S] this block's copies
+  unsigned long long* const peer_full = full + STAGES;                                                         // [S] (of the first block) the other's copies
+  unsigned long long* const empty = peer_full + STAGES;                                                        // [S] products -> copies
+  unsigned long long* const acc_full = empty + STAGES;                                                         // a tile's sums -> their readers
+  unsigned long long* const acc_empty = acc_full + 1;                                                          // (of the first block) read, by every reading warp of both
+  unsigned* const tmem_slot = reinterpret_cast<unsigned*>(acc_empty + 1);
+  __shared__ int failed_s, issued_s;
+  __shared__ unsigned long long drained_s;
+  volatile int* const failed = &failed_s;
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, KB = p.blocks;
+  const unsigned rank = cluster_rank();
+  // whole tiles first, those of one W row range behind one another; then the last, shorter ones
+  const int w_blocks = (p.n + ROWS - 1) / ROWS, w_tiles = (w_blocks + 1) / 2, whole = p.m / nb, tiles = w_tiles * ((p.m + nb - 1) / nb);
+  struct Tile { int w, x0, cols; };
+  auto tile_of = [&](int t) {
+    const bool short_one = t >= w_tiles * whole;
+    Tile r;
+    r.w = (short_one ? t - w_tiles * whole : t / whole) * 2;                      // the first of its blocks of W
+    r.x0 = (short_one ? whole : t % whole) * nb;                                  // its first row of x
+    r.cols = short_one ? (p.m - r.x0 + 31) / 32 * 32 : nb;                          // columns: each block has half of them, whole sixteens
+    return r;
+  };
+  const int first_tile = blockIdx.x / 2, step = gridDim.x / 2;
+
+  if (threadIdx.x == 0) {
+    failed_s = issued_s = 0;
+    mbar_init(&drained_s, 1);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&peer_full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, 2 * L::READERS);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(L::TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();   // both have their barriers and their tensor memory
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const unsigned tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  let_next_launch_in();
+
+  if (warp == 0) {
+    const bool issues = elected();
+    int i = 0, s = 0;
+    unsigned par = 1;   // (the first turn finds every stage free)
+    bool ok = true, waited = false;
+    for (int t = first_tile; ok && t < tiles; t += step) {
+      const Tile at = tile_of(t);
+      // (an odd number of blocks of W: the last one again, for rows that are nobody's)
+      const unsigned char* w = p.w + (size_t)min(at.w + (int)rank, w_blocks - 1) * KB * F::BLOCK_BYTES;
+      const unsigned char* x = p.x + (size_t)(at.x0 / ROWS) * KB * F::BLOCK_BYTES;
+      // of the two blocks of x that the tile's rows are in: rows from..to are this block's half
+      const int off = at.x0 % ROWS, from = off + (int)rank * (at.cols / 2), to = from + at.cols / 2;
+      const unsigned head = from < ROWS ? (min(to, ROWS) - from) * (INPUTS / 2) : 0, tail = to > ROWS ? (to - max(from, ROWS)) * (INPUTS / 2) : 0;   // bytes in either
+      const bool second = off + at.cols > ROWS;
+      for (int kb = 0; kb < KB; ++kb, ++i, w += F::BLOCK_BYTES, x += F::BLOCK_BYTES) {
+        ok = i < STAGES || __all_sync(0xffffffffu, mbar_wait(&empty[s], par, p.err, failed, 11));
+        if (!ok) break;
+        unsigned char* const stage = stages + (size_t)s * L::STAGE_BYTES;
+        if (issues) {
+          mbar_expect_tx(&full[s], F::BLOCK_BYTES + (second ? 2 : 1) * F::SCALE_BYTES + head + tail);
+          bulk_load(stage, w, F::BLOCK_BYTES, &full[s]);   // W depends on no launch that may still be running
+        }
+        if (!waited) {
+          asm volatile("griddepcontrol.wait;" ::: "memory");
+          waited = true;
+        }
+        if (issues) {
+          const unsigned char* const next = x + (size_t)KB * F::BLOCK_BYTES;
+          bulk_load(stage + F::BLOCK_BYTES, x, F::SCALE_BYTES, &full[s]);
+          if (second) bulk_load(stage + F::BLOCK_BYTES + F::SCALE_BYTES, next, F::SCALE_BYTES, &full[s]);
+          if (head) bulk_load(stage + L::X_AT, x + F::SCALE_BYTES + from * (INPUTS / 2), head, &full[s]);
+          if (tail) bulk_load(stage + L::X_AT + head, next + F::SCALE_BYTES + (max(from, ROWS) - ROWS) * (INPUTS / 2), tail, &full[s]);
+        }
+        __syncwarp();
+        if (++s == STAGES) {
+          s = 0;
+          par ^= 1;
+        }
+      }
+    }
+    if (lane == 0) issued_s = i;
+  } else if (warp == 1 && rank == 1) {
+    int s = 0;
+    unsigned par = 0;
+    bool ok = true;
+    for (int t = first_tile; ok && t < tiles; t += step)
+      for (int kb = 0; kb < KB; ++kb) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&full[s], par, p.err, failed, 12));
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_at(&peer_full[s], 0);
+        if (++s == STAGES) {
+          s = 0;
+          par ^= 1;
+        }
+      }
+  } else if (warp == 1) {
+    const bool issues = elected();
+    int s = 0, run = 0;
+    unsigned par = 0, buffer = 0;
+    bool ok = true;
+    for (int t = first_tile; ok && t < tiles; t += step, ++run) {
+      const Tile at = tile_of(t);
+      const unsigned n_bits = (unsigned)(at.cols >> 3) << 17, shift = at.x0 % ROWS / 32;   // shift: columns of scales in front of the tile's
+      ok = run < 1 || __all_sync(0xffffffffu, mbar_wait<true>(acc_empty, (unsigned)((run - 1) & 1), p.err, failed, 14));
+      for (int kb = 0; ok && kb < KB; ++kb) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&full[s], par, p.err, failed, 12) && mbar_wait<true>(&peer_full[s], par, p.err, failed, 13));
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (issues) {
+          unsigned char* const stage = stages + (size_t)s * L::STAGE_BYTES;
+          const unsigned sw = tmem + L::MOST_NB + buffer * L::SCALE_COLS, sx = sw + 4 * F::WORDS;
+          const unsigned long long w_scales = scales_desc(stage), x_scales = scales_desc(stage + F::BLOCK_BYTES);
+          const unsigned long long w = codes_desc(stage + F::SCALE_BYTES), x = codes_desc(stage + L::X_AT);
+#pragma unroll
+          for (int j = 0; j < F::WORDS; ++j) {
+            scales_to_tmem<2>(sw + 4 * j, w_scales + j * (512 >> 4));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) scales_to_tmem<2>(sx + 8 * j + 4 * h, x_scales + ((j * 512 + h * F::SCALE_BYTES) >> 4));
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int word = j * F::WORDS / 4;
+            umma<KIND, 2>(tmem, w + 2 * j, x + 2 * j, idesc<KIND, 256>(KIND == MX ? 2 * (j & 1) : 0) | n_bits, sw + 4 * word, sx + 8 * word + shift, kb > 0 || j > 0);
+          }
+          umma_commit_both(&empty[s]);
+          if (kb == KB - 1) umma_commit_both(acc_full);
+        }
+        __syncwarp();
+        buffer ^= 1;
+        if (++s == STAGES) {
+          s = 0;
+          par ^= 1;
+        }
+      }
+    }
+  } else {
+    const int q = warp & 3, first = (warp - 2) / 4 * L::COLS;   // q: the quarter of tensor memory that this warp may read; first: its first column
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    int run = 0;
+    for (int t = first_tile; t < tiles; t += step, ++run) {
+      const Tile at = tile_of(t);
+      const int row = (at.w + (int)rank) * ROWS + q * 32 + lane, col0 = at.x0 + first, cols = min(min(L::COLS, at.cols - first), p.m - col0);   // cols: may be none
+      const float own = KIND == NV && row < p.n ? __ldg(p.w_factors + row) : 1.f;
+      float x_factor[L::COLS / 32];
+      if constexpr (KIND == NV)
+#pragma unroll
+        for (int c = 0; c < L::COLS / 32; ++c) x_factor[c] = 32 * c + lane < cols ? ld_prev(p.x_factors + col0 + 32 * c + lane) : 1.f;
+      if (!__all_sync(0xffffffffu, mbar_wait(acc_full, (unsigned)(run & 1), p.err, failed, 15))) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const unsigned from = tmem + ((unsigned)(q * 32) << 16) + first;
+      float v[L::COLS / 16][16];
+#pragma unroll
+      for (int c = 0; c < L::COLS / 16; ++c)
+        if (16 * c < cols) tmem_ld16(from + 16 * c, v[c]);
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive_at(acc_empty, 0);
+      write_columns<KIND, L::COLS>(p, reinterpret_cast<O*>(p.y) + (size_t)col0 * p.n + row, row < p.n, cols, v, own, x_factor);
+      __syncwarp();
+    }
+  }
+
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (*failed) {
+    // a wait ran out: give copies and products that may still be in flight a bounded time to end
+    const long long t0 = clock64();
+    auto expired = [&] { return clock64() - t0 > WAIT_CYCLES; };
+    if (threadIdx.x == 0) ring_drain(issued_s, STAGES, [&](int s, unsigned parity) { return mbar_try_wait(&full[s], parity); }, expired);
+    if (warp == 1 && rank == 0 && elected()) {   // the thread that issued the products
+      asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&drained_s)) : "memory");
+      while (!mbar_try_wait(&drained_s, 0) && !expired()) {}
+    }
+    __syncthreads();
+  }
+  cluster_sync();   // neither's memory goes before the other is done with it
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::TMEM_COLS) : "memory");
+  }
+}
+
+template <int KIND, int NB, bool SPLIT, typename O> int configured(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], int blocks, int split, bool dependent, cudaStream_t st) {
+  typedef Layout<KIND, NB, SPLIT> L;
+  static bool asked[64] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return DRYFT_ERR_UNSUPPORTED;
+  if (!asked[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(linear_fp4_kernel<KIND, NB, SPLIT, O>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM_BYTES);
+    if (e != cudaSuccess) return (int)e;
+    asked[dev] = true;
+  }
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(L::THREADS);
+  cfg.dynamicSmemBytes = L::SMEM_BYTES;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 0;
+  if (dependent) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (SPLIT) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = split;
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  return 0;
+}
+template <int KIND, int NB, bool SPLIT, typename O> int run(const Params& p, int blocks, int split, bool dependent, cudaStream_t st) {
+  typedef Layout<KIND, NB, SPLIT> L;
+  const long long tiles = ((long long)p.n + ROWS - 1) / ROWS * ((p.m + NB - 1) / NB);
+  if (NB < ROWS && p.m > NB) return DRYFT_ERR_UNSUPPORTED;   // (a block of x is 128 rows: only tiles of as many follow one another)
+  if (tiles * MOST_BLOCKS > 0x7fffffffll || blocks <= 0 || (SPLIT ? blocks != tiles * split : blocks > tiles)) return DRYFT_ERR_UNSUPPORTED;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  const int rc = configured<KIND, NB, SPLIT, O>(cfg, attr, blocks, split, dependent, st);
+  if (rc) return rc;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_fp4_kernel<KIND, NB, SPLIT, O>, p);
+  return e != cudaSuccess ? (int)e : launch_status();
+}
+template <int KIND, typename O> int run_pairs(const Params& p, int nb, int blocks, bool dependent, cudaStream_t st) {
+  typedef PairLayout<KIND> L;
+  if (nb != 128 && nb != 192 && nb != 256) return DRYFT_ERR_UNSUPPORTED;   // (rows of x of a tile begin at whole or half blocks, and lie in two at most)
+  const long long tiles = ((long long)p.n + 2 * ROWS - 1) / (2 * ROWS) * ((p.m + nb - 1) / nb);
+  if (tiles > 0x3fffffffll || blocks <= 0 || blocks % 2 || blocks > 2 * tiles) return DRYFT_ERR_UNSUPPORTED;
+  auto kern = linear_fp4_pair_kernel<KIND, O>;
   static bool asked[64] = {false};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return DRYFT_ERR_UNSUPPORTED;
@@ -308,37 +680,79 @@ template <int KIND, int NB, typename O> int run(const Params& p, bool dependent,
     if (e != cudaSuccess) return (int)e;
     asked[dev] = true;
   }
-  const long long tiles = (long long)((p.n + ROWS - 1) / ROWS) * ((p.m + NB - 1) / NB);
-  if (tiles > 0x7ffffff0ll) return DRYFT_ERR_UNSUPPORTED;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles < sm_count() ? tiles : sm_count()));
-  cfg.blockDim = dim3(THREADS);
+  cudaLaunchAttribute attr[2];
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(L::THREADS);
   cfg.dynamicSmemBytes = L::SMEM_BYTES;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = dependent ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+  cfg.numAttrs = dependent ? 2 : 1;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, nb);
   return e != cudaSuccess ? (int)e : launch_status();
 }
-template <int KIND, typename O> int by_rows(const Params& p, bool dependent, cudaStream_t st) {
-  if (p.m <= 16) return run<KIND, 16, O>(p, dependent, st);
-  if (p.m <= 32) return run<KIND, 32, O>(p, dependent, st);
-  if (p.m <= 64) return run<KIND, 64, O>(p, dependent, st);
-  if (p.m <= 128) return run<KIND, 128, O>(p, dependent, st);
-  return run<KIND, 256, O>(p, dependent, st);
+template <int KIND, bool SPLIT, typename O> int by_rows(const Params& p, int nb, int blocks, int split, bool dependent, cudaStream_t st) {
+  switch (nb) {
+    case 16: return run<KIND, 16, SPLIT, O>(p, blocks, split, dependent, st);
+    case 32: return run<KIND, 32, SPLIT, O>(p, blocks, split, dependent, st);
+    case 64: return run<KIND, 64, SPLIT, O>(p, blocks, split, dependent, st);
+    case 128: return run<KIND, 128, SPLIT, O>(p, blocks, split, dependent, st);
+    case 256: return run<KIND, 256, SPLIT, O>(p, blocks, split, dependent, st);
+  }
+  return DRYFT_ERR_UNSUPPORTED;
+}
+template <int KIND, typename O> int by_split(const Params& p, int nb, int blocks, int split, bool dependent, cudaStream_t st) {
+  if (split == 0) return run_pairs<KIND, O>(p, nb, blocks, dependent, st);
+  return split > 1 ? by_rows<KIND, true, O>(p, nb, blocks, split, dependent, st) : by_rows<KIND, false, O>(p, nb, blocks, split, dependent, st);
+}
+template <int KIND, int NB> int clusters_of(int split) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (configured<KIND, NB, true, bf16>(cfg, attr, split, split, false, nullptr)) return 0;
+  return cudaOccupancyMaxActiveClusters(&n, linear_fp4_kernel<KIND, NB, true, bf16>, &cfg) == cudaSuccess ? n : 0;
 }
 }  // namespace
 
-// y [m, n] = x w^T; x, w: blocks of 128 rows by 256 inputs (fp4.cuh) with factors for each row (NV); y bfloat16 or float32
-DRYFT_API int dryft_linear_fp4(int kind, int out_bf16, const void* x, const void* x_factors, const void* w, const void* w_factors, void* y, int m, int n, int k, int pdl,
-                               int* err, void* stream) {
+extern "C" int dryft_fp4_quantise(int is_bf16, int kind, int silu, const void* x, long long stride, void* held, void* factors, int rows, int k, int pdl, void* stream);
+
+// How many clusters of `split` blocks are resident at a time.
+DRYFT_API int dryft_linear_fp4_clusters(int nb, int split) {
+  if (split < 2 || split > MOST_BLOCKS) return 0;
+  switch (nb) {
+    case 16: return clusters_of<NV, 16>(split);
+    case 32: return clusters_of<NV, 32>(split);
+    case 64: return clusters_of<NV, 64>(split);
+    case 128: return clusters_of<NV, 128>(split);
+    case 256: return clusters_of<NV, 256>(split);
+  }
+  return 0;
+}
+
+// y [m, n] = x w^T; x, w: blocks of 128 rows by 256 inputs (fp4.cuh) with factors for each row (NV); y bfloat16 or float32.  nb: x rows of a tile, 16 to 256 (against 128
+// rows of W).  split: blocks that share a tile's inputs, as a cluster (1: none do, and `blocks` walk the tiles; 0: pairs of
+// blocks walk tiles of 256 rows of W by nb = 128, 192 or 256 of x).
+DRYFT_API int dryft_linear_fp4(int kind, int out_bf16, const void* x, const void* x_factors, const void* w, const void* w_factors, void* y, int m, int n, int k, int nb,
+                               int blocks, int split, int pdl, int* err, void* stream) {
   if (m <= 0 || n <= 0) return 0;
-  if (k <= 0) return DRYFT_ERR_UNSUPPORTED;
+  if (k <= 0 || split < 0 || split > MOST_BLOCKS || split > blocks_of(k)) return DRYFT_ERR_UNSUPPORTED;
   const Params p = {(const unsigned char*)x, (const unsigned char*)w, (const float*)x_factors, (const float*)w_factors, y, err, m, n, blocks_of(k)};
   const cudaStream_t st = (cudaStream_t)stream;
-  if (kind == NV) return out_bf16 ? by_rows<NV, bf16>(p, pdl, st) : by_rows<NV, float>(p, pdl, st);
-  return out_bf16 ? by_rows<MX, bf16>(p, pdl, st) : by_rows<MX, float>(p, pdl, st);
+  if (kind == NV) return out_bf16 ? by_split<NV, bf16>(p, nb, blocks, split, pdl, st) : by_split<NV, float>(p, nb, blocks, split, pdl, st);
+  return out_bf16 ? by_split<MX, bf16>(p, nb, blocks, split, pdl, st) : by_split<MX, float>(p, nb, blocks, split, pdl, st);
+}
+
+// The same of x as it is: `stride` numbers between its rows (silu: of 2 k numbers, as for dryft_fp4_quantise).  scratch: its form in 4 bits, then (NV) its rows' factors, `factors_at` bytes on.  pdl: 1, the rounding is a programmatic
+// dependent of the launch before it; 2, the product is one of the rounding.
+DRYFT_API int dryft_linear_fp4_rows(int kind, int is_bf16, int silu, int out_bf16, const void* x, long long stride, const void* w, const void* w_factors, void* y, int m, int n, int k,
+                                    int nb, int blocks, int split, unsigned char* scratch, long long factors_at, int pdl, int* err, void* stream) {
+  if (m <= 0 || n <= 0) return 0;
+  const int rc = dryft_fp4_quantise(is_bf16, kind, silu, x, stride, scratch, scratch + factors_at, m, k, pdl & 1, stream);
+  if (rc) return rc;
+  return dryft_linear_fp4(kind, out_bf16, scratch, scratch + factors_at, w, w_factors, y, m, n, k, nb, blocks, split, pdl & 2, err, stream);
 }

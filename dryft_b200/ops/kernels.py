@@ -2737,10 +2737,12 @@ def fp4_lib() -> ctypes.CDLL:
     with _lock:
         if _fp4 is None:
             lib = _load(build.build_library("fp4", FP4_SOURCES))
-            lib.dryft_fp4_quantise.argtypes = [_i, _i, _p, _ll, _p, _p, _i, _i, _i, _p]
+            lib.dryft_fp4_quantise.argtypes = [_i, _i, _i, _p, _ll, _p, _p, _i, _i, _i, _p]
             lib.dryft_fp4_expand.argtypes = [_i, _i, _p, _p, _p, _i, _i, _p]
-            lib.dryft_linear_fp4.argtypes = [_i, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p, _p]
-            for name in ("dryft_fp4_quantise", "dryft_fp4_expand", "dryft_linear_fp4"):
+            lib.dryft_linear_fp4.argtypes = [_i, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p]
+            lib.dryft_linear_fp4_rows.argtypes = [_i, _i, _i, _i, _p, _ll, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p, _ll, _i, _p, _p]
+            lib.dryft_linear_fp4_clusters.argtypes = [_i, _i]
+            for name in ("dryft_fp4_quantise", "dryft_fp4_expand", "dryft_linear_fp4", "dryft_linear_fp4_rows", "dryft_linear_fp4_clusters"):
                 getattr(lib, name).restype = _i
             _fp4 = lib
         return _fp4
@@ -2779,7 +2781,7 @@ class Fp4:
             raise KernelError(f"Fp4: no numbers in [{self.n}, {self.k}]")
         wanted = [(self.held, "held", torch.uint8, _fp4_shape(self.n, self.k, self.kind), 16)]
         if self.kind == "nv":
-            wanted.append((self.factors, "factors", torch.float32, (self.n,), 4))
+            wanted.append((self.factors, "factors", torch.float32, (self.n,), 16))
         elif self.factors is not None:
             raise KernelError("Fp4: rows have factors of their own in the kind 'nv' only")
         for t, name, dtype, shape, word in wanted:
@@ -2841,12 +2843,11 @@ def _fp4_rows(x, name: str) -> int:
     return step
 
 
-def _fp4_quantise(x, step: int, kind: str, pdl: bool) -> Fp4:
-    global launch_count
+def _fp4_quantise(x, step: int, kind: str) -> Fp4:
     m, k = x.shape
     held = torch.empty(_fp4_shape(m, k, kind), dtype=torch.uint8, device=x.device)
     factors = torch.empty(m, dtype=torch.float32, device=x.device) if kind == "nv" else None
-    _ok(fp4_lib().dryft_fp4_quantise(x.dtype == torch.bfloat16, FP4_KINDS[kind], x.data_ptr(), step, held.data_ptr(), _ptr(factors), m, k, pdl, _stream()), "fp4_quantise")
+    _ok(fp4_lib().dryft_fp4_quantise(x.dtype == torch.bfloat16, FP4_KINDS[kind], False, x.data_ptr(), step, held.data_ptr(), _ptr(factors), m, k, False, _stream()), "fp4_quantise")
     return Fp4(held, factors, m, k, kind)
 
 
@@ -2858,7 +2859,7 @@ def fp4_quantise(x, kind: str) -> Fp4:
     step = _fp4_rows(x, "x")
     if x.shape[0] == 0 or x.shape[1] == 0:
         raise KernelError(f"fp4_quantise: no numbers in {tuple(x.shape)}")
-    return _fp4_quantise(x, step, kind, False)
+    return _fp4_quantise(x, step, kind)
 
 
 def fp4_expand(q: Fp4, out=None, out_dtype=torch.bfloat16):
@@ -2873,6 +2874,29 @@ def fp4_expand(q: Fp4, out=None, out_dtype=torch.bfloat16):
         _on_current(out, "out")
     _ok(fp4_lib().dryft_fp4_expand(_act(out, "out"), FP4_KINDS[q.kind], q.held.data_ptr(), _ptr(q.factors), out.data_ptr(), q.n, q.k, _stream()), "fp4_expand")
     return out
+
+
+@functools.lru_cache(maxsize=16)
+def _sm_count(device: int) -> int:
+    return torch.cuda.get_device_properties(device).multi_processor_count
+
+
+def _fp4_tiles(nb: int, m: int, n: int) -> int:
+    return -(-n // 128) * -(-m // nb)
+
+
+@functools.lru_cache(maxsize=64)
+def _fp4_clusters(device: int, nb: int, split: int) -> int:
+    """How many clusters of ``split`` blocks the device holds at a time."""
+    with torch.cuda.device(device):
+        return int(fp4_lib().dryft_linear_fp4_clusters(nb, split))
+
+
+@functools.lru_cache(maxsize=4096)
+def linear_fp4_plan(m: int, n: int, k: int, device: int) -> Tuple[int, int, int]:
+    """How a product is run: x rows of a tile (of 128 outputs), blocks, and how many of them share a tile's inputs."""
+    nb = next((b for b in (16, 32, 64, 128) if m <= b), 256)
+    return nb, min(_fp4_tiles(nb, m, n), _sm_count(device)), 1
 
 
 def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = False, out_dtype=None):
@@ -2908,15 +2932,20 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
     out_bf16 = _act(out, "out")
     if m == 0:
         return out
-    overlap = bool(pdl)
-    if not given:
-        if silu:
-            act = torch.empty((m, w.k), dtype=x.dtype, device=x.device)
-            silu_mul(x, act)
-            x, step = act, w.k
-        x, overlap = _fp4_quantise(x, step, w.kind, bool(pdl)), pdl is not False
-    _ok(fp4_lib().dryft_linear_fp4(FP4_KINDS[w.kind], out_bf16, x.held.data_ptr(), _ptr(x.factors), w.held.data_ptr(), _ptr(w.factors), out.data_ptr(), m, w.n, w.k, overlap,
-                                   error_flag(w.device).data_ptr(), _stream()), "linear_fp4")
+    nb, blocks, split = linear_fp4_plan(m, w.n, w.k, out.get_device())
+    code, lib, err = FP4_KINDS[w.kind], fp4_lib(), error_flag(w.device).data_ptr()
+    if given:
+        _ok(lib.dryft_linear_fp4(code, out_bf16, x.held.data_ptr(), _ptr(x.factors), w.held.data_ptr(), _ptr(w.factors), out.data_ptr(), m, w.n, w.k, nb, blocks, split,
+                                 bool(pdl), err, _stream()), "linear_fp4")
+        return out
+    if silu and x.dtype == torch.float32:
+        act = torch.empty((m, w.k), dtype=x.dtype, device=x.device)
+        silu_mul(x.contiguous(), act)
+        x, step, silu = act, w.k, False
+    rows, wide, size = _fp4_shape(m, w.k, w.kind)
+    scratch = torch.empty(rows * wide * size + 4 * m, dtype=torch.uint8, device=w.device)
+    _ok(lib.dryft_linear_fp4_rows(code, x.dtype == torch.bfloat16, silu, out_bf16, x.data_ptr(), step, w.held.data_ptr(), _ptr(w.factors), out.data_ptr(), m, w.n, w.k, nb, blocks,
+                                  split, scratch.data_ptr(), rows * wide * size, _overlap(pdl), err, _stream()), "linear_fp4", 2)
     return out
 
 
