@@ -39,6 +39,118 @@ __device__ __forceinline__ float scale_value(unsigned byte, bool nv) {
   }
   return byte == MX_NAN ? __uint_as_float(0x7fffffffu) : byte == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);   // (2^-127 has no exponent bits)
 }
+constexpr int UNIT = 16, BLOCK_UNITS = INPUTS / UNIT;   // numbers that a lane has at a time; units of a block's row
+// Sixteen numbers as they lie in memory.
+template <typename T> struct Raw { unsigned w[UNIT * sizeof(T) / 4]; };
+__device__ __forceinline__ float number(const Raw<__nv_bfloat16>& r, int i) { return __uint_as_float(i & 1 ? r.w[i / 2] & 0xffff0000u : r.w[i / 2] << 16); }
+__device__ __forceinline__ float number(const Raw<float>& r, int i) { return __uint_as_float(r.w[i]); }
+
+// From column c on; zeros behind column k.  Through L2 (`ld_prev`): the launch before this one may have written them.
+template <typename T> __device__ __forceinline__ Raw<T> load(const T* row, int c, int k, bool words) {
+  Raw<T> r;
+  constexpr int N = UNIT * sizeof(T) / 16;
+  if (words && c + UNIT <= k) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint4 a = ld_prev(reinterpret_cast<const uint4*>(row + c) + i);
+      r.w[4 * i] = a.x;
+      r.w[4 * i + 1] = a.y;
+      r.w[4 * i + 2] = a.z;
+      r.w[4 * i + 3] = a.w;
+    }
+    return r;
+  }
+#pragma unroll
+  for (int i = 0; i < 4 * N; ++i) r.w[i] = 0;
+#pragma unroll
+  for (int i = 0; i < UNIT; ++i)
+    if (c + i < k) {
+      if (sizeof(T) == 4) r.w[i] = __ldcg(reinterpret_cast<const unsigned*>(row) + c + i);
+      else r.w[i / 2] |= (unsigned)__ldcg(reinterpret_cast<const unsigned short*>(row) + c + i) << (i & 1) * 16;
+    }
+  return r;
+}
+// SILU: the row holds gate numbers, then as many others: silu(gate) rounded, times the other, rounded (the points of `silu_mul`).
+template <typename T, bool SILU> __device__ __forceinline__ Raw<T> load_unit(const T* row, int c, int k, bool words) {
+  Raw<T> r = load(row, c, k, words);
+  if constexpr (SILU) {
+    const Raw<T> up = load(row + k, c, k, words);
+#pragma unroll
+    for (int i = 0; i < UNIT / 2; ++i) {
+      float v[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float g = number(r, 2 * i + e);
+        v[e] = rnd<__nv_bfloat16>(__fdividef(g, 1.f + __expf(-g))) * number(up, 2 * i + e);   // (a few 32-bit ulp: far inside the rounding to bfloat16)
+      }
+      const __nv_bfloat162 two = __floats2bfloat162_rn(v[0], v[1]);
+      r.w[i] = *reinterpret_cast<const unsigned*>(&two);
+    }
+  }
+  return r;
+}
+
+struct Size { unsigned most; bool bad; };   // the bits of the largest finite magnitude as a 32-bit number (bits of magnitudes are in their order); whether one is not finite
+template <typename T> __device__ __forceinline__ Size size_of(const Raw<T>& r) {
+  unsigned most = 0;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < UNIT / 2; ++i) most = __vmaxu2(most, r.w[i] & 0x7fff7fffu);
+    most = max(most & 0xffff0000u, most << 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < UNIT; ++i) most = max(most, r.w[i] & 0x7fffffffu);
+  }
+  if (most < 0x7f800000u) return {most, false};
+  most = 0;
+#pragma unroll
+  for (int i = 0; i < UNIT; ++i) {
+    const unsigned a = __float_as_uint(number(r, i)) & 0x7fffffffu;
+    if (a < 0x7f800000u) most = max(most, a);
+  }
+  return {most, true};
+}
+__device__ __forceinline__ float row_factor(unsigned most) { return fmaxf(__fdiv_rn(__uint_as_float(most), 2688.f), __uint_as_float((127u - 112u) << 23)); }
+// codes of eight numbers times r, the first in the lowest four bits
+template <typename T> __device__ __forceinline__ unsigned codes8(const Raw<T>& x, int first, float r) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = number(x, first + i) * r;
+  unsigned w;
+  asm("{ .reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3}; }"
+      : "=r"(w) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return w;
+}
+
+// A unit's codes, and the word of scales that it begins (where it begins one: NV every fourth unit, MX every eighth).  Neighbouring lanes have neighbouring units; all 32 take part.
+// factor, u: of the row (NV).
+template <int KIND, typename T> __device__ __forceinline__ uint2 round_unit(const Raw<T>& r, float factor, float u, unsigned& word) {
+  Size s = size_of(r);
+  unsigned byte;
+  float by;
+  if (KIND == NV) {
+    unsigned short two;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(0.f), "f"(__uint_as_float(s.most) * u));
+    byte = two & 0xff;
+    by = byte == 0 ? 0.f : __frcp_rn(scale_value(byte, true) * factor);
+    if (s.bad) byte = NV_NAN;
+    word = byte | __shfl_down_sync(0xffffffffu, byte, 1) << 8;
+    word |= __shfl_down_sync(0xffffffffu, word, 2) << 16;
+  } else {
+    s.most = max(s.most, __shfl_xor_sync(0xffffffffu, s.most, 1));
+    s.bad |= __shfl_xor_sync(0xffffffffu, (int)s.bad, 1) != 0;
+    byte = max((int)(s.most >> 23) - 2, 0);
+    by = __uint_as_float((254u - byte) << 23);   // 1 / s: 2^127 at the most
+    if (s.bad) byte = MX_NAN;
+    word = byte | __shfl_down_sync(0xffffffffu, byte, 2) << 8;
+    word |= __shfl_down_sync(0xffffffffu, word, 4) << 16;
+  }
+  return s.bad ? make_uint2(0x22222222u, 0x22222222u) : make_uint2(codes8(r, 0, by), codes8(r, 8, by));
+}
+
 // 32 bytes: a whole sector a lane
 __device__ __forceinline__ void st_words8(void* to, const unsigned* w) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"

@@ -107,26 +107,35 @@ __device__ __forceinline__ void tmem_ld16(unsigned taddr, float (&v)[16]) {
 }
 
 struct Params {
-  const unsigned char *x, *w;          // blocks (fp4.cuh)
+  const unsigned char *x, *w;          // blocks (fp4.cuh); x: or rows as they are (below)
   const float *x_factors, *w_factors;  // NV
   void* y;
   int* err;
   int m, n, blocks;   // blocks: of 256 inputs
+  // of x as it is: numbers of a row, numbers between rows, whether 16-byte words can be read
+  int k;
+  long long x_stride;
+  bool x_words;
 };
 
+constexpr int FUSED_ROWS = 16, FUSED_BLOCKS = 12;   // rows, and blocks of 256 inputs, that a block rounds for itself at most
+// What x is: held in 4 bits, or bfloat16 rows that every block rounds for itself (SILU: of gate numbers and as many others).
+enum Source { HELD = 0, BF16 = 1, SILU = 2 };
+
 // SPLIT: a tile's inputs are shared out among a cluster's blocks.
-template <int KIND, int NB, bool SPLIT> struct Layout {
+template <int KIND, int NB, bool SPLIT, int SRC> struct Layout {
   typedef Format<KIND> F;
+  static constexpr bool FUSED = SRC != HELD;
   // warps that read sums: four take a quarter of the rows each, and PARTS fours a part of the columns, so that each scheduler has several to hide their latencies
-  static constexpr int PARTS = NB <= 16 ? 1 : NB <= 32 ? 2 : 4, READERS = 4 * PARTS, THREADS = (2 + READERS) * 32;
-  static constexpr int BB = NB > ROWS ? 2 : 1;                                   // blocks of the N side in a stage
-  static constexpr int B_CODES = NB * (INPUTS / 2), B_BYTES = BB * F::SCALE_BYTES + B_CODES, STAGE_BYTES = F::BLOCK_BYTES + B_BYTES;   // multiples of 1024
-  static constexpr int RESIDENT = NB > ROWS ? 1 : 2;                                 // blocks of a multiprocessor
-  static constexpr int ROOM = (RESIDENT == 2 ? 110 : 225) * 1024 / STAGE_BYTES, STAGES = ROOM < 12 ? ROOM : 12;
+  static constexpr int PARTS = NB <= 16 ? 1 : NB <= 32 ? 2 : 4, READERS = 4 * PARTS;
+  static constexpr int ROUNDERS = FUSED ? READERS + 4 : 0, THREADS = (2 + (FUSED ? ROUNDERS : READERS)) * 32;   // warps that round x, the readers among them
+  static constexpr int X_BYTES = F::SCALE_BYTES + NB * (INPUTS / 2), STAGE_BYTES = F::BLOCK_BYTES + (FUSED ? 0 : X_BYTES);   // W's block, as much of x's; multiples of 1024
+  static constexpr int X_BLOCKS = FUSED ? FUSED_BLOCKS : 0;                                  // of x, which stay for all tiles
+  static constexpr int RESIDENT = 2, STAGES = (110 * 1024 - X_BLOCKS * X_BYTES) / STAGE_BYTES;   // RESIDENT: blocks of a multiprocessor
   // tensor memory: sums of ACCS tiles, then the scales of two stages
-  static constexpr int ACCS = SPLIT || NB >= 128 ? 1 : 2, SCALE_COLS = 4 * F::WORDS * (1 + BB), NEED_COLS = ACCS * NB + 2 * SCALE_COLS;
+  static constexpr int ACCS = SPLIT || NB >= 128 ? 1 : 2, SCALE_COLS = 8 * F::WORDS, NEED_COLS = ACCS * NB + 2 * SCALE_COLS;
   static constexpr int TMEM_COLS = NEED_COLS <= 128 ? 128 : NEED_COLS <= 256 ? 256 : 512;
-  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + 8 * (2 * STAGES + 4) + 16;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + X_BLOCKS * X_BYTES + 8 * (2 * STAGES + 5) + 16;
   static_assert(RESIDENT * TMEM_COLS <= 512 && RESIDENT * (SMEM_BYTES + 2048) <= 228 * 1024 && STAGES >= 3, "of a block");
   static_assert(!SPLIT || (NB + 7 * 4) * ROWS * 4 <= STAGES * STAGE_BYTES, "sums fit where the stages were");
 };
@@ -166,20 +175,93 @@ __device__ __forceinline__ void write_columns(const Params& p, O* to, bool there
   }
 }
 
-template <int KIND, int NB, bool SPLIT, typename O>
-__global__ void __launch_bounds__(Layout<KIND, NB, SPLIT>::THREADS, Layout<KIND, NB, SPLIT>::RESIDENT) linear_fp4_kernel(const Params p) {
-  typedef Layout<KIND, NB, SPLIT> L;
+// The rounders' part (FUSED): the rows' inputs that this block multiplies, of blocks k0 to k1, into shared memory as the products want them.  NV wants the largest number of whole
+// rows.  A thread has AHEAD units on their way at a time; its first ones stay in registers between looking and rounding, more are read again.
+template <typename L, int KIND, int SRC>
+__device__ __forceinline__ void round_x(const Params& p, int k0, int k1, unsigned char* xs, unsigned* most_s, unsigned long long* x_full) {
   typedef typename L::F F;
-  constexpr int STAGES = L::STAGES, BB = L::BB, READ_THREADS = L::READERS * 32;
+  constexpr int THREADS = L::ROUNDERS * 32, AHEAD = 4;
+  const int id = threadIdx.x - 64, lane = threadIdx.x & 31, own = (k1 - k0) * BLOCK_UNITS, all = p.m * own, rest = p.blocks * BLOCK_UNITS - own, all_rest = p.m * rest;
+  const bf16* const x = reinterpret_cast<const bf16*>(p.x);
+  // i / n, for i + 1/2 and n far below 2^23
+  auto over = [](int i, float by) { return (int)(((float)i + 0.5f) * by); };
+  const float by_own = 1.f / (float)own, by_rest = 1.f / (float)max(rest, 1);
+  auto load = [&](int i, int row) { return load_unit<bf16, SRC == SILU>(x + row * p.x_stride, (k0 * BLOCK_UNITS + i - row * own) * UNIT, p.k, p.x_words); };
+  auto take = [&](Raw<bf16> (&r)[AHEAD], int base) {
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (base + j * THREADS + id < all) r[j] = load(base + j * THREADS + id, over(base + j * THREADS + id, by_own));
+  };
+  Raw<bf16> r[AHEAD] = {};
+  take(r, 0);
+  if (KIND == NV) {
+    auto look = [&](const Raw<bf16>& r, bool there, int row) {   // sixteen neighbouring lanes have one row's
+      unsigned most = there ? size_of(r).most : 0u;
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+      if (there && lane % BLOCK_UNITS == 0) atomicMax(&most_s[row], most);
+    };
+    auto look_all = [&](const Raw<bf16> (&r)[AHEAD], int base, int end, float by) {
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+        if (base + j * THREADS < end) look(r[j], base + j * THREADS + id < end, over(base + j * THREADS + id, by));
+    };
+    for (int base = 0; base < all_rest; base += AHEAD * THREADS) {   // other blocks' inputs
+      Raw<bf16> o[AHEAD] = {};
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const int i = base + j * THREADS + id, row = over(i, by_rest), c = i - row * rest;
+        if (i < all_rest) o[j] = load_unit<bf16, SRC == SILU>(x + row * p.x_stride, (c < k0 * BLOCK_UNITS ? c : c + own) * UNIT, p.k, p.x_words);
+      }
+      look_all(o, base, all_rest, by_rest);
+    }
+    look_all(r, 0, all, by_own);
+    for (int base = AHEAD * THREADS; base < all; base += AHEAD * THREADS) {
+      Raw<bf16> o[AHEAD] = {};
+      take(o, base);
+      look_all(o, base, all, by_own);
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");   // the rounders' own: none of them waits for anything else in front of it
+  }
+  for (int base = 0; base < all; base += AHEAD * THREADS) {
+    if (base > 0) take(r, base);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (base + j * THREADS >= all) break;
+      const int i = base + j * THREADS + id, row = over(min(i, all - 1), by_own), c = i - row * own, unit = c % BLOCK_UNITS;
+      const float factor = KIND == NV ? row_factor(most_s[row]) : 1.f;
+      unsigned word;
+      const uint2 codes = round_unit<KIND>(r[j], factor, KIND == NV ? __frcp_rn(6.f * factor) : 1.f, word);
+      if (i < all) {
+        unsigned char* const block = xs + (size_t)(c / BLOCK_UNITS) * L::X_BYTES;
+        constexpr int PER_WORD = F::WORD_INPUTS / UNIT;
+        *reinterpret_cast<uint2*>(block + F::SCALE_BYTES + code_at(row, unit)) = codes;
+        if (unit % PER_WORD == 0) *reinterpret_cast<unsigned*>(block + scale_word_at(row, unit / PER_WORD)) = word;
+      }
+    }
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // what was written is read by the tensor cores
+  mbar_arrive(x_full);
+}
+
+template <int KIND, int NB, bool SPLIT, int SRC, typename O>
+__global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<KIND, NB, SPLIT, SRC>::RESIDENT) linear_fp4_kernel(const Params p) {
+  typedef Layout<KIND, NB, SPLIT, SRC> L;
+  typedef typename L::F F;
+  constexpr int STAGES = L::STAGES, READ_THREADS = L::READERS * 32;
+  constexpr bool FUSED = L::FUSED;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* const stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  unsigned long long* const full = reinterpret_cast<unsigned long long*>(stages + STAGES * L::STAGE_BYTES);   // [S] copies -> products
+  unsigned char* const xs = stages + STAGES * L::STAGE_BYTES;                                                  // (FUSED) x's blocks
+  unsigned long long* const full = reinterpret_cast<unsigned long long*>(xs + L::X_BLOCKS * L::X_BYTES);       // [S] copies -> products
   unsigned long long* const empty = full + STAGES;                                                             // [S] products -> copies
   unsigned long long* const acc_full = empty + STAGES;                                                         // [2] a tile's sums -> their readers
   unsigned long long* const acc_empty = acc_full + 2;                                                          // [2] read (by every reader) -> products
-  unsigned* const tmem_slot = reinterpret_cast<unsigned*>(acc_empty + 2);
+  unsigned long long* const x_full = acc_empty + 2;                                                            // (FUSED) x is rounded (by every rounder) -> products
+  unsigned* const tmem_slot = reinterpret_cast<unsigned*>(x_full + 1);
   __shared__ int failed_s, issued_s;
   __shared__ unsigned long long drained_s;
+  __shared__ unsigned most_s[FUSED_ROWS];   // (FUSED, NV) bits of the rows' largest magnitudes
   volatile int* const failed = &failed_s;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, KB = p.blocks;
@@ -202,8 +284,10 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT>::THREADS, Layout<KIND,
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], READ_THREADS);
     }
+    if (FUSED) mbar_init(x_full, L::ROUNDERS * 32);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (FUSED && threadIdx.x < FUSED_ROWS) most_s[threadIdx.x] = 0;
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(L::TMEM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -216,39 +300,30 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT>::THREADS, Layout<KIND,
 
   if (warp == 0) {
     const bool issues = elected();
+    auto w_of = [&](int t) { return p.w + ((size_t)(t / x_tiles) * KB + k0) * F::BLOCK_BYTES; };
+    auto x_bytes_of = [&](int t) { return FUSED ? 0 : F::SCALE_BYTES + columns(p.m - t % x_tiles * NB) * (INPUTS / 2); };   // scales, and codes of the rows that there are
+    auto load_w = [&](int t, int kb, int s) {
+      mbar_expect_tx(&full[s], F::BLOCK_BYTES + x_bytes_of(t));
+      bulk_load(stages + (size_t)s * L::STAGE_BYTES, w_of(t) + (size_t)(kb - k0) * F::BLOCK_BYTES, F::BLOCK_BYTES, &full[s]);
+    };
+    // W depends on no launch that may still be running: as much of it as fits is asked for at once
+    const int early = first_tile < tiles ? min(STAGES, k1 - k0) : 0;
+    if (issues)
+      for (int s = 0; s < early; ++s) load_w(first_tile, k0 + s, s);
+    __syncwarp();
+    if (!FUSED) asm volatile("griddepcontrol.wait;" ::: "memory");
     int i = 0, s = 0;
     unsigned par = 1;   // (the first turn finds every stage free)
-    bool ok = true, waited = false;
+    bool ok = true;
     for (int t = first_tile; ok && t < tiles; t += step) {
-      const unsigned char* w = p.w + ((size_t)(t / x_tiles) * KB + k0) * F::BLOCK_BYTES;
-      const unsigned char* x = p.x + ((size_t)(t % x_tiles) * BB * KB + k0) * F::BLOCK_BYTES;
-      const int left = p.m - t % x_tiles * NB;
-      const unsigned x_codes = columns(left) * (INPUTS / 2);                        // bytes of the rows that there are
-      for (int kb = k0; kb < k1; ++kb, ++i, w += F::BLOCK_BYTES, x += F::BLOCK_BYTES) {
+      const unsigned char* x = p.x + ((size_t)(t % x_tiles) * KB + k0) * F::BLOCK_BYTES;
+      const unsigned x_bytes = x_bytes_of(t);
+      for (int kb = k0; kb < k1; ++kb, ++i, x += F::BLOCK_BYTES) {
         ok = i < STAGES || __all_sync(0xffffffffu, mbar_wait(&empty[s], par, p.err, failed, 1));
         if (!ok) break;
-        unsigned char* const to = stages + (size_t)s * L::STAGE_BYTES;
         if (issues) {
-          mbar_expect_tx(&full[s], F::BLOCK_BYTES + (BB == 2 && left > ROWS ? 2 : 1) * F::SCALE_BYTES + x_codes);
-          bulk_load(to, w, F::BLOCK_BYTES, &full[s]);   // W depends on no launch that may still be running
-        }
-        if (!waited) {
-          asm volatile("griddepcontrol.wait;" ::: "memory");
-          waited = true;
-        }
-        if (issues) {
-          if (BB == 1) bulk_load(to + F::BLOCK_BYTES, x, F::SCALE_BYTES + x_codes, &full[s]);
-          else {
-            unsigned char* const scales = to + F::BLOCK_BYTES;
-            unsigned char* const codes = scales + BB * F::SCALE_BYTES;
-            bulk_load(scales, x, F::SCALE_BYTES, &full[s]);
-            bulk_load(codes, x + F::SCALE_BYTES, min(x_codes, (unsigned)CODE_BYTES), &full[s]);
-            if (left > ROWS) {
-              const unsigned char* const next = x + (size_t)KB * F::BLOCK_BYTES;
-              bulk_load(scales + F::SCALE_BYTES, next, F::SCALE_BYTES, &full[s]);
-              bulk_load(codes + CODE_BYTES, next + F::SCALE_BYTES, x_codes - CODE_BYTES, &full[s]);
-            }
-          }
+          if (i >= early) load_w(t, kb, s);
+          if (!FUSED) bulk_load(stages + (size_t)s * L::STAGE_BYTES + F::BLOCK_BYTES, x, x_bytes, &full[s]);
         }
         __syncwarp();
         if (++s == STAGES) {
@@ -262,7 +337,7 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT>::THREADS, Layout<KIND,
     const bool issues = elected();
     int s = 0, run = 0;
     unsigned par = 0, buffer = 0;
-    bool ok = true;
+    bool ok = !FUSED || __all_sync(0xffffffffu, mbar_wait(x_full, 0, p.err, failed, 3));
     for (int t = first_tile; ok && t < tiles; t += step, ++run) {
       const int acc = run % L::ACCS;
       const unsigned d = tmem + acc * NB, n_bits = (unsigned)(columns(p.m - t % x_tiles * NB) >> 3) << 17;
@@ -273,19 +348,19 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT>::THREADS, Layout<KIND,
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (issues) {
           unsigned char* const at = stages + (size_t)s * L::STAGE_BYTES;
-          const unsigned sa = tmem + L::ACCS * NB + buffer * L::SCALE_COLS, sb = sa + 4 * F::WORDS;
-          const unsigned long long a_scales = scales_desc(at), b_scales = scales_desc(at + F::BLOCK_BYTES);
-          const unsigned long long a = codes_desc(at + F::SCALE_BYTES), b = codes_desc(at + F::BLOCK_BYTES + BB * F::SCALE_BYTES);
+          const unsigned sw = tmem + L::ACCS * NB + buffer * L::SCALE_COLS, sx = sw + 4 * F::WORDS;
+          const unsigned char* const x_at = FUSED ? xs + (size_t)(kb - k0) * L::X_BYTES : at + F::BLOCK_BYTES;
+          const unsigned long long w_scales = scales_desc(at), x_scales = scales_desc(x_at);
+          const unsigned long long w = codes_desc(at + F::SCALE_BYTES), x = codes_desc(x_at + F::SCALE_BYTES);
 #pragma unroll
           for (int j = 0; j < F::WORDS; ++j) {
-            scales_to_tmem(sa + 4 * j, a_scales + j * (512 >> 4));
-#pragma unroll
-            for (int h = 0; h < BB; ++h) scales_to_tmem(sb + 4 * BB * j + 4 * h, b_scales + ((j * 512 + h * F::SCALE_BYTES) >> 4));
+            scales_to_tmem(sw + 4 * j, w_scales + j * (512 >> 4));
+            scales_to_tmem(sx + 4 * j, x_scales + j * (512 >> 4));
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int word = j * F::WORDS / 4;
-            umma<KIND>(d, a + 2 * j, b + 2 * j, idesc<KIND>(KIND == MX ? 2 * (j & 1) : 0) | n_bits, sa + 4 * word, sb + 4 * BB * word, kb > k0 || j > 0);
+            umma<KIND>(d, w + 2 * j, x + 2 * j, idesc<KIND>(KIND == MX ? 2 * (j & 1) : 0) | n_bits, sw + 4 * word, sx + 4 * word, kb > k0 || j > 0);
           }
           umma_commit(&empty[s]);
           if (kb == k1 - 1) umma_commit(&acc_full[acc]);
@@ -303,14 +378,16 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT>::THREADS, Layout<KIND,
     constexpr int COLS = NB / L::PARTS;                  // columns that this warp reads, from `first` on
     const int first = (warp - 2) / 4 * COLS;
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    if constexpr (FUSED) round_x<L, KIND, SRC>(p, k0, k1, xs, most_s, x_full);
     int run = 0;
-    for (int t = first_tile; t < tiles; t += step, ++run) {
+    for (int t = warp < 2 + L::READERS ? first_tile : tiles; t < tiles; t += step, ++run) {
       const int acc = run % L::ACCS, row = t / x_tiles * ROWS + q * 32 + lane, col0 = t % x_tiles * NB + first, cols = min(COLS, p.m - col0);   // cols: may be none
       const float own = KIND == NV && row < p.n ? __ldg(p.w_factors + row) : 1.f;
       float x_factor[(COLS + 31) / 32];   // of the columns, a lane each (asked for here, where there is time)
       if constexpr (KIND == NV)
 #pragma unroll
-        for (int c = 0; c < (COLS + 31) / 32; ++c) x_factor[c] = 32 * c + lane < cols ? ld_prev(p.x_factors + col0 + 32 * c + lane) : 1.f;
+        for (int c = 0; c < (COLS + 31) / 32; ++c)
+          x_factor[c] = 32 * c + lane >= cols ? 1.f : FUSED ? row_factor(most_s[col0 + 32 * c + lane]) : ld_prev(p.x_factors + col0 + 32 * c + lane);
       if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[acc], (unsigned)(run / L::ACCS & 1), p.err, failed, 5))) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if constexpr (SPLIT) break;   // (below)
@@ -334,15 +411,17 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT>::THREADS, Layout<KIND,
     const unsigned per_block = (GROUPS + size - 1) / size;
     const int q = warp & 3, part = (warp - 2) / 4;
     const int row = first_tile / x_tiles * ROWS + q * 32 + lane, col0 = first_tile % x_tiles * NB, cols = min(NB, p.m - col0);
-    const float own = KIND == NV && warp >= 2 && row < p.n ? __ldg(p.w_factors + row) : 1.f;
+    const bool reads = warp >= 2 && warp < 2 + L::READERS;
+    const float own = KIND == NV && reads && row < p.n ? __ldg(p.w_factors + row) : 1.f;
     float x_factor[(NB + 31) / 32];
     if constexpr (KIND == NV)
 #pragma unroll
-      for (int c = 0; c < (NB + 31) / 32; ++c) x_factor[c] = warp >= 2 && 32 * c + lane < cols ? ld_prev(p.x_factors + col0 + 32 * c + lane) : 1.f;
+      for (int c = 0; c < (NB + 31) / 32; ++c)
+        x_factor[c] = !reads || 32 * c + lane >= cols ? 1.f : FUSED ? row_factor(most_s[col0 + 32 * c + lane]) : ld_prev(p.x_factors + col0 + 32 * c + lane);
     auto place = [&](unsigned block, unsigned group) { return (unsigned)(((block * per_block + group) * GROUP / 4 * ROWS + q * 32 + lane) * 16); };
     __syncwarp();
     cluster_sync();   // every block's products have ended, so its stages are free
-    if (warp >= 2) {
+    if (reads) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const unsigned from = tmem + ((unsigned)(q * 32) << 16);
 #pragma unroll 1
@@ -359,7 +438,7 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT>::THREADS, Layout<KIND,
     }
     __syncwarp();
     cluster_sync();
-    if (warp >= 2) {
+    if (reads) {
 #pragma unroll 1
       for (unsigned i = part; (rank + size * i) * GROUP < cols; i += L::PARTS) {
         const int c = (rank + size * i) * GROUP;
@@ -424,7 +503,7 @@ template <int KIND> struct PairLayout {
   static_assert(MOST_NB + 2 * SCALE_COLS <= TMEM_COLS && SMEM_BYTES <= 227 * 1024 && STAGE_BYTES % 1024 == 0, "of a block");
 };
 __device__ __forceinline__ void mbar_arrive_at(void* bar, unsigned rank) {   // of a block of the cluster
-  asm volatile("{ .reg .u32 a; mapa.shared::cluster.u32 a, %0, %1; mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a]; }" ::"r"(smem_u32(bar)), "r"(rank) : "memory");
+  asm volatile("{ .reg .u32 a; mapa.shared::cluster.u32 a, %0, %1; mbarrier.arrive.shared::cluster.b64 _, [a]; }" ::"r"(smem_u32(bar)), "r"(rank) : "memory");
 }
 __device__ __forceinline__ void umma_commit_both(void* bar) {   // in both blocks
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((unsigned short)3) : "memory");
@@ -486,36 +565,49 @@ template <int KIND, typename O> __global__ void __launch_bounds__(PairLayout<KIN
 
   if (warp == 0) {
     const bool issues = elected();
+    // of the two blocks of x that a tile's rows are in: rows from..to are this block's half
+    struct Half { int from, to; unsigned head, tail; bool second; };   // bytes in either; whether the tile has rows in the second
+    auto half_of = [&](const Tile& at) {
+      Half h;
+      h.from = at.x0 % ROWS + (int)rank * (at.cols / 2);
+      h.to = h.from + at.cols / 2;
+      h.head = h.from < ROWS ? (min(h.to, ROWS) - h.from) * (INPUTS / 2) : 0;
+      h.tail = h.to > ROWS ? (h.to - max(h.from, ROWS)) * (INPUTS / 2) : 0;
+      h.second = at.x0 % ROWS + at.cols > ROWS;
+      return h;
+    };
+    auto load_w = [&](const Tile& at, const Half& h, int kb, int s) {
+      mbar_expect_tx(&full[s], F::BLOCK_BYTES + (h.second ? 2 : 1) * F::SCALE_BYTES + h.head + h.tail);
+      // (an odd number of blocks of W: the last one again, for rows that are nobody's)
+      bulk_load(stages + (size_t)s * L::STAGE_BYTES, p.w + ((size_t)min(at.w + (int)rank, w_blocks - 1) * KB + kb) * F::BLOCK_BYTES, F::BLOCK_BYTES, &full[s]);
+    };
+    // W depends on no launch that may still be running: as much of it as fits is asked for at once
+    const int early = first_tile < tiles ? min(STAGES, KB) : 0;
+    if (issues && early) {
+      const Tile at = tile_of(first_tile);
+      const Half h = half_of(at);
+      for (int s = 0; s < early; ++s) load_w(at, h, s, s);
+    }
+    __syncwarp();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     int i = 0, s = 0;
     unsigned par = 1;   // (the first turn finds every stage free)
-    bool ok = true, waited = false;
+    bool ok = true;
     for (int t = first_tile; ok && t < tiles; t += step) {
       const Tile at = tile_of(t);
-      // (an odd number of blocks of W: the last one again, for rows that are nobody's)
-      const unsigned char* w = p.w + (size_t)min(at.w + (int)rank, w_blocks - 1) * KB * F::BLOCK_BYTES;
+      const Half h = half_of(at);
       const unsigned char* x = p.x + (size_t)(at.x0 / ROWS) * KB * F::BLOCK_BYTES;
-      // of the two blocks of x that the tile's rows are in: rows from..to are this block's half
-      const int off = at.x0 % ROWS, from = off + (int)rank * (at.cols / 2), to = from + at.cols / 2;
-      const unsigned head = from < ROWS ? (min(to, ROWS) - from) * (INPUTS / 2) : 0, tail = to > ROWS ? (to - max(from, ROWS)) * (INPUTS / 2) : 0;   // bytes in either
-      const bool second = off + at.cols > ROWS;
-      for (int kb = 0; kb < KB; ++kb, ++i, w += F::BLOCK_BYTES, x += F::BLOCK_BYTES) {
+      for (int kb = 0; kb < KB; ++kb, ++i, x += F::BLOCK_BYTES) {
         ok = i < STAGES || __all_sync(0xffffffffu, mbar_wait(&empty[s], par, p.err, failed, 11));
         if (!ok) break;
-        unsigned char* const stage = stages + (size_t)s * L::STAGE_BYTES;
         if (issues) {
-          mbar_expect_tx(&full[s], F::BLOCK_BYTES + (second ? 2 : 1) * F::SCALE_BYTES + head + tail);
-          bulk_load(stage, w, F::BLOCK_BYTES, &full[s]);   // W depends on no launch that may still be running
-        }
-        if (!waited) {
-          asm volatile("griddepcontrol.wait;" ::: "memory");
-          waited = true;
-        }
-        if (issues) {
+          unsigned char* const stage = stages + (size_t)s * L::STAGE_BYTES;
           const unsigned char* const next = x + (size_t)KB * F::BLOCK_BYTES;
+          if (i >= early) load_w(at, h, kb, s);
           bulk_load(stage + F::BLOCK_BYTES, x, F::SCALE_BYTES, &full[s]);
-          if (second) bulk_load(stage + F::BLOCK_BYTES + F::SCALE_BYTES, next, F::SCALE_BYTES, &full[s]);
-          if (head) bulk_load(stage + L::X_AT, x + F::SCALE_BYTES + from * (INPUTS / 2), head, &full[s]);
-          if (tail) bulk_load(stage + L::X_AT + head, next + F::SCALE_BYTES + (max(from, ROWS) - ROWS) * (INPUTS / 2), tail, &full[s]);
+          if (h.second) bulk_load(stage + F::BLOCK_BYTES + F::SCALE_BYTES, next, F::SCALE_BYTES, &full[s]);
+          if (h.head) bulk_load(stage + L::X_AT, x + F::SCALE_BYTES + h.from * (INPUTS / 2), h.head, &full[s]);
+          if (h.tail) bulk_load(stage + L::X_AT + h.head, next + F::SCALE_BYTES + (max(h.from, ROWS) - ROWS) * (INPUTS / 2), h.tail, &full[s]);
         }
         __syncwarp();
         if (++s == STAGES) {
@@ -626,13 +718,13 @@ template <int KIND, typename O> __global__ void __launch_bounds__(PairLayout<KIN
   }
 }
 
-template <int KIND, int NB, bool SPLIT, typename O> int configured(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], int blocks, int split, bool dependent, cudaStream_t st) {
-  typedef Layout<KIND, NB, SPLIT> L;
+template <int KIND, int NB, bool SPLIT, int SRC, typename O> int configured(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], int blocks, int split, bool dependent, cudaStream_t st) {
+  typedef Layout<KIND, NB, SPLIT, SRC> L;
   static bool asked[64] = {false};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return DRYFT_ERR_UNSUPPORTED;
   if (!asked[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(linear_fp4_kernel<KIND, NB, SPLIT, O>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM_BYTES);
+    const cudaError_t e = cudaFuncSetAttribute(linear_fp4_kernel<KIND, NB, SPLIT, SRC, O>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM_BYTES);
     if (e != cudaSuccess) return (int)e;
     asked[dev] = true;
   }
@@ -654,16 +746,16 @@ template <int KIND, int NB, bool SPLIT, typename O> int configured(cudaLaunchCon
   }
   return 0;
 }
-template <int KIND, int NB, bool SPLIT, typename O> int run(const Params& p, int blocks, int split, bool dependent, cudaStream_t st) {
-  typedef Layout<KIND, NB, SPLIT> L;
+template <int KIND, int NB, bool SPLIT, int SRC, typename O> int run(const Params& p, int blocks, int split, bool dependent, cudaStream_t st) {
+  typedef Layout<KIND, NB, SPLIT, SRC> L;
   const long long tiles = ((long long)p.n + ROWS - 1) / ROWS * ((p.m + NB - 1) / NB);
   if (NB < ROWS && p.m > NB) return DRYFT_ERR_UNSUPPORTED;   // (a block of x is 128 rows: only tiles of as many follow one another)
   if (tiles * MOST_BLOCKS > 0x7fffffffll || blocks <= 0 || (SPLIT ? blocks != tiles * split : blocks > tiles)) return DRYFT_ERR_UNSUPPORTED;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
-  const int rc = configured<KIND, NB, SPLIT, O>(cfg, attr, blocks, split, dependent, st);
+  const int rc = configured<KIND, NB, SPLIT, SRC, O>(cfg, attr, blocks, split, dependent, st);
   if (rc) return rc;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_fp4_kernel<KIND, NB, SPLIT, O>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_fp4_kernel<KIND, NB, SPLIT, SRC, O>, p);
   return e != cudaSuccess ? (int)e : launch_status();
 }
 template <int KIND, typename O> int run_pairs(const Params& p, int nb, int blocks, bool dependent, cudaStream_t st) {
@@ -698,11 +790,10 @@ template <int KIND, typename O> int run_pairs(const Params& p, int nb, int block
 }
 template <int KIND, bool SPLIT, typename O> int by_rows(const Params& p, int nb, int blocks, int split, bool dependent, cudaStream_t st) {
   switch (nb) {
-    case 16: return run<KIND, 16, SPLIT, O>(p, blocks, split, dependent, st);
-    case 32: return run<KIND, 32, SPLIT, O>(p, blocks, split, dependent, st);
-    case 64: return run<KIND, 64, SPLIT, O>(p, blocks, split, dependent, st);
-    case 128: return run<KIND, 128, SPLIT, O>(p, blocks, split, dependent, st);
-    case 256: return run<KIND, 256, SPLIT, O>(p, blocks, split, dependent, st);
+    case 16: return run<KIND, 16, SPLIT, HELD, O>(p, blocks, split, dependent, st);
+    case 32: return run<KIND, 32, SPLIT, HELD, O>(p, blocks, split, dependent, st);
+    case 64: return run<KIND, 64, SPLIT, HELD, O>(p, blocks, split, dependent, st);
+    case 128: return run<KIND, 128, SPLIT, HELD, O>(p, blocks, split, dependent, st);
   }
   return DRYFT_ERR_UNSUPPORTED;
 }
@@ -710,12 +801,18 @@ template <int KIND, typename O> int by_split(const Params& p, int nb, int blocks
   if (split == 0) return run_pairs<KIND, O>(p, nb, blocks, dependent, st);
   return split > 1 ? by_rows<KIND, true, O>(p, nb, blocks, split, dependent, st) : by_rows<KIND, false, O>(p, nb, blocks, split, dependent, st);
 }
+template <int KIND, typename O> int by_source(const Params& p, bool silu, int blocks, int split, bool dependent, cudaStream_t st) {
+  if (!silu) return split > 1 ? run<KIND, FUSED_ROWS, true, BF16, O>(p, blocks, split, dependent, st) : run<KIND, FUSED_ROWS, false, BF16, O>(p, blocks, split, dependent, st);
+  if constexpr (sizeof(O) == 2)
+    return split > 1 ? run<KIND, FUSED_ROWS, true, SILU, O>(p, blocks, split, dependent, st) : run<KIND, FUSED_ROWS, false, SILU, O>(p, blocks, split, dependent, st);
+  return DRYFT_ERR_UNSUPPORTED;
+}
 template <int KIND, int NB> int clusters_of(int split) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   int n = 0;
-  if (configured<KIND, NB, true, bf16>(cfg, attr, split, split, false, nullptr)) return 0;
-  return cudaOccupancyMaxActiveClusters(&n, linear_fp4_kernel<KIND, NB, true, bf16>, &cfg) == cudaSuccess ? n : 0;
+  if (configured<KIND, NB, true, HELD, bf16>(cfg, attr, split, split, false, nullptr)) return 0;
+  return cudaOccupancyMaxActiveClusters(&n, linear_fp4_kernel<KIND, NB, true, HELD, bf16>, &cfg) == cudaSuccess ? n : 0;
 }
 }  // namespace
 
@@ -729,30 +826,40 @@ DRYFT_API int dryft_linear_fp4_clusters(int nb, int split) {
     case 32: return clusters_of<NV, 32>(split);
     case 64: return clusters_of<NV, 64>(split);
     case 128: return clusters_of<NV, 128>(split);
-    case 256: return clusters_of<NV, 256>(split);
   }
   return 0;
 }
 
-// y [m, n] = x w^T; x, w: blocks of 128 rows by 256 inputs (fp4.cuh) with factors for each row (NV); y bfloat16 or float32.  nb: x rows of a tile, 16 to 256 (against 128
+// y [m, n] = x w^T; x, w: blocks of 128 rows by 256 inputs (fp4.cuh) with factors for each row (NV); y bfloat16 or float32.  nb: x rows of a tile, 16 to 128 (against 128
 // rows of W).  split: blocks that share a tile's inputs, as a cluster (1: none do, and `blocks` walk the tiles; 0: pairs of
 // blocks walk tiles of 256 rows of W by nb = 128, 192 or 256 of x).
 DRYFT_API int dryft_linear_fp4(int kind, int out_bf16, const void* x, const void* x_factors, const void* w, const void* w_factors, void* y, int m, int n, int k, int nb,
                                int blocks, int split, int pdl, int* err, void* stream) {
   if (m <= 0 || n <= 0) return 0;
   if (k <= 0 || split < 0 || split > MOST_BLOCKS || split > blocks_of(k)) return DRYFT_ERR_UNSUPPORTED;
-  const Params p = {(const unsigned char*)x, (const unsigned char*)w, (const float*)x_factors, (const float*)w_factors, y, err, m, n, blocks_of(k)};
+  const Params p = {(const unsigned char*)x, (const unsigned char*)w, (const float*)x_factors, (const float*)w_factors, y, err, m, n, blocks_of(k), k, 0, false};
   const cudaStream_t st = (cudaStream_t)stream;
   if (kind == NV) return out_bf16 ? by_split<NV, bf16>(p, nb, blocks, split, pdl, st) : by_split<NV, float>(p, nb, blocks, split, pdl, st);
   return out_bf16 ? by_split<MX, bf16>(p, nb, blocks, split, pdl, st) : by_split<MX, float>(p, nb, blocks, split, pdl, st);
 }
 
 // The same of x as it is: `stride` numbers between its rows (silu: of 2 k numbers, as for dryft_fp4_quantise).  scratch: its form in 4 bits, then (NV) its rows' factors, `factors_at` bytes on.  pdl: 1, the rounding is a programmatic
-// dependent of the launch before it; 2, the product is one of the rounding.
+// dependent of the launch before it; 2, the product is one of the rounding.  scratch null: one launch, every block of which rounds x for itself (bfloat16, up to 16 rows, nb = 16, up to 12
+// blocks of 256 inputs a block; silu: to bfloat16 results).
 DRYFT_API int dryft_linear_fp4_rows(int kind, int is_bf16, int silu, int out_bf16, const void* x, long long stride, const void* w, const void* w_factors, void* y, int m, int n, int k,
                                     int nb, int blocks, int split, unsigned char* scratch, long long factors_at, int pdl, int* err, void* stream) {
   if (m <= 0 || n <= 0) return 0;
-  const int rc = dryft_fp4_quantise(is_bf16, kind, silu, x, stride, scratch, scratch + factors_at, m, k, pdl & 1, stream);
+  if (!scratch) {   // rounded by the product's own blocks
+    const int kb = blocks_of(k);
+    if (!is_bf16 || m > FUSED_ROWS || nb != FUSED_ROWS || split < 1 || split > MOST_BLOCKS || split > kb || (kb + split - 1) / split > FUSED_BLOCKS || (silu && !out_bf16))
+      return DRYFT_ERR_UNSUPPORTED;
+    const Params p = {(const unsigned char*)x, (const unsigned char*)w, nullptr, (const float*)w_factors, y, err, m, n, kb, k, stride,
+                      ((uintptr_t)x & 15) == 0 && (m == 1 || stride % 8 == 0) && (!silu || k % 8 == 0)};
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (kind == NV) return out_bf16 ? by_source<NV, bf16>(p, silu, blocks, split, pdl & 1, st) : by_source<NV, float>(p, silu, blocks, split, pdl & 1, st);
+    return out_bf16 ? by_source<MX, bf16>(p, silu, blocks, split, pdl & 1, st) : by_source<MX, float>(p, silu, blocks, split, pdl & 1, st);
+  }
+  const int rc = dryft_fp4_quantise(is_bf16, kind, silu, x, stride, scratch, scratch + factors_at, m, k, pdl, stream);
   if (rc) return rc;
   return dryft_linear_fp4(kind, out_bf16, scratch, scratch + factors_at, w, w_factors, y, m, n, k, nb, blocks, split, pdl & 2, err, stream);
 }

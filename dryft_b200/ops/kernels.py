@@ -15,7 +15,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import threading
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -2773,6 +2773,8 @@ class Fp4:
     n: int
     k: int
     kind: str
+    # Whether a product has read this one as its weight.  The first one is no programmatic dependent of the launch before it, which may be what wrote this.
+    read: list = field(default_factory=list, init=False, repr=False, compare=False)
 
     def __post_init__(self) -> None:
         """What every use relies on is looked at once, here."""
@@ -2846,9 +2848,11 @@ def _fp4_rows(x, name: str) -> int:
 def _fp4_quantise(x, step: int, kind: str) -> Fp4:
     m, k = x.shape
     held = torch.empty(_fp4_shape(m, k, kind), dtype=torch.uint8, device=x.device)
-    factors = torch.empty(m, dtype=torch.float32, device=x.device) if kind == "nv" else None
+    factors = None if kind == "mx" else torch.empty(m, dtype=torch.float32, device=x.device)
     _ok(fp4_lib().dryft_fp4_quantise(x.dtype == torch.bfloat16, FP4_KINDS[kind], False, x.data_ptr(), step, held.data_ptr(), _ptr(factors), m, k, False, _stream()), "fp4_quantise")
-    return Fp4(held, factors, m, k, kind)
+    q = object.__new__(Fp4)   # what __post_init__ looks at is so by construction
+    q.__dict__.update(held=held, factors=factors, n=m, k=k, kind=kind, read=[])
+    return q
 
 
 def fp4_quantise(x, kind: str) -> Fp4:
@@ -2881,22 +2885,66 @@ def _sm_count(device: int) -> int:
     return torch.cuda.get_device_properties(device).multi_processor_count
 
 
-def _fp4_tiles(nb: int, m: int, n: int) -> int:
-    return -(-n // 128) * -(-m // nb)
-
-
-@functools.lru_cache(maxsize=64)
-def _fp4_clusters(device: int, nb: int, split: int) -> int:
-    """How many clusters of ``split`` blocks the device holds at a time."""
+@functools.lru_cache(maxsize=16)
+def _fp4_room(device: int) -> Tuple[int, Tuple[int, ...]]:
+    """Multiprocessors of a device, and how many clusters of 0, 1, 2, ... 8 blocks it holds at a time (two blocks a multiprocessor)."""
     with torch.cuda.device(device):
-        return int(fp4_lib().dryft_linear_fp4_clusters(nb, split))
+        return _sm_count(device), (0, 0) + tuple(2 * int(fp4_lib().dryft_linear_fp4_clusters(16, split)) for split in range(2, 9))
+
+
+def _fp4_plan(m: int, n: int, k: int, sms: int, clusters: Tuple[int, ...]) -> Tuple[int, int, int]:
+    """How a product is run: x rows of a tile, blocks, and how many of them share a tile's inputs as a cluster (1: none do; 0: pairs of blocks with tiles of 256 outputs).
+
+    Up to 128 rows there is one tile for 128 outputs.  Two blocks a multiprocessor walk them, or where there are few, and enough inputs (blocks of 256), a cluster shares a tile:
+    what it costs to add up grows with its columns.  us, whole / shared: 1 row, 2,560 outputs of 4,096 inputs 5.6 / 4.0 (four blocks), of 9,728 11.5 / 5.9 (eight); 6,144 of 2,560
+    4.3 / 4.3; 64 rows, 2,560 of 9,728 15.2 / 8.7 (six), of 4,096 6.4 / 6.5 (two); 128 rows 16.9 / 11.2 and 7.6 / 7.9.
+
+    Above that the least of three estimates, in us, of a run of the same tiles (128 columns), shared or not, and of pairs with 128, 192 or 256 columns.  They are fits
+    to measured times, within a fifth.  200 rows, 2,560 outputs of 4,096 inputs: 8.3 whole, 9.5 shared, 8.4 pairs of 128; of 9,728 inputs 17.0, 11.9, 14.3; 777 rows, 24,576 of
+    4,096: 46.6 whole, pairs of 128, 192 and 256 columns 51.9, 43.7, 40.6; 2,048 rows, 5,120 of 25,600: 132.6; 141, 105, 106; 2,560 of 9,728: 32.9; 35.2, 26.9, 29.6."""
+    units, outs = (k + 255) // 256, (n + 127) // 128
+    if m <= 128:
+        nb = next(b for b in (16, 32, 64, 128) if m <= b)
+        least = 4 if nb <= 32 else 6
+        if units >= 4 * least:
+            split = next((s for s in (8, 6, 5, 4, 3, 2) if s * least <= units and outs <= clusters[s]), 1)
+            if split > 1:
+                return nb, outs * split, split
+        return nb, min(outs, 2 * sms), 1
+    tiles = outs * -(-m // 128)
+    if tiles <= sms:
+        whole = 1.6 + 0.41 * units + 0.015 * tiles
+    else:
+        whole = 2.5 + (0.55 * units + 1.2) * -(-tiles // sms) / 2
+    plans = [(whole, 128, min(tiles, 2 * sms), 1)]
+    if units >= 24:
+        plans += [(7.8 + 0.52 * -(-units // s), 128, tiles * s, s) for s in (6, 5, 4, 3, 2) if tiles <= clusters[s]]
+    for nb, each in ((128, 0.27), (192, 0.29), (256, 0.32)):
+        pairs = (n + 255) // 256 * -(-m // nb)
+        waves = -(-pairs // (sms // 2))
+        plans.append((3.6 + nb / 256 + each * units + (waves - 1) * (0.335 * units + 1.2) * (0.75 + nb / 1024), nb, 2 * min(pairs, sms // 2), 0))
+    return min(plans)[1:]
 
 
 @functools.lru_cache(maxsize=4096)
 def linear_fp4_plan(m: int, n: int, k: int, device: int) -> Tuple[int, int, int]:
-    """How a product is run: x rows of a tile (of 128 outputs), blocks, and how many of them share a tile's inputs."""
-    nb = next((b for b in (16, 32, 64, 128) if m <= b), 256)
-    return nb, min(_fp4_tiles(nb, m, n), _sm_count(device)), 1
+    """``_fp4_plan`` for a device."""
+    return _fp4_plan(m, n, k, *_fp4_room(device))
+
+
+def _fp4_fused(m: int, k: int, kind: str, split: int) -> bool:
+    """Whether every block of a product rounds x for itself, which saves a launch: 16 rows and 12 blocks of 256 inputs a block at most (shared memory), and as long as that is quick:
+    up to 640 times 16 numbers to look at (``"nv"``: whole rows, for their largest).  us, in a graph, in a launch of its own / in the product, 2,560 inputs, 6,144 outputs:
+    ``"mx"``, 1 row 5.8 / 4.9, 4 rows 5.9 / 5.8, 8 rows 6.0 / 7.1; ``"nv"``, 1 row 6.4 / 5.8, 2 rows 6.3 / 6.8, 8 rows 6.5 / 10.3; 9,728 inputs, 2,560 outputs: ``"mx"``, 8 rows
+    7.8 / 6.9, 16 rows 8.2 / 8.7; ``"nv"``, 1 row 8.8 / 8.1, 2 rows 8.8 / 9.0.  And 4.6 us less on the host."""
+    if m > 16:
+        return False
+    units = (k + 255) // 256
+    own = -(-units // split)
+    return own <= 12 and m * 16 * (units if kind == "nv" else own) <= 640
+
+
+_fp4_calls = None   # (product, product of rows as they are)
 
 
 def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = False, out_dtype=None):
@@ -2907,45 +2955,69 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
 
     ``pdl``: a programmatic dependent of the launch before it; ``None``: only the product, of its own rounding; ``False``: no launch overlaps another.  Weights are read once the
     launch in front of the rounding has ended, so they may be as new as that one (with an ``Fp4`` and ``pdl``: older than the launch in front)."""
+    global _fp4_calls, launch_count
     _need_fp4(w, "weight")
+    k, kind = w.k, w.kind
     given = isinstance(x, Fp4)
     if given:
         _need_fp4(x, "x")
         if silu:
             raise KernelError("linear_fp4: silu is taken of float32 or bfloat16 activations")
-        if x.kind != w.kind:
-            raise KernelError(f"linear_fp4: x is held as {x.kind!r}, the weight as {w.kind!r}")
-        m, width = x.n, x.k
+        if x.kind != kind:
+            raise KernelError(f"linear_fp4: x is held as {x.kind!r}, the weight as {kind!r}")
+        m, width, is_bf16 = x.n, x.k, 1
     else:
         step = _fp4_rows(x, "x")
         m, width = x.shape
-    if width != (2 * w.k if silu else w.k):
-        raise KernelError(f"linear_fp4: rows of {2 * w.k if silu else w.k} numbers go with a weight {w.shape}, got {width}")
+        is_bf16 = x.dtype is torch.bfloat16
+    if width != (2 * k if silu else k):
+        raise KernelError(f"linear_fp4: rows of {2 * k if silu else k} numbers go with a weight {w.shape}, got {width}")
     if out is None:
-        dtype = out_dtype or (torch.bfloat16 if given else x.dtype)
-        if dtype not in (torch.float32, torch.bfloat16):
-            raise KernelError(f"linear_fp4: results are float32 or bfloat16, got {dtype}")
-        out = torch.empty((m, w.n), dtype=dtype, device=w.device)
+        if out_dtype is not None and out_dtype not in (torch.float32, torch.bfloat16):
+            raise KernelError(f"linear_fp4: results are float32 or bfloat16, got {out_dtype}")
+        if given or (out_dtype is not None and out_dtype is not x.dtype):
+            out = torch.empty((m, w.n), dtype=out_dtype or torch.bfloat16, device=w.device)
+        else:
+            out = x.new_empty((m, w.n))
     else:
         _need(out, "out", None, (m, w.n))
         _on_current(out, "out")
     out_bf16 = _act(out, "out")
     if m == 0:
         return out
-    nb, blocks, split = linear_fp4_plan(m, w.n, w.k, out.get_device())
-    code, lib, err = FP4_KINDS[w.kind], fp4_lib(), error_flag(w.device).data_ptr()
+    if _fp4_calls is None:
+        lib = fp4_lib()
+        _fp4_calls = (lib.dryft_linear_fp4, lib.dryft_linear_fp4_rows)
+    nb, blocks, split = linear_fp4_plan(m, w.n, k, w.held.get_device())
+    factors = w.factors.data_ptr() if w.factors is not None else 0
+    err = error_flag(w.device).data_ptr()
+    first = not w.read
+    if first:
+        w.read.append(True)
     if given:
-        _ok(lib.dryft_linear_fp4(code, out_bf16, x.held.data_ptr(), _ptr(x.factors), w.held.data_ptr(), _ptr(w.factors), out.data_ptr(), m, w.n, w.k, nb, blocks, split,
-                                 bool(pdl), err, _stream()), "linear_fp4")
+        rc = _fp4_calls[0](FP4_KINDS[kind], out_bf16, x.held.data_ptr(), 0 if x.factors is None else x.factors.data_ptr(), w.held.data_ptr(), factors, out.data_ptr(), m, w.n, k,
+                           nb, blocks, split, bool(pdl) and not first, err, _stream())
+        if rc:
+            _ok(rc, "linear_fp4")
+        launch_count += 1
         return out
-    if silu and x.dtype == torch.float32:
-        act = torch.empty((m, w.k), dtype=x.dtype, device=x.device)
+    if silu and not is_bf16:
+        act = torch.empty((m, k), dtype=x.dtype, device=x.device)
         silu_mul(x.contiguous(), act)
-        x, step, silu = act, w.k, False
-    rows, wide, size = _fp4_shape(m, w.k, w.kind)
-    scratch = torch.empty(rows * wide * size + 4 * m, dtype=torch.uint8, device=w.device)
-    _ok(lib.dryft_linear_fp4_rows(code, x.dtype == torch.bfloat16, silu, out_bf16, x.data_ptr(), step, w.held.data_ptr(), _ptr(w.factors), out.data_ptr(), m, w.n, w.k, nb, blocks,
-                                  split, scratch.data_ptr(), rows * wide * size, _overlap(pdl), err, _stream()), "linear_fp4", 2)
+        x, step, silu = act, k, False
+    if is_bf16 and (out_bf16 or not silu) and _fp4_fused(m, k, kind, split):
+        at = held = 0
+        overlap = bool(pdl) and not first
+    else:
+        rows, wide, size = _fp4_shape(m, k, kind)
+        held = rows * wide * size
+        scratch = w.held.new_empty(held + 4 * m)
+        at, overlap = scratch.data_ptr(), _overlap(pdl)
+    rc = _fp4_calls[1](FP4_KINDS[kind], is_bf16, silu, out_bf16, x.data_ptr(), step, w.held.data_ptr(), factors, out.data_ptr(), m, w.n, k, nb, blocks, split, at, held, overlap,
+                       err, _stream())
+    if rc:
+        _ok(rc, "linear_fp4")
+    launch_count += 2 if at else 1
     return out
 
 

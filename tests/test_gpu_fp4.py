@@ -72,7 +72,7 @@ def test_rounding_of_rare_rows(kind, dtype, k):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("m,n,k", [(1, 128, 64), (1, 128, 256), (16, 128, 512), (5, 389, 83), (17, 200, 1000), (33, 130, 300), (100, 256, 2560), (129, 128, 256), (257, 300, 777),
+@pytest.mark.parametrize("m,n,k", [(1, 128, 64), (1, 128, 256), (2, 256, 5120), (16, 300, 4100), (13, 129, 9728), (16, 128, 512), (5, 389, 83), (17, 200, 1000), (33, 130, 300), (100, 256, 2560), (129, 128, 256), (257, 300, 777),
                                    (700, 384, 320), (8, 40000, 320)])
 def test_products(kind, m, n, k):
     x, w = rows_of(m, k, BF), rows_of(n, k, BF)
