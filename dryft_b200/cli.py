@@ -47,7 +47,7 @@ def _engine(args):
     from .engine.api import Engine
 
     kw = dict(dtype=args.dtype, cuda_graphs=not args.no_cuda_graph, weight_bits=args.weight_bits, cache_bits=args.cache_bits,
-              bits_group=args.bits_group)
+              bits_group=args.bits_group, weight_format=args.weight_format)
     if args.max_batch:
         kw["max_batch"] = args.max_batch
     if args.max_seq_len:
@@ -141,6 +141,8 @@ def main(argv=None) -> int:
         p.add_argument("--max-seq-len", type=int, default=0)
         p.add_argument("--no-cuda-graph", action="store_true")
         p.add_argument("--weight-bits", type=int, default=16, choices=[4, 16], help="4: matrices held in 4 bits")
+        p.add_argument("--weight-format", default="integer", choices=["integer", "mx", "nv"],
+                       help="with --weight-bits 4: whole numbers, or microscaled floating point (groups of 32 / 16), which products round activations to as well")
         p.add_argument("--cache-bits", type=int, default=16, choices=[4, 16], help="4: keys and values held in 4 bits")
         p.add_argument("--bits-group", type=int, default=64, choices=[16, 32, 64, 128], help="numbers that share a scale where something is held in 4 bits")
 

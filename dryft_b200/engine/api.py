@@ -60,6 +60,9 @@ class EngineOptions:
     weight_bits: int = 16
     cache_bits: int = 16
     bits_group: int = 64
+    # What 4-bit matrices are: "integer" (groups as above), or microscaled floating point (csrc/fp4.cuh): "mx", groups of 32 with a power of two, or "nv", groups of 16 with an
+    # 8-bit float and a factor for each row.  Products then round their activations to it too, row by row, and run on the tensor cores' 4-bit instructions: faster, less exact.
+    weight_format: str = "integer"
     tcgen05: bool = True                   # prefill attention and experts' products on tcgen05 / TMEM / TMA where the sizes allow
     # steps of up to this many rows run sublayers that read the same input (a mixer beside a feed-forward, two mixers side
     # by side) on streams of their own, joined before their results are summed: in a captured step they are parallel
@@ -130,7 +133,8 @@ class Engine:
         props = torch.cuda.get_device_properties(dev)
         self.rt = Runtime(dtype=dtype, device=dev, page_size=opts.page_size, sm_count=props.multi_processor_count,
                           small_m_max=opts.small_m_max, stream_m_max=opts.stream_m_max, fuse_decode=opts.fuse_decode, pdl=opts.pdl, tcgen05=opts.tcgen05, norm_ahead=opts.norm_ahead,
-                          branch_rows=opts.branch_rows, weight_bits=opts.weight_bits, cache_bits=opts.cache_bits, bits_group=opts.bits_group)
+                          branch_rows=opts.branch_rows, weight_bits=opts.weight_bits, cache_bits=opts.cache_bits, bits_group=opts.bits_group,
+                          weight_format=opts.weight_format)
         with torch.cuda.device(dev), torch.no_grad():
             self.model = DecoderModel(spec, source, self.rt)
             self.max_seq_len = opts.max_seq_len or min(spec.max_positions, 8192)

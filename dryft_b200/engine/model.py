@@ -15,7 +15,7 @@ import torch
 
 from ..cache.store import KVNeed, SequenceCache, StateNeed
 from ..config.spec import ModelSpec
-from ..ops.kernels import Weight4
+from ..ops.kernels import FP4_KINDS, Fp4, Weight4
 from ..parts.base import BLOCKS, EMBEDDINGS, FAMILIES, FFNS, FOUR_BIT, HEADS, MIXERS, NORMS, Residual, Runtime, StepContext
 
 
@@ -53,6 +53,10 @@ class DecoderModel:
         for what, bits in (("weights", rt.weight_bits), ("a cache", rt.cache_bits)):
             if bits not in (4, 16):
                 raise ValueError(f"{what} in {bits} bits: 16 (the engine's type) or 4")
+        if rt.weight_format not in ("integer", *FP4_KINDS):
+            raise ValueError(f"weight_format is 'integer', 'mx' or 'nv', got {rt.weight_format!r}")
+        if rt.weight_format != "integer" and rt.weight_bits != 4:
+            raise ValueError(f"weight_format {rt.weight_format!r} is a form of weights in 4 bits (weight_bits=4), which are in {rt.weight_bits}")
         if rt.weight_bits == 16 and rt.cache_bits == 16:
             return
         kinds = {"mixer": MIXERS, "ffn": FFNS, "head": HEADS}
@@ -84,9 +88,11 @@ class DecoderModel:
         def visit(obj):
             nonlocal total
             for v in vars(obj).values():
-                if isinstance(v, Weight4) and v.codes.data_ptr() not in seen:
-                    seen.add(v.codes.data_ptr())
-                    total += v.nbytes()
+                if isinstance(v, (Weight4, Fp4)):
+                    key = (v.codes if isinstance(v, Weight4) else v.held).data_ptr()
+                    if key not in seen:
+                        seen.add(key)
+                        total += v.nbytes()
                 if isinstance(v, torch.Tensor) and v.is_floating_point() and v.dim() >= 1:
                     key = v.data_ptr()
                     if key not in seen:

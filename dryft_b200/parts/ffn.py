@@ -80,6 +80,8 @@ class SwiGLU:
         return ss_out, parts, xw_out
 
     def _rows(self, h: torch.Tensor) -> torch.Tensor:
+        if isinstance(self.w_down, K.Fp4):   # the product rounds its rows: what stands in front of it comes along
+            return K.linear_fp4(linear(h, self.w_gate_up, self.rt), self.w_down, pdl=self.rt.pdl, silu=True)
         act = torch.empty((h.shape[0], self.inter), dtype=h.dtype, device=h.device)
         if h.dtype == torch.bfloat16 and self.inter % 16 == 0 and K.linear4_fuses(h.shape[0], self.w_gate_up):
             K.linear4(h, self.w_gate_up, act, pdl=self.rt.pdl, mode="silu")

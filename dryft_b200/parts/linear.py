@@ -66,8 +66,10 @@ def linear(x: torch.Tensor, w: torch.Tensor, rt: Runtime, out_dtype: Optional[to
 
 
 def held(w: torch.Tensor, rt: Runtime):
-    """A part's matrix as the engine holds it: as loaded, or in 4 bits."""
-    return K.pack_weight4(w, K.bits4_group(w.shape[1], rt.bits_group)) if rt.weight_bits == 4 else w
+    """A part's matrix as the engine holds it: as loaded, or in 4 bits, as whole numbers or as microscaled floating point."""
+    if rt.weight_bits != 4:
+        return w
+    return K.fp4_quantise(w, rt.weight_format) if rt.weight_format in K.FP4_KINDS else K.pack_weight4(w, K.bits4_group(w.shape[1], rt.bits_group))
 
 
 def four_bits_fuse(n_rows: int, norm, rt: Runtime, *weights) -> bool:
