@@ -7,11 +7,13 @@ typedef __nv_bfloat16 bf16;
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 
 // A row is 1, 2, 4 or 8 warps' (`span` lanes); a lane has HELD units in registers at a time, `span` apart.  NV wants the row's largest number first: a row that is held whole
-// (bfloat16: up to 16,384 numbers) is read once.
+// (bfloat16: up to 12,288 numbers) is read once.  Its blocks wait for their rows' first numbers, then for each other's maxima: four of them a multiprocessor, with three units a
+// lane, hide more of that than two with four (2,000 rows of 9,728: 15.6 us and 17.8; of 2,560: 6.4 and 7.6).
+template <typename T, int KIND> __host__ __device__ constexpr int held_units() { return sizeof(T) == 4 ? 2 : KIND == NV ? 3 : 4; }
 template <typename T, int KIND, bool SILU>
-__global__ void __launch_bounds__(THREADS) fp4_quantise_kernel(const T* x, long long stride, unsigned char* held, float* factors, int rows, int k, int span, bool words, bool signal) {
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KIND == NV ? 4 : 1) fp4_quantise_kernel(const T* x, long long stride, unsigned char* held, float* factors, int rows, int k, int span, bool words, bool signal) {
   typedef Format<KIND> F;
-  constexpr int HELD = sizeof(T) == 2 ? 4 : 2;
+  constexpr int HELD = held_units<T, KIND>();
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (signal) let_next_launch_in();   // (behind the wait: what comes in may rely on all that was written before this launch)
   __shared__ unsigned most_s[WARPS];
@@ -172,12 +174,12 @@ template <typename... P, typename... A> int launch(void (*kern)(P...), dim3 bloc
 DRYFT_API int dryft_fp4_quantise(int is_bf16, int kind, int silu, const void* x, long long stride, void* held, void* factors, int rows, int k, int pdl, void* stream) {
   if (rows <= 0 || k <= 0) return 0;
   if (silu && !is_bf16) return DRYFT_ERR_UNSUPPORTED;
-  const int item = is_bf16 ? 2 : 4, held_units = is_bf16 ? 4 : 2;
+  const int item = is_bf16 ? 2 : 4, held_at_a_time = !is_bf16 ? held_units<float, NV>() : kind == NV ? held_units<bf16, NV>() : held_units<bf16, MX>();
   const bool words = ((uintptr_t)x & 15) == 0 && (rows == 1 || stride * item % 16 == 0) && (!silu || (long long)k * item % 16 == 0);
   const int units = blocks_of(k) * BLOCK_UNITS;
   // lanes of a row: as many as hold it, or of few rows as many as it has units for (a row's latency is then what counts)
   int span = 32;
-  while (span < THREADS && span * (rows <= 512 ? 1 : held_units) < units) span *= 2;
+  while (span < THREADS && span * (rows <= 512 ? 1 : held_at_a_time) < units) span *= 2;
   const unsigned blocks = (unsigned)((rows + (long long)(THREADS / span) - 1) / (THREADS / span));
   const cudaStream_t st = (cudaStream_t)stream;
   auto run = [&](auto kern, auto* p) { return launch(kern, blocks, pdl & 1, st, p, stride, (unsigned char*)held, (float*)factors, rows, k, span, words, (pdl & 2) != 0); };

@@ -175,17 +175,22 @@ __device__ __forceinline__ void write_columns(const Params& p, O* to, bool there
   }
 }
 
+// The rows' largest magnitudes' bits (FUSED, NV): of this block's inputs, then of whole rows; and what the cluster's blocks sent each other.
+struct Most { unsigned rows[FUSED_ROWS], of[MOST_BLOCKS][FUSED_ROWS]; unsigned long long full; };
+
 // The rounders' part (FUSED): the rows' inputs that this block multiplies, of blocks k0 to k1, into shared memory as the products want them.  NV wants the largest number of whole
-// rows.  A thread has AHEAD units on their way at a time; its first ones stay in registers between looking and rounding, more are read again.
-template <typename L, int KIND, int SRC>
-__device__ __forceinline__ void round_x(const Params& p, int k0, int k1, unsigned char* xs, unsigned* most_s, unsigned long long* x_full) {
+// rows: the blocks of a cluster, which have a row's inputs between them, send each other theirs.  A thread has AHEAD units on their way at a time; its first ones stay in
+// registers between looking and rounding, more are read again.
+template <typename L, int KIND, int SRC, bool SPLIT>
+__device__ __forceinline__ void round_x(const Params& p, int k0, int k1, unsigned char* xs, Most& most_s, unsigned long long* x_full, unsigned rank, unsigned size,
+                                        volatile int* failed) {
   typedef typename L::F F;
   constexpr int THREADS = L::ROUNDERS * 32, AHEAD = 4;
-  const int id = threadIdx.x - 64, lane = threadIdx.x & 31, own = (k1 - k0) * BLOCK_UNITS, all = p.m * own, rest = p.blocks * BLOCK_UNITS - own, all_rest = p.m * rest;
+  const int id = threadIdx.x - 64, lane = threadIdx.x & 31, own = (k1 - k0) * BLOCK_UNITS, all = p.m * own;
   const bf16* const x = reinterpret_cast<const bf16*>(p.x);
   // i / n, for i + 1/2 and n far below 2^23
   auto over = [](int i, float by) { return (int)(((float)i + 0.5f) * by); };
-  const float by_own = 1.f / (float)own, by_rest = 1.f / (float)max(rest, 1);
+  const float by_own = 1.f / (float)own;
   auto load = [&](int i, int row) { return load_unit<bf16, SRC == SILU>(x + row * p.x_stride, (k0 * BLOCK_UNITS + i - row * own) * UNIT, p.k, p.x_words); };
   auto take = [&](Raw<bf16> (&r)[AHEAD], int base) {
 #pragma unroll
@@ -199,29 +204,35 @@ __device__ __forceinline__ void round_x(const Params& p, int k0, int k1, unsigne
       unsigned most = there ? size_of(r).most : 0u;
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-      if (there && lane % BLOCK_UNITS == 0) atomicMax(&most_s[row], most);
+      if (there && lane % BLOCK_UNITS == 0) atomicMax(&most_s.rows[row], most);
     };
-    auto look_all = [&](const Raw<bf16> (&r)[AHEAD], int base, int end, float by) {
+    auto look_all = [&](const Raw<bf16> (&r)[AHEAD], int base) {
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j)
-        if (base + j * THREADS < end) look(r[j], base + j * THREADS + id < end, over(base + j * THREADS + id, by));
+        if (base + j * THREADS < all) look(r[j], base + j * THREADS + id < all, over(base + j * THREADS + id, by_own));
     };
-    for (int base = 0; base < all_rest; base += AHEAD * THREADS) {   // other blocks' inputs
-      Raw<bf16> o[AHEAD] = {};
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        const int i = base + j * THREADS + id, row = over(i, by_rest), c = i - row * rest;
-        if (i < all_rest) o[j] = load_unit<bf16, SRC == SILU>(x + row * p.x_stride, (c < k0 * BLOCK_UNITS ? c : c + own) * UNIT, p.k, p.x_words);
-      }
-      look_all(o, base, all_rest, by_rest);
-    }
-    look_all(r, 0, all, by_own);
+    look_all(r, 0);
     for (int base = AHEAD * THREADS; base < all; base += AHEAD * THREADS) {
       Raw<bf16> o[AHEAD] = {};
       take(o, base);
-      look_all(o, base, all, by_own);
+      look_all(o, base);
     }
-    asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");   // the rounders' own: none of them waits for anything else in front of it
+    // the rounders' own barriers: what a rounder waits for in front of one ends, or runs out
+    asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+    if constexpr (SPLIT) {
+      for (unsigned i = id; i < size * FUSED_ROWS; i += THREADS)
+        asm volatile("{ .reg .u32 a, b; mapa.shared::cluster.u32 a, %0, %3; mapa.shared::cluster.u32 b, %1, %3;\n\t"
+                     "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [a], %2, [b]; }"
+                     ::"r"(smem_u32(&most_s.of[rank][i % FUSED_ROWS])), "r"(smem_u32(&most_s.full)), "r"(most_s.rows[i % FUSED_ROWS]), "r"(i / FUSED_ROWS) : "memory");
+      mbar_wait<true>(&most_s.full, 0, p.err, failed, 6);
+      asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");   // (everybody has sent what `rows` was)
+      if (id < FUSED_ROWS) {
+        unsigned most = 0;
+        for (unsigned b = 0; b < size; ++b) most = max(most, most_s.of[b][id]);
+        most_s.rows[id] = most;
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+    }
   }
   for (int base = 0; base < all; base += AHEAD * THREADS) {
     if (base > 0) take(r, base);
@@ -229,7 +240,7 @@ __device__ __forceinline__ void round_x(const Params& p, int k0, int k1, unsigne
     for (int j = 0; j < AHEAD; ++j) {
       if (base + j * THREADS >= all) break;
       const int i = base + j * THREADS + id, row = over(min(i, all - 1), by_own), c = i - row * own, unit = c % BLOCK_UNITS;
-      const float factor = KIND == NV ? row_factor(most_s[row]) : 1.f;
+      const float factor = KIND == NV ? row_factor(most_s.rows[row]) : 1.f;
       unsigned word;
       const uint2 codes = round_unit<KIND>(r[j], factor, KIND == NV ? __frcp_rn(6.f * factor) : 1.f, word);
       if (i < all) {
@@ -261,7 +272,7 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
   unsigned* const tmem_slot = reinterpret_cast<unsigned*>(x_full + 1);
   __shared__ int failed_s, issued_s;
   __shared__ unsigned long long drained_s;
-  __shared__ unsigned most_s[FUSED_ROWS];   // (FUSED, NV) bits of the rows' largest magnitudes
+  __shared__ Most most_s;
   volatile int* const failed = &failed_s;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, KB = p.blocks;
@@ -285,15 +296,21 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
       mbar_init(&acc_empty[b], READ_THREADS);
     }
     if (FUSED) mbar_init(x_full, L::ROUNDERS * 32);
+    if (FUSED && SPLIT && KIND == NV) mbar_init(&most_s.full, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (FUSED && threadIdx.x < FUSED_ROWS) most_s[threadIdx.x] = 0;
+  if (FUSED && threadIdx.x < FUSED_ROWS) most_s.rows[threadIdx.x] = 0;
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(L::TMEM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if constexpr (FUSED && SPLIT && KIND == NV) {   // the others' barriers are there before anything is sent to them
+    if (threadIdx.x == 0) mbar_expect_tx(&most_s.full, size * FUSED_ROWS * 4);
+    __syncwarp();
+    cluster_sync();
+  }
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const unsigned tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   let_next_launch_in();
@@ -378,7 +395,7 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
     constexpr int COLS = NB / L::PARTS;                  // columns that this warp reads, from `first` on
     const int first = (warp - 2) / 4 * COLS;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if constexpr (FUSED) round_x<L, KIND, SRC>(p, k0, k1, xs, most_s, x_full);
+    if constexpr (FUSED) round_x<L, KIND, SRC, SPLIT>(p, k0, k1, xs, most_s, x_full, rank, size, failed);
     int run = 0;
     for (int t = warp < 2 + L::READERS ? first_tile : tiles; t < tiles; t += step, ++run) {
       const int acc = run % L::ACCS, row = t / x_tiles * ROWS + q * 32 + lane, col0 = t % x_tiles * NB + first, cols = min(COLS, p.m - col0);   // cols: may be none
@@ -387,7 +404,7 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
       if constexpr (KIND == NV)
 #pragma unroll
         for (int c = 0; c < (COLS + 31) / 32; ++c)
-          x_factor[c] = 32 * c + lane >= cols ? 1.f : FUSED ? row_factor(most_s[col0 + 32 * c + lane]) : ld_prev(p.x_factors + col0 + 32 * c + lane);
+          x_factor[c] = 32 * c + lane >= cols ? 1.f : FUSED ? row_factor(most_s.rows[col0 + 32 * c + lane]) : ld_prev(p.x_factors + col0 + 32 * c + lane);
       if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[acc], (unsigned)(run / L::ACCS & 1), p.err, failed, 5))) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if constexpr (SPLIT) break;   // (below)
@@ -417,7 +434,7 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
     if constexpr (KIND == NV)
 #pragma unroll
       for (int c = 0; c < (NB + 31) / 32; ++c)
-        x_factor[c] = !reads || 32 * c + lane >= cols ? 1.f : FUSED ? row_factor(most_s[col0 + 32 * c + lane]) : ld_prev(p.x_factors + col0 + 32 * c + lane);
+        x_factor[c] = !reads || 32 * c + lane >= cols ? 1.f : FUSED ? row_factor(most_s.rows[col0 + 32 * c + lane]) : ld_prev(p.x_factors + col0 + 32 * c + lane);
     auto place = [&](unsigned block, unsigned group) { return (unsigned)(((block * per_block + group) * GROUP / 4 * ROWS + q * 32 + lane) * 16); };
     __syncwarp();
     cluster_sync();   // every block's products have ended, so its stages are free

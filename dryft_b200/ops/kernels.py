@@ -2896,18 +2896,17 @@ def _fp4_plan(m: int, n: int, k: int, sms: int, clusters: Tuple[int, ...]) -> Tu
     """How a product is run: x rows of a tile, blocks, and how many of them share a tile's inputs as a cluster (1: none do; 0: pairs of blocks with tiles of 256 outputs).
 
     Up to 128 rows there is one tile for 128 outputs.  Two blocks a multiprocessor walk them, or where there are few, and enough inputs (blocks of 256), a cluster shares a tile:
-    what it costs to add up grows with its columns.  us, whole / shared: 1 row, 2,560 outputs of 4,096 inputs 5.6 / 4.0 (four blocks), of 9,728 11.5 / 5.9 (eight); 6,144 of 2,560
-    4.3 / 4.3; 64 rows, 2,560 of 9,728 15.2 / 8.7 (six), of 4,096 6.4 / 6.5 (two); 128 rows 16.9 / 11.2 and 7.6 / 7.9.
+    what it costs to add up grows with its columns.  us, whole / shared: 16 rows, 2,560 outputs of 4,096 inputs 5.8 / 4.6 (four blocks), of 9,728 11.6 / 5.9 (eight); 6,144 of 2,560
+    4.8 / 5.0 (two); 64 rows, 2,560 of 4,096 8.5 / 7.4 (four), of 9,728 16.7 / 8.7 (six; eight 9.4), 6,144 of 2,560 6.7 / 7.5; 128 rows 9.8 / 9.8, 18.5 / 11.2 and 8.0 / 9.7.
 
     Above that the least of three estimates, in us, of a run of the same tiles (128 columns), shared or not, and of pairs with 128, 192 or 256 columns.  They are fits
-    to measured times, within a fifth.  200 rows, 2,560 outputs of 4,096 inputs: 8.3 whole, 9.5 shared, 8.4 pairs of 128; of 9,728 inputs 17.0, 11.9, 14.3; 777 rows, 24,576 of
+    to measured times, within a fifth.  200 rows, 2,560 outputs of 4,096 inputs: 10.0 whole, 9.4 shared, 8.5 pairs of 128; of 9,728 inputs 18.5, 11.7, 14.2; 777 rows, 24,576 of
     4,096: 46.6 whole, pairs of 128, 192 and 256 columns 51.9, 43.7, 40.6; 2,048 rows, 5,120 of 25,600: 132.6; 141, 105, 106; 2,560 of 9,728: 32.9; 35.2, 26.9, 29.6."""
     units, outs = (k + 255) // 256, (n + 127) // 128
     if m <= 128:
         nb = next(b for b in (16, 32, 64, 128) if m <= b)
-        least = 4 if nb <= 32 else 6
-        if units >= 4 * least:
-            split = next((s for s in (8, 6, 5, 4, 3, 2) if s * least <= units and outs <= clusters[s]), 1)
+        if units >= 16:
+            split = next((s for s in (8, 6, 5, 4, 3, 2) if 4 * s <= units and outs <= clusters[s] and (s <= 6 or nb <= 32)), 1)
             if split > 1:
                 return nb, outs * split, split
         return nb, min(outs, 2 * sms), 1
@@ -2932,16 +2931,15 @@ def linear_fp4_plan(m: int, n: int, k: int, device: int) -> Tuple[int, int, int]
     return _fp4_plan(m, n, k, *_fp4_room(device))
 
 
-def _fp4_fused(m: int, k: int, kind: str, split: int) -> bool:
-    """Whether every block of a product rounds x for itself, which saves a launch: 16 rows and 12 blocks of 256 inputs a block at most (shared memory), and as long as that is quick:
-    up to 640 times 16 numbers to look at (``"nv"``: whole rows, for their largest).  us, in a graph, in a launch of its own / in the product, 2,560 inputs, 6,144 outputs:
-    ``"mx"``, 1 row 5.8 / 4.9, 4 rows 5.9 / 5.8, 8 rows 6.0 / 7.1; ``"nv"``, 1 row 6.4 / 5.8, 2 rows 6.3 / 6.8, 8 rows 6.5 / 10.3; 9,728 inputs, 2,560 outputs: ``"mx"``, 8 rows
-    7.8 / 6.9, 16 rows 8.2 / 8.7; ``"nv"``, 1 row 8.8 / 8.1, 2 rows 8.8 / 9.0.  And 4.6 us less on the host."""
-    if m > 16:
+def _fp4_fused(m: int, k: int, kind: str, nb: int, split: int) -> bool:
+    """Whether every block of a product rounds x for itself, which saves a launch: 16 rows and 12 blocks of 256 inputs a block at most (shared memory), and as long as that is
+    quick: a block rounds up to 640 times 16 numbers (``"nv"``, where a row's largest number comes first: 256).  us, in a graph, in a launch of its own / in the product, 2,560 inputs,
+    6,144 outputs: ``"mx"``, 1 row 5.8 / 4.9, 4 rows 5.8 / 5.8, 8 rows 6.0 / 7.3; ``"nv"``, 1 row 6.4 / 5.9, 2 rows 6.4 / 6.8; 9,728 inputs, 2,560 outputs, eight blocks a tile: ``"mx"``,
+    1 row 7.6 / 5.9, 8 rows 7.9 / 7.0, 16 rows 7.9 / 8.5; ``"nv"``, 1 row 8.6 / 7.6, 3 rows 8.4 / 7.7, 8 rows 8.8 / 9.4; with silu in front 1 row 10.5 / 8.2.  On the host 4 us less."""
+    if m > 16 or nb != 16 or split < 1:
         return False
-    units = (k + 255) // 256
-    own = -(-units // split)
-    return own <= 12 and m * 16 * (units if kind == "nv" else own) <= 640
+    own = -(-((k + 255) // 256) // split)
+    return own <= 12 and m * 16 * own <= (256 if kind == "nv" else 640)
 
 
 _fp4_calls = None   # (product, product of rows as they are)
@@ -3005,7 +3003,7 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
         act = torch.empty((m, k), dtype=x.dtype, device=x.device)
         silu_mul(x.contiguous(), act)
         x, step, silu = act, k, False
-    if is_bf16 and (out_bf16 or not silu) and _fp4_fused(m, k, kind, split):
+    if is_bf16 and (out_bf16 or not silu) and _fp4_fused(m, k, kind, nb, split):
         at = held = 0
         overlap = bool(pdl) and not first
     else:
