@@ -70,11 +70,43 @@ template <typename T> __device__ __forceinline__ Raw<T> load(const T* row, int c
     }
   return r;
 }
+// The same where rows begin anywhere: the 16-byte words that hold the numbers, shifted.  (A word that holds one byte of a row can be read; a number a load would cross memory 8 times.)
+template <typename T> __device__ __forceinline__ Raw<T> load_shifted(const T* row, int c, int k) {
+  constexpr int N = UNIT * sizeof(T) / 4;
+  Raw<T> r;
+  unsigned w[N + 4];
+  const uintptr_t at = reinterpret_cast<uintptr_t>(row + c), end = reinterpret_cast<uintptr_t>(row + min(c + UNIT, k));
+  const uint4* const p = reinterpret_cast<const uint4*>(at & ~(uintptr_t)15);
+#pragma unroll
+  for (int i = 0; i < (N + 4) / 4; ++i) {
+    const uint4 a = c < k && reinterpret_cast<uintptr_t>(p + i) < end ? ld_prev(p + i) : make_uint4(0u, 0u, 0u, 0u);
+    w[4 * i] = a.x;
+    w[4 * i + 1] = a.y;
+    w[4 * i + 2] = a.z;
+    w[4 * i + 3] = a.w;
+  }
+#pragma unroll
+  for (int i = 0; i < N + 2; ++i) w[i] = at & 8 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < N + 1; ++i) w[i] = at & 4 ? w[i + 1] : w[i];
+#pragma unroll
+  for (int i = 0; i < N; ++i) r.w[i] = __funnelshift_r(w[i], w[i + 1], at & 2 ? 16 : 0);
+  const int left = k - c;   // numbers of the row; zeros behind them
+  if (left < UNIT) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      constexpr int PER = 4 / sizeof(T);
+      if (PER * i >= left) r.w[i] = 0;
+      else if (PER == 2 && 2 * i + 1 >= left) r.w[i] &= 0xffffu;
+    }
+  }
+  return r;
+}
 // SILU: the row holds gate numbers, then as many others: silu(gate) rounded, times the other, rounded (the points of `silu_mul`).
-template <typename T, bool SILU> __device__ __forceinline__ Raw<T> load_unit(const T* row, int c, int k, bool words) {
-  Raw<T> r = load(row, c, k, words);
+template <typename T, bool SILU, bool SHIFTED = false> __device__ __forceinline__ Raw<T> load_unit(const T* row, int c, int k, bool words) {
+  Raw<T> r = SHIFTED ? load_shifted(row, c, k) : load(row, c, k, words);
   if constexpr (SILU) {
-    const Raw<T> up = load(row + k, c, k, words);
+    const Raw<T> up = SHIFTED ? load_shifted(row + k, c, k) : load(row + k, c, k, words);
 #pragma unroll
     for (int i = 0; i < UNIT / 2; ++i) {
       float v[2];
