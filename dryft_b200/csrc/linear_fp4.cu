@@ -516,7 +516,10 @@ template <int KIND> struct PairLayout {
   static constexpr int X_AT = F::BLOCK_BYTES + 2 * F::SCALE_BYTES, STAGE_BYTES = X_AT + MOST_NB / 2 * (INPUTS / 2);   // W's block, x's scales (all of the tile's), half of x's codes
   static constexpr int STAGES = 225 * 1024 / STAGE_BYTES;
   static constexpr int SCALE_COLS = 4 * F::WORDS * 3, TMEM_COLS = 512;
-  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + 8 * (3 * STAGES + 2) + 16;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + 8 * (3 * STAGES + 4) + 16;
+  // tensor memory: sums of two tiles of up to 192 columns, so that a tile's products need not wait until the sums before it are read, or of one of 256; then the scales of two stages
+  static constexpr int TWO_NB = 192;
+  static_assert(2 * TWO_NB + 2 * SCALE_COLS <= TMEM_COLS, "of tensor memory");
   static_assert(MOST_NB + 2 * SCALE_COLS <= TMEM_COLS && SMEM_BYTES <= 227 * 1024 && STAGE_BYTES % 1024 == 0, "of a block");
 };
 __device__ __forceinline__ void mbar_arrive_at(void* bar, unsigned rank) {   // of a block of the cluster
@@ -535,9 +538,10 @@ template <int KIND, typename O> __global__ void __launch_bounds__(PairLayout<KIN
   unsigned long long* const full = reinterpret_cast<unsigned long long*>(stages + STAGES * L::STAGE_BYTES);   // [S] this block's copies
   unsigned long long* const peer_full = full + STAGES;                                                         // [S] (of the first block) the other's copies
   unsigned long long* const empty = peer_full + STAGES;                                                        // [S] products -> copies
-  unsigned long long* const acc_full = empty + STAGES;                                                         // a tile's sums -> their readers
-  unsigned long long* const acc_empty = acc_full + 1;                                                          // (of the first block) read, by every reading warp of both
-  unsigned* const tmem_slot = reinterpret_cast<unsigned*>(acc_empty + 1);
+  unsigned long long* const acc_full = empty + STAGES;                                                         // [2] a tile's sums -> their readers
+  unsigned long long* const acc_empty = acc_full + 2;                                                          // [2] (of the first block) read, by every reading warp of both
+  unsigned* const tmem_slot = reinterpret_cast<unsigned*>(acc_empty + 2);
+  const int accs = nb <= L::TWO_NB ? 2 : 1, acc_cols = nb <= L::TWO_NB ? L::TWO_NB : L::MOST_NB;
   __shared__ int failed_s, issued_s;
   __shared__ unsigned long long drained_s;
   volatile int* const failed = &failed_s;
@@ -565,8 +569,10 @@ template <int KIND, typename O> __global__ void __launch_bounds__(PairLayout<KIN
       mbar_init(&peer_full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(acc_full, 1);
-    mbar_init(acc_empty, 2 * L::READERS);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 2 * L::READERS);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -656,14 +662,16 @@ template <int KIND, typename O> __global__ void __launch_bounds__(PairLayout<KIN
     for (int t = first_tile; ok && t < tiles; t += step, ++run) {
       const Tile at = tile_of(t);
       const unsigned n_bits = (unsigned)(at.cols >> 3) << 17, shift = at.x0 % ROWS / 32;   // shift: columns of scales in front of the tile's
-      ok = run < 1 || __all_sync(0xffffffffu, mbar_wait<true>(acc_empty, (unsigned)((run - 1) & 1), p.err, failed, 14));
+      const int acc = run % accs;
+      const unsigned d = tmem + acc * acc_cols;
+      ok = run < accs || __all_sync(0xffffffffu, mbar_wait<true>(&acc_empty[acc], (unsigned)((run / accs - 1) & 1), p.err, failed, 14));
       for (int kb = 0; ok && kb < KB; ++kb) {
         ok = __all_sync(0xffffffffu, mbar_wait(&full[s], par, p.err, failed, 12) && mbar_wait<true>(&peer_full[s], par, p.err, failed, 13));
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (issues) {
           unsigned char* const stage = stages + (size_t)s * L::STAGE_BYTES;
-          const unsigned sw = tmem + L::MOST_NB + buffer * L::SCALE_COLS, sx = sw + 4 * F::WORDS;
+          const unsigned sw = tmem + accs * acc_cols + buffer * L::SCALE_COLS, sx = sw + 4 * F::WORDS;
           const unsigned long long w_scales = scales_desc(stage), x_scales = scales_desc(stage + F::BLOCK_BYTES);
           const unsigned long long w = codes_desc(stage + F::SCALE_BYTES), x = codes_desc(stage + L::X_AT);
 #pragma unroll
@@ -675,10 +683,10 @@ template <int KIND, typename O> __global__ void __launch_bounds__(PairLayout<KIN
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int word = j * F::WORDS / 4;
-            umma<KIND, 2>(tmem, w + 2 * j, x + 2 * j, idesc<KIND, 256>(KIND == MX ? 2 * (j & 1) : 0) | n_bits, sw + 4 * word, sx + 8 * word + shift, kb > 0 || j > 0);
+            umma<KIND, 2>(d, w + 2 * j, x + 2 * j, idesc<KIND, 256>(KIND == MX ? 2 * (j & 1) : 0) | n_bits, sw + 4 * word, sx + 8 * word + shift, kb > 0 || j > 0);
           }
           umma_commit_both(&empty[s]);
-          if (kb == KB - 1) umma_commit_both(acc_full);
+          if (kb == KB - 1) umma_commit_both(&acc_full[acc]);
         }
         __syncwarp();
         buffer ^= 1;
@@ -700,16 +708,17 @@ template <int KIND, typename O> __global__ void __launch_bounds__(PairLayout<KIN
       if constexpr (KIND == NV)
 #pragma unroll
         for (int c = 0; c < L::COLS / 32; ++c) x_factor[c] = 32 * c + lane < cols ? ld_prev(p.x_factors + col0 + 32 * c + lane) : 1.f;
-      if (!__all_sync(0xffffffffu, mbar_wait(acc_full, (unsigned)(run & 1), p.err, failed, 15))) break;
+      const int acc = run % accs;
+      if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[acc], (unsigned)(run / accs & 1), p.err, failed, 15))) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const unsigned from = tmem + ((unsigned)(q * 32) << 16) + first;
+      const unsigned from = tmem + ((unsigned)(q * 32) << 16) + acc * acc_cols + first;
       float v[L::COLS / 16][16];
 #pragma unroll
       for (int c = 0; c < L::COLS / 16; ++c)
         if (16 * c < cols) tmem_ld16(from + 16 * c, v[c]);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive_at(acc_empty, 0);
+      if (lane == 0) mbar_arrive_at(&acc_empty[acc], 0);
       write_columns<KIND, L::COLS>(p, reinterpret_cast<O*>(p.y) + (size_t)col0 * p.n + row, row < p.n, cols, v, own, x_factor);
       __syncwarp();
     }

@@ -2901,7 +2901,7 @@ def _fp4_plan(m: int, n: int, k: int, sms: int, clusters: Tuple[int, ...]) -> Tu
 
     Above that the least of three estimates, in us, of a run of the same tiles (128 columns), shared or not, and of pairs with 128, 192 or 256 columns.  They are fits
     to measured times, within a fifth.  200 rows, 2,560 outputs of 4,096 inputs: 10.0 whole, 9.4 shared, 8.5 pairs of 128; of 9,728 inputs 18.5, 11.7, 14.2; 777 rows, 24,576 of
-    4,096: 46.6 whole, pairs of 128, 192 and 256 columns 51.9, 43.7, 40.6; 2,048 rows, 5,120 of 25,600: 132.6; 141, 105, 106; 2,560 of 9,728: 32.9; 35.2, 26.9, 29.6."""
+    4,096: 46.4 whole, pairs of 128, 192 and 256 columns 54.7, 43.6, 41.5; 2,048 rows, 5,120 of 25,600: 136.9; 139.8, 102.4, 105.0; 2,560 of 9,728: 33.8; 35.1, 26.1, 30.0."""
     units, outs = (k + 255) // 256, (n + 127) // 128
     if m <= 128:
         nb = next(b for b in (16, 32, 64, 128) if m <= b)
@@ -2921,7 +2921,7 @@ def _fp4_plan(m: int, n: int, k: int, sms: int, clusters: Tuple[int, ...]) -> Tu
     for nb, each in ((128, 0.27), (192, 0.29), (256, 0.32)):
         pairs = (n + 255) // 256 * -(-m // nb)
         waves = -(-pairs // (sms // 2))
-        plans.append((3.6 + nb / 256 + each * units + (waves - 1) * (0.335 * units + 1.2) * (0.75 + nb / 1024), nb, 2 * min(pairs, sms // 2), 0))
+        plans.append((3.6 + nb / 256 + each * units + 0.03 * min(pairs, sms // 2) + (waves - 1) * (0.335 * units + 1.2) * (0.75 + nb / 1024), nb, 2 * min(pairs, sms // 2), 0))
     return min(plans)[1:]
 
 
