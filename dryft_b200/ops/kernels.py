@@ -2900,7 +2900,7 @@ def _fp4_plan(m: int, n: int, k: int, sms: int, clusters: Tuple[int, ...]) -> Tu
     4.8 / 5.0 (two); 64 rows, 2,560 of 4,096 8.5 / 7.4 (four), of 9,728 16.7 / 8.7 (six; eight 9.4), 6,144 of 2,560 6.7 / 7.5; 128 rows 9.8 / 9.8, 18.5 / 11.2 and 8.0 / 9.7.
 
     Above that the least of three estimates, in us, of a run of the same tiles (128 columns), shared or not, and of pairs with 128, 192 or 256 columns.  They are fits
-    to measured times, within a fifth.  200 rows, 2,560 outputs of 4,096 inputs: 10.0 whole, 9.4 shared, 8.5 pairs of 128; of 9,728 inputs 18.5, 11.7, 14.2; 777 rows, 24,576 of
+    to measured times; what they choose takes 0.4 percent longer than the best in the mean of 90 sizes, 7 at the most.  200 rows, 2,560 outputs of 4,096 inputs: 10.0 whole, 9.4 shared, 8.5 pairs of 128; of 9,728 inputs 18.5, 11.7, 14.2; 777 rows, 24,576 of
     4,096: 46.4 whole, pairs of 128, 192 and 256 columns 54.7, 43.6, 41.5; 2,048 rows, 5,120 of 25,600: 136.9; 139.8, 102.4, 105.0; 2,560 of 9,728: 33.8; 35.1, 26.1, 30.0."""
     units, outs = (k + 255) // 256, (n + 127) // 128
     if m <= 128:
@@ -2912,16 +2912,16 @@ def _fp4_plan(m: int, n: int, k: int, sms: int, clusters: Tuple[int, ...]) -> Tu
         return nb, min(outs, 2 * sms), 1
     tiles = outs * -(-m // 128)
     if tiles <= sms:
-        whole = 1.6 + 0.41 * units + 0.015 * tiles
+        whole = 2.1 + 0.41 * units + 0.015 * tiles
     else:
         whole = 2.5 + (0.55 * units + 1.2) * -(-tiles // sms) / 2
     plans = [(whole, 128, min(tiles, 2 * sms), 1)]
     if units >= 24:
-        plans += [(7.8 + 0.52 * -(-units // s), 128, tiles * s, s) for s in (6, 5, 4, 3, 2) if tiles <= clusters[s]]
+        plans += [(7.31 + 0.43 * -(-units // s), 128, tiles * s, s) for s in (6, 5, 4, 3, 2) if tiles <= clusters[s]]
     for nb, each in ((128, 0.27), (192, 0.29), (256, 0.32)):
         pairs = (n + 255) // 256 * -(-m // nb)
         waves = -(-pairs // (sms // 2))
-        plans.append((3.6 + nb / 256 + each * units + 0.03 * min(pairs, sms // 2) + (waves - 1) * (0.335 * units + 1.2) * (0.75 + nb / 1024), nb, 2 * min(pairs, sms // 2), 0))
+        plans.append((3.6 + 1.16 * nb / 256 + each * units + 0.007 * min(pairs, sms // 2) + (waves - 1) * (0.38 * units + 0.97) * (0.74 + 0.26 * nb / 256), nb, 2 * min(pairs, sms // 2), 0))
     return min(plans)[1:]
 
 
