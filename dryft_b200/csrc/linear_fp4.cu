@@ -1,12 +1,22 @@
 // y = x w^T with both operands in microscaled 4-bit floating point (fp4.cuh), on the 5th-generation tensor cores, which multiply such numbers and scales as they lie:
-// tcgen05.mma kind::mxf4 (a scale for 32 inputs) and kind::mxf4nvf4 (for 16), sums of 64 inputs an instruction in 32 bits.
+// tcgen05.mma kind::mxf4 (a scale for 32 inputs) and kind::mxf4nvf4 (for 16), 64 inputs an instruction, summed in 32 bits.  A product of two codes is a multiple of 1/4, so what an
+// instruction sums before the scales is exact: with 25,600 inputs results are off by 4e-8 of the whole, 32-bit multiply-adds in order by 4e-7.
 //
-// Computed transposed: a tile is 128 rows of W, on the M side, against NB rows of x (16 to 256, padded), its 128 x NB sums in tensor memory, a W row a lane.  A stage of the ring is
-// 256 inputs: a block of W and one or two of x, each a copy of consecutive bytes.  The scales go on from shared into tensor memory (tcgen05.cp), in front of the four products of
-// their stage, by the thread that issues those: the copies and products of one thread run in the order that they were issued in.
+// Computed transposed: a tile is 128 rows of W, on the M side, against NB rows of x (16 to 128, padded to whole sixteens), its sums in tensor memory, a W row a lane: results are written
+// a column at a time, 32 lanes' behind one another.  A stage of the ring is 256 inputs: a block of W and one of x, each one copy of consecutive bytes (the layout is the tensor
+// cores' own, so no tensor maps).  The scales go on from shared into tensor memory (tcgen05.cp) in front of the four products of their stage, by the thread that issues those:
+// the copies and products of one thread run in the order that they were issued in; two stages' scales have places of their own.
 //
-// Warps: 0 copies, 1 issues, 2 to 5 read the sums out.  Every wait on a barrier is bounded by a clock; a waiter that gives up raises *err, every role leaves its loop, the
-// block lets its copies and products end and frees its tensor memory.
+// Which form: one tile for up to 128 rows of x; blocks walk the tiles, two a multiprocessor (one's products and copies are the other's time to write), or, where tiles are few, a cluster
+// shares a tile's inputs and adds up through distributed shared memory (SPLIT); up to 16 rows are rounded by every block for itself (SRC).  Many rows: pairs of blocks with one
+// 256-row tile of W between them (below).  ops/kernels.py:_fp4_plan chooses, with both sides' figures.
+//
+// What bounds it.  Few rows: W's bytes.  151,936 outputs of 2,560 inputs, 1 row: 33.6 us, 6,500 GB/s, 99% of a copy's rate; with fewer bytes the launch, first bytes and a tile's end: 8 rows,
+// 19,456 of 2,560 (28 MB) 7.2 us where the bytes are 4.1; 1 row, 6,144 of 2,560 4.6 and 1.35.  Many rows: the ring's round trip.  2,048 rows, 24,576 of 4,096: 83 us, 5.0 PFLOP/s, the tensor
+// pipe 63% busy, L2 42%: five stages of a pair are 190 KB on their way, which return, are multiplied and asked for again in 1.5 us, 0.33 us a stage where its products take 0.27; and a tile's end.
+//
+// Warps: 0 copies, 1 issues, the others read the sums out.  Every wait on a barrier is bounded by a clock; a waiter that gives up raises *err, every role leaves its loop, the block lets its
+// copies and products end and frees its tensor memory.
 #include "fp4.cuh"
 #include "drain.h"
 
@@ -150,12 +160,18 @@ __device__ __forceinline__ unsigned cluster_size() {
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
+// (relaxed: what the blocks of a cluster hand each other completes barriers of its own.  A release waits until all that the block has written is in place: a microsecond.)
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_arrive();
+  cluster_wait();
 }
-// into another block's shared memory, at the address that this block has the like at
-__device__ __forceinline__ void st_cluster(unsigned addr, unsigned rank, float a, float b, float c, float d) {
-  asm volatile("{ .reg .u32 a; mapa.shared::cluster.u32 a, %0, %1; st.shared::cluster.v4.f32 [a], {%2, %3, %4, %5}; }" ::"r"(addr), "r"(rank), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+// 16 bytes into another block's shared memory, at the address that this block has the like at; they complete a barrier there
+__device__ __forceinline__ void send(unsigned addr, unsigned bar, unsigned rank, float a, float b, float c, float d) {
+  asm volatile("{ .reg .u32 a, b; mapa.shared::cluster.u32 a, %0, %2; mapa.shared::cluster.u32 b, %1, %2;\n\t"
+               "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [a], {%3, %4, %5, %6}, [b]; }"
+               ::"r"(addr), "r"(bar), "r"(rank), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
 constexpr int MOST_BLOCKS = 8;   // of a cluster
 
@@ -271,7 +287,7 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
   unsigned long long* const x_full = acc_empty + 2;                                                            // (FUSED) x is rounded (by every rounder) -> products
   unsigned* const tmem_slot = reinterpret_cast<unsigned*>(x_full + 1);
   __shared__ int failed_s, issued_s;
-  __shared__ unsigned long long drained_s;
+  __shared__ unsigned long long drained_s, sums_s;   // sums_s: (SPLIT) what the cluster's blocks send this one has come
   __shared__ Most most_s;
   volatile int* const failed = &failed_s;
 
@@ -281,6 +297,8 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
   const unsigned rank = SPLIT ? cluster_rank() : 0, size = SPLIT ? cluster_size() : 1;
   const int first_tile = blockIdx.x / size, step = SPLIT ? tiles : gridDim.x, k0 = SPLIT ? KB * rank / size : 0, k1 = SPLIT ? KB * (rank + 1) / size : KB;
 
+  // (SPLIT) columns that the blocks of a cluster have in turn
+  constexpr int GROUP = 4, GROUPS = NB / GROUP;
   // columns of a tile that has so many rows of x left: whole sixteens
   auto columns = [](int left) { return left >= NB ? NB : (left + 15) / 16 * 16; };
 
@@ -295,6 +313,7 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], READ_THREADS);
     }
+    if (SPLIT) mbar_init(&sums_s, 1);
     if (FUSED) mbar_init(x_full, L::ROUNDERS * 32);
     if (FUSED && SPLIT && KIND == NV) mbar_init(&most_s.full, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -422,9 +441,8 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
   }
 
   if constexpr (SPLIT) {
-    // Columns go to the cluster's blocks in turn, GROUP at a time: every block sends the others its sums, into what were the stages ([block][group][row][4]), and adds up what it
+    // Columns go to the cluster's blocks in turn, GROUP at a time: every block sends the others its sums, into what were the stages ([block][group][row][4], by asynchronous stores), and adds up what it
     // was sent, in the order of the inputs.  All threads come by here, whatever their waits came to; what is sent when one gave up is nobody's result.
-    constexpr int GROUP = 4, GROUPS = NB / GROUP;
     const unsigned per_block = (GROUPS + size - 1) / size;
     const int q = warp & 3, part = (warp - 2) / 4;
     const int row = first_tile / x_tiles * ROWS + q * 32 + lane, col0 = first_tile % x_tiles * NB, cols = min(NB, p.m - col0);
@@ -436,6 +454,11 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
       for (int c = 0; c < (NB + 31) / 32; ++c)
         x_factor[c] = !reads || 32 * c + lane >= cols ? 1.f : FUSED ? row_factor(most_s.rows[col0 + 32 * c + lane]) : ld_prev(p.x_factors + col0 + 32 * c + lane);
     auto place = [&](unsigned block, unsigned group) { return (unsigned)(((block * per_block + group) * GROUP / 4 * ROWS + q * 32 + lane) * 16); };
+    __syncwarp();
+    if (threadIdx.x == 64) {   // groups rank, rank + size, ... of those that have results, from every block
+      const unsigned groups = (cols + GROUP - 1) / GROUP, mine = groups > rank ? (groups - rank + size - 1) / size : 0;
+      mbar_expect_tx(&sums_s, mine * size * GROUP * ROWS * 4);
+    }
     __syncwarp();
     cluster_sync();   // every block's products have ended, so its stages are free
     if (reads) {
@@ -449,12 +472,13 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
         for (int j = 0; j < 16; j += 4)
           if (c + j < cols) {
             const unsigned g = (c + j) / GROUP;
-            st_cluster(smem_u32(stages) + place(rank, g / size) + (c + j) % GROUP / 4 * ROWS * 16, g % size, v[j], v[j + 1], v[j + 2], v[j + 3]);
+            send(smem_u32(stages) + place(rank, g / size), smem_u32(&sums_s), g % size, v[j], v[j + 1], v[j + 2], v[j + 3]);
           }
       }
     }
+    if (reads) mbar_wait<true>(&sums_s, 0, p.err, failed, 7);
     __syncwarp();
-    cluster_sync();
+    cluster_arrive();   // (a block whose shared memory others may still send to does not end: below)
     if (reads) {
 #pragma unroll 1
       for (unsigned i = part; (rank + size * i) * GROUP < cols; i += L::PARTS) {
@@ -466,7 +490,7 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
         for (unsigned b = 0; b < size; ++b)
 #pragma unroll
           for (int j = 0; j < GROUP; j += 4) {
-            const float4 t = *reinterpret_cast<const float4*>(stages + place(b, i) + j / 4 * ROWS * 16);
+            const float4 t = *reinterpret_cast<const float4*>(stages + place(b, i));
             v[j] += t.x;
             v[j + 1] += t.y;
             v[j + 2] += t.z;
@@ -486,6 +510,8 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
             if (c + j < cols) reinterpret_cast<O*>(p.y)[(size_t)(col0 + c + j) * p.n + row] = from_f32<O>(v[j]);
       }
     }
+    __syncwarp();
+    cluster_wait();
   }
 
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -508,7 +534,7 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
 }
 
 // The same for many rows of x: two blocks on neighbouring multiprocessors have a tile of 256 rows of W (128 each) against `nb` rows of x, of which each holds half: a product's
-// operands then cross from L2 once for twice the work (8 copies' worth of L2 instead of 12, which is what the one-block tiles of 256 wait for).  The first block issues the products of
+// operands then cross from L2 for twice the work (38 KB of a stage a block instead of 54: tiles of 256 columns by one block took 95 us where pairs take 83).  The first block issues the products of
 // both.  The second one's copies complete barriers of its own; its warp 1 passes that on.
 template <int KIND> struct PairLayout {
   typedef Format<KIND> F;
@@ -718,7 +744,7 @@ template <int KIND, typename O> __global__ void __launch_bounds__(PairLayout<KIN
         if (16 * c < cols) tmem_ld16(from + 16 * c, v[c]);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive_at(&acc_empty[acc], 0);
+      if (lane == 0 && t + accs * step < tiles) mbar_arrive_at(&acc_empty[acc], 0);   // (where products wait for it: nothing is on its way to a block that may have ended)
       write_columns<KIND, L::COLS>(p, reinterpret_cast<O*>(p.y) + (size_t)col0 * p.n + row, row < p.n, cols, v, own, x_factor);
       __syncwarp();
     }
@@ -737,6 +763,7 @@ template <int KIND, typename O> __global__ void __launch_bounds__(PairLayout<KIN
     }
     __syncthreads();
   }
+  __syncwarp();
   cluster_sync();   // neither's memory goes before the other is done with it
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");

@@ -2727,6 +2727,7 @@ def weight4_expand(w: Weight4, out, rest: bool = False) -> None:
 
 # ----------------------------------------------------------------------------- microscaled 4-bit floating point: rounding, values, products
 # A number is one of 0, 1/2, 1, 3/2, 2, 3, 4, 6 or minus that, times the scale of its group; csrc/fp4.cuh has the arithmetic and the layout.
+_FP4_MOST = 2**31 - 512                       # of rows, of inputs: the kernels count them in 32 bits
 FP4_KINDS = {"mx": 0, "nv": 1}                # groups of 32 with powers of two; groups of 16 with 8-bit floats, and a factor for each row
 _FP4_BLOCK = {"mx": 16384 + 1024, "nv": 16384 + 2048}   # bytes of 128 rows by 256 inputs: codes and scales
 
@@ -2779,8 +2780,8 @@ class Fp4:
     def __post_init__(self) -> None:
         """What every use relies on is looked at once, here."""
         _fp4_kind(self.kind)
-        if self.n <= 0 or self.k <= 0:
-            raise KernelError(f"Fp4: no numbers in [{self.n}, {self.k}]")
+        if not (0 < self.n < _FP4_MOST and 0 < self.k < _FP4_MOST):
+            raise KernelError(f"Fp4: no numbers, or too many rows or inputs, in [{self.n}, {self.k}]")
         wanted = [(self.held, "held", torch.uint8, _fp4_shape(self.n, self.k, self.kind), 16)]
         if self.kind == "nv":
             wanted.append((self.factors, "factors", torch.float32, (self.n,), 16))
@@ -2841,8 +2842,16 @@ def _fp4_rows(x, name: str) -> int:
     step, one = x.stride()
     if one != 1 and x.shape[1] > 1:
         raise KernelError(f"{name}: the numbers of a row lie behind one another (strides {x.stride()})")
+    if max(x.shape) >= _FP4_MOST:
+        raise KernelError(f"{name}: rows, and numbers of a row, are fewer than {_FP4_MOST}, got {tuple(x.shape)}")
     _on_current(x, name)
     return step
+
+
+def _overlapping(a, b) -> bool:
+    """Whether the stretches of memory that two tensors lie in meet (numbers between a tensor's rows count as its own)."""
+    ends = [t.data_ptr() + (sum((s - 1) * abs(d) for s, d in zip(t.shape, t.stride())) + 1) * t.element_size() for t in (a, b)]
+    return a.data_ptr() < ends[1] and b.data_ptr() < ends[0]
 
 
 def _fp4_quantise(x, step: int, kind: str) -> Fp4:
@@ -2896,8 +2905,9 @@ def _fp4_plan(m: int, n: int, k: int, sms: int, clusters: Tuple[int, ...]) -> Tu
     """How a product is run: x rows of a tile, blocks, and how many of them share a tile's inputs as a cluster (1: none do; 0: pairs of blocks with tiles of 256 outputs).
 
     Up to 128 rows there is one tile for 128 outputs.  Two blocks a multiprocessor walk them, or where there are few, and enough inputs (blocks of 256), a cluster shares a tile:
-    what it costs to add up grows with its columns.  us, whole / shared: 16 rows, 2,560 outputs of 4,096 inputs 5.8 / 4.6 (four blocks), of 9,728 11.6 / 5.9 (eight); 6,144 of 2,560
-    4.8 / 5.0 (two); 64 rows, 2,560 of 4,096 8.5 / 7.4 (four), of 9,728 16.7 / 8.7 (six; eight 9.4), 6,144 of 2,560 6.7 / 7.5; 128 rows 9.8 / 9.8, 18.5 / 11.2 and 8.0 / 9.7.
+    what it costs to add up grows with its columns.  us, whole / shared: 16 rows, 2,560 outputs of 4,096 inputs 6.0 / 4.1 (eight blocks), of 9,728 11.5 / 5.3 (eight); 6,144 of 2,560
+    4.7 / 4.2 (four); 1,024 of 1,024 2.6 / 2.8; 64 rows, 2,560 of 4,096 8.5 / 6.2 (six), of 9,728 16.6 / 8.3 (six; eight 8.7), 6,144 of 2,560 6.6 / 6.5 (five); 128 rows 9.9 / 9.4,
+    18.5 / 11.4 (six; eight 14.5) and 8.0 / 9.4.
 
     Above that the least of three estimates, in us, of a run of the same tiles (128 columns), shared or not, and of pairs with 128, 192 or 256 columns.  They are fits
     to measured times; what they choose takes 0.4 percent longer than the best in the mean of 90 sizes, 7 at the most.  200 rows, 2,560 outputs of 4,096 inputs: 10.0 whole, 9.4 shared, 8.5 pairs of 128; of 9,728 inputs 18.5, 11.7, 14.2; 777 rows, 24,576 of
@@ -2905,8 +2915,8 @@ def _fp4_plan(m: int, n: int, k: int, sms: int, clusters: Tuple[int, ...]) -> Tu
     units, outs = (k + 255) // 256, (n + 127) // 128
     if m <= 128:
         nb = next(b for b in (16, 32, 64, 128) if m <= b)
-        if units >= 16:
-            split = next((s for s in (8, 6, 5, 4, 3, 2) if 4 * s <= units and outs <= clusters[s] and (s <= 6 or nb <= 32)), 1)
+        if units >= (8 if nb <= 32 else 16):
+            split = next((s for s in (8, 6, 5, 4, 3, 2) if 2 * s <= units and outs <= clusters[s] and (s <= 6 or nb <= 32)), 1)
             if split > 1:
                 return nb, outs * split, split
         return nb, min(outs, 2 * sms), 1
@@ -2931,15 +2941,16 @@ def linear_fp4_plan(m: int, n: int, k: int, device: int) -> Tuple[int, int, int]
     return _fp4_plan(m, n, k, *_fp4_room(device))
 
 
-def _fp4_fused(m: int, k: int, kind: str, nb: int, split: int) -> bool:
-    """Whether every block of a product rounds x for itself, which saves a launch: 16 rows and 12 blocks of 256 inputs a block at most (shared memory), and as long as that is
-    quick: a block rounds up to 640 times 16 numbers (``"nv"``, where a row's largest number comes first: 256).  us, in a graph, in a launch of its own / in the product, 2,560 inputs,
-    6,144 outputs: ``"mx"``, 1 row 5.8 / 4.9, 4 rows 5.8 / 5.8, 8 rows 6.0 / 7.3; ``"nv"``, 1 row 6.4 / 5.9, 2 rows 6.4 / 6.8; 9,728 inputs, 2,560 outputs, eight blocks a tile: ``"mx"``,
-    1 row 7.6 / 5.9, 8 rows 7.9 / 7.0, 16 rows 7.9 / 8.5; ``"nv"``, 1 row 8.6 / 7.6, 3 rows 8.4 / 7.7, 8 rows 8.8 / 9.4; with silu in front 1 row 10.5 / 8.2.  On the host 4 us less."""
+def _fp4_fused(m: int, k: int, kind: str, nb: int, split: int, silu: bool = False) -> bool:
+    """Whether every block of a product rounds x for itself, which saves a launch (and 4 us on the host): 16 rows and 12 blocks of 256 inputs a block at most (shared memory), and as long
+    as that is quick: a block rounds up to 900 times 16 numbers; ``"nv"``, where a row's largest number comes first, 320, with
+    silu 640.  us, in a graph, in a launch of its own / in the product: 2,560 inputs, 6,144 outputs, five blocks a tile, ``"mx"`` 1 row 5.3 / 4.3, 16 rows 5.8 / 5.2, ``"nv"`` 5.7 / 5.7 and
+    (12 rows) 6.1 / 6.8; 9,728 inputs, 2,560 outputs, eight blocks a tile, ``"mx"`` 1 row 7.3 / 5.4, 12 rows 7.5 / 7.2, 16 rows 7.5 / 8.1, ``"nv"`` 8.2 / 7.2, 4 rows 8.2 / 7.7, 8 rows 8.4 / 8.8;
+    with silu 1 row 9.8 / 7.5, 8 rows 11.6 / 11.0, 12 rows 11.6 / 12.8; 19,456 outputs of 2,560 inputs, whole tiles, ``"mx"`` 4 rows 8.7 / 8.0, 8 rows 8.8 / 9.6."""
     if m > 16 or nb != 16 or split < 1:
         return False
     own = -(-((k + 255) // 256) // split)
-    return own <= 12 and m * 16 * own <= (256 if kind == "nv" else 640)
+    return own <= 12 and m * 16 * own <= (900 if kind == "mx" else 640 if silu else 320)
 
 
 _fp4_calls = None   # (product, product of rows as they are)
@@ -2951,8 +2962,9 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
 
     ``silu``: ``x`` ``[m, 2 k]`` holds gate columns, then as many others, and the product's operand is ``silu(gate) * other`` (rounding points are ``silu_mul``'s).
 
-    ``pdl``: a programmatic dependent of the launch before it; ``None``: only the product, of its own rounding; ``False``: no launch overlaps another.  Weights are read once the
-    launch in front of the rounding has ended, so they may be as new as that one (with an ``Fp4`` and ``pdl``: older than the launch in front)."""
+    ``pdl``: ``True``, a programmatic dependent of the launch before it: it may ask for weights before that has ended, so they are older than that launch (a weight's first product
+    sees to that itself: it overlaps nothing, so that it may stand right behind ``fp4_quantise``); ``False``: no launch overlaps another; ``None``: only the product its own rounding.
+    Few rows are rounded by the product's blocks (``_fp4_fused``), more in a launch of their own.  ``out`` does not overlap ``x``."""
     global _fp4_calls, launch_count
     _need_fp4(w, "weight")
     k, kind = w.k, w.kind
@@ -2980,6 +2992,8 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
     else:
         _need(out, "out", None, (m, w.n))
         _on_current(out, "out")
+        if not given and m and _overlapping(x, out):
+            raise KernelError("linear_fp4: out and x overlap; some blocks write results while others still read rows")
     out_bf16 = _act(out, "out")
     if m == 0:
         return out
@@ -3003,7 +3017,7 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
         act = torch.empty((m, k), dtype=x.dtype, device=x.device)
         silu_mul(x.contiguous(), act)
         x, step, silu = act, k, False
-    if is_bf16 and (out_bf16 or not silu) and _fp4_fused(m, k, kind, nb, split):
+    if is_bf16 and (out_bf16 or not silu) and _fp4_fused(m, k, kind, nb, split, silu):
         at = held = 0
         overlap = bool(pdl) and not first
     else:

@@ -35,6 +35,7 @@ def test_numbers_that_are_not_rows():
     refused("behind one another", lambda: K.fp4_quantise(torch.zeros(32, 4).t(), "mx"))
     refused("float32 or bfloat16", lambda: K.fp4_quantise(torch.zeros(2, 32, dtype=torch.float16), "mx"))
     refused("tensor", lambda: K.fp4_quantise([[1.0]], "mx"))
+    refused("fewer than", lambda: K.fp4_quantise(torch.zeros(1).expand(2**31, 1), "mx"))
 
 
 def test_tensors_on_the_cpu():

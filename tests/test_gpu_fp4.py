@@ -209,12 +209,12 @@ def test_operands_and_results_of_other_forms(kind):
 
 def test_refusals():
     q = K.fp4_quantise(rows_of(130, 64, BF), "nv")
-    x = rows_of(3, 64, BF)
+    x, square = rows_of(3, 64, BF), rows_of(64, 64, BF)
     for word, call in [("64 numbers", lambda: K.linear_fp4(x[:, :60], q)), ("128 numbers", lambda: K.linear_fp4(x, q, silu=True)), ("Fp4", lambda: K.linear_fp4(x, x)),
                        ("'mx'", lambda: K.linear_fp4(K.fp4_quantise(x, "mx"), q)), ("silu", lambda: K.linear_fp4(K.fp4_quantise(x, "nv"), q, silu=True)),
                        ("float16", lambda: K.linear_fp4(x, q, out_dtype=torch.float16)), ("shape", lambda: K.linear_fp4(x, q, out=torch.empty(3, 129, device="cuda"))),
                        ("contiguous", lambda: K.linear_fp4(x, q, out=torch.empty(130, 3, device="cuda").t())), ("CUDA", lambda: K.linear_fp4(x, q, out=torch.empty(3, 130))),
-                       ("no numbers", lambda: K.fp4_quantise(x[:0], "nv")), ("no numbers", lambda: K.fp4_quantise(x[:, :0], "mx")), ("float16", lambda: K.fp4_expand(q, out_dtype=torch.float16)),
+                       ("overlap", lambda: K.linear_fp4(square, K.fp4_quantise(square, "nv"), out=square)), ("no numbers", lambda: K.fp4_quantise(x[:0], "nv")), ("no numbers", lambda: K.fp4_quantise(x[:, :0], "mx")), ("float16", lambda: K.fp4_expand(q, out_dtype=torch.float16)),
                        ("shape", lambda: K.fp4_expand(q, torch.empty(130, 65, device="cuda"))), ("behind one another", lambda: K.linear_fp4(rows_of(64, 3, BF).t(), q))]:
         with pytest.raises(K.KernelError) as e:
             call()
