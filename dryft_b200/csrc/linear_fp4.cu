@@ -19,6 +19,7 @@
 // copies and products end and frees its tensor memory.
 #include "fp4.cuh"
 #include "drain.h"
+#include <type_traits>
 
 namespace {
 using namespace fp4;
@@ -129,8 +130,8 @@ struct Params {
 };
 
 constexpr int FUSED_ROWS = 16, FUSED_BLOCKS = 12;   // rows, and blocks of 256 inputs, that a block rounds for itself at most
-// What x is: held in 4 bits, or bfloat16 rows that every block rounds for itself (SILU: of gate numbers and as many others).
-enum Source { HELD = 0, BF16 = 1, SILU = 2 };
+// What x is: held in 4 bits, or rows that every block rounds for itself, of bfloat16 (SILU: of gate numbers and as many others) or 32-bit numbers.
+enum Source { HELD = 0, BF16 = 1, SILU = 2, F32 = 3 };
 
 // SPLIT: a tile's inputs are shared out among a cluster's blocks.
 template <int KIND, int NB, bool SPLIT, int SRC> struct Layout {
@@ -201,35 +202,36 @@ template <typename L, int KIND, int SRC, bool SPLIT>
 __device__ __forceinline__ void round_x(const Params& p, int k0, int k1, unsigned char* xs, Most& most_s, unsigned long long* x_full, unsigned rank, unsigned size,
                                         volatile int* failed) {
   typedef typename L::F F;
-  constexpr int THREADS = L::ROUNDERS * 32, AHEAD = 4;
+  typedef typename std::conditional<SRC == F32, float, bf16>::type X;
+  constexpr int THREADS = L::ROUNDERS * 32, AHEAD = SRC == F32 ? 2 : 4;
   const int id = threadIdx.x - 64, lane = threadIdx.x & 31, own = (k1 - k0) * BLOCK_UNITS, all = p.m * own;
-  const bf16* const x = reinterpret_cast<const bf16*>(p.x);
+  const X* const x = reinterpret_cast<const X*>(p.x);
   // i / n, for i + 1/2 and n far below 2^23
   auto over = [](int i, float by) { return (int)(((float)i + 0.5f) * by); };
   const float by_own = 1.f / (float)own;
-  auto load = [&](int i, int row) { return load_unit<bf16, SRC == SILU>(x + row * p.x_stride, (k0 * BLOCK_UNITS + i - row * own) * UNIT, p.k, p.x_words); };
-  auto take = [&](Raw<bf16> (&r)[AHEAD], int base) {
+  auto load = [&](int i, int row) { return load_unit<X, SRC == SILU>(x + row * p.x_stride, (k0 * BLOCK_UNITS + i - row * own) * UNIT, p.k, p.x_words); };
+  auto take = [&](Raw<X> (&r)[AHEAD], int base) {
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j)
       if (base + j * THREADS + id < all) r[j] = load(base + j * THREADS + id, over(base + j * THREADS + id, by_own));
   };
-  Raw<bf16> r[AHEAD] = {};
+  Raw<X> r[AHEAD] = {};
   take(r, 0);
   if (KIND == NV) {
-    auto look = [&](const Raw<bf16>& r, bool there, int row) {   // sixteen neighbouring lanes have one row's
+    auto look = [&](const Raw<X>& r, bool there, int row) {   // sixteen neighbouring lanes have one row's
       unsigned most = there ? size_of(r).most : 0u;
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
       if (there && lane % BLOCK_UNITS == 0) atomicMax(&most_s.rows[row], most);
     };
-    auto look_all = [&](const Raw<bf16> (&r)[AHEAD], int base) {
+    auto look_all = [&](const Raw<X> (&r)[AHEAD], int base) {
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j)
         if (base + j * THREADS < all) look(r[j], base + j * THREADS + id < all, over(base + j * THREADS + id, by_own));
     };
     look_all(r, 0);
     for (int base = AHEAD * THREADS; base < all; base += AHEAD * THREADS) {
-      Raw<bf16> o[AHEAD] = {};
+      Raw<X> o[AHEAD] = {};
       take(o, base);
       look_all(o, base);
     }
@@ -854,7 +856,12 @@ template <int KIND, typename O> int by_split(const Params& p, int nb, int blocks
   if (split == 0) return run_pairs<KIND, O>(p, nb, blocks, dependent, st);
   return split > 1 ? by_rows<KIND, true, O>(p, nb, blocks, split, dependent, st) : by_rows<KIND, false, O>(p, nb, blocks, split, dependent, st);
 }
-template <int KIND, typename O> int by_source(const Params& p, bool silu, int blocks, int split, bool dependent, cudaStream_t st) {
+template <int KIND, typename O> int by_source(const Params& p, bool is_bf16, bool silu, int blocks, int split, bool dependent, cudaStream_t st) {
+  if (!is_bf16) {
+    if constexpr (sizeof(O) == 4)
+      return split > 1 ? run<KIND, FUSED_ROWS, true, F32, O>(p, blocks, split, dependent, st) : run<KIND, FUSED_ROWS, false, F32, O>(p, blocks, split, dependent, st);
+    return DRYFT_ERR_UNSUPPORTED;
+  }
   if (!silu) return split > 1 ? run<KIND, FUSED_ROWS, true, BF16, O>(p, blocks, split, dependent, st) : run<KIND, FUSED_ROWS, false, BF16, O>(p, blocks, split, dependent, st);
   if constexpr (sizeof(O) == 2)
     return split > 1 ? run<KIND, FUSED_ROWS, true, SILU, O>(p, blocks, split, dependent, st) : run<KIND, FUSED_ROWS, false, SILU, O>(p, blocks, split, dependent, st);
@@ -897,20 +904,21 @@ DRYFT_API int dryft_linear_fp4(int kind, int out_bf16, const void* x, const void
 }
 
 // The same of x as it is: `stride` numbers between its rows (silu: of 2 k numbers, as for dryft_fp4_quantise).  scratch: its form in 4 bits, then (NV) its rows' factors, `factors_at` bytes on.  pdl: 1, the rounding is a programmatic
-// dependent of the launch before it; 2, the product is one of the rounding.  scratch null: one launch, every block of which rounds x for itself (bfloat16, up to 16 rows, nb = 16, up to 12
-// blocks of 256 inputs a block; silu: to bfloat16 results).
+// dependent of the launch before it; 2, the product is one of the rounding.  scratch null: one launch, every block of which rounds x for itself (up to 16 rows, nb = 16, up to 12 blocks
+// of 256 inputs a block; bfloat16, with silu to bfloat16 results, or 32-bit numbers without, to 32-bit results).
 DRYFT_API int dryft_linear_fp4_rows(int kind, int is_bf16, int silu, int out_bf16, const void* x, long long stride, const void* w, const void* w_factors, void* y, int m, int n, int k,
                                     int nb, int blocks, int split, unsigned char* scratch, long long factors_at, int pdl, int* err, void* stream) {
   if (m <= 0 || n <= 0) return 0;
   if (!scratch) {   // rounded by the product's own blocks
     const int kb = blocks_of(k);
-    if (!is_bf16 || m > FUSED_ROWS || nb != FUSED_ROWS || split < 1 || split > MOST_BLOCKS || split > kb || (kb + split - 1) / split > FUSED_BLOCKS || (silu && !out_bf16))
+    if ((!is_bf16 && (silu || out_bf16)) || m > FUSED_ROWS || nb != FUSED_ROWS || split < 1 || split > MOST_BLOCKS || split > kb || (kb + split - 1) / split > FUSED_BLOCKS || (silu && !out_bf16))
       return DRYFT_ERR_UNSUPPORTED;
     const Params p = {(const unsigned char*)x, (const unsigned char*)w, nullptr, (const float*)w_factors, y, err, m, n, kb, k, stride,
-                      ((uintptr_t)x & 15) == 0 && (m == 1 || stride % 8 == 0) && (!silu || k % 8 == 0)};
+                      ((uintptr_t)x & 15) == 0 && (m == 1 || stride * (is_bf16 ? 2 : 4) % 16 == 0) && (!silu || k % 8 == 0)};
     const cudaStream_t st = (cudaStream_t)stream;
-    if (kind == NV) return out_bf16 ? by_source<NV, bf16>(p, silu, blocks, split, pdl & 1, st) : by_source<NV, float>(p, silu, blocks, split, pdl & 1, st);
-    return out_bf16 ? by_source<MX, bf16>(p, silu, blocks, split, pdl & 1, st) : by_source<MX, float>(p, silu, blocks, split, pdl & 1, st);
+    const bool ahead = pdl & 1;
+    if (kind == NV) return out_bf16 ? by_source<NV, bf16>(p, is_bf16, silu, blocks, split, ahead, st) : by_source<NV, float>(p, is_bf16, silu, blocks, split, ahead, st);
+    return out_bf16 ? by_source<MX, bf16>(p, is_bf16, silu, blocks, split, ahead, st) : by_source<MX, float>(p, is_bf16, silu, blocks, split, ahead, st);
   }
   const int rc = dryft_fp4_quantise(is_bf16, kind, silu, x, stride, scratch, scratch + factors_at, m, k, pdl, stream);
   if (rc) return rc;

@@ -2818,18 +2818,23 @@ class Fp4:
         return Fp4(self.held[first // 128:(end + 127) // 128], None if self.factors is None else self.factors[first:end], end - first, self.k, self.kind)
 
 
-def _on_current(t, name: str) -> None:
-    """Launches go to the current device's stream: what they read and write is there."""
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)   # (of a process that has a tensor on a device: nothing is left to be begun)
+
+
+def _on_current(t, name: str) -> int:
+    """Launches go to the current device's stream: what they read and write is there.  The device's number."""
     if not t.is_cuda:
         raise KernelError(f"{name}: is on {t.device}; dryft_b200 kernels run on a CUDA device only")
-    if t.get_device() != torch.cuda.current_device():
-        raise KernelError(f"{name}: is on {t.device}, and the current device is cuda:{torch.cuda.current_device()}")
+    at = t.get_device()
+    if at != _current_device():
+        raise KernelError(f"{name}: is on {t.device}, and the current device is cuda:{_current_device()}")
+    return at
 
 
-def _need_fp4(w, name: str) -> None:
+def _need_fp4(w, name: str) -> int:
     if not isinstance(w, Fp4):
         raise KernelError(f"{name}: expected an Fp4 (fp4_quantise makes one), got {type(w).__name__}")
-    _on_current(w.held, name)
+    return _on_current(w.held, name)
 
 
 def _fp4_rows(x, name: str) -> int:
@@ -2837,13 +2842,14 @@ def _fp4_rows(x, name: str) -> int:
     if not isinstance(x, torch.Tensor):
         raise KernelError(f"{name}: expected a tensor, got {type(x).__name__}")
     _act(x, name)
-    if x.dim() != 2:
-        raise KernelError(f"{name}: expected rows of numbers, got shape {tuple(x.shape)}")
+    shape = x.shape
+    if len(shape) != 2:
+        raise KernelError(f"{name}: expected rows of numbers, got shape {tuple(shape)}")
     step, one = x.stride()
-    if one != 1 and x.shape[1] > 1:
+    if one != 1 and shape[1] > 1:
         raise KernelError(f"{name}: the numbers of a row lie behind one another (strides {x.stride()})")
-    if max(x.shape) >= _FP4_MOST:
-        raise KernelError(f"{name}: rows, and numbers of a row, are fewer than {_FP4_MOST}, got {tuple(x.shape)}")
+    if shape[0] >= _FP4_MOST or shape[1] >= _FP4_MOST:
+        raise KernelError(f"{name}: rows, and numbers of a row, are fewer than {_FP4_MOST}, got {tuple(shape)}")
     _on_current(x, name)
     return step
 
@@ -2854,25 +2860,25 @@ def _overlapping(a, b) -> bool:
     return a.data_ptr() < ends[1] and b.data_ptr() < ends[0]
 
 
-def _fp4_quantise(x, step: int, kind: str) -> Fp4:
-    m, k = x.shape
-    held = torch.empty(_fp4_shape(m, k, kind), dtype=torch.uint8, device=x.device)
-    factors = None if kind == "mx" else torch.empty(m, dtype=torch.float32, device=x.device)
-    _ok(fp4_lib().dryft_fp4_quantise(x.dtype == torch.bfloat16, FP4_KINDS[kind], False, x.data_ptr(), step, held.data_ptr(), _ptr(factors), m, k, False, _stream()), "fp4_quantise")
-    q = object.__new__(Fp4)   # what __post_init__ looks at is so by construction
-    q.__dict__.update(held=held, factors=factors, n=m, k=k, kind=kind, read=[])
-    return q
-
-
 def fp4_quantise(x, kind: str) -> Fp4:
     """``x`` ``[rows, k]`` (float32 or bfloat16, rows any distance apart) in microscaled 4-bit floating point: ``"mx"``, groups of 32 numbers with a power of two as their
     scale, or ``"nv"``, groups of 16 with an 8-bit float and a 32-bit factor for each row.  Any ``k``; a last group may be short.  A group with an infinity or a NaN stands for NaN.
     For weights, once, when they are loaded, and for activations that several products read."""
-    _fp4_kind(kind)
+    global launch_count
+    code = _fp4_kind(kind)
     step = _fp4_rows(x, "x")
-    if x.shape[0] == 0 or x.shape[1] == 0:
+    m, k = x.shape
+    if m == 0 or k == 0:
         raise KernelError(f"fp4_quantise: no numbers in {tuple(x.shape)}")
-    return _fp4_quantise(x, step, kind)
+    held = x.new_empty(_fp4_shape(m, k, kind), dtype=torch.uint8)
+    factors = x.new_empty(m, dtype=torch.float32) if code else None
+    rc = fp4_lib().dryft_fp4_quantise(x.dtype is torch.bfloat16, code, False, x.data_ptr(), step, held.data_ptr(), 0 if factors is None else factors.data_ptr(), m, k, False, _stream())
+    if rc:
+        _ok(rc, "fp4_quantise")
+    launch_count += 1
+    q = object.__new__(Fp4)   # what __post_init__ looks at is so by construction
+    q.__dict__.update(held=held, factors=factors, n=m, k=k, kind=kind, read=[])
+    return q
 
 
 def fp4_expand(q: Fp4, out=None, out_dtype=torch.bfloat16):
@@ -2966,8 +2972,8 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
     sees to that itself: it overlaps nothing, so that it may stand right behind ``fp4_quantise``); ``False``: no launch overlaps another; ``None``: only the product its own rounding.
     Few rows are rounded by the product's blocks (``_fp4_fused``), more in a launch of their own.  ``out`` does not overlap ``x``."""
     global _fp4_calls, launch_count
-    _need_fp4(w, "weight")
-    k, kind = w.k, w.kind
+    device = _need_fp4(w, "weight")
+    n, k, kind = w.n, w.k, w.kind
     given = isinstance(x, Fp4)
     if given:
         _need_fp4(x, "x")
@@ -2975,7 +2981,7 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
             raise KernelError("linear_fp4: silu is taken of float32 or bfloat16 activations")
         if x.kind != kind:
             raise KernelError(f"linear_fp4: x is held as {x.kind!r}, the weight as {kind!r}")
-        m, width, is_bf16 = x.n, x.k, 1
+        m, width, is_bf16 = x.n, x.k, True
     else:
         step = _fp4_rows(x, "x")
         m, width = x.shape
@@ -2983,32 +2989,37 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
     if width != (2 * k if silu else k):
         raise KernelError(f"linear_fp4: rows of {2 * k if silu else k} numbers go with a weight {w.shape}, got {width}")
     if out is None:
-        if out_dtype is not None and out_dtype not in (torch.float32, torch.bfloat16):
-            raise KernelError(f"linear_fp4: results are float32 or bfloat16, got {out_dtype}")
-        if given or (out_dtype is not None and out_dtype is not x.dtype):
-            out = torch.empty((m, w.n), dtype=out_dtype or torch.bfloat16, device=w.device)
+        out_bf16 = is_bf16
+        if out_dtype is not None:
+            out_bf16 = out_dtype is torch.bfloat16
+            if not out_bf16 and out_dtype is not torch.float32:
+                raise KernelError(f"linear_fp4: results are float32 or bfloat16, got {out_dtype}")
+        if given or out_bf16 != is_bf16:
+            out = torch.empty((m, n), dtype=torch.bfloat16 if out_bf16 else torch.float32, device=w.held.device)
         else:
-            out = x.new_empty((m, w.n))
+            out = x.new_empty((m, n))
     else:
-        _need(out, "out", None, (m, w.n))
+        _need(out, "out", None, (m, n))
         _on_current(out, "out")
+        out_bf16 = bool(_act(out, "out"))
         if not given and m and _overlapping(x, out):
             raise KernelError("linear_fp4: out and x overlap; some blocks write results while others still read rows")
-    out_bf16 = _act(out, "out")
     if m == 0:
         return out
     if _fp4_calls is None:
         lib = fp4_lib()
         _fp4_calls = (lib.dryft_linear_fp4, lib.dryft_linear_fp4_rows)
-    nb, blocks, split = linear_fp4_plan(m, w.n, k, w.held.get_device())
-    factors = w.factors.data_ptr() if w.factors is not None else 0
-    err = error_flag(w.device).data_ptr()
+    nb, blocks, split = linear_fp4_plan(m, n, k, device)
+    flag = _error_flags.get(device)
+    err = (error_flag(w.held.device) if flag is None else flag).data_ptr()
+    factors = 0 if w.factors is None else w.factors.data_ptr()
+    stream = _stream() if _raw_stream is None else _raw_stream(device)
     first = not w.read
     if first:
         w.read.append(True)
     if given:
-        rc = _fp4_calls[0](FP4_KINDS[kind], out_bf16, x.held.data_ptr(), 0 if x.factors is None else x.factors.data_ptr(), w.held.data_ptr(), factors, out.data_ptr(), m, w.n, k,
-                           nb, blocks, split, bool(pdl) and not first, err, _stream())
+        rc = _fp4_calls[0](FP4_KINDS[kind], out_bf16, x.held.data_ptr(), 0 if x.factors is None else x.factors.data_ptr(), w.held.data_ptr(), factors, out.data_ptr(), m, n, k,
+                           nb, blocks, split, bool(pdl) and not first, err, stream)
         if rc:
             _ok(rc, "linear_fp4")
         launch_count += 1
@@ -3017,19 +3028,20 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
         act = torch.empty((m, k), dtype=x.dtype, device=x.device)
         silu_mul(x.contiguous(), act)
         x, step, silu = act, k, False
-    if is_bf16 and (out_bf16 or not silu) and _fp4_fused(m, k, kind, nb, split, silu):
+    if (out_bf16 or not silu if is_bf16 else not out_bf16) and _fp4_fused(m, k, kind, nb, split, silu):
         at = held = 0
         overlap = bool(pdl) and not first
+        launches = 1
     else:
         rows, wide, size = _fp4_shape(m, k, kind)
         held = rows * wide * size
         scratch = w.held.new_empty(held + 4 * m)
-        at, overlap = scratch.data_ptr(), _overlap(pdl)
-    rc = _fp4_calls[1](FP4_KINDS[kind], is_bf16, silu, out_bf16, x.data_ptr(), step, w.held.data_ptr(), factors, out.data_ptr(), m, w.n, k, nb, blocks, split, at, held, overlap,
-                       err, _stream())
+        at, overlap, launches = scratch.data_ptr(), _overlap(pdl), 2
+    rc = _fp4_calls[1](FP4_KINDS[kind], is_bf16, silu, out_bf16, x.data_ptr(), step, w.held.data_ptr(), factors, out.data_ptr(), m, n, k, nb, blocks, split, at, held, overlap, err,
+                       stream)
     if rc:
         _ok(rc, "linear_fp4")
-    launch_count += 2 if at else 1
+    launch_count += launches
     return out
 
 
