@@ -3015,7 +3015,7 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
     factors = 0 if w.factors is None else w.factors.data_ptr()
     stream = _stream() if _raw_stream is None else _raw_stream(device)
     first = not w.read
-    if first:
+    if first and not torch.cuda.is_current_stream_capturing():   # (what is captured has not run)
         w.read.append(True)
     if given:
         rc = _fp4_calls[0](FP4_KINDS[kind], out_bf16, x.held.data_ptr(), 0 if x.factors is None else x.factors.data_ptr(), w.held.data_ptr(), factors, out.data_ptr(), m, n, k,

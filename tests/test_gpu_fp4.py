@@ -271,6 +271,22 @@ def test_a_weight_right_behind_its_rounding():
             assert torch.equal(K.linear_fp4(K.fp4_quantise(x, "mx"), K.fp4_quantise(v, "mx"), pdl=True), y)
 
 
+def test_a_captured_product_is_not_a_weights_first_one():
+    """What is captured has not run: the first product that does run still overlaps nothing."""
+    x, v = rows_of(2, 512, BF), rows_of(256, 512, BF)
+    K.linear_fp4(x, K.fp4_quantise(v, "nv"))     # (loads the kernels)
+    q, s, g = K.fp4_quantise(v, "nv"), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=s):
+        y = K.linear_fp4(x, q, pdl=True)
+    assert not q.read
+    want = K.linear_fp4(x, q, pdl=True)
+    assert q.read
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
+
+
 def test_results_past_32_bits_of_offset():
     m, n, k = 14400, 151936, 64
     x, w = rows_of(m, k, BF), rows_of(n, k, BF)
