@@ -1,6 +1,7 @@
 // y = x w^T with both operands in microscaled 4-bit floating point (fp4.cuh), on the 5th-generation tensor cores, which multiply such numbers and scales as they lie:
 // tcgen05.mma kind::mxf4 (a scale for 32 inputs) and kind::mxf4nvf4 (for 16), 64 inputs an instruction, summed in 32 bits.  A product of two codes is a multiple of 1/4, so what an
-// instruction sums before the scales is exact: with 25,600 inputs results are off by 4e-8 of the whole, 32-bit multiply-adds in order by 4e-7.
+// instruction sums before the scales is exact: of 25,600 inputs, MX results are the definition's in 32 bits, NV results off by 5e-8 of the whole (a product of the same values in 32
+// bits by the library: 8e-7).
 //
 // Computed transposed: a tile is 128 rows of W, on the M side, against NB rows of x (16 to 128, padded to whole sixteens), its sums in tensor memory, a W row a lane: results are written
 // a column at a time, 32 lanes' behind one another.  A stage of the ring is 256 inputs: a block of W and one of x, each one copy of consecutive bytes (the layout is the tensor
@@ -12,7 +13,7 @@
 // 256-row tile of W between them (below).  ops/kernels.py:_fp4_plan chooses, with both sides' figures.
 //
 // What bounds it.  Few rows: W's bytes.  151,936 outputs of 2,560 inputs, 1 row: 33.6 us, 6,500 GB/s, 99% of a copy's rate; with fewer bytes the launch, first bytes and a tile's end: 8 rows,
-// 19,456 of 2,560 (28 MB) 7.2 us where the bytes are 4.1; 1 row, 6,144 of 2,560 4.6 and 1.35.  Many rows: the ring's round trip.  2,048 rows, 24,576 of 4,096: 83 us, 5.0 PFLOP/s, the tensor
+// 19,456 of 2,560 (28 MB) 7.2 us where the bytes are 4.1; 1 row, 6,144 of 2,560 3.8 and 1.35, 2,560 of 9,728 4.8 and 2.1.  Many rows: the ring's round trip.  2,048 rows, 24,576 of 4,096: 83 us, 5.0 PFLOP/s, the tensor
 // pipe 63% busy, L2 42%: five stages of a pair are 190 KB on their way, which return, are multiplied and asked for again in 1.5 us, 0.33 us a stage where its products take 0.27; and a tile's end.
 //
 // Warps: 0 copies, 1 issues, the others read the sums out.  Every wait on a barrier is bounded by a clock; a waiter that gives up raises *err, every role leaves its loop, the block lets its
