@@ -204,7 +204,7 @@ __device__ __forceinline__ void round_x(const Params& p, int k0, int k1, unsigne
                                         volatile int* failed) {
   typedef typename L::F F;
   typedef typename std::conditional<SRC == F32, float, bf16>::type X;
-  constexpr int THREADS = L::ROUNDERS * 32, AHEAD = SRC == F32 ? 2 : 4;
+  constexpr int THREADS = L::ROUNDERS * 32, AHEAD = 2;   // (four: 0.1 to 0.3 us longer for one to four rows, whose instructions a block meets for the first time)
   const int id = threadIdx.x - 64, lane = threadIdx.x & 31, own = (k1 - k0) * BLOCK_UNITS, all = p.m * own;
   const X* const x = reinterpret_cast<const X*>(p.x);
   // i / n, for i + 1/2 and n far below 2^23

@@ -2947,16 +2947,22 @@ def linear_fp4_plan(m: int, n: int, k: int, device: int) -> Tuple[int, int, int]
     return _fp4_plan(m, n, k, *_fp4_room(device))
 
 
-def _fp4_fused(m: int, k: int, kind: str, nb: int, split: int, silu: bool = False) -> bool:
-    """Whether every block of a product rounds x for itself, which saves a launch (and 4 us on the host): 16 rows and 12 blocks of 256 inputs a block at most (shared memory), and as long
-    as that is quick: a block rounds up to 900 times 16 numbers; ``"nv"``, where a row's largest number comes first, 320, with
-    silu 640.  us, in a graph, in a launch of its own / in the product: 2,560 inputs, 6,144 outputs, five blocks a tile, ``"mx"`` 1 row 5.3 / 4.3, 16 rows 5.8 / 5.2, ``"nv"`` 5.7 / 5.7 and
-    (12 rows) 6.1 / 6.8; 9,728 inputs, 2,560 outputs, eight blocks a tile, ``"mx"`` 1 row 7.3 / 5.4, 12 rows 7.5 / 7.2, 16 rows 7.5 / 8.1, ``"nv"`` 8.2 / 7.2, 4 rows 8.2 / 7.7, 8 rows 8.4 / 8.8;
-    with silu 1 row 9.8 / 7.5, 8 rows 11.6 / 11.0, 12 rows 11.6 / 12.8; 19,456 outputs of 2,560 inputs, whole tiles, ``"mx"`` 4 rows 8.7 / 8.0, 8 rows 8.8 / 9.6."""
+def _fp4_fused(m: int, k: int, kind: str, nb: int, split: int, silu: bool = False, captured: bool = False) -> bool:
+    """Whether every block of a product rounds x for itself, which saves a launch: 16 rows and 12 blocks of 256 inputs a block at most (shared memory), and as long as that is quick.
+
+    A launch costs the host 4 us, more than the kernels differ by: a block rounds up to 900 times 16 numbers; ``"nv"``, where a row's largest number comes first, 320, with silu 640.
+    In a captured graph it costs nothing, and runs while the product asks for weights: then 512, with silu 320; ``"nv"`` none, with silu 240.  us, in a graph, in a launch of its own /
+    in the product: 2,560 inputs, 6,144 outputs, five blocks a tile, ``"mx"`` 1 row 6.0 / 5.8, 16 rows 6.6 / 6.7, ``"nv"`` 6.2 / 6.8 and (8 rows) 6.6 / 7.4; 9,728 inputs, 2,560 outputs, eight
+    blocks a tile, ``"mx"`` 1 row 7.9 / 7.2, 6 rows 8.0 / 7.8, 8 rows 8.1 / 8.4, ``"nv"`` 8.8 / 8.4, 4 rows 8.5 / 9.1; with silu ``"mx"`` 1 row 8.7 / 7.6, 4 rows 8.7 / 8.5, 8 rows 8.9 / 10.7, ``"nv"`` 1
+    row 9.7 / 9.0, 4 rows 9.8 / 10.2, 8 rows 10.6 / 12.5; 19,456 outputs of 2,560 inputs, whole tiles, ``"mx"`` 1 row 8.9 / 8.4, 4 rows 9.1 / 9.2, 8 rows 8.8 / 10.7."""
     if m > 16 or nb != 16 or split < 1:
         return False
     own = -(-((k + 255) // 256) // split)
-    return own <= 12 and m * 16 * own <= (900 if kind == "mx" else 640 if silu else 320)
+    if captured:
+        most = (320 if silu else 512) if kind == "mx" else 240 if silu else 0
+    else:
+        most = 900 if kind == "mx" else 640 if silu else 320
+    return own <= 12 and m * 16 * own <= most
 
 
 _fp4_calls = None   # (product, product of rows as they are)
@@ -3028,7 +3034,9 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
         act = torch.empty((m, k), dtype=x.dtype, device=x.device)
         silu_mul(x.contiguous(), act)
         x, step, silu = act, k, False
-    if (out_bf16 or not silu if is_bf16 else not out_bf16) and _fp4_fused(m, k, kind, nb, split, silu):
+    if (out_bf16 or not silu if is_bf16 else not out_bf16) and _fp4_fused(
+        m, k, kind, nb, split, silu, pdl is True and torch.cuda.is_current_stream_capturing()
+    ):
         at = held = 0
         overlap = bool(pdl) and not first
         launches = 1

@@ -28,7 +28,7 @@ def test_every_plan_is_one_that_the_launcher_takes(seed, sms, clusters):
             assert blocks == tiles * split if split > 1 else 0 < blocks <= tiles
             assert split == 1 or tiles <= clusters[split]   # all at once
         for kind in K.FP4_KINDS:
-            if K._fp4_fused(m, k, kind, nb, split):
+            if K._fp4_fused(m, k, kind, nb, split) or K._fp4_fused(m, k, kind, nb, split, True, True):
                 assert m <= 16 and nb == 16 and split >= 1 and -(-units // split) <= 12
 
 

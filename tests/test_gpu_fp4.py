@@ -287,6 +287,27 @@ def test_a_captured_product_is_not_a_weights_first_one():
     assert torch.equal(y, want)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("silu", [False, True])
+@pytest.mark.parametrize("n,k", [(300, 2560), (1000, 600)])
+def test_captured_products_of_few_rows(kind, silu, n, k):
+    """Rounded in the product or in a launch of its own, which a captured call chooses otherwise than an eager one, results have the same bits."""
+    q = K.fp4_quantise(rows_of(n, k, BF), kind)
+    xs = [rows_of(m, 2 * k if silu else k, BF) for m in (1, 2, 3, 4, 6, 8, 11, 16)]
+    want = [K.linear_fp4(x, q, silu=silu) for x in xs]
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=s):
+        got = [K.linear_fp4(x, q, silu=silu, pdl=True) for x in xs]
+    for _ in range(3):
+        for y in got:
+            y.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, v) for y, v in zip(got, want))
+    K.check_error_flags()
+
+
 def test_results_past_32_bits_of_offset():
     m, n, k = 14400, 151936, 64
     x, w = rows_of(m, k, BF), rows_of(n, k, BF)
