@@ -6,24 +6,24 @@ using namespace fp4;
 typedef __nv_bfloat16 bf16;
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 
-// A row is 1, 2, 4 or 8 warps' (`span` lanes); a lane has HELD units in registers at a time, `span` apart.  NV wants the row's largest number first: a row that is held whole
-// (bfloat16: up to 12,288 numbers) is read once.  Its blocks wait for their rows' first numbers, then for each other's maxima: four of them a multiprocessor, with three units a
-// lane, hide more of that than two with four (2,000 rows of 9,728: 15.6 us and 17.8; of 2,560: 6.4 and 7.6).
+// A row is 1 to 32 warps' (`span` lanes); a lane has HELD units in registers at a time, `span` apart.  NV wants the row's largest number first: a row that is held whole
+// (bfloat16, 256 lanes: up to 12,288 numbers) is read once.  Its blocks wait for their rows' first numbers, then for each other's maxima: 1,024 threads a multiprocessor, of 64 registers,
+// hide more of that than fewer with more in them (2,000 rows of 9,728, NV: 15.6 us and 17.8, MX with silu 25.6 and 35.9, of 2,560 32-bit numbers, NV, 9.1 and 12.0).
 //
-// What bounds it: 2,000 rows of 9,728 in bfloat16 (39 MB read, 10 or 11 written: 7.5 us at a copy's rate) take MX 12.1 us, NV 15.7.  Issue slots are two thirds full (8.0 and 10.6 million
+// What bounds it: 2,000 rows of 9,728 in bfloat16 (39 MB read, 10 or 11 written: 7.5 us at a copy's rate) take MX 12.0 us, NV 15.6.  Issue slots are two thirds full (8.0 and 10.6 million
 // instructions of a warp: 13 and 17 for a number of each lane), and a block's rows come first, then are worked on.  Blocks of 512 or 1,024 threads and roundings in packed bfloat16 were
 // no faster.
 template <typename T, int KIND> __host__ __device__ constexpr int held_units() { return sizeof(T) == 4 ? 2 : KIND == NV ? 3 : 4; }
 // WORDS: rows begin on 16-byte boundaries (silu: both halves of them).
+constexpr int MOST_LANES = 1024;
 template <typename T, int KIND, bool SILU, bool WORDS>
-__global__ void __launch_bounds__(THREADS, WORDS && sizeof(T) == 2 && KIND == NV ? 4 : 1) fp4_quantise_kernel(const T* x, long long stride, unsigned char* held, float* factors,
-                                                                                                              int rows, int k, int span, bool signal) {
+__global__ void __launch_bounds__(WORDS ? MOST_LANES : THREADS, 1) fp4_quantise_kernel(const T* x, long long stride, unsigned char* held, float* factors, int rows, int k, int span, bool signal) {
   typedef Format<KIND> F;
   constexpr int HELD = held_units<T, KIND>();
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (signal) let_next_launch_in();   // (behind the wait: what comes in may rely on all that was written before this launch)
-  __shared__ unsigned most_s[WARPS];
-  const int at = threadIdx.x & (span - 1), row = blockIdx.x * (THREADS / span) + threadIdx.x / span, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ unsigned most_s[MOST_LANES / 32];
+  const int at = threadIdx.x & (span - 1), row = blockIdx.x * (blockDim.x / span) + threadIdx.x / span, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int units = row < rows ? blocks_of(k) * BLOCK_UNITS : 0;   // (a warp is one row's)
   const T* const from = x + (row < rows ? row : 0) * stride;
   auto take = [&](Raw<T> (&r)[HELD], int base) {
@@ -199,10 +199,10 @@ template <typename O, int KIND> __global__ void __launch_bounds__(THREADS) fp4_e
   }
 }
 
-template <typename... P, typename... A> int launch(void (*kern)(P...), dim3 blocks, bool dependent, cudaStream_t st, A... a) {
+template <typename... P, typename... A> int launch(void (*kern)(P...), dim3 blocks, int threads, bool dependent, cudaStream_t st, A... a) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = blocks;
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(threads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -223,12 +223,18 @@ DRYFT_API int dryft_fp4_quantise(int is_bf16, int kind, int silu, const void* x,
   const int item = is_bf16 ? 2 : 4, held_at_a_time = !is_bf16 ? held_units<float, NV>() : kind == NV ? held_units<bf16, NV>() : held_units<bf16, MX>();
   const bool words = ((uintptr_t)x & 15) == 0 && (rows == 1 || stride * item % 16 == 0) && (!silu || (long long)k * item % 16 == 0);
   const int units = blocks_of(k) * BLOCK_UNITS;
-  // lanes of a row: as many as hold it, or of few rows as many as it has units for (a row's latency is then what counts)
+  // Lanes of a row: as many as hold it, or of few rows as many as it has units for (a row's latency is then what counts): up to 256, from where on NV's maxima cost more than units side by
+  // side give (48 rows of 9,728: 3.0 us with 256 lanes, 3.7 with 1,024; MX 2.35 and 2.42, but with silu 4.0 and 3.6).  More than 256: for rows that have a multiprocessor each (25,600 numbers of NV 6.0 and
+  // 4.6, with silu 16.0 and 8.3, of MX 4.0 and 3.2), or where NV would work out a row's numbers, or read 32 bits of each, twice (2,000 rows of 25,600, silu: 90 and with 512 lanes 83, 32-bit
+  // numbers 82 and 76; bfloat16 as it is 38 and 44).
+  const bool few = rows <= 148;
+  const int most = !words ? THREADS : few ? MOST_LANES : kind == NV && (silu || !is_bf16) ? 512 : THREADS;
   int span = 32;
-  while (span < THREADS && span * (rows <= 512 ? 1 : held_at_a_time) < units) span *= 2;
-  const unsigned blocks = (unsigned)((rows + (long long)(THREADS / span) - 1) / (THREADS / span));
+  while (span < most && span * ((few && kind == MX && (silu || !is_bf16)) || (rows <= 512 && span < THREADS) ? 1 : held_at_a_time) < units) span *= 2;
+  const int threads = span > THREADS ? span : THREADS;
+  const unsigned blocks = (unsigned)((rows + (long long)(threads / span) - 1) / (threads / span));
   const cudaStream_t st = (cudaStream_t)stream;
-  auto run = [&](auto kern, auto* p) { return launch(kern, blocks, pdl & 1, st, p, stride, (unsigned char*)held, (float*)factors, rows, k, span, (pdl & 2) != 0); };
+  auto run = [&](auto kern, auto* p) { return launch(kern, blocks, threads, pdl & 1, st, p, stride, (unsigned char*)held, (float*)factors, rows, k, span, (pdl & 2) != 0); };
   auto by_words = [&](auto with, auto without, auto* p) { return words ? run(with, p) : run(without, p); };
   const bf16* const xb = (const bf16*)x;
   const float* const xf = (const float*)x;
@@ -249,8 +255,8 @@ DRYFT_API int dryft_fp4_expand(int is_bf16, int kind, const void* held, const vo
   const long long blocks = (long long)((rows + ROWS - 1) / ROWS) * blocks_of(k);
   if (blocks > 0x7fffffffll) return DRYFT_ERR_UNSUPPORTED;
   const cudaStream_t st = (cudaStream_t)stream;
-  auto run = [&](auto kern, auto* p) { return launch(kern, (unsigned)blocks, false, st, (const unsigned char*)held, (const float*)factors, p, rows, k); };
-  auto shifted = [&](auto kern, auto* p) { return launch(kern, dim3((unsigned)blocks, ROWS / (WARPS * SHIFTED_ROWS)), false, st, (const unsigned char*)held, (const float*)factors, p, rows, k); };
+  auto run = [&](auto kern, auto* p) { return launch(kern, (unsigned)blocks, THREADS, false, st, (const unsigned char*)held, (const float*)factors, p, rows, k); };
+  auto shifted = [&](auto kern, auto* p) { return launch(kern, dim3((unsigned)blocks, ROWS / (WARPS * SHIFTED_ROWS)), THREADS, false, st, (const unsigned char*)held, (const float*)factors, p, rows, k); };
   if (!words && is_bf16) return kind == NV ? shifted(fp4_expand_shifted_kernel<bf16, NV>, (bf16*)out) : shifted(fp4_expand_shifted_kernel<bf16, MX>, (bf16*)out);
   if (!words) return kind == NV ? shifted(fp4_expand_shifted_kernel<float, NV>, (float*)out) : shifted(fp4_expand_shifted_kernel<float, MX>, (float*)out);
   if (is_bf16) return kind == NV ? run(fp4_expand_kernel<bf16, NV>, (bf16*)out) : run(fp4_expand_kernel<bf16, MX>, (bf16*)out);
