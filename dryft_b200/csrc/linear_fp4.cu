@@ -13,8 +13,10 @@
 // 256-row tile of W between them (below).  ops/kernels.py:_fp4_plan chooses, with both sides' figures.
 //
 // What bounds it.  Few rows: W's bytes.  151,936 outputs of 2,560 inputs, 1 row: 33.6 us, 6,500 GB/s, 99% of a copy's rate; with fewer bytes the launch, first bytes and a tile's end: 8 rows,
-// 19,456 of 2,560 (28 MB) 7.2 us where the bytes are 4.1; 1 row, 6,144 of 2,560 3.8 and 1.35, 2,560 of 9,728 4.8 and 2.1.  Many rows: the ring's round trip.  2,048 rows, 24,576 of 4,096: 83 us, 5.0 PFLOP/s, the tensor
-// pipe 63% busy, L2 42%: five stages of a pair are 190 KB on their way, which return, are multiplied and asked for again in 1.5 us, 0.33 us a stage where its products take 0.27; and a tile's end.
+// 19,456 of 2,560 (28 MB) 7.2 us where the bytes are 4.1; 1 row, 6,144 of 2,560 3.8 and 1.35, 2,560 of 9,728 4.8 and 2.1.  Many rows: what
+// enters a multiprocessor.  2,048 rows, 5,120 of 25,600 (pairs with 192 columns): NV 103 us, MX 91.5, 5.9 PFLOP/s, 104 GB/s into each, 15 TB/s in all; 24,576 of 4,096 (256
+// columns): 83 us, 5.0 PFLOP/s, and 75.5.  MX has 0.91 and 0.92 of NV's bytes, takes 0.89 and 0.91 of its time, and has the same products; the tensor pipe is 62% busy.  Larger tiles would
+// read less for as much work, but tensor memory is full.
 //
 // Warps: 0 copies, 1 issues, the others read the sums out.  Every wait on a barrier is bounded by a clock; a waiter that gives up raises *err, every role leaves its loop, the block lets its
 // copies and products end and frees its tensor memory.

@@ -72,6 +72,46 @@ def test_rounding_of_rare_rows(kind, dtype, k):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("m,k", [(3, 25600), (148, 13000), (149, 20000), (520, 12304)])
+def test_rounding_of_wide_rows(kind, dtype, m, k):
+    """Rows that more lanes hold than one block of the usual size has, and rows that no lanes hold; the largest number of a row may lie anywhere."""
+    x = rows_of(m, k, dtype)
+    for r in range(m):
+        x[r, (r * 7919) % k] = 1000.0
+    same_values(K.fp4_expand(K.fp4_quantise(x, kind), out_dtype=F32), P.values(x, kind), F32)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m,k", [(2, 25600), (150, 9728), (520, 12304)])
+def test_silu_of_wide_rows(kind, m, k):
+    """As of the same numbers by `silu_mul`, which has the same bits where both read 16-byte words."""
+    x, q = rows_of(m, 2 * k, BF), K.fp4_quantise(rows_of(130, k, BF), kind)
+    act = torch.empty(m, k, dtype=BF, device="cuda")
+    K.silu_mul(x, act)
+    assert torch.equal(K.linear_fp4(x, q, silu=True), K.linear_fp4(act, q))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_rounding_of_signs_and_of_the_smallest_numbers(kind, dtype):
+    """Infinities and NaN of either sign make their group NaN, and no other; zeros of either sign, numbers without leading bits, negative ones that are the largest of their group."""
+    bits, finite = (torch.int16, 0x7f80) if dtype == BF else (torch.int32, 0x7f800000)
+    x = rows_of(9, 160, dtype)
+    raw = x.view(bits)
+    sign = -(1 << (15 if dtype == BF else 31))
+    raw[0, 40], raw[1, 40], raw[2, 40], raw[3, 40] = finite, finite + 1, finite + sign, finite + 1 + sign
+    raw[4, ::2], raw[4, 1::2] = sign, 0
+    raw[5] = torch.arange(160, device="cuda").to(bits)              # subnormal numbers
+    raw[6] = torch.arange(160, device="cuda").to(bits) + sign
+    x[7, ::16], x[8, 1::32] = -100.0, -3.0e38
+    got = K.fp4_expand(K.fp4_quantise(x, kind), out_dtype=F32)
+    want = P.values(x, kind)
+    same_values(got, want, F32)
+    assert [int(r.isnan().sum()) for r in got] == [P.GROUP[kind]] * 4 + [0] * 5
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("m,n,k", [(1, 128, 64), (1, 128, 256), (2, 256, 5120), (16, 300, 4100), (13, 129, 9728), (16, 128, 512), (5, 389, 83), (17, 200, 1000), (33, 130, 300), (100, 256, 2560), (129, 128, 256), (257, 300, 777),
                                    (700, 384, 320), (8, 40000, 320)])
 def test_products(kind, m, n, k):
