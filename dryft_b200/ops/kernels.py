@@ -2774,7 +2774,7 @@ class Fp4:
     n: int
     k: int
     kind: str
-    # Whether a product has read this one as its weight.  The first one is no programmatic dependent of the launch before it, which may be what wrote this.
+    # Whether a product that may be a programmatic dependent of the launch before it has read this one as its weight.  The first one is not: that launch may be what wrote this.
     read: list = field(default_factory=list, init=False, repr=False, compare=False)
 
     def __post_init__(self) -> None:
@@ -2947,6 +2947,7 @@ def linear_fp4_plan(m: int, n: int, k: int, device: int) -> Tuple[int, int, int]
     return _fp4_plan(m, n, k, *_fp4_room(device))
 
 
+@functools.lru_cache(maxsize=4096)
 def _fp4_fused(m: int, k: int, kind: str, nb: int, split: int, silu: bool = False, captured: bool = False) -> bool:
     """Whether every block of a product rounds x for itself, which saves a launch: 16 rows and 12 blocks of 256 inputs a block at most (shared memory), and as long as that is quick.
 
@@ -3020,8 +3021,9 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
     err = (error_flag(w.held.device) if flag is None else flag).data_ptr()
     factors = 0 if w.factors is None else w.factors.data_ptr()
     stream = _stream() if _raw_stream is None else _raw_stream(device)
-    first = not w.read
-    if first and not torch.cuda.is_current_stream_capturing():   # (what is captured has not run)
+    captured = bool(pdl) and torch.cuda.is_current_stream_capturing()
+    first = bool(pdl) and not w.read     # of those that may overlap the launch before them: it does not
+    if first and not captured:           # (what is captured has not run)
         w.read.append(True)
     if given:
         rc = _fp4_calls[0](FP4_KINDS[kind], out_bf16, x.held.data_ptr(), 0 if x.factors is None else x.factors.data_ptr(), w.held.data_ptr(), factors, out.data_ptr(), m, n, k,
@@ -3034,9 +3036,7 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
         act = torch.empty((m, k), dtype=x.dtype, device=x.device)
         silu_mul(x.contiguous(), act)
         x, step, silu = act, k, False
-    if (out_bf16 or not silu if is_bf16 else not out_bf16) and _fp4_fused(
-        m, k, kind, nb, split, silu, pdl is True and torch.cuda.is_current_stream_capturing()
-    ):
+    if (out_bf16 or not silu if is_bf16 else not out_bf16) and _fp4_fused(m, k, kind, nb, split, silu, captured):
         at = held = 0
         overlap = bool(pdl) and not first
         launches = 1
