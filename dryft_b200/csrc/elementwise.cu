@@ -323,10 +323,9 @@ __global__ void silu_mul_kernel(const T* __restrict__ gu, T* __restrict__ y, int
   float s = rnd<T>(g / (1.f + expf(-g)));
   y[i] = from_f32<T>(s * u);
 }
-// g / (1 + exp(-g)): exact division and exponential in the 32-bit path; where the result is rounded to
-// bfloat16 right away, the fast exponential and division (a few ulp of 32-bit) are far inside that rounding
+// g / (1 + exp(-g)): exact division and exponential in the 32-bit path, fast ones where the result is rounded to bfloat16 right away
 template <typename T> __device__ __forceinline__ float silu_f32(float g) { return g / (1.f + expf(-g)); }
-template <> __device__ __forceinline__ float silu_f32<__nv_bfloat16>(float g) { return __fdividef(g, 1.f + __expf(-g)); }
+template <> __device__ __forceinline__ float silu_f32<__nv_bfloat16>(float g) { return silu_fast(g); }
 // 16 bytes of gate and of up per thread (inter a multiple of the vector width)
 template <typename T>
 __global__ void silu_mul_vec_kernel(const T* __restrict__ gu, T* __restrict__ y, int inter, size_t total_vecs) {

@@ -111,10 +111,7 @@ template <typename T, bool SILU, bool SHIFTED = false> __device__ __forceinline_
     for (int i = 0; i < UNIT / 2; ++i) {
       float v[2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float g = number(r, 2 * i + e);
-        v[e] = rnd<__nv_bfloat16>(__fdividef(g, 1.f + __expf(-g))) * number(up, 2 * i + e);   // (a few 32-bit ulp: far inside the rounding to bfloat16)
-      }
+      for (int e = 0; e < 2; ++e) v[e] = rnd<__nv_bfloat16>(silu_fast(number(r, 2 * i + e))) * number(up, 2 * i + e);
       const __nv_bfloat162 two = __floats2bfloat162_rn(v[0], v[1]);
       r.w[i] = *reinterpret_cast<const unsigned*>(&two);
     }
