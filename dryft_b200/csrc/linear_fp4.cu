@@ -378,6 +378,7 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
     const bool issues = elected();
     int s = 0, run = 0;
     unsigned par = 0, buffer = 0;
+    long long left = first_tile < tiles ? (long long)((unsigned)(tiles - first_tile - 1) / (unsigned)step + 1) * (k1 - k0) : 0;   // stages that this block's products take
     bool ok = !FUSED || __all_sync(0xffffffffu, mbar_wait(x_full, 0, p.err, failed, 3));
     for (int t = first_tile; ok && t < tiles; t += step, ++run) {
       const int acc = run % L::ACCS;
@@ -403,9 +404,10 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
             const int word = j * F::WORDS / 4;
             umma<KIND>(d, w + 2 * j, x + 2 * j, idesc<KIND>(KIND == MX ? 2 * (j & 1) : 0) | n_bits, sw + 4 * word, sx + 4 * word, kb > k0 || j > 0);
           }
-          umma_commit(&empty[s]);
+          if (left > STAGES) umma_commit(&empty[s]);   // (where a copy waits for it: nothing is on its way to a block that may have ended)
           if (kb == k1 - 1) umma_commit(&acc_full[acc]);
         }
+        --left;
         __syncwarp();
         buffer ^= 1;
         if (++s == STAGES) {
@@ -689,6 +691,7 @@ template <int KIND, typename O> __global__ void __launch_bounds__(PairLayout<KIN
     const bool issues = elected();
     int s = 0, run = 0;
     unsigned par = 0, buffer = 0;
+    long long left = first_tile < tiles ? (long long)((unsigned)(tiles - first_tile - 1) / (unsigned)step + 1) * KB : 0;   // stages that this pair's products take
     bool ok = true;
     for (int t = first_tile; ok && t < tiles; t += step, ++run) {
       const Tile at = tile_of(t);
@@ -716,9 +719,10 @@ template <int KIND, typename O> __global__ void __launch_bounds__(PairLayout<KIN
             const int word = j * F::WORDS / 4;
             umma<KIND, 2>(d, w + 2 * j, x + 2 * j, idesc<KIND, 256>(KIND == MX ? 2 * (j & 1) : 0) | n_bits, sw + 4 * word, sx + 8 * word + shift, kb > 0 || j > 0);
           }
-          umma_commit_both(&empty[s]);
+          if (left > STAGES) umma_commit_both(&empty[s]);   // (as above)
           if (kb == KB - 1) umma_commit_both(&acc_full[acc]);
         }
+        --left;
         __syncwarp();
         buffer ^= 1;
         if (++s == STAGES) {

@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+import plain_fp4 as P
 from dryft_b200.ops import kernels as K
 from test_gpu_fp4 import near, rows_of
 
@@ -37,3 +38,23 @@ def test_gates_whose_exponential_is_nearly_too_large(kind, m):
     q = K.fp4_quantise(w[:, :k - 1], kind)
     got, want = K.linear_fp4(odd, q, silu=True), K.linear_fp4(act, q)
     assert int((got != want).any(1).sum()) <= 2 and bool(((got.float() - want.float()).norm(dim=1) <= 0.5 * want.float().norm(dim=1)).all())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m", [16, 100, 300])
+def test_stages_that_end_anywhere_in_a_ring(monkeypatch, kind, m):
+    """Fewer inputs than a ring of stages holds, as many, and more; one tile and several to a block."""
+    n = 700
+    for k in (100, 600, 1100, 1300, 1700, 2100, 2900):
+        x, w = rows_of(m, k, BF), rows_of(n, k, BF)
+        q, h = K.fp4_quantise(w, kind), K.fp4_quantise(x, kind)
+        want, terms = P.product(x, w, kind)
+        room = (k / 64 + 10) * 2.0**-21 * terms + 2.0**-22 * want.abs()
+        plans = [(next(b for b in (16, 32, 64, 128) if m <= b or b == 128), blocks, 1) for blocks in (1, 2, 5)]
+        plans += [(nb, blocks, 0) for nb in (128, 192, 256) for blocks in (2, 4) if m > 16]
+        for plan in plans:
+            monkeypatch.setattr(K, "linear_fp4_plan", lambda *a: plan)
+            for operand in (h, x):
+                y = K.linear_fp4(operand, q, out_dtype=F32)
+                assert bool(((y.double().cpu() - want).abs() <= room).all()), (k, plan)
+    K.check_error_flags()
