@@ -3023,13 +3023,13 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
     stream = _stream() if _raw_stream is None else _raw_stream(device)
     captured = bool(pdl) and torch.cuda.is_current_stream_capturing()
     first = bool(pdl) and not w.read     # of those that may overlap the launch before them: it does not
-    if first and not captured:           # (what is captured has not run)
-        w.read.append(True)
     if given:
         rc = _fp4_calls[0](FP4_KINDS[kind], out_bf16, x.held.data_ptr(), 0 if x.factors is None else x.factors.data_ptr(), w.held.data_ptr(), factors, out.data_ptr(), m, n, k,
                            nb, blocks, split, bool(pdl) and not first, err, stream)
         if rc:
             _ok(rc, "linear_fp4")
+        if first and not captured:       # (what is captured has not run)
+            w.read.append(True)
         launch_count += 1
         return out
     if silu and not is_bf16:
@@ -3049,6 +3049,8 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
                        stream)
     if rc:
         _ok(rc, "linear_fp4")
+    if first and not captured:
+        w.read.append(True)
     launch_count += launches
     return out
 

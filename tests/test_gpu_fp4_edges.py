@@ -58,3 +58,58 @@ def test_stages_that_end_anywhere_in_a_ring(monkeypatch, kind, m):
                 y = K.linear_fp4(operand, q, out_dtype=F32)
                 assert bool(((y.double().cpu() - want).abs() <= room).all()), (k, plan)
     K.check_error_flags()
+
+
+class Launchers:
+    """The two launchers of linear_fp4, with what they were asked and, where wanted, an answer of their own."""
+
+    def __init__(self, monkeypatch, rc=None):
+        lib = K.fp4_lib()
+        self.asked, self.rc, self.real = [], rc, (lib.dryft_linear_fp4, lib.dryft_linear_fp4_rows)
+        monkeypatch.setattr(K, "_fp4_calls", (self.of_held, self.of_rows))
+
+    def of_held(self, *a):
+        self.asked.append(("held", int(a[13])))
+        return self.real[0](*a) if self.rc is None else self.rc
+
+    def of_rows(self, *a):
+        self.asked.append(("within" if not a[15] else "apart", int(a[17])))
+        return self.real[1](*a) if self.rc is None else self.rc
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_the_first_product_of_a_weight_overlaps_nothing(monkeypatch, kind):
+    """Asked to overlap the launch before them, products ask for a weight before that has ended: not so the first one of a weight, whose launch before may be what wrote it."""
+    v, x = rows_of(300, 512, BF), rows_of(1, 512, BF)
+    held, seen = K.fp4_quantise(x, kind), Launchers(monkeypatch)
+    for operand in (held, x):
+        q = K.fp4_quantise(v, kind)
+        results = [K.linear_fp4(operand, q, pdl=True) for _ in range(3)]
+        assert [p for _, p in seen.asked] == [0, 1, 1] and {f for f, _ in seen.asked} == {"held" if operand is held else "within"}
+        assert all(torch.equal(r, results[0]) for r in results)
+        seen.asked.clear()
+    # rows that a launch of their own rounds: that one waits for all before itself, and the product is its dependent
+    q = K.fp4_quantise(v, kind)
+    wide = rows_of(60, 512, BF)
+    K.linear_fp4(wide, q, pdl=True), K.linear_fp4(wide, q), K.linear_fp4(wide, q, pdl=False), K.linear_fp4(x, q), K.linear_fp4(x, q, pdl=False)
+    assert seen.asked == [("apart", 3), ("apart", 2), ("apart", 0), ("within", 0), ("within", 0)]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_product_that_failed_is_not_a_weights_first_one(monkeypatch, kind):
+    v, x, wide = rows_of(300, 512, BF), rows_of(1, 512, BF), rows_of(60, 512, BF)
+    for operand in (x, wide, K.fp4_quantise(x, kind)):
+        q = K.fp4_quantise(v, kind)
+        failing = Launchers(monkeypatch, K.UNSUPPORTED)
+        with pytest.raises(K.KernelError):
+            K.linear_fp4(operand, q, pdl=True)
+        assert len(failing.asked) == 1 and not q.read
+        seen = Launchers(monkeypatch)
+        K.linear_fp4(operand, q, pdl=True)
+        assert seen.asked[0][1] == (3 if operand is wide else 0) and q.read
+    # no memory for the rounded rows
+    q = K.fp4_quantise(v, kind)
+    monkeypatch.setattr(K, "_fp4_shape", lambda *a: (1 << 20, 1 << 20, 1 << 20))
+    with pytest.raises(RuntimeError):
+        K.linear_fp4(wide, q, pdl=True)
+    assert not q.read
