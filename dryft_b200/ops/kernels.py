@@ -2793,6 +2793,10 @@ class Fp4:
             if t.device != self.held.device:
                 raise KernelError("Fp4: held and factors are on two devices")
 
+    def __getstate__(self) -> dict:
+        """A copy has memory of its own, which no product has read."""
+        return {**self.__dict__, "read": []}
+
     @property
     def shape(self) -> Tuple[int, int]:
         return (self.n, self.k)
