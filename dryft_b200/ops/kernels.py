@@ -2774,7 +2774,8 @@ class Fp4:
     n: int
     k: int
     kind: str
-    # Whether a product that may be a programmatic dependent of the launch before it has read this one as its weight.  The first one is not: that launch may be what wrote this.
+    # Whether a product that may be a programmatic dependent of the launch before it has read this one as its weight.  The first one is not: that launch may be what wrote this.  Ranges of
+    # rows have it in common.
     read: list = field(default_factory=list, init=False, repr=False, compare=False)
 
     def __post_init__(self) -> None:
@@ -2819,7 +2820,9 @@ class Fp4:
         first, end, _ = at.indices(self.n)
         if first % 128 or not first < end:
             raise KernelError(f"Fp4: rows {first}..{end} of {self.n}; the first is a multiple of 128")
-        return Fp4(self.held[first // 128:(end + 127) // 128], None if self.factors is None else self.factors[first:end], end - first, self.k, self.kind)
+        part = Fp4(self.held[first // 128:(end + 127) // 128], None if self.factors is None else self.factors[first:end], end - first, self.k, self.kind)
+        part.__dict__["read"] = self.read   # (the same memory, written by the same rounding)
+        return part
 
 
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)   # (of a process that has a tensor on a device: nothing is left to be begun)

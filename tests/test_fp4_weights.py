@@ -25,3 +25,13 @@ def test_a_copy_is_a_matrix_that_no_product_has_read(kind):
         other.read.append(True)
         assert len(w.read) == 1
         assert (other.shape, other.kind) == (w.shape, kind) and torch.equal(other.held, w.held) and (other.factors is None) == (kind == "mx")
+
+
+def test_ranges_of_rows_have_it_in_common_whether_a_product_has_read_them():
+    """They are one memory, written at once: a first product of any is the first one of all."""
+    w = held(400, 300)
+    first, rest = w[:128], w[128:]
+    assert first.read == [] and rest[128:].read == []
+    rest.read.append(True)
+    assert w.read == first.read == rest[128:].read == w[256:].read == [True]
+    assert copy.deepcopy(rest).read == []

@@ -113,3 +113,12 @@ def test_a_product_that_failed_is_not_a_weights_first_one(monkeypatch, kind):
     with pytest.raises(RuntimeError):
         K.linear_fp4(wide, q, pdl=True)
     assert not q.read
+
+
+def test_a_row_range_is_its_matrixs_memory(monkeypatch):
+    """What was written with the whole matrix: a product with a range of its rows is a first one only where none of that matrix was before it."""
+    v, x = rows_of(300, 512, BF), rows_of(1, 512, BF)
+    q = K.fp4_quantise(v, "nv")
+    seen = Launchers(monkeypatch)
+    K.linear_fp4(x, q[128:], pdl=True), K.linear_fp4(x, q[:200], pdl=True), K.linear_fp4(x, q, pdl=True), K.linear_fp4(x, q[128:][:100], pdl=True)
+    assert [p for _, p in seen.asked] == [0, 1, 1, 1]
