@@ -63,6 +63,7 @@ class Attention:
         self.kv_dim = self.n_kv * self.head_dim
         names = [prefix + f"{p}_proj.weight" for p in ("q", "k", "v")]
         self.w_qkv = held(weights.load_fused(names, [self.q_dim, self.kv_dim, self.kv_dim], self.hidden), rt)
+        self.w_q = self.w_qkv[: self.q_dim]   # for a run step that reads another step's cache
         self.w_o = held(weights.load(prefix + "o_proj.weight", "matrix"), rt)
         qk: Optional[PartSpec] = params.get("qk_norm")
         self.qk_eps = 0.0
@@ -157,7 +158,7 @@ class Attention:
         reads ``x`` next; the last product leaves ``x`` weighted for it where the sizes allow.
         Returns ``(ss, ss_parts, xw or None)``."""
         n = x.shape[0]
-        w = self.w_qkv if owns_cache else self.w_qkv[: self.q_dim]
+        w = self.w_qkv if owns_cache else self.w_q
         qkv = torch.empty((n, w.shape[0]), dtype=x.dtype, device=x.device)
         norm_w, eps = fused_rms(norm)
         if isinstance(w, K.Weight4):   # these products sum their rows' squares themselves
@@ -185,7 +186,7 @@ class Attention:
         if owns_cache:
             qkv = linear(h, self.w_qkv, self.rt)
         else:  # a run step that reads another step's cache projects queries only
-            qkv = linear(h, self.w_qkv[: self.q_dim], self.rt)
+            qkv = linear(h, self.w_q, self.rt)
         return linear(self._attend(qkv, ctx, cache, owns_cache), self.w_o, self.rt)
 
     def _attend(self, qkv: torch.Tensor, ctx: StepContext, cache: CacheEntry, owns_cache: bool) -> torch.Tensor:

@@ -122,3 +122,57 @@ def test_a_row_range_is_its_matrixs_memory(monkeypatch):
     seen = Launchers(monkeypatch)
     K.linear_fp4(x, q[128:], pdl=True), K.linear_fp4(x, q[:200], pdl=True), K.linear_fp4(x, q, pdl=True), K.linear_fp4(x, q[128:][:100], pdl=True)
     assert [p for _, p in seen.asked] == [0, 1, 1, 1]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_layer_that_reads_anothers_cache(monkeypatch, kind):
+    """Its queries are a product with a range of its matrix's rows, which is taken once, not at every step; every product against the definition on the inputs that it had."""
+    from dryft_b200.config import register_architecture, unregister_architecture
+    from dryft_b200.config.spec import LayerSpec, ModelSpec, PartSpec, RunStep
+    from dryft_b200.engine.api import Engine
+
+    class Shared:
+        def __init__(self, raw):
+            self.raw = dict(raw)
+
+        def to_dict(self):
+            return dict(self.raw)
+
+        def model_spec(self):
+            norm = PartSpec("rmsnorm", {"size": 64, "eps": 1e-6})
+            attn = PartSpec("attention", {"hidden_size": 64, "num_heads": 5, "num_kv_heads": 5, "head_dim": 32, "scale": 32 ** -0.5, "window": None,
+                                          "qk_norm": PartSpec("rmsnorm", {"size": 32, "eps": 1e-6}), "position": PartSpec("rope", {"rotary_dim": 32, "theta": 1e4})})
+            ffn = PartSpec("swiglu", {"hidden_size": 64, "intermediate_size": 96})
+            layers = tuple(LayerSpec("prenorm", attn, ffn, norm, norm, f"l{i}.attn.", f"l{i}.ffn.", f"l{i}.n1.", f"l{i}.n2.") for i in range(2))
+            return ModelSpec("SharedForCausalLM", 211, 64, 512, PartSpec("embedding", {"vocab_size": 211, "hidden_size": 64}), layers, (RunStep(0), RunStep(1, cache_from=0)), norm,
+                             PartSpec("lm_head", {"vocab_size": 211, "hidden_size": 64, "tied": True}), embedding_prefix="emb.", final_norm_prefix="fn.", head_prefix="head.")
+
+    register_architecture("SharedForCausalLM", Shared)
+    try:
+        eng = Engine.from_config({"architectures": ["SharedForCausalLM"], "hidden_size": 64, "vocab_size": 211}, seed=5, std=0.15, dtype="bfloat16", max_batch=1, max_seq_len=64,
+                                 weight_bits=4, weight_format=kind, cuda_graphs=False)
+        kept, calls, made, look = K.linear_fp4, [], [], K.Fp4.__post_init__
+
+        def linear_fp4(x, w, *a, **kw):
+            y = kept(x, w, *a, **kw)
+            calls.append((x.clone(), w, kw.get("silu", False), y.clone()))
+            return y
+
+        monkeypatch.setattr(K, "linear_fp4", linear_fp4)
+        monkeypatch.setattr(K.Fp4, "__post_init__", lambda self: (made.append(self), look(self))[1])
+        with torch.inference_mode():
+            slots = eng.cache.open_sequences(1)
+            eng.stepper.step(slots, [[1, 2, 3, 4, 5]], [[4]])
+            eng.stepper.step(slots, [[6]], [[0]])
+        assert not made
+        assert [c[1].n for c in calls] == 2 * [480, 64, 192, 64, 160, 64, 192, 64, 211]
+        for x, w, silu, y in calls:
+            x = P.silu_mul(x.cpu()) if silu else x
+            xv, wv = P.values(x, kind), K.fp4_expand(w, out_dtype=F32).double().cpu()
+            want, terms = xv @ wv.T, xv.abs() @ wv.abs().T
+            room = (torch.finfo(y.dtype).eps / 2 + 2.0**-22) * want.abs() + (w.k / 64 + 2) * 2.0**-21 * terms
+            if silu:   # (as in the engine's own test: codes' borders)
+                room = room + xv.norm(dim=1, keepdim=True) * wv.norm(dim=1)[None] / 30
+            assert bool(((y.double().cpu() - want).abs() <= room).all())
+    finally:
+        unregister_architecture("SharedForCausalLM")
