@@ -2959,10 +2959,15 @@ def _fp4_fused(m: int, k: int, kind: str, nb: int, split: int, silu: bool = Fals
     """Whether every block of a product rounds x for itself, which saves a launch: 16 rows and 12 blocks of 256 inputs a block at most (shared memory), and as long as that is quick.
 
     A launch costs the host 4 us, more than the kernels differ by: a block rounds up to 900 times 16 numbers; ``"nv"``, where a row's largest number comes first, 320, with silu 640.
-    In a captured graph it costs nothing, and runs while the product asks for weights: then 512, with silu 320; ``"nv"`` none, with silu 240.  us, in a graph, in a launch of its own /
+    ``captured``: in a captured graph it costs nothing, and runs while the product asks for weights: then 512, with silu 320; ``"nv"`` none, with silu 240.  us, in a graph, in a launch of its own /
     in the product: 2,560 inputs, 6,144 outputs, five blocks a tile, ``"mx"`` 1 row 6.0 / 5.8, 16 rows 6.6 / 6.7, ``"nv"`` 6.2 / 6.8 and (8 rows) 6.6 / 7.4; 9,728 inputs, 2,560 outputs, eight
     blocks a tile, ``"mx"`` 1 row 7.9 / 7.2, 6 rows 8.0 / 7.8, 8 rows 8.1 / 8.4, ``"nv"`` 8.8 / 8.4, 4 rows 8.5 / 9.1; with silu ``"mx"`` 1 row 8.7 / 7.6, 4 rows 8.7 / 8.5, 8 rows 8.9 / 10.7, ``"nv"`` 1
-    row 9.7 / 9.0, 4 rows 9.8 / 10.2, 8 rows 10.6 / 12.5; 19,456 outputs of 2,560 inputs, whole tiles, ``"mx"`` 1 row 8.9 / 8.4, 4 rows 9.1 / 9.2, 8 rows 8.8 / 10.7."""
+    row 9.7 / 9.0, 4 rows 9.8 / 10.2, 8 rows 10.6 / 12.5; 19,456 outputs of 2,560 inputs, whole tiles, ``"mx"`` 1 row 8.9 / 8.4, 4 rows 9.1 / 9.2, 8 rows 8.8 / 10.7.  Other widths, the
+    default ``pdl``: 6,144 of 4,096 ``"mx"`` 4 rows 8.0 / 6.8, 12 rows 8.1 / 8.1, ``"nv"`` 1 row 8.3 / 8.2, 8 rows 8.5 / 9.4; 10,240 of 5,120 ``"mx"`` 4 rows 9.8 / 8.6, 8 rows 9.9 / 10.1,
+    ``"nv"`` 1 row 10.3 / 10.1, 4 rows 10.3 / 11.1; 4,096 of 12,288 with silu ``"mx"`` 2 rows 10.6 / 9.2, 6 rows 10.6 / 12.0, ``"nv"`` 2 rows 11.4 / 11.4, 4 rows 11.7 / 12.9.
+
+    A captured call goes by that (``linear_fp4``) where it may overlap the launch before it, or with silu its own rounding (the default ``pdl``: 2,560 of 9,728 ``"nv"`` 8 rows 10.3 / 13.1).
+    Without silu the default goes by the eager limits, within 10% of the better either way; and so does ``pdl=False``, whose launches run in turn (``"nv"`` 8 rows, 6,144 of 2,560: 8.3 / 7.3)."""
     if m > 16 or nb != 16 or split < 1:
         return False
     own = -(-((k + 255) // 256) // split)
@@ -3028,14 +3033,13 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
     err = (error_flag(w.held.device) if flag is None else flag).data_ptr()
     factors = 0 if w.factors is None else w.factors.data_ptr()
     stream = _stream() if _raw_stream is None else _raw_stream(device)
-    captured = bool(pdl) and torch.cuda.is_current_stream_capturing()
     first = bool(pdl) and not w.read     # of those that may overlap the launch before them: it does not
     if given:
         rc = _fp4_calls[0](FP4_KINDS[kind], out_bf16, x.held.data_ptr(), 0 if x.factors is None else x.factors.data_ptr(), w.held.data_ptr(), factors, out.data_ptr(), m, n, k,
                            nb, blocks, split, bool(pdl) and not first, err, stream)
         if rc:
             _ok(rc, "linear_fp4")
-        if first and not captured:       # (what is captured has not run)
+        if first and not torch.cuda.is_current_stream_capturing():   # (what is captured has not run)
             w.read.append(True)
         launch_count += 1
         return out
@@ -3043,7 +3047,10 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
         act = torch.empty((m, k), dtype=x.dtype, device=x.device)
         silu_mul(x.contiguous(), act)
         x, step, silu = act, k, False
-    if (out_bf16 or not silu if is_bf16 else not out_bf16) and _fp4_fused(m, k, kind, nb, split, silu, captured):
+    within = (out_bf16 or not silu if is_bf16 else not out_bf16) and _fp4_fused(m, k, kind, nb, split, silu)
+    if within and (pdl or silu and pdl is None) and not _fp4_fused(m, k, kind, nb, split, silu, True):   # (the limits of captured calls are the lower ones)
+        within = not torch.cuda.is_current_stream_capturing()
+    if within:
         at = held = 0
         overlap = bool(pdl) and not first
         launches = 1
@@ -3056,7 +3063,7 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
                        stream)
     if rc:
         _ok(rc, "linear_fp4")
-    if first and not captured:
+    if first and not torch.cuda.is_current_stream_capturing():
         w.read.append(True)
     launch_count += launches
     return out

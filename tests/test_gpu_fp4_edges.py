@@ -176,3 +176,30 @@ def test_a_layer_that_reads_anothers_cache(monkeypatch, kind):
             assert bool(((y.double().cpu() - want).abs() <= room).all())
     finally:
         unregister_architecture("SharedForCausalLM")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("silu", [False, True])
+def test_where_captured_calls_round(monkeypatch, kind, silu):
+    """With silu a captured call goes by the limits of captured ones wherever its launches may overlap, not only where it may overlap the launch before it; without silu only there.
+    Launches that run in turn go by the eager limits.  The bits are the same."""
+    n, k = 640, 2560
+    q = K.fp4_quantise(rows_of(n, k, BF), kind)
+    xs = [rows_of(m, 2 * k if silu else k, BF) for m in (1, 2, 3, 4, 6, 8, 11, 16)]
+    seen, forms = Launchers(monkeypatch), {}
+    want = [K.linear_fp4(x, q, silu=silu) for x in xs]
+    eager = [f for f, _ in seen.asked]
+    seen.asked.clear()
+    for pdl in (True, None, False):
+        s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=s):
+            got = [K.linear_fp4(x, q, silu=silu, pdl=pdl) for x in xs]
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        forms[pdl] = [f for f, _ in seen.asked]
+        seen.asked.clear()
+    assert forms[True] != eager or (kind == "mx" and not silu)       # (of these sizes)
+    assert forms[None] == (forms[True] if silu else eager) and forms[False] == eager
+    K.check_error_flags()
