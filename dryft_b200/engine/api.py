@@ -60,9 +60,6 @@ class EngineOptions:
     weight_bits: int = 16
     cache_bits: int = 16
     bits_group: int = 64
-    # What 4-bit matrices are: "integer" (groups as above), or microscaled floating point (csrc/fp4.cuh): "mx", groups of 32 with a power of two, or "nv", groups of 16 with an
-    # 8-bit float and a factor for each row.  Products then round their activations to it too, row by row, and run on the tensor cores' 4-bit instructions: faster, less exact.
-    weight_format: str = "integer"
     tcgen05: bool = True                   # prefill attention and experts' products on tcgen05 / TMEM / TMA where the sizes allow
     # steps of up to this many rows run sublayers that read the same input (a mixer beside a feed-forward, two mixers side
     # by side) on streams of their own, joined before their results are summed: in a captured step they are parallel
@@ -72,6 +69,9 @@ class EngineOptions:
     # step again, from the cache the chunk before left): bounds the step's activations ([tokens, q + 2 kv], the
     # attention output) whatever the prompt length.  None: whole prompts in one step.
     prefill_chunk_tokens: Optional[int] = None
+    # What 4-bit matrices (``weight_bits``) are: "integer" (groups of ``bits_group``), or microscaled floating point (csrc/fp4.cuh): "mx", groups of 32 with a power of two, or "nv", groups of 16 with an
+    # 8-bit float and a factor for each row.  Products then round their activations to it too, row by row, and run on the tensor cores' 4-bit instructions: faster, less exact.
+    weight_format: str = "integer"
 
 
 def _require_cuda(device: str) -> torch.device:

@@ -71,11 +71,11 @@ class Runtime:
     norm_ahead: bool = False     # fused decode: a residual product leaves the stream weighted for the next norm (one rounding fewer than the reference)
     tcgen05: bool = True         # attention of prompts and experts' products on tcgen05.mma / tensor memory / TMA where sizes allow
     weight_bits: int = 16        # 4: the parts' matrices are held in 4 bits (ops/kernels.py:Weight4, Fp4)
-    weight_format: str = "integer"   # 4 bits: whole numbers ("integer"), or floating point with scales ("mx", "nv": products round their activations to it too)
     cache_bits: int = 16         # 4: keys and values are held in 4 bits
     bits_group: int = 64         # numbers that share a scale where something is held in 4 bits (fewer where a size consists of no whole ones)
     branch_rows: int = 0         # steps of up to this many rows run independent sublayers on streams of their own (0: in turn)
     side_streams: list = field(default_factory=list, repr=False, compare=False)
+    weight_format: str = "integer"   # 4 bits: whole numbers ("integer"), or floating point with scales ("mx", "nv": products round their activations to it too)
 
     def branches(self, n_rows: int) -> bool:
         return bool(self.branch_rows) and n_rows <= self.branch_rows and self.device.type == "cuda"

@@ -1,12 +1,15 @@
-"""Matrices in microscaled 4-bit floating point as objects: what copies and row ranges of them share (no GPU needed)."""
+"""Matrices in microscaled 4-bit floating point as objects: what copies and row ranges of them share, and the order of the options beside them (no GPU needed)."""
 
 import copy
+import dataclasses
 import pickle
 
 import pytest
 import torch
 
+from dryft_b200.engine.api import EngineOptions
 from dryft_b200.ops import kernels as K
+from dryft_b200.parts.base import Runtime
 
 
 def held(n, k, kind="nv"):
@@ -35,3 +38,11 @@ def test_ranges_of_rows_have_it_in_common_whether_a_product_has_read_them():
     rest.read.append(True)
     assert w.read == first.read == rest[128:].read == w[256:].read == [True]
     assert copy.deepcopy(rest).read == []
+
+
+def test_options_keep_their_places():
+    """A program that gives options by place goes on meaning what it meant: what came later stands behind."""
+    assert [f.name for f in dataclasses.fields(EngineOptions)][:19] == ["dtype", "max_batch", "max_seq_len", "max_tokens", "page_size", "cuda_graphs", "device", "small_m_max", "stream_m_max", "fuse_decode", "pdl",
+                                         "norm_ahead", "weight_bits", "cache_bits", "bits_group", "tcgen05", "branch_rows", "prefill_chunk_tokens", "weight_format"]
+    assert [f.name for f in dataclasses.fields(Runtime)] == ["dtype", "device", "page_size", "sm_count", "small_m_max", "stream_m_max", "ffn_chunk_rows", "fuse_decode", "pdl", "norm_ahead", "tcgen05", "weight_bits",
+                              "cache_bits", "bits_group", "branch_rows", "side_streams", "weight_format"]
