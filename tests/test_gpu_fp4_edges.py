@@ -203,3 +203,25 @@ def test_where_captured_calls_round(monkeypatch, kind, silu):
     assert forms[True] != eager or (kind == "mx" and not silu)       # (of these sizes)
     assert forms[None] == (forms[True] if silu else eager) and forms[False] == eager
     K.check_error_flags()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m,plan", [(1, None), (4, None), (40, None), (140, (128, 6, 1)), (140, (128, 12, 2)), (140, (128, 4, 0))])
+def test_large_rows_against_small_ones(monkeypatch, kind, m, plan):
+    """Rows of every size as weights against rows of every size as activations: where a sum of the terms' magnitudes is far from both ends of 32 bits, so is the result."""
+    k, n = 512, 300
+    if plan:
+        monkeypatch.setattr(K, "linear_fp4_plan", lambda *a: plan)
+    sizes = [1e-37, 1e-34, 1e-30, 1e-20, 1e-6, 1.0, 1e6, 1e20, 1e30, 1e34, 4e37]
+    w = (torch.randn(n, k, device="cuda") * torch.tensor(sizes, device="cuda").repeat(n // 11 + 1)[:n, None]).to(BF)
+    q = K.fp4_quantise(w, kind)
+    for i in range(0, 11, m if m < 11 else 11):
+        x = (torch.randn(m, k, device="cuda") * torch.tensor(sizes[i:] + sizes[:i], device="cuda").repeat(m // 11 + 1)[:m, None]).to(BF)
+        got = K.linear_fp4(x, q, out_dtype=F32)
+        want, terms = P.product(x, w, kind)
+        fits = terms < 2.0**126                       # (of the rest no 32-bit sum need be a number)
+        assert float(fits.double().mean()) > 0.2
+        # (as in the test of rare rows; numbers below the smallest normal one may be taken for zeros)
+        room = 2.0**-21 * want.abs() + (k / 64 + 2) * 2.0**-21 * terms + (k / 64 + 1) * 2.0**-126
+        off = (got.double().cpu() - want).abs()
+        assert bool((off <= room)[fits].all()), ((~(off <= room)) & fits).nonzero()[:8].tolist()
