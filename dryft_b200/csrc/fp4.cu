@@ -212,7 +212,28 @@ template <typename... P, typename... A> int launch(void (*kern)(P...), dim3 bloc
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, (P)a...);
   return e != cudaSuccess ? (int)e : launch_status();
 }
+// of the current device
+int multiprocessors() {
+  static int of[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
+  if (of[dev] == 0 && cudaDeviceGetAttribute(&of[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) of[dev] = 1;
+  return of[dev];
+}
 }  // namespace
+
+// Lanes of a row: as many as hold it, or of few rows (no more than multiprocessors) as many as it has units for (a row's latency is then what counts): up to 256, from where on NV's maxima cost more
+// than units side by side give (48 rows of 9,728: 3.0 us with 256 lanes, 3.7 with 1,024; MX 2.35 and 2.42, but with silu 4.0 and 3.6).  More than 256: for rows that have a multiprocessor each (25,600
+// numbers of NV 6.0 and 4.6, with silu 16.0 and 8.3, of MX 4.0 and 3.2), or where NV would work out a row's numbers, or read 32 bits of each, twice (2,000 rows of 25,600, silu: 90 and with 512
+// lanes 83, 32-bit numbers 82 and 76; bfloat16 as it is 38 and 44).
+DRYFT_API int dryft_fp4_lanes(int is_bf16, int kind, int silu, int words, int rows, int k, int multiprocessors) {
+  const int held_at_a_time = !is_bf16 ? held_units<float, NV>() : kind == NV ? held_units<bf16, NV>() : held_units<bf16, MX>(), units = blocks_of(k) * BLOCK_UNITS;
+  const bool few = rows <= multiprocessors;
+  const int most = !words ? THREADS : few ? MOST_LANES : kind == NV && (silu || !is_bf16) ? 512 : THREADS;
+  int span = 32;
+  while (span < most && span * ((few && kind == MX && (silu || !is_bf16)) || (rows <= 512 && span < THREADS) ? 1 : held_at_a_time) < units) span *= 2;
+  return span;
+}
 
 // held: blocks of 128 rows by 256 inputs (fp4.cuh); factors: float [rows] (NV).  x: rows of k numbers, `stride` numbers apart, anywhere.  silu (bfloat16): rows of 2 k numbers,
 // silu of the first half times the second.  pdl: 1, a programmatic dependent of the launch before it; 2, the next
@@ -220,17 +241,9 @@ template <typename... P, typename... A> int launch(void (*kern)(P...), dim3 bloc
 DRYFT_API int dryft_fp4_quantise(int is_bf16, int kind, int silu, const void* x, long long stride, void* held, void* factors, int rows, int k, int pdl, void* stream) {
   if (rows <= 0 || k <= 0) return 0;
   if (silu && !is_bf16) return DRYFT_ERR_UNSUPPORTED;
-  const int item = is_bf16 ? 2 : 4, held_at_a_time = !is_bf16 ? held_units<float, NV>() : kind == NV ? held_units<bf16, NV>() : held_units<bf16, MX>();
+  const int item = is_bf16 ? 2 : 4;
   const bool words = ((uintptr_t)x & 15) == 0 && (rows == 1 || stride * item % 16 == 0) && (!silu || (long long)k * item % 16 == 0);
-  const int units = blocks_of(k) * BLOCK_UNITS;
-  // Lanes of a row: as many as hold it, or of few rows as many as it has units for (a row's latency is then what counts): up to 256, from where on NV's maxima cost more than units side by
-  // side give (48 rows of 9,728: 3.0 us with 256 lanes, 3.7 with 1,024; MX 2.35 and 2.42, but with silu 4.0 and 3.6).  More than 256: for rows that have a multiprocessor each (25,600 numbers of NV 6.0 and
-  // 4.6, with silu 16.0 and 8.3, of MX 4.0 and 3.2), or where NV would work out a row's numbers, or read 32 bits of each, twice (2,000 rows of 25,600, silu: 90 and with 512 lanes 83, 32-bit
-  // numbers 82 and 76; bfloat16 as it is 38 and 44).
-  const bool few = rows <= 148;
-  const int most = !words ? THREADS : few ? MOST_LANES : kind == NV && (silu || !is_bf16) ? 512 : THREADS;
-  int span = 32;
-  while (span < most && span * ((few && kind == MX && (silu || !is_bf16)) || (rows <= 512 && span < THREADS) ? 1 : held_at_a_time) < units) span *= 2;
+  const int span = dryft_fp4_lanes(is_bf16, kind, silu, words, rows, k, multiprocessors());
   const int threads = span > THREADS ? span : THREADS;
   const unsigned blocks = (unsigned)((rows + (long long)(threads / span) - 1) / (threads / span));
   const cudaStream_t st = (cudaStream_t)stream;

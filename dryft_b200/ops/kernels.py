@@ -2743,7 +2743,8 @@ def fp4_lib() -> ctypes.CDLL:
             lib.dryft_linear_fp4.argtypes = [_i, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p]
             lib.dryft_linear_fp4_rows.argtypes = [_i, _i, _i, _i, _p, _ll, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p, _ll, _i, _p, _p]
             lib.dryft_linear_fp4_clusters.argtypes = [_i, _i]
-            for name in ("dryft_fp4_quantise", "dryft_fp4_expand", "dryft_linear_fp4", "dryft_linear_fp4_rows", "dryft_linear_fp4_clusters"):
+            lib.dryft_fp4_lanes.argtypes = [_i, _i, _i, _i, _i, _i, _i]
+            for name in ("dryft_fp4_quantise", "dryft_fp4_expand", "dryft_linear_fp4", "dryft_linear_fp4_rows", "dryft_linear_fp4_clusters", "dryft_fp4_lanes"):
                 getattr(lib, name).restype = _i
             _fp4 = lib
         return _fp4
