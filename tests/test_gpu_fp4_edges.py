@@ -1,9 +1,12 @@
-"""Microscaled 4-bit floating point on the GPU at the edges of what its calls allow."""
+"""Microscaled 4-bit floating point on the GPU at the edges of what its calls allow: gates whose exponential nearly overflows, rows of any size against rows of any other, stages
+that end anywhere in a ring, calls that fail, what captured calls and repeated ones choose, and what an engine holds."""
 
 import pytest
 import torch
 
+import helpers as H
 import plain_fp4 as P
+import plain_qwen3
 from dryft_b200.ops import kernels as K
 from test_gpu_fp4 import near, rows_of
 
@@ -225,3 +228,31 @@ def test_large_rows_against_small_ones(monkeypatch, kind, m, plan):
         room = 2.0**-21 * want.abs() + (k / 64 + 2) * 2.0**-21 * terms + (k / 64 + 1) * 2.0**-126
         off = (got.double().cpu() - want).abs()
         assert bool((off <= room)[fits].all()), ((~(off <= room)) & fits).nonzero()[:8].tolist()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("name", ["b", "d"])
+def test_an_engine_holds_what_the_definition_says(model_dirs, monkeypatch, name, dtype, kind):
+    """Codes, scales and factors of every matrix: the definition's values rounded to 32 bits once, which is what (c s) g comes to."""
+    from dryft_b200.engine.api import Engine
+
+    eng = Engine(model_dirs[name], dtype=dtype, max_batch=1, max_seq_len=64, weight_bits=4, weight_format=kind, cuda_graphs=False)
+    t, cfg, used, kept = plain_qwen3.read_model_dir(model_dirs[name])[1], H.config_dict(name), [], K.linear_fp4
+
+    def linear_fp4(x, w, *a, **kw):
+        used.append(w)
+        return kept(x, w, *a, **kw)
+
+    monkeypatch.setattr(K, "linear_fp4", linear_fp4)
+    with torch.inference_mode():
+        eng.stepper.step(eng.cache.open_sequences(1), [[1, 2, 3]], [[2]])
+    want = []
+    for i in range(cfg["num_hidden_layers"]):
+        p = f"model.layers.{i}."
+        for parts in (["self_attn.q", "self_attn.k", "self_attn.v"], ["self_attn.o"], ["mlp.gate", "mlp.up"], ["mlp.down"]):
+            want.append(torch.cat([t[p + part + "_proj.weight"] for part in parts]))
+    want.append(t.get("lm_head.weight", t["model.embed_tokens.weight"]))
+    assert len(used) == len(want)
+    for w, v in zip(used, want):
+        assert torch.equal(K.fp4_expand(w, out_dtype=F32).cpu(), P.values(v.to(dtype), kind).to(F32))
