@@ -2775,8 +2775,8 @@ class Fp4:
     n: int
     k: int
     kind: str
-    # Whether a product that may be a programmatic dependent of the launch before it has read this one as its weight.  The first one is not: that launch may be what wrote this.  Ranges of
-    # rows have it in common.
+    # The streams on which a product that may be a programmatic dependent of the launch before it has read this one as its weight.  The first one there is not: that launch may be what wrote
+    # this.  Ranges of rows have it in common.
     read: list = field(default_factory=list, init=False, repr=False, compare=False)
 
     def __post_init__(self) -> None:
@@ -2988,8 +2988,9 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
 
     ``silu``: ``x`` ``[m, 2 k]`` holds gate columns, then as many others, and the product's operand is ``silu(gate) * other`` (rounding points are ``silu_mul``'s).
 
-    ``pdl``: ``True``, a programmatic dependent of the launch before it: it may ask for weights before that has ended, so they are older than that launch (a weight's first product
-    sees to that itself: it overlaps nothing, so that it may stand right behind ``fp4_quantise``); ``False``: no launch overlaps another; ``None``: only the product its own rounding.
+    ``pdl``: ``True``, a programmatic dependent of the launch before it: it may ask for weights before that has ended, so they are older than the last launch in front of it that is not such a
+    dependent itself (a weight's first product on a stream sees to that: it overlaps nothing, so that it may stand right behind ``fp4_quantise``); ``False``: no launch overlaps another;
+    ``None``: only the product its own rounding.
     Few rows are rounded by the product's blocks (``_fp4_fused``), more in a launch of their own.  ``out`` does not overlap ``x``."""
     global _fp4_calls, launch_count
     device = _need_fp4(w, "weight")
@@ -3033,15 +3034,19 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
     flag = _error_flags.get(device)
     err = (error_flag(w.held.device) if flag is None else flag).data_ptr()
     factors = 0 if w.factors is None else w.factors.data_ptr()
-    stream = _stream() if _raw_stream is None else _raw_stream(device)
-    first = bool(pdl) and not w.read     # of those that may overlap the launch before them: it does not
+    stream = _stream().value if _raw_stream is None else _raw_stream(device)
+    first = bool(pdl) and stream not in w.read     # of those that may overlap the launch before them: it does not
+    if first:
+        # What is captured has not run; and where any product has, the weight is older than the graph.
+        run = not torch.cuda.is_current_stream_capturing()
+        first = run or not w.read
     if given:
         rc = _fp4_calls[0](FP4_KINDS[kind], out_bf16, x.held.data_ptr(), 0 if x.factors is None else x.factors.data_ptr(), w.held.data_ptr(), factors, out.data_ptr(), m, n, k,
                            nb, blocks, split, bool(pdl) and not first, err, stream)
         if rc:
             _ok(rc, "linear_fp4")
-        if first and not torch.cuda.is_current_stream_capturing():   # (what is captured has not run)
-            w.read.append(True)
+        if first and run:
+            w.read.append(stream)
         launch_count += 1
         return out
     if silu and not is_bf16:
@@ -3064,8 +3069,8 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
                        stream)
     if rc:
         _ok(rc, "linear_fp4")
-    if first and not torch.cuda.is_current_stream_capturing():
-        w.read.append(True)
+    if first and run:
+        w.read.append(stream)
     launch_count += launches
     return out
 

@@ -118,6 +118,28 @@ def test_a_product_that_failed_is_not_a_weights_first_one(monkeypatch, kind):
     assert not q.read
 
 
+def test_a_weights_first_product_on_every_stream_overlaps_nothing(monkeypatch):
+    """A product that ran on another stream, behind an event there, says nothing about the launch before this one: it may still be the weight's rounding.  Captured products go by whether
+    any has run: a weight's rounding is not in front of them unless it is captured too, and then none has."""
+    v, x = rows_of(300, 512, BF), rows_of(1, 512, BF)
+    for operand in (x, K.fp4_quantise(x, "nv")):
+        q, other = K.fp4_quantise(v, "nv"), torch.cuda.Stream()
+        seen = Launchers(monkeypatch)
+        other.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(other):
+            results = [K.linear_fp4(operand, q, pdl=True) for _ in range(2)]
+        results += [K.linear_fp4(operand, q[:], pdl=True) for _ in range(2)]
+        assert [p for _, p in seen.asked] == [0, 1, 0, 1]
+        torch.cuda.synchronize()
+        assert all(torch.equal(r, results[0]) for r in results)
+        s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            y = K.linear_fp4(K.fp4_quantise(x, "nv"), q, pdl=True)
+        g.replay()
+        torch.cuda.synchronize()
+        assert seen.asked[-1] == ("held", 1) and torch.equal(y, results[0])
+
+
 def test_a_row_range_is_its_matrixs_memory(monkeypatch):
     """What was written with the whole matrix: a product with a range of its rows is a first one only where none of that matrix was before it."""
     v, x = rows_of(300, 512, BF), rows_of(1, 512, BF)
