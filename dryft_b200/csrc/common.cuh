@@ -29,10 +29,15 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
 // Round a 32-bit intermediate to T and back: a rounding point of the bfloat16 path.
 template <typename T> __device__ __forceinline__ float rnd(float v) { return to_f32<T>(from_f32<T>(v)); }
 
-// silu(g) = g / (1 + exp(-g)) where bfloat16 rounds it right away: the fast exponential (2 + 1.2 |g| ulp) and division (2 ulp) of 32 bits are far inside that rounding.  The
-// division gives 0 for divisors above 2^126 (gates from -87.34 down), so both sides are taken by four: the same bits elsewhere.  Below -88.72 the exponential is infinite and
-// silu is -0, as from the formula in 32 bits.
-__device__ __forceinline__ float silu_fast(float g) { return __fdividef(0.25f * g, fmaf(0.25f, __expf(-g), 0.25f)); }
+// silu(g) = g / (1 + exp(-g)) where bfloat16 rounds it right away: the fast power (of -g log2 e: 1.2 |g| ulp and two) and reciprocal of 32 bits are far inside that rounding.  Both sides are
+// taken by four, so that the reciprocal is a normal number up to the largest finite power (1 / 2^127 would be taken for 0: gates from -87.34 down); a power below the normal numbers
+// is 0, beside 1.  Below -88.72 the power is infinite and silu is -0, as from the formula in 32 bits.
+__device__ __forceinline__ float silu_fast(float g) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * g));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(0.25f, e, 0.25f)));
+  return 0.25f * g * r;
+}
 
 // Data that the launch before this one wrote (activations, sums of squares, the residual stream) is read
 // through L2 only in kernels that may run as programmatic dependents.  Such a grid is resident while its
