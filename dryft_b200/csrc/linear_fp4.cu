@@ -181,24 +181,24 @@ constexpr int MOST_BLOCKS = 8;   // of a cluster
 
 // A row of W's factor (NV), taken in two steps.  A sum of codes times scales is 2^-20 at the least, 2^54 at the most, and the other row's factor 2^-112 to 2^117: times `of` it is far
 // from both ends of 32 bits, whatever that other factor makes of it then; `rest` is a power of two, 1 but for rows of very large or small numbers.
-// (Asked for early, and looked at where it is used: a block of a cluster that looked at it in front of its sums took 0.3 us longer.)
-struct RowFactor { float of, rest; };
-__device__ __forceinline__ RowFactor in_steps(float f) {
-  return f > 0x1p60f ? RowFactor{f * 0x1p-48f, 0x1p48f} : f < 0x1p-80f ? RowFactor{f * 0x1p32f, 0x1p-32f} : RowFactor{f, 1.f};
+// (Asked for early, and looked at where nothing waits for it: a block of a cluster that looked at it in front of its sums took 0.3 us longer.)  `far`: whether a row of the warp's has such a rest.
+struct RowFactor { float of, rest; bool far; };
+template <int KIND> __device__ __forceinline__ RowFactor in_steps(float f) {
+  if (KIND != NV) return {1.f, 1.f, false};
+  const RowFactor r = f > 0x1p60f ? RowFactor{f * 0x1p-48f, 0x1p48f, false} : f < 0x1p-80f ? RowFactor{f * 0x1p32f, 0x1p-32f, false} : RowFactor{f, 1.f, false};
+  return {r.of, r.rest, __any_sync(0xffffffffu, r.rest != 1.f) != 0};
 }
 
 // A warp's results: columns (rows of x) of one row of W a lane.
 template <int KIND, int COLS, typename O>
-__device__ __forceinline__ void write_columns(const Params& p, O* to, bool there, int cols, float (&v)[COLS / 16][16], float w_factor, const float (&x_factor)[(COLS + 31) / 32]) {
-  const RowFactor own = in_steps(w_factor);
-  const bool rest = KIND == NV && __any_sync(0xffffffffu, own.rest != 1.f);
+__device__ __forceinline__ void write_columns(const Params& p, O* to, bool there, int cols, float (&v)[COLS / 16][16], RowFactor own, const float (&x_factor)[(COLS + 31) / 32]) {
 #pragma unroll
   for (int c = 0; c < COLS / 16; ++c) {
     if (16 * c >= cols) break;
     if (KIND == NV)
 #pragma unroll
       for (int j = 0; j < 16; ++j) v[c][j] = v[c][j] * own.of * __shfl_sync(0xffffffffu, x_factor[c / 2], (16 * c + j) % 32);
-    if (rest)
+    if (KIND == NV && own.far)
 #pragma unroll
       for (int j = 0; j < 16; ++j) v[c][j] *= own.rest;
     if (there)   // (apart from the exchanges, which are all lanes')
@@ -391,7 +391,8 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
     const bool issues = elected();
     int s = 0, run = 0;
     unsigned par = 0, buffer = 0;
-    long long left = first_tile < tiles ? (long long)((unsigned)(tiles - first_tile - 1) / (unsigned)step + 1) * (k1 - k0) : 0;   // stages that this block's products take
+    // stages that this block's products take
+    long long left = SPLIT ? k1 - k0 : first_tile < tiles ? (long long)((unsigned)(tiles - first_tile - 1) / (unsigned)step + 1) * (k1 - k0) : 0;
     bool ok = !FUSED || __all_sync(0xffffffffu, mbar_wait(x_full, 0, p.err, failed, 3));
     for (int t = first_tile; ok && t < tiles; t += step, ++run) {
       const int acc = run % L::ACCS;
@@ -449,13 +450,14 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
       if constexpr (SPLIT) break;   // (below)
       // into registers all at once, so that the next tile's products may begin
       const unsigned from = tmem + ((unsigned)(q * 32) << 16) + acc * NB + first;
+      const RowFactor steps = in_steps<KIND>(own);
       float v[COLS / 16][16];
 #pragma unroll
       for (int c = 0; c < COLS / 16; ++c)
         if (16 * c < cols) tmem_ld16(from + 16 * c, v[c]);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       mbar_arrive(&acc_empty[acc]);
-      write_columns<KIND, COLS>(p, reinterpret_cast<O*>(p.y) + (size_t)col0 * p.n + row, row < p.n, cols, v, own, x_factor);
+      write_columns<KIND, COLS>(p, reinterpret_cast<O*>(p.y) + (size_t)col0 * p.n + row, row < p.n, cols, v, steps, x_factor);
       __syncwarp();
     }
   }
@@ -496,6 +498,7 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
           }
       }
     }
+    const RowFactor steps = in_steps<KIND>(own);
     if (reads) mbar_wait<true>(&sums_s, 0, p.err, failed, 7);
     __syncwarp();
     cluster_arrive();   // (a block whose shared memory others may still send to does not end: below)
@@ -517,13 +520,15 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
             v[j + 3] += t.w;
           }
         if (KIND == NV) {
-          const RowFactor steps = in_steps(own);
           float f = x_factor[0];
 #pragma unroll
           for (int h = 1; h < (NB + 31) / 32; ++h)
             if (c >= 32 * h) f = x_factor[h];
 #pragma unroll
-          for (int j = 0; j < GROUP; ++j) v[j] = v[j] * steps.of * __shfl_sync(0xffffffffu, f, (c + j) % 32) * steps.rest;
+          for (int j = 0; j < GROUP; ++j) v[j] = v[j] * steps.of * __shfl_sync(0xffffffffu, f, (c + j) % 32);
+          if (steps.far)
+#pragma unroll
+            for (int j = 0; j < GROUP; ++j) v[j] *= steps.rest;
         }
         if (row < p.n)
 #pragma unroll
@@ -761,6 +766,7 @@ template <int KIND, typename O> __global__ void __launch_bounds__(PairLayout<KIN
       if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[acc], (unsigned)(run / accs & 1), p.err, failed, 15))) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const unsigned from = tmem + ((unsigned)(q * 32) << 16) + acc * acc_cols + first;
+      const RowFactor steps = in_steps<KIND>(own);
       float v[L::COLS / 16][16];
 #pragma unroll
       for (int c = 0; c < L::COLS / 16; ++c)
@@ -768,7 +774,7 @@ template <int KIND, typename O> __global__ void __launch_bounds__(PairLayout<KIN
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0 && t + accs * step < tiles) mbar_arrive_at(&acc_empty[acc], 0);   // (where products wait for it: nothing is on its way to a block that may have ended)
-      write_columns<KIND, L::COLS>(p, reinterpret_cast<O*>(p.y) + (size_t)col0 * p.n + row, row < p.n, cols, v, own, x_factor);
+      write_columns<KIND, L::COLS>(p, reinterpret_cast<O*>(p.y) + (size_t)col0 * p.n + row, row < p.n, cols, v, steps, x_factor);
       __syncwarp();
     }
   }
