@@ -2955,7 +2955,6 @@ def linear_fp4_plan(m: int, n: int, k: int, device: int) -> Tuple[int, int, int]
     return _fp4_plan(m, n, k, *_fp4_room(device))
 
 
-@functools.lru_cache(maxsize=4096)
 def _fp4_fused(m: int, k: int, kind: str, nb: int, split: int, silu: bool = False, captured: bool = False) -> bool:
     """Whether every block of a product rounds x for itself, which saves a launch: 16 rows and 12 blocks of 256 inputs a block at most (shared memory), and as long as that is quick.
 
@@ -2977,6 +2976,12 @@ def _fp4_fused(m: int, k: int, kind: str, nb: int, split: int, silu: bool = Fals
     else:
         most = 900 if kind == "mx" else 640 if silu else 320
     return own <= 12 and m * 16 * own <= most
+
+
+@functools.lru_cache(maxsize=4096)
+def _fp4_fused_both(m: int, k: int, kind: str, nb: int, split: int, silu: bool) -> Tuple[bool, bool]:
+    """``_fp4_fused`` of an eager and of a captured call."""
+    return _fp4_fused(m, k, kind, nb, split, silu), _fp4_fused(m, k, kind, nb, split, silu, True)
 
 
 _fp4_calls = None   # (product, product of rows as they are)
@@ -3053,9 +3058,9 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
         act = torch.empty((m, k), dtype=x.dtype, device=x.device)
         silu_mul(x.contiguous(), act)
         x, step, silu = act, k, False
-    within = (out_bf16 or not silu if is_bf16 else not out_bf16) and _fp4_fused(m, k, kind, nb, split, silu)
-    if within and (pdl or silu and pdl is None) and not _fp4_fused(m, k, kind, nb, split, silu, True):   # (the limits of captured calls are the lower ones)
-        within = not torch.cuda.is_current_stream_capturing()
+    within, captured = _fp4_fused_both(m, k, kind, nb, split, silu) if (out_bf16 or not silu if is_bf16 else not out_bf16) else (False, False)
+    if within != captured and (pdl or silu and pdl is None) and torch.cuda.is_current_stream_capturing():
+        within = captured
     if within:
         at = held = 0
         overlap = bool(pdl) and not first
