@@ -445,12 +445,12 @@ __global__ void __launch_bounds__(Layout<KIND, NB, SPLIT, SRC>::THREADS, Layout<
 #pragma unroll
         for (int c = 0; c < (COLS + 31) / 32; ++c)
           x_factor[c] = 32 * c + lane >= cols ? 1.f : FUSED ? row_factor(most_s.rows[col0 + 32 * c + lane]) : ld_prev(p.x_factors + col0 + 32 * c + lane);
+      const RowFactor steps = in_steps<KIND>(own);   // (here: the products take longer than the factor)
       if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[acc], (unsigned)(run / L::ACCS & 1), p.err, failed, 5))) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if constexpr (SPLIT) break;   // (below)
       // into registers all at once, so that the next tile's products may begin
       const unsigned from = tmem + ((unsigned)(q * 32) << 16) + acc * NB + first;
-      const RowFactor steps = in_steps<KIND>(own);
       float v[COLS / 16][16];
 #pragma unroll
       for (int c = 0; c < COLS / 16; ++c)
@@ -763,10 +763,10 @@ template <int KIND, typename O> __global__ void __launch_bounds__(PairLayout<KIN
 #pragma unroll
         for (int c = 0; c < L::COLS / 32; ++c) x_factor[c] = 32 * c + lane < cols ? ld_prev(p.x_factors + col0 + 32 * c + lane) : 1.f;
       const int acc = run % accs;
+      const RowFactor steps = in_steps<KIND>(own);   // (as above)
       if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[acc], (unsigned)(run / accs & 1), p.err, failed, 15))) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const unsigned from = tmem + ((unsigned)(q * 32) << 16) + acc * acc_cols + first;
-      const RowFactor steps = in_steps<KIND>(own);
       float v[L::COLS / 16][16];
 #pragma unroll
       for (int c = 0; c < L::COLS / 16; ++c)
