@@ -2845,8 +2845,8 @@ def _need_fp4(w, name: str) -> int:
     return _on_current(w.held, name)
 
 
-def _fp4_rows(x, name: str) -> int:
-    """Rows of consecutive numbers, any distance apart; the distance."""
+def _fp4_rows(x, name: str) -> Tuple[int, int]:
+    """Rows of consecutive numbers, any distance apart; the distance, and the device's number."""
     if not isinstance(x, torch.Tensor):
         raise KernelError(f"{name}: expected a tensor, got {type(x).__name__}")
     _act(x, name)
@@ -2858,8 +2858,7 @@ def _fp4_rows(x, name: str) -> int:
         raise KernelError(f"{name}: the numbers of a row lie behind one another (strides {x.stride()})")
     if shape[0] >= _FP4_MOST or shape[1] >= _FP4_MOST:
         raise KernelError(f"{name}: rows, and numbers of a row, are fewer than {_FP4_MOST}, got {tuple(shape)}")
-    _on_current(x, name)
-    return step
+    return step, _on_current(x, name)
 
 
 def _overlapping(a, b) -> bool:
@@ -2874,10 +2873,12 @@ def fp4_quantise(x, kind: str) -> Fp4:
     For weights, once, when they are loaded, and for activations that several products read."""
     global launch_count
     code = _fp4_kind(kind)
-    step = _fp4_rows(x, "x")
+    step, device = _fp4_rows(x, "x")
     m, k = x.shape
     if m == 0 or k == 0:
         raise KernelError(f"fp4_quantise: no numbers in {tuple(x.shape)}")
+    if device not in _error_flags:   # that of the products to come: one that a capture made would be cleared by every replay
+        error_flag(x.device)
     held = x.new_empty(_fp4_shape(m, k, kind), dtype=torch.uint8)
     factors = x.new_empty(m, dtype=torch.float32) if code else None
     rc = fp4_lib().dryft_fp4_quantise(x.dtype is torch.bfloat16, code, False, x.data_ptr(), step, held.data_ptr(), 0 if factors is None else factors.data_ptr(), m, k, False, _stream())
@@ -3009,7 +3010,7 @@ def linear_fp4(x, w: Fp4, out=None, pdl: Optional[bool] = None, silu: bool = Fal
             raise KernelError(f"linear_fp4: x is held as {x.kind!r}, the weight as {kind!r}")
         m, width, is_bf16 = x.n, x.k, True
     else:
-        step = _fp4_rows(x, "x")
+        step, _ = _fp4_rows(x, "x")
         m, width = x.shape
         is_bf16 = x.dtype is torch.bfloat16
     if width != (2 * k if silu else k):

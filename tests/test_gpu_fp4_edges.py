@@ -149,6 +149,22 @@ def test_a_row_range_is_its_matrixs_memory(monkeypatch):
     assert [p for _, p in seen.asked] == [0, 1, 1, 1]
 
 
+def test_a_replay_leaves_the_error_flag_as_it_is(monkeypatch):
+    """Where the first product of a process is captured, its flag is not the graph's: what a wait that gave up has left there stays until somebody reads it."""
+    v, x = rows_of(300, 512, BF), rows_of(3, 512, BF)
+    K.linear_fp4(x, K.fp4_quantise(v, "nv"))     # (loads the kernels)
+    monkeypatch.setattr(K, "_error_flags", {})
+    q, s, g = K.fp4_quantise(v, "nv"), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=s):
+        y = K.linear_fp4(x, q)
+    flag = K.error_flag(x.device)
+    flag.fill_(305)
+    g.replay()
+    torch.cuda.synchronize()
+    assert flag.tolist() == [305] and torch.equal(y, K.linear_fp4(x, q))
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_a_layer_that_reads_anothers_cache(monkeypatch, kind):
     """Its queries are a product with a range of its matrix's rows, which is taken once, not at every step; every product against the definition on the inputs that it had."""
