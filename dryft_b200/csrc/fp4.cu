@@ -8,11 +8,12 @@ constexpr int THREADS = 256, WARPS = THREADS / 32;
 
 // A row is 1 to 32 warps' (`span` lanes); a lane has HELD units in registers at a time, `span` apart.  NV wants the row's largest number first: a row that is held whole
 // (bfloat16, 256 lanes: up to 12,288 numbers) is read once.  Its blocks wait for their rows' first numbers, then for each other's maxima: 1,024 threads a multiprocessor, of 64 registers,
-// hide more of that than fewer with more in them (2,000 rows of 9,728, NV: 15.6 us and 17.8, MX with silu 25.6 and 35.9, of 2,560 32-bit numbers, NV, 9.1 and 12.0).
+// hide more of that than fewer with more in them (2,000 rows of 9,728, NV: 15.2 us, with 96 registers 17.8; MX with silu 24.5, 35.9; of 2,560 32-bit numbers, NV, 9.3, 12.0).  The bound of 64
+// registers is one for all forms that read words, also where blocks have 256 or 512 threads: 32-bit NV spills 176 bytes a thread, NV with silu 88, MX with silu 4.
 //
-// What bounds it: 2,000 rows of 9,728 in bfloat16 (39 MB read, 10 or 11 written: 7.5 us at a copy's rate) take MX 12.0 us, NV 15.6.  Issue slots are two thirds full (8.0 and 10.6 million
-// instructions of a warp: 13 and 17 for a number of each lane), and a block's rows come first, then are worked on.  Blocks of 512 or 1,024 threads and roundings in packed bfloat16 were
-// no faster.
+// What it takes: 2,000 rows of 9,728 in bfloat16 (39 MB read, 10 or 11 written: 7.5 us at a copy's rate) MX 11.7 us, NV 15.2; with silu (78 MB read: 13.4) 24.5 and 29; rows that begin anywhere 16.6 and
+// 22.7.  Nothing is full: issue slots two thirds (8.0 and 10.6 million instructions of a warp, without silu: 13 and 17 for a number of each lane), memory 61%; a block's rows come
+// first, then are worked on, and what is resident beside it does not cover that.  Blocks of 512 or 1,024 threads and roundings in packed bfloat16 were no faster.
 template <typename T, int KIND> __host__ __device__ constexpr int held_units() { return sizeof(T) == 4 ? 2 : KIND == NV ? 3 : 4; }
 // WORDS: rows begin on 16-byte boundaries (silu: both halves of them).
 constexpr int MOST_LANES = 1024;
@@ -79,7 +80,7 @@ __global__ void __launch_bounds__(WORDS ? MOST_LANES : THREADS, 1) fp4_quantise_
 }
 
 // A block of 128 rows by 256 inputs a thread block, two rows a warp at a time: sixteen numbers a lane, whose results are whole sectors, all of a lane's codes asked for first.  Bound by
-// what it writes: 19,456 rows of 2,560 as bfloat16 (28 MB in, 100 out) 22 us, 5,700 GB/s.
+// what it writes: 19,456 rows of 2,560, MX, as bfloat16 (26.5 MB in, 100 out) 22 us, 5,700 GB/s.
 template <typename O, int KIND>
 __global__ void __launch_bounds__(THREADS) fp4_expand_kernel(const unsigned char* held, const float* factors, O* out, int rows, int k) {
   typedef Format<KIND> F;
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(THREADS) fp4_expand_kernel(const unsigned char
 }
 
 // The same where rows of results begin anywhere: a row's 256 numbers a warp at a time, eight a lane, by way of shared memory, so that what crosses memory is 16-byte words, but for a
-// segment's two ends (a number a lane straight to memory: 46 us for 2,000 rows of 9,729, the lanes' work).
+// segment's two ends: 2,000 rows of 9,729 15.3 us as bfloat16 (rows on 32-byte boundaries 9.6), 24.7 in 32 bits; a number a lane straight to memory 46, the lanes' work.
 constexpr int SHIFTED_ROWS = 4;   // rows of a warp
 template <typename O, int KIND> __global__ void __launch_bounds__(THREADS) fp4_expand_shifted_kernel(const unsigned char* held, const float* factors, O* out, int rows, int k) {
   typedef Format<KIND> F;
@@ -223,7 +224,7 @@ int multiprocessors() {
 }  // namespace
 
 // Lanes of a row: as many as hold it, or of few rows (no more than multiprocessors) as many as it has units for (a row's latency is then what counts): up to 256, from where on NV's maxima cost more
-// than units side by side give (48 rows of 9,728: 3.0 us with 256 lanes, 3.7 with 1,024; MX 2.35 and 2.42, but with silu 4.0 and 3.6).  More than 256: for rows that have a multiprocessor each (25,600
+// than units side by side give (48 rows of 9,728: 3.0 us with 256 lanes, 3.7 with 1,024; MX 2.4 either way, but with silu 4.0 and 3.6).  More than 256: for rows that have a multiprocessor each (25,600
 // numbers of NV 6.0 and 4.6, with silu 16.0 and 8.3, of MX 4.0 and 3.2), or where NV would work out a row's numbers, or read 32 bits of each, twice (2,000 rows of 25,600, silu: 90 and with 512
 // lanes 83, 32-bit numbers 82 and 76; bfloat16 as it is 38 and 44).
 DRYFT_API int dryft_fp4_lanes(int is_bf16, int kind, int silu, int words, int rows, int k, int multiprocessors) {

@@ -1,7 +1,7 @@
 // y = x w^T with both operands in microscaled 4-bit floating point (fp4.cuh), on the 5th-generation tensor cores, which multiply such numbers and scales as they lie:
 // tcgen05.mma kind::mxf4 (a scale for 32 inputs) and kind::mxf4nvf4 (for 16), 64 inputs an instruction, summed in 32 bits.  A product of two codes is a multiple of 1/4, so what an
-// instruction sums before the scales is exact: of 25,600 inputs, MX results are the definition's in 32 bits, NV results off by 5e-8 of the whole (a product of the same values in 32
-// bits by the library: 8e-7).
+// instruction sums before the scales is exact.  Measured with normal random operands of 25,600 inputs: MX results are the definition's in 32 bits, NV results off by 5e-8 of the whole (a
+// product of the same values in 32 bits by the library: 8e-7).  Where groups differ far in size a sum is cut off below 2^-21 of its terms' magnitudes, an instruction, at the most.
 //
 // Computed transposed: a tile is 128 rows of W, on the M side, against NB rows of x (16 to 128, padded to whole sixteens), its sums in tensor memory, a W row a lane: results are written
 // a column at a time, 32 lanes' behind one another.  A stage of the ring is 256 inputs: a block of W and one of x, each one copy of consecutive bytes (the layout is the tensor
@@ -13,10 +13,11 @@
 // 256-row tile of W between them (below).  ops/kernels.py:_fp4_plan chooses, with both sides' figures.
 //
 // What bounds it.  Few rows: W's bytes.  151,936 outputs of 2,560 inputs, 1 row: 33.6 us, 6,500 GB/s, 99% of a copy's rate; with fewer bytes the launch, first bytes and a tile's end: 8 rows,
-// 19,456 of 2,560 (28 MB) 7.2 us where the bytes are 4.1; 1 row, 6,144 of 2,560 3.8 and 1.35, 2,560 of 9,728 4.8 and 2.1.  Many rows: what
+// 19,456 of 2,560 (MX, 26.5 MB) 7.2 us where the bytes are 4.1; 1 row (NV), 6,144 of 2,560 4.1 and 1.35, 2,560 of 9,728 4.8 and 2.1.  Many rows: what
 // enters a multiprocessor.  2,048 rows, 5,120 of 25,600 (pairs with 192 columns): NV 103 us, MX 91.5, 5.9 PFLOP/s, 104 GB/s into each, 15 TB/s in all; 24,576 of 4,096 (256
 // columns): 83 us, 5.0 PFLOP/s, and 75.5.  MX has 0.91 and 0.92 of NV's bytes, takes 0.89 and 0.91 of its time, and has the same products; the tensor pipe is 62% busy.  Larger tiles would
-// read less for as much work, but tensor memory is full.
+// read less for as much work: 512 outputs by 192 rows leave tensor memory room for one set of sums and two stages' scales, so that products wait while sums are read, and there are half as
+// many tiles to share out.  Not built.
 //
 // Warps: 0 copies, 1 issues, the others read the sums out.  Every wait on a barrier is bounded by a clock; a waiter that gives up raises *err, every role leaves its loop, the block lets its
 // copies and products end and frees its tensor memory.
@@ -145,6 +146,7 @@ template <int KIND, int NB, bool SPLIT, int SRC> struct Layout {
   static constexpr int ROUNDERS = FUSED ? READERS + 4 : 0, THREADS = (2 + (FUSED ? ROUNDERS : READERS)) * 32;   // warps that round x, the readers among them
   static constexpr int X_BYTES = F::SCALE_BYTES + NB * (INPUTS / 2), STAGE_BYTES = F::BLOCK_BYTES + (FUSED ? 0 : X_BYTES);   // W's block, as much of x's; multiples of 1024
   static constexpr int X_BLOCKS = FUSED ? FUSED_BLOCKS : 0;                                  // of x, which stay for all tiles
+  // (of 64 registers where tiles have 128 columns and are not shared: two forms spill 8 bytes a thread)
   static constexpr int RESIDENT = 2, STAGES = (110 * 1024 - X_BLOCKS * X_BYTES) / STAGE_BYTES;   // RESIDENT: blocks of a multiprocessor
   // tensor memory: sums of ACCS tiles, then the scales of two stages
   static constexpr int ACCS = SPLIT || NB >= 128 ? 1 : 2, SCALE_COLS = 8 * F::WORDS, NEED_COLS = ACCS * NB + 2 * SCALE_COLS;
