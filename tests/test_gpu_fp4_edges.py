@@ -15,6 +15,20 @@ BF, F32 = torch.bfloat16, torch.float32
 KINDS = ("mx", "nv")
 
 
+def test_silu_of_every_gate():
+    """All bfloat16 numbers: within one rounding to bfloat16 (2^-8, or half the smallest number) and the 32-bit function's own error (2^-15, see below) of the definition down to -88.5;
+    zero below, where the 32-bit power is infinite; NaN for NaN and for minus infinity."""
+    g = torch.arange(65536, device="cuda").to(torch.int32).to(torch.int16).view(BF)
+    got = torch.empty(1, 65536, dtype=BF, device="cuda")
+    K.silu_mul(torch.cat([g, torch.ones_like(g)])[None], got)
+    x, got = g.double().cpu(), got[0].double().cpu()
+    want = x * torch.sigmoid(x)
+    assert torch.equal(got.isnan(), want.isnan()) and bool((got[x < -88.75] == 0)[x[x < -88.75] > -float("inf")].all())
+    near_ = (x >= -88.75) & x.isfinite()
+    assert int(near_.sum()) > 48000 and bool(((got - want).abs() <= (2.0**-8 + 2.0**-15) * want.abs() + 2.0**-134)[near_].all())
+    assert float(got[x == float("inf")]) == float("inf")
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("m", [2, 40])
 def test_gates_whose_exponential_is_nearly_too_large(kind, m):
